@@ -310,6 +310,176 @@ int pesti_llama_chain_batch(pesti_sampler* s, const void* d_logits, pesti_dtype 
                             const int32_t* d_history_len, int64_t history_ld, const float* d_u,
                             int32_t* d_out_tokens, int32_t* d_out_kept, void* stream);
 
+/*
+ * Beam search: the third way to choose tokens beside pesti_sample_batch and
+ * pesti_argmax_batch.  No counterpart in the reference, whose generate()
+ * (transformer/model.rs:508-531) follows one sequence.
+ *
+ * G groups (prompts) of W beams each, W <= PESTI_BEAM_MAX_WIDTH.  None of
+ * these calls needs a handle or allocates: they run on the calling thread's
+ * current device, stream-ordered (NULL: the legacy default stream), in the
+ * caller's buffers, and may be captured into a graph.
+ *
+ * pesti_beam_select: the K best continuations of each group, for logits
+ * [G*W, ld] (first V columns of each row; beam w of group g is row g*W + w;
+ * F32, BF16 or F16):
+ *   score(w, v) = cum[w] + log softmax(x[w])[v]
+ *  - scores are compared in 64 bits; within a beam candidates rank by their
+ *    logits, equal logits by the lower token id; equal scores of two beams
+ *    rank by the lower beam;
+ *  - NaN logits count as -inf.  Tokens of probability 0 are never chosen.  In
+ *    a row that holds +inf, the +inf entries share its probability equally;
+ *  - d_cum: [G, W] f32 scores so far (NULL: all 0).  A beam whose score is
+ *    -inf or NaN has no candidates, and its logits are not read (unless d_lse
+ *    is given);
+ *  - d_done: optional [G] u8; groups with a non-zero entry are not read and
+ *    get no candidates;
+ *  - d_score, d_token, d_parent: [G, K], best first, K <= PESTI_BEAM_MAX_CAND:
+ *    score (f32), token, and the beam (0..W-1) it continues.  Slots without a
+ *    candidate hold -inf, -1, -1;
+ *  - d_lse: optional [G, W]: log sum exp of each row's logits (-inf for the
+ *    rows of finished groups);
+ *  - d_ws: device scratch of pesti_beam_select_workspace(...) bytes, 256-byte
+ *    aligned, any contents.  Calls whose GPU work may overlap need scratch of
+ *    their own.
+ * With W = 1 and no d_cum it gives the K largest log-probabilities of each row
+ * (a distillation teacher's list).
+ */
+#define PESTI_BEAM_MAX_WIDTH 64
+#define PESTI_BEAM_MAX_CAND 128
+/* Bytes of scratch, or a negative PESTI_E_* code for refused sizes. */
+int64_t pesti_beam_select_workspace(pesti_dtype dtype, int64_t G, int64_t W, int64_t V, int64_t K);
+int pesti_beam_select(const void* d_logits, pesti_dtype dtype, int64_t G, int64_t W, int64_t V, int64_t ld,
+                      const float* d_cum, const uint8_t* d_done, int64_t K, float* d_score, int32_t* d_token,
+                      int32_t* d_parent, float* d_lse, void* d_ws, int64_t ws_bytes, void* stream);
+
+/*
+ * The loop control of a beam search on the device: pesti_generate_advance's
+ * counterpart for beams.  The state of G groups of W beams is a set of the
+ * caller's device arrays; pesti_beam_reset fills them for a new search (one
+ * live beam per group, score 0).
+ *
+ * pesti_beam_advance takes one step's candidates (pesti_beam_select's outputs)
+ * and, for every group with done == 0, goes through them in rank order:
+ *  - a candidate whose token is in d_stop[0..n_stop) ends a hypothesis if it is
+ *    among the first W ranks: the tokens of its parent (the stop token is not
+ *    kept), with the score s / (count + 1)^length_penalty;
+ *  - the first W others become the live beams 0, 1, ...: tokens[w] is the
+ *    parent's tokens and the new one, cum[w] the candidate's score, last[w] the
+ *    new token, parent[w] its parent.  Beams left over are dead: cum -inf,
+ *    parent -1, the rest as it was;
+ *  - padding (token or parent -1, a parent outside [0, W)) is passed over; a
+ *    dead parent (which pesti_beam_select never names) is taken with the tokens
+ *    that its row holds.
+ * Ended hypotheses go to the group's pool of the W best: a full pool's lowest
+ * score (of equal ones the highest slot) gives way to a higher one.  count
+ * grows by 1.  Then the group finishes:
+ *  - when count reaches min(max_tokens, max_seq_len): the live beams go to the
+ *    pool with cum / count^length_penalty; done = 3 if count is max_seq_len,
+ *    else 2;
+ *  - without a live beam: done = 1;
+ *  - with a full pool, if early_stop is set or no live beam can still reach the
+ *    pool's lowest score (the larger of best / (count + 1)^length_penalty and
+ *    best / limit^length_penalty is no higher): done = 1.
+ * Groups that are done keep their state; their parent entries become -1.
+ * Scores are divided in 64 bits and held in f32.
+ */
+typedef struct {
+  float* cum;          /* [G, W] scores of the live beams */
+  int32_t* last;       /* [G, W] the next step's input tokens */
+  int32_t* parent;     /* [G, W] for pesti_beam_reorder; -1: the beam stays */
+  int32_t* tokens;     /* [G, W, cap] tokens of the live beams */
+  int32_t* count;      /* [G] steps taken: the length of every live beam */
+  uint8_t* done;       /* [G] */
+  int32_t* fin_tokens; /* [G, W, cap] the pool */
+  int32_t* fin_len;    /* [G, W] */
+  float* fin_score;    /* [G, W] -inf in empty slots */
+  int32_t* fin_count;  /* [G] */
+  int64_t cap;         /* >= min(max_tokens, max_seq_len) */
+} pesti_beam_state;
+typedef struct {
+  int64_t max_tokens;
+  int64_t max_seq_len;
+  double length_penalty;
+  int32_t early_stop;
+} pesti_beam_limits;
+int pesti_beam_reset(const pesti_beam_state* state, int64_t G, int64_t W, void* stream);
+int pesti_beam_advance(const pesti_beam_state* state, const float* d_score, const int32_t* d_token,
+                       const int32_t* d_parent, int64_t G, int64_t W, int64_t K, const uint32_t* d_stop,
+                       int64_t n_stop, const pesti_beam_limits* limits, void* stream);
+
+/*
+ * Reorders per-beam states (caches, generator states, page tables, histories)
+ * after a step: for every group g and beam w, row g*W + w of each state's dst
+ * becomes row g*W + d_parent[g*W + w] of its src; a parent outside [0, W) means
+ * the beam itself.  src and dst are the same memory with the same strides (in
+ * place; beams that stay are not touched) or do not overlap.  States must not
+ * share memory with one another (the same dst twice is refused).
+ * A row is `blocks` runs of block_bytes bytes, block_stride bytes apart (for a
+ * cache [rows, heads, room, dim] of which `used` positions are filled: blocks =
+ * heads, block_bytes = used*dim*esize).  Strides are in bytes and not negative.
+ * states: host array, read before the call returns.
+ */
+typedef struct {
+  const void* src;
+  void* dst;
+  int64_t src_row_stride, dst_row_stride;
+  int64_t src_block_stride, dst_block_stride;
+  int64_t blocks, block_bytes;
+} pesti_beam_rows;
+int pesti_beam_reorder(const pesti_beam_rows* states, int64_t n_states, const int32_t* d_parent, int64_t G,
+                       int64_t W, void* stream);
+
+/*
+ * Distillation from a teacher's top logits: the training side of the kept
+ * lists and of pesti_beam_select's log-probabilities.  No counterpart in the
+ * reference.
+ *
+ * Student logits [N, ld] (first V columns; F32, BF16 or F16) at temperature T:
+ * p = softmax(x / T) over all V tokens.  The teacher of row n lists k entries
+ * (token d_idx[n*idx_ld + j], logit or log-probability t = d_val[n*val_ld + j],
+ * val_dtype F32, BF16 or F16), 1 <= k <= PESTI_DISTILL_MAX_TOP; entries whose
+ * token is outside [0, V) (padding) are ignored, a token listed more than once
+ * counts with the sum of its entries.
+ *  - d_teacher_lse NULL: q_j = softmax(t / T) over the listed entries;
+ *  - d_teacher_lse [N] f32, the log sum exp of t / T over the teacher's whole
+ *    vocabulary: q_j = exp(t_j / T - lse), and the rest q_t = max(0, 1 - sum q)
+ *    stands against p_t, the student's mass outside the list.  Where p_t is 0 in
+ *    64 bits, q_t counts as 0.
+ *   loss = w T^2 [ sum_j q_j log(q_j / p_j) + q_t log(q_t / p_t) ]
+ *   grad = d loss / d x (the teacher is a constant)
+ * w = d_weight[n] (NULL: 1).  A row of weight 0 (padding) is not read: its loss
+ * and gradient are 0.  A row without teacher entries has loss and gradient 0.
+ * Entries with q = 0 add nothing to the loss.  A student logit of -inf has
+ * p = 0 (loss +inf where q > 0); a row of -inf alone has p = 0 everywhere.  NaN
+ * and +inf logits make the row's loss and gradient NaN, as NaN in its list does.
+ *
+ * pesti_distill_topk: d_loss [N] f32.  With d_grad ([N, grad_ld], the logits'
+ * type) it writes the gradient of the losses' sum as well, reading the logits
+ * from HBM once (for rows that fit the clusters' shared memory: up to about
+ * 590000 16-bit or 295000 f32 logits; longer ones twice); d_grad may be
+ * d_logits itself (with grad_ld == ld).  With d_stats ([N,
+ * PESTI_DISTILL_STATS] f64) it keeps what pesti_distill_topk_backward needs.
+ * pesti_distill_topk_backward: the gradient of sum_n d_up[n*up_stride] *
+ * loss_n (up_stride 0: one value for all rows) from the forward call's inputs
+ * and stats.
+ * Both run on the calling thread's current device, stream-ordered (NULL: the
+ * legacy default stream), allocate nothing, use no atomics on sums (the same
+ * inputs give the same bits) and may be captured into a graph.
+ */
+#define PESTI_DISTILL_MAX_TOP 256
+#define PESTI_DISTILL_STATS 8
+int pesti_distill_topk(const void* d_logits, pesti_dtype dtype, int64_t N, int64_t V, int64_t ld,
+                       const int32_t* d_idx, int64_t idx_ld, const void* d_val, pesti_dtype val_dtype,
+                       int64_t val_ld, int64_t k, const float* d_teacher_lse, const float* d_weight,
+                       double temperature, float* d_loss, double* d_stats, void* d_grad, int64_t grad_ld,
+                       void* stream);
+int pesti_distill_topk_backward(const void* d_logits, pesti_dtype dtype, int64_t N, int64_t V, int64_t ld,
+                                const int32_t* d_idx, int64_t idx_ld, const void* d_val, pesti_dtype val_dtype,
+                                int64_t val_ld, int64_t k, const float* d_teacher_lse, const float* d_weight,
+                                double temperature, const double* d_stats, const float* d_up, int64_t up_stride,
+                                void* d_grad, int64_t grad_ld, void* stream);
+
 /* Message of the last failure on the calling thread ("" if none). */
 const char* pesti_last_error(void);
 

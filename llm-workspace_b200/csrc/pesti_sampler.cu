@@ -24,6 +24,7 @@
 #include "../../include/pesti_testing.h"
 #include "pesti_kernels.cuh"
 #include "pesti_cluster.cuh"
+#include "pesti_error.h"
 #include "pesti_noalloc.h"
 #include "pesti_shard.cuh"
 #include "pesti_rng.cuh"
@@ -50,6 +51,9 @@ int cuda_fail(cudaError_t e, const char* what) {
   } while (0)
 
 }  // namespace
+
+int pesti_set_error(int code, const char* msg) { return fail(code, msg); }
+int pesti_set_cuda_error(cudaError_t e, const char* what) { return cuda_fail(e, what); }
 
 constexpr size_t kRowSmemLimit = 220 * 1024;
 static_assert(sizeof(pesti::RowShared) + sizeof(pesti::NucSmem) <= kRowSmemLimit, "nucleus rows' shared memory");

@@ -1,0 +1,108 @@
+"""Distillation from a teacher's top logits over the library's logit rows
+(include/pesti_sampler.h): the loss, its gradient, or both in one pass.
+
+The teacher's lists are what the library's teacher side makes: kept lists
+(probabilities: pass their logarithm), or pesti_beam.top_logprobs, whose tokens
+are padded with -1.  Every call runs the CUDA kernels of libpesti_sampler.so on
+the logits' device and the current stream; there is no CPU path.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from pesti_beam import _DTYPES, _launch, _need, _on_device, _ptr, _row_stride, _rows_dtype
+from pesti_sampler import _check, load_library
+
+MAX_TOP = 256  # PESTI_DISTILL_MAX_TOP
+_STATS = 8     # PESTI_DISTILL_STATS
+
+
+def _lists(logits, idx, val, temperature, teacher_lse, weight):
+    """Checks the arguments and returns them in the C call's order."""
+    dtype = _rows_dtype(logits)
+    N, V = logits.shape
+    dev = logits.device
+    _need(V >= 1, "V must be at least 1")
+    for t, name in ((idx, "idx"), (val, "val")):
+        _on_device(t, dev, name)
+        _need(t.dim() == 2 and t.shape[0] == N and (t.shape[1] <= 1 or t.stride(1) == 1),
+              f"{name} must be [N, k] with contiguous rows")
+    _need(idx.shape == val.shape, "idx and val must have the same shape")
+    k = idx.shape[1]
+    _need(1 <= k <= MAX_TOP, f"k must be 1 to {MAX_TOP}")
+    _need(idx.dtype == torch.int32, "idx must be int32")
+    vtype = _DTYPES.get(val.dtype)
+    _need(vtype is not None, "val must be float32, bfloat16 or float16")
+    for t, name in ((teacher_lse, "teacher_lse"), (weight, "weight")):
+        if t is not None:
+            _on_device(t, dev, name)
+            _need(t.dtype == torch.float32 and t.shape == (N,) and t.is_contiguous(),
+                  f"{name} must be a contiguous [N] float32 tensor")
+    return (logits.data_ptr(), dtype, N, V, _row_stride(logits), idx.data_ptr(), idx.stride(0), val.data_ptr(), vtype,
+            val.stride(0), k, _ptr(teacher_lse), _ptr(weight), float(temperature))
+
+
+class _DistillTopk(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, idx, val, temperature, teacher_lse, weight):
+        args = _lists(logits, idx, val, temperature, teacher_lse, weight)
+        N = logits.shape[0]
+        with _launch(logits.device, None) as st:
+            loss = torch.empty(N, dtype=torch.float32, device=logits.device)
+            stats = None
+            if ctx.needs_input_grad[0]:
+                stats = torch.empty(N, _STATS, dtype=torch.float64, device=logits.device)
+            _check(load_library().pesti_distill_topk(*args, loss.data_ptr(), _ptr(stats), None, 0, st))
+        ctx.save_for_backward(logits, idx, val, teacher_lse, weight, stats)
+        ctx.temperature = temperature
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, up):
+        logits, idx, val, teacher_lse, weight, stats = ctx.saved_tensors
+        args = _lists(logits, idx, val, ctx.temperature, teacher_lse, weight)
+        up = up.to(torch.float32)
+        with _launch(logits.device, None) as st:
+            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+            _check(load_library().pesti_distill_topk_backward(*args, _ptr(stats), up.data_ptr(), up.stride(0),
+                                                              grad.data_ptr(), logits.shape[1], st))
+        return grad, None, None, None, None, None
+
+
+def distill_topk(logits, idx, val, temperature: float = 1.0, teacher_lse=None, weight=None):
+    """Each row's distillation loss ([N] float32), differentiable for `logits`.
+
+    logits: [N, V] float32, bfloat16 or float16 student logits (rows may be
+    strided).  idx [N, k] int32 and val [N, k] (float32, bfloat16 or float16):
+    the teacher's tokens and logits or log-probabilities; tokens outside [0, V)
+    are padding.  teacher_lse: None (the list is renormalised), or [N] float32,
+    the log sum exp of the teacher's logits / temperature over its whole
+    vocabulary (0 for log-probabilities at temperature 1): the mass outside the
+    list is then one more outcome.  weight: optional [N] float32; rows of weight
+    0 are not read.  loss = weight * T^2 * KL(teacher || student).
+    The teacher is a constant: no gradient reaches idx, val or teacher_lse."""
+    return _DistillTopk.apply(logits, idx, val, temperature, teacher_lse, weight)
+
+
+def distill_topk_grad(logits, idx, val, temperature: float = 1.0, teacher_lse=None, weight=None, grad=None,
+                      stream=None):
+    """(loss [N], gradient of loss.sum() for the logits) in one pass over them:
+    for a training step that folds what follows the loss into `weight` (a mean's
+    1/N, a mask) and continues with logits.backward(gradient).  grad: the tensor
+    to fill, `logits` itself to overwrite them."""
+    logits = logits.detach()
+    args = _lists(logits, idx, val, temperature, teacher_lse, weight)
+    N, V = logits.shape
+    with _launch(logits.device, stream) as st:
+        loss = torch.empty(N, dtype=torch.float32, device=logits.device)
+        if grad is None:
+            grad = torch.empty(N, V, dtype=logits.dtype, device=logits.device)
+        else:
+            _on_device(grad, logits.device, "grad")
+            _need(grad.shape == logits.shape and grad.dtype == logits.dtype and (V <= 1 or grad.stride(1) == 1),
+                  "grad must match the logits and have contiguous rows")
+        _check(load_library().pesti_distill_topk(*args, loss.data_ptr(), None, grad.data_ptr(), _row_stride(grad), st))
+    return loss, grad

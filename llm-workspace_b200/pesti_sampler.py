@@ -56,8 +56,9 @@ NVCC_FLAGS = [
 
 def build(verbose: bool = False) -> str:
     """Compiles csrc/ into libpesti_sampler.so for sm_100a (in-tree)."""
-    srcs = [os.path.join(CSRC, "pesti_sampler.cu"), os.path.join(CSRC, "pesti_noalloc.cu")]
-    cmd = ["nvcc", *NVCC_FLAGS, "-o", LIB_PATH, *srcs, "-ldl"]
+    srcs = [os.path.join(CSRC, f) for f in ("pesti_sampler.cu", "pesti_noalloc.cu", "pesti_beam.cu",
+                                            "pesti_distill.cu")]
+    cmd = ["nvcc", *NVCC_FLAGS, "--threads", "0", "-o", LIB_PATH, *srcs, "-ldl"]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
     subprocess.run(cmd, check=True)
@@ -131,6 +132,22 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.pesti_llama_chain_batch.argtypes = [vp, vp, c_int, i64, i64, i64, ctypes.POINTER(LlamaChainParams), vp, vp,
                                             i64, vp, vp, vp, vp]
     lib.pesti_llama_chain_batch.restype = c_int
+    lib.pesti_beam_select_workspace.argtypes = [c_int, i64, i64, i64, i64]
+    lib.pesti_beam_select_workspace.restype = i64
+    lib.pesti_beam_select.argtypes = [vp, c_int, i64, i64, i64, i64, vp, vp, i64, vp, vp, vp, vp, vp, i64, vp]
+    lib.pesti_beam_select.restype = c_int
+    lib.pesti_beam_reset.argtypes = [vp, i64, i64, vp]
+    lib.pesti_beam_reset.restype = c_int
+    lib.pesti_beam_advance.argtypes = [vp, vp, vp, vp, i64, i64, i64, vp, i64, vp, vp]
+    lib.pesti_beam_advance.restype = c_int
+    lib.pesti_beam_reorder.argtypes = [vp, i64, vp, i64, i64, vp]
+    lib.pesti_beam_reorder.restype = c_int
+    lib.pesti_distill_topk.argtypes = [vp, c_int, i64, i64, i64, vp, i64, vp, c_int, i64, i64, vp, vp, ctypes.c_double,
+                                       vp, vp, vp, i64, vp]
+    lib.pesti_distill_topk.restype = c_int
+    lib.pesti_distill_topk_backward.argtypes = [vp, c_int, i64, i64, i64, vp, i64, vp, c_int, i64, i64, vp, vp,
+                                                ctypes.c_double, vp, vp, i64, vp, i64, vp]
+    lib.pesti_distill_topk_backward.restype = c_int
     lib.pesti_last_gathered_rows.argtypes = [vp]
     lib.pesti_last_gathered_rows.restype = i64
     lib.pesti_last_gathered_reasons.argtypes = [vp, vp]
