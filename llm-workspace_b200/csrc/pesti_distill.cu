@@ -98,18 +98,14 @@ int set_up(int* sms) {
 
 template <typename T, bool GRAD>
 int launch_row(DistillArgs& a, long long N, int sms, cudaStream_t st) {
-  // The cluster: as many CTAs as keep a row's units in shared memory, more
-  // while the rows alone do not fill the GPU and every warp still has a unit.
+  // One CTA per row while the rows fill the GPU: what a row costs besides its
+  // data (its list, its join) is paid once, and its second reading comes from
+  // L2 (2048 x 152064 bf16: 313 us; clusters of 2, 4, 8 and 16 that keep their
+  // part in shared memory: 358, 483, 678 and 1400 us).  Fewer rows than SMs are
+  // split over clusters while every warp still has a unit.
   long long c = 1;
-  a.keep = 0;
-  if (GRAD) {
-    while (c < MAX_CLUSTER && (a.units + c - 1) / c > kKeepUnits) c *= 2;
-    if ((a.units + c - 1) / c <= kKeepUnits)
-      a.keep = 1;
-    else
-      c = 1;
-  }
-  while (c < MAX_CLUSTER && N * c < 3LL * sms && a.units > c * ROW_WARPS) c *= 2;
+  while (c < MAX_CLUSTER && N * c < sms && a.units > c * ROW_WARPS) c *= 2;
+  a.keep = GRAD && (a.units + c - 1) / c <= kKeepUnits;
   a.per_cta = (a.units + c - 1) / c;
   if (N > 0x7fffffffLL / c) return refuse("N too large");
   cudaLaunchConfig_t cfg = {};

@@ -33,7 +33,7 @@ namespace pesti_rows {
 
 constexpr int MAX_TOP = 256;
 constexpr int HASH = 512;
-constexpr int ROW_WARPS = 8;                          // streaming warps
+constexpr int ROW_WARPS = 15;                         // streaming warps
 constexpr int ROW_THREADS = (ROW_WARPS + 1) * 32;     // and the list's
 constexpr int MAX_CLUSTER = 16;
 constexpr int STATS = 8;
@@ -75,18 +75,48 @@ __device__ __forceinline__ double teacher_value(const DistillArgs& a, long long 
 // e = 2^(x*C - R) relative to the reference of m, in 64 bits.
 __device__ __forceinline__ double exact_term(float x, float m, const DistillArgs& a) {
   if (x != x) return (double)x;
+  if (m == neg_inf()) return 0.0;
   if (is_far(m, a.c)) return x == m ? 1.0 : 0.0;
   return exp2((double)x * a.C - (double)ceilf(m * a.c));
 }
 
-// Exponential terms of a pair for the reference m of its row (far: counts).
-__device__ __forceinline__ float2 terms(float2 x, float2 c2, float2 lo2, float2 r2, float m, bool far) {
-  float2 t = fma2(x, lo2, fma2(x, c2, r2));
-  if (far) {
-    t.x = x.x == m ? 0.0f : x.x != x.x ? x.x : neg_inf();
-    t.y = x.y == m ? 0.0f : x.y != x.y ? x.y : neg_inf();
+// The reference R of a row's or unit's largest logit m (0 where it is not used).
+__device__ __forceinline__ float reference(float m, float c) {
+  return m > neg_inf() && !is_far(m, c) ? ceilf(m * c) : 0.0f;
+}
+
+// A term where m is far: 1 at m itself.
+__device__ __forceinline__ float far_term(float x, float m) { return x == m ? 1.0f : x != x ? x : 0.0f; }
+
+// Sum of a lane's terms of a unit.
+template <typename T>
+__device__ __forceinline__ float sum_terms(const uint4 (&v)[UNIT_VECS], float m, const DistillArgs& a) {
+  float2 s0 = make_float2(0.f, 0.f), s1 = s0;
+  if (m > neg_inf() && is_far(m, a.c)) {
+#pragma unroll
+    for (int i = 0; i < UNIT_VECS; ++i)
+#pragma unroll
+      for (int q = 0; q < Elem<T>::PAIRS; ++q) {
+        const float2 x = Elem<T>::pair(v[i], q);
+        s0 = add2(s0, make_float2(far_term(x.x, m), far_term(x.y, m)));
+      }
+  } else {
+    const float R = reference(m, a.c);
+    const float2 c2 = make_float2(a.c, a.c), lo2 = make_float2(a.c_lo, a.c_lo), r2 = make_float2(-R, -R);
+#pragma unroll
+    for (int i = 0; i < UNIT_VECS; ++i)
+#pragma unroll
+      for (int q = 0; q < Elem<T>::PAIRS; ++q) {
+        const float2 x = Elem<T>::pair(v[i], q);
+        const float2 t = fma2(x, lo2, fma2(x, c2, r2));
+        const float2 e = make_float2(ex2(t.x), ex2(t.y));
+        if (q & 1)
+          s1 = add2(s1, e);
+        else
+          s0 = add2(s0, e);
+      }
   }
-  return make_float2(ex2(t.x), ex2(t.y));
+  return (s0.x + s0.y) + (s1.x + s1.y);
 }
 
 struct Partial {
@@ -94,24 +124,32 @@ struct Partial {
   double s;
 };
 
-__device__ __forceinline__ void join(Partial& a, const Partial& b, float c) {
-  // NaN sums stay NaN: the scale of the lower reference multiplies its sum
-  const float m = fmaxf(a.m, b.m);
-  a.s = a.s * ref_scale(a.m, m, c) + b.s * ref_scale(b.m, m, c);
-  a.m = m;
+// Joins one partial sum per lane; NaN stays NaN (a scale multiplies it).
+__device__ __forceinline__ Partial warp_join(Partial p, float c) {
+  const float m = warp_max(p.m);
+  p.s = warp_reduce_add(p.s * ref_scale(p.m, m, c));
+  p.m = m;
+  return p;
 }
 
 struct RowShared {
   int32_t idx[MAX_TOP];   // -1: no entry
   int32_t hash[HASH];
-  float x[MAX_TOP];
+  float x[MAX_TOP];       // the places' logits
   double q[MAX_TOP];
   double qs[MAX_TOP];     // sum of q over equal tokens
+  double e[MAX_TOP];      // 2^(x C - R) for the largest listed logit's R
   uint8_t first[MAX_TOP]; // first entry of its token
   Partial warp[ROW_WARPS];
   Partial cta;
-  double A, listed, total, q_t, logq_norm, m_all_logs, inv_total;
-  float m_s, m_all;
+  double total, e_scale;  // Q + q_t; factor from e to p
+  float m_s, A;
+};
+
+// What the list's warp knows before the row's sum (the same in every lane).
+struct ListPart {
+  double Q, norm, rest;  // sum of q, log of the teacher's normaliser, max(0, 1 - Q) or 0
+  Partial member;        // listed tokens, each once
 };
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
@@ -175,14 +213,41 @@ __device__ __forceinline__ void store_vec(T* grow, long long lo, long long V, bo
 }
 
 template <typename T>
-__device__ __forceinline__ uint4 grad_vec(const uint4& v, float2 c2, float2 lo2, float2 r2, float m, bool far, float A) {
+__device__ __forceinline__ uint4 grad_vec(const uint4& v, float2 c2, float2 lo2, float2 r2, float A) {
   uint4 g;
 #pragma unroll
   for (int q = 0; q < Elem<T>::PAIRS; ++q) {
-    const float2 e = terms(Elem<T>::pair(v, q), c2, lo2, r2, m, far);
-    Elem<T>::pack(g, q, make_float2(e.x * A, e.y * A));
+    const float2 x = Elem<T>::pair(v, q);
+    const float2 t = fma2(x, lo2, fma2(x, c2, r2));
+    Elem<T>::pack(g, q, make_float2(ex2(t.x) * A, ex2(t.y) * A));
   }
   return g;
+}
+
+// The gradient of a unit outside the list: A times the terms.
+template <typename T>
+__device__ __forceinline__ void store_unit(T* grow, const uint4 (&v)[UNIT_VECS], int head, long long V, bool vec,
+                                           long long u, int lane, float m, float A, const DistillArgs& a) {
+  constexpr int VE = Elem<T>::VE;
+  const long long first = (u * UNIT_SLOTS + lane) * VE - head;
+  if (m > neg_inf() && is_far(m, a.c)) {
+#pragma unroll
+    for (int i = 0; i < UNIT_VECS; ++i) {
+      uint4 g;
+#pragma unroll
+      for (int q = 0; q < Elem<T>::PAIRS; ++q) {
+        const float2 x = Elem<T>::pair(v[i], q);
+        Elem<T>::pack(g, q, make_float2(far_term(x.x, m) * A, far_term(x.y, m) * A));
+      }
+      store_vec<T>(grow, first + i * 32 * VE, V, vec, g);
+    }
+  } else {
+    const float R = reference(m, a.c);
+    const float2 c2 = make_float2(a.c, a.c), lo2 = make_float2(a.c_lo, a.c_lo), r2 = make_float2(-R, -R);
+#pragma unroll
+    for (int i = 0; i < UNIT_VECS; ++i)
+      store_vec<T>(grow, first + i * 32 * VE, V, vec, grad_vec<T>(v[i], c2, lo2, r2, A));
+  }
 }
 
 // Zeros for units [ua, ub) of a gradient row.
@@ -193,71 +258,65 @@ __device__ __forceinline__ void zero_units(T* grow, int head, long long V, bool 
     store_vec<T>(grow, s * Elem<T>::VE - head, V, vec, z);
 }
 
-// The list's warp: teacher probabilities, equal tokens, and the places' logits.
-__device__ __forceinline__ void list_part(RowShared& sh, const DistillArgs& a, long long n, int lane) {
-  constexpr int PER = MAX_TOP / 32;
-  double t[PER];
-  double mt = -(double)pos_inf();
+// The list's warp: teacher probabilities, equal tokens, and the listed tokens' terms.
+__device__ __forceinline__ ListPart list_part(RowShared& sh, const DistillArgs& a, long long n, int lane) {
+  const double inf = (double)pos_inf();
+  ListPart r;
+  double mt = -inf;
+  float mx = neg_inf();
   for (int i = lane; i < HASH; i += 32) sh.hash[i] = -1;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int j = lane + 32 * i;
-    t[i] = -(double)pos_inf();
-    if (j < a.k && sh.idx[j] >= 0) t[i] = teacher_value(a, n, j) / a.T;
-    mt = !(t[i] <= mt) ? t[i] : mt;  // NaN is taken over
+  for (int j = lane; j < a.k; j += 32) {
+    const bool in = sh.idx[j] >= 0;
+    const double t = in ? teacher_value(a, n, j) / a.T : -inf;
+    sh.q[j] = t;
+    mt = !(t <= mt) ? t : mt;  // NaN is taken over
+    if (in) mx = fmaxf(mx, sh.x[j]);
   }
+  mx = warp_max(mx);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const double y = __shfl_xor_sync(FULL, mt, o);
     mt = mt != mt ? mt : !(y <= mt) ? y : mt;
   }
-  double norm;
   if (a.teacher_lse) {
-    norm = (double)a.teacher_lse[n];
+    r.norm = (double)a.teacher_lse[n];
   } else {
-    norm = 0.0;
-    if (mt != -(double)pos_inf()) {
+    r.norm = 0.0;
+    if (mt != -inf) {
       double z = 0.0;
-#pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (lane + 32 * i < a.k) z += exp(t[i] - mt);
-      z = warp_reduce_add(z);
-      norm = mt + log(z);
+      for (int j = lane; j < a.k; j += 32) z += exp(sh.q[j] - mt);
+      r.norm = mt + log(warp_reduce_add(z));
     }
   }
-  double Q = 0.0;
+  r.Q = 0.0;
   bool dup = false;
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int j = lane + 32 * i;
-    if (j < a.k) {
-      const int32_t id = sh.idx[j];
-      const double q = id >= 0 ? exp(t[i] - norm) : 0.0;
-      sh.q[j] = q;
-      sh.qs[j] = q;
-      sh.first[j] = id >= 0;
-      Q += q;
-      if (id >= 0) {
-        uint32_t h = ((uint32_t)id * 2654435761u) >> 23;
-        for (;;) {
-          const int32_t had = atomicCAS(&sh.hash[h], -1, id);
-          if (had == -1) break;
-          if (had == id) {
-            dup = true;
-            break;
-          }
-          h = (h + 1) & (HASH - 1);
+  for (int j = lane; j < a.k; j += 32) {
+    const int32_t id = sh.idx[j];
+    const double q = id >= 0 ? exp(sh.q[j] - r.norm) : 0.0;
+    sh.q[j] = q;
+    sh.qs[j] = q;
+    sh.first[j] = id >= 0;
+    sh.e[j] = id >= 0 ? exact_term(sh.x[j], mx, a) : 0.0;
+    r.Q += q;
+    if (id >= 0) {
+      uint32_t h = ((uint32_t)id * 2654435761u) >> 23;
+      for (;;) {
+        const int32_t had = atomicCAS(&sh.hash[h], -1, id);
+        if (had == -1) break;
+        if (had == id) {
+          dup = true;
+          break;
         }
+        h = (h + 1) & (HASH - 1);
       }
     }
   }
-  Q = warp_reduce_add(Q);
+  r.Q = warp_reduce_add(r.Q);
   if (__any_sync(FULL, dup)) {
     // a token listed twice: the first entry stands for it
-    for (int i = 0; i < PER; ++i) {
-      const int j = lane + 32 * i;
-      if (j < a.k && sh.idx[j] >= 0) {
+    __syncwarp();
+    for (int j = lane; j < a.k; j += 32)
+      if (sh.idx[j] >= 0) {
         double s = 0.0;
         bool first = true;
         for (int o = 0; o < a.k; ++o)
@@ -268,19 +327,20 @@ __device__ __forceinline__ void list_part(RowShared& sh, const DistillArgs& a, l
         sh.qs[j] = s;
         sh.first[j] = first;
       }
-    }
-  }
-  if (lane == 0) {
-    const double rest = 1.0 - Q;
-    sh.listed = Q;
-    sh.q_t = a.teacher_lse ? (rest < 0.0 ? 0.0 : rest) : 0.0;
-    sh.logq_norm = norm;
   }
   __syncwarp();
+  r.member.m = mx;
+  r.member.s = 0.0;
+  for (int j = lane; j < a.k; j += 32)
+    if (sh.first[j]) r.member.s += sh.e[j];
+  r.member.s = warp_reduce_add(r.member.s);
+  const double rest = 1.0 - r.Q;
+  r.rest = a.teacher_lse ? (rest < 0.0 ? 0.0 : rest) : 0.0;
+  return r;
 }
 
 template <typename T, bool GRAD>
-__global__ void __launch_bounds__(ROW_THREADS, 3) distill_row_kernel(const __grid_constant__ DistillArgs a) {
+__global__ void __launch_bounds__(ROW_THREADS, 2) distill_row_kernel(const __grid_constant__ DistillArgs a) {
   extern __shared__ uint4 kept[];
   __shared__ RowShared sh;
   constexpr int VE = Elem<T>::VE;
@@ -299,22 +359,24 @@ __global__ void __launch_bounds__(ROW_THREADS, 3) distill_row_kernel(const __gri
     if (crank == 0 && tid == 0) a.loss[n] = 0.0f;
     return;
   }
-  for (int j = tid; j < a.k; j += ROW_THREADS) {
-    const int32_t id = a.idx[n * a.idx_ld + j];
-    const bool in = id >= 0 && id < a.V;
-    sh.idx[j] = in ? id : -1;
-    sh.x[j] = in ? Elem<T>::load(row, id) : neg_inf();
-  }
-  __syncthreads();
   const bool tail = a.teacher_lse != nullptr;
-  const float2 c2 = make_float2(a.c, a.c), lo2 = make_float2(a.c_lo, a.c_lo);
+  ListPart list;
   if (wid == ROW_WARPS) {
-    list_part(sh, a, n, lane);
+    for (int j = lane; j < a.k; j += 32) {
+      const int32_t id = a.idx[n * a.idx_ld + j];
+      const bool in = id >= 0 && id < a.V;
+      sh.idx[j] = in ? id : -1;
+      sh.x[j] = in ? Elem<T>::load(row, id) : neg_inf();
+    }
+    __syncthreads();
+    list = list_part(sh, a, n, lane);
   } else {
     Partial acc{neg_inf(), 0.0};
-    for (long long u = ua + wid; u < ub; u += ROW_WARPS) {
-      uint4 v[UNIT_VECS];
-      load_unit<T, !GRAD>(v, row, head, a.V, u, lane);
+    uint4 v[UNIT_VECS];
+    long long u = ua + wid;
+    if (u < ub) load_unit<T, !GRAD>(v, row, head, a.V, u, lane);
+    __syncthreads();  // the list is there
+    while (u < ub) {
       if (GRAD && a.keep) {
 #pragma unroll
         for (int i = 0; i < UNIT_VECS; ++i) kept[(u - ua) * UNIT_SLOTS + i * 32 + lane] = v[i];
@@ -324,147 +386,110 @@ __global__ void __launch_bounds__(ROW_THREADS, 3) distill_row_kernel(const __gri
 #pragma unroll
       for (int i = 0; i < UNIT_VECS; ++i) m = fmaxf(m, Elem<T>::vec_max(v[i]));
       m = fmaxf(acc.m, warp_max(m));
-      const bool far = m > neg_inf() && is_far(m, a.c);
-      const float R = m > neg_inf() && !far ? ceilf(m * a.c) : 0.0f;
-      const float2 r2 = make_float2(-R, -R);
-      float2 s0 = make_float2(0.f, 0.f), s1 = s0;
-#pragma unroll
-      for (int i = 0; i < UNIT_VECS; ++i)
-#pragma unroll
-        for (int q = 0; q < Elem<T>::PAIRS; ++q) {
-          const float2 e = terms(Elem<T>::pair(v[i], q), c2, lo2, r2, m, far);
-          if (q & 1)
-            s1 = add2(s1, e);
-          else
-            s0 = add2(s0, e);
-        }
-      acc.s = acc.s * ref_scale(acc.m, m, a.c) + (double)((s0.x + s0.y) + (s1.x + s1.y));
+      acc.s = acc.s * ref_scale(acc.m, m, a.c) + (double)sum_terms<T>(v, m, a);
       acc.m = m;
+      u += ROW_WARPS;
+      if (u < ub) load_unit<T, !GRAD>(v, row, head, a.V, u, lane);
     }
     acc.s = warp_reduce_add(acc.s);  // every lane has the same reference
     if (lane == 0) sh.warp[wid] = acc;
   }
   __syncthreads();
-  if (tid == 0) {
-    Partial p = sh.warp[0];
-    for (int i = 1; i < ROW_WARPS; ++i) join(p, sh.warp[i], a.c);
-    sh.cta = p;
+  Partial s{neg_inf(), 0.0};
+  if (wid == ROW_WARPS) {
+    if (lane < ROW_WARPS) s = sh.warp[lane];
+    s = warp_join(s, a.c);
+    if (lane == 0) sh.cta = s;
   }
-  __syncthreads();
   if (csize > 1) {
     cluster_arrive();
     cluster_wait();
   }
   // the list's warp of every CTA puts the row together
+  const double pos = (double)pos_inf();
+  float m_all = neg_inf();
+  double S = 0.0, scale = 1.0, total = 0.0, q_t = 0.0, A = 0.0;
   if (wid == ROW_WARPS) {
-    __syncwarp();
-    Partial s = csize > 1 ? peer_partial(&sh.cta, 0) : sh.cta;
-    for (uint32_t r = 1; r < csize; ++r) {
-      const Partial p = peer_partial(&sh.cta, r);
-      join(s, p, a.c);
+    if (csize > 1) {
+      s = Partial{neg_inf(), 0.0};
+      if (lane < csize) s = peer_partial(&sh.cta, lane);
+      s = warp_join(s, a.c);
     }
     // all tokens: what was streamed, and the listed ones where they were left out
-    float m_all = s.m;
-    double S = s.s;
-    if (tail) {
-      for (int j = lane; j < a.k; j += 32)
-        if (sh.first[j]) m_all = fmaxf(m_all, sh.x[j]);
-      m_all = warp_max(m_all);
-      double e = 0.0;
-      for (int j = lane; j < a.k; j += 32)
-        if (sh.first[j]) e += exact_term(sh.x[j], m_all, a);
-      S = warp_reduce_add(e) + s.s * ref_scale(s.m, m_all, a.c);
-    }
-    const double pos = (double)pos_inf();
+    m_all = tail ? fmaxf(s.m, list.member.m) : s.m;
+    scale = ref_scale(s.m, m_all, a.c);
+    const double e_scale = ref_scale(list.member.m, m_all, a.c);
+    S = s.s * scale + (tail ? list.member.s * e_scale : 0.0);
     if (m_all == pos_inf()) S = pos - pos;  // +inf logits have no softmax: NaN
-    const bool none = !(m_all > neg_inf()) && S == S;  // every logit is -inf
-    const bool far = !none && is_far(m_all, a.c);
-    const double Rs = is_far(s.m, a.c) || !(s.m > neg_inf()) ? 0.0 : (double)ceilf(s.m * a.c);
-    const double Ra = far || none ? 0.0 : (double)ceilf(m_all * a.c);
-    // log sum exp((x - m_all)/T)
-    const double logS = none ? 0.0 : far ? log(S) : ONE_LN2 * (log2(S) - ((double)m_all * a.C - Ra));
-    double q_t = sh.q_t, logp_t = 0.0;
-    if (tail) {
-      const double scale = ref_scale(s.m, m_all, a.c);
-      if (s.s == 0.0 || scale == 0.0) {
-        q_t = q_t == q_t ? 0.0 : q_t;  // no unlisted token has a probability (that 64 bits hold)
-      } else if (far || is_far(s.m, a.c)) {
-        logp_t = log(s.s) - logS;
-      } else {
-        logp_t = ONE_LN2 * ((log2(s.s) + Rs) - (log2(S) + Ra));
-      }
+    q_t = list.rest;
+    if (s.s == 0.0 || scale == 0.0) q_t = q_t == q_t ? 0.0 : q_t;  // no unlisted token with a probability (in 64 bits)
+    total = list.Q + q_t;
+    // outside the list: grad = A * 2^(x C - Rs)
+    A = S;
+    if (S == S) A = s.s > 0.0 ? a.T * (total * scale / S - (q_t != 0.0 ? q_t / s.s : 0.0)) : 0.0;
+    if (lane == 0) {
+      sh.A = (float)(A * (double)w);
+      sh.total = total;
+      // p of a listed token; a row of -inf alone has none
+      sh.e_scale = S == 0.0 ? 0.0 : e_scale / S;
+      sh.m_s = s.m;
     }
-    const double total = sh.listed + q_t;
+  }
+  if (csize > 1) cluster_arrive();  // done with the others' shared memory
+  if (GRAD) __syncthreads();
+  if (wid == ROW_WARPS) {
     if (crank == 0) {
+      const bool none = !(m_all > neg_inf()) && S == S;  // every logit is -inf
+      const bool far = !none && is_far(m_all, a.c);
+      // log sum exp((x - m_all)/T)
+      const double logS = none ? 0.0 : far ? log(S) : ONE_LN2 * (log2(S) - ((double)m_all * a.C - (double)reference(m_all, a.c)));
       double l = 0.0;
       for (int j = lane; j < a.k; j += 32) {
         const double q = sh.q[j];
         if (sh.idx[j] >= 0 && q != 0.0) {
           const double x = (double)sh.x[j];
           const double logp = none || x == -pos ? (S == S ? -pos : S) : (x - (double)m_all) / a.T - logS;
-          l += q * ((teacher_value(a, n, j) / a.T - sh.logq_norm) - logp);
+          l += q * ((teacher_value(a, n, j) / a.T - list.norm) - logp);
         }
       }
       l = warp_reduce_add(l);
-      if (q_t != 0.0) l += q_t * (log(q_t) - logp_t);
+      // p_t = s.s * scale / S
+      if (q_t != 0.0) l += q_t * (log(q_t) - (log(s.s) + log(scale) - log(S)));
       if (S != S) l = S;
-      if (lane == 0) a.loss[n] = (float)((double)w * a.T * a.T * l);
-    }
-    if (lane == 0) {
-      // outside the list: grad = A * 2^(x C - Rs)
-      double A = S;
-      if (S == S) {
-        A = 0.0;
-        if (s.s > 0.0) {
-          const double share = tail ? ref_scale(s.m, m_all, a.c) : 1.0;
-          A = a.T * (total * share / S - (q_t != 0.0 ? q_t / s.s : 0.0));
+      if (lane == 0) {
+        a.loss[n] = (float)((double)w * a.T * a.T * l);
+        if (a.stats) {
+          double* st = a.stats + n * STATS;
+          st[ST_MS] = (double)s.m;
+          st[ST_A] = A;
+          st[ST_LOGQ] = list.norm;
+          st[ST_TOTAL] = total;
+          st[ST_MALL] = (double)m_all;
+          st[ST_LOGS] = logS;
         }
       }
-      sh.A = A;
-      sh.total = total;
-      sh.m_s = s.m;
-      sh.m_all = m_all;
-      sh.m_all_logs = logS;
-      if (a.stats && crank == 0) {
-        double* st = a.stats + n * STATS;
-        st[ST_MS] = (double)s.m;
-        st[ST_A] = A;
-        st[ST_LOGQ] = sh.logq_norm;
-        st[ST_TOTAL] = total;
-        st[ST_MALL] = (double)m_all;
-        st[ST_LOGS] = logS;
+    }
+  } else if (GRAD) {
+    const float m = sh.m_s, f = sh.A;
+    for (long long u = ua + wid; u < ub; u += ROW_WARPS) {
+      uint4 v[UNIT_VECS];
+      if (a.keep) {
+#pragma unroll
+        for (int i = 0; i < UNIT_VECS; ++i) v[i] = kept[(u - ua) * UNIT_SLOTS + i * 32 + lane];
+      } else {
+        load_unit<T, false>(v, row, head, a.V, u, lane);
       }
+      store_unit<T>(grow, v, head, a.V, vec, u, lane, m, f, a);
     }
   }
-  if (csize > 1) cluster_arrive();  // done with the others' shared memory
   if (GRAD) {
-    __syncthreads();
-    const float m = sh.m_s, A = (float)(sh.A * (double)w);
-    const bool far = m > neg_inf() && is_far(m, a.c);
-    const float R = m > neg_inf() && !far ? ceilf(m * a.c) : 0.0f;
-    const float2 r2 = make_float2(-R, -R);
-    for (long long s = ua * UNIT_SLOTS + tid; s < ub * UNIT_SLOTS; s += ROW_THREADS) {
-      const long long lo = s * VE - head;
-      if (lo >= a.V) break;
-      uint4 v;
-      if (a.keep)
-        v = kept[s - ua * UNIT_SLOTS];
-      else if (lo >= 0 && lo + VE <= a.V)
-        v = *(const uint4*)(row + lo);
-      else
-        v = load_edge<T>(row, lo, a.V);
-      store_vec<T>(grow, lo, a.V, vec, grad_vec<T>(v, c2, lo2, r2, m, far, A));
-    }
     __syncthreads();
     // the listed places of this CTA's part
     const long long from = ua * UNIT_SLOTS * VE - head, to = ub * UNIT_SLOTS * VE - head;
     for (int j = tid; j < a.k; j += ROW_THREADS) {
       const long long id = sh.idx[j];
-      if (id >= 0 && sh.first[j] && id >= from && id < to) {
-        const double x = (double)sh.x[j], m_all = (double)sh.m_all;
-        const double p = x == -(double)pos_inf() && sh.m_all_logs == sh.m_all_logs ? 0.0 : exp((x - m_all) / a.T - sh.m_all_logs);
-        Elem<T>::store(grow, id, (float)((double)w * a.T * (sh.total * p - sh.qs[j])));
-      }
+      if (id >= 0 && sh.first[j] && id >= from && id < to)
+        Elem<T>::store(grow, id, (float)((double)w * a.T * (sh.total * (sh.e[j] * sh.e_scale) - sh.qs[j])));
     }
   }
   if (csize > 1) cluster_wait();
@@ -513,17 +538,8 @@ __global__ void __launch_bounds__(BACK_WARPS * 32) distill_backward_kernel(const
     }
   }
   const float m = (float)st[ST_MS], A = (float)(st[ST_A] * scale);
-  const bool far = m > neg_inf() && is_far(m, a.c);
-  const float R = m > neg_inf() && !far ? ceilf(m * a.c) : 0.0f;
-  const float2 c2 = make_float2(a.c, a.c), lo2 = make_float2(a.c_lo, a.c_lo), r2 = make_float2(-R, -R);
   __syncthreads();
-  if (u < ub) {
-#pragma unroll
-    for (int i = 0; i < UNIT_VECS; ++i) {
-      const long long lo = (u * UNIT_SLOTS + i * 32 + lane) * VE - head;
-      if (lo < a.V) store_vec<T>(grow, lo, a.V, vec, grad_vec<T>(v[i], c2, lo2, r2, m, far, A));
-    }
-  }
+  if (u < ub) store_unit<T>(grow, v, head, a.V, vec, u, lane, m, A, a);
   __syncthreads();
   const int cnt = count;
   for (int i = tid; i < cnt; i += BACK_WARPS * 32) {

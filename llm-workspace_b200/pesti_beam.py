@@ -17,9 +17,9 @@ No call synchronises, except hypotheses() and active(), which read back.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
-from typing import Optional, Sequence
+import functools
+from typing import Sequence
 
 import torch
 
@@ -50,22 +50,36 @@ def _row_stride(t) -> int:
 
 
 def _on_device(t, dev, what: str) -> None:
-    _need(t.device == dev, f"{what} must be on the logits' device")
+    if t.device != dev:
+        raise ValueError(f"{what} must be on the logits' device")
 
 
-@contextlib.contextmanager
-def _launch(device, stream):
-    """The launching context: the tensors' device current, and temporary and
-    result tensors allocated on the stream that uses them.  Yields the stream."""
-    _need(device.type == "cuda", "tensors must be on a CUDA device (there is no CPU path)")
-    with contextlib.ExitStack() as stack:
-        if device.index != torch.cuda.current_device():
-            stack.enter_context(torch.cuda.device(device))
-        current = torch.cuda.current_stream(device).cuda_stream
-        if stream is not None and stream != current:
-            stack.enter_context(torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)))
-            current = stream
-        yield current
+_current_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _launch(device, stream, call):
+    """call(cudaStream_t) with the tensors' device current, and with what it
+    allocates belonging to the stream that uses it."""
+    if device.type != "cuda":
+        raise ValueError("tensors must be on a CUDA device (there is no CPU path)")
+    index = device.index
+    if index == torch.cuda.current_device():
+        current = _current_stream(index)
+        if stream is None or stream == current:
+            return call(current)
+    with torch.cuda.device(device):
+        if stream is None:
+            return call(_current_stream(index))
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+            return call(stream)
+
+
+@functools.lru_cache(maxsize=256)
+def _select_workspace(dtype: int, G: int, W: int, V: int, K: int) -> int:
+    need = load_library().pesti_beam_select_workspace(dtype, G, W, V, K)
+    _check(min(0, need))
+    return need
 
 
 def _ptr(t):
@@ -101,35 +115,38 @@ def beam_select(logits, beams: int, k: int, cum=None, done=None, lse=None, out=N
         _on_device(lse, dev, "lse")
         _need(lse.dtype == torch.float32 and lse.numel() == rows and lse.is_contiguous(),
               "lse must be a contiguous [groups*beams] float32 tensor")
-    lib = load_library()
-    with _launch(dev, stream) as st:
+    if out is not None:
+        for t, want in zip(out, (torch.float32, torch.int32, torch.int32)):
+            _on_device(t, dev, "out")
+            _need(t.dtype == want and t.shape == (G, k) and t.is_contiguous(),
+                  "out must be contiguous [groups, k] float32, int32 and int32 tensors")
+
+    def call(st):
         if out is None:
-            score = torch.empty(G, k, dtype=torch.float32, device=dev)
-            token = torch.empty(G, k, dtype=torch.int32, device=dev)
-            parent = torch.empty(G, k, dtype=torch.int32, device=dev)
+            score = torch.empty((G, k), dtype=torch.float32, device=dev)
+            token = torch.empty((G, k), dtype=torch.int32, device=dev)
+            parent = torch.empty((G, k), dtype=torch.int32, device=dev)
         else:
             score, token, parent = out
-            for t, want in ((score, torch.float32), (token, torch.int32), (parent, torch.int32)):
-                _on_device(t, dev, "out")
-                _need(t.dtype == want and t.shape == (G, k) and t.is_contiguous(),
-                      "out must be contiguous [groups, k] float32, int32 and int32 tensors")
-        if G == 0:
-            return score, token, parent
-        need = lib.pesti_beam_select_workspace(dtype, G, beams, V, k)
-        _check(min(0, need))
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        _check(lib.pesti_beam_select(logits.data_ptr(), dtype, G, beams, V, _row_stride(logits), _ptr(cum), _ptr(done),
-                                     k, score.data_ptr(), token.data_ptr(), parent.data_ptr(), _ptr(lse),
-                                     ws.data_ptr(), need, st))
-    return score, token, parent
+        if G:
+            need = _select_workspace(dtype, G, beams, V, k)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            rc = load_library().pesti_beam_select(
+                logits.data_ptr(), dtype, G, beams, V, _row_stride(logits), _ptr(cum), _ptr(done), k,
+                score.data_ptr(), token.data_ptr(), parent.data_ptr(), _ptr(lse), ws.data_ptr(), need, st)
+            if rc:
+                _check(rc)
+        return score, token, parent
+
+    return _launch(dev, stream, call)
 
 
 def top_logprobs(logits, k: int, stream=None):
     """The k largest log-probabilities of each row of `logits` ([B, V]), as a
     distillation teacher records them: (logprob [B, k] float32, token [B, k]
     int32, lse [B] float32), best first, (-inf, -1) where a row has fewer."""
-    with _launch(logits.device, stream):
-        lse = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
+    lse = _launch(logits.device, stream,
+                  lambda st: torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device))
     logprob, token, _ = beam_select(logits, 1, k, lse=lse, stream=stream)
     return logprob, token, lse
 
@@ -166,37 +183,49 @@ class BeamState:
         self.max_tokens, self.max_seq_len = int(max_tokens), int(max_seq_len)
         self.cap = max(1, min(self.max_tokens, self.max_seq_len))
         dev = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
-        self.device = dev
         G, W, i32 = self.groups, self.beams, torch.int32
-        with _launch(dev, stream):
-            def make(*shape, dtype=i32):
-                return torch.empty(*shape, dtype=dtype, device=dev)
+
+        def make(*shape, dtype=i32):
+            return torch.empty(*shape, dtype=dtype, device=dev)
+
+        def allocate(st):
             self.cum, self.fin_score = make(G, W, dtype=torch.float32), make(G, W, dtype=torch.float32)
             self.last, self.parent, self.fin_len = make(G, W), make(G, W), make(G, W)
             self.tokens, self.fin_tokens = make(G, W, self.cap), make(G, W, self.cap)
             self.count, self.fin_count, self.done = make(G), make(G), make(G, dtype=torch.uint8)
             self.stop = torch.tensor(list(stop_tokens) or [0], dtype=torch.int64).to(i32).to(dev)
+
+        _launch(dev, stream, allocate)
+        dev = self.device = self.cum.device
         self.n_stop = len(stop_tokens)
         self._c = _StateC(*[getattr(self, n).data_ptr() for n, _ in _StateC._fields_[:-1]], self.cap)
         self._limits = _LimitsC(self.max_tokens, self.max_seq_len, float(length_penalty), int(bool(early_stop)))
+        self._at = ctypes.addressof(self._c), self.stop.data_ptr(), ctypes.addressof(self._limits)
         self.reset(stream)
 
     def reset(self, stream=None) -> None:
         """Begins a new search: one live beam per group with score 0."""
-        with _launch(self.device, stream) as st:
-            _check(self._lib.pesti_beam_reset(ctypes.addressof(self._c), self.groups, self.beams, st))
+        _launch(self.device, stream,
+                lambda st: _check(self._lib.pesti_beam_reset(self._at[0], self.groups, self.beams, st)))
 
     def advance(self, score, token, parent, stream=None) -> None:
         """Takes one step's candidates ([groups, k], as beam_select returns them)."""
-        k = score.shape[-1]
-        for t, want in ((score, torch.float32), (token, torch.int32), (parent, torch.int32)):
-            _on_device(t, self.cum.device, "candidates")
-            _need(t.dtype == want and t.shape == (self.groups, k) and t.is_contiguous(),
-                  "candidates must be contiguous [groups, k] float32, int32 and int32 tensors")
-        with _launch(self.device, stream) as st:
-            _check(self._lib.pesti_beam_advance(
-                ctypes.addressof(self._c), score.data_ptr(), token.data_ptr(), parent.data_ptr(), self.groups,
-                self.beams, k, self.stop.data_ptr(), self.n_stop, ctypes.addressof(self._limits), st))
+        shape, dev = score.shape, self.device
+        if not (len(shape) == 2 and shape[0] == self.groups and token.shape == shape and parent.shape == shape
+                and score.dtype == torch.float32 and token.dtype == torch.int32 and parent.dtype == torch.int32
+                and score.is_contiguous() and token.is_contiguous() and parent.is_contiguous()):
+            raise ValueError("candidates must be contiguous [groups, k] float32, int32 and int32 tensors")
+        if not (score.device == dev and token.device == dev and parent.device == dev):
+            raise ValueError("candidates must be on the state's device")
+        state, stop, limits = self._at
+
+        def call(st):
+            rc = self._lib.pesti_beam_advance(state, score.data_ptr(), token.data_ptr(), parent.data_ptr(),
+                                              self.groups, self.beams, shape[1], stop, self.n_stop, limits, st)
+            if rc:
+                _check(rc)
+
+        _launch(dev, stream, call)
 
     def active(self) -> int:
         """Groups still running (a host read: call it now and then)."""
@@ -221,24 +250,39 @@ class _RowsC(ctypes.Structure):
                                       "blocks", "block_bytes")]
 
 
-def _row_blocks(t):
-    """A row of `t` (all but its first dimension) as (blocks, block elements,
-    elements between blocks)."""
-    run, i = 1, t.dim() - 1
-    while i >= 1 and (t.shape[i] == 1 or t.stride(i) == run):
-        run *= t.shape[i]
+@functools.lru_cache(maxsize=1024)
+def _layout(shape, strides):
+    """A row (all but the first dimension) as (blocks, block elements, elements
+    between blocks)."""
+    run, i = 1, len(shape) - 1
+    while i >= 1 and (shape[i] == 1 or strides[i] == run):
+        run *= shape[i]
         i -= 1
     blocks, step, at = 1, 0, 0
     for j in range(i, 0, -1):
-        if t.shape[j] == 1:
+        if shape[j] == 1:
             continue
         if blocks == 1:
-            step = at = t.stride(j)
-        elif t.stride(j) != at:
+            step = at = strides[j]
+        elif strides[j] != at:
             raise ValueError("a state's rows must be contiguous or equally spaced contiguous blocks")
-        blocks *= t.shape[j]
-        at = t.stride(j) * t.shape[j]
+        blocks *= shape[j]
+        at = strides[j] * shape[j]
     return blocks, run, step
+
+
+def _row_blocks(t):
+    return _layout(t.shape, t.stride())
+
+
+@functools.lru_cache(maxsize=1024)
+def _reorder_strides(shape, src, dst, esize: int):
+    """The six numbers of a pesti_beam_rows behind its pointers, in bytes."""
+    blocks, run, step = _layout(shape, src)
+    to = _layout(shape, dst)
+    if to[:2] != (blocks, run):
+        raise ValueError("out must be laid out in the same blocks as its state")
+    return src[0] * esize, dst[0] * esize, step * esize, to[2] * esize, blocks, run * esize
 
 
 def beam_reorder(states, parent, out=None, stream=None):
@@ -256,25 +300,26 @@ def beam_reorder(states, parent, out=None, stream=None):
     _need(parent.dim() == 2 and parent.dtype == torch.int32 and parent.is_contiguous(),
           "parent must be a contiguous [groups, beams] int32 tensor")
     G, W = parent.shape
-    rows = (_RowsC * max(1, len(src)))()
-    for r, a, b in zip(rows, src, dst):
-        _on_device(a, parent.device, "states")
-        _on_device(b, parent.device, "states")
-        _need(a.dim() >= 1 and a.shape[0] == G * W, "a state's first dimension must be groups*beams")
-        _need(a.shape == b.shape and a.dtype == b.dtype, "out must match the states' shapes and types")
-        e = a.element_size()
-        blocks, run, step = _row_blocks(a)
-        if b is a:
-            to = (blocks, run, step)
-        else:
-            to = _row_blocks(b)
-        if to[:2] != (blocks, run):
-            # the two split differently into contiguous blocks: refuse rather than guess
-            raise ValueError("out must be laid out in the same blocks as its state")
-        r.src, r.dst = a.data_ptr(), b.data_ptr()
-        r.src_row_stride, r.dst_row_stride = a.stride(0) * e, b.stride(0) * e
-        r.src_block_stride, r.dst_block_stride = step * e, to[2] * e
-        r.blocks, r.block_bytes = blocks, run * e
-    with _launch(parent.device, stream) as st:
-        _check(load_library().pesti_beam_reorder(ctypes.addressof(rows), len(src), parent.data_ptr(), G, W, st))
+    dev, first, fields = parent.device, G * W, []
+    for a, b in zip(src, dst):
+        shape = a.shape
+        if not shape or shape[0] != first:
+            raise ValueError("a state's first dimension must be groups*beams")
+        if a.device != dev:
+            raise ValueError("states must be on the parents' device")
+        strides = to = a.stride()
+        if b is not a:
+            if b.shape != shape or b.dtype != a.dtype or b.device != dev:
+                raise ValueError("out must match the states' shapes, types and device")
+            to = b.stride()
+        fields += a.data_ptr(), b.data_ptr()
+        fields += _reorder_strides(shape, strides, to, a.element_size())
+    rows = (ctypes.c_int64 * max(1, len(fields)))(*fields)
+
+    def call(st):
+        rc = load_library().pesti_beam_reorder(ctypes.addressof(rows), len(src), parent.data_ptr(), G, W, st)
+        if rc:
+            _check(rc)
+
+    _launch(dev, stream, call)
     return dst[0] if single else dst

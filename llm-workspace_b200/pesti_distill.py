@@ -8,8 +8,6 @@ the logits' device and the current stream; there is no CPU path.
 """
 from __future__ import annotations
 
-from typing import Optional
-
 import torch
 
 from pesti_beam import _DTYPES, _launch, _need, _on_device, _ptr, _row_stride, _rows_dtype
@@ -26,20 +24,24 @@ def _lists(logits, idx, val, temperature, teacher_lse, weight):
     dev = logits.device
     _need(V >= 1, "V must be at least 1")
     for t, name in ((idx, "idx"), (val, "val")):
-        _on_device(t, dev, name)
-        _need(t.dim() == 2 and t.shape[0] == N and (t.shape[1] <= 1 or t.stride(1) == 1),
-              f"{name} must be [N, k] with contiguous rows")
-    _need(idx.shape == val.shape, "idx and val must have the same shape")
+        if t.device != dev:
+            raise ValueError(f"{name} must be on the logits' device")
+        if t.dim() != 2 or t.shape[0] != N or (t.shape[1] > 1 and t.stride(1) != 1):
+            raise ValueError(f"{name} must be [N, k] with contiguous rows")
+    if idx.shape != val.shape:
+        raise ValueError("idx and val must have the same shape")
     k = idx.shape[1]
-    _need(1 <= k <= MAX_TOP, f"k must be 1 to {MAX_TOP}")
-    _need(idx.dtype == torch.int32, "idx must be int32")
+    if not 1 <= k <= MAX_TOP:
+        raise ValueError(f"k must be 1 to {MAX_TOP}")
+    if idx.dtype != torch.int32:
+        raise ValueError("idx must be int32")
     vtype = _DTYPES.get(val.dtype)
-    _need(vtype is not None, "val must be float32, bfloat16 or float16")
+    if vtype is None:
+        raise ValueError("val must be float32, bfloat16 or float16")
     for t, name in ((teacher_lse, "teacher_lse"), (weight, "weight")):
-        if t is not None:
-            _on_device(t, dev, name)
-            _need(t.dtype == torch.float32 and t.shape == (N,) and t.is_contiguous(),
-                  f"{name} must be a contiguous [N] float32 tensor")
+        if t is not None and not (t.device == dev and t.dtype == torch.float32 and t.shape == (N,)
+                                  and t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous [N] float32 tensor on the logits' device")
     return (logits.data_ptr(), dtype, N, V, _row_stride(logits), idx.data_ptr(), idx.stride(0), val.data_ptr(), vtype,
             val.stride(0), k, _ptr(teacher_lse), _ptr(weight), float(temperature))
 
@@ -48,28 +50,39 @@ class _DistillTopk(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, idx, val, temperature, teacher_lse, weight):
         args = _lists(logits, idx, val, temperature, teacher_lse, weight)
-        N = logits.shape[0]
-        with _launch(logits.device, None) as st:
-            loss = torch.empty(N, dtype=torch.float32, device=logits.device)
-            stats = None
-            if ctx.needs_input_grad[0]:
-                stats = torch.empty(N, _STATS, dtype=torch.float64, device=logits.device)
-            _check(load_library().pesti_distill_topk(*args, loss.data_ptr(), _ptr(stats), None, 0, st))
-        ctx.save_for_backward(logits, idx, val, teacher_lse, weight, stats)
-        ctx.temperature = temperature
+        N, dev, keep = logits.shape[0], logits.device, ctx.needs_input_grad[0]
+
+        def call(st):
+            loss = torch.empty(N, dtype=torch.float32, device=dev)
+            stats = torch.empty((N, _STATS), dtype=torch.float64, device=dev) if keep else None
+            rc = load_library().pesti_distill_topk(*args, loss.data_ptr(), _ptr(stats), None, 0, st)
+            if rc:
+                _check(rc)
+            return loss, stats
+
+        loss, stats = _launch(dev, None, call)
+        if keep:
+            ctx.args = args  # addresses of the tensors saved here
+            ctx.save_for_backward(logits, idx, val, teacher_lse, weight, stats)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, up):
-        logits, idx, val, teacher_lse, weight, stats = ctx.saved_tensors
-        args = _lists(logits, idx, val, ctx.temperature, teacher_lse, weight)
-        up = up.to(torch.float32)
-        with _launch(logits.device, None) as st:
+        saved = ctx.saved_tensors  # refuses tensors that were written to since
+        logits, stats = saved[0], saved[5]
+        if up.dtype != torch.float32:
+            up = up.to(torch.float32)
+
+        def call(st):
             grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-            _check(load_library().pesti_distill_topk_backward(*args, _ptr(stats), up.data_ptr(), up.stride(0),
-                                                              grad.data_ptr(), logits.shape[1], st))
-        return grad, None, None, None, None, None
+            rc = load_library().pesti_distill_topk_backward(*ctx.args, stats.data_ptr(), up.data_ptr(), up.stride(0),
+                                                            grad.data_ptr(), logits.shape[1], st)
+            if rc:
+                _check(rc)
+            return grad
+
+        return _launch(logits.device, None, call), None, None, None, None, None
 
 
 def distill_topk(logits, idx, val, temperature: float = 1.0, teacher_lse=None, weight=None):
@@ -96,13 +109,18 @@ def distill_topk_grad(logits, idx, val, temperature: float = 1.0, teacher_lse=No
     logits = logits.detach()
     args = _lists(logits, idx, val, temperature, teacher_lse, weight)
     N, V = logits.shape
-    with _launch(logits.device, stream) as st:
-        loss = torch.empty(N, dtype=torch.float32, device=logits.device)
-        if grad is None:
-            grad = torch.empty(N, V, dtype=logits.dtype, device=logits.device)
-        else:
-            _on_device(grad, logits.device, "grad")
-            _need(grad.shape == logits.shape and grad.dtype == logits.dtype and (V <= 1 or grad.stride(1) == 1),
-                  "grad must match the logits and have contiguous rows")
-        _check(load_library().pesti_distill_topk(*args, loss.data_ptr(), None, grad.data_ptr(), _row_stride(grad), st))
-    return loss, grad
+    dev = logits.device
+    if grad is not None:
+        _on_device(grad, dev, "grad")
+        _need(grad.shape == logits.shape and grad.dtype == logits.dtype and (V <= 1 or grad.stride(1) == 1),
+              "grad must match the logits and have contiguous rows")
+
+    def call(st):
+        loss = torch.empty(N, dtype=torch.float32, device=dev)
+        to = torch.empty((N, V), dtype=logits.dtype, device=dev) if grad is None else grad
+        rc = load_library().pesti_distill_topk(*args, loss.data_ptr(), None, to.data_ptr(), _row_stride(to), st)
+        if rc:
+            _check(rc)
+        return loss, to
+
+    return _launch(dev, stream, call)
