@@ -2,6 +2,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cmath>
 #include <vector>
@@ -39,7 +40,7 @@ int check_sizes(pesti_dtype dtype, int64_t G, int64_t W, int64_t V, int64_t K) {
   if (W < 1 || W > PESTI_BEAM_MAX_WIDTH) return refuse("W must be 1 to 64");
   if (K < 1 || K > PESTI_BEAM_MAX_CAND) return refuse("K must be 1 to 128");
   if (V < 1 || V > 0x7fffffffLL) return refuse("V must be 1 to 2^31-1");
-  // one block per 8 units in the scan, one per row in the pick
+  // one block per 8 units in the scan, one per group in the pick
   const long long per_row = (units_of(dtype, V) + SCAN_WARPS - 1) / SCAN_WARPS;
   if (G > 0x7fffffffLL / W / per_row) return refuse("G * W * V too large");
   return PESTI_OK;
@@ -48,46 +49,96 @@ int check_sizes(pesti_dtype dtype, int64_t G, int64_t W, int64_t V, int64_t K) {
 long long up256(long long n) { return (n + 255) / 256 * 256; }
 
 // Lays the scratch out behind `base` (which may be null, for the size alone).
-long long layout(char* base, long long G, long long W, long long units, long long K, BeamWs* ws) {
-  const long long rows = G * W;
-  long long at = 0;
-  auto take = [&](long long bytes) {
-    char* p = base ? base + at : nullptr;
-    at += up256(bytes);
-    return p;
-  };
-  BeamWs w;
-  w.unit = (float2*)take(rows * units * (long long)sizeof(float2));
-  w.seg = (uint32_t*)take(rows * units * UNIT_VECS * (long long)sizeof(uint32_t));
-  w.top = (RowTop*)take(rows * (long long)sizeof(RowTop));
-  w.x = (float*)take(rows * K * (long long)sizeof(float));
-  w.idx = (int32_t*)take(rows * K * (long long)sizeof(int32_t));
-  w.arrived = (uint32_t*)take(G * (long long)sizeof(uint32_t));
-  if (ws) *ws = w;
-  return at;
+long long layout(char* base, long long rows, long long units, BeamWs* ws) {
+  const long long unit = up256(rows * units * (long long)sizeof(float2));
+  if (ws) {
+    ws->unit = (float2*)base;
+    ws->seg = (uint32_t*)(base + unit);
+  }
+  return unit + up256(rows * units * UNIT_VECS * (long long)sizeof(uint32_t));
+}
+
+constexpr int kMaxDevices = 64;
+constexpr int kPickSmem = 200 * 1024;
+std::atomic<bool> g_pick_ready[kMaxDevices];
+
+template <typename T, int TW>
+cudaError_t allow_pick_teams() {
+  const cudaError_t e =
+      cudaFuncSetAttribute(beam_pick_kernel<T, TW, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPickSmem);
+  if (e != cudaSuccess) return e;
+  return cudaFuncSetAttribute(beam_pick_kernel<T, TW, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPickSmem);
 }
 
 template <typename T>
-int run_select(const void* logits, long long G, long long W, long long V, long long ld, const float* cum,
-               const uint8_t* done, int K, float* score, int32_t* token, int32_t* parent, float* lse,
-               const BeamWs& ws, long long units, cudaStream_t st) {
-  const long long per_row = (units + SCAN_WARPS - 1) / SCAN_WARPS;
-  beam_scan_kernel<T><<<(unsigned)(G * W * per_row), SCAN_WARPS * 32, 0, st>>>(
-      (const T*)logits, ld, V, (int)W, units, per_row, cum, done, lse != nullptr, ws);
-  int rc = launched("beam_scan_kernel launch");
-  if (rc) return rc;
+cudaError_t allow_pick() {
+  const cudaError_t e = allow_pick_teams<T, 3>();
+  return e == cudaSuccess ? allow_pick_teams<T, 7>() : e;
+}
+
+int set_up_pick() {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return pesti_set_cuda_error(e, "cudaGetDevice");
+  if (dev >= kMaxDevices) return refuse("device index out of range");
+  if (g_pick_ready[dev].load(std::memory_order_acquire)) return PESTI_OK;
+  e = allow_pick<float>();
+  if (e == cudaSuccess) e = allow_pick<__nv_bfloat16>();
+  if (e == cudaSuccess) e = allow_pick<__half>();
+  if (e != cudaSuccess) return pesti_set_cuda_error(e, "beam_pick_kernel set-up");
+  g_pick_ready[dev].store(true, std::memory_order_release);
+  return PESTI_OK;
+}
+
+template <typename T, int TW>
+int launch_pick(const void* logits, long long G, long long V, long long ld, PickPlan pl, const float* cum,
+                const uint8_t* done, const BeamWs& ws, float* score, int32_t* token, int32_t* parent, float* lse,
+                cudaStream_t st) {
+  // A list takes what one round of a team's segments appends to a pruned one;
+  // the keys get what is left of the shared memory (longer rows: the maxima of
+  // runs of segments).
+  const long long nseg = pl.units * UNIT_VECS;
+  const long long lists = ((long long)pl.W * pl.K * 8 + 15) / 16 * 16;
+  pl.cap = RANK_CAP + TW * 256;
+  const long long most = (kPickSmem - lists) / pl.teams / 4 - (pl.cap * 2 + TEAM_WORDS + 4);
+  pl.run = (int)((nseg + most - 1) / most);
+  pl.nkeys = (int)((nseg + pl.run - 1) / pl.run);
+  const long long body = std::max(pl.teams * team_bytes(pl.nkeys, pl.cap), lists);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(G * W));
-  cfg.blockDim = dim3(PICK_THREADS);
+  cfg.gridDim = dim3((unsigned)G);
+  cfg.blockDim = dim3((unsigned)(pl.teams * (TW + 1) * 32));
+  cfg.dynamicSmemBytes = (size_t)(lists + body);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, beam_pick_kernel<T>, (const T*)logits, ld, V, (int)W, K, units, cum,
-                                           done, (int)(lse != nullptr), ws, score, token, parent, lse);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, pl.run == 1 ? beam_pick_kernel<T, TW, false> : beam_pick_kernel<T, TW, true>,
+                                           (const T*)logits, ld, V, (const PickPlan)pl, cum, done, ws, score, token,
+                                           parent, lse);
   return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, "beam_pick_kernel launch");
+}
+
+template <typename T>
+int run_select(const void* logits, long long G, long long W, long long V, long long ld, const float* cum,
+               const uint8_t* done, int K, float* score, int32_t* token, int32_t* parent, float* lse,
+               const BeamWs& ws, long long units, cudaStream_t st) {
+  int rc = set_up_pick();
+  if (rc) return rc;
+  const long long per_row = (units + SCAN_WARPS - 1) / SCAN_WARPS;
+  beam_scan_kernel<T><<<(unsigned)(G * W * per_row), SCAN_WARPS * 32, 0, st>>>(
+      (const T*)logits, ld, V, (int)W, units, per_row, cum, done, lse != nullptr, ws);
+  rc = launched("beam_scan_kernel launch");
+  if (rc) return rc;
+  PickPlan pl{};
+  pl.W = (int)W;
+  pl.K = K;
+  pl.units = units;
+  pl.teams = (int)std::min<long long>(W, MAX_TEAMS);
+  // a block of at most 32 warps: as many for each beam as fit
+  if (W <= 4) return launch_pick<T, 7>(logits, G, V, ld, pl, cum, done, ws, score, token, parent, lse, st);
+  return launch_pick<T, 3>(logits, G, V, ld, pl, cum, done, ws, score, token, parent, lse, st);
 }
 
 int check_state(const pesti_beam_state* s, int64_t G, int64_t W) {
@@ -153,7 +204,7 @@ extern "C" {
 int64_t pesti_beam_select_workspace(pesti_dtype dtype, int64_t G, int64_t W, int64_t V, int64_t K) {
   const int rc = check_sizes(dtype, G, W, V, K);
   if (rc) return rc;
-  return layout(nullptr, G, W, units_of(dtype, V), K, nullptr);
+  return layout(nullptr, G * W, units_of(dtype, V), nullptr);
 }
 
 int pesti_beam_select(const void* d_logits, pesti_dtype dtype, int64_t G, int64_t W, int64_t V, int64_t ld,
@@ -168,7 +219,7 @@ int pesti_beam_select(const void* d_logits, pesti_dtype dtype, int64_t G, int64_
   if ((uintptr_t)d_logits % (dtype == PESTI_F32 ? 4 : 2)) return refuse("logits are not aligned to their type");
   const long long units = units_of(dtype, V);
   BeamWs ws;
-  const long long need = layout((char*)d_ws, G, W, units, K, &ws);
+  const long long need = layout((char*)d_ws, G * W, units, &ws);
   if (!d_ws || ws_bytes < need) return refuse("workspace too small");
   if ((uintptr_t)d_ws % 256) return refuse("workspace is not 256-byte aligned");
   rc = need_device();

@@ -13,10 +13,12 @@
 //                     (pesti_rowscan.cuh) in registers and writes the unit's
 //                     maximum m and S = sum 2^(x*c - R), c = f32(log2 e),
 //                     R = ceil(m*c), and its 8 segment maxima.
-//  beam_pick_kernel   one block per row: the K segments with the largest
-//                     maxima hold the K largest logits; they are read again
-//                     and sorted.  The block that finishes a group last
-//                     merges its W lists.
+//  beam_pick_kernel   one block per group.  For each beam, the K segments with
+//                     the largest maxima hold the K largest logits: a team of
+//                     warps finds them (a histogram of the maxima, its K-th
+//                     place), reads them again and sorts what is above the
+//                     K-th maximum, while another warp joins the row's sum.
+//                     Then the block merges the W lists.
 //
 // Accuracy of a row's log sum as the scan gives it, relative to the sum:
 //   2^x by the hardware 2^-22.5; the rounding of x*c - R (one fused
@@ -38,11 +40,10 @@ namespace pesti_rows {
 constexpr int MAX_W = 64;          // beams of a group
 constexpr int MAX_K = 128;         // candidates of a group
 constexpr int SCAN_WARPS = 8;
-constexpr int PICK_THREADS = 256;
-constexpr int MAX_SEG_KEYS = 4096; // segment maxima a block holds (wider rows: maxima of runs of segments)
+constexpr int MAX_TEAMS = 8;
 constexpr int MAX_SEL = MAX_K + MAX_K / 2 + 8;
-constexpr int LIST_CAP = 3072;     // candidates a block holds
-constexpr int RANK_CAP = 256;      // candidates it ranks by counting
+constexpr int BINS = 256;
+constexpr int RANK_CAP = 256;      // candidates that are ranked by counting
 constexpr double LSE_EPS = 3e-6;
 constexpr float LOG2E_F = 1.44269504088896340736f;
 constexpr double LN2 = 0.69314718055994530942;
@@ -57,20 +58,9 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 }
 constexpr uint32_t KEY_NEG_INF = 0x007fffffu;  // order_key(-inf); NaN counts as -inf
 
-struct RowTop {
-  double ref;   // logp(x) = (x - ref) - logs, or -logs for x = +inf when ref is +inf
-  double logs;
-  int n;        // entries of the row's list
-  int pad;
-};
-
 struct BeamWs {
-  float2* unit;      // [rows][units] maximum and sum
-  uint32_t* seg;     // [rows][units*8] order keys of the segment maxima
-  RowTop* top;       // [rows]
-  float* x;          // [rows][K]
-  int32_t* idx;      // [rows][K]
-  uint32_t* arrived; // [G]
+  float2* unit;   // [rows][units] maximum and sum
+  uint32_t* seg;  // [rows][units*8] order keys of the segment maxima
 };
 
 __device__ __forceinline__ bool beam_running(const float* cum, long long row) {
@@ -85,7 +75,6 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32) beam_scan_kernel(const T* __r
   const long long row = blockIdx.x / blocks_per_row;
   const long long ub = blockIdx.x - row * blocks_per_row;
   const long long g = row / W;
-  if (ub == 0 && row == g * W && threadIdx.x == 0) ws.arrived[g] = 0u;
   // rows that take no part are not read
   if (done && done[g]) return;
   if (!every_row && !beam_running(cum, row)) return;
@@ -150,357 +139,495 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32) beam_scan_kernel(const T* __r
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
-// Sum over the block of small counts; `buf` alternates between two rows of 8.
-__device__ __forceinline__ int block_count(int c, int (*buf)[PICK_THREADS / 32], int& turn) {
-  const int s = __reduce_add_sync(FULL, c);
-  if ((threadIdx.x & 31) == 0) buf[turn][threadIdx.x >> 5] = s;
-  __syncthreads();
-  int t = 0;
-#pragma unroll
-  for (int i = 0; i < PICK_THREADS / 32; ++i) t += buf[turn][i];
-  turn ^= 1;
-  return t;
-}
-
-struct PickShared {
-  union {
-    struct {
-      uint32_t keys[MAX_SEG_KEYS];
-      unsigned long long list[LIST_CAP];
-    } row;
-    struct {
-      float x[MAX_W * MAX_K];
-    } merge;
-  };
-  unsigned long long sorted_c[RANK_CAP];
-  double ref[MAX_W], logs[MAX_W], cum[MAX_W];
-  int n[MAX_W];
-  int sel[MAX_SEL];
-  int count[2][PICK_THREADS / 32];
-  int scan[40];
-  double red[40];
-  int nsel, nlist, over, last, end;
-  unsigned long long flagged;
+// The block of a group: `teams` teams of TW warps that select, then as many
+// warps that join sums.  A team's arrays lie in dynamic shared memory behind
+// the x and idx of the group's lists; the merge's scores take their place.
+struct PickPlan {
+  int W, K, teams, nkeys, run, cap;  // run: segments of a key; cap: entries of a team's list
+  long long units;
 };
 
-// Appends the elements of segment s with key >= t to the list (at most LIST_CAP; `over` if there are more).
-template <typename T>
-__device__ __forceinline__ void append_vec(PickShared& sh, const uint4& v, long long first, uint32_t t) {
+template <int TW>
+struct Team {
+  int id, tid;                    // team, thread of the team
+  uint32_t* keys;                 // [nkeys]
+  unsigned long long* list;       // [cap] key << 32 | ~index
+  int* hist;                      // [BINS]
+  int* sel;                       // [MAX_SEL]
+  int* word;                      // 32 words, below
+  int turn;
+};
+enum { TM_NSEL = 0, TM_NLIST = 1, TM_OVER = 2, TM_T = 3, TM_MAX = 4, TM_MIN = 5, TM_CUT = 6, TM_COUNT = 8 };  // COUNT: 2 x 8
+
+constexpr int TEAM_WORDS = BINS + MAX_SEL + 32;
+
+__host__ __device__ __forceinline__ long long team_bytes(int nkeys, int cap) {
+  return ((long long)cap * 8 + (long long)(nkeys + TEAM_WORDS) * 4 + 15) / 16 * 16;
+}
+
+template <int TW>
+__device__ __forceinline__ void team_sync(const Team<TW>& t) {
+  if (TW == 1)
+    __syncwarp();
+  else
+    asm volatile("bar.sync %0, %1;" ::"r"(t.id + 1), "n"(TW * 32) : "memory");
+}
+
+// Sum over the team of one count per thread.
+template <int TW>
+__device__ __forceinline__ int team_count(Team<TW>& t, int c) {
+  const int s = __reduce_add_sync(FULL, c);
+  if (TW == 1) return s;
+  int* buf = t.word + TM_COUNT + t.turn * 8;
+  t.turn ^= 1;
+  if ((t.tid & 31) == 0) buf[t.tid >> 5] = s;
+  team_sync(t);
+  int r = 0;
+#pragma unroll
+  for (int i = 0; i < TW; ++i) r += buf[i];
+  return r;
+}
+
+// Appends a vector's elements >= cut to the team's list (OVER is set if they do not fit).
+template <typename T, int TW>
+__device__ __forceinline__ void append_vec(const Team<TW>& t, int cap, const uint4& v, long long first, float cut) {
+  uint32_t in = 0;
 #pragma unroll
   for (int q = 0; q < Elem<T>::PAIRS; ++q) {
     const float2 x = Elem<T>::pair(v, q);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float f = e ? x.y : x.x;
-      const uint32_t k = order_key(f);
-      if (f == f && k >= t) {
-        const int at = atomicAdd(&sh.nlist, 1);
-        if (at < LIST_CAP)
-          sh.row.list[at] = ((unsigned long long)k << 32) | (uint32_t)~(uint32_t)(first + q * 2 + e);
-        else
-          sh.over = 1;
-      }
-    }
+    in |= (x.x >= cut ? 1u : 0u) << (2 * q) | (x.y >= cut ? 2u : 0u) << (2 * q);
+  }
+  while (in) {
+    const int e = __ffs(in) - 1;
+    in &= in - 1;
+    const int at = atomicAdd(t.word + TM_NLIST, 1);
+    if (at < cap)
+      t.list[at] = ((unsigned long long)order_key(Elem<T>::at(v, e)) << 32) | (uint32_t)~(uint32_t)(first + e);
+    else
+      t.word[TM_OVER] = 1;
   }
 }
 
 template <typename T>
-__device__ __forceinline__ uint4 load_seg_vec(const T* p, int head, long long V, long long seg, int lane,
-                                              long long& first) {
-  first = (seg * 32 + lane) * Elem<T>::VE - head;
+__device__ __forceinline__ uint4 load_seg_vec(const T* p, int head, long long V, long long seg, int lane) {
+  const long long first = (seg * 32 + lane) * Elem<T>::VE - head;
   if (first >= 0 && first + Elem<T>::VE <= V) return __ldg((const uint4*)(p - head) + seg * 32 + lane);
   return load_edge<T>(p, first, V);
 }
 
-// Cuts the list to its largest entries: at least K and at most `most` (entries are distinct).
-__device__ __forceinline__ void prune_list(PickShared& sh, int K, int most, int& turn) {
-  __syncthreads();
-  const int n = sh.nlist;
-  __syncthreads();  // every thread has read it before the next append
-  if (n <= most) return;
+// Cuts the list to its largest entries, at least K and at most RANK_CAP (entries are distinct).
+template <int TW>
+__device__ __noinline__ void prune_list(Team<TW>& t, int K) {
+  constexpr int N = TW * 32, PER = (RANK_CAP + TW * 256 + N - 1) / N;
+  team_sync(t);
+  const int n = t.word[TM_NLIST];
+  team_sync(t);  // every thread has read it before the next append
+  if (n <= RANK_CAP) return;
   unsigned long long lo = 0, hi = ~0ull;
   while (hi - lo > 1) {
     const unsigned long long mid = lo + (hi - lo) / 2;
     int c = 0;
-    for (int i = threadIdx.x; i < n; i += PICK_THREADS) c += sh.row.list[i] >= mid;
-    c = block_count(c, sh.count, turn);
+    for (int i = t.tid; i < n; i += N) c += t.list[i] >= mid;
+    c = team_count(t, c);
     if (c >= K) {
       lo = mid;
-      if (c <= most) break;
+      if (c <= RANK_CAP) break;
     } else {
       hi = mid;
     }
   }
   // entries kept move to the front; each thread holds its own first
-  unsigned long long mine[LIST_CAP / PICK_THREADS];
+  unsigned long long mine[PER];
 #pragma unroll
-  for (int j = 0; j < LIST_CAP / PICK_THREADS; ++j) {
-    const int i = threadIdx.x + j * PICK_THREADS;
-    mine[j] = i < n ? sh.row.list[i] : 0ull;
+  for (int j = 0; j < PER; ++j) {
+    const int i = t.tid + j * N;
+    mine[j] = i < n ? t.list[i] : 0ull;
   }
-  __syncthreads();
-  if (threadIdx.x == 0) sh.nlist = 0;
-  __syncthreads();
+  team_sync(t);
+  if (t.tid == 0) t.word[TM_NLIST] = 0;
+  team_sync(t);
 #pragma unroll
-  for (int j = 0; j < LIST_CAP / PICK_THREADS; ++j)
-    if (mine[j] != 0ull && mine[j] >= lo) sh.row.list[atomicAdd(&sh.nlist, 1)] = mine[j];
-  __syncthreads();
+  for (int j = 0; j < PER; ++j)
+    if (mine[j] != 0ull && mine[j] >= lo) t.list[atomicAdd(t.word + TM_NLIST, 1)] = mine[j];
+  team_sync(t);
 }
+
+// The least key of the segments to read, by bisection, and those segments:
+// for maxima that the histogram does not tell apart.
+template <int TW>
+__device__ __noinline__ uint32_t select_by_bisection(Team<TW>& t, int nkeys, int K, uint32_t kmax, int most) {
+  constexpr int N = TW * 32;
+  uint32_t lo = KEY_NEG_INF + 1, hi = kmax + 1;
+  int above = most + 1;
+  while (hi - lo > 1 && above > most) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    int c = 0;
+    for (int i = t.tid; i < nkeys; i += N) c += t.keys[i] >= mid;
+    c = team_count(t, c);
+    if (c >= K) {
+      lo = mid;
+      above = c;
+    } else {
+      hi = mid;
+    }
+  }
+  if (above <= most) {
+    for (int i = t.tid; i < nkeys; i += N)
+      if (t.keys[i] >= lo) t.sel[atomicAdd(t.word + TM_NSEL, 1)] = i;
+  } else {
+    // many segments share the K-th maximum: those above it, then the first ones at it
+    int c = 0;
+    for (int i = t.tid; i < nkeys; i += N) c += t.keys[i] > lo;
+    const int over = team_count(t, c);
+    if (t.tid < 32) {
+      int left = K - over;
+      for (int i0 = 0; i0 < nkeys; i0 += 32) {
+        const int i = i0 + t.tid;
+        const uint32_t k = i < nkeys ? t.keys[i] : 0u;
+        const uint32_t same = __ballot_sync(FULL, k == lo);
+        const int before = __popc(same & ((1u << t.tid) - 1u));
+        if (k > lo || (k == lo && before < left)) t.sel[atomicAdd(t.word + TM_NSEL, 1)] = i;
+        left -= min(left, __popc(same));
+      }
+    }
+  }
+  return lo;
+}
+
+// Segment i of the selected ones (WIDE: runs of segments).
+template <bool WIDE, int TW>
+__device__ __forceinline__ long long selected(const Team<TW>& t, const PickPlan& pl, int i) {
+  return WIDE ? (long long)t.sel[i / pl.run] * pl.run + i % pl.run : (long long)t.sel[i];
+}
+
+// The elements of the selected segments in rounds that keep the list short.
+template <typename T, int TW, bool WIDE>
+__device__ __noinline__ void append_in_rounds(Team<TW>& t, const PickPlan& pl, const T* p, long long V, int todo,
+                                              float cut) {
+  const int lane = t.tid & 31, head = row_head<T>(p);
+  team_sync(t);
+  if (t.tid == 0) t.word[TM_NLIST] = 0;
+  team_sync(t);
+  for (int i0 = 0; i0 < todo; i0 += TW) {
+    const int i = i0 + (t.tid >> 5);
+    if (i < todo) {
+      const long long sg = selected<WIDE>(t, pl, i);
+      const uint4 v = load_seg_vec<T>(p, head, V, sg, lane);
+      // at most TW * 256 behind at most RANK_CAP
+      append_vec<T, TW>(t, pl.cap, v, (sg * 32 + lane) * Elem<T>::VE - head, cut);
+    }
+    prune_list(t, pl.K);
+  }
+}
+
+// The K largest logits of a row, in order, to x and idx; returns their number.
+// Nearly all of this runs once: its time is instruction fetches and the
+// latency of two dependent reads, so loops stay rolled unless they load.
+template <typename T, int TW, bool WIDE>
+__device__ __forceinline__ int pick_row(Team<TW>& t, const PickPlan& pl, const T* p, long long V, const uint32_t* seg,
+                                        float* xs, int32_t* ids) {
+  constexpr int N = TW * 32;
+  const int lane = t.tid & 31, K = pl.K, nkeys = pl.nkeys;
+  if (WIDE) {
+    const long long nseg = pl.units * UNIT_VECS;
+    for (int i = t.tid; i < nkeys; i += N) {
+      uint32_t k = KEY_NEG_INF;
+      const long long end = min(nseg, (long long)(i + 1) * pl.run);
+      for (long long j = (long long)i * pl.run; j < end; ++j) k = max(k, seg[j]);
+      t.keys[i] = k;
+    }
+  } else {
+    // 16 keys of a thread in flight at once (their number is a multiple of 8)
+    for (int i0 = t.tid * 4; i0 < nkeys; i0 += N * 16) {
+      uint4 k[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i0 + j * N * 4 < nkeys) k[j] = *(const uint4*)(seg + i0 + j * N * 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i0 + j * N * 4 < nkeys) *(uint4*)(t.keys + i0 + j * N * 4) = k[j];
+    }
+  }
+  for (int i = t.tid; i < BINS; i += N) t.hist[i] = 0;
+  if (t.tid < TM_COUNT)
+    t.word[t.tid] = t.tid == TM_T || t.tid == TM_MIN ? (int)0xffffffffu : 0;
+  team_sync(t);
+  uint32_t kmax = KEY_NEG_INF, kmin = 0xffffffffu;
+  int valid = 0;
+#pragma unroll 2
+  for (int i = t.tid; i < nkeys; i += N) {
+    const uint32_t k = t.keys[i];
+    const bool v = k > KEY_NEG_INF;
+    valid += v;
+    kmin = min(kmin, v ? k : 0xffffffffu);
+    kmax = max(kmax, k);
+  }
+  kmax = __reduce_max_sync(FULL, kmax);
+  kmin = __reduce_min_sync(FULL, kmin);
+  if (lane == 0) {
+    atomicMax((uint32_t*)t.word + TM_MAX, kmax);
+    atomicMin((uint32_t*)t.word + TM_MIN, kmin);
+  }
+  valid = team_count(t, valid);
+  kmax = (uint32_t)t.word[TM_MAX];
+  kmin = (uint32_t)t.word[TM_MIN];
+  if (valid == 0) return 0;
+  const int most = K + K / 2 + 8;
+  bool binned = valid > most && kmax != kmin;
+  uint32_t least = KEY_NEG_INF + 1;
+  if (valid <= most) {
+    for (int i = t.tid; i < nkeys; i += N)
+      if (t.keys[i] > KEY_NEG_INF) t.sel[atomicAdd(t.word + TM_NSEL, 1)] = i;
+  }
+  if (binned) {
+    // 256 bins of equal width of the keys, from the largest down (over four powers of two at most)
+    const int sh = max(0, 24 - __clz((int)min(kmax - kmin, 0x1ffffffu)));
+#pragma unroll 2
+    for (int i = t.tid; i < nkeys; i += N) {
+      const uint32_t b = (kmax - t.keys[i]) >> sh;
+      if (b < BINS) atomicAdd(t.hist + b, 1);
+    }
+    team_sync(t);
+    if (t.tid < 32) {
+      // lane l adds up bins 8l..8l+7; the first bin whose running count reaches K
+      const int4 c0 = ((const int4*)t.hist)[2 * lane], c1 = ((const int4*)t.hist)[2 * lane + 1];
+      const int sum = c0.x + c0.y + c0.z + c0.w + c1.x + c1.y + c1.z + c1.w;
+      int upto = warp_incl_scan_add(sum);
+      const uint32_t hit = __ballot_sync(FULL, upto >= K);
+      if (hit == 0) {
+        if (lane == 0) t.word[TM_CUT] = -1;
+      } else if (lane == __ffs(hit) - 1) {
+        upto -= sum;
+        int bin = 8 * lane - 1;
+        while (upto < K) upto += t.hist[++bin];
+        t.word[TM_CUT] = upto <= most ? bin : -1;
+      }
+    }
+    team_sync(t);
+    const int bin = t.word[TM_CUT];
+    binned = bin >= 0;
+    if (binned) {
+      least = 0xffffffffu;
+#pragma unroll 2
+      for (int i = t.tid; i < nkeys; i += N) {
+        const uint32_t k = t.keys[i];
+        if ((kmax - k) >> sh <= (uint32_t)bin) {
+          t.sel[atomicAdd(t.word + TM_NSEL, 1)] = i;
+          least = min(least, k);
+        }
+      }
+      least = __reduce_min_sync(FULL, least);
+    }
+  }
+  if (valid > most && !binned) least = select_by_bisection(t, nkeys, K, kmax, most);
+  if (lane == 0) atomicMin((uint32_t*)t.word + TM_T, least);
+  team_sync(t);
+  const float cut = key_value((uint32_t)t.word[TM_T]);
+  // their elements from the cut up: all at once, or in rounds that keep the list short
+  const int todo = t.word[TM_NSEL] * (WIDE ? pl.run : 1), head = row_head<T>(p);
+  for (int i0 = t.tid >> 5; i0 < todo; i0 += 8 * TW) {
+    uint4 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i0 + j * TW < todo) v[j] = load_seg_vec<T>(p, head, V, selected<WIDE>(t, pl, i0 + j * TW), lane);
+    uint32_t in = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i0 + j * TW < todo) in |= (Elem<T>::vec_max(v[j]) >= cut ? 1u : 0u) << j;
+    while (in) {
+      const int j = __ffs(in) - 1;
+      in &= in - 1;
+      uint4 w = v[0];
+#pragma unroll
+      for (int q = 1; q < 8; ++q)
+        if (q == j) w = v[q];
+      append_vec<T, TW>(t, pl.cap, w, (selected<WIDE>(t, pl, i0 + j * TW) * 32 + lane) * Elem<T>::VE - head, cut);
+    }
+  }
+  team_sync(t);
+  if (t.word[TM_OVER]) append_in_rounds<T, TW, WIDE>(t, pl, p, V, todo, cut);
+  if (t.word[TM_NLIST] > RANK_CAP) prune_list(t, K);
+  const int nl = t.word[TM_NLIST];
+  int tops = 0;
+  for (int i = t.tid; i < nl; i += N) {
+    const unsigned long long c = t.list[i];
+    int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < nl; ++j) rank += t.list[j] > c;
+    if (rank < K) {
+      xs[rank] = key_value((uint32_t)(c >> 32));
+      ids[rank] = (int32_t)~(uint32_t)c;
+    }
+    tops += (uint32_t)(c >> 32) == 0xff800000u;  // +inf
+  }
+  int n = min(nl, K);
+  // a row's +inf entries share its probability; the others have none
+  if (kmax == 0xff800000u) n = min(n, team_count(t, tops));
+  return n;
+}
+
+struct PickShared {
+  double ref[MAX_W], logs[MAX_W], cum[MAX_W];  // logp(x) = (x - ref) - logs, or -logs for x = ref = +inf
+  double red[40];
+  int n[MAX_W];
+  int sorted[RANK_CAP];
+  unsigned long long flagged;
+};
 
 __device__ __forceinline__ double beam_score(const PickShared& sh, int w, float x) {
   return sh.ref[w] == (double)pos_inf() ? sh.cum[w] - sh.logs[w] : sh.cum[w] + (((double)x - sh.ref[w]) - sh.logs[w]);
 }
 
-// Order-preserving image of a double (no NaN).
+// Order-preserving image of a double (no NaN), and back.
 __device__ __forceinline__ unsigned long long order_key64(double d) {
   const unsigned long long b = (unsigned long long)__double_as_longlong(d + 0.0);
   return (b >> 63) ? ~b : (b | 0x8000000000000000ull);
 }
+__device__ __forceinline__ double key_value64(unsigned long long k) {
+  return __longlong_as_double((long long)((k >> 63) ? (k & 0x7fffffffffffffffull) : ~k));
+}
 
-// Ranks the candidates of the group's lists; those with rank < RANK_CAP go to
-// sorted_c as list positions w * K + r.
-__device__ __forceinline__ int rank_candidates(PickShared& sh, int W, int K) {
+// Ranks the candidates of the group's lists; `sorted` gets the positions
+// w * K + r of the first RANK_CAP.  Returns their number.
+__device__ __forceinline__ int rank_candidates(PickShared& sh, const float* xs, unsigned long long* score, int W, int K) {
   int total = 0;
   for (int w = 0; w < W; ++w) total += sh.n[w];
-  for (int j = threadIdx.x; j < W * K; j += PICK_THREADS) {
-    const int w = j / K, r = j - w * K;
-    if (r >= sh.n[w]) continue;
-    const double s = beam_score(sh, w, sh.merge.x[j]);
-    int rank = r;
-    for (int o = 0; o < W && rank < RANK_CAP; ++o) {
-      if (o == w) continue;
-      // entries of beam o ahead of s: equal ones count when o is the lower beam
-      int lo = 0, hi = sh.n[o];
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        const double q = beam_score(sh, o, sh.merge.x[o * K + mid]);
-        if (q > s || (q == s && o < w))
-          lo = mid + 1;
-        else
-          hi = mid;
+  const int all = W * K;
+  for (int j = threadIdx.x; j < all; j += blockDim.x) {
+    const int w = j / K;
+    score[j] = j - w * K < sh.n[w] ? order_key64(beam_score(sh, w, xs[j])) : 0ull;
+  }
+  __syncthreads();
+  for (int j = threadIdx.x; j < all; j += blockDim.x) {
+    const unsigned long long s = score[j];
+    if (s == 0ull) continue;
+    int rank = 0;
+    if (all <= 256) {
+      // ahead: larger, or equal and of a lower beam (or earlier in the list)
+#pragma unroll 4
+      for (int o = 0; o < all; ++o) rank += score[o] + (o < j) > s;
+    } else {
+      const int w = j / K;
+      rank = j - w * K;
+      for (int o = 0; o < W && rank < RANK_CAP; ++o) {
+        if (o == w) continue;
+        int lo = 0, hi = sh.n[o];
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (score[o * K + mid] >= s + (o > w))
+            lo = mid + 1;
+          else
+            hi = mid;
+        }
+        rank += lo;
       }
-      rank += lo;
     }
-    if (rank < RANK_CAP) sh.sorted_c[rank] = (unsigned long long)j;
+    if (rank < RANK_CAP) sh.sorted[rank] = j;
   }
   __syncthreads();
   return total;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(PICK_THREADS) beam_pick_kernel(const T* __restrict__ logits, long long ld,
-                                                                 long long V, int W, int K, long long units,
-                                                                 const float* cum, const uint8_t* done, int every_row,
-                                                                 BeamWs ws, float* out_score, int32_t* out_token,
-                                                                 int32_t* out_parent, float* out_lse) {
+template <typename T, int TW, bool WIDE>
+__global__ void __launch_bounds__(1024) beam_pick_kernel(const T* __restrict__ logits, long long ld, long long V,
+                                                         const __grid_constant__ PickPlan pl, const float* cum,
+                                                         const uint8_t* done, BeamWs ws, float* out_score,
+                                                         int32_t* out_token, int32_t* out_parent, float* out_lse) {
+  extern __shared__ __align__(16) char dyn[];
   __shared__ PickShared sh;
-  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-  const long long row = blockIdx.x;
-  const long long g = row / W;
-  int turn = 0;
+  const int tid = threadIdx.x, lane = tid & 31, W = pl.W, K = pl.K;
+  const long long g = blockIdx.x, row0 = g * W;
+  float* xs = (float*)dyn;
+  int32_t* ids = (int32_t*)(xs + W * K);
+  char* teams = dyn + ((long long)W * K * 8 + 15) / 16 * 16;
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   const bool group_done = done && done[g];
-  const bool live = !group_done && beam_running(cum, row);
-  const T* p = logits + row * ld;
-  const int head = row_head<T>(p);
-  if (tid == 0) {
-    sh.nsel = 0;
-    sh.nlist = 0;
-    sh.over = 0;
-  }
-  double ref = 0.0, logs = 0.0;
-  int n = 0;
-  if (!group_done && (live || every_row)) {
-    // the row's sum, joined from its units in a fixed order
-    const float2* unit = ws.unit + row * units;
-    float m = neg_inf();
-    for (long long u = tid; u < units; u += PICK_THREADS) m = fmaxf(m, unit[u].x);
-    m = block_reduce_max(m, (float*)sh.scan);
-    const bool inf = m == pos_inf(), none = !(m > neg_inf());
-    double s = 0.0;
-    for (long long u = tid; u < units; u += PICK_THREADS) {
-      const float2 a = unit[u];
-      if (a.x > neg_inf()) s += (double)a.y * ref_scale(a.x, m, LOG2E_F);
+  const int wid = tid >> 5;
+  if (wid < pl.teams * TW) {
+    Team<TW> t;
+    t.id = wid / TW;
+    t.tid = tid - t.id * TW * 32;
+    t.turn = 0;
+    t.list = (unsigned long long*)(teams + t.id * team_bytes(pl.nkeys, pl.cap));
+    t.keys = (uint32_t*)(t.list + pl.cap);
+    t.hist = (int*)(t.keys + pl.nkeys);
+    t.sel = t.hist + BINS;
+    t.word = t.sel + MAX_SEL;
+    for (int w = t.id; w < W; w += pl.teams) {
+      int n = 0;
+      if (!group_done && beam_running(cum, row0 + w))
+        n = pick_row<T, TW, WIDE>(t, pl, logits + (row0 + w) * ld, V, ws.seg + (row0 + w) * pl.units * UNIT_VECS, xs + w * K,
+                            ids + w * K);
+      if (t.tid == 0) sh.n[w] = n;
+      team_sync(t);
     }
-    s = block_reduce_add(s, sh.red);
-    if (!none) {
-      // sum 2^(x c - R) = 2^(m c - R) sum 2^((x - m) c)
-      ref = (double)m;
-      logs = is_far(m, LOG2E_F) ? log(s)
-                                : LN2 * (log2(s) - ((double)m * (double)LOG2E_F - (double)ceilf(m * LOG2E_F)));
-    }
-    if (out_lse && tid == 0) out_lse[row] = none ? neg_inf() : inf ? pos_inf() : (float)(ref + logs);
-
-    if (live && !none) {
-      // the segments that hold the K largest logits
-      const long long nseg = units * UNIT_VECS;
-      const int run = (int)((nseg + MAX_SEG_KEYS - 1) / MAX_SEG_KEYS);
-      const int nkeys = (int)((nseg + run - 1) / run);
-      const uint32_t* seg = ws.seg + row * nseg;
-      int valid = 0;
-      for (int i = tid; i < nkeys; i += PICK_THREADS) {
-        uint32_t k = KEY_NEG_INF;
-        const long long end = min(nseg, (long long)(i + 1) * run);
-        for (long long j = (long long)i * run; j < end; ++j) k = max(k, seg[j]);
-        sh.row.keys[i] = k;
-        valid += k > KEY_NEG_INF;
-      }
-      valid = block_count(valid, sh.count, turn);
-      uint32_t t = KEY_NEG_INF + 1;  // every segment with a finite value
-      int above = valid;
-      if (valid > K) {
-        uint32_t lo = t, hi = order_key(m) + 1;
-        const int most = K + K / 2 + 8;
-        while (hi - lo > 1 && above > most) {
-          const uint32_t mid = lo + (hi - lo) / 2;
-          int c = 0;
-          for (int i = tid; i < nkeys; i += PICK_THREADS) c += sh.row.keys[i] >= mid;
-          c = block_count(c, sh.count, turn);
-          if (c >= K) {
-            lo = mid;
-            above = c;
-          } else {
-            hi = mid;
+  } else {
+    for (int w = wid - pl.teams * TW; w < W; w += pl.teams) {
+      // the row's sum, joined from its units in a fixed order
+      const long long row = row0 + w;
+      double ref = 0.0, logs = 0.0;
+      if (!group_done && (out_lse || beam_running(cum, row))) {
+        const float2* unit = ws.unit + row * pl.units;
+        float m = neg_inf();
+        for (long long u = lane; u < pl.units; u += 32) m = fmaxf(m, unit[u].x);
+        m = warp_max(m);
+        if (m > neg_inf()) {
+          double s = 0.0;
+          for (long long u = lane; u < pl.units; u += 32) {
+            const float2 a = unit[u];
+            if (a.x > neg_inf()) s += (double)a.y * ref_scale(a.x, m, LOG2E_F);
           }
+          s = warp_reduce_add(s);
+          // sum 2^(x c - R) = 2^(m c - R) sum 2^((x - m) c)
+          ref = (double)m;
+          logs = is_far(m, LOG2E_F) ? log(s)
+                                    : LN2 * (log2(s) - ((double)m * (double)LOG2E_F - (double)ceilf(m * LOG2E_F)));
         }
-        t = lo;
-        if (above > most) {
-          // many segments share the K-th maximum t: those above it, then the first ones at it
-          const int per = (nkeys + PICK_THREADS - 1) / PICK_THREADS;
-          const int a = tid * per, b = min(nkeys, a + per);
-          int more = 0, same = 0;
-          for (int i = a; i < b; ++i) {
-            more += sh.row.keys[i] > t;
-            same += sh.row.keys[i] == t;
-          }
-          const int over_t = block_count(more, sh.count, turn);
-          int total;
-          int before = block_excl_scan_add(same, sh.scan, total);
-          for (int i = a; i < b; ++i) {
-            const uint32_t k = sh.row.keys[i];
-            const bool take = k > t || (k == t && before < K - over_t);
-            before += k == t;
-            if (take) sh.sel[atomicAdd(&sh.nsel, 1)] = i;
-          }
-          above = 0;
-        }
+        if (out_lse && lane == 0) out_lse[row] = m > neg_inf() ? (float)(ref + (m < pos_inf() ? logs : 0.0)) : m;
+      } else if (out_lse && lane == 0) {
+        out_lse[row] = neg_inf();
       }
-      __syncthreads();
-      if (above > 0) {
-        for (int i = tid; i < nkeys; i += PICK_THREADS)
-          if (sh.row.keys[i] >= t) sh.sel[atomicAdd(&sh.nsel, 1)] = i;
-      }
-      __syncthreads();
-      // their elements from t up: all at once, or in rounds that keep the list short
-      const int nsel = sh.nsel;
-      const long long todo = (long long)nsel * run;
-      for (int i0 = wid; i0 < todo; i0 += 4 * (PICK_THREADS / 32)) {
-        uint4 v[4];
-        long long first[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const long long i = i0 + j * (PICK_THREADS / 32);
-          if (i < todo) {
-            const long long sg = (long long)sh.sel[i / run] * run + i % run;
-            if (sg < nseg) v[j] = load_seg_vec<T>(p, head, V, sg, lane, first[j]);
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const long long i = i0 + j * (PICK_THREADS / 32);
-          if (i < todo && (long long)sh.sel[i / run] * run + i % run < nseg) append_vec<T>(sh, v[j], first[j], t);
-        }
-      }
-      __syncthreads();
-      if (sh.over) {
-        __syncthreads();
-        if (tid == 0) sh.nlist = 0;
-        __syncthreads();
-        for (long long i0 = 0; i0 < todo; i0 += PICK_THREADS / 32) {
-          const long long i = i0 + wid;
-          if (i < todo) {
-            const long long sg = (long long)sh.sel[i / run] * run + i % run;
-            if (sg < nseg) {
-              long long first;
-              const uint4 v = load_seg_vec<T>(p, head, V, sg, lane, first);
-              append_vec<T>(sh, v, first, t);  // at most 2048 more behind at most 1024
-            }
-          }
-          prune_list(sh, K, LIST_CAP - (PICK_THREADS / 32) * 32 * Elem<T>::VE, turn);
-        }
-      }
-      prune_list(sh, K, RANK_CAP, turn);
-      const int nl = sh.nlist;
-      n = min(nl, K);
-      if (tid < nl) {
-        const unsigned long long c = sh.row.list[tid];
-        int rank = 0;
-        for (int j = 0; j < nl; ++j) rank += sh.row.list[j] > c;
-        if (rank < K) {
-          ws.x[row * K + rank] = key_value((uint32_t)(c >> 32));
-          ws.idx[row * K + rank] = (int32_t)~(uint32_t)c;
-        }
-      }
-      if (inf) {
-        // only the +inf entries have a probability
-        const int here = __syncthreads_count(tid < nl && (uint32_t)(sh.row.list[tid] >> 32) == order_key(pos_inf()));
-        n = min(n, here);
+      if (lane == 0) {
+        sh.ref[w] = ref;
+        sh.logs[w] = logs;
+        sh.cum[w] = cum ? (double)cum[row] : 0.0;
       }
     }
-  } else if (out_lse && tid == 0) {
-    out_lse[row] = neg_inf();
-  }
-  if (tid == 0) {
-    RowTop r;
-    r.ref = ref;
-    r.logs = logs;
-    r.n = n;
-    r.pad = 0;
-    ws.top[row] = r;
-  }
-  // the block that finishes the group last merges
-  __threadfence();
-  __syncthreads();
-  if (tid == 0) sh.last = atomicAdd(&ws.arrived[g], 1u) == (uint32_t)(W - 1);
-  __syncthreads();
-  if (!sh.last) return;
-  __threadfence();
-
-  const long long row0 = g * W;
-  for (int w = tid; w < W; w += PICK_THREADS) {
-    const RowTop* r = ws.top + row0 + w;
-    sh.ref[w] = __ldcg(&r->ref);
-    sh.logs[w] = __ldcg(&r->logs);
-    sh.n[w] = __ldcg(&r->n);
-    sh.cum[w] = cum ? (double)cum[row0 + w] : 0.0;
-  }
-  for (int j = tid; j < W * K; j += PICK_THREADS) sh.merge.x[j] = __ldcg(ws.x + row0 * K + j);
-  if (tid == 0) {
-    sh.flagged = 0ull;
-    sh.end = RANK_CAP;
   }
   __syncthreads();
-  const int total = rank_candidates(sh, W, K);
+  unsigned long long* score = (unsigned long long*)teams;
+  const int total = rank_candidates(sh, xs, score, W, K);
   const int have = min(total, RANK_CAP);
   if (W > 1 && total > 1) {
-    // pairs of neighbours whose order the sums do not settle, up to the first clear gap behind the K-th place
-    const int i = tid;
-    bool near = false, apart = false;
-    int wa = 0, wb = 0;
-    if (i + 1 < have) {
-      wa = (int)sh.sorted_c[i] / K;
-      wb = (int)sh.sorted_c[i + 1] / K;
-      const double a = beam_score(sh, wa, sh.merge.x[sh.sorted_c[i]]);
-      const double b = beam_score(sh, wb, sh.merge.x[sh.sorted_c[i + 1]]);
-      near = !(a - b > 2.0 * LSE_EPS) && a < (double)pos_inf();
-      apart = wa != wb;
-      if (!near && i >= K - 1) atomicMin(&sh.end, i);
+    if (wid == 0) {
+      // neighbours whose order the sums do not settle, up to the first clear gap behind the K-th place
+      uint32_t lo = 0, hi = 0;
+      bool open = true;
+      for (int i0 = 0; open && i0 + 1 < have; i0 += 32) {
+        const int i = i0 + lane;
+        bool near = false;
+        int wa = 0, wb = 0;
+        if (i + 1 < have) {
+          const int ja = sh.sorted[i], jb = sh.sorted[i + 1];
+          const double a = key_value64(score[ja]), b = key_value64(score[jb]);
+          near = !(a - b > 2.0 * LSE_EPS) && a < (double)pos_inf();
+          wa = ja / K;
+          wb = jb / K;
+        }
+        const uint32_t gap = __ballot_sync(FULL, !near && i >= K - 1);
+        open = gap == 0;
+        if (near && wa != wb && (open || lane < __ffs(gap) - 1)) {
+          const unsigned long long both = (1ull << wa) | (1ull << wb);
+          lo |= (uint32_t)both;
+          hi |= (uint32_t)(both >> 32);
+        }
+      }
+      lo = __reduce_or_sync(FULL, lo);
+      hi = __reduce_or_sync(FULL, hi);
+      // a run that leaves the ranked part: every row
+      if (lane == 0) sh.flagged = open && total > RANK_CAP ? ~0ull : ((unsigned long long)hi << 32) | lo;
     }
-    __syncthreads();
-    if (near && apart && i < sh.end) atomicOr(&sh.flagged, (1ull << wa) | (1ull << wb));
-    // a run that leaves the ranked part: every row
-    if (tid == 0 && total > RANK_CAP && sh.end == RANK_CAP) sh.flagged = W == 64 ? ~0ull : (1ull << W) - 1ull;
     __syncthreads();
     const unsigned long long flagged = sh.flagged;
     if (flagged) {
@@ -509,7 +636,7 @@ __global__ void __launch_bounds__(PICK_THREADS) beam_pick_kernel(const T* __rest
         const T* q = logits + (row0 + w) * ld;
         const double m = sh.ref[w];
         double s = 0.0;
-        for (long long v = tid; v < V; v += PICK_THREADS) {
+        for (long long v = tid; v < V; v += blockDim.x) {
           const float x = Elem<T>::load(q, v);
           if (x == x) s += exp((double)x - m);
         }
@@ -517,17 +644,17 @@ __global__ void __launch_bounds__(PICK_THREADS) beam_pick_kernel(const T* __rest
         if (tid == 0) sh.logs[w] = log(s);
         __syncthreads();
       }
-      rank_candidates(sh, W, K);
+      rank_candidates(sh, xs, score, W, K);
     }
   }
-  for (int r = tid; r < K; r += PICK_THREADS) {
+  for (int r = tid; r < K; r += blockDim.x) {
     float sc = neg_inf();
     int tk = -1, pa = -1;
     if (r < total) {
-      const int j = (int)sh.sorted_c[r];
+      const int j = sh.sorted[r];
       pa = j / K;
-      sc = (float)beam_score(sh, pa, sh.merge.x[j]);
-      tk = __ldcg(ws.idx + row0 * K + j);
+      sc = (float)key_value64(score[j]);
+      tk = ids[j];
     }
     out_score[g * K + r] = sc;
     out_token[g * K + r] = tk;

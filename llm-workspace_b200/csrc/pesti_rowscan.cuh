@@ -82,6 +82,9 @@ struct Elem<float> {
     v.z = sub == 2 ? b : v.z;
     v.w = sub == 3 ? b : v.w;
   }
+  static __device__ __forceinline__ float at(const uint4& v, int e) {
+    return __uint_as_float(e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w);
+  }
   static __device__ __forceinline__ void pack(uint4& v, int q, float2 f) {
     (q == 0 ? v.x : v.z) = __float_as_uint(f.x);
     (q == 0 ? v.y : v.w) = __float_as_uint(f.y);
@@ -119,6 +122,9 @@ struct Elem<__nv_bfloat16> : Elem16<__nv_bfloat16> {
   static __device__ __forceinline__ void store(void* p, long long i, float v) {
     ((__nv_bfloat16*)p)[i] = __float2bfloat16_rn(v);
   }
+  static __device__ __forceinline__ float at(const uint4& v, int e) {
+    return __uint_as_float((word(v, e >> 1) >> ((e & 1) * 16)) << 16);
+  }
   static __device__ __forceinline__ float2 pair(const uint4& v, int q) {
     const uint32_t w = word(v, q);
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
@@ -143,6 +149,9 @@ struct Elem<__half> : Elem16<__half> {
   }
   static __device__ __forceinline__ void store(void* p, long long i, float v) {
     ((__half*)p)[i] = __float2half_rn(v);
+  }
+  static __device__ __forceinline__ float at(const uint4& v, int e) {
+    return __half2float(__ushort_as_half((unsigned short)(word(v, e >> 1) >> ((e & 1) * 16))));
   }
   static __device__ __forceinline__ float2 pair(const uint4& v, int q) {
     const uint32_t w = word(v, q);
