@@ -72,6 +72,8 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32) beam_scan_kernel(const T* __r
                                                                     long long V, int W, long long units,
                                                                     long long blocks_per_row, const float* cum,
                                                                     const uint8_t* done, int every_row, BeamWs ws) {
+  // the pick's blocks may start (and wait) once the last block here has started
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const long long row = blockIdx.x / blocks_per_row;
   const long long ub = blockIdx.x - row * blocks_per_row;
   const long long g = row / W;
@@ -136,7 +138,6 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32) beam_scan_kernel(const T* __r
     ws.seg[(row * units + u) * UNIT_VECS + lane] = none ? KEY_NEG_INF : order_key(mine);
   }
   if (lane == 0) ws.unit[row * units + u] = make_float2(m, S);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
 // The block of a group: `teams` teams of TW warps that select, then as many
@@ -215,13 +216,17 @@ __device__ __forceinline__ uint4 load_seg_vec(const T* p, int head, long long V,
   return load_edge<T>(p, first, V);
 }
 
+// (Everything is inlined: a call that takes the team would put it in local
+// memory, and its arrays out of the compiler's sight as shared memory; 64 groups
+// of 8: 22 us with calls.)
+
 // Cuts the list to its largest entries, at least K and at most RANK_CAP (entries are distinct).
 template <int TW>
-__device__ __noinline__ void prune_list(Team<TW>& t, int K) {
+__device__ __forceinline__ void prune_list(Team<TW>& t, int K) {
   constexpr int N = TW * 32, PER = (RANK_CAP + TW * 256 + N - 1) / N;
   team_sync(t);
   const int n = t.word[TM_NLIST];
-  team_sync(t);  // every thread has read it before the next append
+  team_sync(t);  // every thread has read it before the next append (and left the last count's buffer)
   if (n <= RANK_CAP) return;
   unsigned long long lo = 0, hi = ~0ull;
   while (hi - lo > 1) {
@@ -255,7 +260,7 @@ __device__ __noinline__ void prune_list(Team<TW>& t, int K) {
 // The least key of the segments to read, by bisection, and those segments:
 // for maxima that the histogram does not tell apart.
 template <int TW>
-__device__ __noinline__ uint32_t select_by_bisection(Team<TW>& t, int nkeys, int K, uint32_t kmax, int most) {
+__device__ __forceinline__ uint32_t select_by_bisection(Team<TW>& t, int nkeys, int K, uint32_t kmax, int most) {
   constexpr int N = TW * 32;
   uint32_t lo = KEY_NEG_INF + 1, hi = kmax + 1;
   int above = most + 1;
@@ -291,6 +296,7 @@ __device__ __noinline__ uint32_t select_by_bisection(Team<TW>& t, int nkeys, int
       }
     }
   }
+  team_sync(t);
   return lo;
 }
 
@@ -302,8 +308,8 @@ __device__ __forceinline__ long long selected(const Team<TW>& t, const PickPlan&
 
 // The elements of the selected segments in rounds that keep the list short.
 template <typename T, int TW, bool WIDE>
-__device__ __noinline__ void append_in_rounds(Team<TW>& t, const PickPlan& pl, const T* p, long long V, int todo,
-                                              float cut) {
+__device__ __forceinline__ void append_in_rounds(Team<TW>& t, const PickPlan& pl, const T* p, long long V, int todo,
+                                                 float cut) {
   const int lane = t.tid & 31, head = row_head<T>(p);
   team_sync(t);
   if (t.tid == 0) t.word[TM_NLIST] = 0;
@@ -498,29 +504,35 @@ __device__ __forceinline__ int rank_candidates(PickShared& sh, const float* xs, 
     score[j] = j - w * K < sh.n[w] ? order_key64(beam_score(sh, w, xs[j])) : 0ull;
   }
   __syncthreads();
+  if (all <= RANK_CAP) {
+    // a warp per candidate: those ahead are larger, or equal and of a lower beam (or earlier in the list)
+    const int lane = threadIdx.x & 31;
+    for (int j = threadIdx.x >> 5; j < all; j += blockDim.x >> 5) {
+      const unsigned long long s = score[j];
+      int rank = 0;
+      for (int o = lane; o < all; o += 32) rank += score[o] + (o < j) > s;
+      rank = __reduce_add_sync(FULL, rank);
+      if (lane == 0 && s != 0ull) sh.sorted[rank] = j;
+    }
+    __syncthreads();
+    return total;
+  }
   for (int j = threadIdx.x; j < all; j += blockDim.x) {
     const unsigned long long s = score[j];
     if (s == 0ull) continue;
-    int rank = 0;
-    if (all <= 256) {
-      // ahead: larger, or equal and of a lower beam (or earlier in the list)
-#pragma unroll 4
-      for (int o = 0; o < all; ++o) rank += score[o] + (o < j) > s;
-    } else {
-      const int w = j / K;
-      rank = j - w * K;
-      for (int o = 0; o < W && rank < RANK_CAP; ++o) {
-        if (o == w) continue;
-        int lo = 0, hi = sh.n[o];
-        while (lo < hi) {
-          const int mid = (lo + hi) >> 1;
-          if (score[o * K + mid] >= s + (o > w))
-            lo = mid + 1;
-          else
-            hi = mid;
-        }
-        rank += lo;
+    const int w = j / K;
+    int rank = j - w * K;
+    for (int o = 0; o < W && rank < RANK_CAP; ++o) {
+      if (o == w) continue;
+      int lo = 0, hi = sh.n[o];
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (score[o * K + mid] >= s + (o > w))
+          lo = mid + 1;
+        else
+          hi = mid;
       }
+      rank += lo;
     }
     if (rank < RANK_CAP) sh.sorted[rank] = j;
   }
