@@ -1,6 +1,7 @@
 // Host side of the distillation entry points (include/pesti_sampler.h).
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <climits>
 #include <cmath>
@@ -26,7 +27,8 @@ int common(DistillArgs& a, const void* d_logits, pesti_dtype dtype, int64_t N, i
   if (!half_or_float(dtype)) return refuse("logits must be f32, bf16 or f16");
   if (!half_or_float(val_dtype)) return refuse("teacher values must be f32, bf16 or f16");
   if (N < 0) return refuse("N < 0");
-  if (V < 1 || V > 0x7fffffffLL) return refuse("V must be 1 to 2^31-1");
+  if (N > 0x7fffffffLL) return refuse("N must be below 2^31");
+  if (V < 1 || V > (1LL << 30)) return refuse("V must be 1 to 2^30");
   if (ld < V) return refuse("ld is below V");
   if (k < 1 || k > PESTI_DISTILL_MAX_TOP) return refuse("k must be 1 to 256");
   // one value may stand for all rows (stride 0)
@@ -63,14 +65,14 @@ struct Device {
 constexpr int kMaxDevices = 64;
 Device g_devices[kMaxDevices];
 
-constexpr int kKeepUnits = 18;  // units (4 KB) of a CTA that stays at three CTAs per SM
+constexpr int kMaxSlots = 3;
 
 template <typename T, bool GRAD>
 cudaError_t allow() {
   cudaError_t e = cudaFuncSetAttribute(distill_row_kernel<T, GRAD>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return e;
   return cudaFuncSetAttribute(distill_row_kernel<T, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              kKeepUnits * UNIT_SLOTS * 16);
+                              ROW_WARPS * MAX_KEEP * 512);
 }
 
 int set_up(int* sms) {
@@ -96,22 +98,40 @@ int set_up(int* sms) {
   return PESTI_OK;
 }
 
+// A warp's part of a row that is split over c CTAs, and its batches.
+template <typename T>
+void split(DistillArgs& a, long long c) {
+  const long long seg = 512 / (long long)sizeof(T), ve = 16 / (long long)sizeof(T);
+  const long long segs = (a.V + ve - 1 + seg - 1) / seg;
+  a.warp_segs = (int)((segs + c * ROW_WARPS - 1) / (c * ROW_WARPS));
+  a.batches = (a.warp_segs + BATCH - 1) / BATCH;
+}
+
 template <typename T, bool GRAD>
 int launch_row(DistillArgs& a, long long N, int sms, cudaStream_t st) {
-  // One CTA per row while the rows fill the GPU: what a row costs besides its
-  // data (its list, its join) is paid once, and its second reading comes from
-  // L2 (2048 x 152064 bf16: 313 us; clusters of 2, 4, 8 and 16 that keep their
-  // part in shared memory: 358, 483, 678 and 1400 us).  Fewer rows than SMs are
-  // split over clusters while every warp still has a unit.
+  // The cluster: as many CTAs as keep a row in shared memory, more while the
+  // rows alone do not fill the GPU and every warp still has a segment.  Without
+  // a gradient nothing stays, and the split only evens out the last round.
   long long c = 1;
-  while (c < MAX_CLUSTER && N * c < sms && a.units > c * ROW_WARPS) c *= 2;
-  a.keep = GRAD && (a.units + c - 1) / c <= kKeepUnits;
-  a.per_cta = (a.units + c - 1) / c;
-  if (N > 0x7fffffffLL / c) return refuse("N too large");
+  split<T>(a, c);
+  a.keep = 0;
+  if (GRAD) {
+    while (c < MAX_CLUSTER && a.warp_segs > MAX_KEEP) split<T>(a, c *= 2);
+    a.keep = a.warp_segs <= MAX_KEEP;
+    if (!a.keep) split<T>(a, c = 1);
+  } else {
+    const long long all = 2LL * sms;
+    auto share = [&](long long k) { return (double)N / (double)((N * k + all - 1) / all) * (double)k / (double)all; };
+    while (c < 4 && N * c > all && share(c) < 0.93) c *= 2;
+  }
+  while (c < MAX_CLUSTER && N * c < sms && a.warp_segs > 1) split<T>(a, c *= 2);
+  split<T>(a, c);
+  a.slots = a.keep ? a.batches : std::min(kMaxSlots, GRAD ? 2 * a.batches : a.batches);
+  a.ring_segs = std::min(a.warp_segs, a.slots * BATCH);
+  a.N = N;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(N * c));
   cfg.blockDim = dim3(ROW_THREADS);
-  cfg.dynamicSmemBytes = a.keep ? (size_t)a.per_cta * UNIT_SLOTS * 16 : 0;
+  cfg.dynamicSmemBytes = (size_t)ROW_WARPS * a.ring_segs * 512;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -120,6 +140,17 @@ int launch_row(DistillArgs& a, long long N, int sms, cudaStream_t st) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  // as many clusters as run at once (clusters of more than two CTAs may leave SMs of a GPC over)
+  long long clusters = N;
+  if (N * c > sms) {
+    cfg.gridDim = dim3((unsigned)c);
+    int most = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&most, distill_row_kernel<T, GRAD>, &cfg);
+    if (e != cudaSuccess) return pesti_set_cuda_error(e, "cudaOccupancyMaxActiveClusters");
+    if (most < 1) return refuse("no room for a cluster");
+    clusters = std::min<long long>(N, most);
+  }
+  cfg.gridDim = dim3((unsigned)(clusters * c));
   const cudaError_t e = cudaLaunchKernelEx(&cfg, distill_row_kernel<T, GRAD>, (const DistillArgs)a);
   return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, "distill_row_kernel launch");
 }
