@@ -455,25 +455,27 @@ int pesti_beam_reorder(const pesti_beam_rows* states, int64_t n_states, const in
  * and +inf logits make the row's loss and gradient NaN, as NaN in its list does.
  *
  * pesti_distill_topk: d_loss [N] f32.  With d_grad ([N, grad_ld], the logits'
- * type) it writes the gradient of the losses' sum as well, reading the logits
- * from HBM once (for rows that fit the clusters' shared memory: up to about
- * 590000 16-bit or 295000 f32 logits; longer ones twice); d_grad may be
- * d_logits itself (with grad_ld == ld).  With d_stats ([N,
- * PESTI_DISTILL_STATS] f64) it keeps what pesti_distill_topk_backward needs.
+ * type) it writes the gradient of the losses' sum as well; d_grad may be
+ * d_logits itself (with grad_ld == ld).  With d_stats ([N, PESTI_DISTILL_STATS(k)] f64) it keeps what
+ * pesti_distill_topk_backward needs.  d_ws: device scratch of
+ * pesti_distill_topk_workspace(...) bytes, 256-byte aligned, any contents; calls
+ * whose GPU work may overlap need scratch of their own.
  * pesti_distill_topk_backward: the gradient of sum_n d_up[n*up_stride] *
  * loss_n (up_stride 0: one value for all rows) from the forward call's inputs
  * and stats.
  * Both run on the calling thread's current device, stream-ordered (NULL: the
- * legacy default stream), allocate nothing, use no atomics on sums (the same
+ * legacy default stream), allocate nothing, add in a fixed order (the same
  * inputs give the same bits) and may be captured into a graph.
  */
 #define PESTI_DISTILL_MAX_TOP 256
-#define PESTI_DISTILL_STATS 8
+#define PESTI_DISTILL_STATS(k) (8 + (k))
+/* Bytes of scratch, or a negative PESTI_E_* code for refused sizes. */
+int64_t pesti_distill_topk_workspace(pesti_dtype dtype, int64_t N, int64_t V, int64_t k);
 int pesti_distill_topk(const void* d_logits, pesti_dtype dtype, int64_t N, int64_t V, int64_t ld,
                        const int32_t* d_idx, int64_t idx_ld, const void* d_val, pesti_dtype val_dtype,
                        int64_t val_ld, int64_t k, const float* d_teacher_lse, const float* d_weight,
                        double temperature, float* d_loss, double* d_stats, void* d_grad, int64_t grad_ld,
-                       void* stream);
+                       void* d_ws, int64_t ws_bytes, void* stream);
 int pesti_distill_topk_backward(const void* d_logits, pesti_dtype dtype, int64_t N, int64_t V, int64_t ld,
                                 const int32_t* d_idx, int64_t idx_ld, const void* d_val, pesti_dtype val_dtype,
                                 int64_t val_ld, int64_t k, const float* d_teacher_lse, const float* d_weight,

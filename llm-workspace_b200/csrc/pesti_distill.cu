@@ -1,8 +1,6 @@
 // Host side of the distillation entry points (include/pesti_sampler.h).
 #include <cuda_runtime.h>
 
-#include <algorithm>
-#include <atomic>
 #include <climits>
 #include <cmath>
 
@@ -59,109 +57,66 @@ int common(DistillArgs& a, const void* d_logits, pesti_dtype dtype, int64_t N, i
   return PESTI_OK;
 }
 
-struct Device {
-  std::atomic<int> sms{0};  // 0: not set up yet
-};
-constexpr int kMaxDevices = 64;
-Device g_devices[kMaxDevices];
-
-constexpr int kMaxSlots = 3;
-
-template <typename T, bool GRAD>
-cudaError_t allow() {
-  cudaError_t e = cudaFuncSetAttribute(distill_row_kernel<T, GRAD>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e != cudaSuccess) return e;
-  return cudaFuncSetAttribute(distill_row_kernel<T, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              ROW_WARPS * MAX_KEEP * 512);
-}
-
-int set_up(int* sms) {
-  int n = 0, dev = 0;
+int need_device() {
+  int n = 0;
   if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0)
     return pesti_set_error(PESTI_E_NO_DEVICE, "no CUDA device available");
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return pesti_set_cuda_error(e, "cudaGetDevice");
-  if (dev >= kMaxDevices) return refuse("device index out of range");
-  int have = g_devices[dev].sms.load(std::memory_order_acquire);
-  if (have == 0) {
-    e = cudaDeviceGetAttribute(&have, cudaDevAttrMultiProcessorCount, dev);
-    if (e == cudaSuccess) e = allow<float, false>();
-    if (e == cudaSuccess) e = allow<float, true>();
-    if (e == cudaSuccess) e = allow<__nv_bfloat16, false>();
-    if (e == cudaSuccess) e = allow<__nv_bfloat16, true>();
-    if (e == cudaSuccess) e = allow<__half, false>();
-    if (e == cudaSuccess) e = allow<__half, true>();
-    if (e != cudaSuccess) return pesti_set_cuda_error(e, "distillation kernels' set-up");
-    g_devices[dev].sms.store(have, std::memory_order_release);
-  }
-  *sms = have;
   return PESTI_OK;
 }
 
-// A warp's part of a row that is split over c CTAs, and its batches.
-template <typename T>
-void split(DistillArgs& a, long long c) {
-  const long long seg = 512 / (long long)sizeof(T), ve = 16 / (long long)sizeof(T);
-  const long long segs = (a.V + ve - 1 + seg - 1) / seg;
-  a.warp_segs = (int)((segs + c * ROW_WARPS - 1) / (c * ROW_WARPS));
-  a.batches = (a.warp_segs + BATCH - 1) / BATCH;
+long long up256(long long n) { return (n + 255) / 256 * 256; }
+
+// Lays the scratch out behind `base` (which may be null, for the size alone).
+long long layout(char* base, DistillArgs& a, long long N, long long units, int k) {
+  const long long parts = up256(N * units * (long long)sizeof(Partial));
+  const long long lists = up256(N * lists_of(k) * (long long)sizeof(double));
+  a.parts = (Partial*)base;
+  a.lists = (double*)(base + parts);
+  a.stats = (double*)(base + parts + lists);
+  return parts + lists + up256(N * stats_of(k) * (long long)sizeof(double));
 }
 
-template <typename T, bool GRAD>
-int launch_row(DistillArgs& a, long long N, int sms, cudaStream_t st) {
-  // The cluster: as many CTAs as keep a row in shared memory, more while the
-  // rows alone do not fill the GPU and every warp still has a segment.  Without
-  // a gradient nothing stays, and the split only evens out the last round.
-  long long c = 1;
-  split<T>(a, c);
-  a.keep = 0;
-  if (GRAD) {
-    while (c < MAX_CLUSTER && a.warp_segs > MAX_KEEP) split<T>(a, c *= 2);
-    a.keep = a.warp_segs <= MAX_KEEP;
-    if (!a.keep) split<T>(a, c = 1);
-  } else {
-    const long long all = 2LL * sms;
-    auto share = [&](long long k) { return (double)N / (double)((N * k + all - 1) / all) * (double)k / (double)all; };
-    while (c < 4 && N * c > all && share(c) < 0.93) c *= 2;
-  }
-  while (c < MAX_CLUSTER && N * c < sms && a.warp_segs > 1) split<T>(a, c *= 2);
-  split<T>(a, c);
-  a.slots = a.keep ? a.batches : std::min(kMaxSlots, GRAD ? 2 * a.batches : a.batches);
-  a.ring_segs = std::min(a.warp_segs, a.slots * BATCH);
-  a.N = N;
+// A launch that may start before its predecessor has ended (and waits for it).
+template <typename... K, typename... A>
+int launch_behind(const char* what, void (*kernel)(K...), long long blocks, int threads, cudaStream_t st, A... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(ROW_THREADS);
-  cfg.dynamicSmemBytes = (size_t)ROW_WARPS * a.ring_segs * 512;
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(threads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)c;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  // as many clusters as run at once (clusters of more than two CTAs may leave SMs of a GPC over)
-  long long clusters = N;
-  if (N * c > sms) {
-    cfg.gridDim = dim3((unsigned)c);
-    int most = 0;
-    const cudaError_t e = cudaOccupancyMaxActiveClusters(&most, distill_row_kernel<T, GRAD>, &cfg);
-    if (e != cudaSuccess) return pesti_set_cuda_error(e, "cudaOccupancyMaxActiveClusters");
-    if (most < 1) return refuse("no room for a cluster");
-    clusters = std::min<long long>(N, most);
-  }
-  cfg.gridDim = dim3((unsigned)(clusters * c));
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, distill_row_kernel<T, GRAD>, (const DistillArgs)a);
-  return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, "distill_row_kernel launch");
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, K(args)...);
+  return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, what);
+}
+
+int launched(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, what);
+}
+
+template <typename T>
+int run(const DistillArgs& a, cudaStream_t st) {
+  const long long per_row = (a.units + UNIT_WARPS - 1) / UNIT_WARPS, lists = (a.N + UNIT_WARPS - 1) / UNIT_WARPS;
+  if (a.N > (0x7fffffffLL - lists) / per_row) return refuse("N * V too large");
+  distill_scan_kernel<T><<<(unsigned)(lists + a.N * per_row), UNIT_WARPS * 32, 0, st>>>(a, lists, per_row);
+  int rc = launched("distill_scan_kernel launch");
+  if (rc) return rc;
+  rc = launch_behind("distill_join_kernel launch", distill_join_kernel<T>, (a.N + JOIN_WARPS - 1) / JOIN_WARPS,
+                     JOIN_WARPS * 32, st, a);
+  if (rc || !a.grad) return rc;
+  return launch_behind("distill_backward_kernel launch", distill_backward_kernel<T>, a.N * per_row, UNIT_WARPS * 32, st,
+                       a, per_row);
 }
 
 template <typename T>
 int launch_backward(const DistillArgs& a, long long N, cudaStream_t st) {
-  const long long per_row = (a.units + BACK_WARPS - 1) / BACK_WARPS;
+  const long long per_row = (a.units + UNIT_WARPS - 1) / UNIT_WARPS;
   if (N > 0x7fffffffLL / per_row) return refuse("N * V too large");
-  distill_backward_kernel<T><<<(unsigned)(N * per_row), BACK_WARPS * 32, 0, st>>>(a, per_row);
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, "distill_backward_kernel launch");
+  distill_backward_kernel<T><<<(unsigned)(N * per_row), UNIT_WARPS * 32, 0, st>>>(a, per_row);
+  return launched("distill_backward_kernel launch");
 }
 
 int check_grad(const void* d_logits, pesti_dtype dtype, int64_t N, int64_t V, int64_t ld, const void* d_grad,
@@ -180,11 +135,22 @@ int check_grad(const void* d_logits, pesti_dtype dtype, int64_t N, int64_t V, in
 
 extern "C" {
 
+int64_t pesti_distill_topk_workspace(pesti_dtype dtype, int64_t N, int64_t V, int64_t k) {
+  if (!half_or_float(dtype)) return refuse("logits must be f32, bf16 or f16");
+  if (N < 0) return refuse("N < 0");
+  if (V < 1 || V > (1LL << 30)) return refuse("V must be 1 to 2^30");
+  if (k < 1 || k > PESTI_DISTILL_MAX_TOP) return refuse("k must be 1 to 256");
+  const long long units = dtype == PESTI_F32 ? row_units<float>(V) : row_units<__half>(V);
+  if (N > 0x7fffffffLL / units) return refuse("N * V too large");
+  DistillArgs a;
+  return layout(nullptr, a, N, units, (int)k);
+}
+
 int pesti_distill_topk(const void* d_logits, pesti_dtype dtype, int64_t N, int64_t V, int64_t ld,
                        const int32_t* d_idx, int64_t idx_ld, const void* d_val, pesti_dtype val_dtype,
                        int64_t val_ld, int64_t k, const float* d_teacher_lse, const float* d_weight,
                        double temperature, float* d_loss, double* d_stats, void* d_grad, int64_t grad_ld,
-                       void* stream) {
+                       void* d_ws, int64_t ws_bytes, void* stream) {
   DistillArgs a;
   int rc = common(a, d_logits, dtype, N, V, ld, d_idx, idx_ld, d_val, val_dtype, val_ld, k, d_teacher_lse, d_weight,
                   temperature);
@@ -196,19 +162,24 @@ int pesti_distill_topk(const void* d_logits, pesti_dtype dtype, int64_t N, int64
     if (rc) return rc;
     if (d_stats && d_grad == d_logits) return refuse("the backward call needs the logits: no stats with a gradient in place");
   }
+  if (N > 0x7fffffffLL / a.units) return refuse("N * V too large");
+  const long long need = layout((char*)d_ws, a, N, a.units, a.k);
+  if (!d_ws || ws_bytes < need) return refuse("workspace too small");
+  if ((uintptr_t)d_ws % 256) return refuse("workspace is not 256-byte aligned");
   a.loss = d_loss;
-  a.stats = d_stats;
+  if (d_stats)
+    a.stats = d_stats;
+  else if (!d_grad)
+    a.stats = nullptr;
   a.grad = d_grad;
   a.grad_ld = grad_ld;
-  int sms = 0;
-  rc = set_up(&sms);
+  a.N = N;
+  rc = need_device();
   if (rc) return rc;
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == PESTI_F32)
-    return d_grad ? launch_row<float, true>(a, N, sms, st) : launch_row<float, false>(a, N, sms, st);
-  if (dtype == PESTI_BF16)
-    return d_grad ? launch_row<__nv_bfloat16, true>(a, N, sms, st) : launch_row<__nv_bfloat16, false>(a, N, sms, st);
-  return d_grad ? launch_row<__half, true>(a, N, sms, st) : launch_row<__half, false>(a, N, sms, st);
+  if (dtype == PESTI_F32) return run<float>(a, st);
+  if (dtype == PESTI_BF16) return run<__nv_bfloat16>(a, st);
+  return run<__half>(a, st);
 }
 
 int pesti_distill_topk_backward(const void* d_logits, pesti_dtype dtype, int64_t N, int64_t V, int64_t ld,
@@ -230,8 +201,8 @@ int pesti_distill_topk_backward(const void* d_logits, pesti_dtype dtype, int64_t
   a.up_stride = up_stride;
   a.grad = d_grad;
   a.grad_ld = grad_ld;
-  int sms = 0;
-  rc = set_up(&sms);
+  a.N = N;
+  rc = need_device();
   if (rc) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == PESTI_F32) return launch_backward<float>(a, N, st);

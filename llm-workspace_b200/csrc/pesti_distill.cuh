@@ -13,24 +13,24 @@
 // So outside the list the gradient is one factor of the row times 2^(x*C - R),
 // C = log2(e)/T; the k listed places are written apart.
 //
-// distill_row_kernel: clusters of CTAs that walk over rows.  A row's segments
-//   (pesti_rowscan.cuh) are split over the cluster's streaming warps.  Each
-//   lane copies its own 16-byte vectors into slots of its own in shared memory
-//   (cp.async), several batches ahead and over the row's end into the next
-//   row, so the copies never pause for what a row costs besides its data.
-//   With a gradient the slots hold the row's part until its sum is known (the
-//   logits cross HBM once) and each is refilled for the next row once its
-//   gradient is written.  One warp works on the next row's list, one joins
-//   the sums, passes them on in the cluster and finishes the row.  (No register
-//   may spill: next to 200 KB of shared memory there is no L1 to speak of.)
-//   p_t is summed from the unlisted tokens themselves: 1 - sum p would lose it
-//   when the list holds nearly all the mass.
-// distill_backward_kernel: the gradient alone, from what the forward pass kept
-//   of each row (8 numbers).
+// A row's units (pesti_rowscan.cuh: 4 KB, held by one warp in registers) pass
+// through three steps, each a device function of one warp:
+//   scan_unit    the unit's largest logit and its sum of terms.  With q_t, listed
+//                tokens are left out: p_t is summed from the unlisted tokens
+//                themselves, since 1 - sum p would lose it when the list holds
+//                nearly all the mass;
+//   list_row     what a row's list gives by itself: teacher probabilities, listed
+//                tokens' terms, equal tokens (in the scans' grid, beside them);
+//   join_row     joins a row's units and its list: loss, the row's factor A and
+//                the gradients of its listed tokens;
+//   grad_unit    the gradient of a unit.
+// Loss: a kernel of scans and lists, then one of joins.  The gradient: one kernel
+// more, so large calls read the logits from HBM twice.
 //
-// Sums: 64 terms of a lane and unit in f32, units, lanes, warps and CTAs in
-// 64 bits in a fixed order.  Everything of the list (k <= 256 entries) is in
-// 64 bits: the loss is a difference of nearly equal logarithms.
+// Sums: 64 terms of a lane and unit in f32, lanes in 64 bits, a unit's sum
+// rounded to f32 once, units in 64 bits, all in a fixed order.  Everything of the
+// list (k <= 256 entries) is in 64 bits: the loss is a difference of nearly equal
+// logarithms.
 #pragma once
 #include "pesti_common.cuh"
 #include "pesti_rowscan.cuh"
@@ -38,19 +38,19 @@
 namespace pesti_rows {
 
 constexpr int MAX_TOP = 256;
-constexpr int HASH = 512;
-constexpr int ROW_WARPS = 12;                         // streaming warps
-constexpr int JOIN_WARP = ROW_WARPS;
-constexpr int ROW_THREADS = (ROW_WARPS + 2) * 32;     // the list warp behind it
-constexpr int MAX_CLUSTER = 16;
-constexpr int BATCH = 4;                              // segments that a warp takes at a time
-constexpr int MAX_KEEP = 15;                          // segments of a warp that stay: two CTAs fit an SM
-constexpr int WAIT_LIMIT = 1 << 20;
-constexpr int STATS = 8;
+constexpr int STATS = 8;       // numbers of a row, and then its list's gradients
+constexpr int UNIT_WARPS = 8;  // warps of a block, a unit each
 constexpr double ONE_LN2 = 0.69314718055994530942;
 
-// Numbers of a row that the backward pass needs.
-enum { ST_MS = 0, ST_A = 1, ST_LOGQ = 2, ST_TOTAL = 3, ST_MALL = 4, ST_LOGS = 5 };
+__host__ __device__ __forceinline__ long long stats_of(int k) { return STATS + k; }
+
+// What the gradient needs of a row.
+enum { ST_MS = 0, ST_A = 1 };
+
+// A unit's largest logit (never NaN) and its sum of terms relative to it.
+struct __align__(8) Partial {
+  float m, s;
+};
 
 struct DistillArgs {
   const void* logits;
@@ -66,18 +66,20 @@ struct DistillArgs {
   double C;       // log2(e) / T
   float c, c_lo;  // C = c + c_lo, c_lo >= 0
   float* loss;
-  double* stats;
+  double* stats;  // [N][stats_of(k)], null when no gradient follows
   void* grad;
   long long grad_ld;
-  long long units;          // backward: units of a row
-  long long N;              // rows
-  int warp_segs;            // segments of a warp's part of a row
-  int batches;              // in batches of BATCH
-  int slots, ring_segs;     // slots and segments of a warp's ring
-  int keep;                 // a slot for every batch: they stay until the gradient is written
-  const float* up;
+  long long N, units;
+  const float* up;  // none: 1
   long long up_stride;
+  Partial* parts;  // [N][units]
+  double* lists;   // [N][lists_of(k)]
 };
+
+// What list_row leaves of a row: numbers, then e = 2^(x C - R) for the largest listed logit's R and the sum of q over
+// equal tokens of every entry (0 where there is none).
+enum { LI_Q = 0, LI_NORM = 1, LI_LOSS = 2, LI_TERMS = 3, LI_MOST = 4, LI_ENTRIES = 6 };
+__host__ __device__ __forceinline__ long long lists_of(int k) { return LI_ENTRIES + 2 * k; }
 
 __device__ __forceinline__ double teacher_value(const DistillArgs& a, long long n, int j) {
   const long long at = n * a.val_ld + j;
@@ -132,189 +134,6 @@ __device__ __forceinline__ float sum_terms(const uint4 (&v)[NV], float m, const 
   }
   return (s0.x + s0.y) + (s1.x + s1.y);
 }
-
-struct Partial {
-  float m;
-  double s;
-};
-
-// Joins one partial sum per lane; NaN stays NaN (a scale multiplies it).
-__device__ __forceinline__ Partial warp_join(Partial p, float c) {
-  const float m = warp_max(p.m);
-  p.s = warp_reduce_add(p.s * ref_scale(p.m, m, c));
-  p.m = m;
-  return p;
-}
-
-// One row's list.
-struct ListBuf {
-  int32_t idx[MAX_TOP];  // -1: no entry
-  float x[MAX_TOP];      // the places' logits
-  double q[MAX_TOP];
-  union {
-    double qs[MAX_TOP];  // sum of q over equal tokens
-    int32_t hash[HASH];  // while equal tokens are looked for
-  };
-  double e[MAX_TOP];       // 2^(x C - R) for the largest listed logit's R
-  uint8_t first[MAX_TOP];  // first entry of its token
-  double Q, norm, rest;    // sum of q, log of the teacher's normaliser, max(0, 1 - Q) or 0
-  Partial member;          // listed tokens, each once
-};
-
-struct RowShared {
-  ListBuf list[2];
-  Partial warp[2][ROW_WARPS];   // by row parity
-  Partial cta[2][MAX_CLUSTER];  // the cluster's sums
-  unsigned long long arrived[2];
-  float m_s, A;  // of the row whose gradient is written
-};
-
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-
-// Named barriers (0 is __syncthreads).  By row parity: the list is there, the list is free, the warps' sums are there; then: the row is known, its part is written.
-enum { BAR_FULL = 1, BAR_EMPTY = 3, BAR_SUMS = 5, BAR_ROW = 7, BAR_DONE = 8 };
-__device__ __forceinline__ void bar_sync(int id, int threads) {
-  __syncwarp();
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(int id, int threads) {
-  __syncwarp();
-  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-
-// Puts a partial sum into CTA `rank`'s shared memory and signs in there.
-__device__ __forceinline__ void send_partial(Partial* to, unsigned long long* bar, uint32_t rank, const Partial& p) {
-  uint32_t at, b;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(to)), "r"(rank));
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"((uint32_t)__cvta_generic_to_shared(bar)), "r"(rank));
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(p.m) : "memory");
-  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at + 8), "d"(p.s) : "memory");
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(b) : "memory");
-}
-// False if the others have not signed in within the limit.
-__device__ __forceinline__ bool wait_partials(unsigned long long* bar, uint32_t parity) {
-  const uint32_t b = (uint32_t)__cvta_generic_to_shared(bar);
-  for (int i = 0; i < WAIT_LIMIT; ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{.reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-        " selp.u32 %0, 1, 0, p;}"
-        : "=r"(ok)
-        : "r"(b), "r"(parity)
-        : "memory");
-    if (ok) return true;
-  }
-  return false;
-}
-
-__device__ __forceinline__ void copy_vec(uint32_t to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// Waits until at most n of the lane's latest groups are in flight.
-__device__ __forceinline__ void copies_wait(int n) {
-  if (n <= 0)
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-  else if (n == 1)
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
-  else if (n == 2)
-    asm volatile("cp.async.wait_group 2;" ::: "memory");
-  else
-    asm volatile("cp.async.wait_group 3;" ::: "memory");
-}
-
-// The rows of a cluster, rows of weight 0 left out: every warp walks over them by itself.
-struct RowWalk {
-  int first, step, at;  // rows first + i * step < N; window of 32 at i = `at`
-  uint32_t left;
-
-  __device__ __forceinline__ RowWalk(int cluster, int clusters) : first(cluster), step(clusters), at(-32), left(0u) {}
-  // The next row, or -1.  `skipped` is called with each row of weight 0 that is passed.
-  template <typename F>
-  __device__ __forceinline__ int next(const DistillArgs& a, F skipped) {
-    while (left == 0u) {
-      at += 32;
-      const long long i = first + (long long)(at + (int)(threadIdx.x & 31)) * step;
-      const bool in = i < a.N;
-      const bool none = in && a.weight && a.weight[i] == 0.0f;
-      left = __ballot_sync(FULL, in && !none);
-      uint32_t zero = __ballot_sync(FULL, none);
-      if ((left | zero) == 0u) return -1;
-      for (; zero; zero &= zero - 1) skipped(first + (at + __ffs(zero) - 1) * step);
-    }
-    const int i = at + __ffs(left) - 1;
-    left &= left - 1;
-    return first + i * step;
-  }
-};
-
-// A warp's part of a row, for one lane.  Offsets within a row fit 32 bits (V <= 2^30).
-template <typename T>
-struct Part {
-  static constexpr int VE = Elem<T>::VE, SEG = 32 * VE;
-  const T* row;
-  int lo;       // element of the lane's first vector
-  int segs;     // segments of the part
-  bool inside;  // every vector lies in the row
-
-  __device__ __forceinline__ Part(const DistillArgs& a, int n, int part, int lane) {
-    row = (const T*)a.logits + (long long)n * a.ld;
-    const int head = row_head<T>(row), V = (int)a.V;
-    const int first = part * a.warp_segs;
-    segs = max(0, min(a.warp_segs, (head + V + SEG - 1) / SEG - first));
-    const int from = first * SEG - head;
-    inside = from >= 0 && from + segs * SEG <= V;
-    lo = from + lane * VE;
-  }
-  __device__ __forceinline__ int count(int b) const {
-    return max(0, min(BATCH, segs - b * BATCH));
-  }
-  __device__ __forceinline__ bool whole(const DistillArgs& a, int at) const { return at >= 0 && at + VE <= (int)a.V; }
-  // Starts the copies of batch b into the lane's slot (one group, empty if there are none).
-  __device__ __forceinline__ void copy(const DistillArgs& a, int b, uint32_t slot) const {
-    const int n = count(b), at = lo + b * BATCH * SEG;
-    const T* from = row + at;
-    if (inside && n == BATCH) {
-#pragma unroll
-      for (int i = 0; i < BATCH; ++i) copy_vec(slot + i * 512, from + i * SEG);
-    } else {
-      for (int i = 0; i < n; ++i)
-        if (whole(a, at + i * SEG)) copy_vec(slot + i * 512, from + i * SEG);
-    }
-    copies_commit();
-  }
-  // Completes what copy() brought: the row's ragged ends, and -inf behind them.
-  __device__ __forceinline__ void settle(const DistillArgs& a, int b, uint4* slot) const {
-    if (inside) return;
-    const int n = count(b), at = lo + b * BATCH * SEG;
-    for (int i = 0; i < n; ++i)
-      if (!whole(a, at + i * SEG)) slot[i * 32] = load_edge<T>(row, at + i * SEG, a.V);
-  }
-  // Sets listed elements to -inf in the lanes' slots (their gradients are written apart).
-  __device__ __forceinline__ void leave_out(const DistillArgs& a, int b, const int32_t* idx, uint4* slot, int lane) const {
-    const int from = lo - lane * VE + b * BATCH * SEG, n = count(b) * SEG;
-    for (int j0 = 0; j0 < a.k; j0 += 32) {
-      const int j = j0 + lane, id = j < a.k ? idx[j] : -1;
-      uint32_t in = __ballot_sync(FULL, id >= 0 && (uint32_t)(id - from) < (uint32_t)n);
-      while (in) {
-        const int e = __shfl_sync(FULL, id, __ffs(in) - 1) - from;
-        in &= in - 1;
-        if (lane == ((e / VE) & 31)) Elem<T>::store(slot + e / SEG * 32, e % VE, neg_inf());
-      }
-    }
-  }
-};
 
 // Gradient of one vector (slot of the aligned address space) of a row.
 template <typename T>
@@ -380,26 +199,78 @@ __device__ __forceinline__ void store_plain(T* to, const uint4 (&v)[NV], float R
   for (int i = 0; i < NV; ++i) *(uint4*)(to + i * 32 * Elem<T>::VE) = grad_vec<T>(v[i], c2, lo2, r2, A);
 }
 
-// A list warp's work on a row: teacher probabilities, equal tokens, the listed tokens' terms.
+// Sets the listed elements of a unit (`first` is its first element) to -inf in the lanes' registers.  (By a mask of the
+// lane's 64 elements: an index into v would put it into local memory.)
 template <typename T>
-__device__ __forceinline__ void list_part(ListBuf& sh, const DistillArgs& a, long long n, int lane) {
+__device__ __forceinline__ void leave_out(uint4 (&v)[UNIT_VECS], const DistillArgs& a, long long n, long long first,
+                                          int lane) {
+  constexpr int VE = Elem<T>::VE;
+  const int32_t* idx = a.idx + n * a.idx_ld;
+  unsigned long long mine = 0ull;
+  for (int j0 = 0; j0 < a.k; j0 += 32) {
+    const int id = j0 + lane < a.k ? idx[j0 + lane] : -1;
+    const long long o = (long long)id - first;
+    uint32_t in = __ballot_sync(FULL, id >= 0 && id < a.V && o >= 0 && o < UNIT_SLOTS * VE);
+    while (in) {
+      const int e = __shfl_sync(FULL, (int)o, __ffs(in) - 1);
+      in &= in - 1;
+      if (lane == ((e / VE) & 31)) mine |= 1ull << (e / (32 * VE) * VE + e % VE);
+    }
+  }
+  if (!__any_sync(FULL, mine != 0ull)) return;
+#pragma unroll
+  for (int i = 0; i < UNIT_VECS; ++i) {
+    const uint32_t m = (uint32_t)(mine >> (i * VE)) & ((1u << VE) - 1u);
+    if (__any_sync(FULL, m)) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        uint4 w = v[i];
+        Elem<T>::put(w, e, Elem<T>::NEG_INF);
+        if ((m >> e) & 1u) v[i] = w;
+      }
+    }
+  }
+}
+
+// A unit's part of its row's sum.
+template <typename T>
+__device__ __forceinline__ Partial scan_unit(const DistillArgs& a, long long n, long long u, int lane) {
+  const T* row = (const T*)a.logits + n * a.ld;
+  const int head = row_head<T>(row);
+  uint4 v[UNIT_VECS];
+  load_unit<T, true>(v, row, head, a.V, u, lane);
+  if (a.teacher_lse) leave_out<T>(v, a, n, u * UNIT_SLOTS * Elem<T>::VE - head, lane);
+  float m = Elem<T>::vec_max(v[0]);
+#pragma unroll
+  for (int i = 1; i < UNIT_VECS; ++i) m = fmaxf(m, Elem<T>::vec_max(v[i]));
+  Partial p;
+  p.m = fmaxf(warp_max(m), neg_inf());  // NaN alone: -inf, with a sum of NaN
+  p.s = (float)warp_reduce_add((double)sum_terms<T>(v, p.m, a));
+  return p;
+}
+
+// A row's list, by one warp.
+template <typename T>
+__device__ __forceinline__ void list_row(const DistillArgs& a, long long n, int lane) {
   const double inf = (double)pos_inf(), invT = 1.0 / a.T;
-  const T* row = (const T*)a.logits + (long long)n * a.ld;
+  const bool tail = a.teacher_lse != nullptr;
+  const T* row = (const T*)a.logits + n * a.ld;
+  const int32_t* idx = a.idx + n * a.idx_ld;
+  double* out = a.lists + n * lists_of(a.k);
+  auto listed = [&](int j) {  // the token of entry j, -1 if there is none
+    const int32_t id = j < a.k ? idx[j] : -1;
+    return id >= 0 && id < a.V ? id : -1;
+  };
+  // the largest teacher value and listed logit
   double mt = -inf;
   float mx = neg_inf();
-  for (int i = lane; i < HASH; i += 32) sh.hash[i] = -1;
 #pragma unroll 2
   for (int j = lane; j < a.k; j += 32) {
-    const int32_t id = a.idx[n * a.idx_ld + j];
+    const int32_t id = listed(j);
     const double t = teacher_value(a, n, j) * invT;
-    const bool in = id >= 0 && id < a.V;
-    const float x = in ? Elem<T>::load(row, id) : neg_inf();
-    sh.idx[j] = in ? id : -1;
-    sh.x[j] = x;
-    sh.q[j] = in ? t : -inf;
-    if (in) {
+    if (id >= 0) {
       mt = !(t <= mt) ? t : mt;  // NaN is taken over
-      mx = fmaxf(mx, x);
+      mx = fmaxf(mx, Elem<T>::load(row, id));
     }
   }
   mx = warp_max(mx);
@@ -408,392 +279,228 @@ __device__ __forceinline__ void list_part(ListBuf& sh, const DistillArgs& a, lon
     const double y = __shfl_xor_sync(FULL, mt, o);
     mt = mt != mt ? mt : !(y <= mt) ? y : mt;
   }
-  // q = exp(t - norm): of the whole vocabulary's sum, or first of the largest
-  double norm = a.teacher_lse ? (double)a.teacher_lse[n] : mt != -inf ? mt : 0.0;
-  double Q = 0.0, ms = 0.0;
-  bool dup = false;
-  __syncwarp();
-  for (int j = lane; j < a.k; j += 32) {
-    const int32_t id = sh.idx[j];
-    double q = 0.0, e = 0.0;
-    bool mine = false;
-    if (id >= 0) {
-      q = exp(sh.q[j] - norm);
-      e = exact_term(sh.x[j], mx, a);
-      uint32_t h = ((uint32_t)id * 2654435761u) >> 23;
-      for (;;) {
-        const int32_t had = atomicCAS(&sh.hash[h], -1, id);
-        mine = had == -1;
-        if (had == -1 || had == id) break;
-        h = (h + 1) & (HASH - 1);
-      }
-      dup = dup || !mine;
-      ms += mine ? e : 0.0;
+  // q = exp(t - norm): of the whole vocabulary's sum, or first of the largest; listed tokens' terms, each token once
+  double norm = tail ? (double)a.teacher_lse[n] : mt != -inf ? mt : 0.0;
+  double Q = 0.0, terms = 0.0, l = 0.0;
+  bool twice = false;  // a token is listed more than once
+  for (int j0 = 0; j0 < a.k; j0 += 32) {
+    const int j = j0 + lane;
+    const int32_t id = listed(j);
+    bool first = id >= 0;
+    for (int o0 = 0; o0 <= j0; o0 += 32) {
+      const int32_t other = listed(o0 + lane);
+#pragma unroll 8
+      for (int o = 0; o < 32; ++o)
+        if (__shfl_sync(FULL, other, o) == id && o0 + o < j) first = false;
     }
-    sh.q[j] = q;
-    sh.e[j] = e;
-    sh.first[j] = mine;
-    Q += q;
+    twice = twice || (id >= 0 && !first);
+    if (j < a.k) {
+      double q = 0.0, e = 0.0;
+      if (id >= 0) {
+        const float x = Elem<T>::load(row, id);
+        const double logq = teacher_value(a, n, j) * invT - norm;
+        q = exp(logq);
+        e = exact_term(x, mx, a);
+        if (q != 0.0) l += q * (logq - (x == neg_inf() ? -inf : ((double)x - (double)mx) * invT));
+        Q += q;
+        terms += first ? e : 0.0;
+      }
+      out[LI_ENTRIES + j] = e;
+      out[LI_ENTRIES + a.k + j] = q;
+    }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     Q += __shfl_xor_sync(FULL, Q, o);
-    ms += __shfl_xor_sync(FULL, ms, o);
+    terms += __shfl_xor_sync(FULL, terms, o);
+    l += __shfl_xor_sync(FULL, l, o);
   }
   double per = 1.0;
-  if (!a.teacher_lse && Q != 0.0) {
+  if (!tail && Q != 0.0) {
+    // q, and sum q log q, for the sum Q of the exponentials: log q = t - norm - log Q
     per = 1.0 / Q;
+    l = l * per - log(Q);
     norm += log(Q);
-    Q *= per;
+    Q = Q == Q ? 1.0 : Q;
   }
-  dup = __any_sync(FULL, dup);
-  if (!a.teacher_lse)
-    for (int j = lane; j < a.k; j += 32) sh.q[j] *= per;
-  __syncwarp();
-  for (int j = lane; j < a.k; j += 32) {
-    double s = sh.q[j];
-    if (dup && sh.idx[j] >= 0) {
-      // a token listed more than once: its first entry stands for all
-      s = 0.0;
-      bool first = true;
-      for (int o = 0; o < a.k; ++o)
-        if (sh.idx[o] == sh.idx[j]) {
-          s += sh.q[o];
-          first = first && o >= j;
+  twice = __any_sync(FULL, twice);
+  if (twice || !tail) {
+    __syncwarp();
+    for (int j0 = 0; j0 < a.k; j0 += 32) {
+      const int j = j0 + lane;
+      const int32_t id = listed(j);
+      if (j < a.k) {
+        double s = out[LI_ENTRIES + a.k + j];
+        if (twice && id >= 0) {
+          // every entry of a token gets the token's sum
+          s = 0.0;
+          for (int o = 0; o < a.k; ++o)
+            if (idx[o] == id) s += exp(teacher_value(a, n, o) * invT - (tail ? norm : mt));
         }
-      sh.first[j] = first;
+        out[LI_ENTRIES + a.k + j] = s * per;
+      }
     }
-    sh.qs[j] = s;
   }
   if (lane == 0) {
-    const double rest = 1.0 - Q;
-    sh.Q = Q;
-    sh.norm = norm;
-    sh.rest = a.teacher_lse ? (rest < 0.0 ? 0.0 : rest) : 0.0;
-    sh.member = Partial{mx, ms};
+    out[LI_Q] = Q;
+    out[LI_NORM] = norm;
+    out[LI_LOSS] = l;
+    out[LI_TERMS] = terms;
+    out[LI_MOST] = (double)mx;
   }
 }
 
-template <typename T, bool GRAD>
-__global__ void __launch_bounds__(ROW_THREADS, 2) distill_row_kernel(const __grid_constant__ DistillArgs a) {
-  extern __shared__ uint4 ring[];
-  __shared__ RowShared sh;
-  constexpr int VE = Elem<T>::VE, SEG = 32 * VE;
-  constexpr int WORKERS = (ROW_WARPS + 1) * 32;  // the streaming warps and one other
-  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-  const uint32_t csize = cluster_size(), crank = cluster_rank();
+// A row's loss, and its numbers for the gradient, by one warp.
+template <typename T>
+__device__ __forceinline__ void join_row(const DistillArgs& a, long long n, int lane) {
+  const double inf = (double)pos_inf(), w = a.weight ? (double)a.weight[n] : 1.0;
   const bool tail = a.teacher_lse != nullptr;
-  if (csize > 1) {
-    if (tid < 2) {
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(&sh.arrived[tid])),
-                   "r"(csize)
-                   : "memory");
-      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    __syncthreads();
-    cluster_arrive();
-    cluster_wait();
+  const double* list = a.lists + n * lists_of(a.k);
+  const Partial* parts = a.parts + n * a.units;
+  const double Q = list[LI_Q], l0 = list[LI_LOSS], terms = list[LI_TERMS];
+  const float mx = (float)list[LI_MOST];
+  // what was scanned
+  float m_s = neg_inf();
+  double s = 0.0;
+#pragma unroll 4
+  for (long long u = lane; u < a.units; u += 32) m_s = fmaxf(m_s, parts[u].m);
+  m_s = warp_max(m_s);
+#pragma unroll 4
+  for (long long u = lane; u < a.units; u += 32) {
+    const Partial p = parts[u];
+    s += (double)p.s * ref_scale(p.m, m_s, a.c);
   }
-  RowWalk rows(blockIdx.x / csize, gridDim.x / csize);
-  int p = 0;
-
-  if (wid < ROW_WARPS) {
-    const int part = (int)crank * ROW_WARPS + wid;
-    uint4* slots = ring + wid * a.ring_segs * 32 + lane;
-    const uint32_t slots_at = (uint32_t)__cvta_generic_to_shared(slots);
-    constexpr int slot_vecs = BATCH * 32;
-    const int batches = a.batches;
-    auto zeros = [&](int n) {
-      if (GRAD) {
-        const Part<T> t(a, n, part, lane);
-        T* grow = (T*)a.grad + (long long)n * a.grad_ld;
-        for (int i = 0; i < t.segs; ++i)
-          store_vec<T>(grow, t.lo + i * SEG, a.V, row_head<T>(grow) == row_head<T>(t.row), make_uint4(0, 0, 0, 0));
-      }
-    };
-    int row = rows.next(a, zeros);
-    // batches of a row that pass through the ring: once, or once more for the gradient
-    const int passes = GRAD && !a.keep ? 2 * batches : batches;
-    Part<T> here(a, max(row, 0), part, lane);
-    if (row >= 0)
-      for (int i = 0; i < a.slots; ++i) here.copy(a, i >= batches ? i - batches : i, slots_at + i * slot_vecs * 16);
-    int slot = 0;
-    while (row >= 0) {
-      const int after = rows.next(a, zeros);
-      const Part<T> then(a, max(after, 0), part, lane);
-      // the batch that takes a freed slot: `slots` ahead in this row, or of the next one
-      auto refill = [&](int pass, int to) {
-        int q = pass + a.slots;
-        const uint32_t at = slots_at + to * slot_vecs * 16;
-        if (q < passes) {
-          here.copy(a, q >= batches ? q - batches : q, at);
-        } else if (after >= 0) {
-          q -= passes;
-          then.copy(a, q >= batches ? q - batches : q, at);
-        } else {
-          copies_commit();
-        }
-      };
-      bar_sync(BAR_FULL + p, WORKERS);
-      Partial acc{neg_inf(), 0.0};
-      auto add_terms = [&](const auto& v, float most) {
-        const float m = fmaxf(acc.m, warp_max(most));
-        acc.s = acc.s * ref_scale(acc.m, m, a.c) + (double)sum_terms<T>(v, m, a);
-        acc.m = m;
-      };
-      for (int b = 0; b < batches; ++b) {
-        uint4* at = slots + slot * slot_vecs;
-        const int n = here.count(b);
-        copies_wait(a.keep ? batches - 1 - b : a.slots - 1);
-        here.settle(a, b, at);
-        if (tail) here.leave_out(a, b, sh.list[p].idx, at, lane);
-        if (n == BATCH) {
-          uint4 v[BATCH];
-#pragma unroll
-          for (int i = 0; i < BATCH; ++i) v[i] = at[i * 32];
-          float m = Elem<T>::vec_max(v[0]);
-#pragma unroll
-          for (int i = 1; i < BATCH; ++i) m = fmaxf(m, Elem<T>::vec_max(v[i]));
-          add_terms(v, m);
-        } else {
-#pragma unroll 1
-          for (int i = 0; i < n; ++i) {
-            const uint4 v[1] = {at[i * 32]};
-            add_terms(v, Elem<T>::vec_max(v[0]));
-          }
-        }
-        if (!a.keep) refill(b, slot);
-        if (++slot == a.slots) slot = 0;
-      }
-      acc.s = warp_reduce_add(acc.s);  // every lane has the same reference
-      if (lane == 0) sh.warp[p][wid] = acc;
-      bar_arrive(BAR_SUMS + p, WORKERS);
-      if (GRAD) {
-        bar_sync(BAR_ROW, WORKERS);
-        const float m = sh.m_s, f = sh.A, near = near_factor<T>(f, m, a), R = reference(m, a.c);
-        T* grow = (T*)a.grad + (long long)row * a.grad_ld;
-        const bool plain =
-            here.inside && row_head<T>(grow) == row_head<T>(here.row) && !(m > neg_inf() && is_far(m, a.c));
-        for (int b = 0; b < batches; ++b) {
-          uint4* at = slots + slot * slot_vecs;
-          const int n = here.count(b), lo = here.lo + b * BATCH * SEG;
-          if (!a.keep) {
-            copies_wait(a.slots - 1);
-            here.settle(a, b, at);
-          }
-          if (plain && n == BATCH) {
-            uint4 v[BATCH];
-#pragma unroll
-            for (int i = 0; i < BATCH; ++i) v[i] = at[i * 32];
-            store_plain<T>(grow + lo, v, R, near, a);
-          } else {
-#pragma unroll 1
-            for (int i = 0; i < n; ++i) store_any<T>(grow, at[i * 32], lo + i * SEG, a.V, m, f, a);
-          }
-          refill(a.keep ? b : batches + b, slot);
-          if (++slot == a.slots) slot = 0;
-        }
-        bar_arrive(BAR_DONE, WORKERS);
-      }
-      row = after;
-      here = then;
-      p ^= 1;
+  s = warp_reduce_add(s);
+  // all tokens: what was scanned, and the listed ones where they were left out
+  const float m_all = tail ? fmaxf(m_s, mx) : m_s;
+  const double scale = ref_scale(m_s, m_all, a.c), e_scale = ref_scale(mx, m_all, a.c);
+  double S = s * scale + (tail ? terms * e_scale : 0.0);
+  if (m_all == pos_inf()) S = inf - inf;  // +inf logits have no softmax: NaN
+  const double rest = 1.0 - Q;
+  double q_t = tail ? (rest < 0.0 ? 0.0 : rest) : 0.0;
+  if (s == 0.0 || scale == 0.0) q_t = q_t == q_t ? 0.0 : q_t;  // no unlisted token with a probability (in 64 bits)
+  const double total = Q + q_t;
+  if (a.stats) {
+    double* st = a.stats + n * stats_of(a.k);
+    // outside the list: grad = A * 2^(x C - Rs)
+    double A = S;
+    if (S == S) A = s > 0.0 ? a.T * (total * scale / S - (q_t != 0.0 ? q_t / s : 0.0)) : 0.0;
+    if (lane == 0) {
+      st[ST_MS] = (double)m_s;
+      st[ST_A] = A;
     }
-  } else if (wid == JOIN_WARP) {
-    uint32_t phase = 0;  // bit p: parity of arrived[p]
-    auto none_lost = [&](int n) {
-      if (crank == 0 && lane == 0) a.loss[n] = 0.0f;
-    };
-    for (int n = rows.next(a, none_lost); n >= 0; n = rows.next(a, none_lost)) {
-      const double w = a.weight ? (double)a.weight[n] : 1.0;
-      ListBuf& list = sh.list[p];
-      bar_sync(BAR_SUMS + p, WORKERS);
-      Partial s{neg_inf(), 0.0};
-      if (lane < ROW_WARPS) s = sh.warp[p][lane];
-      s = warp_join(s, a.c);
-      bool lost = false;
-      if (csize > 1) {
-        if (lane < csize) send_partial(&sh.cta[p][crank], &sh.arrived[p], lane, s);
-        lost = !wait_partials(&sh.arrived[p], (phase >> p) & 1u);
-        phase ^= 1u << p;
-        s = Partial{neg_inf(), 0.0};
-        if (lane < csize) s = sh.cta[p][lane];
-        s = warp_join(s, a.c);
-      }
-      // all tokens: what was streamed, and the listed ones where they were left out
-      const double pos = (double)pos_inf();
-      const float m_all = tail ? fmaxf(s.m, list.member.m) : s.m;
-      const double scale = ref_scale(s.m, m_all, a.c);
-      double e_scale = ref_scale(list.member.m, m_all, a.c);
-      double S = s.s * scale + (tail ? list.member.s * e_scale : 0.0);
-      if (m_all == pos_inf() || lost) S = pos - pos;  // +inf logits have no softmax: NaN
-      double q_t = list.rest;
-      if (s.s == 0.0 || scale == 0.0) q_t = q_t == q_t ? 0.0 : q_t;  // no unlisted token with a probability (in 64 bits)
-      const double total = list.Q + q_t;
-      // outside the list: grad = A * 2^(x C - Rs)
-      double A = S;
-      if (S == S) A = s.s > 0.0 ? a.T * (total * scale / S - (q_t != 0.0 ? q_t / s.s : 0.0)) : 0.0;
-      if (GRAD) {
-        if (lane == 0) {
-          sh.A = (float)(A * w);
-          sh.m_s = s.m;
-        }
-        bar_arrive(BAR_ROW, WORKERS);
-      }
-      // log sum exp((x - m_all)/T); a row of -inf alone has none
-      if (crank == 0) {
-        const bool none = !(m_all > neg_inf()) && S == S;
-        const bool far = !none && is_far(m_all, a.c);
-        const double logS =
-            none ? 0.0 : far ? log(S) : ONE_LN2 * (log2(S) - ((double)m_all * a.C - (double)reference(m_all, a.c)));
-        const double invT = 1.0 / a.T;
-        double l = 0.0;
-        for (int j = lane; j < a.k; j += 32) {
-          const double q = list.q[j];
-          if (list.idx[j] >= 0 && q != 0.0) {
-            const double x = (double)list.x[j];
-            const double logp = none || x == -pos ? (S == S ? -pos : S) : (x - (double)m_all) * invT - logS;
-            l += q * ((teacher_value(a, n, j) * invT - list.norm) - logp);
-          }
-        }
-        l = warp_reduce_add(l);
-        // p_t = s.s * scale / S
-        if (q_t != 0.0) l += q_t * (log(q_t) - (log(s.s) + log(scale) - log(S)));
-        if (S != S) l = S;
-        if (lane == 0) {
-          a.loss[n] = (float)(w * a.T * a.T * l);
-          if (a.stats) {
-            double* st = a.stats + (long long)n * STATS;
-            st[ST_MS] = (double)s.m;
-            st[ST_A] = A;
-            st[ST_LOGQ] = list.norm;
-            st[ST_TOTAL] = total;
-            st[ST_MALL] = (double)m_all;
-            st[ST_LOGS] = logS;
-          }
-        }
-      }
-      if (GRAD) {
-        // the listed places of this CTA's part, behind the rest of it
-        e_scale = S == 0.0 ? 0.0 : e_scale / S;  // from e to p
-        const long long head = row_head<T>((const T*)a.logits + (long long)n * a.ld);
-        const long long from = (long long)crank * ROW_WARPS * a.warp_segs * SEG - head;
-        const long long to = from + (long long)ROW_WARPS * a.warp_segs * SEG;
-        T* grow = (T*)a.grad + (long long)n * a.grad_ld;
-        bar_sync(BAR_DONE, WORKERS);
-        for (int j = lane; j < a.k; j += 32) {
-          const long long id = list.idx[j];
-          if (id >= 0 && list.first[j] && id >= from && id < to)
-            Elem<T>::store(grow, id, (float)(w * a.T * (total * (list.e[j] * e_scale) - list.qs[j])));
-        }
-      }
-      bar_arrive(BAR_EMPTY + p, 64);
-      p ^= 1;
-    }
-  } else {
-    auto nothing = [](int) {};
-    int done = 0;
-    for (int n = rows.next(a, nothing); n >= 0; n = rows.next(a, nothing), p ^= 1) {
-      if (done++ > 1) bar_sync(BAR_EMPTY + p, 64);
-      list_part<T>(sh.list[p], a, n, lane);
-      bar_arrive(BAR_FULL + p, WORKERS);
-    }
-    // the last rows' sign-offs have no other taker
-    if (done > 1) bar_sync(BAR_EMPTY + p, 64);
-    if (done > 0) bar_sync(BAR_EMPTY + (p ^ 1), 64);
+    // p of a listed token is e * to_p; a row of -inf alone has none
+    const double to_p = S == 0.0 ? 0.0 : e_scale / S;
+    for (int j = lane; j < a.k; j += 32)
+      st[STATS + j] = a.T * (total * (list[LI_ENTRIES + j] * to_p) - list[LI_ENTRIES + a.k + j]);
   }
-  if (csize > 1) {
-    cluster_arrive();
-    cluster_wait();
+  if (lane == 0) {
+    // sum q (log q - (x - mx)/T) + Q (log sum exp of (x - mx)/T) + q_t (log q_t - log p_t), p_t = s * scale / S
+    double l = l0;
+    if (m_all > neg_inf() && Q != 0.0) {
+      const double lse =
+          is_far(m_all, a.c) ? log(S) : ONE_LN2 * (log2(S) - ((double)m_all * a.C - (double)reference(m_all, a.c)));
+      l += Q * (((double)m_all - (double)mx) / a.T + lse);
+    }
+    if (q_t != 0.0) l += q_t * (log(q_t) - log(s * scale / S));
+    if (S != S) l = S;
+    a.loss[n] = (float)(w * a.T * a.T * l);
   }
 }
 
-// Zeros for units [ua, ub) of a gradient row.
+// The gradient of a unit, in place too: everything is read before anything is written.
 template <typename T>
-__device__ __forceinline__ void zero_units(T* grow, int head, long long V, bool vec, long long ua, long long ub) {
-  const uint4 z = make_uint4(0, 0, 0, 0);
-  for (long long s = ua * UNIT_SLOTS + threadIdx.x; s < ub * UNIT_SLOTS; s += blockDim.x)
-    store_vec<T>(grow, s * Elem<T>::VE - head, V, vec, z);
-}
-
-constexpr int BACK_WARPS = 8;
-
-// One warp per unit of a row, BACK_WARPS units per block.
-template <typename T>
-__global__ void __launch_bounds__(BACK_WARPS * 32) distill_backward_kernel(const __grid_constant__ DistillArgs a,
-                                                                           long long blocks_per_row) {
-  __shared__ int32_t in_idx[MAX_TOP], in_j[MAX_TOP];
-  __shared__ float in_x[MAX_TOP];
-  __shared__ double in_q[MAX_TOP];
-  __shared__ int count;
+__device__ __forceinline__ void grad_unit(const DistillArgs& a, long long n, long long u, double scale, int lane) {
   constexpr int VE = Elem<T>::VE;
-  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-  const long long n = blockIdx.x / blocks_per_row;
-  const long long ua = (blockIdx.x - n * blocks_per_row) * BACK_WARPS, ub = min(a.units, ua + BACK_WARPS);
-  const T* row = (const T*)a.logits + (long long)n * a.ld;
-  T* grow = (T*)a.grad + (long long)n * a.grad_ld;
+  const T* row = (const T*)a.logits + n * a.ld;
+  T* grow = (T*)a.grad + n * a.grad_ld;
   const int head = row_head<T>(row);
+  uint4 v[UNIT_VECS];
+  load_unit<T, false>(v, row, head, a.V, u, lane);
+  const double* st = a.stats + n * stats_of(a.k);
+  const float m = (float)__ldcg(st + ST_MS), A = (float)(__ldcg(st + ST_A) * scale);
+  const long long first = u * UNIT_SLOTS * VE - head, lo = first + lane * VE;
+  constexpr int span = UNIT_SLOTS * VE;
+  __syncwarp();
+  const bool plain = row_head<T>(grow) == head && first >= 0 && first + span <= a.V && !(m > neg_inf() && is_far(m, a.c));
+  if (plain) {
+    store_plain<T>(grow + lo, v, reference(m, a.c), near_factor<T>(A, m, a), a);
+  } else {
+#pragma unroll
+    for (int i = 0; i < UNIT_VECS; ++i)
+      if (lo + i * 32 * VE < a.V) store_any<T>(grow, v[i], lo + i * 32 * VE, a.V, m, A, a);
+  }
+  // the unit's listed tokens, over what was just written
+  __syncwarp();
+  const int32_t* idx = a.idx + n * a.idx_ld;
+  for (int j = lane; j < a.k; j += 32) {
+    const long long id = idx[j];
+    if (id >= first && id < first + span && id >= 0 && id < a.V)
+      Elem<T>::store(grow, id, (float)(__ldcg(st + STATS + j) * scale));
+  }
+}
+
+// Zeros for a unit of a row that takes no part.
+template <typename T>
+__device__ __forceinline__ void zero_unit(const DistillArgs& a, long long n, long long u, int lane) {
+  T* grow = (T*)a.grad + n * a.grad_ld;
+  const int head = row_head<T>((const T*)a.logits + n * a.ld);
   const bool vec = row_head<T>(grow) == head;
-  const float w = a.weight ? a.weight[n] : 1.0f;
-  if (w == 0.0f) {
-    zero_units<T>(grow, head, a.V, vec, ua, ub);
+  for (int i = 0; i < UNIT_VECS; ++i)
+    store_vec<T>(grow, ((u * UNIT_VECS + i) * 32 + lane) * Elem<T>::VE - head, a.V, vec, make_uint4(0, 0, 0, 0));
+}
+
+__device__ __forceinline__ bool takes_part(const DistillArgs& a, long long n) {
+  return a.weight == nullptr || a.weight[n] != 0.0f;
+}
+
+// The first blocks work on the lists, a warp each; the others on the units.
+template <typename T>
+__global__ void __launch_bounds__(UNIT_WARPS * 32) distill_scan_kernel(const __grid_constant__ DistillArgs a,
+                                                                       long long list_blocks,
+                                                                       long long blocks_per_row) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  if (blockIdx.x < list_blocks) {
+    const long long n = (long long)blockIdx.x * UNIT_WARPS + wid;
+    if (n < a.N && takes_part(a, n)) list_row<T>(a, n, lane);
     return;
   }
-  if (tid == 0) count = 0;
-  __syncthreads();
-  const double* st = a.stats + (long long)n * STATS;
-  const double scale = (double)w * (double)a.up[n * a.up_stride];
-  const long long u = ua + wid;
-  uint4 v[UNIT_VECS];
-  if (u < ub) load_unit<T, false>(v, row, head, a.V, u, lane);
-  // the list's places in this block's part, read before anything is written
-  const long long from = ua * UNIT_SLOTS * VE - head, to = ub * UNIT_SLOTS * VE - head;
-  if (tid < a.k) {
-    const long long id = a.idx[n * a.idx_ld + tid];
-    if (id >= 0 && id < a.V && id >= from && id < to) {
-      const int at = atomicAdd(&count, 1);
-      in_idx[at] = (int32_t)id;
-      in_j[at] = tid;
-      in_x[at] = Elem<T>::load(row, id);
-      in_q[at] = exp(teacher_value(a, n, tid) / a.T - st[ST_LOGQ]);
-    }
+  const long long block = blockIdx.x - list_blocks, n = block / blocks_per_row;
+  const long long u = (block - n * blocks_per_row) * UNIT_WARPS + wid;
+  if (u >= a.units || !takes_part(a, n)) return;
+  const Partial p = scan_unit<T>(a, n, u, lane);
+  if (lane == 0) a.parts[n * a.units + u] = p;
+}
+
+constexpr int JOIN_WARPS = 2;  // warps of a block, a row each
+
+template <typename T>
+__global__ void __launch_bounds__(JOIN_WARPS * 32) distill_join_kernel(const __grid_constant__ DistillArgs a) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const long long n = (long long)blockIdx.x * JOIN_WARPS + (threadIdx.x >> 5);
+  if (n >= a.N) return;
+  if (takes_part(a, n))
+    join_row<T>(a, n, threadIdx.x & 31);
+  else if ((threadIdx.x & 31) == 0)
+    a.loss[n] = 0.0f;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(UNIT_WARPS * 32) distill_backward_kernel(const __grid_constant__ DistillArgs a,
+                                                                           long long blocks_per_row) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const long long n = blockIdx.x / blocks_per_row;
+  const long long u = (blockIdx.x - n * blocks_per_row) * UNIT_WARPS + (threadIdx.x >> 5);
+  if (u >= a.units) return;
+  const int lane = threadIdx.x & 31;
+  if (!takes_part(a, n)) {
+    zero_unit<T>(a, n, u, lane);
+    return;
   }
-  const float m = (float)st[ST_MS], A = (float)(st[ST_A] * scale);
-  __syncthreads();
-  if (u < ub) {
-    const long long lo = (u * UNIT_SLOTS + lane) * VE - head, part = lo - lane * VE;
-    if (vec && part >= 0 && part + UNIT_SLOTS * VE <= a.V && !(m > neg_inf() && is_far(m, a.c))) {
-      store_plain<T>(grow + lo, v, reference(m, a.c), near_factor<T>(A, m, a), a);
-    } else {
-#pragma unroll
-      for (int i = 0; i < UNIT_VECS; ++i)
-        if (lo + i * 32 * VE < a.V) store_any<T>(grow, v[i], lo + i * 32 * VE, a.V, m, A, a);
-    }
-  }
-  __syncthreads();
-  const int cnt = count;
-  for (int i = tid; i < cnt; i += BACK_WARPS * 32) {
-    // entries of the same token add up in the list's order; the first one writes
-    bool first = true;
-    double qs = 0.0;
-    for (int last = -1;;) {
-      int next = MAX_TOP, at = -1;
-      for (int o = 0; o < cnt; ++o)
-        if (in_idx[o] == in_idx[i] && in_j[o] > last && in_j[o] < next) {
-          next = in_j[o];
-          at = o;
-        }
-      if (at < 0) break;
-      if (next < in_j[i]) first = false;
-      qs += in_q[at];
-      last = next;
-    }
-    if (first) {
-      const double x = (double)in_x[i], logs = st[ST_LOGS];
-      const double p = x == -(double)pos_inf() && logs == logs ? 0.0 : exp((x - st[ST_MALL]) / a.T - logs);
-      Elem<T>::store(grow, in_idx[i], (float)(scale * a.T * (st[ST_TOTAL] * p - qs)));
-    }
-  }
+  const double w = a.weight ? (double)a.weight[n] : 1.0;
+  grad_unit<T>(a, n, u, w * (a.up ? (double)a.up[n * a.up_stride] : 1.0), lane);
 }
 
 }  // namespace pesti_rows

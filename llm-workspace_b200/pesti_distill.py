@@ -8,13 +8,27 @@ the logits' device and the current stream; there is no CPU path.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from pesti_beam import _DTYPES, _launch, _need, _on_device, _ptr, _row_stride, _rows_dtype
 from pesti_sampler import _check, load_library
 
 MAX_TOP = 256  # PESTI_DISTILL_MAX_TOP
-_STATS = 8     # PESTI_DISTILL_STATS
+
+
+def _stats(k: int) -> int:
+    """PESTI_DISTILL_STATS(k)."""
+    return 8 + k
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace(dtype: int, N: int, V: int, k: int) -> int:
+    need = load_library().pesti_distill_topk_workspace(dtype, N, V, k)
+    _check(min(0, need))
+    return need
+
 
 
 def _lists(logits, idx, val, temperature, teacher_lse, weight):
@@ -54,8 +68,11 @@ class _DistillTopk(torch.autograd.Function):
 
         def call(st):
             loss = torch.empty(N, dtype=torch.float32, device=dev)
-            stats = torch.empty((N, _STATS), dtype=torch.float64, device=dev) if keep else None
-            rc = load_library().pesti_distill_topk(*args, loss.data_ptr(), _ptr(stats), None, 0, st)
+            stats = torch.empty((N, _stats(args[10])), dtype=torch.float64, device=dev) if keep else None
+            need = _workspace(args[1], N, args[3], args[10])
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            rc = load_library().pesti_distill_topk(*args, loss.data_ptr(), _ptr(stats), None, 0, ws.data_ptr(), need,
+                                                   st)
             if rc:
                 _check(rc)
             return loss, stats
@@ -118,7 +135,10 @@ def distill_topk_grad(logits, idx, val, temperature: float = 1.0, teacher_lse=No
     def call(st):
         loss = torch.empty(N, dtype=torch.float32, device=dev)
         to = torch.empty((N, V), dtype=logits.dtype, device=dev) if grad is None else grad
-        rc = load_library().pesti_distill_topk(*args, loss.data_ptr(), None, to.data_ptr(), _row_stride(to), st)
+        need = _workspace(args[1], N, V, args[10])
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        rc = load_library().pesti_distill_topk(*args, loss.data_ptr(), None, to.data_ptr(), _row_stride(to),
+                                               ws.data_ptr(), need, st)
         if rc:
             _check(rc)
         return loss, to

@@ -143,8 +143,10 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.pesti_beam_reorder.argtypes = [vp, i64, vp, i64, i64, vp]
     lib.pesti_beam_reorder.restype = c_int
     lib.pesti_distill_topk.argtypes = [vp, c_int, i64, i64, i64, vp, i64, vp, c_int, i64, i64, vp, vp, ctypes.c_double,
-                                       vp, vp, vp, i64, vp]
+                                       vp, vp, vp, i64, vp, i64, vp]
     lib.pesti_distill_topk.restype = c_int
+    lib.pesti_distill_topk_workspace.argtypes = [c_int, i64, i64, i64]
+    lib.pesti_distill_topk_workspace.restype = i64
     lib.pesti_distill_topk_backward.argtypes = [vp, c_int, i64, i64, i64, vp, i64, vp, c_int, i64, i64, vp, vp,
                                                 ctypes.c_double, vp, vp, i64, vp, i64, vp]
     lib.pesti_distill_topk_backward.restype = c_int

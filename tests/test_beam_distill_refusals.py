@@ -125,7 +125,7 @@ COMMON = [
 @pytest.mark.parametrize("change,msg", COMMON)
 def test_distill_common_refusals(lib, change, msg):
     a = list({**DISTILL, **change}.values())
-    assert lib.pesti_distill_topk(*a, P, None, None, 0, None) == BAD
+    assert lib.pesti_distill_topk(*a, P, None, None, 0, P, 1 << 30, None) == BAD
     assert msg in lib.pesti_last_error().decode()
     assert lib.pesti_distill_topk_backward(*a, P, P, 1, 2 * P, 100, None) == BAD
     assert msg in lib.pesti_last_error().decode()
@@ -133,7 +133,11 @@ def test_distill_common_refusals(lib, change, msg):
 
 def test_distill_output_refusals(lib):
     a = list(DISTILL.values())
-    f, b = lib.pesti_distill_topk, lib.pesti_distill_topk_backward
+    b = lib.pesti_distill_topk_backward
+
+    def f(*args):
+        return lib.pesti_distill_topk(*args[:-1], P, 1 << 30, args[-1])
+
     assert f(*a, None, None, None, 0, None) == BAD                     # no loss
     assert f(*a, P, None, 2 * P, 99, None) == BAD                      # grad_ld
     assert f(*a, P, None, 2 * P + 2, 100, None) == BAD                 # alignment
@@ -145,6 +149,13 @@ def test_distill_output_refusals(lib):
     assert b(*a, P, P, 1, None, 100, None) == BAD
     assert b(*a, P, P, -1, 2 * P, 100, None) == BAD
     assert f(*list({**DISTILL, "N": 0}.values()), None, None, None, 0, None) == ps.PESTI_OK
+    for ws, size in ((None, 1 << 30), (P, 64), (P + 8, 1 << 30)):
+        assert lib.pesti_distill_topk(*a, P, None, None, 0, ws, size, None) == BAD
+        assert "workspace" in lib.pesti_last_error().decode()
+    need = lib.pesti_distill_topk_workspace
+    assert 0 < need(ps.PESTI_BF16, 4, 1000, 8) < need(ps.PESTI_F32, 40, 100000, 256)
+    for bad in ((ps.PESTI_FP8_E4M3, 4, 100, 8), (0, -1, 100, 8), (0, 4, 0, 8), (0, 4, 100, 257), (0, 1 << 40, 100, 8)):
+        assert need(*bad) == BAD
 
 
 def test_python_checks():

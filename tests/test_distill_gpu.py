@@ -91,12 +91,62 @@ def test_teacher_types(val):
 
 
 @pytest.mark.parametrize("N", [1, 3])
-def test_rows_that_do_not_stay_on_chip(N):
-    """Longer than the largest cluster's shared memory: read twice."""
+def test_long_rows(N):
     x, idx, val, lse = _make(N, 620_003, 16, "bf16", tail=True)
     _compare(x, idx, val, 1.0, lse, None, "bf16")
     x, idx, val, lse = _make(N, 300_001, 16, "f32")
     _compare(x, idx, val, 1.0, lse, None, "f32")
+
+
+# large batches: many rows, many units, rows of weight 0 between others
+@pytest.mark.parametrize("N,V,dtype,tail,pad", [
+    (210, 128256, "bf16", True, 0), (400, 32001, "f32", False, 1), (13, 2_000_003, "f16", True, 0),
+    (9000, 3001, "bf16", True, 1),
+])
+def test_large_calls(N, V, dtype, tail, pad):
+    x, idx, val, lse = _make(N, V, 20, dtype, tail=tail, pad=pad)
+    weight = torch.linspace(0.5, 1.5, N).cuda()
+    weight[::7] = 0.0
+    weight[1::50] = 0.0
+    x[0] = float("nan")  # of weight 0: not read
+    _compare(x, idx, val, 1.0, lse, weight, dtype)
+    first = pd.distill_topk_grad(x, idx, val, teacher_lse=lse, weight=weight)
+    for _ in range(3):
+        again = pd.distill_topk_grad(x, idx, val, teacher_lse=lse, weight=weight)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+    # in place, and nothing between the rows is written
+    behind = x.as_strided((N - 1, 1), (V + pad, 1), V).clone() if pad else None
+    loss, grad = pd.distill_topk_grad(x, idx, val, teacher_lse=lse, weight=weight, grad=x)
+    assert torch.equal(loss, first[0]) and torch.equal(x, first[1])
+    if pad:
+        assert torch.equal(x.as_strided((N - 1, 1), (V + pad, 1), V), behind)
+
+
+def test_large_calls_at_once_and_captured():
+    """Two large calls on two streams at the same time, and in graphs replayed together."""
+    a = [_make(220, 128256, 16, "bf16", tail=True, seed=s) for s in (1, 2)]
+    want = [pd.distill_topk_grad(x, i, v, teacher_lse=l) for x, i, v, l in a]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(4):
+        got = [pd.distill_topk_grad(x, i, v, teacher_lse=l, stream=s.cuda_stream)
+               for (x, i, v, l), s in zip(a, streams)]
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            assert torch.equal(g[0], w[0]) and torch.equal(g[1], w[1])
+    graphs, outs = [], []
+    for x, i, v, l in a:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(pd.distill_topk_grad(x, i, v, teacher_lse=l))
+        graphs.append(g)
+    for _ in range(4):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert torch.equal(o[0], w[0]) and torch.equal(o[1], w[1])
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
