@@ -59,21 +59,16 @@ long long layout(char* base, long long rows, long long units, BeamWs* ws) {
 }
 
 constexpr int kMaxDevices = 64;
-constexpr int kPickSmem = 200 * 1024;
+constexpr int kPickSmem = 200 * 1024;   // most of a block's dynamic shared memory
+constexpr int kTeamKeys = 4096;          // most of a team's keys
 std::atomic<bool> g_pick_ready[kMaxDevices];
-
-template <typename T, int TW>
-cudaError_t allow_pick_teams() {
-  const cudaError_t e =
-      cudaFuncSetAttribute(beam_pick_kernel<T, TW, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPickSmem);
-  if (e != cudaSuccess) return e;
-  return cudaFuncSetAttribute(beam_pick_kernel<T, TW, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPickSmem);
-}
 
 template <typename T>
 cudaError_t allow_pick() {
-  const cudaError_t e = allow_pick_teams<T, 3>();
-  return e == cudaSuccess ? allow_pick_teams<T, 7>() : e;
+  const cudaError_t e =
+      cudaFuncSetAttribute(beam_pick_kernel<T, TEAM, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPickSmem);
+  if (e != cudaSuccess) return e;
+  return cudaFuncSetAttribute(beam_pick_kernel<T, TEAM, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPickSmem);
 }
 
 int set_up_pick() {
@@ -90,33 +85,44 @@ int set_up_pick() {
   return PESTI_OK;
 }
 
-template <typename T, int TW>
-int launch_pick(const void* logits, long long G, long long V, long long ld, PickPlan pl, const float* cum,
-                const uint8_t* done, const BeamWs& ws, float* score, int32_t* token, int32_t* parent, float* lse,
-                cudaStream_t st) {
-  // A list takes what one round of a team's segments appends to a pruned one;
-  // the keys get what is left of the shared memory (longer rows: the maxima of
-  // runs of segments).
-  const long long nseg = pl.units * UNIT_VECS;
-  const long long lists = ((long long)pl.W * pl.K * 8 + 15) / 16 * 16;
-  pl.cap = RANK_CAP + TW * 256;
-  const long long most = (kPickSmem - lists) / pl.teams / 4 - (pl.cap * 2 + TEAM_WORDS + 4);
-  pl.run = (int)((nseg + most - 1) / most);
+template <typename T>
+int launch_pick(const void* logits, long long G, long long W, long long V, long long ld, int K, long long units,
+                const float* cum, const uint8_t* done, const BeamWs& ws, float* score, int32_t* token, int32_t* parent,
+                float* lse, cudaStream_t st) {
+  PickPlan pl{};
+  pl.W = (int)W;
+  pl.K = K;
+  pl.units = units;
+  // two beams at a time in each block, at most eight blocks
+  long long c = std::min<long long>(MAX_PICK_CLUSTER, (W + MAX_TEAMS - 1) / MAX_TEAMS);
+  pl.rows = (int)((W + c - 1) / c);
+  c = (W + pl.rows - 1) / pl.rows;
+  pl.teams = std::min(pl.rows, MAX_TEAMS);
+  // A list takes what one round of a team's segments appends to a pruned one.
+  // Longer rows have keys of runs of segments.
+  const long long nseg = units * UNIT_VECS;
+  const long long lists = (W * K * 8 + 15) / 16 * 16;
+  pl.cap = RANK_CAP + TEAM * 256;
+  pl.run = (int)((nseg + kTeamKeys - 1) / kTeamKeys);
   pl.nkeys = (int)((nseg + pl.run - 1) / pl.run);
   const long long body = std::max(pl.teams * team_bytes(pl.nkeys, pl.cap), lists);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)G);
-  cfg.blockDim = dim3((unsigned)(pl.teams * (TW + 1) * 32));
+  cfg.gridDim = dim3((unsigned)(G * c));
+  cfg.blockDim = dim3((unsigned)(pl.teams * (TEAM + 1) * 32));
   cfg.dynamicSmemBytes = (size_t)(lists + body);
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)c;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, pl.run == 1 ? beam_pick_kernel<T, TW, false> : beam_pick_kernel<T, TW, true>,
-                                           (const T*)logits, ld, V, (const PickPlan)pl, cum, done, ws, score, token,
-                                           parent, lse);
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(
+      &cfg, pl.run == 1 ? beam_pick_kernel<T, TEAM, false> : beam_pick_kernel<T, TEAM, true>, (const T*)logits, ld, V,
+      (const PickPlan)pl, cum, done, ws, score, token, parent, lse);
   return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, "beam_pick_kernel launch");
 }
 
@@ -131,14 +137,7 @@ int run_select(const void* logits, long long G, long long W, long long V, long l
       (const T*)logits, ld, V, (int)W, units, per_row, cum, done, lse != nullptr, ws);
   rc = launched("beam_scan_kernel launch");
   if (rc) return rc;
-  PickPlan pl{};
-  pl.W = (int)W;
-  pl.K = K;
-  pl.units = units;
-  pl.teams = (int)std::min<long long>(W, MAX_TEAMS);
-  // a block of at most 32 warps: as many for each beam as fit
-  if (W <= 4) return launch_pick<T, 7>(logits, G, V, ld, pl, cum, done, ws, score, token, parent, lse, st);
-  return launch_pick<T, 3>(logits, G, V, ld, pl, cum, done, ws, score, token, parent, lse, st);
+  return launch_pick<T>(logits, G, W, V, ld, K, units, cum, done, ws, score, token, parent, lse, st);
 }
 
 int check_state(const pesti_beam_state* s, int64_t G, int64_t W) {

@@ -13,12 +13,13 @@
 //                     (pesti_rowscan.cuh) in registers and writes the unit's
 //                     maximum m and S = sum 2^(x*c - R), c = f32(log2 e),
 //                     R = ceil(m*c), and its 8 segment maxima.
-//  beam_pick_kernel   one block per group.  For each beam, the K segments with
-//                     the largest maxima hold the K largest logits: a team of
-//                     warps finds them (a histogram of the maxima, its K-th
-//                     place), reads them again and sorts what is above the
-//                     K-th maximum, while another warp joins the row's sum.
-//                     Then the block merges the W lists.
+//  beam_pick_kernel   a cluster of blocks per group, two beams at a time in
+//                     each.  For each beam, the K segments with the largest
+//                     maxima hold the K largest logits: a team of warps finds
+//                     them (a histogram of the maxima, its K-th place), reads
+//                     them again and sorts what is above the K-th maximum,
+//                     while another warp joins the row's sum.  The lists go to
+//                     the first block's shared memory, which merges them.
 //
 // Accuracy of a row's log sum as the scan gives it, relative to the sum:
 //   2^x by the hardware 2^-22.5; the rounding of x*c - R (one fused
@@ -39,8 +40,10 @@ namespace pesti_rows {
 
 constexpr int MAX_W = 64;          // beams of a group
 constexpr int MAX_K = 128;         // candidates of a group
-constexpr int SCAN_WARPS = 8;
-constexpr int MAX_TEAMS = 8;
+constexpr int SCAN_WARPS = 4;
+constexpr int TEAM = 7;           // warps of a team
+constexpr int MAX_TEAMS = 2;      // of a block
+constexpr int MAX_PICK_CLUSTER = 8;
 constexpr int MAX_SEL = MAX_K + MAX_K / 2 + 8;
 constexpr int BINS = 256;
 constexpr int RANK_CAP = 256;      // candidates that are ranked by counting
@@ -140,11 +143,12 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32) beam_scan_kernel(const T* __r
   if (lane == 0) ws.unit[row * units + u] = make_float2(m, S);
 }
 
-// The block of a group: `teams` teams of TW warps that select, then as many
-// warps that join sums.  A team's arrays lie in dynamic shared memory behind
-// the x and idx of the group's lists; the merge's scores take their place.
+// A block of a group's cluster: `teams` teams of TW warps that select for beams
+// first, first + 1, ... of the block's `rows`, then as many warps that join
+// sums.  A team's arrays lie in dynamic shared memory behind the x and idx of
+// the group's lists; the merge's scores take their place.
 struct PickPlan {
-  int W, K, teams, nkeys, run, cap;  // run: segments of a key; cap: entries of a team's list
+  int W, K, rows, teams, nkeys, run, cap;  // run: segments of a key; cap: entries of a team's list
   long long units;
 };
 
@@ -540,22 +544,36 @@ __device__ __forceinline__ int rank_candidates(PickShared& sh, const float* xs, 
   return total;
 }
 
+// The address of a shared variable of the cluster's first block.
+template <typename P>
+__device__ __forceinline__ P* in_first(P* p) {
+  unsigned long long r;
+  asm volatile("mapa.u64 %0, %1, %2;" : "=l"(r) : "l"((unsigned long long)p), "r"(0u));
+  return (P*)r;
+}
+
 template <typename T, int TW, bool WIDE>
-__global__ void __launch_bounds__(1024) beam_pick_kernel(const T* __restrict__ logits, long long ld, long long V,
-                                                         const __grid_constant__ PickPlan pl, const float* cum,
-                                                         const uint8_t* done, BeamWs ws, float* out_score,
-                                                         int32_t* out_token, int32_t* out_parent, float* out_lse) {
+__global__ void __launch_bounds__(MAX_TEAMS*(TEAM + 1) * 32) beam_pick_kernel(
+    const T* __restrict__ logits, long long ld, long long V, const __grid_constant__ PickPlan pl, const float* cum,
+    const uint8_t* done, BeamWs ws, float* out_score, int32_t* out_token, int32_t* out_parent, float* out_lse) {
   extern __shared__ __align__(16) char dyn[];
   __shared__ PickShared sh;
   const int tid = threadIdx.x, lane = tid & 31, W = pl.W, K = pl.K;
-  const long long g = blockIdx.x, row0 = g * W;
+  uint32_t csize, crank;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(csize));
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(crank));
+  // every block of the cluster has begun before anything is written to the first one
+  if (csize > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+  const long long g = blockIdx.x / csize, row0 = g * W;
   float* xs = (float*)dyn;
   int32_t* ids = (int32_t*)(xs + W * K);
   char* teams = dyn + ((long long)W * K * 8 + 15) / 16 * 16;
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (csize > 1) asm volatile("barrier.cluster.wait;" ::: "memory");
 
   const bool group_done = done && done[g];
-  const int wid = tid >> 5;
+  const int wid = tid >> 5, from = (int)crank * pl.rows, to = min(W, from + pl.rows);
+  PickShared* first = csize > 1 ? in_first(&sh) : &sh;
   if (wid < pl.teams * TW) {
     Team<TW> t;
     t.id = wid / TW;
@@ -566,16 +584,18 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(const T* __restrict__ l
     t.hist = (int*)(t.keys + pl.nkeys);
     t.sel = t.hist + BINS;
     t.word = t.sel + MAX_SEL;
-    for (int w = t.id; w < W; w += pl.teams) {
+    float* const first_xs = csize > 1 ? in_first(xs) : xs;
+    int32_t* const first_ids = csize > 1 ? in_first(ids) : ids;
+    for (int w = from + t.id; w < to; w += pl.teams) {
       int n = 0;
       if (!group_done && beam_running(cum, row0 + w))
-        n = pick_row<T, TW, WIDE>(t, pl, logits + (row0 + w) * ld, V, ws.seg + (row0 + w) * pl.units * UNIT_VECS, xs + w * K,
-                            ids + w * K);
-      if (t.tid == 0) sh.n[w] = n;
+        n = pick_row<T, TW, WIDE>(t, pl, logits + (row0 + w) * ld, V, ws.seg + (row0 + w) * pl.units * UNIT_VECS,
+                                  first_xs + w * K, first_ids + w * K);
+      if (t.tid == 0) first->n[w] = n;
       team_sync(t);
     }
   } else {
-    for (int w = wid - pl.teams * TW; w < W; w += pl.teams) {
+    for (int w = from + wid - pl.teams * TW; w < to; w += pl.teams) {
       // the row's sum, joined from its units in a fixed order
       const long long row = row0 + w;
       double ref = 0.0, logs = 0.0;
@@ -601,11 +621,17 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(const T* __restrict__ l
         out_lse[row] = neg_inf();
       }
       if (lane == 0) {
-        sh.ref[w] = ref;
-        sh.logs[w] = logs;
-        sh.cum[w] = cum ? (double)cum[row] : 0.0;
+        first->ref[w] = ref;
+        first->logs[w] = logs;
+        first->cum[w] = cum ? (double)cum[row] : 0.0;
       }
     }
+  }
+  if (csize > 1) {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    if (crank != 0) return;
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   }
   __syncthreads();
   unsigned long long* score = (unsigned long long*)teams;
