@@ -59,56 +59,68 @@ long long layout(char* base, long long rows, long long units, BeamWs* ws) {
 }
 
 constexpr int kMaxDevices = 64;
-constexpr int kPickSmem = 200 * 1024;   // most of a block's dynamic shared memory
-constexpr int kTeamKeys = 4096;          // most of a team's keys
-std::atomic<bool> g_pick_ready[kMaxDevices];
+constexpr int kPickSmem = 200 * 1024;  // most of a block's dynamic shared memory
+std::atomic<int> g_pick_sms[kMaxDevices];  // 0: not set up yet
+
+template <typename T, int TW>
+cudaError_t allow_teams() {
+  const cudaError_t e =
+      cudaFuncSetAttribute(beam_pick_kernel<T, TW, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPickSmem);
+  if (e != cudaSuccess) return e;
+  return cudaFuncSetAttribute(beam_pick_kernel<T, TW, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPickSmem);
+}
 
 template <typename T>
 cudaError_t allow_pick() {
-  const cudaError_t e =
-      cudaFuncSetAttribute(beam_pick_kernel<T, TEAM, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPickSmem);
-  if (e != cudaSuccess) return e;
-  return cudaFuncSetAttribute(beam_pick_kernel<T, TEAM, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPickSmem);
+  cudaError_t e = allow_teams<T, 7>();
+  if (e == cudaSuccess) e = allow_teams<T, 3>();
+  return e == cudaSuccess ? allow_teams<T, 1>() : e;
 }
 
-int set_up_pick() {
-  int dev = 0;
+int set_up_pick(int* sms) {
+  int dev = 0, have = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return pesti_set_cuda_error(e, "cudaGetDevice");
   if (dev >= kMaxDevices) return refuse("device index out of range");
-  if (g_pick_ready[dev].load(std::memory_order_acquire)) return PESTI_OK;
-  e = allow_pick<float>();
+  *sms = g_pick_sms[dev].load(std::memory_order_acquire);
+  if (*sms) return PESTI_OK;
+  e = cudaDeviceGetAttribute(&have, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess) e = allow_pick<float>();
   if (e == cudaSuccess) e = allow_pick<__nv_bfloat16>();
   if (e == cudaSuccess) e = allow_pick<__half>();
   if (e != cudaSuccess) return pesti_set_cuda_error(e, "beam_pick_kernel set-up");
-  g_pick_ready[dev].store(true, std::memory_order_release);
+  g_pick_sms[dev].store(have, std::memory_order_release);
+  *sms = have;
   return PESTI_OK;
 }
 
-template <typename T>
-int launch_pick(const void* logits, long long G, long long W, long long V, long long ld, int K, long long units,
-                const float* cum, const uint8_t* done, const BeamWs& ws, float* score, int32_t* token, int32_t* parent,
-                float* lse, cudaStream_t st) {
-  PickPlan pl{};
-  pl.W = (int)W;
-  pl.K = K;
-  pl.units = units;
-  // two beams at a time in each block, at most eight blocks
-  long long c = std::min<long long>(MAX_PICK_CLUSTER, (W + MAX_TEAMS - 1) / MAX_TEAMS);
-  pl.rows = (int)((W + c - 1) / c);
-  c = (W + pl.rows - 1) / pl.rows;
-  pl.teams = std::min(pl.rows, MAX_TEAMS);
+// Beams at a time in a block of teams of TW warps, and the blocks of a group.
+void pick_shape(PickPlan& pl, int tw, long long* c) {
+  const int most = PICK_WARPS / (tw + 1);
+  *c = std::min<long long>(MAX_PICK_CLUSTER, (pl.W + most - 1) / most);
+  pl.rows = (int)((pl.W + *c - 1) / *c);
+  *c = (pl.W + pl.rows - 1) / pl.rows;
+  pl.teams = std::min(pl.rows, most);
+}
+
+template <typename T, int TW>
+int launch_pick(const void* logits, long long G, long long V, long long ld, PickPlan pl, const float* cum,
+                const uint8_t* done, const BeamWs& ws, float* score, int32_t* token, int32_t* parent, float* lse,
+                cudaStream_t st) {
+  long long c;
+  pick_shape(pl, TW, &c);
   // A list takes what one round of a team's segments appends to a pruned one.
   // Longer rows have keys of runs of segments.
-  const long long nseg = units * UNIT_VECS;
-  const long long lists = (W * K * 8 + 15) / 16 * 16;
-  pl.cap = RANK_CAP + TEAM * 256;
-  pl.run = (int)((nseg + kTeamKeys - 1) / kTeamKeys);
+  const long long nseg = pl.units * UNIT_VECS;
+  const long long lists = ((long long)pl.W * pl.K * 8 + 15) / 16 * 16;
+  pl.cap = RANK_CAP + TW * 256;
+  const long long most = (kPickSmem - lists) / pl.teams / 4 - (2 * pl.cap + TEAM_WORDS + 4);
+  pl.run = (int)((nseg + most - 1) / most);
   pl.nkeys = (int)((nseg + pl.run - 1) / pl.run);
   const long long body = std::max(pl.teams * team_bytes(pl.nkeys, pl.cap), lists);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(G * c));
-  cfg.blockDim = dim3((unsigned)(pl.teams * (TEAM + 1) * 32));
+  cfg.blockDim = dim3((unsigned)(pl.teams * (TW + 1) * 32));
   cfg.dynamicSmemBytes = (size_t)(lists + body);
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -121,7 +133,7 @@ int launch_pick(const void* logits, long long G, long long W, long long V, long 
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   const cudaError_t e = cudaLaunchKernelEx(
-      &cfg, pl.run == 1 ? beam_pick_kernel<T, TEAM, false> : beam_pick_kernel<T, TEAM, true>, (const T*)logits, ld, V,
+      &cfg, pl.run == 1 ? beam_pick_kernel<T, TW, false> : beam_pick_kernel<T, TW, true>, (const T*)logits, ld, V,
       (const PickPlan)pl, cum, done, ws, score, token, parent, lse);
   return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, "beam_pick_kernel launch");
 }
@@ -130,14 +142,31 @@ template <typename T>
 int run_select(const void* logits, long long G, long long W, long long V, long long ld, const float* cum,
                const uint8_t* done, int K, float* score, int32_t* token, int32_t* parent, float* lse,
                const BeamWs& ws, long long units, cudaStream_t st) {
-  int rc = set_up_pick();
+  int sms = 0;
+  int rc = set_up_pick(&sms);
   if (rc) return rc;
   const long long per_row = (units + SCAN_WARPS - 1) / SCAN_WARPS;
   beam_scan_kernel<T><<<(unsigned)(G * W * per_row), SCAN_WARPS * 32, 0, st>>>(
       (const T*)logits, ld, V, (int)W, units, per_row, cum, done, lse != nullptr, ws);
   rc = launched("beam_scan_kernel launch");
   if (rc) return rc;
-  return launch_pick<T>(logits, G, W, V, ld, K, units, cum, done, ws, score, token, parent, lse, st);
+  PickPlan pl{};
+  pl.W = (int)W;
+  pl.K = K;
+  pl.units = units;
+  // The widest teams whose blocks all run at once (16 warps of 114 registers
+  // fill an SM): 32 groups of 8 beams take 11.5 us with teams of 7, 16 us with
+  // teams of 3; 64 groups 21.5 us with teams of 7.  Long lists are too much for
+  // teams of one warp (1024 rows of 32000, K 64: 73 us, 47 us with teams of 3).
+  auto at_once = [&](int tw) {
+    long long c;
+    PickPlan q = pl;
+    pick_shape(q, tw, &c);
+    return G * c * q.teams * (tw + 1) <= (long long)sms * PICK_WARPS;
+  };
+  if (at_once(7)) return launch_pick<T, 7>(logits, G, V, ld, pl, cum, done, ws, score, token, parent, lse, st);
+  if (at_once(3) || K > 32) return launch_pick<T, 3>(logits, G, V, ld, pl, cum, done, ws, score, token, parent, lse, st);
+  return launch_pick<T, 1>(logits, G, V, ld, pl, cum, done, ws, score, token, parent, lse, st);
 }
 
 int check_state(const pesti_beam_state* s, int64_t G, int64_t W) {

@@ -13,8 +13,8 @@
 //                     (pesti_rowscan.cuh) in registers and writes the unit's
 //                     maximum m and S = sum 2^(x*c - R), c = f32(log2 e),
 //                     R = ceil(m*c), and its 8 segment maxima.
-//  beam_pick_kernel   a cluster of blocks per group, two beams at a time in
-//                     each.  For each beam, the K segments with the largest
+//  beam_pick_kernel   a cluster of blocks per group, two, four or eight beams
+//                     at a time in each.  For each beam, the K segments with the largest
 //                     maxima hold the K largest logits: a team of warps finds
 //                     them (a histogram of the maxima, its K-th place), reads
 //                     them again and sorts what is above the K-th maximum,
@@ -26,12 +26,12 @@
 //   operation): half an ulp of t = x*c - R, ln 2 * 2^-24 * E[|t|], and
 //   E[|t|] <= 12 since the entropy of 2048 terms is at most 11 bits and R
 //   less than 1 above the largest; c's own
-//   rounding 1.34e-8 * E[m - x] (<= ln V <= 22); 23 additions in f32, 2^-24
-//   each.  Together below 2.4e-6.  Units are joined in 64 bits.  Two
+//   rounding 1.34e-8 * E[m - x] (<= ln V <= 22); 16 additions in f32, 2^-24
+//   each.  Together below 1.95e-6.  Units are joined in 64 bits.  Two
 //   candidates of different beams whose scores differ by less than twice
 //   LSE_EPS are therefore not ordered by these sums: the merge adds up their
-//   rows again in 64 bits, in index order, and ranks once more.  That is one
-//   call in some thousands for random logits.
+//   rows again in 64 bits, in index order, and ranks once more (random logits,
+//   8 beams, K 16: about one group in 1500, which then takes some 20 us more).
 #pragma once
 #include "pesti_common.cuh"
 #include "pesti_rowscan.cuh"
@@ -41,13 +41,12 @@ namespace pesti_rows {
 constexpr int MAX_W = 64;          // beams of a group
 constexpr int MAX_K = 128;         // candidates of a group
 constexpr int SCAN_WARPS = 4;
-constexpr int TEAM = 7;           // warps of a team
-constexpr int MAX_TEAMS = 2;      // of a block
+constexpr int PICK_WARPS = 16;    // of a block: teams of TW warps, and a warp more for each
 constexpr int MAX_PICK_CLUSTER = 8;
 constexpr int MAX_SEL = MAX_K + MAX_K / 2 + 8;
 constexpr int BINS = 256;
 constexpr int RANK_CAP = 256;      // candidates that are ranked by counting
-constexpr double LSE_EPS = 3e-6;
+constexpr double LSE_EPS = 2e-6;
 constexpr float LOG2E_F = 1.44269504088896340736f;
 constexpr double LN2 = 0.69314718055994530942;
 
@@ -102,7 +101,8 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32) beam_scan_kernel(const T* __r
   float S;
   {
     const float2 c2 = make_float2(LOG2E_F, LOG2E_F), r2 = make_float2(-R, -R);
-    float2 a0 = make_float2(0.f, 0.f), a1 = a0;
+    // eight chains of eight additions
+    float2 a[4] = {};
 #pragma unroll
     for (int i = 0; i < UNIT_VECS; ++i) {
 #pragma unroll
@@ -110,13 +110,12 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32) beam_scan_kernel(const T* __r
         float2 t = fma2(Elem<T>::pair(v[i], q), c2, r2);
         t.x = ex2(t.x);
         t.y = ex2(t.y);
-        if (q & 1)
-          a1 = add2(a1, t);
-        else
-          a0 = add2(a0, t);
+        float2& to = a[(i * Elem<T>::PAIRS + q) & 3];
+        to = add2(to, t);
       }
     }
-    S = warp_reduce_add((a0.x + a0.y) + (a1.x + a1.y));
+    const float2 b = add2(add2(a[0], a[1]), add2(a[2], a[3]));
+    S = warp_reduce_add(b.x + b.y);
   }
   if (far || S != S) {
     // the number of maxima, or a sum that leaves NaN out
@@ -480,7 +479,9 @@ struct PickShared {
   double ref[MAX_W], logs[MAX_W], cum[MAX_W];  // logp(x) = (x - ref) - logs, or -logs for x = ref = +inf
   double red[40];
   int n[MAX_W];
-  int sorted[RANK_CAP];
+  int sorted[RANK_CAP], reach[RANK_CAP];
+  int part[MAX_W], part_at[MAX_W];
+  int ranked;
   unsigned long long flagged;
 };
 
@@ -498,8 +499,10 @@ __device__ __forceinline__ double key_value64(unsigned long long k) {
 }
 
 // Ranks the candidates of the group's lists; `sorted` gets the positions
-// w * K + r of the first RANK_CAP.  Returns their number.
+// w * K + r of the first `ranked` (K at least, if there are as many).  Returns
+// the number of candidates.
 __device__ __forceinline__ int rank_candidates(PickShared& sh, const float* xs, unsigned long long* score, int W, int K) {
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, warps = blockDim.x >> 5;
   int total = 0;
   for (int w = 0; w < W; ++w) total += sh.n[w];
   const int all = W * K;
@@ -510,17 +513,72 @@ __device__ __forceinline__ int rank_candidates(PickShared& sh, const float* xs, 
   __syncthreads();
   if (all <= RANK_CAP) {
     // a warp per candidate: those ahead are larger, or equal and of a lower beam (or earlier in the list)
-    const int lane = threadIdx.x & 31;
-    for (int j = threadIdx.x >> 5; j < all; j += blockDim.x >> 5) {
+    for (int j = wid; j < all; j += warps) {
       const unsigned long long s = score[j];
       int rank = 0;
       for (int o = lane; o < all; o += 32) rank += score[o] + (o < j) > s;
       rank = __reduce_add_sync(FULL, rank);
       if (lane == 0 && s != 0ull) sh.sorted[rank] = j;
     }
+    if (threadIdx.x == 0) sh.ranked = total;
     __syncthreads();
     return total;
   }
+  if (wid == 0) {
+    // a score that between K and RANK_CAP candidates reach: lane l counts in the (sorted) lists l and l + 32
+    auto count = [&](unsigned long long t, int w) {
+      int lo = 0, hi = w < W ? sh.n[w] : 0;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (score[w * K + mid] >= t)
+          lo = mid + 1;
+        else
+          hi = mid;
+      }
+      return lo;
+    };
+    unsigned long long lo = 1ull, hi = ~0ull;
+    int have = total;
+    while (have > RANK_CAP && hi - lo > 1) {
+      const unsigned long long mid = lo + (hi - lo) / 2;
+      const int c = __reduce_add_sync(FULL, count(mid, lane) + count(mid, lane + 32));
+      if (c >= K) {
+        lo = mid;
+        have = c;
+      } else {
+        hi = mid;
+      }
+    }
+    // the lists' parts that reach it, one behind the other
+    const int a = count(lo, lane), b = count(lo, lane + 32);
+    const int at_a = warp_incl_scan_add(a) - a, first = __reduce_add_sync(FULL, a);
+    const int at_b = first + warp_incl_scan_add(b) - b;
+    sh.part[lane] = a;
+    sh.part[lane + 32] = b;
+    sh.part_at[lane] = at_a;
+    sh.part_at[lane + 32] = at_b;
+    if (lane == 0) sh.ranked = have;
+  }
+  __syncthreads();
+  const int have = sh.ranked;
+  if (have <= RANK_CAP) {
+    for (int j = threadIdx.x; j < all; j += blockDim.x) {
+      const int w = j / K, r = j - w * K;
+      if (r < sh.part[w]) sh.reach[sh.part_at[w] + r] = j;
+    }
+    __syncthreads();
+    for (int i = wid; i < have; i += warps) {
+      const int j = sh.reach[i];
+      const unsigned long long s = score[j];
+      int rank = 0;
+      for (int o = lane; o < have; o += 32) rank += score[sh.reach[o]] + (o < i) > s;
+      rank = __reduce_add_sync(FULL, rank);
+      if (lane == 0) sh.sorted[rank] = j;
+    }
+    __syncthreads();
+    return total;
+  }
+  // more than RANK_CAP candidates share the K-th score: by bisection in every list
   for (int j = threadIdx.x; j < all; j += blockDim.x) {
     const unsigned long long s = score[j];
     if (s == 0ull) continue;
@@ -540,6 +598,7 @@ __device__ __forceinline__ int rank_candidates(PickShared& sh, const float* xs, 
     }
     if (rank < RANK_CAP) sh.sorted[rank] = j;
   }
+  if (threadIdx.x == 0) sh.ranked = RANK_CAP;
   __syncthreads();
   return total;
 }
@@ -553,7 +612,7 @@ __device__ __forceinline__ P* in_first(P* p) {
 }
 
 template <typename T, int TW, bool WIDE>
-__global__ void __launch_bounds__(MAX_TEAMS*(TEAM + 1) * 32) beam_pick_kernel(
+__global__ void __launch_bounds__(PICK_WARPS * 32) beam_pick_kernel(
     const T* __restrict__ logits, long long ld, long long V, const __grid_constant__ PickPlan pl, const float* cum,
     const uint8_t* done, BeamWs ws, float* out_score, int32_t* out_token, int32_t* out_parent, float* out_lse) {
   extern __shared__ __align__(16) char dyn[];
@@ -636,7 +695,7 @@ __global__ void __launch_bounds__(MAX_TEAMS*(TEAM + 1) * 32) beam_pick_kernel(
   __syncthreads();
   unsigned long long* score = (unsigned long long*)teams;
   const int total = rank_candidates(sh, xs, score, W, K);
-  const int have = min(total, RANK_CAP);
+  const int have = sh.ranked;
   if (W > 1 && total > 1) {
     if (wid == 0) {
       // neighbours whose order the sums do not settle, up to the first clear gap behind the K-th place
@@ -664,7 +723,7 @@ __global__ void __launch_bounds__(MAX_TEAMS*(TEAM + 1) * 32) beam_pick_kernel(
       lo = __reduce_or_sync(FULL, lo);
       hi = __reduce_or_sync(FULL, hi);
       // a run that leaves the ranked part: every row
-      if (lane == 0) sh.flagged = open && total > RANK_CAP ? ~0ull : ((unsigned long long)hi << 32) | lo;
+      if (lane == 0) sh.flagged = open && total > have ? ~0ull : ((unsigned long long)hi << 32) | lo;
     }
     __syncthreads();
     const unsigned long long flagged = sh.flagged;
@@ -674,9 +733,17 @@ __global__ void __launch_bounds__(MAX_TEAMS*(TEAM + 1) * 32) beam_pick_kernel(
         const T* q = logits + (row0 + w) * ld;
         const double m = sh.ref[w];
         double s = 0.0;
-        for (long long v = tid; v < V; v += blockDim.x) {
-          const float x = Elem<T>::load(q, v);
-          if (x == x) s += exp((double)x - m);
+        // 8 logits of a thread in flight
+        for (long long v0 = tid; v0 < V; v0 += 8 * blockDim.x) {
+          float x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const long long v = v0 + i * (long long)blockDim.x;
+            x[i] = v < V ? Elem<T>::load(q, v) : neg_inf();
+          }
+#pragma unroll 2
+          for (int i = 0; i < 8; ++i)
+            if (x[i] == x[i]) s += exp((double)x[i] - m);
         }
         s = block_reduce_add(s, sh.red);
         if (tid == 0) sh.logs[w] = log(s);
@@ -718,10 +785,11 @@ struct BeamStatePtrs {
 
 constexpr int ADV_THREADS = 128;
 
-// One block per group.  The ranks are walked by one thread: which candidates
-// end, which go on, and which slots of the pool they take.  The block then
-// moves the token histories: a thread owns a column of all beams, so rows
-// exchange places without another buffer.
+// One block per group.  One warp walks over the ranks, the pool's scores in its
+// lanes: which candidates end, which go on, and which slots of the pool they
+// take.  The block then moves the token histories: a thread owns a column of
+// all beams, so rows exchange places without another buffer.  A step's time is
+// three dependent reads and the ranks, some 60 cycles each.
 __global__ void __launch_bounds__(ADV_THREADS) beam_advance_kernel(const float* __restrict__ score,
                                                                    const int32_t* __restrict__ token,
                                                                    const int32_t* __restrict__ parent, int W, int K,
@@ -732,71 +800,97 @@ __global__ void __launch_bounds__(ADV_THREADS) beam_advance_kernel(const float* 
   __shared__ uint8_t is_stop[MAX_K];
   __shared__ float cand_s[MAX_K];
   __shared__ int32_t cand_t[MAX_K], cand_p[MAX_K];
-  __shared__ float fin_score[MAX_W], new_cum[MAX_W];
-  __shared__ int32_t fin_len[MAX_W], src[MAX_W], new_par[MAX_W], new_tok[MAX_W];
+  __shared__ float new_cum[MAX_W];
+  __shared__ int32_t src[MAX_W], new_par[MAX_W], new_tok[MAX_W];
   __shared__ double len_pow[3];
-  __shared__ int live_n, fin_n, code;
+  __shared__ int live_n;
+  static_assert(MAX_W == 64 && ADV_THREADS >= MAX_K, "two pool slots a lane, a thread per candidate");
   const long long g = blockIdx.x;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31;
   const long long limit = min(max_tokens, max_seq_len);
-  if (st.done[g]) {
-    if (tid < W) st.parent[g * W + tid] = -1;
-    return;
-  }
+  // everything a step needs is on its way at once
+  const uint8_t was_done = st.done[g];
   const long long c = st.count[g];
-  if (c >= limit) {
-    __syncthreads();  // every thread has read `done`
-    if (tid == 0) st.done[g] = 2;
-    if (tid < W) st.parent[g * W + tid] = -1;
-    return;
-  }
-  for (int r = tid; r < K; r += ADV_THREADS) {
-    const int32_t t = token[g * K + r];
+  const int had = st.fin_count[g];
+  if (tid < K) {
+    const int32_t t = token[g * K + tid];
+    cand_s[tid] = score[g * K + tid];
+    cand_p[tid] = parent[g * K + tid];
+    cand_t[tid] = t;
     bool s = false;
     for (long long j = 0; j < n_stop; ++j) s = s || stop[j] == (uint32_t)t;
-    is_stop[r] = s;
-    cand_s[r] = score[g * K + r];
-    cand_t[r] = t;
-    cand_p[r] = parent[g * K + r];
+    is_stop[tid] = s;
   }
-  for (int w = tid; w < W; w += ADV_THREADS) {
-    fin_score[w] = st.fin_score[g * W + w];
-    fin_len[w] = st.fin_len[g * W + w];
-    src[w] = -1;
-    new_par[w] = -1;
-    new_cum[w] = neg_inf();
+  if (tid < W) {
+    src[tid] = -1;
+    new_par[tid] = -1;
+    new_cum[tid] = neg_inf();
   }
-  if ((tid & 31) == 0 && tid < 96)
-    len_pow[tid >> 5] = pow((double)(tid == 0 ? c + 1 : tid == 32 ? c + 2 : limit), alpha);
+  // the pool: slots lane and lane + 32; slots that are not there never have the lowest score
+  float fin0 = pos_inf(), fin1 = pos_inf();
+  int len0 = 0, len1 = 0;
+  if (tid < 32) {
+    if (lane < W) {
+      fin0 = st.fin_score[g * W + lane];
+      len0 = st.fin_len[g * W + lane];
+    }
+    if (lane + 32 < W) {
+      fin1 = st.fin_score[g * W + lane + 32];
+      len1 = st.fin_len[g * W + lane + 32];
+    }
+  }
+  if (was_done || c >= limit) {
+    __syncthreads();  // every thread has read `done`
+    if (tid == 0 && !was_done) st.done[g] = 2;
+    if (tid < W) st.parent[g * W + tid] = -1;
+    return;
+  }
+  if (lane == 0 && tid >= 32 && tid < 128)
+    len_pow[(tid >> 5) - 1] = pow((double)(tid == 32 ? c + 1 : tid == 64 ? c + 2 : limit), alpha);
   __syncthreads();
-  if (tid == 0) {
-    int live = 0, fins = st.fin_count[g];
-    // slot of a hypothesis in the pool of the W best, or -1; equal lowest scores: the highest slot gives way
+  if (tid < 32) {
+    int live = 0, fins = had;
+    // a hypothesis goes to the pool of the W best; of equal lowest scores the highest slot gives way
+    auto lowest = [&](uint32_t& low) {
+      const uint32_t k0 = lane < W ? order_key(fin0) : 0xffffffffu, k1 = lane + 32 < W ? order_key(fin1) : 0xffffffffu;
+      low = __reduce_min_sync(FULL, min(k0, k1));
+      const uint32_t in1 = __ballot_sync(FULL, k1 == low), in0 = __ballot_sync(FULL, k0 == low);
+      return in1 ? 63 - __clz(in1) : 31 - __clz(in0);
+    };
     auto insert = [&](float norm, int from, int len) {
       int slot = fins;
       if (fins >= W) {
-        slot = 0;
-        for (int w = 1; w < W; ++w)
-          if (fin_score[w] <= fin_score[slot]) slot = w;
-        if (!(norm > fin_score[slot])) return;
+        uint32_t low;
+        slot = lowest(low);
+        if (!(norm > key_value(low))) return;
       } else {
         ++fins;
       }
-      fin_score[slot] = norm;
-      fin_len[slot] = len;
-      src[slot] = from;
+      if (slot == lane) {
+        fin0 = norm;
+        len0 = len;
+      }
+      if (slot == lane + 32) {
+        fin1 = norm;
+        len1 = len;
+      }
+      if (lane == 0) src[slot] = from;
     };
     for (int r = 0; r < K; ++r) {
-      if (cand_t[r] < 0 || cand_p[r] < 0 || cand_p[r] >= W) continue;
+      const int t = cand_t[r], q = cand_p[r];
+      if (t < 0 || q < 0 || q >= W) continue;
       if (is_stop[r]) {
-        if (r < W) insert((float)((double)cand_s[r] / len_pow[0]), cand_p[r], (int)c);
+        if (r < W) insert((float)((double)cand_s[r] / len_pow[0]), q, (int)c);
       } else if (live < W) {
-        new_par[live] = cand_p[r];
-        new_tok[live] = cand_t[r];
-        new_cum[live] = cand_s[r];
+        if (lane == 0) {
+          new_par[live] = q;
+          new_tok[live] = t;
+          new_cum[live] = cand_s[r];
+        }
         ++live;
       }
     }
+    __syncwarp();
     int d = 0;
     if (c + 1 >= limit) {
       for (int w = 0; w < live; ++w) insert((float)((double)new_cum[w] / len_pow[0]), MAX_W + w, (int)c + 1);
@@ -804,17 +898,28 @@ __global__ void __launch_bounds__(ADV_THREADS) beam_advance_kernel(const float* 
     } else if (live == 0) {
       d = 1;
     } else if (fins >= W) {
-      float low = fin_score[0], best = new_cum[0];
-      for (int w = 1; w < W; ++w) {
-        low = fminf(low, fin_score[w]);
-        best = fmaxf(best, new_cum[w]);
-      }
+      uint32_t low;
+      lowest(low);
+      float best = lane < live ? new_cum[lane] : neg_inf();
+      if (lane + 32 < live) best = fmaxf(best, new_cum[lane + 32]);
+      best = warp_max(best);
       const double ahead = fmax((double)best / len_pow[1], (double)best / len_pow[2]);
-      if (early || (double)low >= ahead) d = 1;
+      if (early || (double)key_value(low) >= ahead) d = 1;
     }
-    live_n = live;
-    fin_n = fins;
-    code = d;
+    if (lane < W) {
+      st.fin_score[g * W + lane] = fin0;
+      st.fin_len[g * W + lane] = len0;
+    }
+    if (lane + 32 < W) {
+      st.fin_score[g * W + lane + 32] = fin1;
+      st.fin_len[g * W + lane + 32] = len1;
+    }
+    if (lane == 0) {
+      live_n = live;
+      st.fin_count[g] = fins;
+      st.count[g] = (int32_t)(c + 1);
+      st.done[g] = (uint8_t)d;
+    }
   }
   __syncthreads();
   int32_t* hist = st.tokens + g * W * st.cap;
@@ -832,20 +937,13 @@ __global__ void __launch_bounds__(ADV_THREADS) beam_advance_kernel(const float* 
         if (new_par[w] != w) hist[w * st.cap + i] = tile[w * ADV_THREADS + tid];
     }
   }
-  for (int w = tid; w < W; w += ADV_THREADS) {
-    if (w < live) {
-      hist[w * st.cap + c] = new_tok[w];
-      st.last[g * W + w] = new_tok[w];
+  if (tid < W) {
+    if (tid < live) {
+      hist[tid * st.cap + c] = new_tok[tid];
+      st.last[g * W + tid] = new_tok[tid];
     }
-    st.cum[g * W + w] = new_cum[w];
-    st.parent[g * W + w] = new_par[w];
-    st.fin_score[g * W + w] = fin_score[w];
-    st.fin_len[g * W + w] = fin_len[w];
-  }
-  if (tid == 0) {
-    st.count[g] = (int32_t)(c + 1);
-    st.fin_count[g] = fin_n;
-    st.done[g] = (uint8_t)code;
+    st.cum[g * W + tid] = new_cum[tid];
+    st.parent[g * W + tid] = new_par[tid];
   }
   __syncthreads();
   // beams that reached the limit
