@@ -435,7 +435,7 @@ int pesti_beam_reorder(const pesti_beam_rows* states, int64_t n_states, const in
  * lists and of pesti_beam_select's log-probabilities.  No counterpart in the
  * reference.
  *
- * Student logits [N, ld] (first V <= 2^30 columns; F32, BF16 or F16) at temperature T:
+ * Student logits [N, ld] (first V columns; F32, BF16 or F16) at temperature T:
  * p = softmax(x / T) over all V tokens.  The teacher of row n lists k entries
  * (token d_idx[n*idx_ld + j], logit or log-probability t = d_val[n*val_ld + j],
  * val_dtype F32, BF16 or F16), 1 <= k <= PESTI_DISTILL_MAX_TOP; entries whose

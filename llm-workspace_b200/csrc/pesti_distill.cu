@@ -26,7 +26,7 @@ int common(DistillArgs& a, const void* d_logits, pesti_dtype dtype, int64_t N, i
   if (!half_or_float(val_dtype)) return refuse("teacher values must be f32, bf16 or f16");
   if (N < 0) return refuse("N < 0");
   if (N > 0x7fffffffLL) return refuse("N must be below 2^31");
-  if (V < 1 || V > (1LL << 30)) return refuse("V must be 1 to 2^30");
+  if (V < 1 || V > 0x7fffffffLL) return refuse("V must be 1 to 2^31-1");
   if (ld < V) return refuse("ld is below V");
   if (k < 1 || k > PESTI_DISTILL_MAX_TOP) return refuse("k must be 1 to 256");
   // one value may stand for all rows (stride 0)
@@ -138,7 +138,7 @@ extern "C" {
 int64_t pesti_distill_topk_workspace(pesti_dtype dtype, int64_t N, int64_t V, int64_t k) {
   if (!half_or_float(dtype)) return refuse("logits must be f32, bf16 or f16");
   if (N < 0) return refuse("N < 0");
-  if (V < 1 || V > (1LL << 30)) return refuse("V must be 1 to 2^30");
+  if (V < 1 || V > 0x7fffffffLL) return refuse("V must be 1 to 2^31-1");
   if (k < 1 || k > PESTI_DISTILL_MAX_TOP) return refuse("k must be 1 to 256");
   const long long units = dtype == PESTI_F32 ? row_units<float>(V) : row_units<__half>(V);
   if (N > 0x7fffffffLL / units) return refuse("N * V too large");

@@ -123,14 +123,14 @@ def beam_select(logits, beams: int, k: int, cum=None, done=None, lse=None, out=N
 
     def call(st):
         if out is None:
-            score = torch.empty((G, k), dtype=torch.float32, device=dev)
-            token = torch.empty((G, k), dtype=torch.int32, device=dev)
-            parent = torch.empty((G, k), dtype=torch.int32, device=dev)
+            score = logits.new_empty((G, k), dtype=torch.float32)
+            token = logits.new_empty((G, k), dtype=torch.int32)
+            parent = logits.new_empty((G, k), dtype=torch.int32)
         else:
             score, token, parent = out
         if G:
             need = _select_workspace(dtype, G, beams, V, k)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            ws = logits.new_empty(need, dtype=torch.uint8)
             rc = load_library().pesti_beam_select(
                 logits.data_ptr(), dtype, G, beams, V, _row_stride(logits), _ptr(cum), _ptr(done), k,
                 score.data_ptr(), token.data_ptr(), parent.data_ptr(), _ptr(lse), ws.data_ptr(), need, st)

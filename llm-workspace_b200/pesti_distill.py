@@ -67,10 +67,10 @@ class _DistillTopk(torch.autograd.Function):
         N, dev, keep = logits.shape[0], logits.device, ctx.needs_input_grad[0]
 
         def call(st):
-            loss = torch.empty(N, dtype=torch.float32, device=dev)
-            stats = torch.empty((N, _stats(args[10])), dtype=torch.float64, device=dev) if keep else None
+            loss = logits.new_empty(N, dtype=torch.float32)
+            stats = logits.new_empty((N, _stats(args[10])), dtype=torch.float64) if keep else None
             need = _workspace(args[1], N, args[3], args[10])
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            ws = logits.new_empty(need, dtype=torch.uint8)
             rc = load_library().pesti_distill_topk(*args, loss.data_ptr(), _ptr(stats), None, 0, ws.data_ptr(), need,
                                                    st)
             if rc:
@@ -92,7 +92,7 @@ class _DistillTopk(torch.autograd.Function):
             up = up.to(torch.float32)
 
         def call(st):
-            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+            grad = logits.new_empty(logits.shape)
             rc = load_library().pesti_distill_topk_backward(*ctx.args, stats.data_ptr(), up.data_ptr(), up.stride(0),
                                                             grad.data_ptr(), logits.shape[1], st)
             if rc:
@@ -113,7 +113,8 @@ def distill_topk(logits, idx, val, temperature: float = 1.0, teacher_lse=None, w
     vocabulary (0 for log-probabilities at temperature 1): the mass outside the
     list is then one more outcome.  weight: optional [N] float32; rows of weight
     0 are not read.  loss = weight * T^2 * KL(teacher || student).
-    The teacher is a constant: no gradient reaches idx, val or teacher_lse."""
+    The teacher and the weights are constants: no gradient reaches idx, val,
+    teacher_lse or weight."""
     return _DistillTopk.apply(logits, idx, val, temperature, teacher_lse, weight)
 
 
@@ -133,10 +134,10 @@ def distill_topk_grad(logits, idx, val, temperature: float = 1.0, teacher_lse=No
               "grad must match the logits and have contiguous rows")
 
     def call(st):
-        loss = torch.empty(N, dtype=torch.float32, device=dev)
-        to = torch.empty((N, V), dtype=logits.dtype, device=dev) if grad is None else grad
+        loss = logits.new_empty(N, dtype=torch.float32)
+        to = logits.new_empty((N, V)) if grad is None else grad
         need = _workspace(args[1], N, V, args[10])
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        ws = logits.new_empty(need, dtype=torch.uint8)
         rc = load_library().pesti_distill_topk(*args, loss.data_ptr(), None, to.data_ptr(), _row_stride(to),
                                                ws.data_ptr(), need, st)
         if rc:

@@ -1,8 +1,8 @@
 """Beam search on the GPU against the 64-bit oracle (oracle/beam.py): selection,
 loop control, reordering of states, and a whole search.
 
-Tolerance of a score: the row's log sum is off by at most 3e-6 (the bound the
-kernel's own comment derives), and the score is rounded once to f32 (half a
+Tolerance of a score: the row's log sum is off by at most 3e-6 (above the bound
+that the kernel's own comment derives), and the score is rounded once to f32 (half a
 step, 2^-24 of it).  Tokens and parents are exact."""
 import numpy as np
 import pytest
@@ -49,7 +49,8 @@ def _check(x, W, K, cum=None, done=None):
 @pytest.mark.parametrize("G,W,V,K,pad", [
     (1, 1, 1, 1, 0), (2, 3, 7, 6, 1), (1, 4, 1000, 8, 0), (3, 5, 4099, 10, 1), (2, 16, 32001, 32, 3),
     (1, 64, 2100, 128, 0), (1, 2, 128256, 4, 0), (4, 2, 2048, 128, 0), (1, 7, 100, 128, 5), (5, 1, 32000, 64, 0),
-    (1, 3, 2049, 1, 7),
+    (1, 3, 2049, 1, 7), (2, 2, 3, 20, 0), (1, 33, 5000, 100, 1), (3, 9, 40000, 27, 0), (70, 8, 3000, 16, 0),
+    (400, 3, 2500, 6, 0), (300, 1, 9000, 40, 0),
 ])
 def test_select(dtype, G, W, V, K, pad):
     x = _logits(G * W, V, dtype, pad)
