@@ -303,6 +303,28 @@ __device__ __forceinline__ uint32_t select_by_bisection(Team<TW>& t, int nkeys, 
   return lo;
 }
 
+// The first bin whose running count reaches K goes to CUT, -1 if there is none or the count is above `most`.
+// In step before (the bins are filled) and behind it.
+template <int TW>
+__device__ __forceinline__ void find_bin(const Team<TW>& t, int K, int most) {
+  if (t.tid < 32) {
+    // lane l adds up bins 8l..8l+7
+    const int4 c0 = ((const int4*)t.hist)[2 * t.tid], c1 = ((const int4*)t.hist)[2 * t.tid + 1];
+    const int sum = c0.x + c0.y + c0.z + c0.w + c1.x + c1.y + c1.z + c1.w;
+    int upto = warp_incl_scan_add(sum);
+    const uint32_t hit = __ballot_sync(FULL, upto >= K);
+    if (hit == 0) {
+      if (t.tid == 0) t.word[TM_CUT] = -1;
+    } else if (t.tid == __ffs(hit) - 1) {
+      upto -= sum;
+      int bin = 8 * t.tid - 1;
+      while (upto < K) upto += t.hist[++bin];
+      t.word[TM_CUT] = upto <= most ? bin : -1;
+    }
+  }
+  team_sync(t);
+}
+
 // Segment i of the selected ones (WIDE: runs of segments).
 template <bool WIDE, int TW>
 __device__ __forceinline__ long long selected(const Team<TW>& t, const PickPlan& pl, int i) {
@@ -382,11 +404,13 @@ __device__ __forceinline__ int pick_row(Team<TW>& t, const PickPlan& pl, const T
   kmin = (uint32_t)t.word[TM_MIN];
   if (valid == 0) return 0;
   const int most = K + K / 2 + 8;
-  bool binned = valid > most && kmax != kmin;
+  bool binned = valid > K && kmax != kmin;
   uint32_t least = KEY_NEG_INF + 1;
-  if (valid <= most) {
+  const bool whole = valid <= K || (valid <= most && kmax == kmin);  // every segment with a finite value
+  if (whole) {
     for (int i = t.tid; i < nkeys; i += N)
       if (t.keys[i] > KEY_NEG_INF) t.sel[atomicAdd(t.word + TM_NSEL, 1)] = i;
+    if (valid >= K) least = kmin;
   }
   if (binned) {
     // 256 bins of equal width of the keys, from the largest down (over four powers of two at most)
@@ -397,22 +421,7 @@ __device__ __forceinline__ int pick_row(Team<TW>& t, const PickPlan& pl, const T
       if (b < BINS) atomicAdd(t.hist + b, 1);
     }
     team_sync(t);
-    if (t.tid < 32) {
-      // lane l adds up bins 8l..8l+7; the first bin whose running count reaches K
-      const int4 c0 = ((const int4*)t.hist)[2 * lane], c1 = ((const int4*)t.hist)[2 * lane + 1];
-      const int sum = c0.x + c0.y + c0.z + c0.w + c1.x + c1.y + c1.z + c1.w;
-      int upto = warp_incl_scan_add(sum);
-      const uint32_t hit = __ballot_sync(FULL, upto >= K);
-      if (hit == 0) {
-        if (lane == 0) t.word[TM_CUT] = -1;
-      } else if (lane == __ffs(hit) - 1) {
-        upto -= sum;
-        int bin = 8 * lane - 1;
-        while (upto < K) upto += t.hist[++bin];
-        t.word[TM_CUT] = upto <= most ? bin : -1;
-      }
-    }
-    team_sync(t);
+    find_bin(t, K, most);
     const int bin = t.word[TM_CUT];
     binned = bin >= 0;
     if (binned) {
@@ -428,12 +437,29 @@ __device__ __forceinline__ int pick_row(Team<TW>& t, const PickPlan& pl, const T
       least = __reduce_min_sync(FULL, least);
     }
   }
-  if (valid > most && !binned) least = select_by_bisection(t, nkeys, K, kmax, most);
+  if (!whole && !binned) least = select_by_bisection(t, nkeys, K, kmax, most);
   if (lane == 0) atomicMin((uint32_t*)t.word + TM_T, least);
   team_sync(t);
-  const float cut = key_value((uint32_t)t.word[TM_T]);
+  float cut = key_value((uint32_t)t.word[TM_T]);
   // their elements from the cut up: all at once, or in rounds that keep the list short
   const int todo = t.word[TM_NSEL] * (WIDE ? pl.run : 1), head = row_head<T>(p);
+  if (valid < K) {
+    // fewer segments than K say nothing of the K-th logit: the maxima of their vectors do
+    for (int i = t.tid; i < BINS; i += N) t.hist[i] = 0;
+    team_sync(t);
+    constexpr int sh = 17;  // 64 bins to a power of two
+#pragma unroll 2
+    for (int i = t.tid >> 5; i < todo; i += TW) {
+      const float m = Elem<T>::vec_max(load_seg_vec<T>(p, head, V, selected<WIDE>(t, pl, i), lane));
+      const uint32_t b = (kmax - order_key(m)) >> sh;
+      if (m > neg_inf() && b < BINS) atomicAdd(t.hist + b, 1);
+    }
+    team_sync(t);
+    find_bin(t, K, 0x7fffffff);
+    const int bin = t.word[TM_CUT];
+    const uint32_t down = ((uint32_t)bin + 1u) << sh;
+    if (bin >= 0 && down < kmax - KEY_NEG_INF) cut = key_value(kmax - down + 1u);
+  }
   for (int i0 = t.tid >> 5; i0 < todo; i0 += 8 * TW) {
     uint4 v[8];
 #pragma unroll
