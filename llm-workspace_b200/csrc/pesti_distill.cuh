@@ -38,6 +38,7 @@
 namespace pesti_rows {
 
 constexpr int MAX_TOP = 256;
+constexpr int HASH = 512;
 constexpr int STATS = 8;       // numbers of a row, and then its list's gradients
 constexpr int UNIT_WARPS = 4;  // warps of a block, a unit each
 constexpr double ONE_LN2 = 0.69314718055994530942;
@@ -249,9 +250,9 @@ __device__ __forceinline__ Partial scan_unit(const DistillArgs& a, long long n, 
   return p;
 }
 
-// A row's list, by one warp.
+// A row's list, by one warp.  `hash` (HASH words of shared memory) finds equal tokens.
 template <typename T>
-__device__ __forceinline__ void list_row(const DistillArgs& a, long long n, int lane) {
+__device__ __forceinline__ void list_row(const DistillArgs& a, long long n, int32_t* hash, int lane) {
   const double inf = (double)pos_inf(), invT = 1.0 / a.T;
   const bool tail = a.teacher_lse != nullptr;
   const T* row = (const T*)a.logits + n * a.ld;
@@ -261,10 +262,12 @@ __device__ __forceinline__ void list_row(const DistillArgs& a, long long n, int 
     const int32_t id = j < a.k ? idx[j] : -1;
     return id >= 0 && id < a.V ? id : -1;
   };
+  for (int i = lane; i < HASH; i += 32) hash[i] = -1;
+  __syncwarp();
   // the largest teacher value and listed logit
   double mt = -inf;
   float mx = neg_inf();
-#pragma unroll 2
+#pragma unroll 4
   for (int j = lane; j < a.k; j += 32) {
     const int32_t id = listed(j);
     const double t = teacher_value(a, n, j) * invT;
@@ -286,12 +289,15 @@ __device__ __forceinline__ void list_row(const DistillArgs& a, long long n, int 
   for (int j0 = 0; j0 < a.k; j0 += 32) {
     const int j = j0 + lane;
     const int32_t id = listed(j);
-    bool first = id >= 0;
-    for (int o0 = 0; o0 <= j0; o0 += 32) {
-      const int32_t other = listed(o0 + lane);
-#pragma unroll 8
-      for (int o = 0; o < 32; ++o)
-        if (__shfl_sync(FULL, other, o) == id && o0 + o < j) first = false;
+    bool first = false;  // this entry stands for its token
+    if (id >= 0) {
+      uint32_t h = ((uint32_t)id * 2654435761u) >> 23;
+      for (;;) {
+        const int32_t had = atomicCAS(hash + h, -1, id);
+        first = had == -1;
+        if (had == -1 || had == id) break;
+        h = (h + 1) & (HASH - 1);
+      }
     }
     twice = twice || (id >= 0 && !first);
     if (j < a.k) {
@@ -408,6 +414,44 @@ __device__ __forceinline__ void join_row(const DistillArgs& a, long long n, int 
   }
 }
 
+// Stores a unit's gradient vectors whose elements start d (1 to VE - 1) places before a 16-byte boundary of the
+// gradient: each lane writes the vector that its own and the next lane's make up, the unit's ragged ends go one by one.
+// (461 rows of 256000 bf16 whose logits are padded by one: 333 us with single elements.)
+template <typename T>
+__device__ __forceinline__ void store_shifted(T* to, const uint4 (&g)[UNIT_VECS], int d, int lane) {
+  constexpr int VE = Elem<T>::VE;
+  const int words = d * (int)sizeof(T) / 4, bits = d * (int)sizeof(T) % 4 * 8;
+#pragma unroll
+  for (int i = 0; i < UNIT_VECS; ++i) {
+    // lane 31's neighbour is lane 0 of the next vectors
+    const uint4 out = lane == 0 && i + 1 < UNIT_VECS ? g[i + 1 < UNIT_VECS ? i + 1 : i] : g[i];
+    const int next = (lane + 1) & 31;
+    const uint32_t w[8] = {g[i].x,
+                           g[i].y,
+                           g[i].z,
+                           g[i].w,
+                           __shfl_sync(FULL, out.x, next),
+                           __shfl_sync(FULL, out.y, next),
+                           __shfl_sync(FULL, out.z, next),
+                           __shfl_sync(FULL, out.w, next)};
+    uint32_t r[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t lo = w[k], hi = w[k + 1];
+      if (words == 1) lo = w[k + 1], hi = w[k + 2 < 8 ? k + 2 : 7];
+      if (words == 2) lo = w[k + 2], hi = w[k + 3 < 8 ? k + 3 : 7];
+      if (words == 3) lo = w[k + 3], hi = w[k + 4 < 8 ? k + 4 : 7];
+      r[k] = __funnelshift_r(lo, hi, bits);
+    }
+    if (i + 1 < UNIT_VECS || lane < 31) *(uint4*)(to + i * 32 * VE + d) = make_uint4(r[0], r[1], r[2], r[3]);
+  }
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    if (lane == 0 && e < d) Elem<T>::store(to, e, Elem<T>::at(g[0], e));
+    if (lane == 31 && e >= d) Elem<T>::store(to + (UNIT_VECS - 1) * 32 * VE, e, Elem<T>::at(g[UNIT_VECS - 1], e));
+  }
+}
+
 // The gradient of a unit, in place too: everything is read before anything is written.
 template <typename T>
 __device__ __forceinline__ void grad_unit(const DistillArgs& a, long long n, long long u, double scale, int lane) {
@@ -422,9 +466,18 @@ __device__ __forceinline__ void grad_unit(const DistillArgs& a, long long n, lon
   const long long first = u * UNIT_SLOTS * VE - head, lo = first + lane * VE;
   constexpr int span = UNIT_SLOTS * VE;
   __syncwarp();
-  const bool plain = row_head<T>(grow) == head && first >= 0 && first + span <= a.V && !(m > neg_inf() && is_far(m, a.c));
-  if (plain) {
-    store_plain<T>(grow + lo, v, reference(m, a.c), near_factor<T>(A, m, a), a);
+  const bool inner = first >= 0 && first + span <= a.V && !(m > neg_inf() && is_far(m, a.c));
+  const int past = row_head<T>(grow + lo);  // the vectors' place behind a 16-byte boundary of the gradient
+  if (inner) {
+    const float R = reference(m, a.c), f = near_factor<T>(A, m, a);
+    if (past == 0) {
+      store_plain<T>(grow + lo, v, R, f, a);
+    } else {
+      const float2 c2 = make_float2(a.c, a.c), lo2 = make_float2(a.c_lo, a.c_lo), r2 = make_float2(-R, -R);
+#pragma unroll
+      for (int i = 0; i < UNIT_VECS; ++i) v[i] = grad_vec<T>(v[i], c2, lo2, r2, f);
+      store_shifted<T>(grow + lo, v, VE - past, lane);
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < UNIT_VECS; ++i)
@@ -462,10 +515,11 @@ __global__ void __launch_bounds__(UNIT_WARPS * 32, 10) distill_scan_kernel(const
                                                                        long long list_blocks,
                                                                        long long blocks_per_row) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __shared__ int32_t hash[UNIT_WARPS][HASH];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   if (blockIdx.x < list_blocks) {
     const long long n = (long long)blockIdx.x * UNIT_WARPS + wid;
-    if (n < a.N && takes_part(a, n)) list_row<T>(a, n, lane);
+    if (n < a.N && takes_part(a, n)) list_row<T>(a, n, hash[wid], lane);
     return;
   }
   const long long block = blockIdx.x - list_blocks, n = block / blocks_per_row;
@@ -489,8 +543,9 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) distill_join_kernel(const __g
     a.loss[n] = 0.0f;
 }
 
+// (32 warps an SM: 2048 rows of 152064 bf16 take 168 us, 7.4 TB/s of which some comes from L2.)
 template <typename T>
-__global__ void __launch_bounds__(UNIT_WARPS * 32) distill_backward_kernel(const __grid_constant__ DistillArgs a,
+__global__ void __launch_bounds__(UNIT_WARPS * 32, 8) distill_backward_kernel(const __grid_constant__ DistillArgs a,
                                                                            long long blocks_per_row) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const long long n = blockIdx.x / blocks_per_row;

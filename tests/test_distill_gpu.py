@@ -245,14 +245,16 @@ def test_gradient_in_place(dtype, V):
     assert g2.data_ptr() == x.data_ptr()
 
 
-def test_outputs_of_another_alignment():
-    """Logits and gradient rows that start at different places of a 16-byte line."""
-    x, idx, val, _ = _make(4, 4100, 8, "bf16", pad=0)
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_outputs_of_another_alignment(dtype):
+    """Logits and gradient rows that start at different places of a 16-byte line: every shift between them."""
+    x, idx, val, _ = _make(4, 9100, 8, dtype, pad=0)
     _, want = pd.distill_topk_grad(x, idx, val)
-    buf = torch.full((4, 4111), 7.0, dtype=torch.bfloat16, device="cuda")
-    pd.distill_topk_grad(x, idx, val, grad=buf[:, 3:4103])
-    assert torch.equal(buf[:, 3:4103], want)
-    assert (buf[:, :3] == 7).all() and (buf[:, 4103:] == 7).all()
+    for shift in range(1, 9):
+        buf = torch.full((4, 9117), 7.0, dtype=DT[dtype], device="cuda")
+        pd.distill_topk_grad(x, idx, val, grad=buf[:, shift:shift + 9100])
+        assert torch.equal(buf[:, shift:shift + 9100], want), shift
+        assert (buf[:, :shift] == 7).all() and (buf[:, shift + 9100:] == 7).all()
 
 
 def test_same_bits_every_time():
