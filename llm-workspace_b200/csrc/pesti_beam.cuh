@@ -507,9 +507,26 @@ struct PickShared {
   int n[MAX_W];
   int sorted[RANK_CAP], reach[RANK_CAP];
   int part[MAX_W], part_at[MAX_W];
+  double pow2[256];  // 2^(i/256)
   int ranked;
   unsigned long long flagged;
 };
+
+// e^d for d <= 0 (0 below -700, and for NaN), within 2^-51: a table of 2^(i/256) and a polynomial on |r| <= ln 2 / 512
+// (P. T. P. Tang's table-driven method, ACM Trans. Math. Softw. 15, 1989; r^5/120 is below 2^-54).  A row's sum is
+// bound by the rate of 64-bit operations: 12 of them a logit.
+__device__ __forceinline__ double exp_by_table(const double* pow2, double d) {
+  // 256 / ln 2, and ln 2 / 256 in two parts, the first of 29 bits
+  constexpr double MAGIC = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the rounded integer
+  const double t = fma(d, 369.3299304675746, MAGIC);
+  const int n = __double2loint(t);
+  const double k = t - MAGIC;
+  const double r = fma(k, -0x1.f473de6af278fp-38, fma(k, -0x1.62e42fe000000p-9, d));
+  const double y = fma(r * r, fma(r, fma(r, 1.0 / 24.0, 1.0 / 6.0), 0.5), r);
+  const double e = pow2[n & 255];
+  const double v = fma(e, y, e);
+  return d >= -700.0 ? __hiloint2double(__double2hiint(v) + ((n >> 8) << 20), __double2loint(v)) : 0.0;
+}
 
 __device__ __forceinline__ double beam_score(const PickShared& sh, int w, float x) {
   return sh.ref[w] == (double)pos_inf() ? sh.cum[w] - sh.logs[w] : sh.cum[w] + (((double)x - sh.ref[w]) - sh.logs[w]);
@@ -754,6 +771,8 @@ __global__ void __launch_bounds__(PICK_WARPS * 32) beam_pick_kernel(
     __syncthreads();
     const unsigned long long flagged = sh.flagged;
     if (flagged) {
+      for (int i = tid; i < 256; i += blockDim.x) sh.pow2[i] = exp2((double)i / 256.0);
+      __syncthreads();
       for (int w = 0; w < W; ++w) {
         if (!((flagged >> w) & 1ull) || sh.n[w] == 0 || sh.ref[w] == (double)pos_inf()) continue;
         const T* q = logits + (row0 + w) * ld;
@@ -767,9 +786,8 @@ __global__ void __launch_bounds__(PICK_WARPS * 32) beam_pick_kernel(
             const long long v = v0 + i * (long long)blockDim.x;
             x[i] = v < V ? Elem<T>::load(q, v) : neg_inf();
           }
-#pragma unroll 2
-          for (int i = 0; i < 8; ++i)
-            if (x[i] == x[i]) s += exp((double)x[i] - m);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) s += exp_by_table(sh.pow2, (double)x[i] - m);
         }
         s = block_reduce_add(s, sh.red);
         if (tid == 0) sh.logs[w] = log(s);
