@@ -164,6 +164,7 @@ int run_select(const void* logits, long long G, long long W, long long V, long l
     pick_shape(q, tw, &c);
     return G * c * q.teams * (tw + 1) <= (long long)sms * PICK_WARPS;
   };
+  pl.stay = at_once(7);
   if (at_once(7)) return launch_pick<T, 7>(logits, G, V, ld, pl, cum, done, ws, score, token, parent, lse, st);
   if (at_once(3) || K > 32) return launch_pick<T, 3>(logits, G, V, ld, pl, cum, done, ws, score, token, parent, lse, st);
   return launch_pick<T, 1>(logits, G, V, ld, pl, cum, done, ws, score, token, parent, lse, st);

@@ -31,7 +31,9 @@
 //   candidates of different beams whose scores differ by less than twice
 //   LSE_EPS are therefore not ordered by these sums: the merge adds up their
 //   rows again in 64 bits, in index order, and ranks once more (random logits,
-//   8 beams, K 16: about one group in 1500, which then takes some 20 us more).
+//   8 beams, K 16: about one group in 1500, which then takes some 40 us more;
+//   64-bit operations run at about 16 a cycle and SM, so rows are shared out
+//   over the cluster where its blocks are not needed for other groups).
 #pragma once
 #include "pesti_common.cuh"
 #include "pesti_rowscan.cuh"
@@ -148,6 +150,7 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32) beam_scan_kernel(const T* __r
 // the group's lists; the merge's scores take their place.
 struct PickPlan {
   int W, K, rows, teams, nkeys, run, cap;  // run: segments of a key; cap: entries of a team's list
+  int stay;                                // the cluster's blocks help to add up rows again
   long long units;
 };
 
@@ -508,6 +511,7 @@ struct PickShared {
   int sorted[RANK_CAP], reach[RANK_CAP];
   int part[MAX_W], part_at[MAX_W];
   double pow2[256];  // 2^(i/256)
+  double again[MAX_W][MAX_PICK_CLUSTER];
   int ranked;
   unsigned long long flagged;
 };
@@ -646,11 +650,11 @@ __device__ __forceinline__ int rank_candidates(PickShared& sh, const float* xs, 
   return total;
 }
 
-// The address of a shared variable of the cluster's first block.
+// The address of a shared variable of another block of the cluster.
 template <typename P>
-__device__ __forceinline__ P* in_first(P* p) {
+__device__ __forceinline__ P* in_block(P* p, uint32_t rank) {
   unsigned long long r;
-  asm volatile("mapa.u64 %0, %1, %2;" : "=l"(r) : "l"((unsigned long long)p), "r"(0u));
+  asm volatile("mapa.u64 %0, %1, %2;" : "=l"(r) : "l"((unsigned long long)p), "r"(rank));
   return (P*)r;
 }
 
@@ -675,7 +679,7 @@ __global__ void __launch_bounds__(PICK_WARPS * 32) beam_pick_kernel(
 
   const bool group_done = done && done[g];
   const int wid = tid >> 5, from = (int)crank * pl.rows, to = min(W, from + pl.rows);
-  PickShared* first = csize > 1 ? in_first(&sh) : &sh;
+  PickShared* first = csize > 1 ? in_block(&sh, 0) : &sh;
   if (wid < pl.teams * TW) {
     Team<TW> t;
     t.id = wid / TW;
@@ -686,8 +690,8 @@ __global__ void __launch_bounds__(PICK_WARPS * 32) beam_pick_kernel(
     t.hist = (int*)(t.keys + pl.nkeys);
     t.sel = t.hist + BINS;
     t.word = t.sel + MAX_SEL;
-    float* const first_xs = csize > 1 ? in_first(xs) : xs;
-    int32_t* const first_ids = csize > 1 ? in_first(ids) : ids;
+    float* const first_xs = csize > 1 ? in_block(xs, 0) : xs;
+    int32_t* const first_ids = csize > 1 ? in_block(ids, 0) : ids;
     for (int w = from + t.id; w < to; w += pl.teams) {
       int n = 0;
       if (!group_done && beam_running(cum, row0 + w))
@@ -732,18 +736,21 @@ __global__ void __launch_bounds__(PICK_WARPS * 32) beam_pick_kernel(
   if (csize > 1) {
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-    if (crank != 0) return;
+    if (crank != 0 && !pl.stay) return;
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   }
+  const uint32_t parts = pl.stay ? csize : 1u;  // blocks that add up rows again
   __syncthreads();
   unsigned long long* score = (unsigned long long*)teams;
-  const int total = rank_candidates(sh, xs, score, W, K);
-  const int have = sh.ranked;
-  if (W > 1 && total > 1) {
+  int total = 0;
+  unsigned long long flagged = 0ull;
+  if (crank == 0) {
+    total = rank_candidates(sh, xs, score, W, K);
+    const int have = sh.ranked;
     if (wid == 0) {
       // neighbours whose order the sums do not settle, up to the first clear gap behind the K-th place
       uint32_t lo = 0, hi = 0;
-      bool open = true;
+      bool open = W > 1;
       for (int i0 = 0; open && i0 + 1 < have; i0 += 32) {
         const int i = i0 + lane;
         bool near = false;
@@ -765,37 +772,65 @@ __global__ void __launch_bounds__(PICK_WARPS * 32) beam_pick_kernel(
       }
       lo = __reduce_or_sync(FULL, lo);
       hi = __reduce_or_sync(FULL, hi);
-      // a run that leaves the ranked part: every row
-      if (lane == 0) sh.flagged = open && total > have ? ~0ull : ((unsigned long long)hi << 32) | lo;
-    }
-    __syncthreads();
-    const unsigned long long flagged = sh.flagged;
-    if (flagged) {
-      for (int i = tid; i < 256; i += blockDim.x) sh.pow2[i] = exp2((double)i / 256.0);
-      __syncthreads();
-      for (int w = 0; w < W; ++w) {
-        if (!((flagged >> w) & 1ull) || sh.n[w] == 0 || sh.ref[w] == (double)pos_inf()) continue;
-        const T* q = logits + (row0 + w) * ld;
-        const double m = sh.ref[w];
-        double s = 0.0;
-        // 8 logits of a thread in flight
-        for (long long v0 = tid; v0 < V; v0 += 8 * blockDim.x) {
-          float x[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const long long v = v0 + i * (long long)blockDim.x;
-            x[i] = v < V ? Elem<T>::load(q, v) : neg_inf();
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) s += exp_by_table(sh.pow2, (double)x[i] - m);
-        }
-        s = block_reduce_add(s, sh.red);
-        if (tid == 0) sh.logs[w] = log(s);
-        __syncthreads();
+      // a run that leaves the ranked part: every row.  The blocks that stayed are told.
+      flagged = open && total > have ? ~0ull : ((unsigned long long)hi << 32) | lo;
+      for (uint32_t r = 1; r < parts; ++r) {
+        if (lane == 0) *in_block(&sh.flagged, r) = flagged;
+        if (flagged)
+          for (int w = lane; w < W; w += 32) *in_block(&sh.ref[w], r) = sh.ref[w];
       }
-      rank_candidates(sh, xs, score, W, K);
+      if (lane == 0) sh.flagged = flagged;
     }
   }
+  if (parts > 1) {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    if (crank != 0) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  }
+  __syncthreads();
+  flagged = sh.flagged;
+  if (flagged) {
+    if (parts > 1 && crank == 0) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    for (int i = tid; i < 256; i += blockDim.x) sh.pow2[i] = exp2((double)i / 256.0);
+    __syncthreads();
+    // each block its part of every row; the parts are as long for every row, and joined in order
+    const long long part = (V + parts - 1) / parts, begin = crank * part, stop = min(V, begin + part);
+    for (int w = 0; w < W; ++w) {
+      if (!((flagged >> w) & 1ull) || sh.ref[w] == (double)pos_inf()) continue;
+      const T* q = logits + (row0 + w) * ld;
+      const double m = sh.ref[w];
+      double s = 0.0;
+      // 16 logits of a thread in flight
+      for (long long v0 = begin + tid; v0 < stop; v0 += 16 * blockDim.x) {
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const long long v = v0 + i * (long long)blockDim.x;
+          x[i] = v < stop ? Elem<T>::load(q, v) : neg_inf();
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s += exp_by_table(sh.pow2, (double)x[i] - m);
+      }
+      s = block_reduce_add(s, sh.red);
+      if (tid == 0) first->again[w][crank] = s;
+    }
+    if (parts > 1) {
+      __syncwarp();
+      asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+      if (crank != 0) return;
+      asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    }
+    __syncthreads();
+    for (int w = tid; w < W; w += blockDim.x)
+      if (((flagged >> w) & 1ull) && sh.ref[w] != (double)pos_inf()) {
+        double s = 0.0;
+        for (uint32_t r = 0; r < parts; ++r) s += sh.again[w][r];
+        sh.logs[w] = log(s);
+      }
+    __syncthreads();
+    rank_candidates(sh, xs, score, W, K);
+  }
+  if (crank != 0) return;
   for (int r = tid; r < K; r += blockDim.x) {
     float sc = neg_inf();
     int tk = -1, pa = -1;
