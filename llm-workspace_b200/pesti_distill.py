@@ -30,7 +30,6 @@ def _workspace(dtype: int, N: int, V: int, k: int) -> int:
     return need
 
 
-
 def _lists(logits, idx, val, temperature, teacher_lse, weight):
     """Checks the arguments and returns them in the C call's order."""
     dtype = _rows_dtype(logits)
@@ -79,21 +78,24 @@ class _DistillTopk(torch.autograd.Function):
 
         loss, stats = _launch(dev, None, call)
         if keep:
-            ctx.args = args  # addresses of the tensors saved here
+            ctx.temperature = temperature
             ctx.save_for_backward(logits, idx, val, teacher_lse, weight, stats)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, up):
-        saved = ctx.saved_tensors  # refuses tensors that were written to since
-        logits, stats = saved[0], saved[5]
+        # refuses tensors that were written to since; hooks (activation checkpointing, offloading to the host) may
+        # hand back others of the same values, at other addresses and with other strides
+        logits, idx, val, teacher_lse, weight, stats = ctx.saved_tensors
+        args = _lists(logits, idx, val, ctx.temperature, teacher_lse, weight)
+        stats = stats.contiguous()
         if up.dtype != torch.float32:
             up = up.to(torch.float32)
 
         def call(st):
             grad = logits.new_empty(logits.shape)
-            rc = load_library().pesti_distill_topk_backward(*ctx.args, stats.data_ptr(), up.data_ptr(), up.stride(0),
+            rc = load_library().pesti_distill_topk_backward(*args, stats.data_ptr(), up.data_ptr(), up.stride(0),
                                                             grad.data_ptr(), logits.shape[1], st)
             if rc:
                 _check(rc)

@@ -13,6 +13,7 @@ step of the type, or of its smallest subnormal."""
 import numpy as np
 import pytest
 import torch
+from torch.utils.checkpoint import checkpoint
 
 import distill as OD
 import pesti_beam as pb
@@ -323,6 +324,50 @@ def test_autograd_through_a_head():
     assert (gW.float() - want).norm() <= 3 * 2.0 ** -8 * want.norm()
     with torch.no_grad():
         assert not pd.distill_topk(logits, idx, val).requires_grad
+
+
+@pytest.mark.parametrize("tail", [False, True])
+def test_saved_tensors_may_move(tail):
+    # hooks hand other tensors to the backward call: copies whose rows are padded, the originals overwritten
+    x, idx, val, lse = _make(5, 2051, 7, "bf16", pad=3, tail=tail)
+    up = torch.rand(5, device="cuda")
+
+    def padded(t):
+        t = t.detach()
+        room = t.new_zeros(t.shape[0], *[n + 5 for n in t.shape[1:]])
+        view = room[tuple(slice(0, n) for n in t.shape)]
+        return view.copy_(t)
+
+    def gradient(hooks):
+        y = x.clone().requires_grad_()
+        i, v, l = idx.clone(), val.clone(), lse.clone() if tail else None
+        if not hooks:
+            pd.distill_topk(y, i, v, 2.0, l).backward(up)
+            return y.grad
+        with torch.autograd.graph.saved_tensors_hooks(padded, lambda t: t):
+            loss = pd.distill_topk(y, i, v, 2.0, l)
+        with torch.no_grad():
+            y.zero_(), v.zero_(), i.zero_()
+            if tail:
+                l.zero_()
+        loss.backward(up)
+        return y.grad
+
+    assert torch.equal(gradient(False), gradient(True))
+
+
+def test_checkpointed_loss():
+    x, idx, val, _ = _make(6, 3001, 9, "f32")
+    head = torch.nn.Linear(16, 3001, device="cuda")
+    h = torch.randn(6, 16, device="cuda")
+
+    def loss(h):
+        return pd.distill_topk(head(h), idx, val, 1.5)
+
+    want = torch.autograd.grad(loss(h).sum(), head.weight)[0]
+    kept = checkpoint(loss, h.clone().requires_grad_(), use_reentrant=False)
+    junk = [torch.full((6, 3001), 7.0, device="cuda") for _ in range(4)]  # takes the memory of what was not kept
+    assert torch.equal(torch.autograd.grad(kept.sum(), head.weight)[0], want), junk
 
 
 def test_captured_step():
