@@ -209,6 +209,11 @@ int vec_bytes(const pesti_beam_rows& s, int W) {
   return bits % 4 == 0 ? 4 : 1;
 }
 
+// Tiles of a group.
+__int128 reorder_tiles(const pesti_beam_rows& s, int vec) {
+  return (__int128)((s.block_bytes / vec + REORDER_THREADS - 1) / REORDER_THREADS) * s.blocks;
+}
+
 int flush_reorder(ReorderArgs& a, long long& tiles, int vec, const int32_t* parent, int W, cudaStream_t st) {
   if (a.n == 0) return PESTI_OK;
   int rc;
@@ -333,6 +338,8 @@ int pesti_beam_reorder(const pesti_beam_rows* states, int64_t n_states, const in
     } else if (p < q + b && q < p + a) {
       return refuse("src and dst overlap");
     }
+    // refused before anything is launched
+    if (reorder_tiles(s, vec_bytes(s, (int)W)) * G > 0x7fffffff) return refuse("state too large");
   }
   if (G == 0 || n_states == 0) return PESTI_OK;
   // a state given twice would be moved twice
@@ -359,9 +366,8 @@ int pesti_beam_reorder(const pesti_beam_rows* states, int64_t n_states, const in
       const pesti_beam_rows& s = states[i];
       if (s.blocks == 0 || s.block_bytes == 0 || vec_bytes(s, (int)W) != vec) continue;
       const long long vecs = s.block_bytes / vec, per = (vecs + REORDER_THREADS - 1) / REORDER_THREADS;
-      const __int128 mine = (__int128)per * s.blocks * G;
-      if (mine > 0x7fffffff) return refuse("state too large");
-      if (a.n == REORDER_MAX || tiles + (long long)mine > 0x7fffffffLL) {
+      const long long mine = per * s.blocks * G;
+      if (a.n == REORDER_MAX || tiles + mine > 0x7fffffffLL) {
         rc = flush_reorder(a, tiles, vec, d_parent, (int)W, st);
         if (rc) return rc;
       }
@@ -369,7 +375,7 @@ int pesti_beam_reorder(const pesti_beam_rows* states, int64_t n_states, const in
                                 s.dst_row_stride,   s.src_block_stride, s.dst_block_stride,
                                 vecs,               per,                s.blocks,
                                 tiles};
-      tiles += (long long)mine;
+      tiles += mine;
     }
     rc = flush_reorder(a, tiles, vec, d_parent, (int)W, st);
     if (rc) return rc;

@@ -105,6 +105,13 @@ def test_reorder_refusals(lib, rows, more):
     assert lib.pesti_last_error()
 
 
+def test_reorder_refuses_before_it_launches(lib):
+    # a state of more tiles than a grid has, behind one that could be moved
+    large = _rows(src=2 * P, dst=2 * P, src_row=1, dst_row=1, src_blk=8, dst_blk=8, blocks=1 << 31, nbytes=1)
+    assert _reorder(lib, [_rows(), large]) == BAD
+    assert "too large" in lib.pesti_last_error().decode()
+
+
 def test_reorder_of_nothing(lib):
     assert _reorder(lib, [], parent=None) == ps.PESTI_OK
     assert _reorder(lib, [_rows()], parent=None, G=0) == ps.PESTI_OK
