@@ -183,6 +183,8 @@ class BeamState:
         self.max_tokens, self.max_seq_len = int(max_tokens), int(max_seq_len)
         self.cap = max(1, min(self.max_tokens, self.max_seq_len))
         dev = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
+        if dev.type == "cuda" and dev.index is None:
+            dev = torch.device("cuda", torch.cuda.current_device())
         G, W, i32 = self.groups, self.beams, torch.int32
 
         def make(*shape, dtype=i32):

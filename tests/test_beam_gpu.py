@@ -220,6 +220,12 @@ def test_advance_without_stop_tokens_and_reset():
     assert torch.isneginf(st.cum[:, 1:]).all() and (st.cum[:, 0] == 0).all() and (st.parent == -1).all()
 
 
+@pytest.mark.parametrize("device", [0, "cuda", "cuda:0", torch.device("cuda")])
+def test_state_devices(device):
+    st = pb.BeamState(2, 3, 4, 8, device=device)
+    assert st.device == torch.device("cuda", 0) and st.active() == 2
+
+
 def _permuted(x, parent, W):
     n = x.shape[0]
     idx = [g * W + (p if 0 <= p < W else w) for g, line in enumerate(parent.tolist()) for w, p in enumerate(line)]
