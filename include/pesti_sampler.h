@@ -342,6 +342,8 @@ int pesti_llama_chain_batch(pesti_sampler* s, const void* d_logits, pesti_dtype 
  *  - d_ws: device scratch of pesti_beam_select_workspace(...) bytes, 256-byte
  *    aligned, any contents.  Calls whose GPU work may overlap need scratch of
  *    their own.
+ * Outputs overlap neither inputs nor one another (d_score may be d_cum if
+ * K == W: a group's scores are read before they are written).
  * With W = 1 and no d_cum it gives the K largest log-probabilities of each row
  * (a distillation teacher's list).
  */
@@ -456,8 +458,9 @@ int pesti_beam_reorder(const pesti_beam_rows* states, int64_t n_states, const in
  *
  * pesti_distill_topk: d_loss [N] f32.  With d_grad ([N, grad_ld], the logits'
  * type) it writes the gradient of the losses' sum as well; d_grad may be
- * d_logits itself (with grad_ld == ld).  With d_stats ([N, PESTI_DISTILL_STATS(k)] f64) it keeps what
- * pesti_distill_topk_backward needs.  d_ws: device scratch of
+ * d_logits itself (with grad_ld == ld).  With d_stats ([N,
+ * PESTI_DISTILL_STATS(k)] f64) it keeps what pesti_distill_topk_backward needs.
+ * Other outputs overlap neither inputs nor one another.  d_ws: device scratch of
  * pesti_distill_topk_workspace(...) bytes, 256-byte aligned, any contents; calls
  * whose GPU work may overlap need scratch of their own.
  * pesti_distill_topk_backward: the gradient of sum_n d_up[n*up_stride] *

@@ -35,6 +35,7 @@ int common(DistillArgs& a, const void* d_logits, pesti_dtype dtype, int64_t N, i
   if (N == 0) return PESTI_OK;
   if (!d_logits || !d_idx || !d_val) return refuse("null logits or teacher list");
   if ((uintptr_t)d_logits % esize(dtype)) return refuse("logits are not aligned to their type");
+  if ((uintptr_t)d_val % esize(val_dtype)) return refuse("teacher values are not aligned to their type");
   a = DistillArgs{};
   a.logits = d_logits;
   a.ld = ld;

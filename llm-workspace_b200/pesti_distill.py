@@ -144,6 +144,8 @@ def distill_topk_grad(logits, idx, val, temperature: float = 1.0, teacher_lse=No
                                                ws.data_ptr(), need, st)
         if rc:
             _check(rc)
+        if grad is not None and not grad.is_inference():
+            torch.autograd.graph.increment_version(grad)  # a backward pass that needs its old values is refused
         return loss, to
 
     return _launch(dev, stream, call)

@@ -126,6 +126,7 @@ COMMON = [
     (dict(val_ld=-8), "negative stride"), (dict(T=0.0), "temperature"), (dict(T=float("nan")), "temperature"),
     (dict(T=-1.0), "temperature"), (dict(T=float("inf")), "temperature"), (dict(T=1e-4), "temperature"),
     (dict(logits=None), "null"), (dict(idx=None), "null"), (dict(val=None), "null"), (dict(logits=P + 1), "not aligned"),
+    (dict(val=P + 2), "teacher values are not aligned"), (dict(vtype=ps.PESTI_BF16, val=P + 1), "teacher values are not"),
 ]
 
 

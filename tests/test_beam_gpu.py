@@ -220,6 +220,16 @@ def test_advance_without_stop_tokens_and_reset():
     assert torch.isneginf(st.cum[:, 1:]).all() and (st.cum[:, 0] == 0).all() and (st.parent == -1).all()
 
 
+@pytest.mark.parametrize("G,W", [(3, 1), (5, 8), (2, 40)])
+def test_select_scores_in_place(G, W):
+    x = _logits(G * W, 5003, "bf16", seed=4)
+    cum = -torch.rand(G, W, device="cuda") * 3
+    want = pb.beam_select(x, W, W, cum=cum.clone())
+    token, parent = torch.empty(2, G, W, dtype=torch.int32, device="cuda")
+    got = pb.beam_select(x, W, W, cum=cum, out=(cum, token, parent))
+    assert got[0] is cum and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 @pytest.mark.parametrize("device", [0, "cuda", "cuda:0", torch.device("cuda")])
 def test_state_devices(device):
     st = pb.BeamState(2, 3, 4, 8, device=device)

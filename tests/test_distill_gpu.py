@@ -326,6 +326,15 @@ def test_autograd_through_a_head():
         assert not pd.distill_topk(logits, idx, val).requires_grad
 
 
+def test_overwritten_logits_have_no_backward():
+    x, idx, val, _ = _make(4, 500, 5, "f32")
+    y = x.clone().requires_grad_()
+    loss = pd.distill_topk(y, idx, val)
+    pd.distill_topk_grad(y, idx, val, grad=y.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.sum().backward()
+
+
 @pytest.mark.parametrize("tail", [False, True])
 def test_saved_tensors_may_move(tail):
     # hooks hand other tensors to the backward call: copies whose rows are padded, the originals overwritten
