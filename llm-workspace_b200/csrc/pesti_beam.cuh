@@ -71,6 +71,11 @@ __device__ __forceinline__ bool beam_running(const float* cum, long long row) {
   return cum == nullptr || cum[row] > neg_inf();
 }
 
+// A warp a unit, bound by HBM where rows are many: 512 rows of 152064 f32 take
+// 47.4 us, 6.6 TB/s; 256 rows of 128256 bf16, whose elements need twice the
+// instructions a byte, 15.6 us, 4.2 TB/s (issue slots half used, 29 warps an SM);
+// 4 rows of 32000 f32 4.4 us, a load's latency and the launch.  Blocks are
+// small so that a finished warp's place is taken again soon.
 template <typename T>
 __global__ void __launch_bounds__(SCAN_WARPS * 32) beam_scan_kernel(const T* __restrict__ logits, long long ld,
                                                                     long long V, int W, long long units,
@@ -658,6 +663,10 @@ __device__ __forceinline__ P* in_block(P* p, uint32_t rank) {
   return (P*)r;
 }
 
+// Bound by latency: dependent reads (keys, segments), the steps between them
+// and their first instruction fetches.  9.3 us for one group of 4 beams x 32000
+// f32, 13.4 us for 32 groups of 8 x 128256 bf16, 13.0 us for 64 groups of 8 x
+// 152064 f32, a few of which the scan's end hides.
 template <typename T, int TW, bool WIDE>
 __global__ void __launch_bounds__(PICK_WARPS * 32) beam_pick_kernel(
     const T* __restrict__ logits, long long ld, long long V, const __grid_constant__ PickPlan pl, const float* cum,
@@ -868,7 +877,9 @@ constexpr int ADV_THREADS = 128;
 // lanes: which candidates end, which go on, and which slots of the pool they
 // take.  The block then moves the token histories: a thread owns a column of
 // all beams, so rows exchange places without another buffer.  A step's time is
-// three dependent reads and the ranks, some 60 cycles each.
+// three dependent reads and the ranks, some 60 cycles each: 4.6 us for 4 beams
+// and 8 candidates, 9.2 us for 128 groups of 8 and 16 (steps of a captured
+// search; the bytes moved are some KB a group).
 __global__ void __launch_bounds__(ADV_THREADS) beam_advance_kernel(const float* __restrict__ score,
                                                                    const int32_t* __restrict__ token,
                                                                    const int32_t* __restrict__ parent, int W, int K,
@@ -1076,6 +1087,9 @@ struct ReorderArgs {
 // A thread owns one vector position of all beams of a group: it reads every
 // beam's new value before it writes one, so source and destination may be the
 // same memory.  In place, beams that stay where they are are not touched.
+// Bound by HBM: 32 caches of 64 beams x 4 heads x 1100 x 128 bf16 take 539 us
+// out of place (the rows written and the distinct parents read: 7.1 TB/s), two
+// of them 36 us.
 template <typename Vec, int WB>
 __global__ void __launch_bounds__(REORDER_THREADS) beam_reorder_kernel(const __grid_constant__ ReorderArgs a,
                                                                        const int32_t* __restrict__ parent, int W) {

@@ -416,7 +416,7 @@ __device__ __forceinline__ void join_row(const DistillArgs& a, long long n, int 
 
 // Stores a unit's gradient vectors whose elements start d (1 to VE - 1) places before a 16-byte boundary of the
 // gradient: each lane writes the vector that its own and the next lane's make up, the unit's ragged ends go one by one.
-// (461 rows of 256000 bf16 whose logits are padded by one: 333 us with single elements.)
+// (Loss and gradient of 461 rows of 256000 bf16 whose logits are padded by one: 134 us, 333 us with single elements.)
 template <typename T>
 __device__ __forceinline__ void store_shifted(T* to, const uint4 (&g)[UNIT_VECS], int d, int lane) {
   constexpr int VE = Elem<T>::VE;
@@ -531,6 +531,7 @@ __global__ void __launch_bounds__(UNIT_WARPS * 32, 10) distill_scan_kernel(const
 
 constexpr int JOIN_WARPS = 2;  // warps of a block, a row each
 
+// Bound by latency (a row's units, then 64-bit logarithms): 8.4 us for 2048 rows of 152064 bf16, 7 us for 1024 of 128256.
 template <typename T>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) distill_join_kernel(const __grid_constant__ DistillArgs a) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
