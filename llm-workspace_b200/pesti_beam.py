@@ -37,10 +37,13 @@ def _need(cond: bool, msg: str) -> None:
 
 
 def _rows_dtype(logits) -> int:
-    _need(logits.dim() == 2, "logits must be [rows, V]")
-    dtype = _DTYPES.get(logits.dtype)
-    _need(dtype is not None, "logits must be float32, bfloat16 or float16")
-    _need(logits.shape[1] <= 1 or logits.stride(1) == 1, "logits rows must be contiguous")
+    dtype, strides = _DTYPES.get(logits.dtype), logits.stride()
+    if len(strides) != 2:
+        raise ValueError("logits must be [rows, V]")
+    if dtype is None:
+        raise ValueError("logits must be float32, bfloat16 or float16")
+    if strides[1] != 1 and logits.shape[1] > 1:
+        raise ValueError("logits rows must be contiguous")
     return dtype
 
 

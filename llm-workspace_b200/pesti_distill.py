@@ -32,31 +32,30 @@ def _workspace(dtype: int, N: int, V: int, k: int) -> int:
 
 def _lists(logits, idx, val, temperature, teacher_lse, weight):
     """Checks the arguments and returns them in the C call's order."""
-    dtype = _rows_dtype(logits)
-    N, V = logits.shape
-    dev = logits.device
-    _need(V >= 1, "V must be at least 1")
-    for t, name in ((idx, "idx"), (val, "val")):
-        if t.device != dev:
-            raise ValueError(f"{name} must be on the logits' device")
-        if t.dim() != 2 or t.shape[0] != N or (t.shape[1] > 1 and t.stride(1) != 1):
-            raise ValueError(f"{name} must be [N, k] with contiguous rows")
-    if idx.shape != val.shape:
+    dtype, vtype = _rows_dtype(logits), _DTYPES.get(val.dtype)
+    (N, V), dev, shape = logits.shape, logits.device, idx.shape
+    (ld, _), to_idx, to_val = logits.stride(), idx.stride(), val.stride()
+    if V < 1:
+        raise ValueError("V must be at least 1")
+    if idx.device != dev or val.device != dev:
+        raise ValueError("idx and val must be on the logits' device")
+    if shape != val.shape:
         raise ValueError("idx and val must have the same shape")
-    k = idx.shape[1]
+    if len(shape) != 2 or shape[0] != N or (shape[1] > 1 and (to_idx[1] != 1 or to_val[1] != 1)):
+        raise ValueError("idx and val must be [N, k] with contiguous rows")
+    k = shape[1]
     if not 1 <= k <= MAX_TOP:
         raise ValueError(f"k must be 1 to {MAX_TOP}")
     if idx.dtype != torch.int32:
         raise ValueError("idx must be int32")
-    vtype = _DTYPES.get(val.dtype)
     if vtype is None:
         raise ValueError("val must be float32, bfloat16 or float16")
     for t, name in ((teacher_lse, "teacher_lse"), (weight, "weight")):
         if t is not None and not (t.device == dev and t.dtype == torch.float32 and t.shape == (N,)
                                   and t.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous [N] float32 tensor on the logits' device")
-    return (logits.data_ptr(), dtype, N, V, _row_stride(logits), idx.data_ptr(), idx.stride(0), val.data_ptr(), vtype,
-            val.stride(0), k, _ptr(teacher_lse), _ptr(weight), float(temperature))
+    return (logits.data_ptr(), dtype, N, V, ld if N > 1 else max(ld, V), idx.data_ptr(), to_idx[0], val.data_ptr(),
+            vtype, to_val[0], k, _ptr(teacher_lse), _ptr(weight), float(temperature))
 
 
 class _DistillTopk(torch.autograd.Function):
