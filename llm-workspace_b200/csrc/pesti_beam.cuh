@@ -783,11 +783,10 @@ __global__ void __launch_bounds__(PICK_WARPS * 32) beam_pick_kernel(
       hi = __reduce_or_sync(FULL, hi);
       // a run that leaves the ranked part: every row.  The blocks that stayed are told.
       flagged = open && total > have ? ~0ull : ((unsigned long long)hi << 32) | lo;
-      for (uint32_t r = 1; r < parts; ++r) {
-        if (lane == 0) *in_block(&sh.flagged, r) = flagged;
-        if (flagged)
+      if (lane > 0 && lane < parts) *in_block(&sh.flagged, lane) = flagged;
+      if (flagged)
+        for (uint32_t r = 1; r < parts; ++r)
           for (int w = lane; w < W; w += 32) *in_block(&sh.ref[w], r) = sh.ref[w];
-      }
       if (lane == 0) sh.flagged = flagged;
     }
   }
