@@ -13,7 +13,8 @@ device, and the reordering of per-beam states.
 With S stop tokens, (1 + S) * beams candidates always leave enough live beams.
 Every call runs the CUDA kernels of libpesti_sampler.so on the tensors' device
 and the current stream (or `stream`, a cudaStream_t); there is no CPU path.
-No call synchronises, except hypotheses() and active(), which read back.
+No call synchronises, except hypotheses() and active(), which read back on the
+current stream.
 """
 from __future__ import annotations
 
@@ -274,10 +275,6 @@ def _layout(shape, strides):
         blocks *= shape[j]
         at = strides[j] * shape[j]
     return blocks, run, step
-
-
-def _row_blocks(t):
-    return _layout(t.shape, t.stride())
 
 
 @functools.lru_cache(maxsize=1024)

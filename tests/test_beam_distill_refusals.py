@@ -205,12 +205,14 @@ def test_python_checks():
     (lambda: torch.zeros(6, 3, 8)[:, ::2], (2, 8, 16)),
 ])
 def test_row_blocks(make, want):
-    assert pb._row_blocks(make()) == want
+    t = make()
+    assert pb._layout(t.shape, t.stride()) == want
 
 
 def test_row_blocks_refuses_two_strides():
     with pytest.raises(ValueError):
-        pb._row_blocks(torch.zeros(6, 4, 5, 8)[:, :3, :4, :2])
+        t = torch.zeros(6, 4, 5, 8)[:, :3, :4, :2]
+        pb._layout(t.shape, t.stride())
 
 
 def test_oracle_against_a_direct_search():
