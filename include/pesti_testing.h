@@ -44,6 +44,20 @@ int pesti_testing_set_cluster(int mode);
  * as exact): the classification's cheap exp assumes it is below
  * PESTI_EX2_APPROX_RELERR. */
 int pesti_test_ex2_approx_max_relerr(double* out);
+
+/* How pesti_beam_select lays its second kernel out for these sizes on a device
+ * of `sms` SMs (computed on the host): a group has `blocks` blocks of `teams`
+ * teams of `team_warps` warps; a row's `segments` segment maxima become `keys`
+ * keys of `run` segments each.  Team t's shared memory begins at byte team_at +
+ * t * team_stride, its keys and its histogram (which is read 16 bytes at a
+ * time) keys_at and hist_at bytes behind that; `bytes` of at most `most_bytes`
+ * in all. */
+typedef struct {
+  int64_t segments, team_warps, teams, blocks, stay, run, keys;
+  int64_t team_at, team_stride, keys_at, hist_at, bytes, most_bytes;
+} pesti_testing_plan;
+int pesti_testing_beam_plan(pesti_dtype dtype, int64_t G, int64_t W, int64_t V, int64_t K, int sms,
+                            pesti_testing_plan* plan);
 #ifdef __cplusplus
 }
 #endif

@@ -8,6 +8,7 @@
 #include <vector>
 
 #include "../../include/pesti_sampler.h"
+#include "../../include/pesti_testing.h"
 #include "pesti_beam.cuh"
 #include "pesti_error.h"
 
@@ -103,31 +104,43 @@ void pick_shape(PickPlan& pl, int tw, long long* c) {
   pl.teams = std::min(pl.rows, most);
 }
 
+// Blocks of a group, and a block's dynamic shared memory.
+struct PickLaunch {
+  long long blocks, bytes;
+};
+
+// The plan for teams of `tw` warps; W, K and units are set.
+PickLaunch plan_pick(PickPlan& pl, int tw) {
+  PickLaunch to;
+  pick_shape(pl, tw, &to.blocks);
+  // A list takes what one round of a team's segments appends to a pruned one.
+  // Longer rows have keys of runs of segments (empty ones at the end, so that
+  // their number is a multiple of 4: the histogram behind them is read 16 bytes
+  // at a time).
+  const long long nseg = pl.units * UNIT_VECS, lists = list_bytes(pl.W, pl.K);
+  pl.cap = RANK_CAP + tw * 256;
+  const long long most = ((kPickSmem - lists) / pl.teams / 4 - (2 * pl.cap + TEAM_WORDS + 4)) / 4 * 4;
+  pl.run = (int)((nseg + most - 1) / most);
+  pl.nkeys = (int)(((nseg + pl.run - 1) / pl.run + 3) / 4 * 4);
+  to.bytes = lists + std::max(pl.teams * team_bytes(pl.nkeys, pl.cap), lists);
+  return to;
+}
+
 template <typename T, int TW>
 int launch_pick(const void* logits, long long G, long long V, long long ld, PickPlan pl, const float* cum,
                 const uint8_t* done, const BeamWs& ws, float* score, int32_t* token, int32_t* parent, float* lse,
                 cudaStream_t st) {
-  long long c;
-  pick_shape(pl, TW, &c);
-  // A list takes what one round of a team's segments appends to a pruned one.
-  // Longer rows have keys of runs of segments.
-  const long long nseg = pl.units * UNIT_VECS;
-  const long long lists = ((long long)pl.W * pl.K * 8 + 15) / 16 * 16;
-  pl.cap = RANK_CAP + TW * 256;
-  const long long most = (kPickSmem - lists) / pl.teams / 4 - (2 * pl.cap + TEAM_WORDS + 4);
-  pl.run = (int)((nseg + most - 1) / most);
-  pl.nkeys = (int)((nseg + pl.run - 1) / pl.run);
-  const long long body = std::max(pl.teams * team_bytes(pl.nkeys, pl.cap), lists);
+  const PickLaunch to = plan_pick(pl, TW);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(G * c));
+  cfg.gridDim = dim3((unsigned)(G * to.blocks));
   cfg.blockDim = dim3((unsigned)(pl.teams * (TW + 1) * 32));
-  cfg.dynamicSmemBytes = (size_t)(lists + body);
+  cfg.dynamicSmemBytes = (size_t)to.bytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)c;
+  attr[1].val.clusterDim.x = (unsigned)to.blocks;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
@@ -136,6 +149,24 @@ int launch_pick(const void* logits, long long G, long long V, long long ld, Pick
       &cfg, pl.run == 1 ? beam_pick_kernel<T, TW, false> : beam_pick_kernel<T, TW, true>, (const T*)logits, ld, V,
       (const PickPlan)pl, cum, done, ws, score, token, parent, lse);
   return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, "beam_pick_kernel launch");
+}
+
+// The widest teams whose blocks all run at once (16 warps of 114 registers
+// fill an SM): 32 groups of 8 beams take 11.5 us with teams of 7, 16 us with
+// teams of 3; 64 groups 21.5 us with teams of 7, 13 us with teams of 3.  Long
+// lists are too much for teams of one warp (1024 rows of 32000, K 64: 73 us,
+// 47 us with teams of 3).  Where teams of 7 fit, the blocks are not wanted
+// for other groups and stay for rows to add up again: that costs every call
+// 0.2 us, and brings two rows of 152064 f32 from 185 to 39 us.
+int team_warps(PickPlan& pl, long long G, int sms) {
+  auto at_once = [&](int tw) {
+    long long c;
+    PickPlan q = pl;
+    pick_shape(q, tw, &c);
+    return G * c * q.teams * (tw + 1) <= (long long)sms * PICK_WARPS;
+  };
+  pl.stay = at_once(7);
+  return pl.stay ? 7 : at_once(3) || pl.K > 32 ? 3 : 1;
 }
 
 template <typename T>
@@ -154,23 +185,11 @@ int run_select(const void* logits, long long G, long long W, long long V, long l
   pl.W = (int)W;
   pl.K = K;
   pl.units = units;
-  // The widest teams whose blocks all run at once (16 warps of 114 registers
-  // fill an SM): 32 groups of 8 beams take 11.5 us with teams of 7, 16 us with
-  // teams of 3; 64 groups 21.5 us with teams of 7, 13 us with teams of 3.  Long
-  // lists are too much for teams of one warp (1024 rows of 32000, K 64: 73 us,
-  // 47 us with teams of 3).  Where teams of 7 fit, the blocks are not wanted
-  // for other groups and stay for rows to add up again: that costs every call
-  // 0.2 us, and brings two rows of 152064 f32 from 185 to 39 us.
-  auto at_once = [&](int tw) {
-    long long c;
-    PickPlan q = pl;
-    pick_shape(q, tw, &c);
-    return G * c * q.teams * (tw + 1) <= (long long)sms * PICK_WARPS;
-  };
-  pl.stay = at_once(7);
-  if (at_once(7)) return launch_pick<T, 7>(logits, G, V, ld, pl, cum, done, ws, score, token, parent, lse, st);
-  if (at_once(3) || K > 32) return launch_pick<T, 3>(logits, G, V, ld, pl, cum, done, ws, score, token, parent, lse, st);
-  return launch_pick<T, 1>(logits, G, V, ld, pl, cum, done, ws, score, token, parent, lse, st);
+  switch (team_warps(pl, G, sms)) {
+    case 7: return launch_pick<T, 7>(logits, G, V, ld, pl, cum, done, ws, score, token, parent, lse, st);
+    case 3: return launch_pick<T, 3>(logits, G, V, ld, pl, cum, done, ws, score, token, parent, lse, st);
+    default: return launch_pick<T, 1>(logits, G, V, ld, pl, cum, done, ws, score, token, parent, lse, st);
+  }
 }
 
 int check_state(const pesti_beam_state* s, int64_t G, int64_t W) {
@@ -270,6 +289,33 @@ int pesti_beam_select(const void* d_logits, pesti_dtype dtype, int64_t G, int64_
                               units, st);
   return run_select<float>(d_logits, G, W, V, ld, d_cum, d_done, (int)K, d_score, d_token, d_parent, d_lse, ws, units,
                            st);
+}
+
+int pesti_testing_beam_plan(pesti_dtype dtype, int64_t G, int64_t W, int64_t V, int64_t K, int sms,
+                            pesti_testing_plan* plan) {
+  const int rc = check_sizes(dtype, G, W, V, K);
+  if (rc) return rc;
+  if (!plan) return refuse("null plan");
+  PickPlan pl{};
+  pl.W = (int)W;
+  pl.K = (int)K;
+  pl.units = units_of(dtype, V);
+  const int tw = team_warps(pl, G, sms);
+  const PickLaunch to = plan_pick(pl, tw);
+  plan->segments = pl.units * UNIT_VECS;
+  plan->team_warps = tw;
+  plan->teams = pl.teams;
+  plan->blocks = to.blocks;
+  plan->stay = pl.stay;
+  plan->run = pl.run;
+  plan->keys = pl.nkeys;
+  plan->team_at = list_bytes(pl.W, pl.K);
+  plan->team_stride = team_bytes(pl.nkeys, pl.cap);
+  plan->keys_at = keys_offset(pl.cap);
+  plan->hist_at = hist_offset(pl.nkeys, pl.cap);
+  plan->bytes = to.bytes;
+  plan->most_bytes = kPickSmem;
+  return PESTI_OK;
 }
 
 int pesti_beam_reset(const pesti_beam_state* state, int64_t G, int64_t W, void* stream) {

@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32) beam_scan_kernel(const T* __r
 // sums.  A team's arrays lie in dynamic shared memory behind the x and idx of
 // the group's lists; the merge's scores take their place.
 struct PickPlan {
-  int W, K, rows, teams, nkeys, run, cap;  // run: segments of a key; cap: entries of a team's list
+  int W, K, rows, teams, nkeys, run, cap;  // nkeys: a multiple of 4; run: segments of a key; cap: entries of a team's list
   int stay;                                // the cluster's blocks help to add up rows again
   long long units;
 };
@@ -173,8 +173,14 @@ enum { TM_NSEL = 0, TM_NLIST = 1, TM_OVER = 2, TM_T = 3, TM_MAX = 4, TM_MIN = 5,
 
 constexpr int TEAM_WORDS = BINS + MAX_SEL + 32;
 
+// The block's dynamic shared memory: the lists, then a team's list, keys, and words (the histogram first) for every team.
+__host__ __device__ __forceinline__ long long list_bytes(int W, int K) { return ((long long)W * K * 8 + 15) / 16 * 16; }
+__host__ __device__ __forceinline__ long long keys_offset(int cap) { return (long long)cap * 8; }
+__host__ __device__ __forceinline__ long long hist_offset(int nkeys, int cap) {
+  return keys_offset(cap) + (long long)nkeys * 4;
+}
 __host__ __device__ __forceinline__ long long team_bytes(int nkeys, int cap) {
-  return ((long long)cap * 8 + (long long)(nkeys + TEAM_WORDS) * 4 + 15) / 16 * 16;
+  return (hist_offset(nkeys, cap) + TEAM_WORDS * 4 + 15) / 16 * 16;
 }
 
 template <int TW>
@@ -682,7 +688,7 @@ __global__ void __launch_bounds__(PICK_WARPS * 32) beam_pick_kernel(
   const long long g = blockIdx.x / csize, row0 = g * W;
   float* xs = (float*)dyn;
   int32_t* ids = (int32_t*)(xs + W * K);
-  char* teams = dyn + ((long long)W * K * 8 + 15) / 16 * 16;
+  char* teams = dyn + list_bytes(W, K);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (csize > 1) asm volatile("barrier.cluster.wait;" ::: "memory");
 
@@ -694,9 +700,10 @@ __global__ void __launch_bounds__(PICK_WARPS * 32) beam_pick_kernel(
     t.id = wid / TW;
     t.tid = tid - t.id * TW * 32;
     t.turn = 0;
-    t.list = (unsigned long long*)(teams + t.id * team_bytes(pl.nkeys, pl.cap));
-    t.keys = (uint32_t*)(t.list + pl.cap);
-    t.hist = (int*)(t.keys + pl.nkeys);
+    char* const mine = teams + t.id * team_bytes(pl.nkeys, pl.cap);
+    t.list = (unsigned long long*)mine;
+    t.keys = (uint32_t*)(mine + keys_offset(pl.cap));
+    t.hist = (int*)(mine + hist_offset(pl.nkeys, pl.cap));
     t.sel = t.hist + BINS;
     t.word = t.sel + MAX_SEL;
     float* const first_xs = csize > 1 ? in_block(xs, 0) : xs;

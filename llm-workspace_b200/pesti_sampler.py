@@ -136,6 +136,8 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.pesti_beam_select_workspace.restype = i64
     lib.pesti_beam_select.argtypes = [vp, c_int, i64, i64, i64, i64, vp, vp, i64, vp, vp, vp, vp, vp, i64, vp]
     lib.pesti_beam_select.restype = c_int
+    lib.pesti_testing_beam_plan.argtypes = [c_int, i64, i64, i64, i64, c_int, vp]
+    lib.pesti_testing_beam_plan.restype = c_int
     lib.pesti_beam_reset.argtypes = [vp, i64, i64, vp]
     lib.pesti_beam_reset.restype = c_int
     lib.pesti_beam_advance.argtypes = [vp, vp, vp, vp, i64, i64, i64, vp, i64, vp, vp]
