@@ -50,9 +50,9 @@ int common(DistillArgs& a, const void* d_logits, pesti_dtype dtype, int64_t N, i
   a.weight = d_weight;
   a.T = temperature;
   a.C = 1.4426950408889634074 / a.T;
-  // rounded down, so that c_lo >= 0 and -inf stays -inf in x*c + x*c_lo
+  // below C, so that c_lo > 0 and -inf stays -inf in x*c + x*c_lo (with c_lo = 0, as T = 1/ln 2 would have it, NaN)
   a.c = (float)a.C;
-  if ((double)a.c > a.C) a.c = std::nextafter(a.c, 0.0f);
+  if ((double)a.c >= a.C) a.c = std::nextafter(a.c, 0.0f);
   a.c_lo = (float)(a.C - (double)a.c);
   a.units = dtype == PESTI_F32 ? row_units<float>(V) : row_units<__half>(V);
   return PESTI_OK;

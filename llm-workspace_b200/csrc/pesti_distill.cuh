@@ -65,7 +65,7 @@ struct DistillArgs {
   const float* weight;
   double T;
   double C;       // log2(e) / T
-  float c, c_lo;  // C = c + c_lo, c_lo >= 0
+  float c, c_lo;  // C = c + c_lo, 0 < c_lo <= 2^-23 C
   float* loss;
   double* stats;  // [N][stats_of(k)], null when no gradient follows
   void* grad;
@@ -153,7 +153,7 @@ __device__ __forceinline__ void store_vec(T* grow, long long lo, long long V, bo
 }
 
 // 16-bit gradients leave x*c_lo out but for its value at m, which goes into A (near_factor): the rest,
-// |(x - m) c_lo| < 2^-24 |(x - m) C|, is far below their rounding.
+// |(x - m) c_lo| <= 2^-23 |(x - m) C|, is far below their rounding.
 template <typename T>
 __device__ __forceinline__ float near_factor(float A, float m, const DistillArgs& a) {
   return sizeof(T) == 2 && m > neg_inf() && !is_far(m, a.c) ? A * ex2(m * a.c_lo) : A;

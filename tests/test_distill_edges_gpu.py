@@ -1,0 +1,34 @@
+"""Distillation calls that the other tests pass by, against the 64-bit oracle
+(oracle/distill.py): temperatures whose log2(e)/T is an f32, lists without a
+probability whose tokens repeat, teachers that require a gradient.  Tolerances
+are test_distill_gpu.py's."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import pesti_distill as pd
+from test_distill_gpu import _compare, _make
+
+pytestmark = pytest.mark.gpu
+
+NEG = float("-inf")
+LOG2E = 1.4426950408889634
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("T", [1 / math.log(2), 2 / math.log(2), 0.5 / math.log(2), LOG2E / 1.25])
+def test_temperatures_of_round_bases(dtype, tail, T):
+    """The softmax to base 2 (4, the root of 2), over whole and ragged units, masked and not."""
+    assert float(np.float32(LOG2E / T)) == LOG2E / T
+    for V, pad in ((4096, 0), (3001, 1), (5, 0)):
+        x, idx, val, lse = _make(4, V, 4, dtype, pad=pad, tail=tail, T=T)
+        up = torch.tensor([1.0, -0.5, 2.0, 1.5]).cuda()
+        _compare(x, idx, val, T, lse, None, dtype, up)
+        unlisted = torch.ones(4, V, dtype=torch.bool).cuda().scatter_(1, idx.long(), False)
+        x[1][unlisted[1] & (torch.arange(V).cuda() % 3 == 0)] = NEG
+        x[2][unlisted[2]] = NEG
+        x[3] = NEG
+        _compare(x, idx, val, T, lse, None, dtype, up)
