@@ -282,8 +282,9 @@ __device__ __forceinline__ void list_row(const DistillArgs& a, long long n, int3
     const double y = __shfl_xor_sync(FULL, mt, o);
     mt = mt != mt ? mt : !(y <= mt) ? y : mt;
   }
-  // q = exp(t - norm): of the whole vocabulary's sum, or first of the largest; listed tokens' terms, each token once
-  double norm = tail ? (double)a.teacher_lse[n] : mt != -inf ? mt : 0.0;
+  // q = exp(t - ref): of the whole vocabulary's sum, or first of the largest; listed tokens' terms, each token once
+  const double ref = tail ? (double)a.teacher_lse[n] : mt != -inf ? mt : 0.0;
+  double norm = ref;
   double Q = 0.0, terms = 0.0, l = 0.0;
   bool twice = false;  // a token is listed more than once
   for (int j0 = 0; j0 < a.k; j0 += 32) {
@@ -304,7 +305,7 @@ __device__ __forceinline__ void list_row(const DistillArgs& a, long long n, int3
       double q = 0.0, e = 0.0;
       if (id >= 0) {
         const float x = Elem<T>::load(row, id);
-        const double logq = teacher_value(a, n, j) * invT - norm;
+        const double logq = teacher_value(a, n, j) * invT - ref;
         q = exp(logq);
         e = exact_term(x, mx, a);
         if (q != 0.0) l += q * (logq - (x == neg_inf() ? -inf : ((double)x - (double)mx) * invT));
@@ -341,7 +342,7 @@ __device__ __forceinline__ void list_row(const DistillArgs& a, long long n, int3
           // every entry of a token gets the token's sum
           s = 0.0;
           for (int o = 0; o < a.k; ++o)
-            if (idx[o] == id) s += exp(teacher_value(a, n, o) * invT - (tail ? norm : mt));
+            if (idx[o] == id) s += exp(teacher_value(a, n, o) * invT - ref);
         }
         out[LI_ENTRIES + a.k + j] = s * per;
       }

@@ -32,3 +32,21 @@ def test_temperatures_of_round_bases(dtype, tail, T):
         x[2][unlisted[2]] = NEG
         x[3] = NEG
         _compare(x, idx, val, T, lse, None, dtype, up)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("weighted", [False, True])
+def test_equal_tokens_without_probability(dtype, tail, weighted):
+    """Rows padded as token 0 with -inf, wholly and behind real entries."""
+    x, idx, val, lse = _make(5, 3001, 12, dtype, tail=tail)
+    idx[0], val[0] = 0, NEG
+    idx[1, 5:], val[1, 5:] = 0, NEG
+    idx[2, 3], val[2] = idx[2, 9], NEG
+    idx[3, :6], val[3] = -1, NEG
+    idx[3, 6:] = 2999
+    weight = torch.tensor([0.5, 1.0, 2.0, 0.25, 0.0]).cuda() if weighted else None
+    _, grad = _compare(x, idx, val, 1.0, lse, weight, dtype)
+    assert torch.isfinite(grad).all()
+    if not tail:
+        assert not grad[0].any() and not grad[2].any() and not grad[3].any()
