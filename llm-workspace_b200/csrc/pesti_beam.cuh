@@ -125,22 +125,22 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32) beam_scan_kernel(const T* __r
     S = warp_reduce_add(b.x + b.y);
   }
   if (far || S != S) {
-    // the number of maxima, or a sum that leaves NaN out
-    S = 0.f;
+    // the number of maxima, or a sum that leaves NaN out (one chain of 32 or 64 terms a lane, so in 64 bits)
+    double s = 0.0;
 #pragma unroll 1
     for (int i = 0; i < UNIT_VECS; ++i) {
       const uint4 w = i == 0 ? v[0] : i == 1 ? v[1] : i == 2 ? v[2] : i == 3 ? v[3] : i == 4 ? v[4] : i == 5 ? v[5] : i == 6 ? v[6] : v[7];
       for (int q = 0; q < Elem<T>::PAIRS; ++q) {
         const float2 x = Elem<T>::pair(w, q);
         if (far) {
-          S += (x.x == m ? 1.f : 0.f) + (x.y == m ? 1.f : 0.f);
+          s += (x.x == m ? 1.0 : 0.0) + (x.y == m ? 1.0 : 0.0);
         } else {
-          if (x.x == x.x) S += ex2(fmaf(x.x, LOG2E_F, -R));
-          if (x.y == x.y) S += ex2(fmaf(x.y, LOG2E_F, -R));
+          if (x.x == x.x) s += (double)ex2(fmaf(x.x, LOG2E_F, -R));
+          if (x.y == x.y) s += (double)ex2(fmaf(x.y, LOG2E_F, -R));
         }
       }
     }
-    S = warp_reduce_add(S);
+    S = (float)warp_reduce_add(s);
   }
   if (lane < UNIT_VECS) {
     const bool none = !(mine > neg_inf());

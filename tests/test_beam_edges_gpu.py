@@ -1,0 +1,28 @@
+"""Beam search calls that the other tests pass by, against the 64-bit oracle
+(oracle/beam.py).  Tolerances are test_beam_gpu.py's unless stated."""
+import numpy as np
+import pytest
+import torch
+
+import beam as OB
+import pesti_beam as pb
+from test_beam_gpu import DT, NEG, _check, _drive, _logits
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_log_sums_of_rows_with_nan(dtype):
+    """A NaN in a row leaves its log sum as close as the kernel states, 1.95e-6,
+    and rounded once to f32.  Every lane adds one term of 1 and terms just below
+    half an f32 step of it, each of which a running f32 sum loses."""
+    unit = 1024 if dtype == "f32" else 2048
+    x = torch.full((3, 2 * unit), -16.75, dtype=DT[dtype], device="cuda")
+    x[:, torch.arange(32) * (unit // 256)] = 0.0
+    x[1, unit - 1] = float("nan")
+    x[2, ::unit - 1] = float("nan")
+    lse = torch.empty(3, device="cuda")
+    pb.beam_select(x, 1, 4, lse=lse)
+    want = np.array([OB.row_logp(r)[1] for r in x.float().cpu().numpy()])
+    off = np.abs(lse.cpu().numpy().astype(np.float64) - want)
+    assert np.all(off <= 1.95e-6 + np.abs(want) * 2.0 ** -24), off
