@@ -557,8 +557,8 @@ __device__ __forceinline__ double key_value64(unsigned long long k) {
 }
 
 // Ranks the candidates of the group's lists; `sorted` gets the positions
-// w * K + r of the first `ranked` (K at least, if there are as many).  Returns
-// the number of candidates.
+// w * K + r of the first min(ranked, RANK_CAP) (K at least, if there are as
+// many).  Returns the number of candidates.
 __device__ __forceinline__ int rank_candidates(PickShared& sh, const float* xs, unsigned long long* score, int W, int K) {
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, warps = blockDim.x >> 5;
   int total = 0;
@@ -656,7 +656,6 @@ __device__ __forceinline__ int rank_candidates(PickShared& sh, const float* xs, 
     }
     if (rank < RANK_CAP) sh.sorted[rank] = j;
   }
-  if (threadIdx.x == 0) sh.ranked = RANK_CAP;
   __syncthreads();
   return total;
 }
@@ -762,7 +761,7 @@ __global__ void __launch_bounds__(PICK_WARPS * 32) beam_pick_kernel(
   unsigned long long flagged = 0ull;
   if (crank == 0) {
     total = rank_candidates(sh, xs, score, W, K);
-    const int have = sh.ranked;
+    const int have = min(sh.ranked, RANK_CAP);
     if (wid == 0) {
       // neighbours whose order the sums do not settle, up to the first clear gap behind the K-th place
       uint32_t lo = 0, hi = 0;

@@ -26,3 +26,13 @@ def test_log_sums_of_rows_with_nan(dtype):
     want = np.array([OB.row_logp(r)[1] for r in x.float().cpu().numpy()])
     off = np.abs(lse.cpu().numpy().astype(np.float64) - want)
     assert np.all(off <= 1.95e-6 + np.abs(want) * 2.0 ** -24), off
+
+
+@pytest.mark.parametrize("G,W,K", [(1, 4, 128), (100, 8, 64), (300, 64, 128)])
+def test_many_equal_candidates_many_times(G, W, K):
+    """Every candidate of many groups has the same score: lower beams and tokens first, in every call."""
+    x = torch.zeros(G * W, 1500, device="cuda")
+    token = torch.arange(K, dtype=torch.int32, device="cuda").expand(G, K)
+    for _ in range(20):
+        _, t, p = pb.beam_select(x, W, K)
+        assert torch.equal(t, token) and not p.any()
