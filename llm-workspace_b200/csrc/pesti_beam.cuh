@@ -524,6 +524,7 @@ struct PickShared {
   double pow2[256];  // 2^(i/256)
   double again[MAX_W][MAX_PICK_CLUSTER];
   int ranked;
+  unsigned long long next;  // the best score that is not among the ranked (0: none)
   unsigned long long flagged;
 };
 
@@ -578,7 +579,10 @@ __device__ __forceinline__ int rank_candidates(PickShared& sh, const float* xs, 
       rank = __reduce_add_sync(FULL, rank);
       if (lane == 0 && s != 0ull) sh.sorted[rank] = j;
     }
-    if (threadIdx.x == 0) sh.ranked = total;
+    if (threadIdx.x == 0) {
+      sh.ranked = total;
+      sh.next = 0ull;
+    }
     __syncthreads();
     return total;
   }
@@ -615,7 +619,16 @@ __device__ __forceinline__ int rank_candidates(PickShared& sh, const float* xs, 
     sh.part[lane + 32] = b;
     sh.part_at[lane] = at_a;
     sh.part_at[lane + 32] = at_b;
-    if (lane == 0) sh.ranked = have;
+    // the best of the lists' rests; where too many share one score, that score itself
+    auto rest = [&](int w, int n) { return w < W && n < sh.n[w] ? score[w * K + n] : 0ull; };
+    unsigned long long next = max(rest(lane, a), rest(lane + 32, b));
+    const uint32_t high = __reduce_max_sync(FULL, (uint32_t)(next >> 32));
+    const uint32_t low = __reduce_max_sync(FULL, (uint32_t)(next >> 32) == high ? (uint32_t)next : 0u);
+    next = ((unsigned long long)high << 32) | low;
+    if (lane == 0) {
+      sh.ranked = have;
+      sh.next = have <= RANK_CAP ? next : lo;
+    }
   }
   __syncthreads();
   const int have = sh.ranked;
@@ -766,18 +779,20 @@ __global__ void __launch_bounds__(PICK_WARPS * 32) beam_pick_kernel(
       // neighbours whose order the sums do not settle, up to the first clear gap behind the K-th place
       uint32_t lo = 0, hi = 0;
       bool open = W > 1;
-      for (int i0 = 0; open && i0 + 1 < have; i0 += 32) {
+      for (int i0 = 0; open && i0 < have; i0 += 32) {
         const int i = i0 + lane;
         bool near = false;
         int wa = 0, wb = 0;
-        if (i + 1 < have) {
-          const int ja = sh.sorted[i], jb = sh.sorted[i + 1];
-          const double a = key_value64(score[ja]), b = key_value64(score[jb]);
+        // the last of the ranked is compared with the best behind them
+        if (i + 1 < have || (i + 1 == have && sh.next != 0ull)) {
+          const bool last = i + 1 == have;
+          const int ja = sh.sorted[i], jb = last ? ja : sh.sorted[i + 1];
+          const double a = key_value64(score[ja]), b = key_value64(last ? sh.next : score[jb]);
           near = !(a - b > 2.0 * LSE_EPS) && a < (double)pos_inf();
           wa = ja / K;
           wb = jb / K;
         }
-        const uint32_t gap = __ballot_sync(FULL, !near && i >= K - 1);
+        const uint32_t gap = __ballot_sync(FULL, !near && i >= K - 1 && i < have);
         open = gap == 0;
         if (near && wa != wb && (open || lane < __ffs(gap) - 1)) {
           const unsigned long long both = (1ull << wa) | (1ull << wb);

@@ -28,6 +28,28 @@ def test_log_sums_of_rows_with_nan(dtype):
     assert np.all(off <= 1.95e-6 + np.abs(want) * 2.0 ** -24), off
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("G,lse", [(1, False), (40, False), (60, True)])
+def test_equal_candidates_beside_dead_beams(dtype, G, lse):
+    """More candidates share the K-th score than are ranked by counting, and some
+    beams have no candidates: dead, NaN, masked wholly."""
+    W, V, K = 10, 3000, 32 if G == 60 else 64
+    x = torch.zeros(G * W, V, dtype=DT[dtype], device="cuda").view(G, W, V)
+    x[:, 2] = float("nan")
+    x[:, 4] = NEG
+    x[:, 5] = 7.0
+    cum = torch.zeros(G, W, device="cuda")
+    cum[:, 2] = NEG
+    cum[:, 7] = float("nan")
+    cum[:, 9] = NEG
+    got = [pb.beam_select(x.view(G * W, V), W, K, cum=cum, lse=out)
+           for out in (None, torch.empty(G * W, device="cuda"))][int(lse)]
+    want = OB.select(x[0].float().cpu().numpy(), W, K, cum[:1].cpu().numpy())
+    for g in range(G):
+        assert np.array_equal(got[1][g].cpu().numpy(), want[1][0]) and np.array_equal(got[2][g].cpu().numpy(), want[2][0])
+        assert np.all(np.abs(got[0][g].cpu().numpy() - want[0][0]) <= 3e-6 + np.abs(want[0][0]) * 2.0 ** -24)
+
+
 @pytest.mark.parametrize("G,W,K", [(1, 4, 128), (100, 8, 64), (300, 64, 128)])
 def test_many_equal_candidates_many_times(G, W, K):
     """Every candidate of many groups has the same score: lower beams and tokens first, in every call."""
