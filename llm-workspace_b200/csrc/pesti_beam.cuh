@@ -802,8 +802,13 @@ __global__ void __launch_bounds__(PICK_WARPS * 32) beam_pick_kernel(
       }
       lo = __reduce_or_sync(FULL, lo);
       hi = __reduce_or_sync(FULL, hi);
-      // a run that leaves the ranked part: every row.  The blocks that stayed are told.
-      flagged = open && total > have ? ~0ull : ((unsigned long long)hi << 32) | lo;
+      if (open && total > have) {
+        // a run that leaves the ranked part: every row with candidates (the others may not be read)
+        lo = __ballot_sync(FULL, lane < W && sh.n[lane] > 0);
+        hi = __ballot_sync(FULL, lane + 32 < W && sh.n[lane + 32] > 0);
+      }
+      // the blocks that stayed are told
+      flagged = ((unsigned long long)hi << 32) | lo;
       if (lane > 0 && lane < parts) *in_block(&sh.flagged, lane) = flagged;
       if (flagged)
         for (uint32_t r = 1; r < parts; ++r)

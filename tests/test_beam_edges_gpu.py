@@ -58,3 +58,18 @@ def test_many_equal_candidates_many_times(G, W, K):
     for _ in range(20):
         _, t, p = pb.beam_select(x, W, K)
         assert torch.equal(t, token) and not p.any()
+
+
+@pytest.mark.parametrize("G", [1, 30])
+def test_equal_candidates_of_few_live_beams(G):
+    """Three of 64 beams live, their 384 candidates equal; the rows of the others hold NaN."""
+    W, V, K = 64, 1200, 128
+    x = torch.full((G, W, V), float("nan"), device="cuda")
+    cum = torch.full((G, W), NEG, device="cuda")
+    x[:, [5, 31, 63]] = 2.0
+    cum[:, [5, 31, 63]] = -1.0
+    s, t, p = pb.beam_select(x.view(G * W, V), W, K, cum=cum)
+    assert torch.equal(t, torch.arange(K, dtype=torch.int32, device="cuda").expand(G, K)) and (p == 5).all()
+    # one rounding to f32 of a sum in 64 bits
+    want = -1.0 - float(np.log(V))
+    assert (s.double() - want).abs().max() <= abs(want) * 2.0 ** -24 + 1e-12
