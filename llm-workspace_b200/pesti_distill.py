@@ -116,6 +116,13 @@ def distill_topk(logits, idx, val, temperature: float = 1.0, teacher_lse=None, w
     0 are not read.  loss = weight * T^2 * KL(teacher || student).
     The teacher and the weights are constants: no gradient reaches idx, val,
     teacher_lse or weight."""
+    # what is not differentiable must not make the loss require a gradient
+    if val.requires_grad:
+        val = val.detach()
+    if teacher_lse is not None and teacher_lse.requires_grad:
+        teacher_lse = teacher_lse.detach()
+    if weight is not None and weight.requires_grad:
+        weight = weight.detach()
     return _DistillTopk.apply(logits, idx, val, temperature, teacher_lse, weight)
 
 

@@ -50,3 +50,21 @@ def test_equal_tokens_without_probability(dtype, tail, weighted):
     assert torch.isfinite(grad).all()
     if not tail:
         assert not grad[0].any() and not grad[2].any() and not grad[3].any()
+
+
+def test_the_teacher_is_a_constant():
+    """Values, weights and log sums that require a gradient get none, whether or not the logits do."""
+    x, idx, val, lse = _make(6, 2000, 7, "f32", tail=True)
+    w = torch.linspace(0.5, 1.0, 6).cuda()
+    want = pd.distill_topk(x, idx, val, 1.0, lse, w)
+    leaf = x.clone().requires_grad_()
+    for t in (val, lse, w):
+        t.requires_grad_()
+    loss = pd.distill_topk(x, idx, val, 1.0, lse, w)
+    assert torch.equal(loss, want) and not loss.requires_grad
+    (loss.sum() + 3.0 * val.sum() + 2.0 * lse.sum() + w.sum()).backward()
+    assert (val.grad == 3.0).all() and (lse.grad == 2.0).all() and (w.grad == 1.0).all()
+    pd.distill_topk(leaf, idx, val, 1.0, lse, w).sum().backward()
+    assert (val.grad == 3.0).all() and (lse.grad == 2.0).all() and (w.grad == 1.0).all()
+    _, unit = pd.distill_topk_grad(x, idx, val.detach(), 1.0, lse.detach(), w.detach())
+    assert torch.allclose(leaf.grad, unit, rtol=4 * 2.0 ** -24, atol=1e-12)
