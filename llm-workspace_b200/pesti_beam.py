@@ -58,6 +58,10 @@ def _on_device(t, dev, what: str) -> None:
         raise ValueError(f"{what} must be on the logits' device")
 
 
+# For a list of tensors that a call wrote: a backward pass that needs their old values is refused.
+_written = getattr(torch._C, "_increment_version", torch.autograd.graph.increment_version)
+
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _current_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
@@ -68,7 +72,7 @@ def _launch(device, stream, call):
     if device.type != "cuda":
         raise ValueError("tensors must be on a CUDA device (there is no CPU path)")
     index = device.index
-    if index == torch.cuda.current_device():
+    if index == _current_device():
         current = _current_stream(index)
         if stream is None or stream == current:
             return call(current)
@@ -140,6 +144,10 @@ def beam_select(logits, beams: int, k: int, cum=None, done=None, lse=None, out=N
                 score.data_ptr(), token.data_ptr(), parent.data_ptr(), _ptr(lse), ws.data_ptr(), need, st)
             if rc:
                 _check(rc)
+            if out is not None:
+                _written(out)
+            if lse is not None:
+                _written((lse,))
         return score, token, parent
 
     return _launch(dev, stream, call)
@@ -187,8 +195,9 @@ class BeamState:
         self.max_tokens, self.max_seq_len = int(max_tokens), int(max_seq_len)
         self.cap = max(1, min(self.max_tokens, self.max_seq_len))
         dev = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
-        if dev.type == "cuda" and dev.index is None:
-            dev = torch.device("cuda", torch.cuda.current_device())
+        if dev.type == "cuda":
+            current = torch.cuda.current_device()  # sets CUDA up
+            dev = torch.device("cuda", current if dev.index is None else dev.index)
         G, W, i32 = self.groups, self.beams, torch.int32
 
         def make(*shape, dtype=i32):
@@ -206,6 +215,7 @@ class BeamState:
         self.n_stop = len(stop_tokens)
         self._c = _StateC(*[getattr(self, n).data_ptr() for n, _ in _StateC._fields_[:-1]], self.cap)
         self._limits = _LimitsC(self.max_tokens, self.max_seq_len, float(length_penalty), int(bool(early_stop)))
+        self._arrays = [getattr(self, n) for n, _ in _StateC._fields_[:-1]]
         self._at = ctypes.addressof(self._c), self.stop.data_ptr(), ctypes.addressof(self._limits)
         self.reset(stream)
 
@@ -213,15 +223,17 @@ class BeamState:
         """Begins a new search: one live beam per group with score 0."""
         _launch(self.device, stream,
                 lambda st: _check(self._lib.pesti_beam_reset(self._at[0], self.groups, self.beams, st)))
+        _written(self._arrays)
 
     def advance(self, score, token, parent, stream=None) -> None:
         """Takes one step's candidates ([groups, k], as beam_select returns them)."""
-        shape, dev = score.shape, self.device
+        shape, dev, i32 = score.shape, self.device, torch.int32
         if not (len(shape) == 2 and shape[0] == self.groups and token.shape == shape and parent.shape == shape
-                and score.dtype == torch.float32 and token.dtype == torch.int32 and parent.dtype == torch.int32
+                and score.dtype == torch.float32 and token.dtype == i32 and parent.dtype == i32
                 and score.is_contiguous() and token.is_contiguous() and parent.is_contiguous()):
             raise ValueError("candidates must be contiguous [groups, k] float32, int32 and int32 tensors")
-        if not (score.device == dev and token.device == dev and parent.device == dev):
+        index = dev.index
+        if not (score.get_device() == index and token.get_device() == index and parent.get_device() == index):
             raise ValueError("candidates must be on the state's device")
         state, stop, limits = self._at
 
@@ -232,6 +244,7 @@ class BeamState:
                 _check(rc)
 
         _launch(dev, stream, call)
+        _written(self._arrays)
 
     def active(self) -> int:
         """Groups still running (a host read: call it now and then)."""
@@ -324,4 +337,5 @@ def beam_reorder(states, parent, out=None, stream=None):
             _check(rc)
 
     _launch(dev, stream, call)
+    _written(dst)
     return dst[0] if single else dst

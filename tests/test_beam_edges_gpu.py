@@ -50,6 +50,49 @@ def test_equal_candidates_beside_dead_beams(dtype, G, lse):
         assert np.all(np.abs(got[0][g].cpu().numpy() - want[0][0]) <= 3e-6 + np.abs(want[0][0]) * 2.0 ** -24)
 
 
+def test_written_tensors_have_new_versions():
+    """A backward pass that needs the old values of what a call overwrote is refused."""
+    states = [torch.rand(4, 3, device="cuda"), torch.rand(4, 2, 5, 2, device="cuda")]
+    parent = torch.tensor([[1, 0, 3, 2]], dtype=torch.int32, device="cuda")
+    for t in states:
+        y = torch.ones_like(t, requires_grad=True)
+        z = (y * t).sum()
+        pb.beam_reorder([t, torch.zeros(4, 1, device="cuda")], parent)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            z.backward()
+    # out of place: the outputs, not the states
+    a, b = torch.rand(4, 3, device="cuda"), torch.empty(4, 3, device="cuda")
+    before = a._version, b._version, parent._version
+    pb.beam_reorder(a, parent, out=b)
+    assert a._version == before[0] and b._version > before[1] and parent._version == before[2]
+
+    x, cum = _logits(4, 1000, "f32"), torch.zeros(1, 4, device="cuda")
+    out = (torch.empty(1, 8, device="cuda"), *torch.empty(2, 1, 8, dtype=torch.int32, device="cuda"))
+    lse = torch.empty(4, device="cuda")
+    written, read = (*out, lse), (x, cum)
+    before = [t._version for t in (*written, *read)]
+    pb.beam_select(x, 4, 8, cum=cum, lse=lse, out=out)
+    after = [t._version for t in (*written, *read)]
+    assert all(p < q for p, q in zip(before[:4], after[:4])) and before[4:] == after[4:]
+
+    st = pb.BeamState(1, 4, max_tokens=5, max_seq_len=9)
+    table = torch.rand(1000, 3, device="cuda", requires_grad=True)
+    z = torch.nn.functional.embedding(st.last, table).sum()
+    st.advance(*out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+    names = ("cum", "last", "parent", "tokens", "count", "done", "fin_tokens", "fin_len", "fin_score", "fin_count")
+    before = [getattr(st, n)._version for n in names]
+    st.reset()
+    assert all(getattr(st, n)._version > v for n, v in zip(names, before))
+    with torch.inference_mode():  # tensors without versions
+        s = torch.rand(4, 3, device="cuda")
+        want = s[[1, 0, 3, 2]]
+        assert torch.equal(pb.beam_reorder(s, parent), want)
+        st = pb.BeamState(1, 4, max_tokens=5, max_seq_len=9)
+        st.advance(*pb.beam_select(x, 4, 8, cum=st.cum, done=st.done, lse=torch.empty(4, device="cuda")))
+
+
 @pytest.mark.parametrize("G,W,K", [(1, 4, 128), (100, 8, 64), (300, 64, 128)])
 def test_many_equal_candidates_many_times(G, W, K):
     """Every candidate of many groups has the same score: lower beams and tokens first, in every call."""
