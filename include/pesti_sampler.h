@@ -378,7 +378,8 @@ int pesti_beam_select(const void* d_logits, pesti_dtype dtype, int64_t G, int64_
  * grows by 1.  Then the group finishes:
  *  - when count reaches min(max_tokens, max_seq_len): the live beams go to the
  *    pool with cum / count^length_penalty; done = 3 if count is max_seq_len,
- *    else 2;
+ *    else 2 (a group that is there before the step, as with a limit of 0, ends
+ *    with the same codes and nothing more);
  *  - without a live beam: done = 1;
  *  - with a full pool, if early_stop is set or no live beam can still reach the
  *    pool's lowest score (the larger of best / (count + 1)^length_penalty and

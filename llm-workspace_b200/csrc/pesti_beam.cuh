@@ -956,7 +956,7 @@ __global__ void __launch_bounds__(ADV_THREADS) beam_advance_kernel(const float* 
   }
   if (was_done || c >= limit) {
     __syncthreads();  // every thread has read `done`
-    if (tid == 0 && !was_done) st.done[g] = 2;
+    if (tid == 0 && !was_done) st.done[g] = c >= max_seq_len ? 3 : 2;
     if (tid < W) st.parent[g * W + tid] = -1;
     return;
   }

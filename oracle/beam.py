@@ -77,7 +77,7 @@ class Beams:
         if self.done:
             return
         if self.count >= self.limit:
-            self.done = 2
+            self.done = 3 if self.count >= self.max_seq_len else 2
             return
         live = []
         for r, (s, t, p) in enumerate(zip(score, token, parent)):

@@ -93,6 +93,16 @@ def test_written_tensors_have_new_versions():
         st.advance(*pb.beam_select(x, 4, 8, cum=st.cum, done=st.done, lse=torch.empty(4, device="cuda")))
 
 
+@pytest.mark.parametrize("kw,code", [
+    (dict(max_tokens=0, max_seq_len=0), 3), (dict(max_tokens=7, max_seq_len=0), 3), (dict(max_tokens=0, max_seq_len=7), 2),
+])
+def test_limit_of_nothing(kw, code):
+    """A search whose limit is 0 ends at once: 3 where count is max_seq_len, else 2."""
+    st, _ = _drive(3, 4, 8, 2, 5, [3], **kw)
+    assert st.done.tolist() == [code] * 3 and st.count.tolist() == [0] * 3 and st.fin_count.tolist() == [0] * 3
+    assert (st.parent == -1).all()
+
+
 @pytest.mark.parametrize("G,W,K", [(1, 4, 128), (100, 8, 64), (300, 64, 128)])
 def test_many_equal_candidates_many_times(G, W, K):
     """Every candidate of many groups has the same score: lower beams and tokens first, in every call."""
