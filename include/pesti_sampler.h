@@ -417,7 +417,8 @@ int pesti_beam_advance(const pesti_beam_state* state, const float* d_score, cons
  * becomes row g*W + d_parent[g*W + w] of its src; a parent outside [0, W) means
  * the beam itself.  src and dst are the same memory with the same strides (in
  * place; beams that stay are not touched) or do not overlap.  States must not
- * share memory with one another (the same dst twice is refused).
+ * share memory with one another (the same dst twice is refused), and no dst
+ * with d_parent (refused).
  * A row is `blocks` runs of block_bytes bytes, block_stride bytes apart (for a
  * cache [rows, heads, room, dim] of which `used` positions are filled: blocks =
  * heads, block_bytes = used*dim*esize).  Strides are in bytes and not negative.

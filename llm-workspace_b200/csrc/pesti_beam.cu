@@ -361,7 +361,7 @@ int pesti_beam_reorder(const pesti_beam_rows* states, int64_t n_states, const in
   if (n_states < 0 || G < 0) return refuse("n_states or G < 0");
   if (W < 1 || W > PESTI_BEAM_MAX_WIDTH) return refuse("W must be 1 to 64");
   if (n_states > 0 && !states) return refuse("null states");
-  if (G > LLONG_MAX / W) return refuse("G * W too large");
+  if (G > LLONG_MAX / W / (long long)sizeof(int32_t)) return refuse("G * W too large");
   for (int64_t i = 0; i < n_states; ++i) {
     const pesti_beam_rows& s = states[i];
     if (s.blocks < 0 || s.block_bytes < 0) return refuse("blocks or block_bytes < 0");
@@ -404,6 +404,14 @@ int pesti_beam_reorder(const pesti_beam_rows* states, int64_t n_states, const in
     }
   }
   if (!d_parent) return refuse("null parents");
+  // every block reads the parents, some behind others' writes
+  for (int64_t i = 0; i < n_states; ++i) {
+    const pesti_beam_rows& s = states[i];
+    if (s.blocks == 0 || s.block_bytes == 0) continue;
+    const char *p = (const char*)d_parent, *q = (const char*)s.dst;
+    const long long b = extent(G * W, s.dst_row_stride, s.blocks, s.dst_block_stride, s.block_bytes);
+    if (p < q + b && q < p + G * W * (long long)sizeof(int32_t)) return refuse("the parents overlap a state");
+  }
   int rc = need_device();
   if (rc) return rc;
   cudaStream_t st = (cudaStream_t)stream;

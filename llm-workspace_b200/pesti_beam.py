@@ -307,7 +307,8 @@ def beam_reorder(states, parent, out=None, stream=None):
     states: a tensor or a list of tensors of any type whose first dimension is
     groups*beams (for caches [rows, heads, room, dim], pass cache[:, :, :used]).
     In place, or into `out` (tensors of the same shapes).  States must not share
-    memory.  Returns the reordered states."""
+    memory, and what is written none with `parent`.  Returns the reordered
+    states."""
     single = isinstance(states, torch.Tensor)
     src = [states] if single else list(states)
     dst = src if out is None else ([out] if single else list(out))

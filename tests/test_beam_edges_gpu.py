@@ -126,3 +126,19 @@ def test_equal_candidates_of_few_live_beams(G):
     # one rounding to f32 of a sum in 64 bits
     want = -1.0 - float(np.log(V))
     assert (s.double() - want).abs().max() <= abs(want) * 2.0 ** -24 + 1e-12
+
+
+def test_reorder_beside_its_parents():
+    """States that lie next to the parents in one buffer, and states read from them."""
+    buf = torch.arange(64, dtype=torch.int32, device="cuda")
+    parent = buf[16:24].view(2, 4)
+    parent.copy_(torch.tensor([[1, 0, 3, 3], [2, 2, -1, 0]]))
+    idx = torch.tensor([1, 0, 3, 3, 6, 6, 6, 4], device="cuda")
+    before, behind = buf[:16].view(8, 2), buf[24:].view(8, 5)
+    want = before[idx].clone(), behind[idx].clone()
+    pb.beam_reorder([before, behind], parent)
+    assert torch.equal(before, want[0]) and torch.equal(behind, want[1])
+    out = pb.beam_reorder(parent.view(8), parent, out=torch.empty(8, dtype=torch.int32, device="cuda"))
+    assert torch.equal(out, parent.view(8)[idx])
+    with pytest.raises(Exception, match="parents overlap"):
+        pb.beam_reorder(parent.view(8), parent)
