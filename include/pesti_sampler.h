@@ -454,6 +454,8 @@ int pesti_beam_reorder(const pesti_beam_rows* states, int64_t n_states, const in
  *   grad = d loss / d x (the teacher is a constant)
  * w = d_weight[n] (NULL: 1).  A row of weight 0 (padding) is not read: its loss
  * and gradient are 0.  A row without teacher entries has loss and gradient 0.
+ * Where the largest logit is 2^29 T ln 2 or more in magnitude (masks of a
+ * type's lowest value), smaller ones count as p = 0.
  * Entries with q = 0 add nothing to the loss.  A student logit of -inf has
  * p = 0 (loss +inf where q > 0); a row of -inf alone has p = 0 everywhere.  NaN
  * and +inf logits make the row's loss and gradient NaN, as NaN in its list does.

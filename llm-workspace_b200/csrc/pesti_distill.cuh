@@ -41,6 +41,10 @@ constexpr int MAX_TOP = 256;
 constexpr int HASH = 512;
 constexpr int STATS = 8;       // numbers of a row, and then its list's gradients
 constexpr int UNIT_WARPS = 4;  // warps of a block, a unit each
+// From here on only a row's largest logit counts (pesti_rowscan.cuh).  Below, m*c_lo is at most 2^-23 * 2^29 = 64 and R's
+// rounding 16, so that terms stay within 2^+-80; at 2^30 they would leave f32.  The next smaller f32 lies 32 binary
+// orders below.
+constexpr float FAR_SPLIT = 536870912.0f;
 constexpr double ONE_LN2 = 0.69314718055994530942;
 
 __host__ __device__ __forceinline__ long long stats_of(int k) { return STATS + k; }
@@ -93,13 +97,13 @@ __device__ __forceinline__ double teacher_value(const DistillArgs& a, long long 
 __device__ __forceinline__ double exact_term(float x, float m, const DistillArgs& a) {
   if (x != x) return (double)x;
   if (m == neg_inf()) return 0.0;
-  if (is_far(m, a.c)) return x == m ? 1.0 : 0.0;
+  if (is_far(m, a.c, FAR_SPLIT)) return x == m ? 1.0 : 0.0;
   return exp2((double)x * a.C - (double)ceilf(m * a.c));
 }
 
 // The reference R of a row's or unit's largest logit m (0 where it is not used).
 __device__ __forceinline__ float reference(float m, float c) {
-  return m > neg_inf() && !is_far(m, c) ? ceilf(m * c) : 0.0f;
+  return m > neg_inf() && !is_far(m, c, FAR_SPLIT) ? ceilf(m * c) : 0.0f;
 }
 
 // A term where m is far: 1 at m itself.
@@ -109,7 +113,7 @@ __device__ __forceinline__ float far_term(float x, float m) { return x == m ? 1.
 template <typename T, int NV>
 __device__ __forceinline__ float sum_terms(const uint4 (&v)[NV], float m, const DistillArgs& a) {
   float2 s0 = make_float2(0.f, 0.f), s1 = s0;
-  if (m > neg_inf() && is_far(m, a.c)) {
+  if (m > neg_inf() && is_far(m, a.c, FAR_SPLIT)) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -156,7 +160,7 @@ __device__ __forceinline__ void store_vec(T* grow, long long lo, long long V, bo
 // |(x - m) c_lo| <= 2^-23 |(x - m) C|, is far below their rounding.
 template <typename T>
 __device__ __forceinline__ float near_factor(float A, float m, const DistillArgs& a) {
-  return sizeof(T) == 2 && m > neg_inf() && !is_far(m, a.c) ? A * ex2(m * a.c_lo) : A;
+  return sizeof(T) == 2 && m > neg_inf() && !is_far(m, a.c, FAR_SPLIT) ? A * ex2(m * a.c_lo) : A;
 }
 template <typename T>
 __device__ __forceinline__ uint4 grad_vec(const uint4& v, float2 c2, float2 lo2, float2 r2, float A) {
@@ -177,7 +181,7 @@ template <typename T>
 __device__ __forceinline__ void store_any(T* grow, const uint4& v, long long lo, long long V, float m, float A,
                                           const DistillArgs& a) {
   uint4 g;
-  if (m > neg_inf() && is_far(m, a.c)) {
+  if (m > neg_inf() && is_far(m, a.c, FAR_SPLIT)) {
 #pragma unroll
     for (int q = 0; q < Elem<T>::PAIRS; ++q) {
       const float2 x = Elem<T>::pair(v, q);
@@ -375,12 +379,12 @@ __device__ __forceinline__ void join_row(const DistillArgs& a, long long n, int 
 #pragma unroll 4
   for (long long u = lane; u < a.units; u += 32) {
     const Partial p = parts[u];
-    s += (double)p.s * ref_scale(p.m, m_s, a.c);
+    s += (double)p.s * ref_scale(p.m, m_s, a.c, FAR_SPLIT);
   }
   s = warp_reduce_add(s);
   // all tokens: what was scanned, and the listed ones where they were left out
   const float m_all = tail ? fmaxf(m_s, mx) : m_s;
-  const double scale = ref_scale(m_s, m_all, a.c), e_scale = ref_scale(mx, m_all, a.c);
+  const double scale = ref_scale(m_s, m_all, a.c, FAR_SPLIT), e_scale = ref_scale(mx, m_all, a.c, FAR_SPLIT);
   double S = s * scale + (tail ? terms * e_scale : 0.0);
   if (m_all == pos_inf()) S = inf - inf;  // +inf logits have no softmax: NaN
   const double rest = 1.0 - Q;
@@ -406,7 +410,7 @@ __device__ __forceinline__ void join_row(const DistillArgs& a, long long n, int 
     double l = l0;
     if (m_all > neg_inf() && Q != 0.0) {
       const double lse =
-          is_far(m_all, a.c) ? log(S) : ONE_LN2 * (log2(S) - ((double)m_all * a.C - (double)reference(m_all, a.c)));
+          is_far(m_all, a.c, FAR_SPLIT) ? log(S) : ONE_LN2 * (log2(S) - ((double)m_all * a.C - (double)reference(m_all, a.c)));
       l += Q * (((double)m_all - (double)mx) / a.T + lse);
     }
     if (q_t != 0.0) l += q_t * (log(q_t) - log(s * scale / S));
@@ -467,7 +471,7 @@ __device__ __forceinline__ void grad_unit(const DistillArgs& a, long long n, lon
   const long long first = u * UNIT_SLOTS * VE - head, lo = first + lane * VE;
   constexpr int span = UNIT_SLOTS * VE;
   __syncwarp();
-  const bool inner = first >= 0 && first + span <= a.V && !(m > neg_inf() && is_far(m, a.c));
+  const bool inner = first >= 0 && first + span <= a.V && !(m > neg_inf() && is_far(m, a.c, FAR_SPLIT));
   const int past = row_head<T>(grow + lo);  // the vectors' place behind a 16-byte boundary of the gradient
   if (inner) {
     const float R = reference(m, a.c), f = near_factor<T>(A, m, a);

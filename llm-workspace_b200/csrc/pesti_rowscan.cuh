@@ -238,7 +238,7 @@ __device__ __forceinline__ void load_unit(uint4 (&v)[UNIT_VECS], const T* row, i
 //    smaller f32 is more than 44/c * log2(e) below m: every x but m itself
 //    vanishes against m, and the sum is the number of x equal to m.
 constexpr float FAR = 1073741824.0f;
-__device__ __forceinline__ bool is_far(float m, float c) { return !(fabsf(m * c) < FAR); }
+__device__ __forceinline__ bool is_far(float m, float c, float far = FAR) { return !(fabsf(m * c) < far); }
 
 // 2^d for an integer-valued d <= 0 (0 below the range of a double).
 __device__ __forceinline__ double pow2i(double d) {
@@ -246,9 +246,9 @@ __device__ __forceinline__ double pow2i(double d) {
 }
 
 // Factor from the reference of m_old to that of m_new >= m_old.
-__device__ __forceinline__ double ref_scale(float m_old, float m_new, float c) {
+__device__ __forceinline__ double ref_scale(float m_old, float m_new, float c, float far = FAR) {
   if (m_old == m_new) return 1.0;
-  if (!(m_old > neg_inf()) || is_far(m_old, c) || is_far(m_new, c)) return 0.0;
+  if (!(m_old > neg_inf()) || is_far(m_old, c, far) || is_far(m_new, c, far)) return 0.0;
   return pow2i((double)ceilf(m_old * c) - (double)ceilf(m_new * c));
 }
 

@@ -68,3 +68,26 @@ def test_the_teacher_is_a_constant():
     assert (val.grad == 3.0).all() and (lse.grad == 2.0).all() and (w.grad == 1.0).all()
     _, unit = pd.distill_topk_grad(x, idx, val.detach(), 1.0, lse.detach(), w.detach())
     assert torch.allclose(leaf.grad, unit, rtol=4 * 2.0 ** -24, atol=1e-12)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("T", [0.7, LOG2E / (1 + 2.0 ** -23 - 2.0 ** -40)])
+@pytest.mark.parametrize("largest", [1.0e9, 7.0e8, 5.2e8, 3.0e8])
+def test_logits_of_hundreds_of_millions(dtype, tail, T, largest):
+    """Below the magnitude where only a row's largest logit counts, and just above it, at temperatures whose
+    log2(e)/T lies nearly an f32 step above an f32."""
+    m = largest * T / LOG2E
+    x, idx, val, lse = _make(6, 2500, 6, dtype, tail=tail, T=T)
+    x = x.contiguous()
+    x[0] = m
+    x[1] = -m
+    x[2, ::2] = m        # half of them; the others, of order 1, have no probability
+    x[3] = -m
+    x[3, ::3] = -3.0 * m
+    x[4, idx[4].long()] = m
+    x[5] = m
+    x[5, 7] = -m
+    up = torch.linspace(0.5, 2.0, 6).cuda()
+    _, grad = _compare(x, idx, val, T, lse, None, dtype, up)
+    assert torch.isfinite(grad).all()
