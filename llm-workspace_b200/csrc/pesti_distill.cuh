@@ -83,7 +83,7 @@ struct DistillArgs {
 
 // What list_row leaves of a row: numbers, then e = 2^(x C - R) for the largest listed logit's R and the sum of q over
 // equal tokens of every entry (0 where there is none).
-enum { LI_Q = 0, LI_NORM = 1, LI_LOSS = 2, LI_TERMS = 3, LI_MOST = 4, LI_ENTRIES = 6 };
+enum { LI_Q = 0, LI_LOSS = 1, LI_TERMS = 2, LI_MOST = 3, LI_ENTRIES = 4 };
 __host__ __device__ __forceinline__ long long lists_of(int k) { return LI_ENTRIES + 2 * k; }
 
 __device__ __forceinline__ double teacher_value(const DistillArgs& a, long long n, int j) {
@@ -288,7 +288,6 @@ __device__ __forceinline__ void list_row(const DistillArgs& a, long long n, int3
   }
   // q = exp(t - ref): of the whole vocabulary's sum, or first of the largest; listed tokens' terms, each token once
   const double ref = tail ? (double)a.teacher_lse[n] : mt != -inf ? mt : 0.0;
-  double norm = ref;
   double Q = 0.0, terms = 0.0, l = 0.0;
   bool twice = false;  // a token is listed more than once
   for (int j0 = 0; j0 < a.k; j0 += 32) {
@@ -328,10 +327,9 @@ __device__ __forceinline__ void list_row(const DistillArgs& a, long long n, int3
   }
   double per = 1.0;
   if (!tail && Q != 0.0) {
-    // q, and sum q log q, for the sum Q of the exponentials: log q = t - norm - log Q
+    // q, and sum q log q, for the sum Q of the exponentials: log q = t - ref - log Q
     per = 1.0 / Q;
     l = l * per - log(Q);
-    norm += log(Q);
     Q = Q == Q ? 1.0 : Q;
   }
   twice = __any_sync(FULL, twice);
@@ -354,7 +352,6 @@ __device__ __forceinline__ void list_row(const DistillArgs& a, long long n, int3
   }
   if (lane == 0) {
     out[LI_Q] = Q;
-    out[LI_NORM] = norm;
     out[LI_LOSS] = l;
     out[LI_TERMS] = terms;
     out[LI_MOST] = (double)mx;
