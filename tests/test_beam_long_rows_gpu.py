@@ -7,7 +7,7 @@ import torch
 
 import beam as OB
 import pesti_beam as pb
-from test_beam_gpu import DT, NEG
+from test_beam_gpu import DT, NEG, _check
 from test_beam_plan import plan
 
 pytestmark = pytest.mark.gpu
@@ -98,3 +98,71 @@ def test_runs_of_segments_in_large_batches(dtype, G, W, V, K, run, team):
             _fill(row, kind)
     cum = -torch.rand(G, W, device="cuda")
     _check_live(x, live, W, K, cum)
+
+
+def _batch(rows, G):
+    """G groups of the same rows, each group's turned by one beam more."""
+    return torch.cat([rows.roll(g, 0) for g in range(G)])
+
+
+# W, G, K and the warps of a team; the cluster's blocks do not stay
+TEAMS = [(10, 40, 20, 3), (10, 60, 20, 1), (10, 60, 64, 3), (3, 250, 6, 1), (16, 30, 128, 3)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("W,G,K,team", TEAMS)
+def test_masks_in_large_batches(dtype, W, G, K, team):
+    V = 5003
+    p = _plan(dtype, G, W, V, K)
+    assert p["team_warps"] == team and p["stay"] == 0
+    x = torch.randn(W, V, generator=torch.Generator().manual_seed(W)).mul(3.0).to(DT[dtype]).cuda()
+    x[0] = NEG
+    x[1] = NEG
+    x[1, 4711] = -2.0
+    x[2] = NEG
+    x[2, 17::1001] = torch.arange(len(range(17, V, 1001))).to(x.dtype).cuda()
+    if W > 3:
+        x[3, ::3] = float("nan")
+        x[4, 99] = x[4, 4000] = float("inf")
+        x[5] = torch.finfo(x.dtype).min
+        x[6, 1:] = torch.finfo(x.dtype).min
+        x[7] = float("nan")
+    cum = -torch.rand(G, W, generator=torch.Generator().manual_seed(G)).cuda()
+    cum[::3, 1] = NEG
+    cum[::5, 2] = float("nan")
+    done = torch.arange(G).cuda() % 11 == 7
+    _check(_batch(x, G), W, K, cum, done)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("W,G,K,team", TEAMS)
+def test_ties_in_large_batches(dtype, W, G, K, team):
+    """Rows of few values, so that a list is filled in rounds and more candidates are equal than are ranked."""
+    V = 3001
+    p = _plan(dtype, G, W, V, K)
+    assert p["team_warps"] == team and p["stay"] == 0
+    at = torch.arange(V).cuda()
+    x = torch.zeros(W, V, dtype=DT[dtype], device="cuda")
+    x[1] = at.div(3, rounding_mode="floor").neg().to(x.dtype)
+    x[2] = (at % 3).to(x.dtype)
+    if W > 3:
+        x[3] = at.to(x.dtype)
+        x[4] = 7.0
+        x[5, 2000:] = 1.0
+        x[6, ::2] = -0.0
+    _check(_batch(x, G), W, K)
+    cum = -0.5 * (torch.arange(G * W).view(G, W) % 2).float().cuda()
+    _check(_batch(x, G), W, K, cum)
+
+
+@pytest.mark.parametrize("shift", [0.0, 1e-7, 4e-7, 2e-6])
+@pytest.mark.parametrize("W,G,K,team,blocks", [(6, 60, 24, 3, 2), (8, 80, 24, 1, 1), (12, 40, 40, 3, 3)])
+def test_near_ties_in_large_batches(shift, W, G, K, team, blocks):
+    """Equal rows with scores a few f32 steps apart, at different alignments: one block adds the rows up again."""
+    V = 9011
+    p = _plan("f32", G, W, V, K)
+    assert p["team_warps"] == team and p["blocks"] == blocks and p["stay"] == 0
+    buf = torch.zeros(G * W, V + 2).cuda()
+    buf[:, :V] = torch.randn(V, generator=torch.Generator().manual_seed(V)).mul(3.0).cuda()
+    cum = (torch.stack([torch.randperm(W, generator=torch.Generator().manual_seed(g)) for g in range(G)]) * shift).cuda()
+    _check(buf[:, :V], W, K, cum)
