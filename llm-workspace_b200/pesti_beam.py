@@ -216,7 +216,8 @@ class BeamState:
         self._c = _StateC(*[getattr(self, n).data_ptr() for n, _ in _StateC._fields_[:-1]], self.cap)
         self._limits = _LimitsC(self.max_tokens, self.max_seq_len, float(length_penalty), int(bool(early_stop)))
         self._arrays = [getattr(self, n) for n, _ in _StateC._fields_[:-1]]
-        self._at = ctypes.addressof(self._c), self.stop.data_ptr(), ctypes.addressof(self._limits)
+        self._at = (ctypes.addressof(self._c), self.stop.data_ptr(), ctypes.addressof(self._limits),
+                    self._lib.pesti_beam_advance)
         self.reset(stream)
 
     def reset(self, stream=None) -> None:
@@ -228,18 +229,18 @@ class BeamState:
     def advance(self, score, token, parent, stream=None) -> None:
         """Takes one step's candidates ([groups, k], as beam_select returns them)."""
         shape, dev, i32 = score.shape, self.device, torch.int32
-        if not (len(shape) == 2 and shape[0] == self.groups and token.shape == shape and parent.shape == shape
+        if not (len(shape) == 2 and shape[0] == self.groups and shape == token.shape == parent.shape
                 and score.dtype == torch.float32 and token.dtype == i32 and parent.dtype == i32
                 and score.is_contiguous() and token.is_contiguous() and parent.is_contiguous()):
             raise ValueError("candidates must be contiguous [groups, k] float32, int32 and int32 tensors")
         index = dev.index
         if not (score.get_device() == index and token.get_device() == index and parent.get_device() == index):
             raise ValueError("candidates must be on the state's device")
-        state, stop, limits = self._at
+        state, stop, limits, advance = self._at
 
         def call(st):
-            rc = self._lib.pesti_beam_advance(state, score.data_ptr(), token.data_ptr(), parent.data_ptr(),
-                                              self.groups, self.beams, shape[1], stop, self.n_stop, limits, st)
+            rc = advance(state, score.data_ptr(), token.data_ptr(), parent.data_ptr(), shape[0], self.beams, shape[1],
+                         stop, self.n_stop, limits, st)
             if rc:
                 _check(rc)
 
