@@ -79,7 +79,9 @@ def _launch(device, stream, call):
     with torch.cuda.device(device):
         if stream is None:
             return call(_current_stream(index))
-        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+        # (an ExternalStream of handle 0 would be a stream of its own)
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device) if stream
+                               else torch.cuda.default_stream(device)):
             return call(stream)
 
 

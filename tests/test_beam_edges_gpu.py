@@ -142,3 +142,18 @@ def test_reorder_beside_its_parents():
     assert torch.equal(out, parent.view(8)[idx])
     with pytest.raises(Exception, match="parents overlap"):
         pb.beam_reorder(parent.view(8), parent)
+
+
+def test_the_default_stream_by_its_handle():
+    """stream=0 is the legacy default stream, also from within another stream: what a call allocates belongs to it."""
+    side, index = torch.cuda.Stream(), torch.cuda.current_device()
+    x = _logits(8, 5000, "bf16")
+    want = pb.beam_select(x, 4, 8)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        seen = pb._launch(torch.device("cuda", index), 0, lambda st: (st, torch.cuda.current_stream().cuda_stream))
+        assert seen == (0, 0)
+        assert torch.cuda.current_stream() == side
+        got = pb.beam_select(x, 4, 8, stream=0)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
