@@ -155,7 +155,10 @@ int launch_pick(const void* logits, long long G, long long V, long long ld, Pick
 // fill an SM): 32 groups of 8 beams take 11.5 us with teams of 7, 16 us with
 // teams of 3; 64 groups 21.5 us with teams of 7, 13 us with teams of 3.  Long
 // lists are too much for teams of one warp (1024 rows of 32000, K 64: 73 us,
-// 47 us with teams of 3).  Where teams of 7 fit, the blocks are not wanted
+// 47 us with teams of 3); shorter ones are not (whole calls with teams of one
+// and of 3: 128 groups of 8 x 32000 bf16, K 16 35 and 39 us; 256 groups of 8 x
+// 32000 f32 82 and 92 us; 64 groups of 16 x 32000 bf16, K 32 51 and 55 us; only
+// single beams of K 32 59 and 53 us).  Where teams of 7 fit, the blocks are not wanted
 // for other groups and stay for rows to add up again: that costs every call
 // 0.2 us, and brings two rows of 152064 f32 from 185 to 39 us.
 int team_warps(PickPlan& pl, long long G, int sms) {

@@ -27,13 +27,19 @@
 //   E[|t|] <= 12 since the entropy of 2048 terms is at most 11 bits and R
 //   less than 1 above the largest; c's own
 //   rounding 1.34e-8 * E[m - x] (<= ln V <= 22); 16 additions in f32, 2^-24
-//   each.  Together below 1.95e-6.  Units are joined in 64 bits.  Two
-//   candidates of different beams whose scores differ by less than twice
-//   LSE_EPS are therefore not ordered by these sums: the merge adds up their
-//   rows again in 64 bits, in index order, and ranks once more (random logits,
-//   8 beams, K 16: about one group in 1500, which then takes some 40 us more;
+//   each (units with NaN add in 64 bits).  Together below 1.95e-6.  (Beyond
+//   |m*c| = 2^23 the rounding of m*c moves R by up to 32, but there logits lie
+//   so far apart that nearly all mass has t of the largest: half an ulp of it
+//   is at most 6.6e-7, within what c's rounding and the spread of t leave.)
+//   Units are joined in 64 bits.  Two candidates of different beams whose
+//   scores differ by less than twice LSE_EPS are therefore not ordered by these
+//   sums: the merge adds up their rows again in 64 bits, in index order, and
+//   ranks once more (random logits, 8 beams, K 16: about one group in 1500).
 //   64-bit operations run at about 16 a cycle and SM, so rows are shared out
-//   over the cluster where its blocks are not needed for other groups).
+//   over the cluster where its blocks are not needed for other groups: two rows
+//   add 33 us to a call of 32 groups of 8 x 152064 f32 (49 -> 82 us), eight 119.
+//   In larger batches one block adds them up: two rows add 111 us to 64 groups
+//   (76 -> 186 us), eight 430, and with more groups a call more often holds one.
 #pragma once
 #include "pesti_common.cuh"
 #include "pesti_rowscan.cuh"
@@ -154,8 +160,9 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32) beam_scan_kernel(const T* __r
 // sums.  A team's arrays lie in dynamic shared memory behind the x and idx of
 // the group's lists; the merge's scores take their place.
 struct PickPlan {
-  int W, K, rows, teams, nkeys, run, cap;  // nkeys: a multiple of 4; run: segments of a key; cap: entries of a team's list
-  int stay;                                // the cluster's blocks help to add up rows again
+  // nkeys: a multiple of 4; run: segments of a key; cap: entries of a team's list
+  int W, K, rows, teams, nkeys, run, cap;
+  int stay;  // the cluster's blocks help to add up rows again
   long long units;
 };
 
@@ -173,7 +180,7 @@ enum { TM_NSEL = 0, TM_NLIST = 1, TM_OVER = 2, TM_T = 3, TM_MAX = 4, TM_MIN = 5,
 
 constexpr int TEAM_WORDS = BINS + MAX_SEL + 32;
 
-// The block's dynamic shared memory: the lists, then a team's list, keys, and words (the histogram first) for every team.
+// The block's dynamic shared memory: the lists, then for every team its list, keys and words (the histogram first).
 __host__ __device__ __forceinline__ long long list_bytes(int W, int K) { return ((long long)W * K * 8 + 15) / 16 * 16; }
 __host__ __device__ __forceinline__ long long keys_offset(int cap) { return (long long)cap * 8; }
 __host__ __device__ __forceinline__ long long hist_offset(int nkeys, int cap) {

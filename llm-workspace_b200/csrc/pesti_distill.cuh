@@ -41,9 +41,9 @@ constexpr int MAX_TOP = 256;
 constexpr int HASH = 512;
 constexpr int STATS = 8;       // numbers of a row, and then its list's gradients
 constexpr int UNIT_WARPS = 4;  // warps of a block, a unit each
-// From here on only a row's largest logit counts (pesti_rowscan.cuh).  Below, m*c_lo is at most 2^-23 * 2^29 = 64 and R's
-// rounding 16, so that terms stay within 2^+-80; at 2^30 they would leave f32.  The next smaller f32 lies 32 binary
-// orders below.
+// |m*c| from which on only a row's largest logit counts (pesti_rowscan.cuh).  Below it m*c_lo is at most 2^-23 * 2^29 =
+// 64 and R's rounding 16, so that terms stay within 2^+-80; with 2^30 they would leave f32.  The next smaller f32 lies
+// 32 powers of two below.
 constexpr float FAR_SPLIT = 536870912.0f;
 constexpr double ONE_LN2 = 0.69314718055994530942;
 
@@ -407,7 +407,9 @@ __device__ __forceinline__ void join_row(const DistillArgs& a, long long n, int 
     double l = l0;
     if (m_all > neg_inf() && Q != 0.0) {
       const double lse =
-          is_far(m_all, a.c, FAR_SPLIT) ? log(S) : ONE_LN2 * (log2(S) - ((double)m_all * a.C - (double)reference(m_all, a.c)));
+          is_far(m_all, a.c, FAR_SPLIT)
+              ? log(S)
+              : ONE_LN2 * (log2(S) - ((double)m_all * a.C - (double)reference(m_all, a.c)));
       l += Q * (((double)m_all - (double)mx) / a.T + lse);
     }
     if (q_t != 0.0) l += q_t * (log(q_t) - log(s * scale / S));

@@ -236,7 +236,8 @@ __device__ __forceinline__ void load_unit(uint4 (&v)[UNIT_VECS], const T* row, i
 //    joined by an exact power of two;
 //  - where |m*c| >= 2^30 (masks of the type's lowest value, +inf) the next
 //    smaller f32 is more than 44/c * log2(e) below m: every x but m itself
-//    vanishes against m, and the sum is the number of x equal to m.
+//    vanishes against m, and the sum is the number of x equal to m.  (A caller
+//    may set the limit lower.)
 constexpr float FAR = 1073741824.0f;
 __device__ __forceinline__ bool is_far(float m, float c, float far = FAR) { return !(fabsf(m * c) < far); }
 

@@ -46,7 +46,8 @@ def test_equal_candidates_beside_dead_beams(dtype, G, lse):
            for out in (None, torch.empty(G * W, device="cuda"))][int(lse)]
     want = OB.select(x[0].float().cpu().numpy(), W, K, cum[:1].cpu().numpy())
     for g in range(G):
-        assert np.array_equal(got[1][g].cpu().numpy(), want[1][0]) and np.array_equal(got[2][g].cpu().numpy(), want[2][0])
+        assert np.array_equal(got[1][g].cpu().numpy(), want[1][0])
+        assert np.array_equal(got[2][g].cpu().numpy(), want[2][0])
         assert np.all(np.abs(got[0][g].cpu().numpy() - want[0][0]) <= 3e-6 + np.abs(want[0][0]) * 2.0 ** -24)
 
 
@@ -94,7 +95,8 @@ def test_written_tensors_have_new_versions():
 
 
 @pytest.mark.parametrize("kw,code", [
-    (dict(max_tokens=0, max_seq_len=0), 3), (dict(max_tokens=7, max_seq_len=0), 3), (dict(max_tokens=0, max_seq_len=7), 2),
+    (dict(max_tokens=0, max_seq_len=0), 3), (dict(max_tokens=7, max_seq_len=0), 3),
+    (dict(max_tokens=0, max_seq_len=7), 2),
 ])
 def test_limit_of_nothing(kw, code):
     """A search whose limit is 0 ends at once: 3 where count is max_seq_len, else 2."""

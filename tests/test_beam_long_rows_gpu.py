@@ -164,5 +164,6 @@ def test_near_ties_in_large_batches(shift, W, G, K, team, blocks):
     assert p["team_warps"] == team and p["blocks"] == blocks and p["stay"] == 0
     buf = torch.zeros(G * W, V + 2).cuda()
     buf[:, :V] = torch.randn(V, generator=torch.Generator().manual_seed(V)).mul(3.0).cuda()
-    cum = (torch.stack([torch.randperm(W, generator=torch.Generator().manual_seed(g)) for g in range(G)]) * shift).cuda()
+    order = [torch.randperm(W, generator=torch.Generator().manual_seed(g)) for g in range(G)]
+    cum = (torch.stack(order) * shift).cuda()
     _check(buf[:, :V], W, K, cum)

@@ -35,8 +35,8 @@ def _holds(p, W, K):
 
 # rows that do not fit a key per segment, by hand: groups, beams, columns, candidates, segments of a key
 LONG = [
-    (ps.PESTI_F32, 1, 1, 12_101_363, 8, 3), (ps.PESTI_F32, 1, 2, 5_401_162, 16, 3), (ps.PESTI_F32, 1, 2, 4_000_003, 16, 2),
-    (ps.PESTI_F32, 40, 64, 1_601_048, 128, 3), (ps.PESTI_F32, 80, 8, 1_300_001, 16, 3),
+    (ps.PESTI_F32, 1, 1, 12_101_363, 8, 3), (ps.PESTI_F32, 1, 2, 5_401_162, 16, 3),
+    (ps.PESTI_F32, 1, 2, 4_000_003, 16, 2), (ps.PESTI_F32, 40, 64, 1_601_048, 128, 3), (ps.PESTI_F32, 80, 8, 1_300_001, 16, 3),
     (ps.PESTI_F32, 40, 8, 2_700_001, 16, 3), (ps.PESTI_BF16, 1, 4, 10_900_007, 8, 3),
 ]
 
