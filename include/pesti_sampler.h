@@ -489,6 +489,56 @@ int pesti_distill_topk_backward(const void* d_logits, pesti_dtype dtype, int64_t
                                 double temperature, const double* d_stats, const float* d_up, int64_t up_stride,
                                 void* d_grad, int64_t grad_ld, void* stream);
 
+/*
+ * Cross entropy straight from the hidden states that the vocabulary projection
+ * (Linear::forward, llm-runner/src/transformer/linear.rs:51-70) makes logits of:
+ * the loss of training and of scoring, with its gradients.  The logits z =
+ * hidden * head^T are not kept.  No counterpart in the reference.
+ *
+ * hidden [N, h_ld] (first D columns) and head [V, w_ld] (first D columns), both
+ * BF16 or both F16; head 16-byte aligned, w_ld a multiple of 8.  d_target [N]
+ * of target_bytes 4 (int32) or 8 (int64).  Rows whose target is outside [0, V)
+ * and rows of weight 0 are padding: they are not read and cost nothing, their
+ * loss and gradients are 0.  w = d_weight[n] (NULL: 1).
+ *   lse  = log sum_v exp z_v
+ *   loss = w [ lse - (1 - label_smoothing) z_t - label_smoothing / V sum_v z_v
+ *              + z_loss lse^2 ]
+ *   G_v  = up w [ (1 + 2 z_loss lse) exp(z_v - lse) - (1 - label_smoothing) [v = t]
+ *              - label_smoothing / V ]
+ *   grad_hidden = G head,  grad_head = G^T hidden      (in the inputs' type)
+ * Products are summed in f32, the rows' sums of exponentials joined in 64 bits;
+ * G is rounded once to the inputs' type (F16: times a power of two that brings
+ * its largest value to about 2^14; what is 2^38 below that is lost).  Logits
+ * that are NaN or +inf make their row's loss NaN, and the gradients that the row
+ * has part in.
+ *
+ * pesti_linear_ce: d_loss [N] f32, optionally d_lse [N] f32 (0 for padding) and
+ * the gradients of the losses' sum (either may be NULL): d_grad_hidden [N,
+ * gh_ld], d_grad_head [V, gw_ld] (16-byte aligned, gw_ld a multiple of 8).
+ * pesti_linear_ce_backward: the gradients of sum_n d_up[n*up_stride] * loss_n
+ * (up_stride 0: one value for all rows) from the forward call's inputs and lse.
+ * Outputs overlap neither inputs nor one another.  d_ws: device scratch of
+ * pesti_linear_ce_workspace(...) bytes for what the call computes (passes:
+ * PESTI_LINEAR_CE_FORWARD, _GRADS, or both), 256-byte aligned, any contents;
+ * calls whose GPU work may overlap need scratch of their own.
+ * Both run on the calling thread's current device, stream-ordered (NULL: the
+ * legacy default stream), allocate nothing, add in a fixed order (the same
+ * inputs give the same bits) and may be captured into a graph.
+ */
+#define PESTI_LINEAR_CE_FORWARD 1
+#define PESTI_LINEAR_CE_GRADS 2
+/* Bytes of scratch, or a negative PESTI_E_* code for refused sizes. */
+int64_t pesti_linear_ce_workspace(pesti_dtype dtype, int64_t N, int64_t V, int64_t D, int passes);
+int pesti_linear_ce(const void* d_hidden, pesti_dtype dtype, int64_t N, int64_t D, int64_t h_ld, const void* d_head,
+                    int64_t V, int64_t w_ld, const void* d_target, int target_bytes, const float* d_weight,
+                    double label_smoothing, double z_loss, float* d_loss, float* d_lse, void* d_grad_hidden,
+                    int64_t gh_ld, void* d_grad_head, int64_t gw_ld, void* d_ws, int64_t ws_bytes, void* stream);
+int pesti_linear_ce_backward(const void* d_hidden, pesti_dtype dtype, int64_t N, int64_t D, int64_t h_ld,
+                             const void* d_head, int64_t V, int64_t w_ld, const void* d_target, int target_bytes,
+                             const float* d_weight, double label_smoothing, double z_loss, const float* d_lse,
+                             const float* d_up, int64_t up_stride, void* d_grad_hidden, int64_t gh_ld,
+                             void* d_grad_head, int64_t gw_ld, void* d_ws, int64_t ws_bytes, void* stream);
+
 /* Message of the last failure on the calling thread ("" if none). */
 const char* pesti_last_error(void);
 

@@ -1,0 +1,438 @@
+// Host side of the cross entropy from hidden states (include/pesti_sampler.h).
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+
+#include "../../include/pesti_sampler.h"
+#include "pesti_error.h"
+#include "pesti_lce.cuh"
+#include "pesti_tensor_map.h"
+
+namespace {
+
+using namespace pesti_lce;
+
+int refuse(const char* msg) { return pesti_set_error(PESTI_E_INVALID_ARG, msg); }
+
+long long up_to(long long n, long long to) { return (n + to - 1) / to * to; }
+
+struct Call {
+  const void* hidden;
+  pesti_dtype dtype;
+  int64_t N, D, h_ld;
+  const void* head;
+  int64_t V, w_ld;
+  const void* target;
+  int target_bytes;
+  const float* weight;
+  double eps, zeta;
+};
+
+int check_sizes(pesti_dtype dtype, int64_t N, int64_t V, int64_t D) {
+  if (dtype != PESTI_BF16 && dtype != PESTI_F16) return refuse("hidden states and head must be bf16 or f16");
+  if (N < 0) return refuse("N < 0");
+  if (N > 1 << 24) return refuse("N must be at most 2^24");
+  if (V < 1 || V > 1 << 24) return refuse("V must be 1 to 2^24");
+  if (D < 1 || D > 1 << 20) return refuse("D must be 1 to 2^20");
+  if (up_to(N, 256) / 128 * (up_to(V, BN) / BN) > 0x3fffffff) return refuse("N * V too large");
+  if (up_to(V, BN) / 128 * (up_to(D, BN) / BN) > 0x3fffffff) return refuse("V * D too large");
+  if (up_to(N, 256) / 128 * (up_to(D, BN) / BN) > 0xffffff) return refuse("N * D too large");
+  return PESTI_OK;
+}
+
+int check(const Call& c) {
+  const int rc = check_sizes(c.dtype, c.N, c.V, c.D);
+  if (rc) return rc;
+  if (c.h_ld < c.D && c.N > 1) return refuse("h_ld is below D");
+  if (c.w_ld < c.D) return refuse("w_ld is below D");
+  if (c.w_ld % 8 || c.w_ld > 1LL << 36) return refuse("w_ld must be a multiple of 8");
+  if (c.target_bytes != 4 && c.target_bytes != 8) return refuse("targets must be of 4 or 8 bytes");
+  if (!(c.eps >= 0.0 && c.eps < 1.0)) return refuse("label_smoothing must be 0 to below 1");
+  if (!(c.zeta >= 0.0 && c.zeta <= 1e6)) return refuse("z_loss must be 0 to 1e6");
+  if (c.N == 0) return PESTI_OK;
+  if (!c.hidden || !c.head || !c.target) return refuse("null hidden states, head or targets");
+  if ((uintptr_t)c.hidden % 2) return refuse("hidden states are not aligned to their type");
+  if ((uintptr_t)c.head % 16) return refuse("head is not 16-byte aligned");
+  if ((uintptr_t)c.target % c.target_bytes) return refuse("targets are not aligned to their type");
+  if ((uintptr_t)c.weight % 4) return refuse("weights are not aligned to their type");
+  return PESTI_OK;
+}
+
+bool overlap(const void* p, __int128 np, const void* q, __int128 nq) {
+  return (__int128)(uintptr_t)p < (__int128)(uintptr_t)q + nq && (__int128)(uintptr_t)q < (__int128)(uintptr_t)p + np;
+}
+
+int check_grads(const Call& c, const void* dh, int64_t dh_ld, const void* dw, int64_t dw_ld) {
+  const __int128 h = ((__int128)(c.N - 1) * c.h_ld + c.D) * 2, w = ((__int128)(c.V - 1) * c.w_ld + c.D) * 2;
+  const __int128 oh = ((__int128)(c.N - 1) * dh_ld + c.D) * 2, ow = ((__int128)(c.V - 1) * dw_ld + c.D) * 2;
+  if (dh) {
+    if (dh_ld < c.D && c.N > 1) return refuse("dh_ld is below D");
+    if ((uintptr_t)dh % 2) return refuse("the hidden states' gradient is not aligned to its type");
+    if (overlap(dh, oh, c.hidden, h) || overlap(dh, oh, c.head, w)) return refuse("inputs and gradients overlap");
+  }
+  if (dw) {
+    if (dw_ld < c.D) return refuse("dw_ld is below D");
+    if (dw_ld % 8 || dw_ld > 1LL << 36) return refuse("dw_ld must be a multiple of 8");
+    if ((uintptr_t)dw % 16) return refuse("the head's gradient is not 16-byte aligned");
+    if (overlap(dw, ow, c.hidden, h) || overlap(dw, ow, c.head, w)) return refuse("inputs and gradients overlap");
+    if (dh && overlap(dh, oh, dw, ow)) return refuse("gradients overlap");
+  }
+  return PESTI_OK;
+}
+
+// How the gradients' work is cut: pieces of the vocabulary whose G stays below about 256 MB, and K of the hidden
+// states' gradient in `splits` ranges.
+struct Cut {
+  long long piece;
+  int splits, k_split;
+};
+
+constexpr int SMS = 148;
+
+Cut cut_of(int64_t N, int64_t V, int64_t D) {
+  Cut c;
+  const long long rows = up_to(N, 256);
+  const long long most = std::max<long long>(8192, (256LL << 20) / (2 * rows));
+  const long long pieces = (V + most - 1) / most;
+  c.piece = up_to((V + pieces - 1) / pieces, BN);
+  // The time of a number of splits, in stages of a tile (64 of K, 0.3 us): whole rounds of tiles over the SMs, 16
+  // stages to fill and empty a tile, and the parts' way through HBM.
+  const long long tiles = rows / 128 * ((D + BN - 1) / BN), k = (c.piece + BK - 1) / BK;
+  const double part = (double)N * D * 8 / 6.5e12 / 0.3e-6;
+  double best = 1e30;
+  c.splits = 1;
+  for (int s = 1; s <= 64 && s * 4 <= k + 3; ++s) {
+    if (s > 1 && (long long)s * rows * D * 4 > 512LL << 20) break;
+    const double t = (double)((tiles * s + SMS - 1) / SMS) * ((k + s - 1) / s + 16) + s * part;
+    if (t < best) {
+      best = t;
+      c.splits = s;
+    }
+  }
+  c.k_split = (int)((k + c.splits - 1) / c.splits);
+  return c;
+}
+
+struct Layout {
+  Plan* plan;
+  int *idx, *packed, *place;
+  RowCoef* coef;
+  float* zt;
+  uint16_t* rows;
+  float2* parts;
+  float* zsum;
+  uint16_t* grad;
+  float* part32;
+  long long rows_pad, ldc, ld32;
+  Cut cut;
+  long long bytes;
+};
+
+// `forward`: with the tiles' statistics; `grads`: with a piece of G and the parts of the hidden states' gradient.
+Layout layout(char* base, int64_t N, int64_t V, int64_t D, bool forward, bool grads) {
+  Layout l = {};
+  long long at = 0;
+  auto take = [&](long long bytes) {
+    char* p = base + at;
+    at += up_to(bytes, 1024);
+    return p;
+  };
+  l.rows_pad = up_to(N, 256);
+  l.ldc = up_to(D, 8);
+  l.ld32 = up_to(D, 4);
+  l.plan = (Plan*)take(sizeof(Plan));
+  l.idx = (int*)take(l.rows_pad * 4);
+  l.packed = (int*)take(l.rows_pad * 4);
+  l.place = (int*)take(l.rows_pad * 4);
+  l.coef = (RowCoef*)take(l.rows_pad * sizeof(RowCoef));
+  l.zt = (float*)take(l.rows_pad * 4);
+  l.rows = (uint16_t*)take(l.rows_pad * l.ldc * 2);
+  const long long tiles = up_to(V, BN) / BN;
+  if (forward) {
+    l.parts = (float2*)take(tiles * l.rows_pad * 8);
+    l.zsum = (float*)take(tiles * l.rows_pad * 4);
+  }
+  if (grads) {
+    l.cut = cut_of(N, V, D);
+    l.grad = (uint16_t*)take(l.rows_pad * l.cut.piece * 2);
+    l.part32 = (float*)take(l.cut.splits * l.rows_pad * l.ld32 * 4);
+  }
+  l.bytes = at;
+  return l;
+}
+
+int need_device(int& sms) {
+  int n = 0, dev = 0;
+  if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0)
+    return pesti_set_error(PESTI_E_NO_DEVICE, "no CUDA device available");
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, "device query");
+}
+
+template <int CG, bool BF16, bool A_MN, bool B_MN, Epilogue E>
+int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const GemmArgs& g, int sms,
+                cudaStream_t st) {
+  auto kernel = head_gemm_kernel<CG, BF16, A_MN, B_MN, E>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(CG));
+  if (e != cudaSuccess) return pesti_set_cuda_error(e, "head_gemm_kernel shared memory");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(sms / CG * CG));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem_bytes(CG);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kernel, a, b, out, g);
+  return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, "head_gemm_kernel launch");
+}
+
+int launched(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, what);
+}
+
+RowArgs row_args(const Call& c, const Layout& l) {
+  RowArgs r = {};
+  r.plan = l.plan;
+  r.hidden = c.hidden;
+  r.N = c.N;
+  r.D = c.D;
+  r.h_ld = c.h_ld;
+  r.V = c.V;
+  r.target = c.target;
+  r.target_bytes = c.target_bytes;
+  r.weight = c.weight;
+  r.eps = (float)c.eps;
+  r.zeta = (float)c.zeta;
+  r.idx = l.idx;
+  r.packed = l.packed;
+  r.place = l.place;
+  r.coef = l.coef;
+  r.zt = l.zt;
+  r.rows = l.rows;
+  r.ldc = l.ldc;
+  r.rows_pad = l.rows_pad;
+  r.tiles = (int)(up_to(c.V, BN) / BN);
+  r.part32 = l.part32;
+  r.ld32 = l.ld32;
+  r.splits = l.cut.splits;
+  return r;
+}
+
+GemmArgs gemm_args(const Layout& l) {
+  GemmArgs g = {};
+  g.plan = l.plan;
+  g.splits = 1;
+  g.k_split = INT_MAX;
+  g.target = l.packed;
+  g.rows_pad = l.rows_pad;
+  g.coef = l.coef;
+  g.zt = l.zt;
+  return g;
+}
+
+constexpr int CG = 1;
+
+// Packed rows and plan are there.  Statistics of all tiles, then the rows' losses.
+template <bool BF16>
+int forward(const Call& c, const Layout& l, RowArgs r, bool grads, int sms, cudaStream_t st) {
+  CUtensorMap rows, head;
+  int rc = pesti_tensor_map(&rows, c.dtype, l.rows, c.D, l.rows_pad, l.ldc * 2, 64, 128);
+  if (!rc) rc = pesti_tensor_map(&head, c.dtype, c.head, c.D, c.V, c.w_ld * 2, 64, 128);
+  if (rc) return rc;
+  GemmArgs g = gemm_args(l);
+  g.m_tiles = -1;
+  g.n_tiles = r.tiles;
+  g.k_iters = (int)((c.D + BK - 1) / BK);
+  g.fast_m = 1;
+  g.V = (int)c.V;
+  g.parts = l.parts;
+  g.zsum = c.eps != 0.0 ? l.zsum : nullptr;
+  rc = launch_gemm<CG, BF16, false, false, STATS>(rows, head, rows, g, sms, st);
+  if (rc) return rc;
+  r.parts = l.parts;
+  r.zsum = g.zsum;
+  const unsigned blocks = (unsigned)((c.N + 7) / 8);
+  if (grads)
+    lce_join_kernel<true><<<blocks, 256, 0, st>>>(r);
+  else
+    lce_join_kernel<false><<<blocks, 256, 0, st>>>(r);
+  return launched("lce_join_kernel launch");
+}
+
+// Packed rows, plan and coefficients are there.
+template <bool BF16>
+int backward(const Call& c, const Layout& l, RowArgs r, void* dh, int64_t dh_ld, void* dw, int64_t dw_ld, int sms,
+             cudaStream_t st) {
+  CUtensorMap rows_k, rows_mn, head_k, head_mn, out_w, out_h;
+  int rc = pesti_tensor_map(&rows_k, c.dtype, l.rows, c.D, l.rows_pad, l.ldc * 2, 64, 128);
+  if (!rc) rc = pesti_tensor_map(&rows_mn, c.dtype, l.rows, c.D, l.rows_pad, l.ldc * 2, 64, 64);
+  if (!rc) rc = pesti_tensor_map(&head_k, c.dtype, c.head, c.D, c.V, c.w_ld * 2, 64, 128);
+  if (!rc) rc = pesti_tensor_map(&head_mn, c.dtype, c.head, c.D, c.V, c.w_ld * 2, 64, 64);
+  if (!rc && dw) rc = pesti_tensor_map(&out_w, c.dtype, dw, c.D, c.V, dw_ld * 2, 64, 32);
+  if (!rc && dh) rc = pesti_tensor_map(&out_h, PESTI_F32, l.part32, c.D, l.cut.splits * l.rows_pad, l.ld32 * 4, 32, 32);
+  if (rc) return rc;
+  const int d_tiles = (int)((c.D + BN - 1) / BN);
+  for (long long v0 = 0; v0 < c.V; v0 += l.cut.piece) {
+    const long long width = std::min<long long>(l.cut.piece, c.V - v0);
+    CUtensorMap grad_out, grad_k, grad_mn;
+    rc = pesti_tensor_map(&grad_out, c.dtype, l.grad, width, l.rows_pad, l.cut.piece * 2, 64, 32);
+    if (!rc) rc = pesti_tensor_map(&grad_k, c.dtype, l.grad, width, l.rows_pad, l.cut.piece * 2, 64, 128);
+    if (!rc) rc = pesti_tensor_map(&grad_mn, c.dtype, l.grad, width, l.rows_pad, l.cut.piece * 2, 64, 64);
+    if (rc) return rc;
+    GemmArgs g = gemm_args(l);  // G of this piece
+    g.m_tiles = -1;
+    g.n_tiles = (int)((width + BN - 1) / BN);
+    g.k_iters = (int)((c.D + BK - 1) / BK);
+    g.fast_m = 1;
+    g.v0 = (int)v0;
+    g.b_row0 = (int)v0;
+    g.V = (int)c.V;
+    g.out_x = (int)width;
+    g.out_y = (int)l.rows_pad;
+    rc = launch_gemm<CG, BF16, false, false, GRAD>(rows_k, head_k, grad_out, g, sms, st);
+    if (rc) return rc;
+    if (dw) {  // dW = G^T h
+      g = gemm_args(l);
+      g.m_tiles = (int)((width + 128 * CG - 1) / (128 * CG));
+      g.n_tiles = d_tiles;
+      g.k_iters = -1;
+      g.v0 = (int)v0;
+      g.out_x = (int)c.D;
+      g.out_y = (int)c.V;
+      rc = launch_gemm<CG, BF16, true, true, OUT16>(grad_mn, rows_mn, out_w, g, sms, st);
+      if (rc) return rc;
+    }
+    if (dh) {  // dh += G W
+      g = gemm_args(l);
+      g.m_tiles = -1;
+      g.n_tiles = d_tiles;
+      g.k_iters = (int)((width + BK - 1) / BK);
+      g.splits = l.cut.splits;
+      g.k_split = l.cut.k_split;
+      g.b_k0 = v0;
+      g.add = v0 != 0;
+      g.out_x = (int)c.D;
+      g.out_y = INT_MAX;
+      rc = launch_gemm<CG, BF16, false, true, PART32>(grad_k, head_mn, out_h, g, sms, st);
+      if (rc) return rc;
+    }
+  }
+  if (!dh) return PESTI_OK;
+  r.d_hidden = dh;
+  r.dh_ld = dh_ld;
+  lce_finish_kernel<BF16><<<(unsigned)c.N, 256, 0, st>>>(r);
+  return launched("lce_finish_kernel launch");
+}
+
+template <bool BACKWARD>
+int pack(const Call& c, const RowArgs& r, cudaStream_t st) {
+  lce_plan_kernel<BACKWARD><<<1, 1024, 0, st>>>(r);
+  int rc = launched("lce_plan_kernel launch");
+  if (rc) return rc;
+  lce_gather_kernel<<<(unsigned)r.rows_pad, 256, 0, st>>>(r);
+  return launched("lce_gather_kernel launch");
+}
+
+int check_scratch(const void* ws, int64_t have, long long need) {
+  if (!ws || have < need) return refuse("workspace too small");
+  if ((uintptr_t)ws % 256) return refuse("workspace is not 256-byte aligned");
+  return PESTI_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t pesti_linear_ce_workspace(pesti_dtype dtype, int64_t N, int64_t V, int64_t D, int passes) {
+  const int rc = check_sizes(dtype, N, V, D);
+  if (rc) return rc;
+  if (passes < 1 || passes > 3) return refuse("passes must be 1 to 3");
+  return layout(nullptr, N, V, D, passes & 1, passes & 2).bytes;
+}
+
+int pesti_linear_ce(const void* d_hidden, pesti_dtype dtype, int64_t N, int64_t D, int64_t h_ld, const void* d_head,
+                    int64_t V, int64_t w_ld, const void* d_target, int target_bytes, const float* d_weight,
+                    double label_smoothing, double z_loss, float* d_loss, float* d_lse, void* d_grad_hidden,
+                    int64_t gh_ld, void* d_grad_head, int64_t gw_ld, void* d_ws, int64_t ws_bytes, void* stream) {
+  const Call c = {d_hidden, dtype, N, D, h_ld, d_head, V, w_ld, d_target, target_bytes, d_weight, label_smoothing,
+                  z_loss};
+  int rc = check(c);
+  if (rc) return rc;
+  if (N == 0 && !d_grad_head) return PESTI_OK;
+  if (N && !d_loss) return refuse("null loss");
+  const bool grads = d_grad_hidden || d_grad_head;
+  if (grads) {
+    rc = check_grads(c, d_grad_hidden, gh_ld, d_grad_head, gw_ld);
+    if (rc) return rc;
+  }
+  int sms = 0;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (N == 0) {
+    rc = need_device(sms);
+    if (rc) return rc;
+    const cudaError_t e = cudaMemset2DAsync(d_grad_head, gw_ld * 2, 0, D * 2, V, st);
+    return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, "cudaMemset2DAsync");
+  }
+  rc = check_scratch(d_ws, ws_bytes, layout(nullptr, N, V, D, true, grads).bytes);
+  if (rc) return rc;
+  rc = need_device(sms);
+  if (rc) return rc;
+  const Layout l = layout((char*)d_ws, N, V, D, true, grads);
+  RowArgs r = row_args(c, l);
+  r.loss = d_loss;
+  r.lse = d_lse;
+  rc = pack<false>(c, r, st);
+  if (rc) return rc;
+  rc = dtype == PESTI_BF16 ? forward<true>(c, l, r, grads, sms, st) : forward<false>(c, l, r, grads, sms, st);
+  if (rc || !grads) return rc;
+  return dtype == PESTI_BF16 ? backward<true>(c, l, r, d_grad_hidden, gh_ld, d_grad_head, gw_ld, sms, st)
+                             : backward<false>(c, l, r, d_grad_hidden, gh_ld, d_grad_head, gw_ld, sms, st);
+}
+
+int pesti_linear_ce_backward(const void* d_hidden, pesti_dtype dtype, int64_t N, int64_t D, int64_t h_ld,
+                             const void* d_head, int64_t V, int64_t w_ld, const void* d_target, int target_bytes,
+                             const float* d_weight, double label_smoothing, double z_loss, const float* d_lse,
+                             const float* d_up, int64_t up_stride, void* d_grad_hidden, int64_t gh_ld,
+                             void* d_grad_head, int64_t gw_ld, void* d_ws, int64_t ws_bytes, void* stream) {
+  const Call c = {d_hidden, dtype, N, D, h_ld, d_head, V, w_ld, d_target, target_bytes, d_weight, label_smoothing,
+                  z_loss};
+  int rc = check(c);
+  if (rc) return rc;
+  if (up_stride < 0) return refuse("negative stride");
+  if (!d_grad_hidden && !d_grad_head) return refuse("no gradient is asked for");
+  if (N == 0 && !d_grad_head) return PESTI_OK;
+  if (N && (!d_lse || !d_up)) return refuse("null lse or upstream gradient");
+  rc = check_grads(c, d_grad_hidden, gh_ld, d_grad_head, gw_ld);
+  if (rc) return rc;
+  int sms = 0;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (N == 0) {
+    rc = need_device(sms);
+    if (rc) return rc;
+    const cudaError_t e = cudaMemset2DAsync(d_grad_head, gw_ld * 2, 0, D * 2, V, st);
+    return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, "cudaMemset2DAsync");
+  }
+  rc = check_scratch(d_ws, ws_bytes, layout(nullptr, N, V, D, false, true).bytes);
+  if (rc) return rc;
+  rc = need_device(sms);
+  if (rc) return rc;
+  const Layout l = layout((char*)d_ws, N, V, D, false, true);
+  RowArgs r = row_args(c, l);
+  r.lse_in = d_lse;
+  r.up = d_up;
+  r.up_stride = up_stride;
+  rc = pack<true>(c, r, st);
+  if (rc) return rc;
+  return dtype == PESTI_BF16 ? backward<true>(c, l, r, d_grad_hidden, gh_ld, d_grad_head, gw_ld, sms, st)
+                             : backward<false>(c, l, r, d_grad_hidden, gh_ld, d_grad_head, gw_ld, sms, st);
+}
+
+}  // extern "C"

@@ -1,0 +1,611 @@
+// Cross entropy from hidden states, without keeping the logits (pesti_linear_ce*).
+//
+//   z = h W^T,  lse = log sum exp z,  loss = a [lse - (1 - eps) z_t - eps mean(z) + zeta lse^2]
+//   G = dloss/dz = c1 p - c2 [v = t] - c3,  c1 = a up (1 + 2 zeta lse), c2 = a up (1 - eps), c3 = a up eps / V
+//   dh = G W,  dW = G^T h
+//
+// Three products of one size each way, and the logits' product again, since they are not kept: 8 N V D operations
+// with gradients.  All four run in head_gemm_kernel, which differs in its operands' majors and in what becomes of the
+// accumulators.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "pesti_common.cuh"
+#include "pesti_umma.cuh"
+
+namespace pesti_lce {
+
+using namespace pesti_umma;
+
+constexpr int BN = 256;              // columns of a tile
+constexpr int BK = 64;               // of K per stage: one 128-byte swizzled row
+constexpr int EPI_WARPS = 4;         // a quarter of the accumulators' 128 rows each
+constexpr int THREADS = (EPI_WARPS + 2) * 32;
+constexpr int A_BYTES = 128 * BK * 2;
+constexpr int OUT_BYTES = 32 * 128;  // a warp's 32 rows of 128 bytes on their way out
+constexpr float LOG2E = 1.44269504f;
+
+__host__ __device__ constexpr int b_bytes(int cg) { return BN / cg * BK * 2; }
+__host__ __device__ constexpr int stages(int cg) { return cg == 1 ? 4 : 6; }
+__host__ __device__ constexpr int smem_bytes(int cg) {
+  return 1024 + stages(cg) * (A_BYTES + b_bytes(cg)) + EPI_WARPS * 2 * OUT_BYTES + 256;
+}
+
+// What the host does not know: written by the plan kernel, on the device.
+struct Plan {
+  int active;     // rows with a target and a weight
+  unsigned gmax;  // bits of an f32 that no |G| exceeds (f16 only)
+  int failed;     // a wait gave up
+};
+
+struct RowCoef {
+  float c, c1, c2, c3;  // p = 2^(z log2e - c)
+};
+
+enum Epilogue { STATS, GRAD, OUT16, PART32 };
+
+struct GemmArgs {
+  Plan* plan;
+  int m_tiles, n_tiles;  // a negative count: from the active rows
+  int k_iters;           // likewise
+  int splits, k_split;   // K in `splits` ranges of k_split stages
+  int fast_m;            // the row tiles run fastest (else the column tiles)
+  long long a_k0, b_k0;  // where K begins in A and B (rows of an MN-major operand, columns of a K-major one)
+  int a_row0, b_row0;    // where the tiles' rows begin in A and B
+  // STATS and GRAD
+  const int* target;  // [rows], of the packed rows
+  int v0, V;          // the tiles' first token, and the vocabulary
+  float2* parts;      // [tiles, rows_pad] (maximum, sum) of a tile's logits, in powers of two
+  float* zsum;        // [tiles, rows_pad] their plain sum, or null
+  float* zt;          // [rows] the target's logit
+  long long rows_pad;
+  const RowCoef* coef;
+  int add;            // PART32: add to what is there
+  int out_x, out_y;   // where the output ends
+};
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (BF16)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// The power of two that brings |G| below 2^15: f16 holds p down to 2^-39 of the largest |G| then, and the scale is
+// taken out of the sums exactly.  bf16 has the range of f32 and needs none.
+template <bool BF16>
+__device__ __forceinline__ int grad_shift(const Plan* plan) {
+  if (BF16) return 0;
+  const float m = __uint_as_float(plan->gmax);
+  if (!(m > 0.0f) || isinf(m)) return 0;
+  const int s = 14 - ilogbf(m);
+  return max(-100, min(100, s));
+}
+
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+
+// One block (CG 1) or a pair of them (CG 2) takes tiles of 128 CG x 256, one after another.  Warp 4 copies the stages
+// in, one thread of warp 5 issues the products, warps 0 to 3 empty one set of accumulators while the other is filled.
+template <int CG, bool BF16, bool A_MN, bool B_MN, Epilogue E>
+__global__ void __launch_bounds__(THREADS, 1)
+    head_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                     const __grid_constant__ CUtensorMap map_out, const GemmArgs g) {
+  constexpr int ST = stages(CG), B_BYTES = b_bytes(CG), STAGE = A_BYTES + B_BYTES, TM = 128 * CG;
+  extern __shared__ char raw[];
+  const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
+  const uint32_t out0 = base + ST * STAGE;
+  const uint32_t bars = out0 + EPI_WARPS * 2 * OUT_BYTES;
+  const uint32_t full = bars, empty = bars + 8 * ST, acc_full = empty + 8 * ST, acc_empty = acc_full + 16;
+  __shared__ uint32_t tmem_base;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 1 ? 0 : cluster_rank();
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      bar_init(full + 8 * s, 1);
+      bar_init(empty + 8 * s, 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      bar_init(acc_full + 8 * s, 1);
+      bar_init(acc_empty + 8 * s, CG * EPI_WARPS);
+    }
+    bar_init_fence();
+  }
+  if (warp == 5) tmem_alloc<CG>(smem_addr(&tmem_base), 512);
+  fence_before();
+  if constexpr (CG == 2) cluster_sync();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_base;
+
+  const int active = g.plan->active;
+  const int m_tiles = g.m_tiles < 0 ? (active + TM - 1) / TM : g.m_tiles;
+  const int n_tiles = g.n_tiles;
+  const int k_iters = g.k_iters < 0 ? (active + BK - 1) / BK : g.k_iters;
+  const int per_split = m_tiles * n_tiles, tiles = per_split * g.splits;
+  const int first = blockIdx.x / CG, step = gridDim.x / CG;
+
+  // tile -> (row tile, column tile, first stage of K, stages of K); 16 tiles of the fast side at a time
+  auto locate = [&](int tile, int& m, int& n, int& split, int& k0, int& kn) {
+    split = tile / per_split;
+    const int r = tile - split * per_split;
+    const int fast = g.fast_m ? m_tiles : n_tiles, slow = g.fast_m ? n_tiles : m_tiles;
+    const int group = r / (16 * slow), at = r - group * 16 * slow, width = min(16, fast - group * 16);
+    const int f = group * 16 + at % width, s = at / width;
+    m = g.fast_m ? f : s;
+    n = g.fast_m ? s : f;
+    k0 = split * g.k_split;
+    kn = max(0, min(g.k_split, k_iters - k0));
+  };
+
+  if (warp == 4) {
+    if (elect_one()) {
+      tma_prefetch(&map_a);
+      tma_prefetch(&map_b);
+      int s = 0, ph = 0;
+      bool ok = true;
+      for (int tile = first; tile < tiles && ok; tile += step) {
+        int m, n, split, k0, kn;
+        locate(tile, m, n, split, k0, kn);
+        const int row_a = g.a_row0 + m * TM + (int)rank * 128, row_b = g.b_row0 + n * BN + (int)rank * (BN / CG);
+        for (int k = 0; k < kn; ++k) {
+          if (!bar_wait(empty + 8 * s, ph ^ 1)) {
+            ok = false;
+            break;
+          }
+          const uint32_t bar = CG == 1 ? full + 8 * s : peer_addr(full + 8 * s, 0);
+          if (rank == 0) bar_expect(full + 8 * s, CG * STAGE);
+          const uint32_t a = base + s * STAGE, b = a + A_BYTES;
+          const int ka = (int)(g.a_k0 + (long long)(k0 + k) * BK), kb = (int)(g.b_k0 + (long long)(k0 + k) * BK);
+          if constexpr (A_MN) {
+            for (int i = 0; i < 2; ++i) tma_load<CG>(a + i * 8192, &map_a, bar, row_a + 64 * i, ka);
+          } else {
+            tma_load<CG>(a, &map_a, bar, ka, row_a);
+          }
+          if constexpr (B_MN) {
+            for (int i = 0; i < 4 / CG; ++i) tma_load<CG>(b + i * 8192, &map_b, bar, row_b + 64 * i, kb);
+          } else {
+            for (int i = 0; i < 2 / CG; ++i) tma_load<CG>(b + i * A_BYTES, &map_b, bar, kb, row_b + 128 * i);
+          }
+          if (++s == ST) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+      // every stage is read, and the products' arrivals have reached this block
+      for (int i = 0; i < ST && ok; ++i) {
+        ok = bar_wait(empty + 8 * s, ph ^ 1);
+        if (++s == ST) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+      if (!ok) {
+        atomicExch(&g.plan->failed, 1);
+        for (int i = 0; i < ST && rank == 0; ++i) bar_wait(full + 8 * i, ph);  // copies in flight
+      }
+    }
+  } else if (warp == 5) {
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t desc = mma_desc(BF16, A_MN, B_MN, TM, BN);
+      int s = 0, ph = 0, acc = 0, acc_ph = 0;
+      bool ok = true;
+      for (int tile = first; tile < tiles && ok; tile += step) {
+        int m, n, split, k0, kn;
+        locate(tile, m, n, split, k0, kn);
+        if (!bar_wait(acc_empty + 8 * acc, acc_ph ^ 1)) {
+          ok = false;
+          break;
+        }
+        fence_after();
+        const uint32_t d = tmem + acc * BN;
+        for (int k = 0; k < kn; ++k) {
+          if (!bar_wait(full + 8 * s, ph)) {
+            ok = false;
+            break;
+          }
+          fence_after();
+          const uint32_t a = base + s * STAGE, b = a + A_BYTES;
+          const uint64_t da = operand_desc(a, 8192), db = operand_desc(b, 8192);
+#pragma unroll
+          for (int j = 0; j < BK / 16; ++j)  // 16 of K: 32 bytes of a row, or 16 rows of 128 bytes
+            mma_f16<CG>(d, da + j * (A_MN ? 128 : 2), db + j * (B_MN ? 128 : 2), desc, k > 0 || j > 0);
+          mma_commit<CG>(empty + 8 * s);
+          if (++s == ST) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+        if (ok) mma_commit<CG>(acc_full + 8 * acc);
+        acc ^= 1;
+        if (acc == 0) acc_ph ^= 1;
+      }
+      if (!ok) {
+        atomicExch(&g.plan->failed, 1);
+      }
+    }
+  } else {
+    const int shift = (E == GRAD || E == OUT16) ? grad_shift<BF16>(g.plan) : 0;
+    const float scale = pow2(E == OUT16 ? -shift : shift);
+    const uint32_t out = out0 + warp * 2 * OUT_BYTES;
+    const uint32_t row_out = out + lane * 128, swz = (lane & 7) << 4;
+    const uint32_t acc_empty_to = CG == 1 ? acc_empty : peer_addr(acc_empty, 0);
+    int acc = 0, acc_ph = 0, buf = 0;
+    for (int tile = first; tile < tiles; tile += step) {
+      int m, n, split, k0, kn;
+      locate(tile, m, n, split, k0, kn);
+      if (!bar_wait(acc_full + 8 * acc, acc_ph)) {
+        atomicExch(&g.plan->failed, 1);
+        break;
+      }
+      fence_after();
+      const int warp_row = m * TM + (int)rank * 128 + warp * 32, row = warp_row + lane;
+      const uint32_t from = tmem + acc * BN + ((uint32_t)warp << 21);
+      const int col0 = n * BN;
+
+      // 128 bytes of each of the warp's rows: written swizzled, so that eight lanes write to eight banks' groups
+      auto begin_out = [&]() {
+        if (lane == 0) store_wait_read<1>();
+        __syncwarp();
+      };
+      auto put16 = [&](int chunk, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_out + buf * OUT_BYTES +
+                                                                      ((uint32_t)(chunk << 4) ^ swz)),
+                     "r"(x), "r"(y), "r"(z), "r"(w)
+                     : "memory");
+      };
+      auto end_out = [&](int x, int y, bool add) {
+        fence_smem_async();
+        __syncwarp();
+        if (lane == 0) {
+          if (y < g.out_y) {
+            if (add)
+              tma_add(&map_out, out + buf * OUT_BYTES, x, y);
+            else
+              tma_store(&map_out, out + buf * OUT_BYTES, x, y);
+          }
+          store_commit();  // one group for each buffer filled, or the waits would count wrongly
+        }
+        buf ^= 1;
+      };
+
+      if constexpr (E == STATS) {
+        const bool live = row < active;
+        const int t = live ? g.target[row] - (g.v0 + col0) : -1;
+        float mx = -INFINITY, sum = 0.0f, zs = 0.0f, zt = 0.0f;
+        const int left = g.V - (g.v0 + col0);
+#pragma unroll 1
+        for (int c = 0; c < BN && c < left; c += 32) {
+          uint32_t v[32];
+          tmem_load32(from + c, v);
+          tmem_load_wait();
+          if (__any_sync(PESTI_FULL_MASK, t >= c && t < c + 32)) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (t == c + j) zt = __uint_as_float(v[j]);
+          }
+          if (c + 32 > left) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (c + j >= left) v[j] = 0xff800000u;  // -inf
+          }
+          if (g.zsum) {
+            float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < 32; ++j) a[j & 3] += c + j < left ? __uint_as_float(v[j]) : 0.0f;
+            zs += (a[0] + a[1]) + (a[2] + a[3]);
+          }
+          float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int j = 0; j < 32; ++j) most[j & 3] = fmaxf(most[j & 3], __uint_as_float(v[j]));
+          const float now = fmaxf(mx, fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * LOG2E);
+          const float ref = now == -INFINITY ? 0.0f : now;
+          float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int j = 0; j < 32; ++j) a[j & 3] += ex2(fmaf(__uint_as_float(v[j]), LOG2E, -ref));
+          sum = sum * ex2(mx - ref) + ((a[0] + a[1]) + (a[2] + a[3]));
+          mx = now;
+        }
+        if (live) {
+          const long long at = (long long)((g.v0 + col0) / BN) * g.rows_pad + row;
+          g.parts[at] = make_float2(mx, sum);
+          if (g.zsum) g.zsum[at] = zs;
+          if (t >= 0 && t < BN) g.zt[row] = zt;
+        }
+      } else if constexpr (E == GRAD) {
+        const bool live = row < active;
+        RowCoef k = {0.0f, 0.0f, 0.0f, 0.0f};
+        int t = -1;
+        if (live) {
+          k = g.coef[row];
+          t = g.target[row] - (g.v0 + col0);
+        }
+        const float c1 = k.c1 * scale, c2 = k.c2 * scale, c3 = k.c3 * scale;
+#pragma unroll 1
+        for (int c = 0; c < BN && col0 + c < g.out_x; c += 64) {
+          begin_out();
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t v[32];
+            tmem_load32(from + c + 32 * h, v);
+            tmem_load_wait();
+            const int at = c + 32 * h;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const float p = ex2(fmaf(__uint_as_float(v[j]), LOG2E, -k.c));
+              v[j] = __float_as_uint(fmaf(c1, p, -c3));
+            }
+            if (__any_sync(PESTI_FULL_MASK, t >= at && t < at + 32)) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (t == at + j) v[j] = __float_as_uint(__uint_as_float(v[j]) - c2);
+            }
+            if (!live) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = 0;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint32_t w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                w[i] = pack2<BF16>(__uint_as_float(v[8 * j + 2 * i]), __uint_as_float(v[8 * j + 2 * i + 1]));
+              put16(4 * h + j, w[0], w[1], w[2], w[3]);
+            }
+          }
+          end_out(col0 + c, warp_row, false);
+        }
+      } else if constexpr (E == OUT16) {
+#pragma unroll 1
+        for (int c = 0; c < BN && col0 + c < g.out_x; c += 64) {
+          begin_out();
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t v[32];
+            tmem_load32(from + c + 32 * h, v);
+            tmem_load_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = kn ? __float_as_uint(__uint_as_float(v[j]) * scale) : 0u;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint32_t w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                w[i] = pack2<BF16>(__uint_as_float(v[8 * j + 2 * i]), __uint_as_float(v[8 * j + 2 * i + 1]));
+              put16(4 * h + j, w[0], w[1], w[2], w[3]);
+            }
+          }
+          end_out(col0 + c, g.v0 + warp_row, false);
+        }
+      } else {
+        if (warp_row < active) {
+#pragma unroll 1
+          for (int c = 0; c < BN && col0 + c < g.out_x; c += 32) {
+            begin_out();
+            uint32_t v[32];
+            tmem_load32(from + c, v);
+            tmem_load_wait();
+            if (kn == 0) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = 0;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) put16(j, v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            end_out(col0 + c, (int)(split * g.rows_pad) + warp_row, g.add != 0);
+          }
+        }
+      }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive_cluster(acc_empty_to + 8 * acc);
+      acc ^= 1;
+      if (acc == 0) acc_ph ^= 1;
+    }
+    if (lane == 0) store_wait_all();
+  }
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync();
+  fence_after();
+  if (warp == 5) tmem_free<CG>(tmem, 512);
+}
+
+struct RowArgs {
+  Plan* plan;
+  const void* hidden;
+  long long N, D, h_ld, V;
+  const void* target;
+  int target_bytes;
+  const float* weight;
+  float eps, zeta;
+  // of the packed rows
+  int* idx;     // [rows_pad] original row
+  int* packed;  // [rows_pad] target token
+  int* place;   // [N] packed row, or -1
+  RowCoef* coef;
+  float* zt;
+  void* rows;  // [rows_pad, ldc]
+  long long ldc, rows_pad;
+  // forward
+  const float2* parts;
+  const float* zsum;
+  int tiles;
+  float* loss;
+  float* lse;
+  // backward
+  const float* lse_in;
+  const float* up;
+  long long up_stride;
+  // finish
+  const float* part32;
+  long long ld32;
+  int splits;
+  void* d_hidden;
+  long long dh_ld;
+};
+
+__device__ __forceinline__ RowCoef coef_of(const RowArgs& a, float factor, float lse) {
+  RowCoef k;
+  k.c = lse * LOG2E;
+  k.c1 = factor * fmaf(2.0f * a.zeta, lse, 1.0f);
+  k.c2 = factor * (1.0f - a.eps);
+  k.c3 = factor * a.eps / (float)a.V;
+  return k;
+}
+
+__device__ __forceinline__ unsigned bound_of(const RowCoef& k) {
+  return __float_as_uint(fabsf(k.c1) + fabsf(k.c2) + fabsf(k.c3));
+}
+
+// One block: packs the rows that count, in their order.  BACKWARD: their coefficients as well.
+template <bool BACKWARD>
+__global__ void __launch_bounds__(1024) lce_plan_kernel(const RowArgs a) {
+  __shared__ int scratch[33];
+  __shared__ unsigned most[33];
+  int before = 0;
+  unsigned bound = 0;
+  for (long long n0 = 0; n0 < a.N; n0 += 1024) {
+    const long long n = n0 + threadIdx.x;
+    long long t = -1;
+    float w = 1.0f;
+    if (n < a.N) {
+      t = a.target_bytes == 8 ? ((const long long*)a.target)[n] : ((const int*)a.target)[n];
+      if (a.weight) w = a.weight[n];
+    }
+    const bool live = t >= 0 && t < a.V && w != 0.0f;
+    int total;
+    const int at = before + block_excl_scan_add<int>(live ? 1 : 0, scratch, total);
+    if (n < a.N) {
+      a.place[n] = live ? at : -1;
+      if (!BACKWARD && !live) {
+        a.loss[n] = 0.0f;
+        if (a.lse) a.lse[n] = 0.0f;
+      }
+    }
+    if (live) {
+      a.idx[at] = (int)n;
+      a.packed[at] = (int)t;
+      if (BACKWARD) {
+        const RowCoef k = coef_of(a, w * a.up[n * a.up_stride], a.lse_in[n]);
+        a.coef[at] = k;
+        bound = max(bound, bound_of(k));
+      }
+    }
+    before += total;
+  }
+  if (BACKWARD) bound = block_reduce_max<unsigned>(bound, most);
+  if (threadIdx.x == 0) {
+    a.plan->active = before;
+    a.plan->gmax = bound;
+    a.plan->failed = 0;
+  }
+}
+
+// The packed rows, behind them zeros to a whole tile.
+__global__ void __launch_bounds__(256) lce_gather_kernel(const RowArgs a) {
+  const int active = a.plan->active, tile_end = (active + 255) / 256 * 256;
+  const long long i = blockIdx.x;
+  if (i >= tile_end) return;
+  uint16_t* to = (uint16_t*)a.rows + i * a.ldc;
+  if (i >= active) {
+    for (long long d = threadIdx.x * 8; d < a.ldc; d += 2048) *(uint4*)(to + d) = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const uint16_t* from = (const uint16_t*)a.hidden + (long long)a.idx[i] * a.h_ld;
+  if (((uintptr_t)from & 15) == 0) {
+    long long d = threadIdx.x * 8;
+    for (; d + 8 <= a.D; d += 2048) *(uint4*)(to + d) = *(const uint4*)(from + d);
+    for (; d < a.D && d + 8 > a.D; d += 2048)
+      for (long long e = d; e < a.D; ++e) to[e] = from[e];
+  } else {
+    for (long long d = threadIdx.x; d < a.D; d += 256) to[d] = from[d];
+  }
+}
+
+// A row's tiles joined: 8 rows a block, 32 threads a row.  GRADS: the coefficients of its gradient too (up = 1).
+template <bool GRADS>
+__global__ void __launch_bounds__(256) lce_join_kernel(const RowArgs a) {
+  __shared__ float sm[8][8];
+  __shared__ double ss[8][8], sz[8][8];
+  const int r = threadIdx.x & 7, part = threadIdx.x >> 3, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int active = a.plan->active;
+  const long long i = (long long)blockIdx.x * 8 + r;
+  if ((long long)blockIdx.x * 8 >= active) return;
+  float m = -INFINITY;
+  double s = 0.0, z = 0.0;
+  auto join = [&](float m2, double s2) {
+    const float most = fmaxf(m, m2), ref = most == -INFINITY ? 0.0f : most;
+    s = s * (double)exp2f(m - ref) + s2 * (double)exp2f(m2 - ref);
+    m = most;
+  };
+  if (i < active) {
+    for (int t = part; t < a.tiles; t += 32) {
+      const float2 p = a.parts[(long long)t * a.rows_pad + i];
+      join(p.x, p.y);
+      if (a.zsum) z += a.zsum[(long long)t * a.rows_pad + i];
+    }
+  }
+#pragma unroll
+  for (int o = 8; o < 32; o <<= 1) {
+    const float m2 = __shfl_xor_sync(PESTI_FULL_MASK, m, o);
+    const double s2 = __shfl_xor_sync(PESTI_FULL_MASK, s, o);
+    z += __shfl_xor_sync(PESTI_FULL_MASK, z, o);
+    join(m2, s2);
+  }
+  if (lane < 8) {
+    sm[warp][r] = m;
+    ss[warp][r] = s;
+    sz[warp][r] = z;
+  }
+  __syncthreads();
+  if (threadIdx.x >= 8 || i >= active) return;
+  for (int w = 1; w < 8; ++w) {
+    join(sm[w][r], ss[w][r]);
+    z += sz[w][r];
+  }
+  const int n = a.idx[i];
+  const double lse = ((double)m + log2(s)) / (double)LOG2E;
+  const float w = a.weight ? a.weight[n] : 1.0f;
+  double loss = lse - (double)(1.0f - a.eps) * a.zt[i] + (double)a.zeta * lse * lse;
+  if (a.eps != 0.0f) loss -= (double)a.eps * z / (double)a.V;
+  if (a.plan->failed) loss = NAN;
+  a.loss[n] = (float)(w * loss);
+  if (a.lse) a.lse[n] = (float)lse;
+  if (GRADS) {
+    const RowCoef k = coef_of(a, w, (float)lse);
+    a.coef[i] = k;
+    atomicMax(&a.plan->gmax, bound_of(k));
+  }
+}
+
+// The hidden states' gradient: the parts summed in their order, to the rows' own places; padded rows get zeros.
+template <bool BF16>
+__global__ void __launch_bounds__(256) lce_finish_kernel(const RowArgs a) {
+  const long long n = blockIdx.x;
+  const int i = a.place[n];
+  uint16_t* to = (uint16_t*)a.d_hidden + n * a.dh_ld;
+  const float scale = a.plan->failed ? NAN : pow2(-grad_shift<BF16>(a.plan));
+  const float* from = a.part32 + i * a.ld32;
+  for (long long d = threadIdx.x; d < a.D; d += 256) {
+    float v = 0.0f;
+    if (i >= 0) {
+      for (int s = 0; s < a.splits; ++s) v += from[s * a.rows_pad * a.ld32 + d];
+      v *= scale;
+    }
+    to[d] = (uint16_t)pack2<BF16>(v, 0.0f);
+  }
+}
+
+}  // namespace pesti_lce

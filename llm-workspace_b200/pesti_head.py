@@ -1,0 +1,131 @@
+"""The vocabulary projection around the library's logit rows (include/pesti_sampler.h):
+
+    linear_cross_entropy, linear_cross_entropy_grad
+        the loss of training and scoring straight from the hidden states and the
+        projection's weight, with its gradients; the logits are not kept
+
+    loss = linear_cross_entropy(hidden, head, target)       # [N], differentiable
+    loss.sum().backward()
+
+Every call runs the CUDA kernels of libpesti_sampler.so on the tensors' device
+and the current stream (or `stream`, a cudaStream_t); there is no CPU path, and
+no call synchronises.
+"""
+from __future__ import annotations
+
+import functools
+
+import torch
+
+from pesti_beam import _launch, _need, _ptr
+from pesti_sampler import PESTI_BF16, PESTI_F16, _check, load_library
+
+_HALVES = {torch.bfloat16: PESTI_BF16, torch.float16: PESTI_F16}
+_FORWARD, _GRADS = 1, 2  # PESTI_LINEAR_CE_*
+
+
+@functools.lru_cache(maxsize=256)
+def _ce_workspace(dtype: int, N: int, V: int, D: int, passes: int) -> int:
+    need = load_library().pesti_linear_ce_workspace(dtype, N, V, D, passes)
+    _check(min(0, need))
+    return need
+
+
+def _ce_args(hidden, head, target, weight, label_smoothing, z_loss):
+    """Checks the arguments and returns them in the C call's order."""
+    dtype = _HALVES.get(hidden.dtype)
+    _need(dtype is not None and head.dtype == hidden.dtype, "hidden and head must both be bfloat16 or both float16")
+    _need(hidden.dim() == 2 and head.dim() == 2 and hidden.shape[1] == head.shape[1],
+          "hidden must be [N, D] and head [V, D]")
+    (N, D), V, dev = hidden.shape, head.shape[0], hidden.device
+    _need(D >= 1 and V >= 1, "D and V must be at least 1")
+    _need(head.device == dev and target.device == dev, "head and target must be on the hidden states' device")
+    _need(D == 1 or (hidden.stride(1) == 1 and head.stride(1) == 1), "rows of hidden and head must be contiguous")
+    _need(target.shape == (N,) and target.dtype in (torch.int64, torch.int32) and target.is_contiguous(),
+          "target must be a contiguous [N] int64 or int32 tensor")
+    if weight is not None:
+        _need(weight.device == dev and weight.dtype == torch.float32 and weight.shape == (N,)
+              and weight.is_contiguous(), "weight must be a contiguous [N] float32 tensor on the hidden states' device")
+    w_ld = head.stride(0) if V > 1 else -(-D // 8) * 8
+    return (hidden.data_ptr(), dtype, N, D, hidden.stride(0) if N > 1 else D, head.data_ptr(), V, w_ld,
+            target.data_ptr(), target.element_size(), _ptr(weight), float(label_smoothing), float(z_loss))
+
+
+def _rows_like(t, rows: int, D: int):
+    """[rows, D] with rows that begin at multiples of 16 bytes."""
+    return t.new_empty((rows, -(-D // 8) * 8))[:, :D]
+
+
+def _ce_forward(args, like, lse: bool, grad_hidden: bool, grad_head: bool, st):
+    dtype, N, D, V = args[1], args[2], args[3], args[6]
+    loss = like.new_empty(N, dtype=torch.float32)
+    lse = like.new_empty(N, dtype=torch.float32) if lse else None
+    gh = like.new_empty((N, D)) if grad_hidden else None
+    gw = _rows_like(like, V, D) if grad_head else None
+    need = _ce_workspace(dtype, N, V, D, _FORWARD | (_GRADS if grad_hidden or grad_head else 0))
+    ws = like.new_empty(need, dtype=torch.uint8)
+    _check(load_library().pesti_linear_ce(*args, loss.data_ptr(), _ptr(lse), _ptr(gh), D, _ptr(gw),
+                                          -(-D // 8) * 8, ws.data_ptr(), need, st))
+    return loss, lse, gh, gw
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, head, target, weight, label_smoothing, z_loss):
+        args = _ce_args(hidden, head, target, weight, label_smoothing, z_loss)
+        keep = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
+        loss, lse, _, _ = _launch(hidden.device, None, lambda st: _ce_forward(args, hidden, keep, False, False, st))
+        if keep:
+            ctx.more = label_smoothing, z_loss
+            ctx.save_for_backward(hidden, head, target, weight, lse)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, up):
+        # hooks (activation checkpointing, offloading) may hand back tensors at other addresses and of other strides
+        hidden, head, target, weight, lse = ctx.saved_tensors
+        args = _ce_args(hidden, head, target, weight, *ctx.more)
+        lse = lse.contiguous()
+        if up.dtype != torch.float32:
+            up = up.to(torch.float32)
+        dtype, N, D, V = args[1], args[2], args[3], args[6]
+
+        def call(st):
+            gh = hidden.new_empty((N, D)) if ctx.needs_input_grad[0] else None
+            gw = _rows_like(head, V, D) if ctx.needs_input_grad[1] else None
+            need = _ce_workspace(dtype, N, V, D, _GRADS)
+            ws = hidden.new_empty(need, dtype=torch.uint8)
+            _check(load_library().pesti_linear_ce_backward(
+                *args, lse.data_ptr(), up.data_ptr(), up.stride(0), _ptr(gh), D, _ptr(gw), -(-D // 8) * 8,
+                ws.data_ptr(), need, st))
+            return gh, gw
+
+        return *_launch(hidden.device, None, call), None, None, None, None
+
+
+def linear_cross_entropy(hidden, head, target, weight=None, label_smoothing: float = 0.0, z_loss: float = 0.0):
+    """Each row's cross entropy under softmax(hidden @ head.T) ([N] float32),
+    differentiable for `hidden` and `head`.
+
+    hidden [N, D] and head [V, D]: bfloat16 or float16, both the same (rows may
+    be strided; head's begin at multiples of 16 bytes).  target [N] int64 or
+    int32: rows whose target is outside [0, V) are padding.  weight: optional
+    [N] float32.  Padded rows and rows of weight 0 are not read and cost nothing:
+    their loss and gradients are 0.
+    loss = weight * (lse - (1 - label_smoothing) * z[target] - label_smoothing * mean(z) + z_loss * lse^2)
+    The weights are constants: no gradient reaches them."""
+    if weight is not None and weight.requires_grad:
+        weight = weight.detach()
+    return _LinearCrossEntropy.apply(hidden, head, target, weight, label_smoothing, z_loss)
+
+
+def linear_cross_entropy_grad(hidden, head, target, weight=None, label_smoothing: float = 0.0, z_loss: float = 0.0,
+                              stream=None):
+    """(loss [N], gradients of loss.sum() for hidden and head) in one call: for a
+    training step that folds what follows the loss into `weight` (a mean's 1/N, a
+    mask)."""
+    hidden, head = hidden.detach(), head.detach()
+    args = _ce_args(hidden, head, target, weight, label_smoothing, z_loss)
+    loss, _, gh, gw = _launch(hidden.device, stream, lambda st: _ce_forward(args, hidden, False, True, True, st))
+    return loss, gh, gw

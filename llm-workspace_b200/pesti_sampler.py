@@ -57,7 +57,7 @@ NVCC_FLAGS = [
 def build(verbose: bool = False) -> str:
     """Compiles csrc/ into libpesti_sampler.so for sm_100a (in-tree)."""
     srcs = [os.path.join(CSRC, f) for f in ("pesti_sampler.cu", "pesti_noalloc.cu", "pesti_beam.cu",
-                                            "pesti_distill.cu")]
+                                            "pesti_distill.cu", "pesti_lce.cu")]
     cmd = ["nvcc", *NVCC_FLAGS, "--threads", "0", "-o", LIB_PATH, *srcs, "-ldl"]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
@@ -152,6 +152,13 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.pesti_distill_topk_backward.argtypes = [vp, c_int, i64, i64, i64, vp, i64, vp, c_int, i64, i64, vp, vp,
                                                 ctypes.c_double, vp, vp, i64, vp, i64, vp]
     lib.pesti_distill_topk_backward.restype = c_int
+    lib.pesti_linear_ce_workspace.argtypes = [c_int, i64, i64, i64, c_int]
+    lib.pesti_linear_ce_workspace.restype = i64
+    head = [vp, c_int, i64, i64, i64, vp, i64, i64, vp, c_int, vp, ctypes.c_double, ctypes.c_double]
+    lib.pesti_linear_ce.argtypes = head + [vp, vp, vp, i64, vp, i64, vp, i64, vp]
+    lib.pesti_linear_ce.restype = c_int
+    lib.pesti_linear_ce_backward.argtypes = head + [vp, vp, i64, vp, i64, vp, i64, vp, i64, vp]
+    lib.pesti_linear_ce_backward.restype = c_int
     lib.pesti_last_gathered_rows.argtypes = [vp]
     lib.pesti_last_gathered_rows.restype = i64
     lib.pesti_last_gathered_reasons.argtypes = [vp, vp]
