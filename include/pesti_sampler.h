@@ -539,6 +539,45 @@ int pesti_linear_ce_backward(const void* d_hidden, pesti_dtype dtype, int64_t N,
                              const float* d_up, int64_t up_stride, void* d_grad_hidden, int64_t gh_ld,
                              void* d_grad_head, int64_t gw_ld, void* d_ws, int64_t ws_bytes, void* stream);
 
+/*
+ * The vocabulary projection's weight in 4 bits with group scales, and logits
+ * from it for the few rows of a decode step.  No counterpart in the reference
+ * (its Linear is f32, llm-runner/src/transformer/linear.rs).
+ *
+ * Of head [V, ld] (first D columns; F32, BF16 or F16) every `group` (32, 64 or
+ * 128) columns of a row share a scale:
+ *   s = bf16(-m / 8), m the group's largest value by magnitude, the first of
+ *       equal ones;  q = clamp(round-half-even(w / s), -8, 7)  (0 where s is 0)
+ * A group with an infinity or a NaN is held as NaN.
+ * Layout, with B = ceil(D / 128) blocks a row: d_q has 64 B bytes a row, d_scale
+ * 128 B / group bf16 a row, both 16-byte aligned.  In a block's 16 32-bit words,
+ * word 4t + j (t, j = 0..3) holds columns 32j + 8t to 32j + 8t + 7 as q + 8, the
+ * first in its lowest 4 bits; columns from D on hold 8 (q = 0).
+ *
+ * pesti_q4_quantize fills d_q and d_scale.  pesti_q4_dequantize writes q s
+ * (exact in F32, else rounded once).  Buffers do not overlap (refused).
+ * pesti_q4_logits: d_logits [B, ld] (first V columns; F32, BF16 or F16) = x
+ * [B, x_ld] (first D columns; F32, BF16 or F16) times the held weight.
+ * Products of x and q are exact, summed in f32 over a group and then over the
+ * groups with their scales, and rounded once.  The weight is read once for
+ * every 64 rows of 16-bit x, or 21 of F32.  The logits overlap no input
+ * (refused).  d_ws: device scratch of pesti_q4_logits_workspace(...) bytes,
+ * 256-byte aligned, any contents; calls whose GPU work may overlap need scratch
+ * of their own.
+ * All run on the calling thread's current device, stream-ordered (NULL: the
+ * legacy default stream), allocate nothing, add in a fixed order (the same
+ * inputs give the same bits) and may be captured into a graph.
+ */
+int pesti_q4_quantize(const void* d_head, pesti_dtype dtype, int64_t V, int64_t D, int64_t ld, int64_t group,
+                      void* d_q, void* d_scale, void* stream);
+int pesti_q4_dequantize(const void* d_q, const void* d_scale, int64_t V, int64_t D, int64_t group, void* d_head,
+                        pesti_dtype dtype, int64_t ld, void* stream);
+/* Bytes of scratch, or a negative PESTI_E_* code for refused sizes. */
+int64_t pesti_q4_logits_workspace(pesti_dtype dtype, int64_t B, int64_t D);
+int pesti_q4_logits(const void* d_x, pesti_dtype dtype, int64_t B, int64_t D, int64_t x_ld, const void* d_q,
+                    const void* d_scale, int64_t V, int64_t group, void* d_logits, pesti_dtype out_dtype, int64_t ld,
+                    void* d_ws, int64_t ws_bytes, void* stream);
+
 /* Message of the last failure on the calling thread ("" if none). */
 const char* pesti_last_error(void);
 

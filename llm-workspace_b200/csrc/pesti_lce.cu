@@ -45,7 +45,7 @@ int check_sizes(pesti_dtype dtype, int64_t N, int64_t V, int64_t D) {
 int check(const Call& c) {
   const int rc = check_sizes(c.dtype, c.N, c.V, c.D);
   if (rc) return rc;
-  if (c.h_ld < c.D && c.N > 1) return refuse("h_ld is below D");
+  if (c.h_ld < 0) return refuse("negative stride");  // one row may stand for all (stride 0)
   if (c.w_ld < c.D) return refuse("w_ld is below D");
   if (c.w_ld % 8 || c.w_ld > 1LL << 36) return refuse("w_ld must be a multiple of 8");
   if (c.target_bytes != 4 && c.target_bytes != 8) return refuse("targets must be of 4 or 8 bytes");
@@ -93,7 +93,7 @@ constexpr int SMS = 148;
 
 Cut cut_of(int64_t N, int64_t V, int64_t D) {
   Cut c;
-  const long long rows = up_to(N, 256);
+  const long long rows = std::max<long long>(256, up_to(N, 256));
   const long long most = std::max<long long>(8192, (256LL << 20) / (2 * rows));
   const long long pieces = (V + most - 1) / most;
   c.piece = up_to((V + pieces - 1) / pieces, BN);

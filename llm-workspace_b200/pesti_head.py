@@ -4,8 +4,16 @@
         the loss of training and scoring straight from the hidden states and the
         projection's weight, with its gradients; the logits are not kept
 
+    quantize_head, QuantizedHead
+        that weight in 4 bits with group scales, and back
+    head_logits
+        logits from it, for pesti_sampler and pesti_beam
+
     loss = linear_cross_entropy(hidden, head, target)       # [N], differentiable
     loss.sum().backward()
+    held = quantize_head(head)
+    logits = head_logits(hidden, held)                      # [B, V]
+    tokens = sampler.sample_batch(logits, config, u)        # or sampler.sample_hidden(hidden, held, config, u)
 
 Every call runs the CUDA kernels of libpesti_sampler.so on the tensors' device
 and the current stream (or `stream`, a cudaStream_t); there is no CPU path, and
@@ -17,7 +25,7 @@ import functools
 
 import torch
 
-from pesti_beam import _launch, _need, _ptr
+from pesti_beam import _DTYPES, _launch, _need, _ptr, _row_stride, _written
 from pesti_sampler import PESTI_BF16, PESTI_F16, _check, load_library
 
 _HALVES = {torch.bfloat16: PESTI_BF16, torch.float16: PESTI_F16}
@@ -129,3 +137,120 @@ def linear_cross_entropy_grad(hidden, head, target, weight=None, label_smoothing
     args = _ce_args(hidden, head, target, weight, label_smoothing, z_loss)
     loss, _, gh, gw = _launch(hidden.device, stream, lambda st: _ce_forward(args, hidden, False, True, True, st))
     return loss, gh, gw
+
+
+_BLOCK = 128  # columns of a block of the held layout
+
+
+class QuantizedHead:
+    """A [V, D] weight in 4 bits with a scale for every `group` columns of a row
+    (quantize_head), about (4.5, 4.25 or 4.125) / 16 of its bfloat16 size.
+
+    packed [V, ceil(D / 128) * 64] uint8 and padded_scale bfloat16 are the
+    library's layout (pesti_q4_quantize); scale [V, ceil(D / group)] is a view of
+    the scales that count."""
+
+    def __init__(self, packed, padded_scale, D: int, group: int):
+        self.packed, self.padded_scale, self.D, self.group = packed, padded_scale, int(D), int(group)
+
+    @property
+    def V(self) -> int:
+        return self.packed.shape[0]
+
+    @property
+    def device(self):
+        return self.packed.device
+
+    @property
+    def scale(self):
+        return self.padded_scale[:, :-(-self.D // self.group)]
+
+    def dequantize(self, dtype=torch.bfloat16, out=None, stream=None):
+        """The [V, D] weight that is held (or `out` filled with it): float32 holds it exactly."""
+        dev = self.device
+        if out is not None:
+            _need(out.device == dev and out.shape == (self.V, self.D) and out.dtype in _DTYPES
+                  and (self.D == 1 or out.stride(1) == 1),
+                  "out must be a [V, D] float32, bfloat16 or float16 tensor with contiguous rows on the held weight's "
+                  "device")
+        else:
+            _need(dtype in _DTYPES, "dtype must be float32, bfloat16 or float16")
+
+        def call(st):
+            to = out if out is not None else torch.empty((self.V, self.D), dtype=dtype, device=dev)
+            _check(load_library().pesti_q4_dequantize(
+                self.packed.data_ptr(), self.padded_scale.data_ptr(), self.V, self.D, self.group, to.data_ptr(),
+                _DTYPES[to.dtype], _row_stride(to), st))
+            if out is not None:
+                _written((out,))
+            return to
+
+        return _launch(dev, stream, call)
+
+
+def quantize_head(head, group: int = 64, stream=None) -> QuantizedHead:
+    """pesti_q4_quantize: `head` [V, D] (float32, bfloat16 or float16, rows may be
+    strided) in 4 bits with a bfloat16 scale for every `group` (32, 64 or 128)
+    columns.  A group's scale is minus an eighth of its largest value by
+    magnitude; its values are the nearest of the scale's multiples -8 to 7.  A
+    group with an infinity or a NaN is held as NaN."""
+    _need(head.dim() == 2 and head.dtype in _DTYPES, "head must be a [V, D] float32, bfloat16 or float16 tensor")
+    V, D = head.shape
+    _need(D == 1 or head.stride(1) == 1, "head rows must be contiguous")
+    _need(group in (32, 64, 128), "group must be 32, 64 or 128")
+    head = head.detach()
+
+    def call(st):
+        blocks = -(-D // _BLOCK)
+        packed = torch.empty((V, blocks * (_BLOCK // 2)), dtype=torch.uint8, device=head.device)
+        scale = torch.empty((V, blocks * (_BLOCK // group)), dtype=torch.bfloat16, device=head.device)
+        _check(load_library().pesti_q4_quantize(head.data_ptr(), _DTYPES[head.dtype], V, D, _row_stride(head), group,
+                                                packed.data_ptr(), scale.data_ptr(), st))
+        return QuantizedHead(packed, scale, D, group)
+
+    return _launch(head.device, stream, call)
+
+
+@functools.lru_cache(maxsize=256)
+def _logits_workspace(dtype: int, B: int, D: int) -> int:
+    need = load_library().pesti_q4_logits_workspace(dtype, B, D)
+    _check(min(0, need))
+    return need
+
+
+def head_logits(x, held: QuantizedHead, dtype=None, out=None, stream=None):
+    """pesti_q4_logits: x [B, D] times the held weight, [B, V] logits.
+
+    x: float32, bfloat16 or float16 (rows may be strided); products are exact and
+    summed in float32, times the scales in float32.  dtype: the logits' type
+    (None: x's), or out: the [B, V] tensor to fill (rows may be strided).  Made
+    for the few rows of a decode step: the weight is read once for every 64 rows
+    of 16-bit x, or 21 of float32."""
+    _need(x.dim() == 2 and x.dtype in _DTYPES, "x must be a [B, D] float32, bfloat16 or float16 tensor")
+    (B, D), dev = x.shape, x.device
+    _need(D == held.D, "x and the held weight have different D")
+    _need(held.device == dev, "x and the held weight must be on the same device")
+    _need(D == 1 or x.stride(1) == 1, "x rows must be contiguous")
+    if out is not None:
+        _need(out.device == dev and out.shape == (B, held.V) and out.dtype in _DTYPES
+              and (held.V == 1 or out.stride(1) == 1),
+              "out must be a [B, V] float32, bfloat16 or float16 tensor with contiguous rows on x's device")
+    else:
+        dtype = dtype or x.dtype
+        _need(dtype in _DTYPES, "dtype must be float32, bfloat16 or float16")
+    x = x.detach()
+    code = _DTYPES[x.dtype]
+
+    def call(st):
+        to = out if out is not None else x.new_empty((B, held.V), dtype=dtype)
+        if B:
+            need = _logits_workspace(code, B, D)
+            ws = x.new_empty(need, dtype=torch.uint8)
+            _check(load_library().pesti_q4_logits(
+                x.data_ptr(), code, B, D, _row_stride(x), held.packed.data_ptr(), held.padded_scale.data_ptr(),
+                held.V, held.group, to.data_ptr(), _DTYPES[to.dtype], _row_stride(to), ws.data_ptr(), need, st))
+            if out is not None:
+                _written((out,))
+        return to
+
+    return _launch(dev, stream, call)

@@ -57,7 +57,7 @@ NVCC_FLAGS = [
 def build(verbose: bool = False) -> str:
     """Compiles csrc/ into libpesti_sampler.so for sm_100a (in-tree)."""
     srcs = [os.path.join(CSRC, f) for f in ("pesti_sampler.cu", "pesti_noalloc.cu", "pesti_beam.cu",
-                                            "pesti_distill.cu", "pesti_lce.cu")]
+                                            "pesti_distill.cu", "pesti_lce.cu", "pesti_q4.cu")]
     cmd = ["nvcc", *NVCC_FLAGS, "--threads", "0", "-o", LIB_PATH, *srcs, "-ldl"]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
@@ -159,6 +159,14 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.pesti_linear_ce.restype = c_int
     lib.pesti_linear_ce_backward.argtypes = head + [vp, vp, i64, vp, i64, vp, i64, vp, i64, vp]
     lib.pesti_linear_ce_backward.restype = c_int
+    lib.pesti_q4_quantize.argtypes = [vp, c_int, i64, i64, i64, i64, vp, vp, vp]
+    lib.pesti_q4_quantize.restype = c_int
+    lib.pesti_q4_dequantize.argtypes = [vp, vp, i64, i64, i64, vp, c_int, i64, vp]
+    lib.pesti_q4_dequantize.restype = c_int
+    lib.pesti_q4_logits_workspace.argtypes = [c_int, i64, i64]
+    lib.pesti_q4_logits_workspace.restype = i64
+    lib.pesti_q4_logits.argtypes = [vp, c_int, i64, i64, i64, vp, vp, i64, i64, vp, c_int, i64, vp, i64, vp]
+    lib.pesti_q4_logits.restype = c_int
     lib.pesti_last_gathered_rows.argtypes = [vp]
     lib.pesti_last_gathered_rows.restype = i64
     lib.pesti_last_gathered_reasons.argtypes = [vp, vp]
@@ -374,6 +382,17 @@ class Sampler:
         if kept_width > 0:
             return out, kp, ki, kc
         return out
+
+    def sample_hidden(self, hidden, held, configs: Union[SamplingConfig, Sequence[SamplingConfig]], u, out=None,
+                      greedy_if_zero_t: bool = True, argmax_first: bool = False, kept_width: int = 0, stream=None):
+        """A decode step from the hidden states: sample_batch over the f32 logits of
+        `hidden` ([B, D]) and the projection's weight in 4 bits (`held`, a
+        pesti_head.QuantizedHead)."""
+        import torch
+        from pesti_head import head_logits
+        logits = head_logits(hidden, held, dtype=torch.float32, stream=stream)
+        return self.sample_batch(logits, configs, u, out=out, greedy_if_zero_t=greedy_if_zero_t,
+                                 argmax_first=argmax_first, kept_width=kept_width, stream=stream)
 
     def sample_batch_sharded(self, comm: "Comm", logits_shard, configs, u, out=None,
                              greedy_if_zero_t: bool = True, argmax_first: bool = False,
