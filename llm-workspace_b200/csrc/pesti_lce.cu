@@ -82,14 +82,11 @@ int check_grads(const Call& c, const void* dh, int64_t dh_ld, const void* dw, in
   return PESTI_OK;
 }
 
-// How the gradients' work is cut: pieces of the vocabulary whose G stays below about 256 MB, and K of the hidden
-// states' gradient in `splits` ranges.
+// How the gradients' work is cut: pieces of the vocabulary whose G stays below about 256 MB; the hidden states'
+// gradient sums ranges of a piece's K in parts of their own, up to 512 MB of them.
 struct Cut {
-  long long piece;
-  int splits, k_split;
+  long long piece, part_room;
 };
-
-constexpr int SMS = 148;
 
 Cut cut_of(int64_t N, int64_t V, int64_t D) {
   Cut c;
@@ -97,21 +94,7 @@ Cut cut_of(int64_t N, int64_t V, int64_t D) {
   const long long most = std::max<long long>(8192, (256LL << 20) / (2 * rows));
   const long long pieces = (V + most - 1) / most;
   c.piece = up_to((V + pieces - 1) / pieces, BN);
-  // The time of a number of splits, in stages of a tile (64 of K, 0.3 us): whole rounds of tiles over the SMs, 16
-  // stages to fill and empty a tile, and the parts' way through HBM.
-  const long long tiles = rows / 128 * ((D + BN - 1) / BN), k = (c.piece + BK - 1) / BK;
-  const double part = (double)N * D * 8 / 6.5e12 / 0.3e-6;
-  double best = 1e30;
-  c.splits = 1;
-  for (int s = 1; s <= 64 && s * 4 <= k + 3; ++s) {
-    if (s > 1 && (long long)s * rows * D * 4 > 512LL << 20) break;
-    const double t = (double)((tiles * s + SMS - 1) / SMS) * ((k + s - 1) / s + 16) + s * part;
-    if (t < best) {
-      best = t;
-      c.splits = s;
-    }
-  }
-  c.k_split = (int)((k + c.splits - 1) / c.splits);
+  c.part_room = std::max(rows, std::min(64 * rows, (512LL << 20) / (4 * up_to(D, 4)) / 256 * 256));
   return c;
 }
 
@@ -157,7 +140,7 @@ Layout layout(char* base, int64_t N, int64_t V, int64_t D, bool forward, bool gr
   if (grads) {
     l.cut = cut_of(N, V, D);
     l.grad = (uint16_t*)take(l.rows_pad * l.cut.piece * 2);
-    l.part32 = (float*)take(l.cut.splits * l.rows_pad * l.ld32 * 4);
+    l.part32 = (float*)take(l.cut.part_room * l.ld32 * 4);
   }
   l.bytes = at;
   return l;
@@ -172,33 +155,37 @@ int need_device(int& sms) {
   return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, "device query");
 }
 
+// Every kernel waits on the device for the one before it, so it may be launched while that one still runs.
+template <typename... K, typename... A>
+int launch(const char* what, void (*kernel)(K...), int cg, long long blocks, int threads, int smem, cudaStream_t st,
+           const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cg;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cg > 1 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, K(args)...);
+  return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, what);
+}
+
 template <int CG, bool BF16, bool A_MN, bool B_MN, Epilogue E>
 int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const GemmArgs& g, int sms,
                 cudaStream_t st) {
   auto kernel = head_gemm_kernel<CG, BF16, A_MN, B_MN, E>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(CG));
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(CG));
   if (e != cudaSuccess) return pesti_set_cuda_error(e, "head_gemm_kernel shared memory");
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(sms / CG * CG));
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = smem_bytes(CG);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kernel, a, b, out, g);
-  return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, "head_gemm_kernel launch");
+  return launch("head_gemm_kernel launch", kernel, CG, sms / CG * CG, THREADS, smem_bytes(CG), st, a, b, out, g);
 }
 
-int launched(const char* what) {
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, what);
-}
-
-RowArgs row_args(const Call& c, const Layout& l) {
+RowArgs row_args(const Call& c, const Layout& l, int cg, int sms) {
   RowArgs r = {};
   r.plan = l.plan;
   r.hidden = c.hidden;
@@ -222,15 +209,17 @@ RowArgs row_args(const Call& c, const Layout& l) {
   r.tiles = (int)(up_to(c.V, BN) / BN);
   r.part32 = l.part32;
   r.ld32 = l.ld32;
-  r.splits = l.cut.splits;
+  r.k_piece = (int)(l.cut.piece / BK);
+  r.part_room = l.cut.part_room;
+  r.tile_rows = 128 * cg;
+  r.units = sms / cg;
   return r;
 }
 
 GemmArgs gemm_args(const Layout& l) {
   GemmArgs g = {};
   g.plan = l.plan;
-  g.splits = 1;
-  g.k_split = INT_MAX;
+  g.a_box = 128;
   g.target = l.packed;
   g.rows_pad = l.rows_pad;
   g.coef = l.coef;
@@ -238,17 +227,24 @@ GemmArgs gemm_args(const Layout& l) {
   return g;
 }
 
-constexpr int CG = 1;
+// Pairs of blocks read each operand's tile half as often, which is what large products need (4096 x 128256 x 4096: 12.7
+// ms against 14.7 with single blocks); up to 128 rows the products are bound by reading the head, and a pair's second
+// block would only add empty rows (16 x 152064 x 2048: 142 us against 122).
+int blocks_per_tile(int64_t N) { return N > 128 ? 2 : 1; }
+
+// Few rows: only the 32-row boxes that hold some are copied.
+int a_box(int64_t N) { return N > 96 ? 128 : 32; }
 
 // Packed rows and plan are there.  Statistics of all tiles, then the rows' losses.
-template <bool BF16>
+template <int CG, bool BF16>
 int forward(const Call& c, const Layout& l, RowArgs r, bool grads, int sms, cudaStream_t st) {
   CUtensorMap rows, head;
-  int rc = pesti_tensor_map(&rows, c.dtype, l.rows, c.D, l.rows_pad, l.ldc * 2, 64, 128);
+  int rc = pesti_tensor_map(&rows, c.dtype, l.rows, c.D, l.rows_pad, l.ldc * 2, 64, a_box(c.N));
   if (!rc) rc = pesti_tensor_map(&head, c.dtype, c.head, c.D, c.V, c.w_ld * 2, 64, 128);
   if (rc) return rc;
   GemmArgs g = gemm_args(l);
   g.m_tiles = -1;
+  g.a_box = a_box(c.N);
   g.n_tiles = r.tiles;
   g.k_iters = (int)((c.D + BK - 1) / BK);
   g.fast_m = 1;
@@ -259,36 +255,33 @@ int forward(const Call& c, const Layout& l, RowArgs r, bool grads, int sms, cuda
   if (rc) return rc;
   r.parts = l.parts;
   r.zsum = g.zsum;
-  const unsigned blocks = (unsigned)((c.N + 7) / 8);
-  if (grads)
-    lce_join_kernel<true><<<blocks, 256, 0, st>>>(r);
-  else
-    lce_join_kernel<false><<<blocks, 256, 0, st>>>(r);
-  return launched("lce_join_kernel launch");
+  return launch("lce_join_kernel launch", grads ? lce_join_kernel<true> : lce_join_kernel<false>, 1, (c.N + 7) / 8, 256,
+                0, st, r);
 }
 
 // Packed rows, plan and coefficients are there.
-template <bool BF16>
+template <int CG, bool BF16>
 int backward(const Call& c, const Layout& l, RowArgs r, void* dh, int64_t dh_ld, void* dw, int64_t dw_ld, int sms,
              cudaStream_t st) {
   CUtensorMap rows_k, rows_mn, head_k, head_mn, out_w, out_h;
-  int rc = pesti_tensor_map(&rows_k, c.dtype, l.rows, c.D, l.rows_pad, l.ldc * 2, 64, 128);
+  int rc = pesti_tensor_map(&rows_k, c.dtype, l.rows, c.D, l.rows_pad, l.ldc * 2, 64, a_box(c.N));
   if (!rc) rc = pesti_tensor_map(&rows_mn, c.dtype, l.rows, c.D, l.rows_pad, l.ldc * 2, 64, 64);
   if (!rc) rc = pesti_tensor_map(&head_k, c.dtype, c.head, c.D, c.V, c.w_ld * 2, 64, 128);
   if (!rc) rc = pesti_tensor_map(&head_mn, c.dtype, c.head, c.D, c.V, c.w_ld * 2, 64, 64);
   if (!rc && dw) rc = pesti_tensor_map(&out_w, c.dtype, dw, c.D, c.V, dw_ld * 2, 64, 32);
-  if (!rc && dh) rc = pesti_tensor_map(&out_h, PESTI_F32, l.part32, c.D, l.cut.splits * l.rows_pad, l.ld32 * 4, 32, 32);
+  if (!rc && dh) rc = pesti_tensor_map(&out_h, PESTI_F32, l.part32, c.D, l.cut.part_room, l.ld32 * 4, 32, 32);
   if (rc) return rc;
   const int d_tiles = (int)((c.D + BN - 1) / BN);
   for (long long v0 = 0; v0 < c.V; v0 += l.cut.piece) {
     const long long width = std::min<long long>(l.cut.piece, c.V - v0);
     CUtensorMap grad_out, grad_k, grad_mn;
     rc = pesti_tensor_map(&grad_out, c.dtype, l.grad, width, l.rows_pad, l.cut.piece * 2, 64, 32);
-    if (!rc) rc = pesti_tensor_map(&grad_k, c.dtype, l.grad, width, l.rows_pad, l.cut.piece * 2, 64, 128);
+    if (!rc) rc = pesti_tensor_map(&grad_k, c.dtype, l.grad, width, l.rows_pad, l.cut.piece * 2, 64, a_box(c.N));
     if (!rc) rc = pesti_tensor_map(&grad_mn, c.dtype, l.grad, width, l.rows_pad, l.cut.piece * 2, 64, 64);
     if (rc) return rc;
     GemmArgs g = gemm_args(l);  // G of this piece
     g.m_tiles = -1;
+    g.a_box = a_box(c.N);
     g.n_tiles = (int)((width + BN - 1) / BN);
     g.k_iters = (int)((c.D + BK - 1) / BK);
     g.fast_m = 1;
@@ -313,10 +306,9 @@ int backward(const Call& c, const Layout& l, RowArgs r, void* dh, int64_t dh_ld,
     if (dh) {  // dh += G W
       g = gemm_args(l);
       g.m_tiles = -1;
+      g.a_box = a_box(c.N);
       g.n_tiles = d_tiles;
       g.k_iters = (int)((width + BK - 1) / BK);
-      g.splits = l.cut.splits;
-      g.k_split = l.cut.k_split;
       g.b_k0 = v0;
       g.add = v0 != 0;
       g.out_x = (int)c.D;
@@ -328,17 +320,20 @@ int backward(const Call& c, const Layout& l, RowArgs r, void* dh, int64_t dh_ld,
   if (!dh) return PESTI_OK;
   r.d_hidden = dh;
   r.dh_ld = dh_ld;
-  lce_finish_kernel<BF16><<<(unsigned)c.N, 256, 0, st>>>(r);
-  return launched("lce_finish_kernel launch");
+  return launch("lce_finish_kernel launch", lce_finish_kernel<BF16>, 1, c.N, 256, 0, st, r);
+}
+
+int backward(const Call& c, const Layout& l, const RowArgs& r, int cg, void* dh, int64_t dh_ld, void* dw, int64_t dw_ld,
+             int sms, cudaStream_t st) {
+  const bool bf16 = c.dtype == PESTI_BF16;
+  if (cg == 1) return (bf16 ? backward<1, true> : backward<1, false>)(c, l, r, dh, dh_ld, dw, dw_ld, sms, st);
+  return (bf16 ? backward<2, true> : backward<2, false>)(c, l, r, dh, dh_ld, dw, dw_ld, sms, st);
 }
 
 template <bool BACKWARD>
-int pack(const Call& c, const RowArgs& r, cudaStream_t st) {
-  lce_plan_kernel<BACKWARD><<<1, 1024, 0, st>>>(r);
-  int rc = launched("lce_plan_kernel launch");
-  if (rc) return rc;
-  lce_gather_kernel<<<(unsigned)r.rows_pad, 256, 0, st>>>(r);
-  return launched("lce_gather_kernel launch");
+int pack(const RowArgs& r, cudaStream_t st) {
+  const int rc = launch("lce_plan_kernel launch", lce_plan_kernel<BACKWARD>, 1, 1, 1024, 0, st, r);
+  return rc ? rc : launch("lce_gather_kernel launch", lce_gather_kernel, 1, r.rows_pad, 256, 0, st, r);
 }
 
 int check_scratch(const void* ws, int64_t have, long long need) {
@@ -386,15 +381,17 @@ int pesti_linear_ce(const void* d_hidden, pesti_dtype dtype, int64_t N, int64_t 
   rc = need_device(sms);
   if (rc) return rc;
   const Layout l = layout((char*)d_ws, N, V, D, true, grads);
-  RowArgs r = row_args(c, l);
+  const int cg = blocks_per_tile(N);
+  RowArgs r = row_args(c, l, cg, sms);
   r.loss = d_loss;
   r.lse = d_lse;
-  rc = pack<false>(c, r, st);
+  rc = pack<false>(r, st);
   if (rc) return rc;
-  rc = dtype == PESTI_BF16 ? forward<true>(c, l, r, grads, sms, st) : forward<false>(c, l, r, grads, sms, st);
+  const bool bf16 = dtype == PESTI_BF16;
+  rc = cg == 1 ? (bf16 ? forward<1, true> : forward<1, false>)(c, l, r, grads, sms, st)
+               : (bf16 ? forward<2, true> : forward<2, false>)(c, l, r, grads, sms, st);
   if (rc || !grads) return rc;
-  return dtype == PESTI_BF16 ? backward<true>(c, l, r, d_grad_hidden, gh_ld, d_grad_head, gw_ld, sms, st)
-                             : backward<false>(c, l, r, d_grad_hidden, gh_ld, d_grad_head, gw_ld, sms, st);
+  return backward(c, l, r, cg, d_grad_hidden, gh_ld, d_grad_head, gw_ld, sms, st);
 }
 
 int pesti_linear_ce_backward(const void* d_hidden, pesti_dtype dtype, int64_t N, int64_t D, int64_t h_ld,
@@ -425,14 +422,14 @@ int pesti_linear_ce_backward(const void* d_hidden, pesti_dtype dtype, int64_t N,
   rc = need_device(sms);
   if (rc) return rc;
   const Layout l = layout((char*)d_ws, N, V, D, false, true);
-  RowArgs r = row_args(c, l);
+  const int cg = blocks_per_tile(N);
+  RowArgs r = row_args(c, l, cg, sms);
   r.lse_in = d_lse;
   r.up = d_up;
   r.up_stride = up_stride;
-  rc = pack<true>(c, r, st);
+  rc = pack<true>(r, st);
   if (rc) return rc;
-  return dtype == PESTI_BF16 ? backward<true>(c, l, r, d_grad_hidden, gh_ld, d_grad_head, gw_ld, sms, st)
-                             : backward<false>(c, l, r, d_grad_hidden, gh_ld, d_grad_head, gw_ld, sms, st);
+  return backward(c, l, r, cg, d_grad_hidden, gh_ld, d_grad_head, gw_ld, sms, st);
 }
 
 }  // extern "C"

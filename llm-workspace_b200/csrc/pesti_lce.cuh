@@ -36,6 +36,8 @@ __host__ __device__ constexpr int smem_bytes(int cg) {
 struct Plan {
   int active;     // rows with a target and a weight
   unsigned gmax;  // bits of an f32 that no |G| exceeds (f16 only)
+  int splits;     // ranges of K in the hidden states' gradient
+  int part_rows;  // rows of a range's part: the active ones, to a whole tile
   int failed;     // a wait gave up
 };
 
@@ -49,10 +51,10 @@ struct GemmArgs {
   Plan* plan;
   int m_tiles, n_tiles;  // a negative count: from the active rows
   int k_iters;           // likewise
-  int splits, k_split;   // K in `splits` ranges of k_split stages
   int fast_m;            // the row tiles run fastest (else the column tiles)
   long long a_k0, b_k0;  // where K begins in A and B (rows of an MN-major operand, columns of a K-major one)
   int a_row0, b_row0;    // where the tiles' rows begin in A and B
+  int a_box;             // rows of a copy of a K-major A: 128, or 32 where few rows count
   // STATS and GRAD
   const int* target;  // [rows], of the packed rows
   int v0, V;          // the tiles' first token, and the vocabulary
@@ -127,12 +129,15 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   fence_after();
   const uint32_t tmem = tmem_base;
+  depend_wait();
+  depend_launch();
 
   const int active = g.plan->active;
   const int m_tiles = g.m_tiles < 0 ? (active + TM - 1) / TM : g.m_tiles;
   const int n_tiles = g.n_tiles;
   const int k_iters = g.k_iters < 0 ? (active + BK - 1) / BK : g.k_iters;
-  const int per_split = m_tiles * n_tiles, tiles = per_split * g.splits;
+  const int splits = E == PART32 ? g.plan->splits : 1, k_split = (k_iters + splits - 1) / splits;
+  const int per_split = m_tiles * n_tiles, tiles = per_split * splits;
   const int first = blockIdx.x / CG, step = gridDim.x / CG;
 
   // tile -> (row tile, column tile, first stage of K, stages of K); 16 tiles of the fast side at a time
@@ -144,8 +149,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int f = group * 16 + at % width, s = at / width;
     m = g.fast_m ? f : s;
     n = g.fast_m ? s : f;
-    k0 = split * g.k_split;
-    kn = max(0, min(g.k_split, k_iters - k0));
+    k0 = split * k_split;
+    kn = max(0, min(k_split, k_iters - k0));
   };
 
   if (warp == 4) {
@@ -157,20 +162,24 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int tile = first; tile < tiles && ok; tile += step) {
         int m, n, split, k0, kn;
         locate(tile, m, n, split, k0, kn);
-        const int row_a = g.a_row0 + m * TM + (int)rank * 128, row_b = g.b_row0 + n * BN + (int)rank * (BN / CG);
+        const int row_a = g.a_row0 + m * TM + (int)rank * 128;
+        // rows of A that nothing comes of stay what they were in shared memory: they reach no row but their own
+        const int boxes = A_MN || g.a_box == 128 ? 1 : max(1, min(4, (active - row_a + 31) / 32));
+        const uint32_t bytes = CG * STAGE - (A_MN || g.a_box == 128 ? 0 : A_BYTES - boxes * (A_BYTES / 4));
+        const int row_b = g.b_row0 + n * BN + (int)rank * (BN / CG);
         for (int k = 0; k < kn; ++k) {
           if (!bar_wait(empty + 8 * s, ph ^ 1)) {
             ok = false;
             break;
           }
           const uint32_t bar = CG == 1 ? full + 8 * s : peer_addr(full + 8 * s, 0);
-          if (rank == 0) bar_expect(full + 8 * s, CG * STAGE);
+          if (rank == 0) bar_expect(full + 8 * s, bytes);
           const uint32_t a = base + s * STAGE, b = a + A_BYTES;
           const int ka = (int)(g.a_k0 + (long long)(k0 + k) * BK), kb = (int)(g.b_k0 + (long long)(k0 + k) * BK);
           if constexpr (A_MN) {
             for (int i = 0; i < 2; ++i) tma_load<CG>(a + i * 8192, &map_a, bar, row_a + 64 * i, ka);
           } else {
-            tma_load<CG>(a, &map_a, bar, ka, row_a);
+            for (int i = 0; i < boxes; ++i) tma_load<CG>(a + i * (A_BYTES / 4), &map_a, bar, ka, row_a + 32 * i);
           }
           if constexpr (B_MN) {
             for (int i = 0; i < 4 / CG; ++i) tma_load<CG>(b + i * 8192, &map_b, bar, row_b + 64 * i, kb);
@@ -402,7 +411,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) put16(j, v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-            end_out(col0 + c, (int)(split * g.rows_pad) + warp_row, g.add != 0);
+            end_out(col0 + c, split * g.plan->part_rows + warp_row, g.add != 0);
           }
         }
       }
@@ -451,7 +460,9 @@ struct RowArgs {
   // finish
   const float* part32;
   long long ld32;
-  int splits;
+  int tile_rows, units;  // of its tiles, and how many are worked on at once
+  int k_piece;          // stages of K in a piece of the vocabulary
+  long long part_room;  // rows that all parts have together
   void* d_hidden;
   long long dh_ld;
 };
@@ -469,9 +480,22 @@ __device__ __forceinline__ unsigned bound_of(const RowCoef& k) {
   return __float_as_uint(fabsf(k.c1) + fabsf(k.c2) + fabsf(k.c3));
 }
 
+// Into how many ranges the hidden states' gradient cuts a piece's K.  Its time in stages of a tile (64 of K, 0.28 us):
+// whole rounds of tiles over the pairs of SMs, 16 stages to begin and empty a tile, and each part's way out to HBM and
+// back.  One thread tries one count.
+__device__ __forceinline__ unsigned split_time(const RowArgs& a, int active, int splits, int tile_rows, int units) {
+  const long long rows = (active + 255) / 256 * 256, tiles = (active + tile_rows - 1) / tile_rows * ((a.D + BN - 1) / BN);
+  if (splits > 1 && (splits * rows > a.part_room || splits * 4 > a.k_piece)) return 0xffffffffu;
+  const long long rounds = (tiles * splits + units - 1) / units;
+  const float part = (float)active * (float)a.D * 8.0f / 6.5e6f / 0.28f;
+  return (unsigned)fminf(4e9f, (float)rounds * (float)((a.k_piece + splits - 1) / splits + 16) + (float)splits * part);
+}
+
 // One block: packs the rows that count, in their order.  BACKWARD: their coefficients as well.
 template <bool BACKWARD>
 __global__ void __launch_bounds__(1024) lce_plan_kernel(const RowArgs a) {
+  depend_wait();
+  depend_launch();
   __shared__ int scratch[33];
   __shared__ unsigned most[33];
   int before = 0;
@@ -506,6 +530,20 @@ __global__ void __launch_bounds__(1024) lce_plan_kernel(const RowArgs a) {
     before += total;
   }
   if (BACKWARD) bound = block_reduce_max<unsigned>(bound, most);
+  if (threadIdx.x < 32 && a.part_room) {
+    unsigned best = split_time(a, before, threadIdx.x + 1, a.tile_rows, a.units), at = threadIdx.x + 1;
+    const unsigned more = split_time(a, before, threadIdx.x + 33, a.tile_rows, a.units);
+    if (more < best) {
+      best = more;
+      at = threadIdx.x + 33;
+    }
+    const unsigned least = warp_reduce_min<unsigned>(best);
+    at = warp_reduce_min<unsigned>(best == least ? at : 1000u);
+    if (threadIdx.x == 0) {
+      a.plan->splits = (int)at;
+      a.plan->part_rows = (before + 255) / 256 * 256;
+    }
+  }
   if (threadIdx.x == 0) {
     a.plan->active = before;
     a.plan->gmax = bound;
@@ -515,6 +553,8 @@ __global__ void __launch_bounds__(1024) lce_plan_kernel(const RowArgs a) {
 
 // The packed rows, behind them zeros to a whole tile.
 __global__ void __launch_bounds__(256) lce_gather_kernel(const RowArgs a) {
+  depend_wait();
+  depend_launch();
   const int active = a.plan->active, tile_end = (active + 255) / 256 * 256;
   const long long i = blockIdx.x;
   if (i >= tile_end) return;
@@ -539,6 +579,8 @@ template <bool GRADS>
 __global__ void __launch_bounds__(256) lce_join_kernel(const RowArgs a) {
   __shared__ float sm[8][8];
   __shared__ double ss[8][8], sz[8][8];
+  depend_wait();
+  depend_launch();
   const int r = threadIdx.x & 7, part = threadIdx.x >> 3, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int active = a.plan->active;
   const long long i = (long long)blockIdx.x * 8 + r;
@@ -591,20 +633,40 @@ __global__ void __launch_bounds__(256) lce_join_kernel(const RowArgs a) {
 }
 
 // The hidden states' gradient: the parts summed in their order, to the rows' own places; padded rows get zeros.
+// Four columns a thread, four parts at a time in flight.
 template <bool BF16>
 __global__ void __launch_bounds__(256) lce_finish_kernel(const RowArgs a) {
+  depend_wait();
+  depend_launch();
   const long long n = blockIdx.x;
-  const int i = a.place[n];
+  const int i = a.place[n], splits = a.plan->splits;
   uint16_t* to = (uint16_t*)a.d_hidden + n * a.dh_ld;
   const float scale = a.plan->failed ? NAN : pow2(-grad_shift<BF16>(a.plan));
-  const float* from = a.part32 + i * a.ld32;
-  for (long long d = threadIdx.x; d < a.D; d += 256) {
-    float v = 0.0f;
-    if (i >= 0) {
-      for (int s = 0; s < a.splits; ++s) v += from[s * a.rows_pad * a.ld32 + d];
-      v *= scale;
+  const long long part = (long long)a.plan->part_rows * a.ld32;
+  const float* from = a.part32 + (long long)max(i, 0) * a.ld32;
+  const bool whole = ((uintptr_t)to & 7) == 0;
+  for (long long d = threadIdx.x * 4; d < a.D; d += 1024) {
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (i >= 0) {  // (columns of a part are padded to four)
+#pragma unroll 4
+      for (int s = 0; s < splits; ++s) {
+        const float4 x = __ldcs((const float4*)(from + s * part + d));
+        v.x += x.x;
+        v.y += x.y;
+        v.z += x.z;
+        v.w += x.w;
+      }
     }
-    to[d] = (uint16_t)pack2<BF16>(v, 0.0f);
+    // a NaN scale marks a wait that gave up, in padded rows too
+    const uint2 w = make_uint2(pack2<BF16>(v.x * scale, v.y * scale), pack2<BF16>(v.z * scale, v.w * scale));
+    if (whole && d + 4 <= a.D) {
+      *(uint2*)(to + d) = w;
+    } else {
+      const uint16_t h[4] = {(uint16_t)w.x, (uint16_t)(w.x >> 16), (uint16_t)w.y, (uint16_t)(w.y >> 16)};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (d + j < a.D) to[d + j] = h[j];
+    }
   }
 }
 

@@ -75,6 +75,11 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
+// Waits for the kernel before this one in the stream (where it was launched to overlap with it), and lets the one
+// behind be launched: its blocks come in as this one's leave, and wait in turn.
+__device__ __forceinline__ void depend_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void depend_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // --- bulk tensor copies (x: the contiguous coordinate, always a multiple of 16 bytes here)
 
 __device__ __forceinline__ void tma_prefetch(const CUtensorMap* map) {
