@@ -63,7 +63,11 @@ int check_plain(const void* w, pesti_dtype dtype, int64_t V, int64_t D, int64_t 
   return PESTI_OK;
 }
 
-constexpr int PER = 4;
+// Blocks of a row that a team of lanes takes at once.
+template <typename T>
+constexpr int per(bool there) {
+  return there ? (sizeof(T) == 4 ? 2 : 4) : 4;
+}
 
 template <typename T, int GROUP>
 int convert(bool there, const void* w, int64_t V, int64_t D, int64_t ld, void* q, void* scale, cudaStream_t st) {
@@ -74,14 +78,16 @@ int convert(bool there, const void* w, int64_t V, int64_t D, int64_t ld, void* q
   a.scale = (__nv_bfloat16*)scale;
   a.D = (int)D;
   a.blocks = (int)blocks_of(D);
-  a.total = V * a.blocks;
-  a.vec = (uintptr_t)w % 16 == 0 && (V == 1 || ld * sizeof(T) % 16 == 0);
-  const long long grid = (a.total + 16 * PER - 1) / (16 * PER);
+  a.runs = (a.blocks + per<T>(there) - 1) / per<T>(there);
+  a.total = V * a.runs;
+  const int align = there || sizeof(T) == 4 ? 32 : 16, teams = there ? 32 : 16;  // of a thread block
+  a.vec = (uintptr_t)w % align == 0 && (V == 1 || ld * sizeof(T) % align == 0);
+  const long long grid = (a.total + teams - 1) / teams;
   if (grid > INT_MAX) return refuse("V * D too large");
   if (there)
-    q4_quantize_kernel<T, GROUP, PER><<<(unsigned)grid, 256, 0, st>>>(a);
+    q4_quantize_kernel<T, GROUP, per<T>(true)><<<(unsigned)grid, 256, 0, st>>>(a);
   else
-    q4_dequantize_kernel<T, GROUP, PER><<<(unsigned)grid, 256, 0, st>>>(a);
+    q4_dequantize_kernel<T, GROUP, per<T>(false)><<<(unsigned)grid, 256, 0, st>>>(a);
   return launched("q4 conversion launch");
 }
 

@@ -46,112 +46,230 @@ struct Held {
   long long ld;
   uint32_t* q;
   __nv_bfloat16* scale;
-  int D, blocks;     // of a row
-  long long total;   // blocks in all
-  int vec;           // whole vectors of 8 columns can be read or written
+  int D, blocks, runs;  // blocks of a row, and runs of PER blocks that half a warp takes
+  long long total;      // runs in all
+  int vec;              // whole vectors of 8 columns can be read or written
 };
 
-// Eight columns from `at`; 0 behind the row's end.
-template <typename T>
-__device__ __forceinline__ void load8(const T* row, int at, int D, bool vec, float (&v)[8]) {
-  if (vec && at + 8 <= D) {
-    uint4 raw[sizeof(T) / 2];
+// The row and the first block of a team of LANES lanes.
+template <typename T, int PER, int LANES>
+__device__ __forceinline__ bool place_of(const Held<T>& a, long long& row, int& block) {
+  const long long run = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  row = a.total >> 32 ? run / a.runs : (uint32_t)run / (uint32_t)a.runs;
+  block = (int)(run - row * a.runs) * PER;
+  return run < a.total;
+}
+
+// Quotients w / s as codes q + 8, rounded to whole numbers, halves to even, exactly.  t = 384 + w / s to 2^-15 (the
+// spacing of numbers about 384), off by at most 2^-20 before that, since |w / s| < 8.1; adding 1.5 * 2^23 rounds it to
+// whole numbers, which the sum's last bits hold.
+//  16-bit w: of 11 bits, and s of 8, so that a quotient that is no half is at least 2^-13 from one: rounding to 2^-15
+//  brings back the halves and moves nothing across one.
+//  f32 w: quotients within 2^-14 of a half are looked at again, with the exact remainder (w has 24 bits, q s at most
+//  12, and a quotient off by less than one leaves an f32).
+constexpr float WHOLE = 12582912.0f;  // 1.5 * 2^23
+
+__device__ __forceinline__ uint32_t codes_of(const float (&v)[8], float s, bool check) {
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  uint32_t word = 0;
+  float far = 0.0f;
+  // (the eight sums' upper bits, 0x4b400000, add up to this constant)
+  constexpr uint32_t UPPER = 0x4b400000u + (0x4b400000u << 4) + (0x4b400000u << 8);
 #pragma unroll
-    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) raw[i] = __ldcs((const uint4*)(row + at) + i);
-    const T* p = (const T*)raw;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_f32(p[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = at + i < D ? to_f32(row[at + i]) : 0.0f;
+  for (int j = 7; j >= 0; --j) {
+    const float t = fminf(fmaf(v[j], inv, 384.0f), 391.0f), c = t + (WHOLE + 8.0f - 384.0f);
+    word = (word << 4) + fbits(c);
+    if (check) far = fmaxf(far, fabsf((c - (WHOLE + 8.0f - 384.0f)) - t));
   }
+  word -= UPPER;
+  if (check && far >= 0.5f - 0x1p-14f) {
+    word = 0;
+#pragma unroll 1
+    for (int j = 7; j >= 0; --j) {
+      float w = v[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i)
+        if (i == j) w = v[i];
+      float q = rintf(w * inv);
+      const float r = fmaf(-q, s, w), r2 = 2.0f * fabsf(r), a = fabsf(s);
+      if (r2 > a || (r2 == a && ((int)q & 1))) q += (r > 0.0f) == (s > 0.0f) ? 1.0f : -1.0f;
+      word = (word << 4) + (uint32_t)((int)fminf(q, 7.0f) + 8);
+    }
+  }
+  return word;
 }
 
-// The nearest whole number to w / s, halves to even: the product's rounding is checked with the exact remainder (w has
-// 24 bits, q s at most 12, and the remainder of a quotient off by less than one is an f32).
-__device__ __forceinline__ float round_quotient(float w, float s, float inv) {
-  float q = rintf(w * inv);
-  const float r = fmaf(-q, s, w), r2 = 2.0f * fabsf(r), a = fabsf(s);
-  if (r2 > a || (r2 == a && (((int)q) & 1))) q += (r > 0.0f) == (s > 0.0f) ? 1.0f : -1.0f;
-  return q;
+// The larger of two pairs, NaN where one of them is.
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b, bool f16) {
+  uint32_t r;
+  if (f16)
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 
-// Sixteen lanes a block of 128 columns, 8 columns and one word each; PER blocks at once for the loads in flight.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Sixteen columns of a lane as they were read: f32, or pairs of 16 bits.
+template <typename T>
+struct Sixteen {
+  static constexpr int WORDS = 4 * sizeof(T);
+  uint32_t v[WORDS];
+
+  __device__ __forceinline__ void load(const T* row, int at, int D, bool vec) {
+    if (vec && at + 16 <= D) {
+#pragma unroll
+      for (int i = 0; i < WORDS; i += 8)
+        asm volatile("ld.global.cs.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]),
+                       "=r"(v[i + 6]), "=r"(v[i + 7])
+                     : "l"((const uint32_t*)(row + at) + i));
+    } else {
+      T* p = (T*)v;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) p[i] = at + i < D ? row[at + i] : from_f32<T>(0.0f);
+    }
+  }
+
+  __device__ __forceinline__ float at(int i) const { return to_f32(((const T*)v)[i]); }
+
+  // The largest value and the largest negated one of GROUP / 16 lanes' columns.
+  template <int GROUP>
+  __device__ __forceinline__ void ends(float& hi, float& neg) const {
+    if constexpr (sizeof(T) == 4) {
+      hi = bitsf(v[0]);
+      neg = -hi;
+#pragma unroll
+      for (int i = 1; i < WORDS; ++i) {
+        hi = max_nan(hi, bitsf(v[i]));
+        neg = max_nan(neg, -bitsf(v[i]));
+      }
+#pragma unroll
+      for (int o = 1; o < GROUP / 16; o <<= 1) {
+        hi = max_nan(hi, __shfl_xor_sync(PESTI_FULL_MASK, hi, o));
+        neg = max_nan(neg, __shfl_xor_sync(PESTI_FULL_MASK, neg, o));
+      }
+    } else {
+      constexpr bool F16 = std::is_same<T, __half>::value;
+      constexpr uint32_t SIGNS = 0x80008000u;
+      uint32_t a = v[0], b = v[0] ^ SIGNS;
+#pragma unroll
+      for (int i = 1; i < WORDS; ++i) {
+        a = max2_nan(a, v[i], F16);
+        b = max2_nan(b, v[i] ^ SIGNS, F16);
+      }
+      uint32_t both = max2_nan(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632), F16);  // (value, negated)
+#pragma unroll
+      for (int o = 1; o < GROUP / 16; o <<= 1) both = max2_nan(both, __shfl_xor_sync(PESTI_FULL_MASK, both, o), F16);
+      const T* p = (const T*)&both;
+      hi = to_f32(p[0]);
+      neg = to_f32(p[1]);
+    }
+  }
+};
+
+// Eight lanes a block of 128 columns, 16 columns and two words each; PER blocks at once for the loads in flight.  The
+// 16-bit forms are bound by instructions (10 a column; 8 columns a lane took 19 more a column): 128256 x 4096 bf16, see
+// q4_dequantize_kernel for the way back.
 template <typename T, int GROUP, int PER>
 __global__ void __launch_bounds__(256) q4_quantize_kernel(const Held<T> a) {
-  const int half = threadIdx.x >> 4, i = threadIdx.x & 15, lane = threadIdx.x & 31;
-  const long long b0 = ((long long)blockIdx.x * 16 + half) * PER;
-  float v[PER][8];
+  const int i = threadIdx.x & 7, lane = threadIdx.x & 31;
+  long long row;
+  int b0;
+  const bool there = place_of<T, PER, 8>(a, row, b0);
+  const int n = there ? min(PER, a.blocks - b0) : 0;
+  Sixteen<T> in[PER];
+  const T* from = a.w + row * a.ld;
+#pragma unroll
+  for (int u = 0; u < PER; ++u)
+    if (u < n) in[u].load(from, (b0 + u) * BLOCK + 16 * i, a.D, a.vec);
+  const long long b = row * a.blocks + b0;
+  uint32_t* to = a.q + b * (BLOCK / 8) + word_of(2 * i);  // (the other word is 4 behind it)
+  __nv_bfloat16* scale = a.scale + b * (BLOCK / GROUP) + i / (GROUP / 16);
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
-    const long long b = b0 + u;
-    if (b < a.total) {
-      const long long row = b / a.blocks;
-      load8(a.w + row * a.ld, (int)(b - row * a.blocks) * BLOCK + 8 * i, a.D, a.vec, v[u]);
+    float hi, neg;
+    in[u].template ends<GROUP>(hi, neg);
+    float m = hi > neg ? hi : -neg;
+    if (__any_sync(PESTI_FULL_MASK, hi == neg)) {  // both signs: the one that comes first
+      int first = 32 * 32;
+#pragma unroll
+      for (int j = 15; j >= 0; --j)
+        if (fabsf(in[u].at(j)) == hi) first = 2 * (16 * lane + j) + (in[u].at(j) < 0.0f ? 1 : 0);
+#pragma unroll
+      for (int o = 1; o < GROUP / 16; o <<= 1) first = min(first, __shfl_xor_sync(PESTI_FULL_MASK, first, o));
+      if (hi == neg) m = first & 1 ? -hi : hi;
     }
-  }
-#pragma unroll
-  for (int u = 0; u < PER; ++u) {
-    const long long b = b0 + u;
-    float m = v[u][0];
-#pragma unroll
-    for (int j = 1; j < 8; ++j)
-      if ((fbits(v[u][j]) & 0x7fffffffu) > (fbits(m) & 0x7fffffffu)) m = v[u][j];
-#pragma unroll
-    for (int o = 1; o < GROUP / 8; o <<= 1) {
-      const float other = __shfl_xor_sync(PESTI_FULL_MASK, m, o);
-      const uint32_t x = fbits(other) & 0x7fffffffu, y = fbits(m) & 0x7fffffffu;
-      if (x > y || (x == y && (lane & o))) m = other;
-    }
-    if (b >= a.total) continue;
+    if (u >= n) continue;
     __nv_bfloat16 held = __float2bfloat16_rn(m * -0.125f);
     float s = __bfloat162float(held);
-    uint32_t word = 0x88888888u;
+    uint32_t word[2] = {0x88888888u, 0x88888888u};
     if (!isfinite(m)) {
       held = __float2bfloat16_rn(NAN);
     } else if (s != 0.0f) {
-      const float up = fabsf(s) < 0x1p-100f ? 0x1p64f : 1.0f;  // 1 / s is finite then
-      s *= up;
-      const float inv = 1.0f / s;
-      word = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float q = fminf(7.0f, fmaxf(-8.0f, round_quotient(v[u][j] * up, s, inv)));
-        word |= (uint32_t)((int)q + 8) << (4 * j);
+      for (int h = 0; h < 2; ++h) {
+        float v[8], t = s;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = in[u].at(8 * h + j);
+        if (fabsf(s) < 0x1p-100f) {  // so that 1 / s is finite, and quotients by subnormal scales at most 8
+          t = s * 0x1p64f;
+          const float most = 8.0f * fabsf(t);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = fminf(most, fmaxf(-most, v[j] * 0x1p64f));
+        }
+        word[h] = codes_of(v, t, sizeof(T) == 4);
       }
     }
-    a.q[b * (BLOCK / 8) + word_of(i)] = word;
-    if (i % (GROUP / 8) == 0) a.scale[b * (BLOCK / GROUP) + i / (GROUP / 8)] = held;
+    to[u * (BLOCK / 8)] = word[0];
+    to[u * (BLOCK / 8) + 4] = word[1];
+    if (i % (GROUP / 16) == 0) scale[u * (BLOCK / GROUP)] = held;
   }
 }
 
+// Two lanes of a team of sixteen hold neighbouring words; f32 rows are written 32 bytes a lane, 16-bit ones 16.
 template <typename T, int GROUP, int PER>
 __global__ void __launch_bounds__(256) q4_dequantize_kernel(const Held<T> a) {
-  const int half = threadIdx.x >> 4, i = threadIdx.x & 15;
-  const long long b0 = ((long long)blockIdx.x * 16 + half) * PER;
+  const int i = threadIdx.x & 15;
+  long long row;
+  int b0;
+  if (!place_of<T, PER, 16>(a, row, b0)) return;
+  const int n = min(PER, a.blocks - b0);
+  const long long b = row * a.blocks + b0;
+  const uint32_t* from = a.q + b * (BLOCK / 8) + word_of(i);
+  const __nv_bfloat16* scale = a.scale + b * (BLOCK / GROUP) + i / (GROUP / 8);
   uint32_t w[PER];
   float s[PER];
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
-    if (b0 + u < a.total) {
-      w[u] = a.q[(b0 + u) * (BLOCK / 8) + word_of(i)];
-      s[u] = __bfloat162float(a.scale[(b0 + u) * (BLOCK / GROUP) + i / (GROUP / 8)]);
+    if (u < n) {
+      w[u] = __ldcs(from + u * (BLOCK / 8));
+      s[u] = __bfloat162float(scale[u * (BLOCK / GROUP)]);
     }
   }
+  T* to = const_cast<T*>(a.w) + row * a.ld;
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
-    const long long b = b0 + u;
-    if (b >= a.total) continue;
-    const long long row = b / a.blocks;
-    const int at = (int)(b - row * a.blocks) * BLOCK + 8 * i;
-    T* to = const_cast<T*>(a.w) + row * a.ld;
-    uint4 raw[sizeof(T) / 2];
+    if (u >= n) continue;
+    const int at = (b0 + u) * BLOCK + 8 * i;
+    uint32_t raw[2 * sizeof(T)];
     T* v = (T*)raw;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = from_f32<T>((float)((int)((w[u] >> (4 * j)) & 15) - 8) * s[u]);
+    for (int j = 0; j < 8; ++j)  // 2^23 + 8 + q from the nibble, less 2^23 + 8
+      v[j] = from_f32<T>((bitsf(((w[u] >> (4 * j)) & 15u) | 0x4b000000u) - 8388616.0f) * s[u]);
     if (a.vec && at + 8 <= a.D) {
-#pragma unroll
-      for (int j = 0; j < (int)(sizeof(T) / 2); ++j) __stcs((uint4*)(to + at) + j, raw[j]);
+      if constexpr (sizeof(T) == 4)
+        asm volatile("st.global.cs.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + at), "r"(raw[0]),
+                     "r"(raw[1]), "r"(raw[2]), "r"(raw[3]), "r"(raw[4]), "r"(raw[5]), "r"(raw[6]), "r"(raw[7])
+                     : "memory");
+      else
+        __stcs((uint4*)(to + at), make_uint4(raw[0], raw[1], raw[2], raw[3]));
     } else {
       for (int j = 0; j < 8 && at + j < a.D; ++j) to[at + j] = v[j];
     }
