@@ -106,47 +106,103 @@ int convert(bool there, pesti_dtype dtype, int64_t group, const void* w, int64_t
   return convert<__half>(there, group, w, V, D, ld, q, scale, st);
 }
 
-// Column tiles of a pass over the weight, and the rows of x that fill them.
-int column_tiles(int64_t columns) { return columns <= 8 ? 1 : columns <= 16 ? 2 : columns <= 32 ? 4 : 8; }
+constexpr int MOST_ROWS = 64;           // of x, a pass over the weight
+constexpr int SHARED_BYTES = 200 << 10;  // for x
+constexpr int SMS = 148;
+
+int column_tiles(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 ? 4 : 8; }
 
 int pieces_of(pesti_dtype d) { return d == PESTI_F32 ? 3 : 1; }
 
-long long frag_bytes(int64_t D, int tiles) { return blocks_of(D) * 4 * tiles * 32 * 16; }
+// Bytes of fragments of a block of x.
+long long block_bytes(int pieces, int columns) { return 16LL * pieces * columns * 16; }
 
-template <typename T, int GROUP, int NT>
+bool fits_whole(int64_t D, int pieces, int64_t rows) {
+  return blocks_of(D) * block_bytes(pieces, (int)rows) <= SHARED_BYTES && rows <= 16;
+}
+
+// How a pass shares its tiles and their K out: the least time of the busiest SM, by the weight's bytes that it reads (44
+// bytes a nanosecond) and a microsecond and a half per round of tiles, where few warps have too little in flight.
+void share_out(LogitArgs& a, int nt, int sms) {
+  double best = 1e30;
+  for (int kw = 1; kw <= 8 && kw <= a.blocks; kw *= 2) {
+    for (int w = kw; w <= most_warps(nt); w += kw) {
+      const int slots = w / kw;
+      const long long rounds = (a.tiles + (long long)sms * slots - 1) / ((long long)sms * slots);
+      const double bytes = (double)rounds * slots * a.blocks * (ROWS * BLOCK_BYTES);
+      const double t = bytes / (w >= 12 ? 44.0 : 44.0 * w / 12) + 1500.0 * rounds + (kw > 1 ? 300.0 * rounds : 0.0);
+      if (t < best) {
+        best = t;
+        a.warps = w;
+        a.k_warps = kw;
+      }
+    }
+  }
+}
+
+template <typename... K, typename... A>
+int launch(const char* what, void (*kernel)(K...), long long blocks, int threads, int smem, cudaStream_t st,
+           const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, K(args)...);
+  return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, what);
+}
+
+template <typename T, int GROUP, int NT, bool RING>
 int logits_pass(LogitArgs a, cudaStream_t st) {
-  q4_fragments_kernel<T, NT><<<(unsigned)a.blocks, 128, 0, st>>>(a);
-  int rc = launched("q4_fragments_kernel launch");
-  if (rc) return rc;
-  a.k_warps = a.blocks >= 16 ? 8 : a.blocks >= 8 ? 4 : a.blocks >= 4 ? 2 : 1;
-  const int rows = WARPS / a.k_warps * ROWS;
-  q4_logits_kernel<std::is_same<T, __half>::value, GROUP, NT>
-      <<<(unsigned)((a.V + rows - 1) / rows), WARPS * 32, 0, st>>>(a);
-  return launched("q4_logits_kernel launch");
+  constexpr int P = sizeof(T) == 4 ? 3 : 1;
+  share_out(a, NT, SMS);
+  long long smem = 0;
+  if (RING) {
+    const int rc = launch("q4_fragments_kernel launch", q4_fragments_kernel<T>, a.blocks, 256, 0, st, a, 8 * NT);
+    if (rc) return rc;
+    const long long block = block_bytes(P, 8 * NT);
+    a.stage_blocks = a.k_warps;  // a block for each warp of a tile
+    a.stages = (int)std::min<long long>(8, SHARED_BYTES / (block * a.stage_blocks));
+    smem = a.stages * a.stage_blocks * block;
+  } else {
+    smem = a.blocks * block_bytes(P, a.rows);
+  }
+  smem += (long long)(a.warps - a.warps / a.k_warps) * 8 * NT * 32 * 4;
+  auto kernel = q4_logits_kernel<T, GROUP, NT, RING>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return pesti_set_cuda_error(e, "q4_logits_kernel shared memory");
+  const int slots = a.warps / a.k_warps;
+  return launch("q4_logits_kernel launch", kernel, std::min<long long>(SMS, (a.tiles + slots - 1) / slots),
+                (a.warps + (RING ? 1 : 0)) * 32, (int)smem, st, a);
 }
 
 template <typename T, int GROUP>
-int logits_tiles(const LogitArgs& a, int tiles, cudaStream_t st) {
-  if (tiles == 1) return logits_pass<T, GROUP, 1>(a, st);
-  if (tiles == 2) return logits_pass<T, GROUP, 2>(a, st);
-  if (tiles == 4) return logits_pass<T, GROUP, 4>(a, st);
-  return logits_pass<T, GROUP, 8>(a, st);
+int logits_tiles(const LogitArgs& a, cudaStream_t st) {
+  const bool whole = fits_whole(a.D, sizeof(T) == 4 ? 3 : 1, a.rows);
+  switch (column_tiles(a.rows)) {
+    case 1: return whole ? logits_pass<T, GROUP, 1, false>(a, st) : logits_pass<T, GROUP, 1, true>(a, st);
+    case 2: return whole ? logits_pass<T, GROUP, 2, false>(a, st) : logits_pass<T, GROUP, 2, true>(a, st);
+    case 4: return logits_pass<T, GROUP, 4, true>(a, st);
+    default: return logits_pass<T, GROUP, 8, true>(a, st);
+  }
 }
 
 template <typename T>
 int logits(LogitArgs a, int64_t group, int64_t B, pesti_dtype out, cudaStream_t st) {
   const char* x = (const char*)a.x;
   char* y = (char*)a.y;
-  const int most = 64 / a.pieces;
-  for (int64_t r = 0; r < B; r += most) {
-    a.rows = (int)std::min<int64_t>(most, B - r);
-    a.columns = a.rows * a.pieces;
+  for (int64_t r = 0; r < B; r += MOST_ROWS) {
+    a.rows = (int)std::min<int64_t>(MOST_ROWS, B - r);
     a.x = x + r * a.x_ld * sizeof(T);
     a.y = y + r * a.y_ld * esize(out);
-    const int tiles = column_tiles(a.columns);
-    const int rc = group == 32   ? logits_tiles<T, 32>(a, tiles, st)
-                   : group == 64 ? logits_tiles<T, 64>(a, tiles, st)
-                                 : logits_tiles<T, 128>(a, tiles, st);
+    const int rc = group == 32   ? logits_tiles<T, 32>(a, st)
+                   : group == 64 ? logits_tiles<T, 64>(a, st)
+                                 : logits_tiles<T, 128>(a, st);
     if (rc) return rc;
   }
   return PESTI_OK;
@@ -177,8 +233,9 @@ int64_t pesti_q4_logits_workspace(pesti_dtype dtype, int64_t B, int64_t D) {
   if (B < 0) return refuse("B < 0");
   if (B > 1 << 24) return refuse("B must be at most 2^24");
   if (D < 1 || D > 1 << 20) return refuse("D must be 1 to 2^20");
-  const int p = pieces_of(dtype);
-  return frag_bytes(D, column_tiles(std::min<int64_t>(B, 64 / p) * p));
+  const int64_t rows = std::min<int64_t>(B, MOST_ROWS);
+  if (B <= MOST_ROWS && fits_whole(D, pieces_of(dtype), rows)) return 256;
+  return blocks_of(D) * block_bytes(pieces_of(dtype), 8 * column_tiles(rows));
 }
 
 int pesti_q4_logits(const void* d_x, pesti_dtype dtype, int64_t B, int64_t D, int64_t x_ld, const void* d_q,
@@ -208,11 +265,11 @@ int pesti_q4_logits(const void* d_x, pesti_dtype dtype, int64_t B, int64_t D, in
   a.x = d_x;
   a.x_ld = x_ld;
   a.D = (int)D;
-  a.pieces = pieces_of(dtype);
   a.q = (const uint4*)d_q;
   a.scale = (const __nv_bfloat16*)d_scale;
   a.V = (int)V;
   a.blocks = (int)blocks_of(D);
+  a.tiles = (int)((V + ROWS - 1) / ROWS);
   a.frags = (uint4*)d_ws;
   a.y = d_logits;
   a.y_ld = ld;

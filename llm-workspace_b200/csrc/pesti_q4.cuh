@@ -10,7 +10,10 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "pesti_common.cuh"
+#include "pesti_umma.cuh"
 
 namespace pesti_q4 {
 
@@ -281,50 +284,58 @@ __global__ void __launch_bounds__(256) q4_dequantize_kernel(const Held<T> a) {
 struct LogitArgs {
   const void* x;
   long long x_ld;
-  int rows, D, pieces, columns;  // columns = rows * pieces: f32 rows are three bf16 ones
+  int rows, D;  // of x; at most 64 rows
   const uint4* q;
   const __nv_bfloat16* scale;
-  int V, blocks;
-  uint4* frags;  // [blocks][4][NT][32]
+  int V, blocks, tiles;  // 32 rows of the weight a tile
+  uint4* frags;          // [blocks][4][pieces][8 NT][4], where x does not fit shared memory whole
   void* y;
   long long y_ld;
-  int out;  // 0 f32, 1 bf16, 2 f16
-  int k_warps;
+  int out;               // 0 f32, 1 bf16, 2 f16
+  int warps, k_warps;    // warps that multiply, and how many of them share a tile's K
+  int stage_blocks, stages;
 };
 
-// x as the products' fragments: word j of a block and column tile n, lane (column g, t): the pairs that a word of
-// weights unpacks to.  f32 is cut into three bf16 whose sum it is, exactly.
-template <typename T, int NT>
-__global__ void __launch_bounds__(128) q4_fragments_kernel(const LogitArgs a) {
-  const int b = blockIdx.x, j = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  for (int n = 0; n < NT; ++n) {
-    const int c = n * 8 + g, row = c / a.pieces, piece = c - row * a.pieces;
-    uint16_t v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int d = b * BLOCK + 32 * j + 8 * t + i;
-      v[i] = 0;
-      if (row >= a.rows || d >= a.D) continue;
-      const T x = ((const T*)a.x)[row * a.x_ld + d];
-      if constexpr (sizeof(T) == 2) {
-        v[i] = *(const uint16_t*)&x;
-      } else {
-        float rest = x;
-        uint32_t bits = fbits(rest);
-        for (int p = 0; p < piece; ++p) {
-          const bool whole = (bits & 0x7f800000u) == 0x7f800000u;  // inf and NaN are in the first piece
-          rest = whole ? 0.0f : rest - bitsf(bits & 0xffff0000u);
-          bits = fbits(rest);
-        }
-        v[i] = (uint16_t)(bits >> 16);
-        if (is_nan(rest)) v[i] |= 0x40;
-      }
+// The bf16 or f16 bits of piece `p` of an x: f32 is cut into three bf16 whose sum it is, exactly.
+template <typename T>
+__device__ __forceinline__ uint32_t piece_of(T x, int p) {
+  if constexpr (sizeof(T) == 2) {
+    return *(const uint16_t*)&x;
+  } else {
+    float rest = x;
+    uint32_t bits = fbits(rest);
+    for (int i = 0; i < p; ++i) {
+      const bool whole = (bits & 0x7f800000u) == 0x7f800000u;  // inf and NaN are in the first piece
+      rest = whole ? 0.0f : rest - bitsf(bits & 0xffff0000u);
+      bits = fbits(rest);
     }
-    uint4 f;
-    uint32_t* p = (uint32_t*)&f;
+    return bits >> 16 | (is_nan(rest) ? 0x40u : 0u);
+  }
+}
+
+// Four pairs of x for lane t of a quad, word j of block b: columns 32 j + 8 t + (i, i + 4), as a word of weights unpacks.
+template <typename T>
+__device__ __forceinline__ uint4 fragment_of(const T* row, int b, int j, int t, int piece, int D) {
+  const int at = b * BLOCK + 32 * j + 8 * t;
+  uint32_t v[8], f[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = (uint32_t)v[i] | (uint32_t)v[i + 4] << 16;
-    a.frags[((long long)(b * 4 + j) * NT + n) * 32 + lane] = f;
+  for (int i = 0; i < 8; ++i) v[i] = at + i < D ? piece_of(row[at + i], piece) : 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = v[i] | v[i + 4] << 16;
+  return make_uint4(f[0], f[1], f[2], f[3]);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) q4_fragments_kernel(const LogitArgs a, int columns) {
+  pesti_umma::depend_wait();
+  pesti_umma::depend_launch();
+  constexpr int P = sizeof(T) == 4 ? 3 : 1;
+  const int per_block = 16 * P * columns;
+  for (int e = threadIdx.x; e < per_block; e += 256) {
+    const int t = e & 3, c = (e >> 2) % columns, jp = (e >> 2) / columns, p = jp % P, j = jp / P;
+    uint4 f = make_uint4(0, 0, 0, 0);
+    if (c < a.rows) f = fragment_of((const T*)a.x + c * a.x_ld, blockIdx.x, j, t, p, a.D);
+    a.frags[(long long)blockIdx.x * per_block + e] = f;
   }
 }
 
@@ -357,64 +368,159 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-constexpr int WARPS = 8;
-constexpr int ROWS = 32;  // of the weight, per warp
+constexpr int ROWS = 32;  // of the weight, per warp and tile
 
-__device__ __forceinline__ void store_logit(const LogitArgs& a, int row, int v, float y) {
-  const long long at = row * a.y_ld + v;
-  if (a.out == 0)
-    ((float*)a.y)[at] = y;
-  else if (a.out == 1)
-    ((__nv_bfloat16*)a.y)[at] = __float2bfloat16_rn(y);
-  else
-    ((__half*)a.y)[at] = __float2half_rn(y);
+__host__ __device__ constexpr int most_warps(int nt) { return nt <= 2 ? 15 : nt == 4 ? 11 : 7; }
+
+// A lane's weights of one block: 16 bytes of four rows (8 apart), and their groups' scales.
+template <int GROUP>
+struct Weights {
+  uint4 w[4];
+  uint2 s[4];  // up to four bf16
+
+  __device__ __forceinline__ void load(const uint4* const (&q)[4], const __nv_bfloat16* const (&sc)[4], int b) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = __ldcs(q[i] + b * (BLOCK_BYTES / 16));
+      const __nv_bfloat16* p = sc[i] + b * (BLOCK / GROUP);
+      if constexpr (GROUP == 32)
+        s[i] = __ldg((const uint2*)p);
+      else if constexpr (GROUP == 64)
+        s[i].x = __ldg((const uint32_t*)p);
+      else
+        s[i].x = __ldg((const uint16_t*)p);
+    }
+  }
+
+  __device__ __forceinline__ float scale(int i, int g) const {
+    const uint32_t v = g < 2 ? s[i].x : s[i].y;
+    return bitsf(g & 1 ? v & 0xffff0000u : v << 16);
+  }
+};
+
+__device__ __forceinline__ void multipliers_sync(int threads) {
+  asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");
 }
 
-// A warp multiplies 32 rows of the weight by all columns over its share of K; the k_warps warps of a row tile join
-// their sums in shared memory, in their order.
-template <bool F16, int GROUP, int NT>
-__global__ void __launch_bounds__(WARPS * 32) q4_logits_kernel(const LogitArgs a) {
-  __shared__ float sums[WARPS][8][ROWS + 1];  // a column tile at a time
+// A warp multiplies 32 rows of the weight by all columns of x over its share of K (every k_warps-th block), and goes on
+// to its next tile; the k_warps warps of a tile join their sums in shared memory, in their order.  Blocks of weights are
+// loaded two ahead of their products.  Columns past x's last row hold zeros.
+// RING: x passes through shared memory in stages, copied by a warp of its own, again for every round of tiles.
+// Otherwise x is laid out there once, by all warps, while the first weights are on their way.
+template <typename T, int GROUP, int NT, bool RING>
+__global__ void __launch_bounds__((most_warps(NT) + 1) * 32) q4_logits_kernel(const LogitArgs a) {
+  using namespace pesti_umma;
+  constexpr bool F16 = std::is_same<T, __half>::value;
+  constexpr int P = sizeof(T) == 4 ? 3 : 1, COLUMNS = 8 * NT;
+  extern __shared__ uint4 xs[];
+  __shared__ uint64_t bars[16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int kw = a.k_warps, wr = WARPS / kw, part = warp % kw, tile = warp / kw;
-  const int row0 = (blockIdx.x * wr + tile) * ROWS;
-  const int b0 = a.blocks * part / kw, b1 = a.blocks * (part + 1) / kw;
+  const int kw = a.k_warps, slots = a.warps / kw, part = warp % kw, slot = warp / kw;
+  const int columns = RING ? COLUMNS : a.rows;  // in shared memory
+  const int per_block = 16 * P * columns;       // 16-byte fragments of a block of x
+  const int rounds = (a.tiles + gridDim.x * slots - 1) / (gridDim.x * slots);
+  const uint32_t full = smem_addr(bars), empty = full + 64;
+  float* sums = (float*)(xs + (long long)(RING ? a.stages * a.stage_blocks : a.blocks) * per_block);
+
+  if (RING && threadIdx.x == 0) {
+    for (int s = 0; s < a.stages; ++s) {
+      bar_init(full + 8 * s, 1);
+      bar_init(empty + 8 * s, a.warps);
+    }
+    bar_init_fence();
+  }
+  if (RING) __syncthreads();
+  depend_launch();
+
+  if (RING && warp == a.warps) {  // copies x
+    if (lane == 0) {
+      depend_wait();
+      int s = 0, ph = 0;
+      bool ok = true;
+      for (int r = 0; r < rounds && ok; ++r) {
+        for (int b = 0; b < a.blocks; b += a.stage_blocks) {
+          ok = bar_wait(empty + 8 * s, ph ^ 1);
+          if (!ok) break;
+          const uint32_t bytes = min(a.stage_blocks, a.blocks - b) * per_block * 16;
+          bar_expect(full + 8 * s, bytes);
+          bulk_load(smem_addr(xs + (long long)s * a.stage_blocks * per_block), a.frags + (long long)b * per_block,
+                    full + 8 * s, bytes);
+          if (++s == a.stages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+    }
+    return;
+  }
+
+  // the next block to load: its tile's round, and its place
   const uint4* q[4];
   const __nv_bfloat16* sc[4];
+  auto rows_of = [&](int round) {
+    const int tile = min(((int)blockIdx.x + round * (int)gridDim.x) * slots + slot, a.tiles - 1);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const long long row = min(row0 + g + 8 * i, a.V - 1);
-    q[i] = a.q + (row * a.blocks) * (BLOCK_BYTES / 16) + t;
-    sc[i] = a.scale + (row * a.blocks) * (BLOCK / GROUP);
+    for (int i = 0; i < 4; ++i) {
+      const long long row = min(tile * ROWS + g + 8 * i, a.V - 1);
+      q[i] = a.q + (row * a.blocks) * (BLOCK_BYTES / 16) + t;
+      sc[i] = a.scale + (row * a.blocks) * (BLOCK / GROUP);
+    }
+  };
+  int load_round = 0, load_b = part;
+  rows_of(0);
+  Weights<GROUP> held[2];
+  auto load = [&](Weights<GROUP>& w) {
+    if (load_round >= rounds) return;
+    w.load(q, sc, load_b);
+    load_b += kw;
+    if (load_b >= a.blocks) {
+      load_b = part;
+      if (++load_round < rounds) rows_of(load_round);
+    }
+  };
+  load(held[0]);
+  load(held[1]);
+
+  if (!RING) {
+    depend_wait();
+    for (int e = threadIdx.x; e < a.blocks * per_block; e += a.warps * 32) {
+      const int tt = e & 3, rest = e >> 2, c = rest % columns, bjp = rest / columns, p = bjp % P, bj = bjp / P;
+      xs[e] = fragment_of((const T*)a.x + c * a.x_ld, bj >> 2, bj & 3, tt, p, a.D);
+    }
+    __syncthreads();
   }
-  float acc[2][NT][4] = {};
-  if (row0 < a.V) {
-    for (int b = b0; b < b1; ++b) {
-      uint4 w[4];
+
+  float acc[2][NT][4];
+  int s = 0, ph = 0, which = 0;
+  bool ok = true;
+
+  // the products of block b with the fragments at `x`
+  auto multiply = [&](Weights<GROUP>& w, const uint4* x) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = __ldcs(q[i] + b * (BLOCK_BYTES / 16));
+    for (int gr = 0; gr < BLOCK / GROUP; ++gr) {
+      float part_acc[2][NT][4] = {};
 #pragma unroll
-      for (int gr = 0; gr < BLOCK / GROUP; ++gr) {
-        float part_acc[2][NT][4] = {};
+      for (int jj = 0; jj < GROUP / 32; ++jj) {
+        const int j = gr * (GROUP / 32) + jj;
+        uint32_t fa[2][2][4];
 #pragma unroll
-        for (int jj = 0; jj < GROUP / 32; ++jj) {
-          const int j = gr * (GROUP / 32) + jj;
-          uint32_t word[4];
+        for (int m = 0; m < 2; ++m)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) word[i] = ((const uint32_t*)&w[i])[j];
-          uint32_t fa[2][2][4];
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t w0 = ((const uint32_t*)&w.w[2 * m])[j], w1 = ((const uint32_t*)&w.w[2 * m + 1])[j];
+            fa[m][h][0] = unpack<F16>(w0, 2 * h);
+            fa[m][h][1] = unpack<F16>(w1, 2 * h);
+            fa[m][h][2] = unpack<F16>(w0, 2 * h + 1);
+            fa[m][h][3] = unpack<F16>(w1, 2 * h + 1);
+          }
 #pragma unroll
-          for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              fa[m][h][0] = unpack<F16>(word[2 * m], 2 * h);
-              fa[m][h][1] = unpack<F16>(word[2 * m + 1], 2 * h);
-              fa[m][h][2] = unpack<F16>(word[2 * m], 2 * h + 1);
-              fa[m][h][3] = unpack<F16>(word[2 * m + 1], 2 * h + 1);
-            }
+        for (int p = 0; p < P; ++p) {
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const uint4 f = a.frags[((long long)(b * 4 + j) * NT + n) * 32 + lane];
+            uint4 f = make_uint4(0, 0, 0, 0);
+            const int c = n * 8 + g;
+            if (RING || c < columns) f = x[((j * P + p) * columns + c) * 4 + t];
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
               mma<F16>(part_acc[m][n], fa[m][0], f.x, f.y);
@@ -422,60 +528,101 @@ __global__ void __launch_bounds__(WARPS * 32) q4_logits_kernel(const LogitArgs a
             }
           }
         }
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          const float s0 = __bfloat162float(sc[2 * m][b * (BLOCK / GROUP) + gr]);
-          const float s1 = __bfloat162float(sc[2 * m + 1][b * (BLOCK / GROUP) + gr]);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            acc[m][n][0] = fmaf(s0, part_acc[m][n][0], acc[m][n][0]);
-            acc[m][n][1] = fmaf(s0, part_acc[m][n][1], acc[m][n][1]);
-            acc[m][n][2] = fmaf(s1, part_acc[m][n][2], acc[m][n][2]);
-            acc[m][n][3] = fmaf(s1, part_acc[m][n][3], acc[m][n][3]);
-          }
-        }
       }
-    }
-  }
-  // columns of f32 rows do not cross a tile: the host gives them NT * 8 / 3 rows, so tiles are joined one by one
-  __shared__ float rest[WARPS][ROWS];  // what a row's pieces before this tile sum to
-#pragma unroll 1
-  for (int n = 0; n < NT; ++n) {
-    __syncthreads();
-#pragma unroll
-    for (int nn = 0; nn < NT; ++nn) {
-      if (nn != n) continue;
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        sums[warp][2 * t][16 * m + g] = acc[m][nn][0];
-        sums[warp][2 * t + 1][16 * m + g] = acc[m][nn][1];
-        sums[warp][2 * t][16 * m + g + 8] = acc[m][nn][2];
-        sums[warp][2 * t + 1][16 * m + g + 8] = acc[m][nn][3];
+        const float s0 = w.scale(2 * m, gr), s1 = w.scale(2 * m + 1, gr);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          acc[m][n][0] = fmaf(s0, part_acc[m][n][0], acc[m][n][0]);
+          acc[m][n][1] = fmaf(s0, part_acc[m][n][1], acc[m][n][1]);
+          acc[m][n][2] = fmaf(s1, part_acc[m][n][2], acc[m][n][2]);
+          acc[m][n][3] = fmaf(s1, part_acc[m][n][3], acc[m][n][3]);
+        }
       }
     }
-    __syncthreads();
-    if (a.pieces == 1) {
-      for (int e = threadIdx.x; e < wr * 8 * ROWS; e += WARPS * 32) {
-        const int r = e % ROWS, c = e / ROWS % 8, w = e / (8 * ROWS) * kw;
-        const int v = (blockIdx.x * wr + w / kw) * ROWS + r;
-        if (n * 8 + c >= a.columns || v >= a.V) continue;
-        float y = 0.0f;
-        for (int k = 0; k < kw; ++k) y += sums[w + k][c][r];
-        store_logit(a, n * 8 + c, v, y);
+    load(w);
+  };
+
+  for (int r = 0; r < rounds; ++r) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.0f;
+    if (RING) {
+      for (int b0 = 0; b0 < a.blocks; b0 += a.stage_blocks) {
+        if (ok) ok = bar_wait(full + 8 * s, ph);
+        const uint4* x = xs + (long long)s * a.stage_blocks * per_block;
+        const int b1 = min(b0 + a.stage_blocks, a.blocks);
+        for (int b = b0 + part; b < b1; b += kw) {
+          if (which)
+            multiply(held[1], x + (b - b0) * per_block);
+          else
+            multiply(held[0], x + (b - b0) * per_block);
+          which ^= 1;
+        }
+        __syncwarp();
+        if (lane == 0) bar_arrive_cluster(empty + 8 * s);
+        if (++s == a.stages) {
+          s = 0;
+          ph ^= 1;
+        }
       }
     } else {
-      for (int e = threadIdx.x; e < wr * ROWS; e += WARPS * 32) {
-        const int r = e % ROWS, w = e / ROWS * kw, v = (blockIdx.x * wr + w / kw) * ROWS + r;
-        float y = n ? rest[w][r] : 0.0f;
-        for (int c = 0; c < 8 && n * 8 + c < a.columns; ++c) {
-          for (int k = 0; k < kw; ++k) y += sums[w + k][c][r];
-          if ((n * 8 + c) % 3 == 2) {
-            if (v < a.V) store_logit(a, (n * 8 + c) / 3, v, y);
-            y = 0.0f;
-          }
-        }
-        rest[w][r] = y;
+      for (int b = part; b < a.blocks; b += kw) {
+        if (which)
+          multiply(held[1], xs + b * per_block);
+        else
+          multiply(held[0], xs + b * per_block);
+        which ^= 1;
       }
+    }
+    const int tile = ((int)blockIdx.x + r * (int)gridDim.x) * slots + slot;
+    if (kw > 1) {
+      // [slot][part - 1][values][lane]
+      float* to = sums + ((long long)slot * (kw - 1) + (part - 1)) * (8 * NT) * 32 + lane;
+      if (part) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to[((m * NT + n) * 4 + e) * 32] = acc[m][n][e];
+      }
+      multipliers_sync(a.warps * 32);
+      if (!part) {
+        for (int k = 1; k < kw; ++k) {
+          const float* from = sums + ((long long)slot * (kw - 1) + (k - 1)) * (8 * NT) * 32 + lane;
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[m][n][e] += from[((m * NT + n) * 4 + e) * 32];
+        }
+      }
+      multipliers_sync(a.warps * 32);
+    }
+    if (part == 0 && tile < a.tiles) {
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int c = n * 8 + 2 * t + (e & 1), v = tile * ROWS + 16 * m + 8 * (e >> 1) + g;
+            if (c >= a.rows || v >= a.V) continue;
+            const float y = ok ? acc[m][n][e] : NAN;  // NaN: a wait gave up
+            const long long at = c * a.y_ld + v;
+            if (a.out == 0)
+              ((float*)a.y)[at] = y;
+            else if (a.out == 1)
+              ((__nv_bfloat16*)a.y)[at] = __float2bfloat16_rn(y);
+            else
+              ((__half*)a.y)[at] = __float2half_rn(y);
+          }
     }
   }
 }
