@@ -550,7 +550,8 @@ int pesti_linear_ce_backward(const void* d_hidden, pesti_dtype dtype, int64_t N,
  *       equal ones;  q = clamp(round-half-even(w / s), -8, 7)  (0 where s is 0)
  * A group with an infinity or a NaN is held as NaN.
  * Layout, with B = ceil(D / 128) blocks a row: d_q has 64 B bytes a row, d_scale
- * 128 B / group bf16 a row, both 16-byte aligned.  In a block's 16 32-bit words,
+ * 128 B / group bf16 a row, to a multiple of 8 (zeros behind the last
+ * block's); both are 16-byte aligned.  In a block's 16 32-bit words,
  * word 4t + j (t, j = 0..3) holds columns 32j + 8t to 32j + 8t + 7 as q + 8, the
  * first in its lowest 4 bits; columns from D on hold 8 (q = 0).
  *
@@ -560,7 +561,7 @@ int pesti_linear_ce_backward(const void* d_hidden, pesti_dtype dtype, int64_t N,
  * [B, x_ld] (first D columns; F32, BF16 or F16) times the held weight.
  * Products of x and q are exact, summed in f32 over a group and then over the
  * groups with their scales, and rounded once.  The weight is read once for
- * every 64 rows of 16-bit x, or 21 of F32.  The logits overlap no input
+ * every 64 rows of x.  The logits overlap no input
  * (refused).  d_ws: device scratch of pesti_q4_logits_workspace(...) bytes,
  * 256-byte aligned, any contents; calls whose GPU work may overlap need scratch
  * of their own.

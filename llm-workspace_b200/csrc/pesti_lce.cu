@@ -239,8 +239,8 @@ int a_box(int64_t N) { return N > 96 ? 128 : 32; }
 template <int CG, bool BF16>
 int forward(const Call& c, const Layout& l, RowArgs r, bool grads, int sms, cudaStream_t st) {
   CUtensorMap rows, head;
-  int rc = pesti_tensor_map(&rows, c.dtype, l.rows, c.D, l.rows_pad, l.ldc * 2, 64, a_box(c.N));
-  if (!rc) rc = pesti_tensor_map(&head, c.dtype, c.head, c.D, c.V, c.w_ld * 2, 64, 128);
+  int rc = pesti_tensor_map(&rows, pesti_map_type(c.dtype), l.rows, c.D, l.rows_pad, l.ldc * 2, 64, a_box(c.N));
+  if (!rc) rc = pesti_tensor_map(&head, pesti_map_type(c.dtype), c.head, c.D, c.V, c.w_ld * 2, 64, 128);
   if (rc) return rc;
   GemmArgs g = gemm_args(l);
   g.m_tiles = -1;
@@ -264,20 +264,20 @@ template <int CG, bool BF16>
 int backward(const Call& c, const Layout& l, RowArgs r, void* dh, int64_t dh_ld, void* dw, int64_t dw_ld, int sms,
              cudaStream_t st) {
   CUtensorMap rows_k, rows_mn, head_k, head_mn, out_w, out_h;
-  int rc = pesti_tensor_map(&rows_k, c.dtype, l.rows, c.D, l.rows_pad, l.ldc * 2, 64, a_box(c.N));
-  if (!rc) rc = pesti_tensor_map(&rows_mn, c.dtype, l.rows, c.D, l.rows_pad, l.ldc * 2, 64, 64);
-  if (!rc) rc = pesti_tensor_map(&head_k, c.dtype, c.head, c.D, c.V, c.w_ld * 2, 64, 128);
-  if (!rc) rc = pesti_tensor_map(&head_mn, c.dtype, c.head, c.D, c.V, c.w_ld * 2, 64, 64);
-  if (!rc && dw) rc = pesti_tensor_map(&out_w, c.dtype, dw, c.D, c.V, dw_ld * 2, 64, 32);
-  if (!rc && dh) rc = pesti_tensor_map(&out_h, PESTI_F32, l.part32, c.D, l.cut.part_room, l.ld32 * 4, 32, 32);
+  int rc = pesti_tensor_map(&rows_k, pesti_map_type(c.dtype), l.rows, c.D, l.rows_pad, l.ldc * 2, 64, a_box(c.N));
+  if (!rc) rc = pesti_tensor_map(&rows_mn, pesti_map_type(c.dtype), l.rows, c.D, l.rows_pad, l.ldc * 2, 64, 64);
+  if (!rc) rc = pesti_tensor_map(&head_k, pesti_map_type(c.dtype), c.head, c.D, c.V, c.w_ld * 2, 64, 128);
+  if (!rc) rc = pesti_tensor_map(&head_mn, pesti_map_type(c.dtype), c.head, c.D, c.V, c.w_ld * 2, 64, 64);
+  if (!rc && dw) rc = pesti_tensor_map(&out_w, pesti_map_type(c.dtype), dw, c.D, c.V, dw_ld * 2, 64, 32);
+  if (!rc && dh) rc = pesti_tensor_map(&out_h, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, l.part32, c.D, l.cut.part_room, l.ld32 * 4, 32, 32);
   if (rc) return rc;
   const int d_tiles = (int)((c.D + BN - 1) / BN);
   for (long long v0 = 0; v0 < c.V; v0 += l.cut.piece) {
     const long long width = std::min<long long>(l.cut.piece, c.V - v0);
     CUtensorMap grad_out, grad_k, grad_mn;
-    rc = pesti_tensor_map(&grad_out, c.dtype, l.grad, width, l.rows_pad, l.cut.piece * 2, 64, 32);
-    if (!rc) rc = pesti_tensor_map(&grad_k, c.dtype, l.grad, width, l.rows_pad, l.cut.piece * 2, 64, a_box(c.N));
-    if (!rc) rc = pesti_tensor_map(&grad_mn, c.dtype, l.grad, width, l.rows_pad, l.cut.piece * 2, 64, 64);
+    rc = pesti_tensor_map(&grad_out, pesti_map_type(c.dtype), l.grad, width, l.rows_pad, l.cut.piece * 2, 64, 32);
+    if (!rc) rc = pesti_tensor_map(&grad_k, pesti_map_type(c.dtype), l.grad, width, l.rows_pad, l.cut.piece * 2, 64, a_box(c.N));
+    if (!rc) rc = pesti_tensor_map(&grad_mn, pesti_map_type(c.dtype), l.grad, width, l.rows_pad, l.cut.piece * 2, 64, 64);
     if (rc) return rc;
     GemmArgs g = gemm_args(l);  // G of this piece
     g.m_tiles = -1;

@@ -8,6 +8,7 @@
 #include "../../include/pesti_sampler.h"
 #include "pesti_error.h"
 #include "pesti_q4.cuh"
+#include "pesti_tensor_map.h"
 
 namespace {
 
@@ -31,15 +32,21 @@ int check_held(int64_t V, int64_t D, int64_t group, const void* q, const void* s
 
 long long blocks_of(int64_t D) { return (D + BLOCK - 1) / BLOCK; }
 
+// Scales of a row, in whole 16 bytes.
+int scale_row(int64_t D, int64_t group) { return (int)((blocks_of(D) * (BLOCK / group) + 7) / 8 * 8); }
+
 bool overlap(const void* p, __int128 np, const void* q, __int128 nq) {
   return (__int128)(uintptr_t)p < (__int128)(uintptr_t)q + nq && (__int128)(uintptr_t)q < (__int128)(uintptr_t)p + np;
 }
 
-int need_device() {
-  int n = 0;
+int need_device(int* sms = nullptr) {
+  int n = 0, dev = 0;
   if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0)
     return pesti_set_error(PESTI_E_NO_DEVICE, "no CUDA device available");
-  return PESTI_OK;
+  if (!sms) return PESTI_OK;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
+  return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, "device query");
 }
 
 int launched(const char* what) {
@@ -56,9 +63,10 @@ int check_plain(const void* w, pesti_dtype dtype, int64_t V, int64_t D, int64_t 
   if (!w) return refuse("null head");
   if ((uintptr_t)w % esize(dtype)) return refuse("the head is not aligned to its type");
   const long long n = V * blocks_of(D);
+  const __int128 scales = (__int128)V * scale_row(D, group) * 2;
   const __int128 plain = ((__int128)(V - 1) * ld + D) * esize(dtype);
-  if (overlap(w, plain, q, (__int128)n * BLOCK_BYTES) || overlap(w, plain, scale, (__int128)n * (BLOCK / group) * 2) ||
-      overlap(q, (__int128)n * BLOCK_BYTES, scale, (__int128)n * (BLOCK / group) * 2))
+  if (overlap(w, plain, q, (__int128)n * BLOCK_BYTES) || overlap(w, plain, scale, scales) ||
+      overlap(q, (__int128)n * BLOCK_BYTES, scale, scales))
     return refuse("head, weights and scales overlap");
   return PESTI_OK;
 }
@@ -78,6 +86,7 @@ int convert(bool there, const void* w, int64_t V, int64_t D, int64_t ld, void* q
   a.scale = (__nv_bfloat16*)scale;
   a.D = (int)D;
   a.blocks = (int)blocks_of(D);
+  a.scale_ld = scale_row(D, GROUP);
   a.runs = (a.blocks + per<T>(there) - 1) / per<T>(there);
   a.total = V * a.runs;
   const int align = there || sizeof(T) == 4 ? 32 : 16, teams = there ? 32 : 16;  // of a thread block
@@ -106,31 +115,29 @@ int convert(bool there, pesti_dtype dtype, int64_t group, const void* w, int64_t
   return convert<__half>(there, group, w, V, D, ld, q, scale, st);
 }
 
-constexpr int MOST_ROWS = 64;           // of x, a pass over the weight
-constexpr int SHARED_BYTES = 200 << 10;  // for x
-constexpr int SMS = 148;
-
-int column_tiles(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 ? 4 : 8; }
+constexpr int MOST_ROWS = 64;            // of x, a pass over the weight
+constexpr int FEW_ROWS = 8;              // a column tile of the products by warps
+constexpr int SHARED_BYTES = 200 << 10;  // for x, or for the stages
 
 int pieces_of(pesti_dtype d) { return d == PESTI_F32 ? 3 : 1; }
 
-// Bytes of fragments of a block of x.
-long long block_bytes(int pieces, int columns) { return 16LL * pieces * columns * 16; }
+int columns_of(int64_t rows) { return (int)(rows + 15) / 16 * 16; }
 
-bool fits_whole(int64_t D, int pieces, int64_t rows) {
-  return blocks_of(D) * block_bytes(pieces, (int)rows) <= SHARED_BYTES && rows <= 16;
+// Few rows of x that fit shared memory whole.
+bool few(int64_t D, int pieces, int64_t rows) {
+  return rows <= FEW_ROWS && blocks_of(D) * rows * pieces * (BLOCK * 2) <= SHARED_BYTES;
 }
 
 // How a pass shares its tiles and their K out: the least time of the busiest SM, by the weight's bytes that it reads (44
-// bytes a nanosecond) and a microsecond and a half per round of tiles, where few warps have too little in flight.
-void share_out(LogitArgs& a, int nt, int sms) {
+// bytes a nanosecond, with 20 warps or more) and a microsecond and a half per round of tiles.
+void share_out(LogitArgs& a, int sms) {
   double best = 1e30;
   for (int kw = 1; kw <= 8 && kw <= a.blocks; kw *= 2) {
-    for (int w = kw; w <= most_warps(nt); w += kw) {
+    for (int w = kw; w <= MOST_WARPS; w += kw) {
       const int slots = w / kw;
       const long long rounds = (a.tiles + (long long)sms * slots - 1) / ((long long)sms * slots);
       const double bytes = (double)rounds * slots * a.blocks * (ROWS * BLOCK_BYTES);
-      const double t = bytes / (w >= 12 ? 44.0 : 44.0 * w / 12) + 1500.0 * rounds + (kw > 1 ? 300.0 * rounds : 0.0);
+      const double t = bytes / (w >= 20 ? 44.0 : 44.0 * w / 20) + (kw > 1 ? 1800.0 : 1500.0) * rounds;
       if (t < best) {
         best = t;
         a.warps = w;
@@ -143,6 +150,9 @@ void share_out(LogitArgs& a, int nt, int sms) {
 template <typename... K, typename... A>
 int launch(const char* what, void (*kernel)(K...), long long blocks, int threads, int smem, cudaStream_t st,
            const A&... args) {
+  cudaError_t e = cudaSuccess;
+  if (smem > 48 << 10) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return pesti_set_cuda_error(e, what);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3(threads);
@@ -153,56 +163,46 @@ int launch(const char* what, void (*kernel)(K...), long long blocks, int threads
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, K(args)...);
+  e = cudaLaunchKernelEx(&cfg, kernel, K(args)...);
   return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, what);
 }
 
-template <typename T, int GROUP, int NT, bool RING>
-int logits_pass(LogitArgs a, cudaStream_t st) {
-  constexpr int P = sizeof(T) == 4 ? 3 : 1;
-  share_out(a, NT, SMS);
-  long long smem = 0;
-  if (RING) {
-    const int rc = launch("q4_fragments_kernel launch", q4_fragments_kernel<T>, a.blocks, 256, 0, st, a, 8 * NT);
-    if (rc) return rc;
-    const long long block = block_bytes(P, 8 * NT);
-    a.stage_blocks = a.k_warps;  // a block for each warp of a tile
-    a.stages = (int)std::min<long long>(8, SHARED_BYTES / (block * a.stage_blocks));
-    smem = a.stages * a.stage_blocks * block;
-  } else {
-    smem = a.blocks * block_bytes(P, a.rows);
-  }
-  smem += (long long)(a.warps - a.warps / a.k_warps) * 8 * NT * 32 * 4;
-  auto kernel = q4_logits_kernel<T, GROUP, NT, RING>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return pesti_set_cuda_error(e, "q4_logits_kernel shared memory");
-  const int slots = a.warps / a.k_warps;
-  return launch("q4_logits_kernel launch", kernel, std::min<long long>(SMS, (a.tiles + slots - 1) / slots),
-                (a.warps + (RING ? 1 : 0)) * 32, (int)smem, st, a);
-}
-
 template <typename T, int GROUP>
-int logits_tiles(const LogitArgs& a, cudaStream_t st) {
-  const bool whole = fits_whole(a.D, sizeof(T) == 4 ? 3 : 1, a.rows);
-  switch (column_tiles(a.rows)) {
-    case 1: return whole ? logits_pass<T, GROUP, 1, false>(a, st) : logits_pass<T, GROUP, 1, true>(a, st);
-    case 2: return whole ? logits_pass<T, GROUP, 2, false>(a, st) : logits_pass<T, GROUP, 2, true>(a, st);
-    case 4: return logits_pass<T, GROUP, 4, true>(a, st);
-    default: return logits_pass<T, GROUP, 8, true>(a, st);
+int pass(LogitArgs a, int sms, cudaStream_t st) {
+  constexpr int P = sizeof(T) == 4 ? 3 : 1;
+  if (few(a.D, P, a.rows)) {
+    a.tiles = (a.V + ROWS - 1) / ROWS;
+    share_out(a, sms);
+    const int slots = a.warps / a.k_warps;
+    const int smem = a.blocks * a.rows * P * (BLOCK * 2) + 16 + (a.warps - slots) * 4 * 32 * 4;
+    return launch("q4_logits_kernel launch", q4_logits_kernel<T, GROUP>,
+                  std::min<long long>(sms, (a.tiles + slots - 1) / slots), a.warps * 32, smem, st, a);
   }
+  a.tiles = (a.V + TILE - 1) / TILE;
+  a.columns = columns_of(a.rows);
+  CUtensorMap weights;
+  const long long row = (long long)a.blocks * BLOCK_BYTES;
+  int rc = pesti_tensor_map(&weights, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.q, row, a.V, row, BLOCK_BYTES, TILE,
+                            CU_TENSOR_MAP_SWIZZLE_64B);
+  if (!rc) rc = launch("q4_operand_kernel launch", q4_operand_kernel<T>, a.blocks, 256, 0, st, a);
+  if (rc) return rc;
+  const int stage = SLOTS * TILE_BYTES + a.columns * P * (BLOCK * 2);
+  a.stages = std::min(8, SHARED_BYTES / stage);
+  return launch("q4_wide_kernel launch", q4_wide_kernel<T, GROUP>, std::min(sms, a.tiles), WIDE_THREADS,
+                1024 + a.stages * stage, st, weights, a);
 }
 
 template <typename T>
-int logits(LogitArgs a, int64_t group, int64_t B, pesti_dtype out, cudaStream_t st) {
+int logits(LogitArgs a, int64_t group, int64_t B, pesti_dtype out, int sms, cudaStream_t st) {
   const char* x = (const char*)a.x;
   char* y = (char*)a.y;
   for (int64_t r = 0; r < B; r += MOST_ROWS) {
     a.rows = (int)std::min<int64_t>(MOST_ROWS, B - r);
     a.x = x + r * a.x_ld * sizeof(T);
     a.y = y + r * a.y_ld * esize(out);
-    const int rc = group == 32   ? logits_tiles<T, 32>(a, st)
-                   : group == 64 ? logits_tiles<T, 64>(a, st)
-                                 : logits_tiles<T, 128>(a, st);
+    const int rc = group == 32   ? pass<T, 32>(a, sms, st)
+                   : group == 64 ? pass<T, 64>(a, sms, st)
+                                 : pass<T, 128>(a, sms, st);
     if (rc) return rc;
   }
   return PESTI_OK;
@@ -233,9 +233,8 @@ int64_t pesti_q4_logits_workspace(pesti_dtype dtype, int64_t B, int64_t D) {
   if (B < 0) return refuse("B < 0");
   if (B > 1 << 24) return refuse("B must be at most 2^24");
   if (D < 1 || D > 1 << 20) return refuse("D must be 1 to 2^20");
-  const int64_t rows = std::min<int64_t>(B, MOST_ROWS);
-  if (B <= MOST_ROWS && fits_whole(D, pieces_of(dtype), rows)) return 256;
-  return blocks_of(D) * block_bytes(pieces_of(dtype), 8 * column_tiles(rows));
+  if (few(D, pieces_of(dtype), B)) return 256;
+  return blocks_of(D) * columns_of(std::min<int64_t>(B, MOST_ROWS)) * pieces_of(dtype) * (BLOCK * 2);
 }
 
 int pesti_q4_logits(const void* d_x, pesti_dtype dtype, int64_t B, int64_t D, int64_t x_ld, const void* d_q,
@@ -255,11 +254,12 @@ int pesti_q4_logits(const void* d_x, pesti_dtype dtype, int64_t B, int64_t D, in
   const __int128 nx = ((__int128)(B - 1) * x_ld + D) * esize(dtype), ny = ((__int128)(B - 1) * ld + V) * esize(out_dtype);
   const __int128 nb = (__int128)V * blocks_of(D);
   if (overlap(d_logits, ny, d_x, nx) || overlap(d_logits, ny, d_q, nb * BLOCK_BYTES) ||
-      overlap(d_logits, ny, d_scale, nb * (BLOCK / group) * 2))
+      overlap(d_logits, ny, d_scale, (__int128)V * scale_row(D, group) * 2))
     return refuse("inputs and logits overlap");
   if (!d_ws || ws_bytes < need) return refuse("workspace too small");
   if ((uintptr_t)d_ws % 256) return refuse("workspace is not 256-byte aligned");
-  rc = need_device();
+  int sms = 0;
+  rc = need_device(&sms);
   if (rc) return rc;
   LogitArgs a = {};
   a.x = d_x;
@@ -269,15 +269,15 @@ int pesti_q4_logits(const void* d_x, pesti_dtype dtype, int64_t B, int64_t D, in
   a.scale = (const __nv_bfloat16*)d_scale;
   a.V = (int)V;
   a.blocks = (int)blocks_of(D);
-  a.tiles = (int)((V + ROWS - 1) / ROWS);
-  a.frags = (uint4*)d_ws;
+  a.scale_ld = scale_row(D, group);
+  a.operand = (uint4*)d_ws;
   a.y = d_logits;
   a.y_ld = ld;
   a.out = out_dtype == PESTI_F32 ? 0 : out_dtype == PESTI_BF16 ? 1 : 2;
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == PESTI_F32) return logits<float>(a, group, B, out_dtype, st);
-  if (dtype == PESTI_BF16) return logits<__nv_bfloat16>(a, group, B, out_dtype, st);
-  return logits<__half>(a, group, B, out_dtype, st);
+  if (dtype == PESTI_F32) return logits<float>(a, group, B, out_dtype, sms, st);
+  if (dtype == PESTI_BF16) return logits<__nv_bfloat16>(a, group, B, out_dtype, sms, st);
+  return logits<__half>(a, group, B, out_dtype, sms, st);
 }
 
 }  // extern "C"

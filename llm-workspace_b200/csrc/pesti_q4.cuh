@@ -19,6 +19,7 @@ namespace pesti_q4 {
 
 constexpr int BLOCK = 128;  // columns
 constexpr int BLOCK_BYTES = BLOCK / 2;
+constexpr int MOST_WARPS = 24;  // of a block that multiplies few rows
 
 template <typename T>
 __device__ __forceinline__ float to_f32(T v) {
@@ -49,7 +50,8 @@ struct Held {
   long long ld;
   uint32_t* q;
   __nv_bfloat16* scale;
-  int D, blocks, runs;  // blocks of a row, and runs of PER blocks that half a warp takes
+  int D, blocks, runs;  // blocks of a row, and runs of PER blocks that a team takes
+  int scale_ld;         // scales of a row
   long long total;      // runs in all
   int vec;              // whole vectors of 8 columns can be read or written
 };
@@ -194,7 +196,7 @@ __global__ void __launch_bounds__(256) q4_quantize_kernel(const Held<T> a) {
     if (u < n) in[u].load(from, (b0 + u) * BLOCK + 16 * i, a.D, a.vec);
   const long long b = row * a.blocks + b0;
   uint32_t* to = a.q + b * (BLOCK / 8) + word_of(2 * i);  // (the other word is 4 behind it)
-  __nv_bfloat16* scale = a.scale + b * (BLOCK / GROUP) + i / (GROUP / 16);
+  __nv_bfloat16* scale = a.scale + row * a.scale_ld + b0 * (BLOCK / GROUP) + i / (GROUP / 16);
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
     float hi, neg;
@@ -234,6 +236,8 @@ __global__ void __launch_bounds__(256) q4_quantize_kernel(const Held<T> a) {
     to[u * (BLOCK / 8) + 4] = word[1];
     if (i % (GROUP / 16) == 0) scale[u * (BLOCK / GROUP)] = held;
   }
+  if (there && i == 0 && b0 + n == a.blocks)  // the row's last: zeros to whole 16 bytes
+    for (int e = a.blocks * (BLOCK / GROUP); e < a.scale_ld; ++e) a.scale[row * a.scale_ld + e] = __nv_bfloat16(0.0f);
 }
 
 // Two lanes of a team of sixteen hold neighbouring words; f32 rows are written 32 bytes a lane, 16-bit ones 16.
@@ -246,7 +250,7 @@ __global__ void __launch_bounds__(256) q4_dequantize_kernel(const Held<T> a) {
   const int n = min(PER, a.blocks - b0);
   const long long b = row * a.blocks + b0;
   const uint32_t* from = a.q + b * (BLOCK / 8) + word_of(i);
-  const __nv_bfloat16* scale = a.scale + b * (BLOCK / GROUP) + i / (GROUP / 8);
+  const __nv_bfloat16* scale = a.scale + row * a.scale_ld + b0 * (BLOCK / GROUP) + i / (GROUP / 8);
   uint32_t w[PER];
   float s[PER];
 #pragma unroll
@@ -287,14 +291,25 @@ struct LogitArgs {
   int rows, D;  // of x; at most 64 rows
   const uint4* q;
   const __nv_bfloat16* scale;
-  int V, blocks, tiles;  // 32 rows of the weight a tile
-  uint4* frags;          // [blocks][4][pieces][8 NT][4], where x does not fit shared memory whole
+  int V, blocks, tiles;
+  uint4* operand;        // x for the tensor cores (q4_operand_kernel)
+  int columns, stages;   // its rows, to a multiple of 16, and how many blocks are in shared memory at once
   void* y;
   long long y_ld;
   int out;               // 0 f32, 1 bf16, 2 f16
   int warps, k_warps;    // warps that multiply, and how many of them share a tile's K
-  int stage_blocks, stages;
+  int scale_ld;          // scales of a row
 };
+
+__device__ __forceinline__ void store_logit(const LogitArgs& a, int row, int v, float y) {
+  const long long at = row * a.y_ld + v;
+  if (a.out == 0)
+    ((float*)a.y)[at] = y;
+  else if (a.out == 1)
+    ((__nv_bfloat16*)a.y)[at] = __float2bfloat16_rn(y);
+  else
+    ((__half*)a.y)[at] = __float2half_rn(y);
+}
 
 // The bf16 or f16 bits of piece `p` of an x: f32 is cut into three bf16 whose sum it is, exactly.
 template <typename T>
@@ -325,20 +340,6 @@ __device__ __forceinline__ uint4 fragment_of(const T* row, int b, int j, int t, 
   return make_uint4(f[0], f[1], f[2], f[3]);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) q4_fragments_kernel(const LogitArgs a, int columns) {
-  pesti_umma::depend_wait();
-  pesti_umma::depend_launch();
-  constexpr int P = sizeof(T) == 4 ? 3 : 1;
-  const int per_block = 16 * P * columns;
-  for (int e = threadIdx.x; e < per_block; e += 256) {
-    const int t = e & 3, c = (e >> 2) % columns, jp = (e >> 2) / columns, p = jp % P, j = jp / P;
-    uint4 f = make_uint4(0, 0, 0, 0);
-    if (c < a.rows) f = fragment_of((const T*)a.x + c * a.x_ld, blockIdx.x, j, t, p, a.D);
-    a.frags[(long long)blockIdx.x * per_block + e] = f;
-  }
-}
-
 // Nibbles i and i + 4 of a word as two 16-bit floats q: the nibble becomes the mantissa's low end of 128 (bf16) or
 // 1024 (f16), and 8 more than that is taken off, exactly.
 template <bool F16>
@@ -355,34 +356,36 @@ __device__ __forceinline__ uint32_t unpack(uint32_t word, int i) {
   }
 }
 
-template <bool F16>
+// c (+)= A B over 16 of K.
+template <bool F16, bool ADD>
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  const float z0 = ADD ? c[0] : 0.0f, z1 = ADD ? c[1] : 0.0f, z2 = ADD ? c[2] : 0.0f, z3 = ADD ? c[3] : 0.0f;
   if constexpr (F16)
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %11, %12, %13};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(z0), "f"(z1), "f"(z2), "f"(z3));
   else
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        "{%10, %11, %12, %13};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(z0), "f"(z1), "f"(z2), "f"(z3));
 }
 
-constexpr int ROWS = 32;  // of the weight, per warp and tile
+constexpr int ROWS = 16;  // of the weight, per warp and tile
 
-__host__ __device__ constexpr int most_warps(int nt) { return nt <= 2 ? 15 : nt == 4 ? 11 : 7; }
-
-// A lane's weights of one block: 16 bytes of four rows (8 apart), and their groups' scales.
+// A lane's weights of one block: 16 bytes of two rows (8 apart), and their groups' scales.
 template <int GROUP>
 struct Weights {
-  uint4 w[4];
-  uint2 s[4];  // up to four bf16
+  uint4 w[2];
+  uint2 s[2];  // up to four bf16
 
-  __device__ __forceinline__ void load(const uint4* const (&q)[4], const __nv_bfloat16* const (&sc)[4], int b) {
+  __device__ __forceinline__ void load(const char* q, uint32_t q_at, uint32_t q_far, const char* sc, uint32_t s_at,
+                                       uint32_t s_far) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      w[i] = __ldcs(q[i] + b * (BLOCK_BYTES / 16));
-      const __nv_bfloat16* p = sc[i] + b * (BLOCK / GROUP);
+    for (int i = 0; i < 2; ++i) {
+      w[i] = __ldcs((const uint4*)(q + (q_at + i * q_far)));
+      const char* p = sc + (s_at + i * s_far);
       if constexpr (GROUP == 32)
         s[i] = __ldg((const uint2*)p);
       else if constexpr (GROUP == 64)
@@ -398,81 +401,42 @@ struct Weights {
   }
 };
 
-__device__ __forceinline__ void multipliers_sync(int threads) {
-  asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");
-}
-
-// A warp multiplies 32 rows of the weight by all columns of x over its share of K (every k_warps-th block), and goes on
-// to its next tile; the k_warps warps of a tile join their sums in shared memory, in their order.  Blocks of weights are
-// loaded two ahead of their products.  Columns past x's last row hold zeros.
-// RING: x passes through shared memory in stages, copied by a warp of its own, again for every round of tiles.
-// Otherwise x is laid out there once, by all warps, while the first weights are on their way.
-template <typename T, int GROUP, int NT, bool RING>
-__global__ void __launch_bounds__((most_warps(NT) + 1) * 32) q4_logits_kernel(const LogitArgs a) {
-  using namespace pesti_umma;
+// Up to 8 rows of x: a warp multiplies 16 rows of the weight by all of them over its share of K (every k_warps-th
+// block), and goes on to its next tile; the k_warps warps of a tile join their sums in shared memory, in their order.
+// x is laid out in shared memory once, while the first weights are on their way; weights are loaded two blocks ahead.
+template <typename T, int GROUP>
+__global__ void __launch_bounds__(MOST_WARPS * 32, 1) q4_logits_kernel(const LogitArgs a) {
   constexpr bool F16 = std::is_same<T, __half>::value;
-  constexpr int P = sizeof(T) == 4 ? 3 : 1, COLUMNS = 8 * NT;
+  constexpr int P = sizeof(T) == 4 ? 3 : 1;
   extern __shared__ uint4 xs[];
-  __shared__ uint64_t bars[16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int kw = a.k_warps, slots = a.warps / kw, part = warp % kw, slot = warp / kw;
-  const int columns = RING ? COLUMNS : a.rows;  // in shared memory
-  const int per_block = 16 * P * columns;       // 16-byte fragments of a block of x
+  const int columns = a.rows, per_block = 16 * P * columns;  // 16-byte fragments of a block of x
   const int rounds = (a.tiles + gridDim.x * slots - 1) / (gridDim.x * slots);
-  const uint32_t full = smem_addr(bars), empty = full + 64;
-  float* sums = (float*)(xs + (long long)(RING ? a.stages * a.stage_blocks : a.blocks) * per_block);
+  float* sums = (float*)(xs + a.blocks * per_block + 1);
+  pesti_umma::depend_wait();
+  pesti_umma::depend_launch();
 
-  if (RING && threadIdx.x == 0) {
-    for (int s = 0; s < a.stages; ++s) {
-      bar_init(full + 8 * s, 1);
-      bar_init(empty + 8 * s, a.warps);
-    }
-    bar_init_fence();
-  }
-  if (RING) __syncthreads();
-  depend_launch();
-
-  if (RING && warp == a.warps) {  // copies x
-    if (lane == 0) {
-      depend_wait();
-      int s = 0, ph = 0;
-      bool ok = true;
-      for (int r = 0; r < rounds && ok; ++r) {
-        for (int b = 0; b < a.blocks; b += a.stage_blocks) {
-          ok = bar_wait(empty + 8 * s, ph ^ 1);
-          if (!ok) break;
-          const uint32_t bytes = min(a.stage_blocks, a.blocks - b) * per_block * 16;
-          bar_expect(full + 8 * s, bytes);
-          bulk_load(smem_addr(xs + (long long)s * a.stage_blocks * per_block), a.frags + (long long)b * per_block,
-                    full + 8 * s, bytes);
-          if (++s == a.stages) {
-            s = 0;
-            ph ^= 1;
-          }
-        }
-      }
-    }
-    return;
-  }
-
-  // the next block to load: its tile's round, and its place
-  const uint4* q[4];
-  const __nv_bfloat16* sc[4];
+  // the next block to load
+  const uint32_t q_row = a.blocks * BLOCK_BYTES, s_row = a.scale_ld * 2;
+  uint32_t q_lane, q_far, s_lane, s_far;
+  const char *q, *sc;
   auto rows_of = [&](int round) {
     const int tile = min(((int)blockIdx.x + round * (int)gridDim.x) * slots + slot, a.tiles - 1);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const long long row = min(tile * ROWS + g + 8 * i, a.V - 1);
-      q[i] = a.q + (row * a.blocks) * (BLOCK_BYTES / 16) + t;
-      sc[i] = a.scale + (row * a.blocks) * (BLOCK / GROUP);
-    }
+    q = (const char*)a.q + (long long)tile * ROWS * q_row;
+    sc = (const char*)a.scale + (long long)tile * ROWS * s_row;
+    const int last = a.V - 1 - tile * ROWS, r0 = min(g, last), r1 = min(g + 8, last);
+    q_lane = r0 * q_row + t * 16;
+    q_far = (r1 - r0) * q_row;
+    s_lane = r0 * s_row;
+    s_far = (r1 - r0) * s_row;
   };
   int load_round = 0, load_b = part;
   rows_of(0);
   Weights<GROUP> held[2];
   auto load = [&](Weights<GROUP>& w) {
     if (load_round >= rounds) return;
-    w.load(q, sc, load_b);
+    w.load(q, q_lane + load_b * BLOCK_BYTES, q_far, sc, s_lane + load_b * (2 * BLOCK / GROUP), s_far);
     load_b += kw;
     if (load_b >= a.blocks) {
       load_b = part;
@@ -482,149 +446,333 @@ __global__ void __launch_bounds__((most_warps(NT) + 1) * 32) q4_logits_kernel(co
   load(held[0]);
   load(held[1]);
 
-  if (!RING) {
-    depend_wait();
-    for (int e = threadIdx.x; e < a.blocks * per_block; e += a.warps * 32) {
-      const int tt = e & 3, rest = e >> 2, c = rest % columns, bjp = rest / columns, p = bjp % P, bj = bjp / P;
-      xs[e] = fragment_of((const T*)a.x + c * a.x_ld, bj >> 2, bj & 3, tt, p, a.D);
-    }
-    __syncthreads();
+  for (int e = threadIdx.x; e < a.blocks * per_block; e += a.warps * 32) {
+    const int tt = e & 3, rest = e >> 2, c = rest % columns, bjp = rest / columns, p = bjp % P, bj = bjp / P;
+    xs[e] = fragment_of((const T*)a.x + c * a.x_ld, bj >> 2, bj & 3, tt, p, a.D);
   }
+  if (threadIdx.x == 0) xs[a.blocks * per_block] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  // the lane's fragments; columns without a row read the zeros behind x
+  const bool there = g < columns;
+  const uint4* mine = there ? xs + g * 4 + t : xs + a.blocks * per_block;
+  const int x_block = there ? per_block : 0, x_step = there ? 4 * columns : 0;
 
-  float acc[2][NT][4];
-  int s = 0, ph = 0, which = 0;
-  bool ok = true;
-
-  // the products of block b with the fragments at `x`
+  float acc[4];
   auto multiply = [&](Weights<GROUP>& w, const uint4* x) {
 #pragma unroll
     for (int gr = 0; gr < BLOCK / GROUP; ++gr) {
-      float part_acc[2][NT][4] = {};
+      float sum[4];
 #pragma unroll
       for (int jj = 0; jj < GROUP / 32; ++jj) {
         const int j = gr * (GROUP / 32) + jj;
-        uint32_t fa[2][2][4];
+        uint32_t fa[2][4];
+        const uint32_t w0 = ((const uint32_t*)&w.w[0])[j], w1 = ((const uint32_t*)&w.w[1])[j];
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t w0 = ((const uint32_t*)&w.w[2 * m])[j], w1 = ((const uint32_t*)&w.w[2 * m + 1])[j];
-            fa[m][h][0] = unpack<F16>(w0, 2 * h);
-            fa[m][h][1] = unpack<F16>(w1, 2 * h);
-            fa[m][h][2] = unpack<F16>(w0, 2 * h + 1);
-            fa[m][h][3] = unpack<F16>(w1, 2 * h + 1);
-          }
+        for (int h = 0; h < 2; ++h) {
+          fa[h][0] = unpack<F16>(w0, 2 * h);
+          fa[h][1] = unpack<F16>(w1, 2 * h);
+          fa[h][2] = unpack<F16>(w0, 2 * h + 1);
+          fa[h][3] = unpack<F16>(w1, 2 * h + 1);
+        }
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            uint4 f = make_uint4(0, 0, 0, 0);
-            const int c = n * 8 + g;
-            if (RING || c < columns) f = x[((j * P + p) * columns + c) * 4 + t];
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-              mma<F16>(part_acc[m][n], fa[m][0], f.x, f.y);
-              mma<F16>(part_acc[m][n], fa[m][1], f.z, f.w);
-            }
-          }
+          const uint4 f = x[(j * P + p) * x_step];
+          if (jj == 0 && p == 0)
+            mma<F16, false>(sum, fa[0], f.x, f.y);
+          else
+            mma<F16, true>(sum, fa[0], f.x, f.y);
+          mma<F16, true>(sum, fa[1], f.z, f.w);
         }
       }
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        const float s0 = w.scale(2 * m, gr), s1 = w.scale(2 * m + 1, gr);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          acc[m][n][0] = fmaf(s0, part_acc[m][n][0], acc[m][n][0]);
-          acc[m][n][1] = fmaf(s0, part_acc[m][n][1], acc[m][n][1]);
-          acc[m][n][2] = fmaf(s1, part_acc[m][n][2], acc[m][n][2]);
-          acc[m][n][3] = fmaf(s1, part_acc[m][n][3], acc[m][n][3]);
-        }
-      }
+      const float s0 = w.scale(0, gr), s1 = w.scale(1, gr);
+      acc[0] = fmaf(s0, sum[0], acc[0]);
+      acc[1] = fmaf(s0, sum[1], acc[1]);
+      acc[2] = fmaf(s1, sum[2], acc[2]);
+      acc[3] = fmaf(s1, sum[3], acc[3]);
     }
     load(w);
   };
 
+  int which = 0;
   for (int r = 0; r < rounds; ++r) {
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int e = 0; e < 4; ++e) acc[e] = 0.0f;
+    for (int b = part; b < a.blocks; b += kw) {
+      if (which)
+        multiply(held[1], mine + b * x_block);
+      else
+        multiply(held[0], mine + b * x_block);
+      which ^= 1;
+    }
+    const int tile = ((int)blockIdx.x + r * (int)gridDim.x) * slots + slot;
+    if (kw > 1) {  // [slot][part - 1][value][lane]
+      float* to = sums + (slot * (kw - 1) + (part - 1)) * 4 * 32 + lane;
+      if (part) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+        for (int e = 0; e < 4; ++e) to[e * 32] = acc[e];
+      }
+      __syncthreads();
+      if (!part) {
+        for (int k = 0; k < kw - 1; ++k)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.0f;
-    if (RING) {
-      for (int b0 = 0; b0 < a.blocks; b0 += a.stage_blocks) {
-        if (ok) ok = bar_wait(full + 8 * s, ph);
-        const uint4* x = xs + (long long)s * a.stage_blocks * per_block;
-        const int b1 = min(b0 + a.stage_blocks, a.blocks);
-        for (int b = b0 + part; b < b1; b += kw) {
-          if (which)
-            multiply(held[1], x + (b - b0) * per_block);
-          else
-            multiply(held[0], x + (b - b0) * per_block);
-          which ^= 1;
-        }
+          for (int e = 0; e < 4; ++e) acc[e] += sums[((slot * (kw - 1) + k) * 4 + e) * 32 + lane];
+      }
+      __syncthreads();
+    }
+    if (part || tile >= a.tiles) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = 2 * t + (e & 1), v = tile * ROWS + 8 * (e >> 1) + g;
+      if (c < a.rows && v < a.V) store_logit(a, c, v, acc[e]);
+    }
+  }
+}
+
+// --- more rows: products on the tensor cores' own memory
+//
+// A product's 128 x 64 operand of weights is unpacked into tensor memory, exactly, as whole numbers; x comes from shared
+// memory; the sums of a group come back, times its scale, into registers, where a thread adds up one row of the weight
+// for all rows of x.  So the weights pass through shared memory once, in 4 bits.
+
+// x as the products' second operand, [blocks][2][pieces][columns][128 bytes]: half a block's 64 columns in the order
+// that words of weights unpack in, 16-byte chunks exchanged as 128-byte swizzled atoms hold them.
+template <typename T>
+__global__ void __launch_bounds__(256) q4_operand_kernel(const LogitArgs a) {
+  pesti_umma::depend_wait();
+  pesti_umma::depend_launch();
+  constexpr int P = sizeof(T) == 4 ? 3 : 1;
+  const int per_block = 2 * P * a.columns * 8, b = blockIdx.x;
+  for (int e = threadIdx.x; e < per_block; e += 256) {
+    const int c = e & 7, n = (e >> 3) % a.columns, hp = (e >> 3) / a.columns, p = hp % P, h = hp / P;
+    uint4 f = make_uint4(0, 0, 0, 0);
+    if (n < a.rows) f = fragment_of((const T*)a.x + n * a.x_ld, b, 2 * h + (c >> 2), c & 3, p, a.D);
+    a.operand[(long long)b * per_block + (e & ~7) + (c ^ (n & 7))] = f;
+  }
+}
+
+constexpr int TILE = 128;                      // rows of the weight
+constexpr int SLOTS = 2;                       // tiles at once
+constexpr int WIDE_THREADS = (8 * SLOTS + 2) * 32;
+constexpr int TILE_BYTES = TILE * BLOCK_BYTES;  // of a block of weights
+
+// Where a slot's buffers are in tensor memory: two of 64 of K, and two of sums.
+__device__ __forceinline__ uint32_t a_column(int slot, int buf) { return slot * 256 + buf * 32; }
+__device__ __forceinline__ uint32_t d_column(int slot, int buf) { return slot * 256 + 64 + buf * 64; }
+
+// Warps 0 to 7 unpack (four a slot, a quarter of the rows each), 8 to 15 add up, 16 copies, 17 issues the products.
+template <typename T, int GROUP>
+__global__ void __launch_bounds__(WIDE_THREADS, 1)
+    q4_wide_kernel(const __grid_constant__ CUtensorMap weights, const LogitArgs a) {
+  using namespace pesti_umma;
+  constexpr bool F16 = std::is_same<T, __half>::value;
+  constexpr int P = sizeof(T) == 4 ? 3 : 1;
+  extern __shared__ char raw[];
+  const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
+  const uint32_t x_half = a.columns * 128, x_bytes = 2 * P * x_half, stage = SLOTS * TILE_BYTES + x_bytes;
+  __shared__ uint64_t bars[16 + 8 * SLOTS];
+  __shared__ uint32_t tmem_base;
+  const uint32_t full = smem_addr(bars), empty = full + 64, a_full = empty + 64, a_empty = a_full + 16 * SLOTS,
+                 d_full = a_empty + 16 * SLOTS, d_empty = d_full + 16 * SLOTS;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < a.stages; ++s) {
+      bar_init(full + 8 * s, 1);
+      bar_init(empty + 8 * s, 4 * SLOTS + 1);
+    }
+    for (int s = 0; s < 2 * SLOTS; ++s) {
+      bar_init(a_full + 8 * s, 4);
+      bar_init(a_empty + 8 * s, 1);
+      bar_init(d_full + 8 * s, 1);
+      bar_init(d_empty + 8 * s, 4);
+    }
+    bar_init_fence();
+  }
+  if (warp == 17) tmem_alloc<1>(smem_addr(&tmem_base), 512);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_base;
+  depend_launch();
+
+  const int per_round = gridDim.x * SLOTS, rounds = (a.tiles + per_round - 1) / per_round;
+  auto tile_of = [&](int round, int slot) { return round * per_round + slot * (int)gridDim.x + (int)blockIdx.x; };
+
+  if (warp < 4 * SLOTS) {  // unpacks
+    const int slot = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t quarter = (uint32_t)(warp & 3) << 21;
+    int s = 0, ph = 0, buf = 0, buf_ph = 0;
+    bool ok = true;
+    for (int r = 0; r < rounds && ok; ++r) {
+      const bool there = tile_of(r, slot) < a.tiles;
+      for (int b = 0; b < a.blocks && ok; ++b) {
+        if (!(ok = bar_wait(full + 8 * s, ph))) break;
+        uint4 w[4];
+        const uint32_t at = base + s * stage + slot * TILE_BYTES + row * BLOCK_BYTES;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(w[t].x), "=r"(w[t].y), "=r"(w[t].z), "=r"(w[t].w)
+                       : "r"(at + ((t ^ ((row >> 1) & 3)) << 4)));
         __syncwarp();
-        if (lane == 0) bar_arrive_cluster(empty + 8 * s);
+        if (lane == 0) bar_arrive(empty + 8 * s);
+        if (++s == a.stages) {
+          s = 0;
+          ph ^= 1;
+        }
+        if (!there) continue;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t v[32];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const uint32_t word = ((const uint32_t*)&w[c & 3])[2 * h + (c >> 2)];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[4 * c + i] = unpack<F16>(word, i);
+          }
+          if (!(ok = bar_wait(a_empty + 8 * (2 * slot + buf), buf_ph ^ 1))) break;
+          fence_after();
+          tmem_store32(tmem + a_column(slot, buf) + quarter, v);
+          tmem_store_wait();
+          fence_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive(a_full + 8 * (2 * slot + buf));
+          buf ^= 1;
+          if (buf == 0) buf_ph ^= 1;
+        }
+      }
+    }
+  } else if (warp < 8 * SLOTS) {  // adds up
+    depend_wait();
+    const int slot = (warp - 4 * SLOTS) >> 2;
+    const uint32_t quarter = (uint32_t)(warp & 3) << 21;
+    int buf = 0, buf_ph = 0;
+    bool ok = true;
+    for (int r = 0; r < rounds && ok; ++r) {
+      const int tile = tile_of(r, slot);
+      if (tile >= a.tiles) break;
+      const int v = tile * TILE + (warp & 3) * 32 + lane;
+      const uint4* scales = (const uint4*)(a.scale + (long long)min(v, a.V - 1) * a.scale_ld);
+      float acc[64];
+#pragma unroll
+      for (int c = 0; c < 64; ++c) acc[c] = 0.0f;
+      const int groups = a.blocks * (BLOCK / GROUP);
+      uint4 eight = __ldg(scales), next = eight;
+      for (int g = 0; g < groups && ok; ++g) {
+        if ((g & 7) == 0) {
+          if (g) eight = next;
+          if (g + 8 < groups) next = __ldg(scales + (g >> 3) + 1);
+        }
+        const uint32_t two = g & 4 ? (g & 2 ? eight.w : eight.z) : (g & 2 ? eight.y : eight.x);
+        const float scale = bitsf(g & 1 ? two & 0xffff0000u : two << 16);
+        if (!(ok = bar_wait(d_full + 8 * (2 * slot + buf), buf_ph))) break;
+        fence_after();
+#pragma unroll
+        for (int c = 0; c < 64; c += 16) {
+          if (c < a.columns) {
+            uint32_t sum[16];
+            tmem_load16(tmem + d_column(slot, buf) + quarter + c, sum);
+            tmem_load_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[c + i] = fmaf(scale, bitsf(sum[i]), acc[c + i]);
+          }
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(d_empty + 8 * (2 * slot + buf));
+        buf ^= 1;
+        if (buf == 0) buf_ph ^= 1;
+      }
+      if (v < a.V) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          if (c < a.rows) store_logit(a, c, v, ok ? acc[c] : NAN);  // NaN: a wait gave up
+      }
+    }
+  } else if (warp == 8 * SLOTS) {  // copies
+    if (elect_one()) {
+      tma_prefetch(&weights);
+      depend_wait();
+      int s = 0, ph = 0;
+      bool ok = true;
+      for (int r = 0; r < rounds && ok; ++r) {
+        for (int b = 0; b < a.blocks; ++b) {
+          if (!(ok = bar_wait(empty + 8 * s, ph ^ 1))) break;
+          const uint32_t to = base + s * stage;
+          int there = 0;
+          for (int slot = 0; slot < SLOTS; ++slot) there += tile_of(r, slot) < a.tiles;
+          bar_expect(full + 8 * s, there * TILE_BYTES + x_bytes);
+          for (int slot = 0; slot < there; ++slot)
+            tma_load<1>(to + slot * TILE_BYTES, &weights, full + 8 * s, b * BLOCK_BYTES, tile_of(r, slot) * TILE);
+          bulk_load(to + SLOTS * TILE_BYTES, (const char*)a.operand + (long long)b * x_bytes, full + 8 * s, x_bytes);
+          if (++s == a.stages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+      for (int i = 0; i < a.stages && ok; ++i) {  // every stage is read
+        ok = bar_wait(empty + 8 * s, ph ^ 1);
         if (++s == a.stages) {
           s = 0;
           ph ^= 1;
         }
       }
-    } else {
-      for (int b = part; b < a.blocks; b += kw) {
-        if (which)
-          multiply(held[1], xs + b * per_block);
-        else
-          multiply(held[0], xs + b * per_block);
-        which ^= 1;
-      }
+      if (!ok)
+        for (int i = 0; i < a.stages; ++i) bar_wait(full + 8 * i, ph);  // copies in flight
     }
-    const int tile = ((int)blockIdx.x + r * (int)gridDim.x) * slots + slot;
-    if (kw > 1) {
-      // [slot][part - 1][values][lane]
-      float* to = sums + ((long long)slot * (kw - 1) + (part - 1)) * (8 * NT) * 32 + lane;
-      if (part) {
+  } else {  // issues the products
+    if (elect_one()) {
+      const uint32_t desc = mma_desc(!F16, false, false, TILE, a.columns);
+      int s = 0, ph = 0, abuf = 0, a_ph = 0, dbuf[SLOTS] = {}, d_ph[SLOTS] = {};
+      bool ok = true;
+      for (int r = 0; r < rounds && ok; ++r) {
+        int there = 0;
+        for (int slot = 0; slot < SLOTS; ++slot) there += tile_of(r, slot) < a.tiles;
+        for (int b = 0; b < a.blocks && ok; ++b) {
+          if (!(ok = bar_wait(full + 8 * s, ph))) break;
+          const uint32_t x = base + s * stage + SLOTS * TILE_BYTES;
+          for (int h = 0; h < 2 && ok; ++h) {
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+            for (int slot = 0; slot < SLOTS; ++slot) {
+              if (slot >= there || !ok) continue;
+              if (!(ok = bar_wait(a_full + 8 * (2 * slot + abuf), a_ph))) break;
+              fence_after();
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+              for (int k = 0; k < 4; ++k) {
+                const int at = 64 * h + 16 * k;  // in the block
+                if (at % GROUP == 0) {
+                  if (!(ok = bar_wait(d_empty + 8 * (2 * slot + dbuf[slot]), d_ph[slot] ^ 1))) break;
+                  fence_after();
+                }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) to[((m * NT + n) * 4 + e) * 32] = acc[m][n][e];
-      }
-      multipliers_sync(a.warps * 32);
-      if (!part) {
-        for (int k = 1; k < kw; ++k) {
-          const float* from = sums + ((long long)slot * (kw - 1) + (k - 1)) * (8 * NT) * 32 + lane;
-#pragma unroll
-          for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) acc[m][n][e] += from[((m * NT + n) * 4 + e) * 32];
+                for (int p = 0; p < P; ++p)
+                  mma_f16_tmem(tmem + d_column(slot, dbuf[slot]), tmem + a_column(slot, abuf) + 8 * k,
+                               operand_desc(x + (h * P + p) * x_half, 0) + 2 * k, desc, at % GROUP != 0 || p > 0);
+                if ((at + 16) % GROUP == 0) {
+                  mma_commit<1>(d_full + 8 * (2 * slot + dbuf[slot]));
+                  dbuf[slot] ^= 1;
+                  if (dbuf[slot] == 0) d_ph[slot] ^= 1;
+                }
+              }
+              if (ok) mma_commit<1>(a_empty + 8 * (2 * slot + abuf));
+            }
+            abuf ^= 1;
+            if (abuf == 0) a_ph ^= 1;
+          }
+          if (ok) mma_commit<1>(empty + 8 * s);
+          if (++s == a.stages) {
+            s = 0;
+            ph ^= 1;
+          }
         }
       }
-      multipliers_sync(a.warps * 32);
-    }
-    if (part == 0 && tile < a.tiles) {
-#pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int c = n * 8 + 2 * t + (e & 1), v = tile * ROWS + 16 * m + 8 * (e >> 1) + g;
-            if (c >= a.rows || v >= a.V) continue;
-            const float y = ok ? acc[m][n][e] : NAN;  // NaN: a wait gave up
-            const long long at = c * a.y_ld + v;
-            if (a.out == 0)
-              ((float*)a.y)[at] = y;
-            else if (a.out == 1)
-              ((__nv_bfloat16*)a.y)[at] = __float2bfloat16_rn(y);
-            else
-              ((__half*)a.y)[at] = __float2half_rn(y);
-          }
     }
   }
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 17) tmem_free<1>(tmem, 512);
 }
 
 }  // namespace pesti_q4

@@ -203,7 +203,7 @@ def quantize_head(head, group: int = 64, stream=None) -> QuantizedHead:
     def call(st):
         blocks = -(-D // _BLOCK)
         packed = torch.empty((V, blocks * (_BLOCK // 2)), dtype=torch.uint8, device=head.device)
-        scale = torch.empty((V, blocks * (_BLOCK // group)), dtype=torch.bfloat16, device=head.device)
+        scale = torch.empty((V, -(-blocks * (_BLOCK // group) // 8) * 8), dtype=torch.bfloat16, device=head.device)
         _check(load_library().pesti_q4_quantize(head.data_ptr(), _DTYPES[head.dtype], V, D, _row_stride(head), group,
                                                 packed.data_ptr(), scale.data_ptr(), st))
         return QuantizedHead(packed, scale, D, group)
@@ -225,7 +225,7 @@ def head_logits(x, held: QuantizedHead, dtype=None, out=None, stream=None):
     summed in float32, times the scales in float32.  dtype: the logits' type
     (None: x's), or out: the [B, V] tensor to fill (rows may be strided).  Made
     for the few rows of a decode step: the weight is read once for every 64 rows
-    of 16-bit x, or 21 of float32."""
+    of x."""
     _need(x.dim() == 2 and x.dtype in _DTYPES, "x must be a [B, D] float32, bfloat16 or float16 tensor")
     (B, D), dev = x.shape, x.device
     _need(D == held.D, "x and the held weight have different D")
