@@ -549,12 +549,12 @@ int pesti_linear_ce_backward(const void* d_hidden, pesti_dtype dtype, int64_t N,
  *   s = bf16(-m / 8), m the group's largest value by magnitude, the first of
  *       equal ones;  q = clamp(round-half-even(w / s), -8, 7)  (0 where s is 0)
  * A group with an infinity or a NaN is held as NaN.
- * Layout, with B = ceil(D / 128) blocks a row: d_q has 64 B bytes a row, d_scale
- * 128 B / group bf16 a row, to a multiple of 8 (zeros behind the last
- * block's); both are 16-byte aligned.  In a block's 16 32-bit words,
- * word 4t + j (t, j = 0..3) holds columns 32j + 8t to 32j + 8t + 7 as q + 8, the
- * first in its lowest 4 bits; columns from D on hold 8 (q = 0).
- *
+ * Layout: tiles of 16 rows and 128 columns.  d_q: 1024 bytes a tile, [ceil(V /
+ * 16)][ceil(D / 128)][16 rows][4 chunks][4 words]; d_scale: bf16 [ceil(V / 16)]
+ * [ceil(D / 128)][16 rows][128 / group]; both 16-byte aligned.  Chunk c of row r
+ * (0 to 15) of a tile has t = c ^ (r / 2 % 4); its 32-bit word j holds the tile's
+ * columns 32j + 8t to 32j + 8t + 7 as q + 8, the first in its lowest 4 bits.
+ * Columns from D on and rows from V on hold 8 (q = 0), rows from V on scales of 0.
  * pesti_q4_quantize fills d_q and d_scale.  pesti_q4_dequantize writes q s
  * (exact in F32, else rounded once).  Buffers do not overlap (refused).
  * pesti_q4_logits: d_logits [B, ld] (first V columns; F32, BF16 or F16) = x

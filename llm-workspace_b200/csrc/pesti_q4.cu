@@ -32,8 +32,10 @@ int check_held(int64_t V, int64_t D, int64_t group, const void* q, const void* s
 
 long long blocks_of(int64_t D) { return (D + BLOCK - 1) / BLOCK; }
 
-// Scales of a row, in whole 16 bytes.
-int scale_row(int64_t D, int64_t group) { return (int)((blocks_of(D) * (BLOCK / group) + 7) / 8 * 8); }
+// Tiles of the held weight; its bytes are TILE_BYTES of q a tile, and ROWS * BLOCK / group scales.
+long long tiles_of(int64_t V, int64_t D) { return (V + ROWS - 1) / ROWS * blocks_of(D); }
+
+constexpr int TILE_BYTES = TILE_WORDS * 4;
 
 bool overlap(const void* p, __int128 np, const void* q, __int128 nq) {
   return (__int128)(uintptr_t)p < (__int128)(uintptr_t)q + nq && (__int128)(uintptr_t)q < (__int128)(uintptr_t)p + np;
@@ -62,11 +64,9 @@ int check_plain(const void* w, pesti_dtype dtype, int64_t V, int64_t D, int64_t 
   if (ld < D && V > 1) return refuse("ld is below D");
   if (!w) return refuse("null head");
   if ((uintptr_t)w % esize(dtype)) return refuse("the head is not aligned to its type");
-  const long long n = V * blocks_of(D);
-  const __int128 scales = (__int128)V * scale_row(D, group) * 2;
+  const __int128 tiles = tiles_of(V, D), held = tiles * TILE_BYTES, scales = tiles * (ROWS * BLOCK / group) * 2;
   const __int128 plain = ((__int128)(V - 1) * ld + D) * esize(dtype);
-  if (overlap(w, plain, q, (__int128)n * BLOCK_BYTES) || overlap(w, plain, scale, scales) ||
-      overlap(q, (__int128)n * BLOCK_BYTES, scale, scales))
+  if (overlap(w, plain, q, held) || overlap(w, plain, scale, scales) || overlap(q, held, scale, scales))
     return refuse("head, weights and scales overlap");
   return PESTI_OK;
 }
@@ -86,9 +86,9 @@ int convert(bool there, const void* w, int64_t V, int64_t D, int64_t ld, void* q
   a.scale = (__nv_bfloat16*)scale;
   a.D = (int)D;
   a.blocks = (int)blocks_of(D);
-  a.scale_ld = scale_row(D, GROUP);
+  a.V = (int)V;
   a.runs = (a.blocks + per<T>(there) - 1) / per<T>(there);
-  a.total = V * a.runs;
+  a.total = (there ? (V + ROWS - 1) / ROWS * ROWS : V) * a.runs;
   const int align = there || sizeof(T) == 4 ? 32 : 16, teams = there ? 32 : 16;  // of a thread block
   a.vec = (uintptr_t)w % align == 0 && (V == 1 || ld * sizeof(T) % align == 0);
   const long long grid = (a.total + teams - 1) / teams;
@@ -128,23 +128,22 @@ bool few(int64_t D, int pieces, int64_t rows) {
   return rows <= FEW_ROWS && blocks_of(D) * rows * pieces * (BLOCK * 2) <= SHARED_BYTES;
 }
 
-// How a pass shares its tiles and their K out: the least time of the busiest SM, by the weight's bytes that it reads (44
-// bytes a nanosecond, with 20 warps or more) and a microsecond and a half per round of tiles.
-void share_out(LogitArgs& a, int sms) {
+// How a pass with few rows shares its stacks and K out: the least time of the busiest SM, by the weight's bytes that it
+// reads (44 bytes a nanosecond), half a microsecond per round of stacks, and 50 ns for each part of a sum that is joined.
+int k_warps_of(long long stacks, int blocks, int warps, int sms) {
   double best = 1e30;
-  for (int kw = 1; kw <= 8 && kw <= a.blocks; kw *= 2) {
-    for (int w = kw; w <= MOST_WARPS; w += kw) {
-      const int slots = w / kw;
-      const long long rounds = (a.tiles + (long long)sms * slots - 1) / ((long long)sms * slots);
-      const double bytes = (double)rounds * slots * a.blocks * (ROWS * BLOCK_BYTES);
-      const double t = bytes / (w >= 20 ? 44.0 : 44.0 * w / 20) + (kw > 1 ? 1800.0 : 1500.0) * rounds;
-      if (t < best) {
-        best = t;
-        a.warps = w;
-        a.k_warps = kw;
-      }
+  int at = 1;
+  for (int kw = 1; kw <= warps && kw <= blocks; ++kw) {
+    if (warps % kw) continue;
+    const int slots = warps / kw, turns = (blocks + kw - 1) / kw;
+    const long long rounds = (stacks + (long long)sms * slots - 1) / ((long long)sms * slots);
+    const double t = (double)rounds * (warps * turns * (STACK * TILE_BYTES) / 44.0 + 500.0 + 50.0 * kw);
+    if (t < best) {
+      best = t;
+      at = kw;
     }
   }
+  return at;
 }
 
 template <typename... K, typename... A>
@@ -167,29 +166,37 @@ int launch(const char* what, void (*kernel)(K...), long long blocks, int threads
   return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, what);
 }
 
+template <typename T, int GROUP, int COLUMNS>
+int wide_pass(const LogitArgs& a, int sms, const CUtensorMap& weights, cudaStream_t st) {
+  return launch("q4_wide_kernel launch", q4_wide_kernel<T, GROUP, COLUMNS>, std::min(sms, a.stacks), WIDE_THREADS,
+                1024 + a.stages * (SLOTS * WIDE_BYTES + COLUMNS * (sizeof(T) == 4 ? 3 : 1) * (BLOCK * 2)), st, weights,
+                a);
+}
+
 template <typename T, int GROUP>
 int pass(LogitArgs a, int sms, cudaStream_t st) {
   constexpr int P = sizeof(T) == 4 ? 3 : 1;
   if (few(a.D, P, a.rows)) {
-    a.tiles = (a.V + ROWS - 1) / ROWS;
-    share_out(a, sms);
-    const int slots = a.warps / a.k_warps;
-    const int smem = a.blocks * a.rows * P * (BLOCK * 2) + 16 + (a.warps - slots) * 4 * 32 * 4;
+    a.stacks = (a.V + STACK * ROWS - 1) / (STACK * ROWS);
+    a.k_warps = k_warps_of(a.stacks, a.blocks, few_warps(P), sms);
+    const int slots = few_warps(P) / a.k_warps;
+    const int smem = a.blocks * a.rows * P * (BLOCK * 2) + 16 + (few_warps(P) - slots) * STACK * 4 * 32 * 4;
     return launch("q4_logits_kernel launch", q4_logits_kernel<T, GROUP>,
-                  std::min<long long>(sms, (a.tiles + slots - 1) / slots), a.warps * 32, smem, st, a);
+                  std::min<long long>(sms, (a.stacks + slots - 1) / slots), few_warps(P) * 32, smem, st, a);
   }
-  a.tiles = (a.V + TILE - 1) / TILE;
-  a.columns = columns_of(a.rows);
+  a.stacks = (a.V + WIDE - 1) / WIDE;
+  const int columns = columns_of(a.rows);
   CUtensorMap weights;
-  const long long row = (long long)a.blocks * BLOCK_BYTES;
-  int rc = pesti_tensor_map(&weights, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.q, row, a.V, row, BLOCK_BYTES, TILE,
-                            CU_TENSOR_MAP_SWIZZLE_64B);
-  if (!rc) rc = launch("q4_operand_kernel launch", q4_operand_kernel<T>, a.blocks, 256, 0, st, a);
+  const long long row = (long long)a.blocks * TILE_BYTES;
+  int rc = pesti_tensor_map(&weights, CU_TENSOR_MAP_DATA_TYPE_UINT32, a.q, row / 4, (a.V + ROWS - 1) / ROWS, row,
+                            TILE_WORDS, WIDE / ROWS, CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (!rc) rc = launch("q4_operand_kernel launch", q4_operand_kernel<T>, a.blocks, 256, 0, st, a, columns);
   if (rc) return rc;
-  const int stage = SLOTS * TILE_BYTES + a.columns * P * (BLOCK * 2);
-  a.stages = std::min(8, SHARED_BYTES / stage);
-  return launch("q4_wide_kernel launch", q4_wide_kernel<T, GROUP>, std::min(sms, a.tiles), WIDE_THREADS,
-                1024 + a.stages * stage, st, weights, a);
+  a.stages = std::min(8, SHARED_BYTES / (SLOTS * WIDE_BYTES + columns * P * (BLOCK * 2)));
+  if (columns == 16) return wide_pass<T, GROUP, 16>(a, sms, weights, st);
+  if (columns == 32) return wide_pass<T, GROUP, 32>(a, sms, weights, st);
+  if (columns == 48) return wide_pass<T, GROUP, 48>(a, sms, weights, st);
+  return wide_pass<T, GROUP, 64>(a, sms, weights, st);
 }
 
 template <typename T>
@@ -252,9 +259,9 @@ int pesti_q4_logits(const void* d_x, pesti_dtype dtype, int64_t B, int64_t D, in
   if ((uintptr_t)d_x % esize(dtype)) return refuse("x is not aligned to its type");
   if ((uintptr_t)d_logits % esize(out_dtype)) return refuse("logits are not aligned to their type");
   const __int128 nx = ((__int128)(B - 1) * x_ld + D) * esize(dtype), ny = ((__int128)(B - 1) * ld + V) * esize(out_dtype);
-  const __int128 nb = (__int128)V * blocks_of(D);
-  if (overlap(d_logits, ny, d_x, nx) || overlap(d_logits, ny, d_q, nb * BLOCK_BYTES) ||
-      overlap(d_logits, ny, d_scale, (__int128)V * scale_row(D, group) * 2))
+  const __int128 tiles = tiles_of(V, D);
+  if (overlap(d_logits, ny, d_x, nx) || overlap(d_logits, ny, d_q, tiles * TILE_BYTES) ||
+      overlap(d_logits, ny, d_scale, tiles * (ROWS * BLOCK / group) * 2))
     return refuse("inputs and logits overlap");
   if (!d_ws || ws_bytes < need) return refuse("workspace too small");
   if ((uintptr_t)d_ws % 256) return refuse("workspace is not 256-byte aligned");
@@ -269,7 +276,6 @@ int pesti_q4_logits(const void* d_x, pesti_dtype dtype, int64_t B, int64_t D, in
   a.scale = (const __nv_bfloat16*)d_scale;
   a.V = (int)V;
   a.blocks = (int)blocks_of(D);
-  a.scale_ld = scale_row(D, group);
   a.operand = (uint4*)d_ws;
   a.y = d_logits;
   a.y_ld = ld;

@@ -3,9 +3,11 @@
 //   s = bf16(-m / 8), m the group's largest value by magnitude (the first of equal ones)
 //   q = clamp(rint(w / s), -8, 7),  y = x (q s)^T
 //
-// Layout.  A row is padded to blocks of 128 columns of 64 bytes; word 4 t + j of a block (t, j = 0..3) holds columns
-// 32 j + 8 t to + 7, eight nibbles q + 8 from its low end.  So 16 bytes at word 4 t are what lane t of a quad of an
-// m16n8k16 product needs for four steps of 32 columns, none of which crosses a group.
+// Layout.  Tiles of 16 rows and 128 columns of 1024 bytes, [ceil(V / 16)][ceil(D / 128)][16 rows][64 bytes].  A row's
+// 16-byte chunk t is at place t ^ (row / 2 % 4), and its word j holds columns 32 j + 8 t to + 7: eight nibbles q + 8
+// from its low end.  So a chunk is what lane t of a quad of an m16n8k16 product needs for four steps of 32 columns, none
+// of which crosses a group; a warp reads a tile in two whole loads; and threads that take a row of a tile each read
+// their chunks from shared memory without bank conflicts.  Scales: [ceil(V / 16)][ceil(D / 128)][16 rows][128 / group].
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -19,7 +21,6 @@ namespace pesti_q4 {
 
 constexpr int BLOCK = 128;  // columns
 constexpr int BLOCK_BYTES = BLOCK / 2;
-constexpr int MOST_WARPS = 24;  // of a block that multiplies few rows
 
 template <typename T>
 __device__ __forceinline__ float to_f32(T v) {
@@ -41,8 +42,17 @@ __device__ __forceinline__ T from_f32(float v) {
     return __float2bfloat16_rn(v);
 }
 
-// The word of columns 8 i to 8 i + 7 of a block: i = 4 j + t is at 4 t + j.
-__device__ __forceinline__ int word_of(int i) { return (i & 3) * 4 + (i >> 2); }
+constexpr int ROWS = 16;                          // of a tile
+constexpr int TILE_WORDS = ROWS * BLOCK_BYTES / 4;
+
+// Where chunk t of a row is among the row's four.
+__host__ __device__ __forceinline__ int chunk_at(int row, int t) { return t ^ (row >> 1 & 3); }
+
+// The tile of a row's block, and in it the word of its columns 8 i to 8 i + 7, i = 4 j + t.
+__device__ __forceinline__ long long tile_of(long long row, int blocks, int block) { return (row >> 4) * blocks + block; }
+__device__ __forceinline__ int word_of(int row, int i) {
+  return (row & 15) * (BLOCK_BYTES / 4) + chunk_at(row, i & 3) * 4 + (i >> 2);
+}
 
 template <typename T>
 struct Held {
@@ -51,7 +61,7 @@ struct Held {
   uint32_t* q;
   __nv_bfloat16* scale;
   int D, blocks, runs;  // blocks of a row, and runs of PER blocks that a team takes
-  int scale_ld;         // scales of a row
+  int V;
   long long total;      // runs in all
   int vec;              // whole vectors of 8 columns can be read or written
 };
@@ -193,10 +203,12 @@ __global__ void __launch_bounds__(256) q4_quantize_kernel(const Held<T> a) {
   const T* from = a.w + row * a.ld;
 #pragma unroll
   for (int u = 0; u < PER; ++u)
-    if (u < n) in[u].load(from, (b0 + u) * BLOCK + 16 * i, a.D, a.vec);
-  const long long b = row * a.blocks + b0;
-  uint32_t* to = a.q + b * (BLOCK / 8) + word_of(2 * i);  // (the other word is 4 behind it)
-  __nv_bfloat16* scale = a.scale + row * a.scale_ld + b0 * (BLOCK / GROUP) + i / (GROUP / 16);
+    if (u < n && row < a.V) in[u].load(from, (b0 + u) * BLOCK + 16 * i, a.D, a.vec);
+  const long long b = tile_of(row, a.blocks, b0);
+  const bool real = row < a.V;  // (rows to a whole tile are held as zeros)
+  uint32_t* to = a.q + b * TILE_WORDS;
+  const int word0 = word_of(row, 2 * i), word1 = word_of(row, 2 * i + 1);
+  __nv_bfloat16* scale = a.scale + (b * ROWS + (row & 15)) * (BLOCK / GROUP) + i / (GROUP / 16);
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
     float hi, neg;
@@ -232,12 +244,10 @@ __global__ void __launch_bounds__(256) q4_quantize_kernel(const Held<T> a) {
         word[h] = codes_of(v, t, sizeof(T) == 4);
       }
     }
-    to[u * (BLOCK / 8)] = word[0];
-    to[u * (BLOCK / 8) + 4] = word[1];
-    if (i % (GROUP / 16) == 0) scale[u * (BLOCK / GROUP)] = held;
+    to[u * TILE_WORDS + word0] = real ? word[0] : 0x88888888u;
+    to[u * TILE_WORDS + word1] = real ? word[1] : 0x88888888u;
+    if (i % (GROUP / 16) == 0) scale[u * ROWS * (BLOCK / GROUP)] = real ? held : __nv_bfloat16(0.0f);
   }
-  if (there && i == 0 && b0 + n == a.blocks)  // the row's last: zeros to whole 16 bytes
-    for (int e = a.blocks * (BLOCK / GROUP); e < a.scale_ld; ++e) a.scale[row * a.scale_ld + e] = __nv_bfloat16(0.0f);
 }
 
 // Two lanes of a team of sixteen hold neighbouring words; f32 rows are written 32 bytes a lane, 16-bit ones 16.
@@ -248,16 +258,16 @@ __global__ void __launch_bounds__(256) q4_dequantize_kernel(const Held<T> a) {
   int b0;
   if (!place_of<T, PER, 16>(a, row, b0)) return;
   const int n = min(PER, a.blocks - b0);
-  const long long b = row * a.blocks + b0;
-  const uint32_t* from = a.q + b * (BLOCK / 8) + word_of(i);
-  const __nv_bfloat16* scale = a.scale + row * a.scale_ld + b0 * (BLOCK / GROUP) + i / (GROUP / 8);
+  const long long b = tile_of(row, a.blocks, b0);
+  const uint32_t* from = a.q + b * TILE_WORDS + word_of(row, i);
+  const __nv_bfloat16* scale = a.scale + (b * ROWS + (row & 15)) * (BLOCK / GROUP) + i / (GROUP / 8);
   uint32_t w[PER];
   float s[PER];
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
     if (u < n) {
-      w[u] = __ldcs(from + u * (BLOCK / 8));
-      s[u] = __bfloat162float(scale[u * (BLOCK / GROUP)]);
+      w[u] = __ldcs(from + u * TILE_WORDS);
+      s[u] = __bfloat162float(scale[u * ROWS * (BLOCK / GROUP)]);
     }
   }
   T* to = const_cast<T*>(a.w) + row * a.ld;
@@ -291,14 +301,13 @@ struct LogitArgs {
   int rows, D;  // of x; at most 64 rows
   const uint4* q;
   const __nv_bfloat16* scale;
-  int V, blocks, tiles;
+  int V, blocks, stacks;  // stacks of 64 rows, or of 128
   uint4* operand;        // x for the tensor cores (q4_operand_kernel)
-  int columns, stages;   // its rows, to a multiple of 16, and how many blocks are in shared memory at once
+  int stages;            // blocks in shared memory at once
   void* y;
   long long y_ld;
   int out;               // 0 f32, 1 bf16, 2 f16
-  int warps, k_warps;    // warps that multiply, and how many of them share a tile's K
-  int scale_ld;          // scales of a row
+  int k_warps;           // warps that share a stack's K
 };
 
 __device__ __forceinline__ void store_logit(const LogitArgs& a, int row, int v, float y) {
@@ -372,26 +381,23 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(z0), "f"(z1), "f"(z2), "f"(z3));
 }
 
-constexpr int ROWS = 16;  // of the weight, per warp and tile
-
-// A lane's weights of one block: 16 bytes of two rows (8 apart), and their groups' scales.
+// A lane's weights of a tile: 16 bytes of two rows (8 apart), and their groups' scales.
 template <int GROUP>
 struct Weights {
   uint4 w[2];
   uint2 s[2];  // up to four bf16
 
-  __device__ __forceinline__ void load(const char* q, uint32_t q_at, uint32_t q_far, const char* sc, uint32_t s_at,
-                                       uint32_t s_far) {
+  __device__ __forceinline__ void load(const uint4* q, const __nv_bfloat16* sc) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      w[i] = __ldcs((const uint4*)(q + (q_at + i * q_far)));
-      const char* p = sc + (s_at + i * s_far);
+      w[i] = __ldcs(q + i * (TILE_WORDS / 8));
+      const __nv_bfloat16* p = sc + i * 8 * (BLOCK / GROUP);
       if constexpr (GROUP == 32)
-        s[i] = __ldg((const uint2*)p);
+        s[i] = __ldcs((const uint2*)p);
       else if constexpr (GROUP == 64)
-        s[i].x = __ldg((const uint32_t*)p);
+        s[i].x = __ldcs((const uint32_t*)p);
       else
-        s[i].x = __ldg((const uint16_t*)p);
+        s[i].x = __ldcs((const uint16_t*)p);
     }
   }
 
@@ -401,52 +407,59 @@ struct Weights {
   }
 };
 
-// Up to 8 rows of x: a warp multiplies 16 rows of the weight by all of them over its share of K (every k_warps-th
-// block), and goes on to its next tile; the k_warps warps of a tile join their sums in shared memory, in their order.
-// x is laid out in shared memory once, while the first weights are on their way; weights are loaded two blocks ahead.
+constexpr int STACK = 4;  // tiles of a warp, one above the other: x's fragments of a block serve them all
+
+// Warps that multiply: their registers hold a stack's sums and next weights and the fragments of a block of x.
+__host__ __device__ constexpr int few_warps(int pieces) { return pieces == 1 ? 16 : 12; }
+
+// Up to 8 rows of x: a warp multiplies a stack of 64 rows of the weight by all of them over its share of K (every
+// k_warps-th block), and goes on to its next stack; the k_warps warps of a stack join their sums in shared memory, in
+// their order.  x is laid out in shared memory once, while the first weights are on their way; a tile's weights are
+// loaded a block ahead.
 template <typename T, int GROUP>
-__global__ void __launch_bounds__(MOST_WARPS * 32, 1) q4_logits_kernel(const LogitArgs a) {
+__global__ void __launch_bounds__(few_warps(sizeof(T) == 4 ? 3 : 1) * 32, 1) q4_logits_kernel(const LogitArgs a) {
   constexpr bool F16 = std::is_same<T, __half>::value;
-  constexpr int P = sizeof(T) == 4 ? 3 : 1;
+  constexpr int P = sizeof(T) == 4 ? 3 : 1, WARPS = few_warps(P);
   extern __shared__ uint4 xs[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int kw = a.k_warps, slots = a.warps / kw, part = warp % kw, slot = warp / kw;
+  const int kw = a.k_warps, slots = WARPS / kw, part = warp % kw, slot = warp / kw;
   const int columns = a.rows, per_block = 16 * P * columns;  // 16-byte fragments of a block of x
-  const int rounds = (a.tiles + gridDim.x * slots - 1) / (gridDim.x * slots);
+  const int rounds = (a.stacks + gridDim.x * slots - 1) / (gridDim.x * slots);
   float* sums = (float*)(xs + a.blocks * per_block + 1);
   pesti_umma::depend_wait();
   pesti_umma::depend_launch();
 
-  // the next block to load
-  const uint32_t q_row = a.blocks * BLOCK_BYTES, s_row = a.scale_ld * 2;
-  uint32_t q_lane, q_far, s_lane, s_far;
-  const char *q, *sc;
-  auto rows_of = [&](int round) {
-    const int tile = min(((int)blockIdx.x + round * (int)gridDim.x) * slots + slot, a.tiles - 1);
-    q = (const char*)a.q + (long long)tile * ROWS * q_row;
-    sc = (const char*)a.scale + (long long)tile * ROWS * s_row;
-    const int last = a.V - 1 - tile * ROWS, r0 = min(g, last), r1 = min(g + 8, last);
-    q_lane = r0 * q_row + t * 16;
-    q_far = (r1 - r0) * q_row;
-    s_lane = r0 * s_row;
-    s_far = (r1 - r0) * s_row;
-  };
+  // the block to load next, of the stack of `load_round`
+  const uint4* q;
+  const __nv_bfloat16* sc;
   int load_round = 0, load_b = part;
-  rows_of(0);
-  Weights<GROUP> held[2];
-  auto load = [&](Weights<GROUP>& w) {
-    if (load_round >= rounds) return;
-    w.load(q, q_lane + load_b * BLOCK_BYTES, q_far, sc, s_lane + load_b * (2 * BLOCK / GROUP), s_far);
+  Weights<GROUP> held[STACK];
+  auto stack_of = [&](int round) { return (round * (int)gridDim.x + (int)blockIdx.x) * slots + slot; };
+  auto begin = [&]() {
+    const long long tile = (long long)min(stack_of(load_round), a.stacks - 1) * STACK * a.blocks + part;
+    q = a.q + tile * (TILE_WORDS / 4) + g * 4 + chunk_at(g, t);
+    sc = a.scale + (tile * ROWS + g) * (BLOCK / GROUP);
+  };
+  auto load = [&](int i) {
+    // a tile past the last row's is the last one again
+    const int up = min(i, (a.V - 1) / ROWS - min(stack_of(load_round), a.stacks - 1) * STACK) * a.blocks;
+    held[i].load(q + up * (TILE_WORDS / 4), sc + up * (ROWS * BLOCK / GROUP));
+  };
+  auto advance = [&]() {
     load_b += kw;
+    q += kw * (TILE_WORDS / 4);
+    sc += kw * (ROWS * BLOCK / GROUP);
     if (load_b >= a.blocks) {
       load_b = part;
-      if (++load_round < rounds) rows_of(load_round);
+      if (++load_round < rounds) begin();
     }
   };
-  load(held[0]);
-  load(held[1]);
+  begin();
+#pragma unroll
+  for (int i = 0; i < STACK; ++i) load(i);
+  advance();
 
-  for (int e = threadIdx.x; e < a.blocks * per_block; e += a.warps * 32) {
+  for (int e = threadIdx.x; e < a.blocks * per_block; e += WARPS * 32) {
     const int tt = e & 3, rest = e >> 2, c = rest % columns, bjp = rest / columns, p = bjp % P, bj = bjp / P;
     xs[e] = fragment_of((const T*)a.x + c * a.x_ld, bj >> 2, bj & 3, tt, p, a.D);
   }
@@ -457,73 +470,72 @@ __global__ void __launch_bounds__(MOST_WARPS * 32, 1) q4_logits_kernel(const Log
   const uint4* mine = there ? xs + g * 4 + t : xs + a.blocks * per_block;
   const int x_block = there ? per_block : 0, x_step = there ? 4 * columns : 0;
 
-  float acc[4];
-  auto multiply = [&](Weights<GROUP>& w, const uint4* x) {
-#pragma unroll
-    for (int gr = 0; gr < BLOCK / GROUP; ++gr) {
-      float sum[4];
-#pragma unroll
-      for (int jj = 0; jj < GROUP / 32; ++jj) {
-        const int j = gr * (GROUP / 32) + jj;
-        uint32_t fa[2][4];
-        const uint32_t w0 = ((const uint32_t*)&w.w[0])[j], w1 = ((const uint32_t*)&w.w[1])[j];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          fa[h][0] = unpack<F16>(w0, 2 * h);
-          fa[h][1] = unpack<F16>(w1, 2 * h);
-          fa[h][2] = unpack<F16>(w0, 2 * h + 1);
-          fa[h][3] = unpack<F16>(w1, 2 * h + 1);
-        }
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
-          const uint4 f = x[(j * P + p) * x_step];
-          if (jj == 0 && p == 0)
-            mma<F16, false>(sum, fa[0], f.x, f.y);
-          else
-            mma<F16, true>(sum, fa[0], f.x, f.y);
-          mma<F16, true>(sum, fa[1], f.z, f.w);
-        }
-      }
-      const float s0 = w.scale(0, gr), s1 = w.scale(1, gr);
-      acc[0] = fmaf(s0, sum[0], acc[0]);
-      acc[1] = fmaf(s0, sum[1], acc[1]);
-      acc[2] = fmaf(s1, sum[2], acc[2]);
-      acc[3] = fmaf(s1, sum[3], acc[3]);
-    }
-    load(w);
-  };
-
-  int which = 0;
   for (int r = 0; r < rounds; ++r) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] = 0.0f;
+    float acc[STACK][4] = {};
     for (int b = part; b < a.blocks; b += kw) {
-      if (which)
-        multiply(held[1], mine + b * x_block);
-      else
-        multiply(held[0], mine + b * x_block);
-      which ^= 1;
-    }
-    const int tile = ((int)blockIdx.x + r * (int)gridDim.x) * slots + slot;
-    if (kw > 1) {  // [slot][part - 1][value][lane]
-      float* to = sums + (slot * (kw - 1) + (part - 1)) * 4 * 32 + lane;
-      if (part) {
+      uint4 f[4][P];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) to[e * 32] = acc[e];
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int p = 0; p < P; ++p) f[j][p] = mine[b * x_block + (j * P + p) * x_step];
+#pragma unroll
+      for (int i = 0; i < STACK; ++i) {
+        const Weights<GROUP>& w = held[i];
+#pragma unroll
+        for (int gr = 0; gr < BLOCK / GROUP; ++gr) {
+          float sum[4];
+#pragma unroll
+          for (int jj = 0; jj < GROUP / 32; ++jj) {
+            const int j = gr * (GROUP / 32) + jj;
+            uint32_t fa[2][4];
+            const uint32_t w0 = ((const uint32_t*)&w.w[0])[j], w1 = ((const uint32_t*)&w.w[1])[j];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              fa[h][0] = unpack<F16>(w0, 2 * h);
+              fa[h][1] = unpack<F16>(w1, 2 * h);
+              fa[h][2] = unpack<F16>(w0, 2 * h + 1);
+              fa[h][3] = unpack<F16>(w1, 2 * h + 1);
+            }
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+              if (jj == 0 && p == 0)
+                mma<F16, false>(sum, fa[0], f[j][p].x, f[j][p].y);
+              else
+                mma<F16, true>(sum, fa[0], f[j][p].x, f[j][p].y);
+              mma<F16, true>(sum, fa[1], f[j][p].z, f[j][p].w);
+            }
+          }
+          const float s0 = w.scale(0, gr), s1 = w.scale(1, gr);
+          acc[i][0] = fmaf(s0, sum[0], acc[i][0]);
+          acc[i][1] = fmaf(s0, sum[1], acc[i][1]);
+          acc[i][2] = fmaf(s1, sum[2], acc[i][2]);
+          acc[i][3] = fmaf(s1, sum[3], acc[i][3]);
+        }
+        if (load_round < rounds) load(i);
+      }
+      advance();
+    }
+    const int stack = stack_of(r);
+    if (kw > 1) {  // [slot][part - 1][value][lane]
+      if (part) {
+        float* to = sums + (slot * (kw - 1) + (part - 1)) * STACK * 4 * 32 + lane;
+#pragma unroll
+        for (int e = 0; e < STACK * 4; ++e) to[e * 32] = acc[e >> 2][e & 3];
       }
       __syncthreads();
       if (!part) {
         for (int k = 0; k < kw - 1; ++k)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[e] += sums[((slot * (kw - 1) + k) * 4 + e) * 32 + lane];
+          for (int e = 0; e < STACK * 4; ++e)
+            acc[e >> 2][e & 3] += sums[((slot * (kw - 1) + k) * STACK * 4 + e) * 32 + lane];
       }
       __syncthreads();
     }
-    if (part || tile >= a.tiles) continue;
+    if (part || stack >= a.stacks) continue;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int c = 2 * t + (e & 1), v = tile * ROWS + 8 * (e >> 1) + g;
-      if (c < a.rows && v < a.V) store_logit(a, c, v, acc[e]);
+    for (int e = 0; e < STACK * 4; ++e) {
+      const int c = 2 * t + (e & 1), v = (stack * STACK + (e >> 2)) * ROWS + 8 * (e >> 1 & 1) + g;
+      if (c < a.rows && v < a.V) store_logit(a, c, v, acc[e >> 2][e & 3]);
     }
   }
 }
@@ -537,51 +549,54 @@ __global__ void __launch_bounds__(MOST_WARPS * 32, 1) q4_logits_kernel(const Log
 // x as the products' second operand, [blocks][2][pieces][columns][128 bytes]: half a block's 64 columns in the order
 // that words of weights unpack in, 16-byte chunks exchanged as 128-byte swizzled atoms hold them.
 template <typename T>
-__global__ void __launch_bounds__(256) q4_operand_kernel(const LogitArgs a) {
+__global__ void __launch_bounds__(256) q4_operand_kernel(const LogitArgs a, int columns) {
   pesti_umma::depend_wait();
   pesti_umma::depend_launch();
   constexpr int P = sizeof(T) == 4 ? 3 : 1;
-  const int per_block = 2 * P * a.columns * 8, b = blockIdx.x;
+  const int per_block = 2 * P * columns * 8, b = blockIdx.x;
   for (int e = threadIdx.x; e < per_block; e += 256) {
-    const int c = e & 7, n = (e >> 3) % a.columns, hp = (e >> 3) / a.columns, p = hp % P, h = hp / P;
+    const int c = e & 7, n = (e >> 3) % columns, hp = (e >> 3) / columns, p = hp % P, h = hp / P;
     uint4 f = make_uint4(0, 0, 0, 0);
     if (n < a.rows) f = fragment_of((const T*)a.x + n * a.x_ld, b, 2 * h + (c >> 2), c & 3, p, a.D);
     a.operand[(long long)b * per_block + (e & ~7) + (c ^ (n & 7))] = f;
   }
 }
 
-constexpr int TILE = 128;                      // rows of the weight
-constexpr int SLOTS = 2;                       // tiles at once
+constexpr int WIDE = 128;                       // rows of the weight, eight tiles
+constexpr int SLOTS = 2;                        // of them at once
 constexpr int WIDE_THREADS = (8 * SLOTS + 2) * 32;
-constexpr int TILE_BYTES = TILE * BLOCK_BYTES;  // of a block of weights
+constexpr int WIDE_BYTES = WIDE * BLOCK_BYTES;  // of a block
+constexpr int A_BUFS = 4;                       // of 64 of K, unpacked
 
-// Where a slot's buffers are in tensor memory: two of 64 of K, and two of sums.
+// Where a slot's buffers are in tensor memory: unpacked weights, and two of sums.
 __device__ __forceinline__ uint32_t a_column(int slot, int buf) { return slot * 256 + buf * 32; }
-__device__ __forceinline__ uint32_t d_column(int slot, int buf) { return slot * 256 + 64 + buf * 64; }
+__device__ __forceinline__ uint32_t d_column(int slot, int buf) { return slot * 256 + 128 + buf * 64; }
 
 // Warps 0 to 7 unpack (four a slot, a quarter of the rows each), 8 to 15 add up, 16 copies, 17 issues the products.
-template <typename T, int GROUP>
+template <typename T, int GROUP, int COLUMNS>
 __global__ void __launch_bounds__(WIDE_THREADS, 1)
     q4_wide_kernel(const __grid_constant__ CUtensorMap weights, const LogitArgs a) {
   using namespace pesti_umma;
   constexpr bool F16 = std::is_same<T, __half>::value;
   constexpr int P = sizeof(T) == 4 ? 3 : 1;
+  constexpr uint32_t x_half = COLUMNS * 128, x_bytes = 2 * P * x_half, stage = SLOTS * WIDE_BYTES + x_bytes;
   extern __shared__ char raw[];
   const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
-  const uint32_t x_half = a.columns * 128, x_bytes = 2 * P * x_half, stage = SLOTS * TILE_BYTES + x_bytes;
-  __shared__ uint64_t bars[16 + 8 * SLOTS];
+  __shared__ uint64_t bars[16 + SLOTS * (2 * A_BUFS + 4)];
   __shared__ uint32_t tmem_base;
-  const uint32_t full = smem_addr(bars), empty = full + 64, a_full = empty + 64, a_empty = a_full + 16 * SLOTS,
-                 d_full = a_empty + 16 * SLOTS, d_empty = d_full + 16 * SLOTS;
+  const uint32_t full = smem_addr(bars), empty = full + 64, a_full = empty + 64, a_empty = a_full + 8 * A_BUFS * SLOTS,
+                 d_full = a_empty + 8 * A_BUFS * SLOTS, d_empty = d_full + 16 * SLOTS;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < a.stages; ++s) {
       bar_init(full + 8 * s, 1);
       bar_init(empty + 8 * s, 4 * SLOTS + 1);
     }
-    for (int s = 0; s < 2 * SLOTS; ++s) {
+    for (int s = 0; s < A_BUFS * SLOTS; ++s) {
       bar_init(a_full + 8 * s, 4);
       bar_init(a_empty + 8 * s, 1);
+    }
+    for (int s = 0; s < 2 * SLOTS; ++s) {
       bar_init(d_full + 8 * s, 1);
       bar_init(d_empty + 8 * s, 4);
     }
@@ -592,10 +607,11 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
   __syncthreads();
   fence_after();
   const uint32_t tmem = tmem_base;
+  depend_wait();
   depend_launch();
 
-  const int per_round = gridDim.x * SLOTS, rounds = (a.tiles + per_round - 1) / per_round;
-  auto tile_of = [&](int round, int slot) { return round * per_round + slot * (int)gridDim.x + (int)blockIdx.x; };
+  const int per_round = gridDim.x * SLOTS, rounds = (a.stacks + per_round - 1) / per_round;
+  auto stack_of = [&](int round, int slot) { return round * per_round + slot * (int)gridDim.x + (int)blockIdx.x; };
 
   if (warp < 4 * SLOTS) {  // unpacks
     const int slot = warp >> 2, row = (warp & 3) * 32 + lane;
@@ -603,16 +619,16 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
     int s = 0, ph = 0, buf = 0, buf_ph = 0;
     bool ok = true;
     for (int r = 0; r < rounds && ok; ++r) {
-      const bool there = tile_of(r, slot) < a.tiles;
+      const bool there = stack_of(r, slot) < a.stacks;
       for (int b = 0; b < a.blocks && ok; ++b) {
         if (!(ok = bar_wait(full + 8 * s, ph))) break;
         uint4 w[4];
-        const uint32_t at = base + s * stage + slot * TILE_BYTES + row * BLOCK_BYTES;
+        const uint32_t at = base + s * stage + slot * WIDE_BYTES + row * BLOCK_BYTES;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
           asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                        : "=r"(w[t].x), "=r"(w[t].y), "=r"(w[t].z), "=r"(w[t].w)
-                       : "r"(at + ((t ^ ((row >> 1) & 3)) << 4)));
+                       : "r"(at + (chunk_at(row, t) << 4)));
         __syncwarp();
         if (lane == 0) bar_arrive(empty + 8 * s);
         if (++s == a.stages) {
@@ -629,81 +645,101 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[4 * c + i] = unpack<F16>(word, i);
           }
-          if (!(ok = bar_wait(a_empty + 8 * (2 * slot + buf), buf_ph ^ 1))) break;
+          if (!(ok = bar_wait(a_empty + 8 * (A_BUFS * slot + buf), buf_ph ^ 1))) break;
           fence_after();
           tmem_store32(tmem + a_column(slot, buf) + quarter, v);
           tmem_store_wait();
           fence_before();
           __syncwarp();
-          if (lane == 0) bar_arrive(a_full + 8 * (2 * slot + buf));
-          buf ^= 1;
-          if (buf == 0) buf_ph ^= 1;
+          if (lane == 0) bar_arrive(a_full + 8 * (A_BUFS * slot + buf));
+          if (++buf == A_BUFS) {
+            buf = 0;
+            buf_ph ^= 1;
+          }
         }
       }
     }
   } else if (warp < 8 * SLOTS) {  // adds up
-    depend_wait();
+    constexpr int PER = BLOCK / GROUP;  // groups of a block
+    constexpr int CHUNK = COLUMNS == 32 ? 32 : 16;  // (more columns leave no registers for more at once)
     const int slot = (warp - 4 * SLOTS) >> 2;
     const uint32_t quarter = (uint32_t)(warp & 3) << 21;
     int buf = 0, buf_ph = 0;
     bool ok = true;
     for (int r = 0; r < rounds && ok; ++r) {
-      const int tile = tile_of(r, slot);
-      if (tile >= a.tiles) break;
-      const int v = tile * TILE + (warp & 3) * 32 + lane;
-      const uint4* scales = (const uint4*)(a.scale + (long long)min(v, a.V - 1) * a.scale_ld);
-      float acc[64];
-#pragma unroll
-      for (int c = 0; c < 64; ++c) acc[c] = 0.0f;
-      const int groups = a.blocks * (BLOCK / GROUP);
-      uint4 eight = __ldg(scales), next = eight;
-      for (int g = 0; g < groups && ok; ++g) {
-        if ((g & 7) == 0) {
-          if (g) eight = next;
-          if (g + 8 < groups) next = __ldg(scales + (g >> 3) + 1);
+      const int stack = stack_of(r, slot);
+      if (stack >= a.stacks) break;
+      const int v = stack * WIDE + (warp & 3) * 32 + lane;
+      const long long tile = tile_of(min(v, a.V - 1), a.blocks, 0);
+      const __nv_bfloat16* scales = a.scale + (tile * ROWS + (v & 15)) * PER;
+      auto scale_of = [&](int b) {
+        uint2 s = make_uint2(0, 0);
+        if (b < a.blocks) {
+          const __nv_bfloat16* p = scales + b * (ROWS * PER);
+          if constexpr (GROUP == 32)
+            s = __ldcs((const uint2*)p);
+          else if constexpr (GROUP == 64)
+            s.x = __ldcs((const uint32_t*)p);
+          else
+            s.x = __ldcs((const uint16_t*)p);
         }
-        const uint32_t two = g & 4 ? (g & 2 ? eight.w : eight.z) : (g & 2 ? eight.y : eight.x);
-        const float scale = bitsf(g & 1 ? two & 0xffff0000u : two << 16);
-        if (!(ok = bar_wait(d_full + 8 * (2 * slot + buf), buf_ph))) break;
-        fence_after();
+        return s;
+      };
+      float acc[COLUMNS];
 #pragma unroll
-        for (int c = 0; c < 64; c += 16) {
-          if (c < a.columns) {
-            uint32_t sum[16];
-            tmem_load16(tmem + d_column(slot, buf) + quarter + c, sum);
+      for (int c = 0; c < COLUMNS; ++c) acc[c] = 0.0f;
+      uint2 next = scale_of(0), after = scale_of(1);
+      for (int b = 0; b < a.blocks && ok; ++b) {
+        const uint2 now = next;
+        next = after;
+        after = scale_of(b + 2);
+#pragma unroll
+        for (int g = 0; g < PER; ++g) {
+          const uint32_t two = g < 2 ? now.x : now.y;
+          const float scale = bitsf(g & 1 ? two & 0xffff0000u : two << 16);
+          if (!(ok = bar_wait(d_full + 8 * (2 * slot + buf), buf_ph))) break;
+          fence_after();
+          const uint32_t from = tmem + d_column(slot, buf) + quarter;
+#pragma unroll
+          for (int c = 0; c < COLUMNS; c += CHUNK) {
+            uint32_t sum[CHUNK];
+            if constexpr (CHUNK == 32)
+              tmem_load32(from + c, sum);
+            else
+              tmem_load16(from + c, sum);
             tmem_load_wait();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[c + i] = fmaf(scale, bitsf(sum[i]), acc[c + i]);
+            for (int i = 0; i < CHUNK; ++i) acc[c + i] = fmaf(scale, bitsf(sum[i]), acc[c + i]);
           }
+          fence_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive(d_empty + 8 * (2 * slot + buf));
+          buf ^= 1;
+          if (buf == 0) buf_ph ^= 1;
         }
-        fence_before();
-        __syncwarp();
-        if (lane == 0) bar_arrive(d_empty + 8 * (2 * slot + buf));
-        buf ^= 1;
-        if (buf == 0) buf_ph ^= 1;
       }
       if (v < a.V) {
 #pragma unroll
-        for (int c = 0; c < 64; ++c)
+        for (int c = 0; c < COLUMNS; ++c)
           if (c < a.rows) store_logit(a, c, v, ok ? acc[c] : NAN);  // NaN: a wait gave up
       }
     }
   } else if (warp == 8 * SLOTS) {  // copies
     if (elect_one()) {
       tma_prefetch(&weights);
-      depend_wait();
       int s = 0, ph = 0;
       bool ok = true;
       for (int r = 0; r < rounds && ok; ++r) {
+        int there = 0;
+        for (int slot = 0; slot < SLOTS; ++slot) there += stack_of(r, slot) < a.stacks;
         for (int b = 0; b < a.blocks; ++b) {
           if (!(ok = bar_wait(empty + 8 * s, ph ^ 1))) break;
           const uint32_t to = base + s * stage;
-          int there = 0;
-          for (int slot = 0; slot < SLOTS; ++slot) there += tile_of(r, slot) < a.tiles;
-          bar_expect(full + 8 * s, there * TILE_BYTES + x_bytes);
+          bar_expect(full + 8 * s, there * WIDE_BYTES + x_bytes);
           for (int slot = 0; slot < there; ++slot)
-            tma_load<1>(to + slot * TILE_BYTES, &weights, full + 8 * s, b * BLOCK_BYTES, tile_of(r, slot) * TILE);
-          bulk_load(to + SLOTS * TILE_BYTES, (const char*)a.operand + (long long)b * x_bytes, full + 8 * s, x_bytes);
+            tma_load<1>(to + slot * WIDE_BYTES, &weights, full + 8 * s, b * TILE_WORDS,
+                        stack_of(r, slot) * (WIDE / ROWS));
+          bulk_load(to + SLOTS * WIDE_BYTES, (const char*)a.operand + (long long)b * x_bytes, full + 8 * s, x_bytes);
           if (++s == a.stages) {
             s = 0;
             ph ^= 1;
@@ -722,20 +758,20 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
     }
   } else {  // issues the products
     if (elect_one()) {
-      const uint32_t desc = mma_desc(!F16, false, false, TILE, a.columns);
+      constexpr uint32_t desc = mma_desc(!F16, false, false, WIDE, COLUMNS);
       int s = 0, ph = 0, abuf = 0, a_ph = 0, dbuf[SLOTS] = {}, d_ph[SLOTS] = {};
       bool ok = true;
       for (int r = 0; r < rounds && ok; ++r) {
         int there = 0;
-        for (int slot = 0; slot < SLOTS; ++slot) there += tile_of(r, slot) < a.tiles;
+        for (int slot = 0; slot < SLOTS; ++slot) there += stack_of(r, slot) < a.stacks;
         for (int b = 0; b < a.blocks && ok; ++b) {
           if (!(ok = bar_wait(full + 8 * s, ph))) break;
-          const uint32_t x = base + s * stage + SLOTS * TILE_BYTES;
+          const uint32_t x = base + s * stage + SLOTS * WIDE_BYTES;
           for (int h = 0; h < 2 && ok; ++h) {
 #pragma unroll
             for (int slot = 0; slot < SLOTS; ++slot) {
               if (slot >= there || !ok) continue;
-              if (!(ok = bar_wait(a_full + 8 * (2 * slot + abuf), a_ph))) break;
+              if (!(ok = bar_wait(a_full + 8 * (A_BUFS * slot + abuf), a_ph))) break;
               fence_after();
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
@@ -754,10 +790,12 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
                   if (dbuf[slot] == 0) d_ph[slot] ^= 1;
                 }
               }
-              if (ok) mma_commit<1>(a_empty + 8 * (2 * slot + abuf));
+              if (ok) mma_commit<1>(a_empty + 8 * (A_BUFS * slot + abuf));
             }
-            abuf ^= 1;
-            if (abuf == 0) a_ph ^= 1;
+            if (++abuf == A_BUFS) {
+              abuf = 0;
+              a_ph ^= 1;
+            }
           }
           if (ok) mma_commit<1>(empty + 8 * s);
           if (++s == a.stages) {

@@ -13,7 +13,7 @@ static inline CUtensorMapDataType pesti_map_type(pesti_dtype dtype) {
 }
 
 // `rows` rows of `columns` elements, row_bytes apart (a multiple of 16); boxes of box_columns x box_rows, whose rows are
-// 128 bytes (or 64, swizzled as such).  Elements outside the matrix are read as 0 and not written.
+// 128 bytes where they are swizzled.  Elements outside the matrix are read as 0 and not written.
 static inline int pesti_tensor_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, long long columns,
                                    long long rows, long long row_bytes, int box_columns, int box_rows,
                                    CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {

@@ -139,23 +139,19 @@ def linear_cross_entropy_grad(hidden, head, target, weight=None, label_smoothing
     return loss, gh, gw
 
 
-_BLOCK = 128  # columns of a block of the held layout
+_BLOCK, _ROWS = 128, 16  # of a tile of the held layout
 
 
 class QuantizedHead:
     """A [V, D] weight in 4 bits with a scale for every `group` columns of a row
     (quantize_head), about (4.5, 4.25 or 4.125) / 16 of its bfloat16 size.
 
-    packed [V, ceil(D / 128) * 64] uint8 and padded_scale bfloat16 are the
-    library's layout (pesti_q4_quantize); scale [V, ceil(D / group)] is a view of
-    the scales that count."""
+    packed [ceil(V / 16), ceil(D / 128), 16, 64] uint8 and tile_scale
+    [ceil(V / 16), ceil(D / 128), 16, 128 / group] bfloat16 are the library's
+    layout (pesti_q4_quantize); scale is tile_scale by rows, [V, ceil(D / group)]."""
 
-    def __init__(self, packed, padded_scale, D: int, group: int):
-        self.packed, self.padded_scale, self.D, self.group = packed, padded_scale, int(D), int(group)
-
-    @property
-    def V(self) -> int:
-        return self.packed.shape[0]
+    def __init__(self, packed, tile_scale, V: int, D: int, group: int):
+        self.packed, self.tile_scale, self.V, self.D, self.group = packed, tile_scale, int(V), int(D), int(group)
 
     @property
     def device(self):
@@ -163,7 +159,8 @@ class QuantizedHead:
 
     @property
     def scale(self):
-        return self.padded_scale[:, :-(-self.D // self.group)]
+        by_rows = self.tile_scale.transpose(1, 2).reshape(self.tile_scale.shape[0] * _ROWS, -1)
+        return by_rows[:self.V, :-(-self.D // self.group)]
 
     def dequantize(self, dtype=torch.bfloat16, out=None, stream=None):
         """The [V, D] weight that is held (or `out` filled with it): float32 holds it exactly."""
@@ -179,7 +176,7 @@ class QuantizedHead:
         def call(st):
             to = out if out is not None else torch.empty((self.V, self.D), dtype=dtype, device=dev)
             _check(load_library().pesti_q4_dequantize(
-                self.packed.data_ptr(), self.padded_scale.data_ptr(), self.V, self.D, self.group, to.data_ptr(),
+                self.packed.data_ptr(), self.tile_scale.data_ptr(), self.V, self.D, self.group, to.data_ptr(),
                 _DTYPES[to.dtype], _row_stride(to), st))
             if out is not None:
                 _written((out,))
@@ -201,12 +198,12 @@ def quantize_head(head, group: int = 64, stream=None) -> QuantizedHead:
     head = head.detach()
 
     def call(st):
-        blocks = -(-D // _BLOCK)
-        packed = torch.empty((V, blocks * (_BLOCK // 2)), dtype=torch.uint8, device=head.device)
-        scale = torch.empty((V, -(-blocks * (_BLOCK // group) // 8) * 8), dtype=torch.bfloat16, device=head.device)
+        tiles = -(-V // _ROWS), -(-D // _BLOCK), _ROWS
+        packed = torch.empty((*tiles, _BLOCK // 2), dtype=torch.uint8, device=head.device)
+        scale = torch.empty((*tiles, _BLOCK // group), dtype=torch.bfloat16, device=head.device)
         _check(load_library().pesti_q4_quantize(head.data_ptr(), _DTYPES[head.dtype], V, D, _row_stride(head), group,
                                                 packed.data_ptr(), scale.data_ptr(), st))
-        return QuantizedHead(packed, scale, D, group)
+        return QuantizedHead(packed, scale, V, D, group)
 
     return _launch(head.device, stream, call)
 
@@ -247,7 +244,7 @@ def head_logits(x, held: QuantizedHead, dtype=None, out=None, stream=None):
             need = _logits_workspace(code, B, D)
             ws = x.new_empty(need, dtype=torch.uint8)
             _check(load_library().pesti_q4_logits(
-                x.data_ptr(), code, B, D, _row_stride(x), held.packed.data_ptr(), held.padded_scale.data_ptr(),
+                x.data_ptr(), code, B, D, _row_stride(x), held.packed.data_ptr(), held.tile_scale.data_ptr(),
                 held.V, held.group, to.data_ptr(), _DTYPES[to.dtype], _row_stride(to), ws.data_ptr(), need, st))
             if out is not None:
                 _written((out,))

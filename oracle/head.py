@@ -58,10 +58,14 @@ def held_values(q, scale, group):
     return q.double() * scale.double().repeat_interleave(group, 1)[:, :q.shape[1]]
 
 
-def unpack(packed, D):
-    """q [V, D] from the library's layout: word 4t + j of a block of 128 columns
-    holds columns 32j + 8t to 32j + 8t + 7, the first lowest."""
-    V = packed.shape[0]
-    b = packed.cpu().view(V, -1, 4, 4, 4).long()             # block, t, j, byte
-    nib = torch.stack([b & 15, b >> 4], -1).reshape(V, b.shape[1], 4, 4, 8)
-    return (nib.permute(0, 1, 3, 2, 4).reshape(V, -1)[:, :D] - 8).to(packed.device)
+def unpack(packed, V, D):
+    """q [V, D] from the library's layout, tiles of 16 rows and 128 columns: word j
+    of chunk t ^ (row // 2 % 4) of a row holds the tile's columns 32j + 8t to
+    32j + 8t + 7, the first lowest."""
+    T, B = packed.shape[:2]
+    b = packed.cpu().view(T, B, 16, 4, 4, 4).long()          # tile, block, row, chunk, j, byte
+    nib = torch.stack([b & 15, b >> 4], -1).reshape(T, B, 16, 4, 4, 8)
+    row, t = torch.arange(16)[:, None], torch.arange(4)[None, :]
+    nib = nib[:, :, row, t ^ (row // 2 % 4)]                  # tile, block, row, t, j, column
+    q = nib.permute(0, 2, 1, 4, 3, 5).reshape(T * 16, B * 128)
+    return (q[:V, :D] - 8).to(packed.device)

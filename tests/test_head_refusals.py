@@ -125,7 +125,7 @@ def test_python_refusals():
                       ((w, 48), "group"), ((w,), "CUDA device")]:
         with pytest.raises(ValueError, match=msg):
             ph.quantize_head(*args)
-    held = ph.QuantizedHead(torch.zeros(10, 64, dtype=torch.uint8), torch.zeros(10, 2).bfloat16(), 64, 64)
+    held = ph.QuantizedHead(torch.zeros(1, 1, 16, 64, dtype=torch.uint8), torch.zeros(1, 1, 16, 2).bfloat16(), 10, 64, 64)
     assert held.V == 10 and held.scale.shape == (10, 1)
     for args, msg in [((h[0], held), "x must"), ((h.int(), held), "x must"), ((h[:, :32], held), "different D"),
                       ((h.t().contiguous().t(), held), "contiguous"), ((h, held, torch.int32), "dtype must"),

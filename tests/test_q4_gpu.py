@@ -32,7 +32,7 @@ def _check_held(head, group):
     V, D = head.shape
     q, scale = OH.quantize(head, group)
     assert torch.equal(held.scale, scale) and held.scale.shape == (V, -(-D // group))
-    assert torch.equal(OH.unpack(held.packed, D).double(), q)
+    assert torch.equal(OH.unpack(held.packed, V, D).double(), q)
     want = OH.held_values(q, scale, group)
     for dtype in (torch.float32, torch.bfloat16, torch.float16):
         assert torch.equal(held.dequantize(dtype), want.float().to(dtype))
@@ -76,7 +76,7 @@ def test_tiny_scales():
     q, scale = OH.quantize(w, 32)
     # m / -8 of a subnormal f32 is rounded once more, to f32's steps of 2^-149, far below bfloat16's of 2^-133
     assert torch.equal(held.scale, scale)
-    assert torch.equal(OH.unpack(held.packed, 64).double(), q)
+    assert torch.equal(OH.unpack(held.packed, 16, 64).double(), q)
 
 
 def test_groups_that_are_not_finite():
@@ -98,7 +98,7 @@ def test_strided_weights(dtype):
     room = torch.full((50, 311), float("nan"), dtype=head.dtype, device="cuda")[:, 5:305]
     room.copy_(head)
     got = ph.quantize_head(room, 32)
-    assert torch.equal(got.packed, want.packed) and torch.equal(got.padded_scale, want.padded_scale)
+    assert torch.equal(got.packed, want.packed) and torch.equal(got.tile_scale, want.tile_scale)
     out = torch.full((50, 311), 7.0, dtype=head.dtype, device="cuda")
     version = out._version
     got.dequantize(out=out[:, 5:305])
@@ -220,7 +220,7 @@ def test_offsets_beyond_32_bits():
     held = ph.quantize_head(w, 128)
     del w
     want = ph.quantize_head(part, 128)
-    assert torch.equal(held.packed.view(700, 1000, -1), want.packed.expand(700, 1000, -1))
+    assert torch.equal(held.scale.view(700, 1000, -1), want.scale.expand(700, 1000, -1))
     x = torch.randn(1, D, device="cuda").bfloat16()
     # K may be shared out otherwise for another V: two sums of the same products, each off by the bound above
     back = want.dequantize(torch.float32).double()
