@@ -435,24 +435,30 @@ __global__ void __launch_bounds__(few_warps(sizeof(T) == 4 ? 3 : 1) * 32, 1) q4_
   int load_round = 0, load_b = part;
   Weights<GROUP> held[STACK];
   auto stack_of = [&](int round) { return (round * (int)gridDim.x + (int)blockIdx.x) * slots + slot; };
+  int q_up[STACK], s_up[STACK];
   auto begin = [&]() {
-    const long long tile = (long long)min(stack_of(load_round), a.stacks - 1) * STACK * a.blocks + part;
+    const int stack = min(stack_of(load_round), a.stacks - 1);
+    const long long tile = (long long)stack * STACK * a.blocks + part;
     q = a.q + tile * (TILE_WORDS / 4) + g * 4 + chunk_at(g, t);
     sc = a.scale + (tile * ROWS + g) * (BLOCK / GROUP);
+#pragma unroll
+    for (int i = 0; i < STACK; ++i) {  // a tile past the last row's is the last one again
+      const int up = min(i, (a.V - 1) / ROWS - stack * STACK) * a.blocks;
+      q_up[i] = up * (TILE_WORDS / 4);
+      s_up[i] = up * (ROWS * BLOCK / GROUP);
+    }
   };
-  auto load = [&](int i) {
-    // a tile past the last row's is the last one again
-    const int up = min(i, (a.V - 1) / ROWS - min(stack_of(load_round), a.stacks - 1) * STACK) * a.blocks;
-    held[i].load(q + up * (TILE_WORDS / 4), sc + up * (ROWS * BLOCK / GROUP));
-  };
+  auto load = [&](int i) { held[i].load(q + q_up[i], sc + s_up[i]); };
   auto advance = [&]() {
     load_b += kw;
-    q += kw * (TILE_WORDS / 4);
-    sc += kw * (ROWS * BLOCK / GROUP);
-    if (load_b >= a.blocks) {
+    if (load_b < a.blocks) {
+      q += kw * (TILE_WORDS / 4);
+      sc += kw * (ROWS * BLOCK / GROUP);
+    } else if (load_round + 1 < rounds) {
       load_b = part;
-      if (++load_round < rounds) begin();
-    }
+      ++load_round;
+      begin();
+    }  // behind the last block of all it stays where it is, and loads that once more
   };
   begin();
 #pragma unroll
@@ -511,7 +517,7 @@ __global__ void __launch_bounds__(few_warps(sizeof(T) == 4 ? 3 : 1) * 32, 1) q4_
           acc[i][2] = fmaf(s1, sum[2], acc[i][2]);
           acc[i][3] = fmaf(s1, sum[3], acc[i][3]);
         }
-        if (load_round < rounds) load(i);
+        load(i);
       }
       advance();
     }
@@ -564,15 +570,16 @@ __global__ void __launch_bounds__(256) q4_operand_kernel(const LogitArgs a, int 
 
 constexpr int WIDE = 128;                       // rows of the weight, eight tiles
 constexpr int SLOTS = 2;                        // of them at once
-constexpr int WIDE_THREADS = (8 * SLOTS + 2) * 32;
+constexpr int WIDE_THREADS = (9 * SLOTS + 1) * 32;
 constexpr int WIDE_BYTES = WIDE * BLOCK_BYTES;  // of a block
-constexpr int A_BUFS = 4;                       // of 64 of K, unpacked
 
-// Where a slot's buffers are in tensor memory: unpacked weights, and two of sums.
-__device__ __forceinline__ uint32_t a_column(int slot, int buf) { return slot * 256 + buf * 32; }
+// Where a slot's buffers are in tensor memory: two blocks of unpacked weights, and two groups' sums.
+__device__ __forceinline__ uint32_t a_column(int slot, int buf) { return slot * 256 + buf * 64; }
 __device__ __forceinline__ uint32_t d_column(int slot, int buf) { return slot * 256 + 128 + buf * 64; }
 
-// Warps 0 to 7 unpack (four a slot, a quarter of the rows each), 8 to 15 add up, 16 copies, 17 issues the products.
+// Warps 0 to 7 unpack (four a slot, a quarter of the rows each), 8 to 15 add up, 16 copies, 17 and 18 issue a slot's
+// products.  Issuing is what the rest waits for (a commit takes as long as ten products of 64 rows), so that a block's
+// buffers are handed back by the warps that see its last sums, and only sums are committed.
 template <typename T, int GROUP, int COLUMNS>
 __global__ void __launch_bounds__(WIDE_THREADS, 1)
     q4_wide_kernel(const __grid_constant__ CUtensorMap weights, const LogitArgs a) {
@@ -582,21 +589,19 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
   constexpr uint32_t x_half = COLUMNS * 128, x_bytes = 2 * P * x_half, stage = SLOTS * WIDE_BYTES + x_bytes;
   extern __shared__ char raw[];
   const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
-  __shared__ uint64_t bars[16 + SLOTS * (2 * A_BUFS + 4)];
+  __shared__ uint64_t bars[16 + 8 * SLOTS];
   __shared__ uint32_t tmem_base;
-  const uint32_t full = smem_addr(bars), empty = full + 64, a_full = empty + 64, a_empty = a_full + 8 * A_BUFS * SLOTS,
-                 d_full = a_empty + 8 * A_BUFS * SLOTS, d_empty = d_full + 16 * SLOTS;
+  const uint32_t full = smem_addr(bars), empty = full + 64, a_full = empty + 64, a_empty = a_full + 16 * SLOTS,
+                 d_full = a_empty + 16 * SLOTS, d_empty = d_full + 16 * SLOTS;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < a.stages; ++s) {
       bar_init(full + 8 * s, 1);
-      bar_init(empty + 8 * s, 4 * SLOTS + 1);
-    }
-    for (int s = 0; s < A_BUFS * SLOTS; ++s) {
-      bar_init(a_full + 8 * s, 4);
-      bar_init(a_empty + 8 * s, 1);
+      bar_init(empty + 8 * s, 8 * SLOTS);  // read by the warps that unpack, and its products done
     }
     for (int s = 0; s < 2 * SLOTS; ++s) {
+      bar_init(a_full + 8 * s, 4);
+      bar_init(a_empty + 8 * s, 4);
       bar_init(d_full + 8 * s, 1);
       bar_init(d_empty + 8 * s, 4);
     }
@@ -645,18 +650,18 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[4 * c + i] = unpack<F16>(word, i);
           }
-          if (!(ok = bar_wait(a_empty + 8 * (A_BUFS * slot + buf), buf_ph ^ 1))) break;
-          fence_after();
-          tmem_store32(tmem + a_column(slot, buf) + quarter, v);
-          tmem_store_wait();
-          fence_before();
-          __syncwarp();
-          if (lane == 0) bar_arrive(a_full + 8 * (A_BUFS * slot + buf));
-          if (++buf == A_BUFS) {
-            buf = 0;
-            buf_ph ^= 1;
+          if (h == 0) {
+            if (!(ok = bar_wait(a_empty + 8 * (2 * slot + buf), buf_ph ^ 1))) break;
+            fence_after();
           }
+          tmem_store32(tmem + a_column(slot, buf) + 32 * h + quarter, v);
         }
+        tmem_store_wait();
+        fence_before();
+        __syncwarp();
+        if (lane == 0 && ok) bar_arrive(a_full + 8 * (2 * slot + buf));
+        buf ^= 1;
+        if (buf == 0) buf_ph ^= 1;
       }
     }
   } else if (warp < 8 * SLOTS) {  // adds up
@@ -664,11 +669,22 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
     constexpr int CHUNK = COLUMNS == 32 ? 32 : 16;  // (more columns leave no registers for more at once)
     const int slot = (warp - 4 * SLOTS) >> 2;
     const uint32_t quarter = (uint32_t)(warp & 3) << 21;
-    int buf = 0, buf_ph = 0;
+    int buf = 0, buf_ph = 0, s = 0, ph = 0, a_buf = 0;
     bool ok = true;
     for (int r = 0; r < rounds && ok; ++r) {
       const int stack = stack_of(r, slot);
-      if (stack >= a.stacks) break;
+      if (stack >= a.stacks) {  // nothing of these stages is this slot's
+        for (int b = 0; b < a.blocks && ok; ++b) {
+          ok = bar_wait(full + 8 * s, ph);
+          __syncwarp();
+          if (lane == 0) bar_arrive(empty + 8 * s);
+          if (++s == a.stages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+        continue;
+      }
       const int v = stack * WIDE + (warp & 3) * 32 + lane;
       const long long tile = tile_of(min(v, a.V - 1), a.blocks, 0);
       const __nv_bfloat16* scales = a.scale + (tile * ROWS + (v & 15)) * PER;
@@ -699,6 +715,17 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
           const float scale = bitsf(g & 1 ? two & 0xffff0000u : two << 16);
           if (!(ok = bar_wait(d_full + 8 * (2 * slot + buf), buf_ph))) break;
           fence_after();
+          if (g == PER - 1) {  // the block's products are done
+            if (lane == 0) {
+              bar_arrive(a_empty + 8 * (2 * slot + a_buf));
+              bar_arrive(empty + 8 * s);
+            }
+            a_buf ^= 1;
+            if (++s == a.stages) {
+              s = 0;
+              ph ^= 1;
+            }
+          }
           const uint32_t from = tmem + d_column(slot, buf) + quarter;
 #pragma unroll
           for (int c = 0; c < COLUMNS; c += CHUNK) {
@@ -756,52 +783,42 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
       if (!ok)
         for (int i = 0; i < a.stages; ++i) bar_wait(full + 8 * i, ph);  // copies in flight
     }
-  } else {  // issues the products
-    if (elect_one()) {
-      constexpr uint32_t desc = mma_desc(!F16, false, false, WIDE, COLUMNS);
-      int s = 0, ph = 0, abuf = 0, a_ph = 0, dbuf[SLOTS] = {}, d_ph[SLOTS] = {};
-      bool ok = true;
-      for (int r = 0; r < rounds && ok; ++r) {
-        int there = 0;
-        for (int slot = 0; slot < SLOTS; ++slot) there += stack_of(r, slot) < a.stacks;
-        for (int b = 0; b < a.blocks && ok; ++b) {
-          if (!(ok = bar_wait(full + 8 * s, ph))) break;
-          const uint32_t x = base + s * stage + SLOTS * WIDE_BYTES;
-          for (int h = 0; h < 2 && ok; ++h) {
+  } else {  // issues a slot's products; the warp runs through as one, so that addresses are uniform
+    constexpr uint32_t desc = mma_desc(!F16, false, false, WIDE, COLUMNS);
+    const int slot = __shfl_sync(PESTI_FULL_MASK, warp, 0) - (8 * SLOTS + 1);
+    int s = 0, ph = 0, abuf = 0, a_ph = 0, dbuf = 0, d_ph = 0;
+    bool ok = true;
+    for (int r = 0; r < rounds && ok; ++r) {
+      if (stack_of(r, slot) >= a.stacks) break;
+      for (int b = 0; b < a.blocks && ok; ++b) {
+        ok = __all_sync(PESTI_FULL_MASK, bar_wait(full + 8 * s, ph));
+        if (ok) ok = __all_sync(PESTI_FULL_MASK, bar_wait(a_full + 8 * (2 * slot + abuf), a_ph));
+        if (!ok) break;
+        const uint32_t x = base + s * stage + SLOTS * WIDE_BYTES;
 #pragma unroll
-            for (int slot = 0; slot < SLOTS; ++slot) {
-              if (slot >= there || !ok) continue;
-              if (!(ok = bar_wait(a_full + 8 * (A_BUFS * slot + abuf), a_ph))) break;
-              fence_after();
+        for (int at = 0; at < BLOCK; at += GROUP) {
+          ok = __all_sync(PESTI_FULL_MASK, bar_wait(d_empty + 8 * (2 * slot + dbuf), d_ph ^ 1));
+          if (!ok) break;
+          fence_after();
+          if (elect_one()) {
+            const uint32_t d = tmem + d_column(slot, dbuf), from = tmem + a_column(slot, abuf);
+            const uint64_t xd = operand_desc(x, 0);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const int at = 64 * h + 16 * k;  // in the block
-                if (at % GROUP == 0) {
-                  if (!(ok = bar_wait(d_empty + 8 * (2 * slot + dbuf[slot]), d_ph[slot] ^ 1))) break;
-                  fence_after();
-                }
+            for (int k = at; k < at + GROUP; k += 16)
 #pragma unroll
-                for (int p = 0; p < P; ++p)
-                  mma_f16_tmem(tmem + d_column(slot, dbuf[slot]), tmem + a_column(slot, abuf) + 8 * k,
-                               operand_desc(x + (h * P + p) * x_half, 0) + 2 * k, desc, at % GROUP != 0 || p > 0);
-                if ((at + 16) % GROUP == 0) {
-                  mma_commit<1>(d_full + 8 * (2 * slot + dbuf[slot]));
-                  dbuf[slot] ^= 1;
-                  if (dbuf[slot] == 0) d_ph[slot] ^= 1;
-                }
-              }
-              if (ok) mma_commit<1>(a_empty + 8 * (A_BUFS * slot + abuf));
-            }
-            if (++abuf == A_BUFS) {
-              abuf = 0;
-              a_ph ^= 1;
-            }
+              for (int p = 0; p < P; ++p)
+                mma_f16_tmem(d, from + k / 2, xd + ((k / 64 * P + p) * x_half >> 4) + k % 64 / 8, desc, k > at || p > 0);
+            mma_commit<1>(d_full + 8 * (2 * slot + dbuf));
           }
-          if (ok) mma_commit<1>(empty + 8 * s);
-          if (++s == a.stages) {
-            s = 0;
-            ph ^= 1;
-          }
+          __syncwarp();
+          dbuf ^= 1;
+          if (dbuf == 0) d_ph ^= 1;
+        }
+        abuf ^= 1;
+        if (abuf == 0) a_ph ^= 1;
+        if (++s == a.stages) {
+          s = 0;
+          ph ^= 1;
         }
       }
     }

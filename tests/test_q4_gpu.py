@@ -135,6 +135,15 @@ def test_logits(dtype, group, B, V, D):
     assert torch.equal(ph.head_logits(x, held, dtype=torch.float16), a.to(torch.float16))
 
 
+@pytest.mark.parametrize("B", [3, 20])
+@pytest.mark.parametrize("V", [18_900, 19_000, 37_900, 40_000, 76_001])
+def test_rounds(B, V):
+    """More rows of the weight than all SMs hold at once, and last rounds that fill some of them."""
+    held, want = _check_held(_weight(V, 256, "bf16"), 64)
+    x = torch.randn(B, 256, generator=torch.Generator().manual_seed(V)).bfloat16().cuda()
+    _check_logits(x, held, want, torch.float32)
+
+
 @pytest.mark.parametrize("B", [1, 5, 64])
 def test_wide_values_of_x(B):
     """f32 rows of all magnitudes, f16 subnormals, bf16 extremes, infinities and NaN."""
