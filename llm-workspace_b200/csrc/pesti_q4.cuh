@@ -618,7 +618,9 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
   const int per_round = gridDim.x * SLOTS, rounds = (a.stacks + per_round - 1) / per_round;
   auto stack_of = [&](int round, int slot) { return round * per_round + slot * (int)gridDim.x + (int)blockIdx.x; };
 
+  // 96 registers a thread at the start; eight warps' 24 go to eight others
   if (warp < 4 * SLOTS) {  // unpacks
+    give_registers<72>();
     const int slot = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t quarter = (uint32_t)(warp & 3) << 21;
     int s = 0, ph = 0, buf = 0, buf_ph = 0;
@@ -665,8 +667,9 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
       }
     }
   } else if (warp < 8 * SLOTS) {  // adds up
-    constexpr int PER = BLOCK / GROUP;  // groups of a block
-    constexpr int CHUNK = COLUMNS == 32 ? 32 : 16;  // (more columns leave no registers for more at once)
+    take_registers<120>();
+    constexpr int PER = BLOCK / GROUP;             // groups of a block
+    constexpr int CHUNK = COLUMNS == 64 ? 32 : COLUMNS;  // columns in registers at once, beside their sums
     const int slot = (warp - 4 * SLOTS) >> 2;
     const uint32_t quarter = (uint32_t)(warp & 3) << 21;
     int buf = 0, buf_ph = 0, s = 0, ph = 0, a_buf = 0;
@@ -729,18 +732,18 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
           const uint32_t from = tmem + d_column(slot, buf) + quarter;
 #pragma unroll
           for (int c = 0; c < COLUMNS; c += CHUNK) {
-            uint32_t sum[CHUNK];
-            if constexpr (CHUNK == 32)
-              tmem_load32(from + c, sum);
-            else
-              tmem_load16(from + c, sum);
-            tmem_load_wait();
+            uint32_t sum[CHUNK / 16][16];
 #pragma unroll
-            for (int i = 0; i < CHUNK; ++i) acc[c + i] = fmaf(scale, bitsf(sum[i]), acc[c + i]);
+            for (int i = 0; i < CHUNK / 16; ++i) tmem_load16(from + c + 16 * i, sum[i]);
+            tmem_load_wait();
+            if (c + CHUNK == COLUMNS) {
+              fence_before();
+              __syncwarp();
+              if (lane == 0) bar_arrive(d_empty + 8 * (2 * slot + buf));
+            }
+#pragma unroll
+            for (int i = 0; i < CHUNK; ++i) acc[c + i] = fmaf(scale, bitsf(sum[i / 16][i % 16]), acc[c + i]);
           }
-          fence_before();
-          __syncwarp();
-          if (lane == 0) bar_arrive(d_empty + 8 * (2 * slot + buf));
           buf ^= 1;
           if (buf == 0) buf_ph ^= 1;
         }
