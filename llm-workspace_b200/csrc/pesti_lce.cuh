@@ -20,16 +20,21 @@ using namespace pesti_umma;
 
 constexpr int BN = 256;              // columns of a tile
 constexpr int BK = 64;               // of K per stage: one 128-byte swizzled row
-constexpr int EPI_WARPS = 4;         // a quarter of the accumulators' 128 rows each
+constexpr int EPI_WARPS = 8;         // a quarter of the accumulators' 128 rows and half of their columns each
+constexpr int HALF = BN / 2;
 constexpr int THREADS = (EPI_WARPS + 2) * 32;
 constexpr int A_BYTES = 128 * BK * 2;
 constexpr int OUT_BYTES = 32 * 128;  // a warp's 32 rows of 128 bytes on their way out
+// Stages that logits are summed over in the tensor cores at once; the sums of several are added in registers.  The
+// cores' own sums are cut off and not rounded, every 16 of K, and always towards 0: over 4096 of K that shrank the
+// largest logits by 5e-6 of themselves, four times as much as in parts of 1024.
+constexpr int PART_K = 16;
 constexpr float LOG2E = 1.44269504f;
 
 __host__ __device__ constexpr int b_bytes(int cg) { return BN / cg * BK * 2; }
 __host__ __device__ constexpr int stages(int cg) { return cg == 1 ? 4 : 6; }
 __host__ __device__ constexpr int smem_bytes(int cg) {
-  return 1024 + stages(cg) * (A_BYTES + b_bytes(cg)) + EPI_WARPS * 2 * OUT_BYTES + 256;
+  return 1024 + stages(cg) * (A_BYTES + b_bytes(cg)) + EPI_WARPS * OUT_BYTES + 256;
 }
 
 // What the host does not know: written by the plan kernel, on the device.
@@ -96,8 +101,8 @@ __device__ __forceinline__ int grad_shift(const Plan* plan) {
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
 
-// One block (CG 1) or a pair of them (CG 2) takes tiles of 128 CG x 256, one after another.  Warp 4 copies the stages
-// in, one thread of warp 5 issues the products, warps 0 to 3 empty one set of accumulators while the other is filled.
+// One block (CG 1) or a pair of them (CG 2) takes tiles of 128 CG x 256, one after another.  Warp 8 copies the stages
+// in, one thread of warp 9 issues the products, warps 0 to 7 empty one set of accumulators while the other is filled.
 template <int CG, bool BF16, bool A_MN, bool B_MN, Epilogue E>
 __global__ void __launch_bounds__(THREADS, 1)
     head_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
@@ -106,8 +111,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   extern __shared__ char raw[];
   const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
   const uint32_t out0 = base + ST * STAGE;
-  const uint32_t bars = out0 + EPI_WARPS * 2 * OUT_BYTES;
-  const uint32_t full = bars, empty = bars + 8 * ST, acc_full = empty + 8 * ST, acc_empty = acc_full + 16;
+  const uint32_t bars = out0 + EPI_WARPS * OUT_BYTES;
+  const uint32_t full = bars, empty = bars + 8 * ST, acc_full = empty + 8 * ST, acc_empty = acc_full + 16,
+                 given = acc_empty + 16, taken = given + 32;
   __shared__ uint32_t tmem_base;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 1 ? 0 : cluster_rank();
@@ -121,9 +127,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       bar_init(acc_full + 8 * s, 1);
       bar_init(acc_empty + 8 * s, CG * EPI_WARPS);
     }
+    for (int s = 0; s < 8; ++s) bar_init(given + 8 * s, 1);  // given and taken, of each quarter
     bar_init_fence();
   }
-  if (warp == 5) tmem_alloc<CG>(smem_addr(&tmem_base), 512);
+  if (warp == EPI_WARPS + 1) tmem_alloc<CG>(smem_addr(&tmem_base), 512);
   fence_before();
   if constexpr (CG == 2) cluster_sync();
   __syncthreads();
@@ -153,7 +160,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     kn = max(0, min(k_split, k_iters - k0));
   };
 
-  if (warp == 4) {
+  auto parts_of = [&](int kn) { return E == STATS ? (kn + PART_K - 1) / PART_K : 1; };
+
+  if (warp == EPI_WARPS) {
     if (elect_one()) {
       tma_prefetch(&map_a);
       tma_prefetch(&map_b);
@@ -205,7 +214,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int i = 0; i < ST && rank == 0; ++i) bar_wait(full + 8 * i, ph);  // copies in flight
       }
     }
-  } else if (warp == 5) {
+  } else if (warp == EPI_WARPS + 1) {
     if (rank == 0 && elect_one()) {
       constexpr uint32_t desc = mma_desc(BF16, A_MN, B_MN, TM, BN);
       int s = 0, ph = 0, acc = 0, acc_ph = 0;
@@ -213,32 +222,36 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int tile = first; tile < tiles && ok; tile += step) {
         int m, n, split, k0, kn;
         locate(tile, m, n, split, k0, kn);
-        if (!bar_wait(acc_empty + 8 * acc, acc_ph ^ 1)) {
-          ok = false;
-          break;
-        }
-        fence_after();
-        const uint32_t d = tmem + acc * BN;
-        for (int k = 0; k < kn; ++k) {
-          if (!bar_wait(full + 8 * s, ph)) {
+        const int parts = parts_of(kn);
+        for (int part = 0; part < parts && ok; ++part) {
+          if (!bar_wait(acc_empty + 8 * acc, acc_ph ^ 1)) {
             ok = false;
             break;
           }
           fence_after();
-          const uint32_t a = base + s * STAGE, b = a + A_BYTES;
-          const uint64_t da = operand_desc(a, 8192), db = operand_desc(b, 8192);
+          const uint32_t d = tmem + acc * BN;
+          const int k_end = kn * (part + 1) / parts, k_begin = kn * part / parts;
+          for (int k = k_begin; k < k_end; ++k) {
+            if (!bar_wait(full + 8 * s, ph)) {
+              ok = false;
+              break;
+            }
+            fence_after();
+            const uint32_t a = base + s * STAGE, b = a + A_BYTES;
+            const uint64_t da = operand_desc(a, 8192), db = operand_desc(b, 8192);
 #pragma unroll
-          for (int j = 0; j < BK / 16; ++j)  // 16 of K: 32 bytes of a row, or 16 rows of 128 bytes
-            mma_f16<CG>(d, da + j * (A_MN ? 128 : 2), db + j * (B_MN ? 128 : 2), desc, k > 0 || j > 0);
-          mma_commit<CG>(empty + 8 * s);
-          if (++s == ST) {
-            s = 0;
-            ph ^= 1;
+            for (int j = 0; j < BK / 16; ++j)  // 16 of K: 32 bytes of a row, or 16 rows of 128 bytes
+              mma_f16<CG>(d, da + j * (A_MN ? 128 : 2), db + j * (B_MN ? 128 : 2), desc, k > k_begin || j > 0);
+            mma_commit<CG>(empty + 8 * s);
+            if (++s == ST) {
+              s = 0;
+              ph ^= 1;
+            }
           }
+          if (ok) mma_commit<CG>(acc_full + 8 * acc);
+          acc ^= 1;
+          if (acc == 0) acc_ph ^= 1;
         }
-        if (ok) mma_commit<CG>(acc_full + 8 * acc);
-        acc ^= 1;
-        if (acc == 0) acc_ph ^= 1;
       }
       if (!ok) {
         atomicExch(&g.plan->failed, 1);
@@ -247,31 +260,39 @@ __global__ void __launch_bounds__(THREADS, 1)
   } else {
     const int shift = (E == GRAD || E == OUT16) ? grad_shift<BF16>(g.plan) : 0;
     const float scale = pow2(E == OUT16 ? -shift : shift);
-    const uint32_t out = out0 + warp * 2 * OUT_BYTES;
+    const int quarter = warp & 3, half0 = (warp >> 2) * HALF;
+    const uint32_t out = out0 + warp * OUT_BYTES;
     const uint32_t row_out = out + lane * 128, swz = (lane & 7) << 4;
     const uint32_t acc_empty_to = CG == 1 ? acc_empty : peer_addr(acc_empty, 0);
-    int acc = 0, acc_ph = 0, buf = 0;
-    for (int tile = first; tile < tiles; tile += step) {
+    int acc = 0, acc_ph = 0, pair_ph = 0;
+    bool ok = true;
+    for (int tile = first; tile < tiles && ok; tile += step) {
       int m, n, split, k0, kn;
       locate(tile, m, n, split, k0, kn);
-      if (!bar_wait(acc_full + 8 * acc, acc_ph)) {
-        atomicExch(&g.plan->failed, 1);
-        break;
-      }
-      fence_after();
-      const int warp_row = m * TM + (int)rank * 128 + warp * 32, row = warp_row + lane;
-      const uint32_t from = tmem + acc * BN + ((uint32_t)warp << 21);
-      const int col0 = n * BN;
+      const int warp_row = m * TM + (int)rank * 128 + quarter * 32, row = warp_row + lane;
+      const int col0 = n * BN + half0;
+      auto wait_acc = [&]() {
+        ok = bar_wait(acc_full + 8 * acc, acc_ph);
+        if (!ok) atomicExch(&g.plan->failed, 1);
+        fence_after();
+        return tmem + acc * BN + half0 + ((uint32_t)quarter << 21);
+      };
+      auto leave_acc = [&]() {
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive_cluster(acc_empty_to + 8 * acc);
+        acc ^= 1;
+        if (acc == 0) acc_ph ^= 1;
+      };
 
       // 128 bytes of each of the warp's rows: written swizzled, so that eight lanes write to eight banks' groups
       auto begin_out = [&]() {
-        if (lane == 0) store_wait_read<1>();
+        if (lane == 0) store_wait_read<0>();
         __syncwarp();
       };
       auto put16 = [&](int chunk, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_out + buf * OUT_BYTES +
-                                                                      ((uint32_t)(chunk << 4) ^ swz)),
-                     "r"(x), "r"(y), "r"(z), "r"(w)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_out + ((uint32_t)(chunk << 4) ^ swz)), "r"(x),
+                     "r"(y), "r"(z), "r"(w)
                      : "memory");
       };
       auto end_out = [&](int x, int y, bool add) {
@@ -280,59 +301,90 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (lane == 0) {
           if (y < g.out_y) {
             if (add)
-              tma_add(&map_out, out + buf * OUT_BYTES, x, y);
+              tma_add(&map_out, out, x, y);
             else
-              tma_store(&map_out, out + buf * OUT_BYTES, x, y);
+              tma_store(&map_out, out, x, y);
           }
-          store_commit();  // one group for each buffer filled, or the waits would count wrongly
+          store_commit();
         }
-        buf ^= 1;
       };
 
       if constexpr (E == STATS) {
         const bool live = row < active;
         const int t = live ? g.target[row] - (g.v0 + col0) : -1;
+        float z[HALF];
+        const int parts = parts_of(kn);
+#pragma unroll 1
+        for (int part = 0; part < parts && ok; ++part) {
+          const uint32_t from = wait_acc();
+#pragma unroll
+          for (int c = 0; c < HALF; c += 32) {
+            uint32_t v[32];
+            tmem_load32(from + c, v);
+            tmem_load_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) z[c + j] = __uint_as_float(v[j]) + (part ? z[c + j] : 0.0f);
+          }
+          leave_acc();
+        }
         float mx = -INFINITY, sum = 0.0f, zs = 0.0f, zt = 0.0f;
         const int left = g.V - (g.v0 + col0);
-#pragma unroll 1
-        for (int c = 0; c < BN && c < left; c += 32) {
-          uint32_t v[32];
-          tmem_load32(from + c, v);
-          tmem_load_wait();
+#pragma unroll
+        for (int c = 0; c < HALF; c += 32) {
+          if (c >= left) continue;
           if (__any_sync(PESTI_FULL_MASK, t >= c && t < c + 32)) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (t == c + j) zt = __uint_as_float(v[j]);
+              if (t == c + j) zt = z[c + j];
           }
           if (c + 32 > left) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (c + j >= left) v[j] = 0xff800000u;  // -inf
+              if (c + j >= left) z[c + j] = -INFINITY;
           }
           if (g.zsum) {
             float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int j = 0; j < 32; ++j) a[j & 3] += c + j < left ? __uint_as_float(v[j]) : 0.0f;
+            for (int j = 0; j < 32; ++j) a[j & 3] += c + j < left ? z[c + j] : 0.0f;
             zs += (a[0] + a[1]) + (a[2] + a[3]);
           }
           float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int j = 0; j < 32; ++j) most[j & 3] = fmaxf(most[j & 3], __uint_as_float(v[j]));
+          for (int j = 0; j < 32; ++j) most[j & 3] = fmaxf(most[j & 3], z[c + j]);
           const float now = fmaxf(mx, fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * LOG2E);
           const float ref = now == -INFINITY ? 0.0f : now;
           float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int j = 0; j < 32; ++j) a[j & 3] += ex2(fmaf(__uint_as_float(v[j]), LOG2E, -ref));
+          for (int j = 0; j < 32; ++j) a[j & 3] += ex2(fmaf(z[c + j], LOG2E, -ref));
           sum = sum * ex2(mx - ref) + ((a[0] + a[1]) + (a[2] + a[3]));
           mx = now;
         }
-        if (live) {
-          const long long at = (long long)((g.v0 + col0) / BN) * g.rows_pad + row;
-          g.parts[at] = make_float2(mx, sum);
-          if (g.zsum) g.zsum[at] = zs;
-          if (t >= 0 && t < BN) g.zt[row] = zt;
+        if (t >= 0 && t < HALF) g.zt[row] = zt;
+        // the tile's other half: its warp hands its sums over in shared memory
+        float* other = (float*)(raw + (out0 - smem_addr(raw))) + quarter * 128 + lane;
+        if (half0) {
+          ok = ok && bar_wait(taken + 8 * quarter, pair_ph ^ 1);
+          other[0] = mx;
+          other[32] = sum;
+          other[64] = zs;
+          __syncwarp();
+          if (lane == 0) bar_arrive(given + 8 * quarter);
+        } else {
+          ok = ok && bar_wait(given + 8 * quarter, pair_ph);
+          const float m2 = other[0], s2 = other[32], z2 = other[64];
+          __syncwarp();
+          if (lane == 0) bar_arrive(taken + 8 * quarter);
+          const float now = fmaxf(mx, m2), ref = now == -INFINITY ? 0.0f : now;
+          if (live) {
+            const long long at = (long long)((g.v0 + col0) / BN) * g.rows_pad + row;
+            g.parts[at] = make_float2(now, sum * ex2(mx - ref) + s2 * ex2(m2 - ref));
+            if (g.zsum) g.zsum[at] = zs + z2;
+          }
         }
+        pair_ph ^= 1;
+        if (!ok) atomicExch(&g.plan->failed, 1);
       } else if constexpr (E == GRAD) {
+        const uint32_t from = wait_acc();
         const bool live = row < active;
         RowCoef k = {0.0f, 0.0f, 0.0f, 0.0f};
         int t = -1;
@@ -342,7 +394,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         const float c1 = k.c1 * scale, c2 = k.c2 * scale, c3 = k.c3 * scale;
 #pragma unroll 1
-        for (int c = 0; c < BN && col0 + c < g.out_x; c += 64) {
+        for (int c = 0; c < HALF && col0 + c < g.out_x; c += 64) {
           begin_out();
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -375,9 +427,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           end_out(col0 + c, warp_row, false);
         }
+        leave_acc();
       } else if constexpr (E == OUT16) {
+        const uint32_t from = wait_acc();
 #pragma unroll 1
-        for (int c = 0; c < BN && col0 + c < g.out_x; c += 64) {
+        for (int c = 0; c < HALF && col0 + c < g.out_x; c += 64) {
           begin_out();
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -397,10 +451,12 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           end_out(col0 + c, g.v0 + warp_row, false);
         }
+        leave_acc();
       } else {
+        const uint32_t from = wait_acc();
         if (warp_row < active) {
 #pragma unroll 1
-          for (int c = 0; c < BN && col0 + c < g.out_x; c += 32) {
+          for (int c = 0; c < HALF && col0 + c < g.out_x; c += 32) {
             begin_out();
             uint32_t v[32];
             tmem_load32(from + c, v);
@@ -414,12 +470,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             end_out(col0 + c, split * g.plan->part_rows + warp_row, g.add != 0);
           }
         }
+        leave_acc();
       }
-      fence_before();
-      __syncwarp();
-      if (lane == 0) bar_arrive_cluster(acc_empty_to + 8 * acc);
-      acc ^= 1;
-      if (acc == 0) acc_ph ^= 1;
     }
     if (lane == 0) store_wait_all();
   }
@@ -428,7 +480,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   if constexpr (CG == 2) cluster_sync();
   fence_after();
-  if (warp == 5) tmem_free<CG>(tmem, 512);
+  if (warp == EPI_WARPS + 1) tmem_free<CG>(tmem, 512);
 }
 
 struct RowArgs {
