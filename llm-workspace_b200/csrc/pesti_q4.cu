@@ -88,10 +88,10 @@ int convert(bool there, const void* w, int64_t V, int64_t D, int64_t ld, void* q
   a.blocks = (int)blocks_of(D);
   a.V = (int)V;
   a.runs = (a.blocks + per<T>(there) - 1) / per<T>(there);
-  a.total = (there ? (V + ROWS - 1) / ROWS * ROWS : V) * a.runs;
-  const int align = there || sizeof(T) == 4 ? 32 : 16, teams = there ? 32 : 16;  // of a thread block
+  a.total = (V + ROWS - 1) / ROWS * (there ? ROWS : 1) * a.runs;
+  const int align = there || sizeof(T) == 4 ? 32 : 16, runs = there ? 32 : 1;  // of a thread block
   a.vec = (uintptr_t)w % align == 0 && (V == 1 || ld * sizeof(T) % align == 0);
-  const long long grid = (a.total + teams - 1) / teams;
+  const long long grid = (a.total + runs - 1) / runs;
   if (grid > INT_MAX) return refuse("V * D too large");
   if (there)
     q4_quantize_kernel<T, GROUP, per<T>(true)><<<(unsigned)grid, 256, 0, st>>>(a);

@@ -60,19 +60,17 @@ struct Held {
   long long ld;
   uint32_t* q;
   __nv_bfloat16* scale;
-  int D, blocks, runs;  // blocks of a row, and runs of PER blocks that a team takes
+  int D, blocks, runs;  // blocks of a row, and runs of PER blocks that its team takes
   int V;
-  long long total;      // runs in all
+  long long total;      // runs of all rows, or of all tiles
   int vec;              // whole vectors of 8 columns can be read or written
 };
 
-// The row and the first block of a team of LANES lanes.
-template <typename T, int PER, int LANES>
-__device__ __forceinline__ bool place_of(const Held<T>& a, long long& row, int& block) {
-  const long long run = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-  row = a.total >> 32 ? run / a.runs : (uint32_t)run / (uint32_t)a.runs;
-  block = (int)(run - row * a.runs) * PER;
-  return run < a.total;
+// What a team of lanes takes of `total` runs: which of the first index's, and which of `runs` behind it.
+__device__ __forceinline__ bool place_of(long long team, long long total, int runs, long long& first, int& run) {
+  first = total >> 32 ? team / runs : (uint32_t)team / (uint32_t)runs;
+  run = (int)(team - first * runs);
+  return team < total;
 }
 
 // Quotients w / s as codes q + 8, rounded to whole numbers, halves to even, exactly.  t = 384 + w / s to 2^-15 (the
@@ -195,9 +193,11 @@ struct Sixteen {
 template <typename T, int GROUP, int PER>
 __global__ void __launch_bounds__(256) q4_quantize_kernel(const Held<T> a) {
   const int i = threadIdx.x & 7, lane = threadIdx.x & 31;
+  // teams along a row, which reads best
   long long row;
   int b0;
-  const bool there = place_of<T, PER, 8>(a, row, b0);
+  const bool there = place_of((long long)blockIdx.x * 32 + (threadIdx.x >> 3), a.total, a.runs, row, b0);
+  b0 *= PER;
   const int n = there ? min(PER, a.blocks - b0) : 0;
   Sixteen<T> in[PER];
   const T* from = a.w + row * a.ld;
@@ -254,9 +254,13 @@ __global__ void __launch_bounds__(256) q4_quantize_kernel(const Held<T> a) {
 template <typename T, int GROUP, int PER>
 __global__ void __launch_bounds__(256) q4_dequantize_kernel(const Held<T> a) {
   const int i = threadIdx.x & 15;
+  // sixteen teams for a tile's sixteen rows, which are read whole
   long long row;
   int b0;
-  if (!place_of<T, PER, 16>(a, row, b0)) return;
+  if (!place_of(blockIdx.x, a.total, a.runs, row, b0)) return;
+  row = row * ROWS + (threadIdx.x >> 4);
+  b0 *= PER;
+  if (row >= a.V) return;
   const int n = min(PER, a.blocks - b0);
   const long long b = tile_of(row, a.blocks, b0);
   const uint32_t* from = a.q + b * TILE_WORDS + word_of(row, i);

@@ -159,7 +159,10 @@ class QuantizedHead:
 
     @property
     def scale(self):
-        by_rows = self.tile_scale.transpose(1, 2).reshape(self.tile_scale.shape[0] * _ROWS, -1)
+        tiles, blocks, rows, per = self.tile_scale.shape
+        by_rows = self.tile_scale.new_empty((tiles * rows, blocks * per))
+        whole = {1: torch.int16, 2: torch.int32, 4: torch.int64}[per]  # a row's scales of a tile, moved as one number
+        by_rows.view(whole).view(tiles, rows, blocks).copy_(self.tile_scale.view(whole).squeeze(3).transpose(1, 2))
         return by_rows[:self.V, :-(-self.D // self.group)]
 
     def dequantize(self, dtype=torch.bfloat16, out=None, stream=None):
