@@ -6,6 +6,7 @@
 #include <cmath>
 
 #include "../../include/pesti_sampler.h"
+#include "pesti_device.h"
 #include "pesti_error.h"
 #include "pesti_lce.cuh"
 #include "pesti_tensor_map.h"
@@ -146,14 +147,9 @@ Layout layout(char* base, int64_t N, int64_t V, int64_t D, bool forward, bool gr
   return l;
 }
 
-int need_device(int& sms) {
-  int n = 0, dev = 0;
-  if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0)
-    return pesti_set_error(PESTI_E_NO_DEVICE, "no CUDA device available");
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, "device query");
-}
+struct Device {
+  int index, sms;
+};
 
 // Every kernel waits on the device for the one before it, so it may be launched while that one still runs.
 template <typename... K, typename... A>
@@ -177,12 +173,13 @@ int launch(const char* what, void (*kernel)(K...), int cg, long long blocks, int
 }
 
 template <int CG, bool BF16, bool A_MN, bool B_MN, Epilogue E>
-int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const GemmArgs& g, int sms,
+int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const GemmArgs& g, Device dev,
                 cudaStream_t st) {
   auto kernel = head_gemm_kernel<CG, BF16, A_MN, B_MN, E>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(CG));
-  if (e != cudaSuccess) return pesti_set_cuda_error(e, "head_gemm_kernel shared memory");
-  return launch("head_gemm_kernel launch", kernel, CG, sms / CG * CG, THREADS, smem_bytes(CG), st, a, b, out, g);
+  static PestiShared shared;
+  const int rc = pesti_allow_shared(shared, kernel, dev.index, smem_bytes(CG), "head_gemm_kernel shared memory");
+  if (rc) return rc;
+  return launch("head_gemm_kernel launch", kernel, CG, dev.sms / CG * CG, THREADS, smem_bytes(CG), st, a, b, out, g);
 }
 
 RowArgs row_args(const Call& c, const Layout& l, int cg, int sms) {
@@ -237,7 +234,7 @@ int a_box(int64_t N) { return N > 96 ? 128 : 32; }
 
 // Packed rows and plan are there.  Statistics of all tiles, then the rows' losses.
 template <int CG, bool BF16>
-int forward(const Call& c, const Layout& l, RowArgs r, bool grads, int sms, cudaStream_t st) {
+int forward(const Call& c, const Layout& l, RowArgs r, bool grads, Device dev, cudaStream_t st) {
   CUtensorMap rows, head;
   int rc = pesti_tensor_map(&rows, pesti_map_type(c.dtype), l.rows, c.D, l.rows_pad, l.ldc * 2, 64, a_box(c.N));
   if (!rc) rc = pesti_tensor_map(&head, pesti_map_type(c.dtype), c.head, c.D, c.V, c.w_ld * 2, 64, 128);
@@ -251,7 +248,7 @@ int forward(const Call& c, const Layout& l, RowArgs r, bool grads, int sms, cuda
   g.V = (int)c.V;
   g.parts = l.parts;
   g.zsum = c.eps != 0.0 ? l.zsum : nullptr;
-  rc = launch_gemm<CG, BF16, false, false, STATS>(rows, head, rows, g, sms, st);
+  rc = launch_gemm<CG, BF16, false, false, STATS>(rows, head, rows, g, dev, st);
   if (rc) return rc;
   r.parts = l.parts;
   r.zsum = g.zsum;
@@ -261,8 +258,8 @@ int forward(const Call& c, const Layout& l, RowArgs r, bool grads, int sms, cuda
 
 // Packed rows, plan and coefficients are there.
 template <int CG, bool BF16>
-int backward(const Call& c, const Layout& l, RowArgs r, void* dh, int64_t dh_ld, void* dw, int64_t dw_ld, int sms,
-             cudaStream_t st) {
+int backward(const Call& c, const Layout& l, RowArgs r, void* dh, int64_t dh_ld, void* dw, int64_t dw_ld,
+             Device dev, cudaStream_t st) {
   CUtensorMap rows_k, rows_mn, head_k, head_mn, out_w, out_h;
   int rc = pesti_tensor_map(&rows_k, pesti_map_type(c.dtype), l.rows, c.D, l.rows_pad, l.ldc * 2, 64, a_box(c.N));
   if (!rc) rc = pesti_tensor_map(&rows_mn, pesti_map_type(c.dtype), l.rows, c.D, l.rows_pad, l.ldc * 2, 64, 64);
@@ -290,7 +287,7 @@ int backward(const Call& c, const Layout& l, RowArgs r, void* dh, int64_t dh_ld,
     g.V = (int)c.V;
     g.out_x = (int)width;
     g.out_y = (int)l.rows_pad;
-    rc = launch_gemm<CG, BF16, false, false, GRAD>(rows_k, head_k, grad_out, g, sms, st);
+    rc = launch_gemm<CG, BF16, false, false, GRAD>(rows_k, head_k, grad_out, g, dev, st);
     if (rc) return rc;
     if (dw) {  // dW = G^T h
       g = gemm_args(l);
@@ -300,7 +297,7 @@ int backward(const Call& c, const Layout& l, RowArgs r, void* dh, int64_t dh_ld,
       g.v0 = (int)v0;
       g.out_x = (int)c.D;
       g.out_y = (int)c.V;
-      rc = launch_gemm<CG, BF16, true, true, OUT16>(grad_mn, rows_mn, out_w, g, sms, st);
+      rc = launch_gemm<CG, BF16, true, true, OUT16>(grad_mn, rows_mn, out_w, g, dev, st);
       if (rc) return rc;
     }
     if (dh) {  // dh += G W
@@ -313,7 +310,7 @@ int backward(const Call& c, const Layout& l, RowArgs r, void* dh, int64_t dh_ld,
       g.add = v0 != 0;
       g.out_x = (int)c.D;
       g.out_y = INT_MAX;
-      rc = launch_gemm<CG, BF16, false, true, PART32>(grad_k, head_mn, out_h, g, sms, st);
+      rc = launch_gemm<CG, BF16, false, true, PART32>(grad_k, head_mn, out_h, g, dev, st);
       if (rc) return rc;
     }
   }
@@ -324,10 +321,10 @@ int backward(const Call& c, const Layout& l, RowArgs r, void* dh, int64_t dh_ld,
 }
 
 int backward(const Call& c, const Layout& l, const RowArgs& r, int cg, void* dh, int64_t dh_ld, void* dw, int64_t dw_ld,
-             int sms, cudaStream_t st) {
+             Device dev, cudaStream_t st) {
   const bool bf16 = c.dtype == PESTI_BF16;
-  if (cg == 1) return (bf16 ? backward<1, true> : backward<1, false>)(c, l, r, dh, dh_ld, dw, dw_ld, sms, st);
-  return (bf16 ? backward<2, true> : backward<2, false>)(c, l, r, dh, dh_ld, dw, dw_ld, sms, st);
+  if (cg == 1) return (bf16 ? backward<1, true> : backward<1, false>)(c, l, r, dh, dh_ld, dw, dw_ld, dev, st);
+  return (bf16 ? backward<2, true> : backward<2, false>)(c, l, r, dh, dh_ld, dw, dw_ld, dev, st);
 }
 
 template <bool BACKWARD>
@@ -368,30 +365,30 @@ int pesti_linear_ce(const void* d_hidden, pesti_dtype dtype, int64_t N, int64_t 
     rc = check_grads(c, d_grad_hidden, gh_ld, d_grad_head, gw_ld);
     if (rc) return rc;
   }
-  int sms = 0;
+  Device dev = {};
   cudaStream_t st = (cudaStream_t)stream;
   if (N == 0) {
-    rc = need_device(sms);
+    rc = pesti_current_device(dev.index, dev.sms);
     if (rc) return rc;
     const cudaError_t e = cudaMemset2DAsync(d_grad_head, gw_ld * 2, 0, D * 2, V, st);
     return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, "cudaMemset2DAsync");
   }
   rc = check_scratch(d_ws, ws_bytes, layout(nullptr, N, V, D, true, grads).bytes);
   if (rc) return rc;
-  rc = need_device(sms);
+  rc = pesti_current_device(dev.index, dev.sms);
   if (rc) return rc;
   const Layout l = layout((char*)d_ws, N, V, D, true, grads);
   const int cg = blocks_per_tile(N);
-  RowArgs r = row_args(c, l, cg, sms);
+  RowArgs r = row_args(c, l, cg, dev.sms);
   r.loss = d_loss;
   r.lse = d_lse;
   rc = pack<false>(r, st);
   if (rc) return rc;
   const bool bf16 = dtype == PESTI_BF16;
-  rc = cg == 1 ? (bf16 ? forward<1, true> : forward<1, false>)(c, l, r, grads, sms, st)
-               : (bf16 ? forward<2, true> : forward<2, false>)(c, l, r, grads, sms, st);
+  rc = cg == 1 ? (bf16 ? forward<1, true> : forward<1, false>)(c, l, r, grads, dev, st)
+               : (bf16 ? forward<2, true> : forward<2, false>)(c, l, r, grads, dev, st);
   if (rc || !grads) return rc;
-  return backward(c, l, r, cg, d_grad_hidden, gh_ld, d_grad_head, gw_ld, sms, st);
+  return backward(c, l, r, cg, d_grad_hidden, gh_ld, d_grad_head, gw_ld, dev, st);
 }
 
 int pesti_linear_ce_backward(const void* d_hidden, pesti_dtype dtype, int64_t N, int64_t D, int64_t h_ld,
@@ -409,27 +406,27 @@ int pesti_linear_ce_backward(const void* d_hidden, pesti_dtype dtype, int64_t N,
   if (N && (!d_lse || !d_up)) return refuse("null lse or upstream gradient");
   rc = check_grads(c, d_grad_hidden, gh_ld, d_grad_head, gw_ld);
   if (rc) return rc;
-  int sms = 0;
+  Device dev = {};
   cudaStream_t st = (cudaStream_t)stream;
   if (N == 0) {
-    rc = need_device(sms);
+    rc = pesti_current_device(dev.index, dev.sms);
     if (rc) return rc;
     const cudaError_t e = cudaMemset2DAsync(d_grad_head, gw_ld * 2, 0, D * 2, V, st);
     return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, "cudaMemset2DAsync");
   }
   rc = check_scratch(d_ws, ws_bytes, layout(nullptr, N, V, D, false, true).bytes);
   if (rc) return rc;
-  rc = need_device(sms);
+  rc = pesti_current_device(dev.index, dev.sms);
   if (rc) return rc;
   const Layout l = layout((char*)d_ws, N, V, D, false, true);
   const int cg = blocks_per_tile(N);
-  RowArgs r = row_args(c, l, cg, sms);
+  RowArgs r = row_args(c, l, cg, dev.sms);
   r.lse_in = d_lse;
   r.up = d_up;
   r.up_stride = up_stride;
   rc = pack<true>(r, st);
   if (rc) return rc;
-  return backward(c, l, r, cg, d_grad_hidden, gh_ld, d_grad_head, gw_ld, sms, st);
+  return backward(c, l, r, cg, d_grad_hidden, gh_ld, d_grad_head, gw_ld, dev, st);
 }
 
 }  // extern "C"

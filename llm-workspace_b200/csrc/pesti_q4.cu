@@ -6,6 +6,7 @@
 #include <type_traits>
 
 #include "../../include/pesti_sampler.h"
+#include "pesti_device.h"
 #include "pesti_error.h"
 #include "pesti_q4.cuh"
 #include "pesti_tensor_map.h"
@@ -41,15 +42,9 @@ bool overlap(const void* p, __int128 np, const void* q, __int128 nq) {
   return (__int128)(uintptr_t)p < (__int128)(uintptr_t)q + nq && (__int128)(uintptr_t)q < (__int128)(uintptr_t)p + np;
 }
 
-int need_device(int* sms = nullptr) {
-  int n = 0, dev = 0;
-  if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0)
-    return pesti_set_error(PESTI_E_NO_DEVICE, "no CUDA device available");
-  if (!sms) return PESTI_OK;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
-  return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, "device query");
-}
+struct Device {
+  int index, sms;
+};
 
 int launched(const char* what) {
   const cudaError_t e = cudaGetLastError();
@@ -149,9 +144,6 @@ int k_warps_of(long long stacks, int blocks, int warps, int sms) {
 template <typename... K, typename... A>
 int launch(const char* what, void (*kernel)(K...), long long blocks, int threads, int smem, cudaStream_t st,
            const A&... args) {
-  cudaError_t e = cudaSuccess;
-  if (smem > 48 << 10) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return pesti_set_cuda_error(e, what);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3(threads);
@@ -162,27 +154,35 @@ int launch(const char* what, void (*kernel)(K...), long long blocks, int threads
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kernel, K(args)...);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, K(args)...);
   return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, what);
 }
 
 template <typename T, int GROUP, int COLUMNS>
-int wide_pass(const LogitArgs& a, int sms, const CUtensorMap& weights, cudaStream_t st) {
-  return launch("q4_wide_kernel launch", q4_wide_kernel<T, GROUP, COLUMNS>, std::min(sms, a.stacks), WIDE_THREADS,
-                1024 + a.stages * (SLOTS * WIDE_BYTES + COLUMNS * (sizeof(T) == 4 ? 3 : 1) * (BLOCK * 2)), st, weights,
-                a);
+int wide_pass(const LogitArgs& a, Device dev, const CUtensorMap& weights, cudaStream_t st) {
+  constexpr int P = sizeof(T) == 4 ? 3 : 1;
+  const auto kernel = q4_wide_kernel<T, GROUP, COLUMNS>;
+  const int smem = 1024 + a.stages * (SLOTS * WIDE_BYTES + COLUMNS * P * (BLOCK * 2));
+  static PestiShared shared;
+  const int rc = pesti_allow_shared(shared, kernel, dev.index, smem, "q4_wide_kernel shared memory");
+  if (rc) return rc;
+  return launch("q4_wide_kernel launch", kernel, std::min(dev.sms, a.stacks), WIDE_THREADS, smem, st, weights, a);
 }
 
 template <typename T, int GROUP>
-int pass(LogitArgs a, int sms, cudaStream_t st) {
+int pass(LogitArgs a, Device dev, cudaStream_t st) {
   constexpr int P = sizeof(T) == 4 ? 3 : 1;
   if (few(a.D, P, a.rows)) {
     a.stacks = (a.V + STACK * ROWS - 1) / (STACK * ROWS);
-    a.k_warps = k_warps_of(a.stacks, a.blocks, few_warps(P), sms);
+    a.k_warps = k_warps_of(a.stacks, a.blocks, few_warps(P), dev.sms);
     const int slots = few_warps(P) / a.k_warps;
     const int smem = a.blocks * a.rows * P * (BLOCK * 2) + 16 + (few_warps(P) - slots) * STACK * 4 * 32 * 4;
-    return launch("q4_logits_kernel launch", q4_logits_kernel<T, GROUP>,
-                  std::min<long long>(sms, (a.stacks + slots - 1) / slots), few_warps(P) * 32, smem, st, a);
+    const auto kernel = q4_logits_kernel<T, GROUP>;
+    static PestiShared shared;
+    const int rc = pesti_allow_shared(shared, kernel, dev.index, smem, "q4_logits_kernel shared memory");
+    if (rc) return rc;
+    return launch("q4_logits_kernel launch", kernel, std::min<long long>(dev.sms, (a.stacks + slots - 1) / slots),
+                  few_warps(P) * 32, smem, st, a);
   }
   a.stacks = (a.V + WIDE - 1) / WIDE;
   const int columns = columns_of(a.rows);
@@ -193,23 +193,23 @@ int pass(LogitArgs a, int sms, cudaStream_t st) {
   if (!rc) rc = launch("q4_operand_kernel launch", q4_operand_kernel<T>, a.blocks, 256, 0, st, a, columns);
   if (rc) return rc;
   a.stages = std::min(8, SHARED_BYTES / (SLOTS * WIDE_BYTES + columns * P * (BLOCK * 2)));
-  if (columns == 16) return wide_pass<T, GROUP, 16>(a, sms, weights, st);
-  if (columns == 32) return wide_pass<T, GROUP, 32>(a, sms, weights, st);
-  if (columns == 48) return wide_pass<T, GROUP, 48>(a, sms, weights, st);
-  return wide_pass<T, GROUP, 64>(a, sms, weights, st);
+  if (columns == 16) return wide_pass<T, GROUP, 16>(a, dev, weights, st);
+  if (columns == 32) return wide_pass<T, GROUP, 32>(a, dev, weights, st);
+  if (columns == 48) return wide_pass<T, GROUP, 48>(a, dev, weights, st);
+  return wide_pass<T, GROUP, 64>(a, dev, weights, st);
 }
 
 template <typename T>
-int logits(LogitArgs a, int64_t group, int64_t B, pesti_dtype out, int sms, cudaStream_t st) {
+int logits(LogitArgs a, int64_t group, int64_t B, pesti_dtype out, Device dev, cudaStream_t st) {
   const char* x = (const char*)a.x;
   char* y = (char*)a.y;
   for (int64_t r = 0; r < B; r += MOST_ROWS) {
     a.rows = (int)std::min<int64_t>(MOST_ROWS, B - r);
     a.x = x + r * a.x_ld * sizeof(T);
     a.y = y + r * a.y_ld * esize(out);
-    const int rc = group == 32   ? pass<T, 32>(a, sms, st)
-                   : group == 64 ? pass<T, 64>(a, sms, st)
-                                 : pass<T, 128>(a, sms, st);
+    const int rc = group == 32   ? pass<T, 32>(a, dev, st)
+                   : group == 64 ? pass<T, 64>(a, dev, st)
+                                 : pass<T, 128>(a, dev, st);
     if (rc) return rc;
   }
   return PESTI_OK;
@@ -222,14 +222,16 @@ extern "C" {
 int pesti_q4_quantize(const void* d_head, pesti_dtype dtype, int64_t V, int64_t D, int64_t ld, int64_t group,
                       void* d_q, void* d_scale, void* stream) {
   int rc = check_plain(d_head, dtype, V, D, ld, group, d_q, d_scale);
-  if (!rc) rc = need_device();
+  Device dev = {};
+  if (!rc) rc = pesti_current_device(dev.index, dev.sms);
   return rc ? rc : convert(true, dtype, group, d_head, V, D, ld, d_q, d_scale, (cudaStream_t)stream);
 }
 
 int pesti_q4_dequantize(const void* d_q, const void* d_scale, int64_t V, int64_t D, int64_t group, void* d_head,
                         pesti_dtype dtype, int64_t ld, void* stream) {
   int rc = check_plain(d_head, dtype, V, D, ld, group, d_q, d_scale);
-  if (!rc) rc = need_device();
+  Device dev = {};
+  if (!rc) rc = pesti_current_device(dev.index, dev.sms);
   return rc ? rc
             : convert(false, dtype, group, d_head, V, D, ld, const_cast<void*>(d_q), const_cast<void*>(d_scale),
                       (cudaStream_t)stream);
@@ -265,8 +267,8 @@ int pesti_q4_logits(const void* d_x, pesti_dtype dtype, int64_t B, int64_t D, in
     return refuse("inputs and logits overlap");
   if (!d_ws || ws_bytes < need) return refuse("workspace too small");
   if ((uintptr_t)d_ws % 256) return refuse("workspace is not 256-byte aligned");
-  int sms = 0;
-  rc = need_device(&sms);
+  Device dev = {};
+  rc = pesti_current_device(dev.index, dev.sms);
   if (rc) return rc;
   LogitArgs a = {};
   a.x = d_x;
@@ -281,9 +283,9 @@ int pesti_q4_logits(const void* d_x, pesti_dtype dtype, int64_t B, int64_t D, in
   a.y_ld = ld;
   a.out = out_dtype == PESTI_F32 ? 0 : out_dtype == PESTI_BF16 ? 1 : 2;
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == PESTI_F32) return logits<float>(a, group, B, out_dtype, sms, st);
-  if (dtype == PESTI_BF16) return logits<__nv_bfloat16>(a, group, B, out_dtype, sms, st);
-  return logits<__half>(a, group, B, out_dtype, sms, st);
+  if (dtype == PESTI_F32) return logits<float>(a, group, B, out_dtype, dev, st);
+  if (dtype == PESTI_BF16) return logits<__nv_bfloat16>(a, group, B, out_dtype, dev, st);
+  return logits<__half>(a, group, B, out_dtype, dev, st);
 }
 
 }  // extern "C"

@@ -29,6 +29,7 @@ from pesti_beam import _DTYPES, _launch, _need, _ptr, _row_stride, _written
 from pesti_sampler import PESTI_BF16, PESTI_F16, _check, load_library
 
 _HALVES = {torch.bfloat16: PESTI_BF16, torch.float16: PESTI_F16}
+_TARGETS = {torch.int64: 8, torch.int32: 4}
 _FORWARD, _GRADS = 1, 2  # PESTI_LINEAR_CE_*
 
 
@@ -41,39 +42,47 @@ def _ce_workspace(dtype: int, N: int, V: int, D: int, passes: int) -> int:
 
 def _ce_args(hidden, head, target, weight, label_smoothing, z_loss):
     """Checks the arguments and returns them in the C call's order."""
-    dtype = _HALVES.get(hidden.dtype)
-    _need(dtype is not None and head.dtype == hidden.dtype, "hidden and head must both be bfloat16 or both float16")
-    _need(hidden.dim() == 2 and head.dim() == 2 and hidden.shape[1] == head.shape[1],
-          "hidden must be [N, D] and head [V, D]")
-    (N, D), V, dev = hidden.shape, head.shape[0], hidden.device
-    _need(D >= 1 and V >= 1, "D and V must be at least 1")
-    _need(head.device == dev and target.device == dev, "head and target must be on the hidden states' device")
-    _need(D == 1 or (hidden.stride(1) == 1 and head.stride(1) == 1), "rows of hidden and head must be contiguous")
-    _need(target.shape == (N,) and target.dtype in (torch.int64, torch.int32) and target.is_contiguous(),
-          "target must be a contiguous [N] int64 or int32 tensor")
-    if weight is not None:
-        _need(weight.device == dev and weight.dtype == torch.float32 and weight.shape == (N,)
-              and weight.is_contiguous(), "weight must be a contiguous [N] float32 tensor on the hidden states' device")
-    w_ld = head.stride(0) if V > 1 else -(-D // 8) * 8
-    return (hidden.data_ptr(), dtype, N, D, hidden.stride(0) if N > 1 else D, head.data_ptr(), V, w_ld,
-            target.data_ptr(), target.element_size(), _ptr(weight), float(label_smoothing), float(z_loss))
+    kind, dev, shape, to_hidden, to_head = hidden.dtype, hidden.device, hidden.shape, hidden.stride(), head.stride()
+    dtype = _HALVES.get(kind)
+    if dtype is None or head.dtype != kind:
+        raise ValueError("hidden and head must both be bfloat16 or both float16")
+    if len(to_hidden) != 2 or len(to_head) != 2 or shape[1] != head.shape[1]:
+        raise ValueError("hidden must be [N, D] and head [V, D]")
+    (N, D), V = shape, head.shape[0]
+    if D < 1 or V < 1:
+        raise ValueError("D and V must be at least 1")
+    if head.device != dev or target.device != dev:
+        raise ValueError("head and target must be on the hidden states' device")
+    if D > 1 and (to_hidden[1] != 1 or to_head[1] != 1):
+        raise ValueError("rows of hidden and head must be contiguous")
+    size = _TARGETS.get(target.dtype)
+    if size is None or target.shape != (N,) or not target.is_contiguous():
+        raise ValueError("target must be a contiguous [N] int64 or int32 tensor")
+    if weight is not None and not (weight.device == dev and weight.dtype == torch.float32 and weight.shape == (N,)
+                                   and weight.is_contiguous()):
+        raise ValueError("weight must be a contiguous [N] float32 tensor on the hidden states' device")
+    return (hidden.data_ptr(), dtype, N, D, to_hidden[0] if N > 1 else D, head.data_ptr(), V,
+            to_head[0] if V > 1 else -(-D // 8) * 8, target.data_ptr(), size, _ptr(weight), float(label_smoothing),
+            float(z_loss))
 
 
 def _rows_like(t, rows: int, D: int):
     """[rows, D] with rows that begin at multiples of 16 bytes."""
-    return t.new_empty((rows, -(-D // 8) * 8))[:, :D]
+    return t.new_empty((rows, D)) if D % 8 == 0 else t.new_empty((rows, -(-D // 8) * 8))[:, :D]
 
 
-def _ce_forward(args, like, lse: bool, grad_hidden: bool, grad_head: bool, st):
+def _ce_forward(args, like, lse: bool, grads: bool, st):
     dtype, N, D, V = args[1], args[2], args[3], args[6]
     loss = like.new_empty(N, dtype=torch.float32)
     lse = like.new_empty(N, dtype=torch.float32) if lse else None
-    gh = like.new_empty((N, D)) if grad_hidden else None
-    gw = _rows_like(like, V, D) if grad_head else None
-    need = _ce_workspace(dtype, N, V, D, _FORWARD | (_GRADS if grad_hidden or grad_head else 0))
+    gh = like.new_empty((N, D)) if grads else None
+    gw = _rows_like(like, V, D) if grads else None
+    need = _ce_workspace(dtype, N, V, D, _FORWARD | _GRADS if grads else _FORWARD)
     ws = like.new_empty(need, dtype=torch.uint8)
-    _check(load_library().pesti_linear_ce(*args, loss.data_ptr(), _ptr(lse), _ptr(gh), D, _ptr(gw),
-                                          -(-D // 8) * 8, ws.data_ptr(), need, st))
+    rc = load_library().pesti_linear_ce(*args, loss.data_ptr(), _ptr(lse), _ptr(gh), D, _ptr(gw), -(-D // 8) * 8,
+                                        ws.data_ptr(), need, st)
+    if rc:
+        _check(rc)
     return loss, lse, gh, gw
 
 
@@ -82,7 +91,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def forward(ctx, hidden, head, target, weight, label_smoothing, z_loss):
         args = _ce_args(hidden, head, target, weight, label_smoothing, z_loss)
         keep = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
-        loss, lse, _, _ = _launch(hidden.device, None, lambda st: _ce_forward(args, hidden, keep, False, False, st))
+        loss, lse, _, _ = _launch(hidden.device, None, lambda st: _ce_forward(args, hidden, keep, False, st))
         if keep:
             ctx.more = label_smoothing, z_loss
             ctx.save_for_backward(hidden, head, target, weight, lse)
@@ -104,9 +113,11 @@ class _LinearCrossEntropy(torch.autograd.Function):
             gw = _rows_like(head, V, D) if ctx.needs_input_grad[1] else None
             need = _ce_workspace(dtype, N, V, D, _GRADS)
             ws = hidden.new_empty(need, dtype=torch.uint8)
-            _check(load_library().pesti_linear_ce_backward(
+            rc = load_library().pesti_linear_ce_backward(
                 *args, lse.data_ptr(), up.data_ptr(), up.stride(0), _ptr(gh), D, _ptr(gw), -(-D // 8) * 8,
-                ws.data_ptr(), need, st))
+                ws.data_ptr(), need, st)
+            if rc:
+                _check(rc)
             return gh, gw
 
         return *_launch(hidden.device, None, call), None, None, None, None
@@ -135,7 +146,7 @@ def linear_cross_entropy_grad(hidden, head, target, weight=None, label_smoothing
     mask)."""
     hidden, head = hidden.detach(), head.detach()
     args = _ce_args(hidden, head, target, weight, label_smoothing, z_loss)
-    loss, _, gh, gw = _launch(hidden.device, stream, lambda st: _ce_forward(args, hidden, False, True, True, st))
+    loss, _, gh, gw = _launch(hidden.device, stream, lambda st: _ce_forward(args, hidden, False, True, st))
     return loss, gh, gw
 
 
