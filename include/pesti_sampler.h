@@ -562,8 +562,8 @@ int pesti_linear_ce_backward(const void* d_hidden, pesti_dtype dtype, int64_t N,
  * Products of x and q are exact, summed in f32 over a group and then over the
  * groups with their scales, and rounded once.  The weight is read once for
  * every 64 rows of x.  The logits overlap no input
- * (refused).  d_ws: device scratch of pesti_q4_logits_workspace(...) bytes,
- * 256-byte aligned, any contents; calls whose GPU work may overlap need scratch
+ * (refused).  d_ws: device scratch of pesti_q4_logits_workspace(...) bytes
+ * (0 for few rows: NULL will do), 256-byte aligned, any contents; calls whose GPU work may overlap need scratch
  * of their own.
  * All run on the calling thread's current device, stream-ordered (NULL: the
  * legacy default stream), allocate nothing, add in a fixed order (the same

@@ -129,7 +129,7 @@ int k_warps_of(long long stacks, int blocks, int warps, int sms) {
   double best = 1e30;
   int at = 1;
   for (int kw = 1; kw <= warps && kw <= blocks; ++kw) {
-    if (warps % kw) continue;
+    if (warps % kw || (kw > 1 && warps / kw > MOST_SLOTS)) continue;
     const int slots = warps / kw, turns = (blocks + kw - 1) / kw;
     const long long rounds = (stacks + (long long)sms * slots - 1) / ((long long)sms * slots);
     const double t = (double)rounds * (warps * turns * (STACK * TILE_BYTES) / 44.0 + 500.0 + 50.0 * kw);
@@ -206,6 +206,7 @@ int logits(LogitArgs a, int64_t group, int64_t B, pesti_dtype out, Device dev, c
   for (int64_t r = 0; r < B; r += MOST_ROWS) {
     a.rows = (int)std::min<int64_t>(MOST_ROWS, B - r);
     a.x = x + r * a.x_ld * sizeof(T);
+    a.x_vec = (uintptr_t)a.x % 16 == 0 && a.x_ld * sizeof(T) % 16 == 0;
     a.y = y + r * a.y_ld * esize(out);
     const int rc = group == 32   ? pass<T, 32>(a, dev, st)
                    : group == 64 ? pass<T, 64>(a, dev, st)
@@ -242,7 +243,7 @@ int64_t pesti_q4_logits_workspace(pesti_dtype dtype, int64_t B, int64_t D) {
   if (B < 0) return refuse("B < 0");
   if (B > 1 << 24) return refuse("B must be at most 2^24");
   if (D < 1 || D > 1 << 20) return refuse("D must be 1 to 2^20");
-  if (few(D, pieces_of(dtype), B)) return 256;
+  if (few(D, pieces_of(dtype), B)) return 0;
   return blocks_of(D) * columns_of(std::min<int64_t>(B, MOST_ROWS)) * pieces_of(dtype) * (BLOCK * 2);
 }
 
@@ -265,7 +266,7 @@ int pesti_q4_logits(const void* d_x, pesti_dtype dtype, int64_t B, int64_t D, in
   if (overlap(d_logits, ny, d_x, nx) || overlap(d_logits, ny, d_q, tiles * TILE_BYTES) ||
       overlap(d_logits, ny, d_scale, tiles * (ROWS * BLOCK / group) * 2))
     return refuse("inputs and logits overlap");
-  if (!d_ws || ws_bytes < need) return refuse("workspace too small");
+  if (need && (!d_ws || ws_bytes < need)) return refuse("workspace too small");
   if ((uintptr_t)d_ws % 256) return refuse("workspace is not 256-byte aligned");
   Device dev = {};
   rc = pesti_current_device(dev.index, dev.sms);

@@ -303,6 +303,7 @@ struct LogitArgs {
   const void* x;
   long long x_ld;
   int rows, D;  // of x; at most 64 rows
+  int x_vec;    // whole vectors of 8 columns can be read
   const uint4* q;
   const __nv_bfloat16* scale;
   int V, blocks, stacks;  // stacks of 64 rows, or of 128
@@ -324,33 +325,44 @@ __device__ __forceinline__ void store_logit(const LogitArgs& a, int row, int v, 
     ((__half*)a.y)[at] = __float2half_rn(y);
 }
 
-// The bf16 or f16 bits of piece `p` of an x: f32 is cut into three bf16 whose sum it is, exactly.
+// Eight columns of x from `at` for lane t of a quad, as the pairs (i, i + 4) that a word of weights unpacks to: one
+// fragment for a 16-bit x, three for f32, which is cut into three bf16 whose sum it is, exactly.
 template <typename T>
-__device__ __forceinline__ uint32_t piece_of(T x, int p) {
-  if constexpr (sizeof(T) == 2) {
-    return *(const uint16_t*)&x;
-  } else {
-    float rest = x;
-    uint32_t bits = fbits(rest);
-    for (int i = 0; i < p; ++i) {
-      const bool whole = (bits & 0x7f800000u) == 0x7f800000u;  // inf and NaN are in the first piece
-      rest = whole ? 0.0f : rest - bitsf(bits & 0xffff0000u);
-      bits = fbits(rest);
+__device__ __forceinline__ void fragments_of(const T* row, int at, int D, bool vec, uint4 (&f)[sizeof(T) == 4 ? 3 : 1]) {
+  constexpr int P = sizeof(T) == 4 ? 3 : 1;
+  uint32_t raw[2 * sizeof(T)];
+  if (vec && at + 8 <= D) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      const uint4 w = *((const uint4*)(row + at) + i);
+      raw[4 * i] = w.x;
+      raw[4 * i + 1] = w.y;
+      raw[4 * i + 2] = w.z;
+      raw[4 * i + 3] = w.w;
     }
-    return bits >> 16 | (is_nan(rest) ? 0x40u : 0u);
+  } else {
+    T* v = (T*)raw;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = at + i < D ? row[at + i] : from_f32<T>(0.0f);
   }
-}
-
-// Four pairs of x for lane t of a quad, word j of block b: columns 32 j + 8 t + (i, i + 4), as a word of weights unpacks.
-template <typename T>
-__device__ __forceinline__ uint4 fragment_of(const T* row, int b, int j, int t, int piece, int D) {
-  const int at = b * BLOCK + 32 * j + 8 * t;
-  uint32_t v[8], f[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = at + i < D ? piece_of(row[at + i], piece) : 0u;
+  for (int p = 0; p < P; ++p) {
+    uint32_t bits[8];  // in the upper half
 #pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = v[i] | v[i + 4] << 16;
-  return make_uint4(f[0], f[1], f[2], f[3]);
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (P == 1) {
+        bits[i] = i & 1 ? raw[i / 2] : raw[i / 2] << 16;
+      } else {
+        bits[i] = raw[i];
+        // an infinity or a NaN is in the first piece (with a bit in its upper half)
+        const bool whole = (raw[i] & 0x7f800000u) == 0x7f800000u;
+        if (whole && (raw[i] & 0x7fffffu)) bits[i] |= 0x400000u;
+        raw[i] = whole ? 0u : fbits(bitsf(raw[i]) - bitsf(raw[i] & 0xffff0000u));
+      }
+    }
+    f[p] = make_uint4(__byte_perm(bits[0], bits[4], 0x7632), __byte_perm(bits[1], bits[5], 0x7632),
+                      __byte_perm(bits[2], bits[6], 0x7632), __byte_perm(bits[3], bits[7], 0x7632));
+  }
 }
 
 // Nibbles i and i + 4 of a word as two 16-bit floats q: the nibble becomes the mantissa's low end of 128 (bf16) or
@@ -416,6 +428,15 @@ constexpr int STACK = 4;  // tiles of a warp, one above the other: x's fragments
 // Warps that multiply: their registers hold a stack's sums and next weights and the fragments of a block of x.
 __host__ __device__ constexpr int few_warps(int pieces) { return pieces == 1 ? 16 : 12; }
 
+// Barriers 1 to 7 and 8 to 14 of a block, one for each slot.
+constexpr int MOST_SLOTS = 7;
+__device__ __forceinline__ void named_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void named_arrive(int id, int threads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
 // Up to 8 rows of x: a warp multiplies a stack of 64 rows of the weight by all of them over its share of K (every
 // k_warps-th block), and goes on to its next stack; the k_warps warps of a stack join their sums in shared memory, in
 // their order.  x is laid out in shared memory once, while the first weights are on their way; a tile's weights are
@@ -469,9 +490,13 @@ __global__ void __launch_bounds__(few_warps(sizeof(T) == 4 ? 3 : 1) * 32, 1) q4_
   for (int i = 0; i < STACK; ++i) load(i);
   advance();
 
-  for (int e = threadIdx.x; e < a.blocks * per_block; e += WARPS * 32) {
-    const int tt = e & 3, rest = e >> 2, c = rest % columns, bjp = rest / columns, p = bjp % P, bj = bjp / P;
-    xs[e] = fragment_of((const T*)a.x + c * a.x_ld, bj >> 2, bj & 3, tt, p, a.D);
+  for (int c = 0; c < columns; ++c) {
+    for (int e = threadIdx.x; e < a.blocks * 16; e += WARPS * 32) {
+      uint4 f[P];
+      fragments_of((const T*)a.x + c * a.x_ld, 8 * e, a.D, a.x_vec, f);  // block, j, t
+#pragma unroll
+      for (int p = 0; p < P; ++p) xs[((e >> 2) * P + p) * columns * 4 + c * 4 + (e & 3)] = f[p];
+    }
   }
   if (threadIdx.x == 0) xs[a.blocks * per_block] = make_uint4(0, 0, 0, 0);
   __syncthreads();
@@ -526,20 +551,22 @@ __global__ void __launch_bounds__(few_warps(sizeof(T) == 4 ? 3 : 1) * 32, 1) q4_
       advance();
     }
     const int stack = stack_of(r);
-    if (kw > 1) {  // [slot][part - 1][value][lane]
+    if (kw > 1) {  // [slot][part - 1][value][lane]; only the part that joins waits for the others
+      const int threads = kw * 32;
       if (part) {
+        if (r) named_sync(8 + slot, threads);  // the last round's sums are read
         float* to = sums + (slot * (kw - 1) + (part - 1)) * STACK * 4 * 32 + lane;
 #pragma unroll
         for (int e = 0; e < STACK * 4; ++e) to[e * 32] = acc[e >> 2][e & 3];
-      }
-      __syncthreads();
-      if (!part) {
+        named_arrive(1 + slot, threads);
+      } else {
+        named_sync(1 + slot, threads);
         for (int k = 0; k < kw - 1; ++k)
 #pragma unroll
           for (int e = 0; e < STACK * 4; ++e)
             acc[e >> 2][e & 3] += sums[((slot * (kw - 1) + k) * STACK * 4 + e) * 32 + lane];
+        if (r + 1 < rounds) named_arrive(8 + slot, threads);
       }
-      __syncthreads();
     }
     if (part || stack >= a.stacks) continue;
 #pragma unroll
@@ -563,12 +590,14 @@ __global__ void __launch_bounds__(256) q4_operand_kernel(const LogitArgs a, int 
   pesti_umma::depend_wait();
   pesti_umma::depend_launch();
   constexpr int P = sizeof(T) == 4 ? 3 : 1;
-  const int per_block = 2 * P * columns * 8, b = blockIdx.x;
-  for (int e = threadIdx.x; e < per_block; e += 256) {
-    const int c = e & 7, n = (e >> 3) % columns, hp = (e >> 3) / columns, p = hp % P, h = hp / P;
-    uint4 f = make_uint4(0, 0, 0, 0);
-    if (n < a.rows) f = fragment_of((const T*)a.x + n * a.x_ld, b, 2 * h + (c >> 2), c & 3, p, a.D);
-    a.operand[(long long)b * per_block + (e & ~7) + (c ^ (n & 7))] = f;
+  const int b = blockIdx.x;
+  for (int e = threadIdx.x; e < 16 * columns; e += 256) {
+    const int c = e & 7, h = e >> 3 & 1, n = e >> 4;
+    uint4 f[P] = {};
+    if (n < a.rows) fragments_of((const T*)a.x + n * a.x_ld, b * BLOCK + 8 * (8 * h + c), a.D, a.x_vec, f);
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+      a.operand[((long long)((b * 2 + h) * P + p) * columns + n) * 8 + (c ^ (n & 7))] = f[p];
   }
 }
 

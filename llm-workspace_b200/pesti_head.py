@@ -256,10 +256,12 @@ def head_logits(x, held: QuantizedHead, dtype=None, out=None, stream=None):
         to = out if out is not None else x.new_empty((B, held.V), dtype=dtype)
         if B:
             need = _logits_workspace(code, B, D)
-            ws = x.new_empty(need, dtype=torch.uint8)
-            _check(load_library().pesti_q4_logits(
+            ws = x.new_empty(need, dtype=torch.uint8) if need else None
+            rc = load_library().pesti_q4_logits(
                 x.data_ptr(), code, B, D, _row_stride(x), held.packed.data_ptr(), held.tile_scale.data_ptr(),
-                held.V, held.group, to.data_ptr(), _DTYPES[to.dtype], _row_stride(to), ws.data_ptr(), need, st))
+                held.V, held.group, to.data_ptr(), _DTYPES[to.dtype], _row_stride(to), _ptr(ws), need, st)
+            if rc:
+                _check(rc)
             if out is not None:
                 _written((out,))
         return to

@@ -88,7 +88,7 @@ def test_conversion_refusals(lib, change, msg):
         assert msg in lib.pesti_last_error().decode()
 
 
-LOGITS = dict(x=P, dtype=ps.PESTI_BF16, B=3, D=300, x_ld=300, q=Q, scale=R, V=100, group=64, logits=S,
+LOGITS = dict(x=P, dtype=ps.PESTI_BF16, B=30, D=300, x_ld=300, q=Q, scale=R, V=100, group=64, logits=S,
               out=ps.PESTI_F32, ld=100, ws=P, ws_bytes=1 << 30, stream=None)
 
 
