@@ -111,16 +111,16 @@ int convert(bool there, pesti_dtype dtype, int64_t group, const void* w, int64_t
 }
 
 constexpr int MOST_ROWS = 64;            // of x, a pass over the weight
-constexpr int FEW_ROWS = 8;              // a column tile of the products by warps
 constexpr int SHARED_BYTES = 200 << 10;  // for x, or for the stages
 
-int pieces_of(pesti_dtype d) { return d == PESTI_F32 ? 3 : 1; }
+int pieces_of(pesti_dtype d) { return d == PESTI_F32 ? pieces<float> : 1; }
 
 int columns_of(int64_t rows) { return (int)(rows + 15) / 16 * 16; }
 
-// Few rows of x that fit shared memory whole.
+// Few rows of x that fit shared memory whole.  A column tile of the products by warps holds 8; f32 rows cost them two
+// products (us for 4 / 8 / on tensor memory, 128256 x 4096: 82 / 88 / 89; 32001 x 1000: 12 / 14 / 11).
 bool few(int64_t D, int pieces, int64_t rows) {
-  return rows <= FEW_ROWS && blocks_of(D) * rows * pieces * (BLOCK * 2) <= SHARED_BYTES;
+  return rows <= (pieces == 1 ? 8 : 4) && blocks_of(D) * rows * pieces * (BLOCK * 2) <= SHARED_BYTES;
 }
 
 // How a pass with few rows shares its stacks and K out: the least time of the busiest SM, by the weight's bytes that it
@@ -158,10 +158,9 @@ int launch(const char* what, void (*kernel)(K...), long long blocks, int threads
   return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, what);
 }
 
-template <typename T, int GROUP, int COLUMNS>
+template <bool BF16, int P, int GROUP, int COLUMNS>
 int wide_pass(const LogitArgs& a, Device dev, const CUtensorMap& weights, cudaStream_t st) {
-  constexpr int P = sizeof(T) == 4 ? 3 : 1;
-  const auto kernel = q4_wide_kernel<T, GROUP, COLUMNS>;
+  const auto kernel = q4_wide_kernel<BF16, P, GROUP, COLUMNS>;
   const int smem = 1024 + a.stages * (SLOTS * WIDE_BYTES + COLUMNS * P * (BLOCK * 2));
   static PestiShared shared;
   const int rc = pesti_allow_shared(shared, kernel, dev.index, smem, "q4_wide_kernel shared memory");
@@ -171,18 +170,18 @@ int wide_pass(const LogitArgs& a, Device dev, const CUtensorMap& weights, cudaSt
 
 template <typename T, int GROUP>
 int pass(LogitArgs a, Device dev, cudaStream_t st) {
-  constexpr int P = sizeof(T) == 4 ? 3 : 1;
+  constexpr int P = pieces<T>;
   if (few(a.D, P, a.rows)) {
     a.stacks = (a.V + STACK * ROWS - 1) / (STACK * ROWS);
-    a.k_warps = k_warps_of(a.stacks, a.blocks, few_warps(P), dev.sms);
-    const int slots = few_warps(P) / a.k_warps;
-    const int smem = a.blocks * a.rows * P * (BLOCK * 2) + 16 + (few_warps(P) - slots) * STACK * 4 * 32 * 4;
+    a.k_warps = k_warps_of(a.stacks, a.blocks, FEW_WARPS, dev.sms);
+    const int slots = FEW_WARPS / a.k_warps;
+    const int smem = a.blocks * a.rows * P * (BLOCK * 2) + 16 + (FEW_WARPS - slots) * STACK * 4 * 32 * 4;
     const auto kernel = q4_logits_kernel<T, GROUP>;
     static PestiShared shared;
     const int rc = pesti_allow_shared(shared, kernel, dev.index, smem, "q4_logits_kernel shared memory");
     if (rc) return rc;
     return launch("q4_logits_kernel launch", kernel, std::min<long long>(dev.sms, (a.stacks + slots - 1) / slots),
-                  few_warps(P) * 32, smem, st, a);
+                  FEW_WARPS * 32, smem, st, a);
   }
   a.stacks = (a.V + WIDE - 1) / WIDE;
   const int columns = columns_of(a.rows);
@@ -190,13 +189,13 @@ int pass(LogitArgs a, Device dev, cudaStream_t st) {
   const long long row = (long long)a.blocks * TILE_BYTES;
   int rc = pesti_tensor_map(&weights, CU_TENSOR_MAP_DATA_TYPE_UINT32, a.q, row / 4, (a.V + ROWS - 1) / ROWS, row,
                             TILE_WORDS, WIDE / ROWS, CU_TENSOR_MAP_SWIZZLE_NONE);
-  if (!rc) rc = launch("q4_operand_kernel launch", q4_operand_kernel<T>, a.blocks, 256, 0, st, a, columns);
+  if (!rc) rc = launch("q4_operand_kernel launch", q4_operand_kernel<T>, columns, 256, 0, st, a, columns);
   if (rc) return rc;
   a.stages = std::min(8, SHARED_BYTES / (SLOTS * WIDE_BYTES + columns * P * (BLOCK * 2)));
-  if (columns == 16) return wide_pass<T, GROUP, 16>(a, dev, weights, st);
-  if (columns == 32) return wide_pass<T, GROUP, 32>(a, dev, weights, st);
-  if (columns == 48) return wide_pass<T, GROUP, 48>(a, dev, weights, st);
-  return wide_pass<T, GROUP, 64>(a, dev, weights, st);
+  if (columns == 16) return wide_pass<in_bf16<T>, P, GROUP, 16>(a, dev, weights, st);
+  if (columns == 32) return wide_pass<in_bf16<T>, P, GROUP, 32>(a, dev, weights, st);
+  if (columns == 48) return wide_pass<in_bf16<T>, P, GROUP, 48>(a, dev, weights, st);
+  return wide_pass<in_bf16<T>, P, GROUP, 64>(a, dev, weights, st);
 }
 
 template <typename T>
@@ -244,7 +243,9 @@ int64_t pesti_q4_logits_workspace(pesti_dtype dtype, int64_t B, int64_t D) {
   if (B > 1 << 24) return refuse("B must be at most 2^24");
   if (D < 1 || D > 1 << 20) return refuse("D must be 1 to 2^20");
   if (few(D, pieces_of(dtype), B)) return 0;
-  return blocks_of(D) * columns_of(std::min<int64_t>(B, MOST_ROWS)) * pieces_of(dtype) * (BLOCK * 2);
+  // the operand, and each row's power of two
+  const int64_t columns = columns_of(std::min<int64_t>(B, MOST_ROWS));
+  return columns * (blocks_of(D) * pieces_of(dtype) * (BLOCK * 2) + 8);
 }
 
 int pesti_q4_logits(const void* d_x, pesti_dtype dtype, int64_t B, int64_t D, int64_t x_ld, const void* d_q,

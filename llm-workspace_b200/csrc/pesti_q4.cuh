@@ -325,73 +325,116 @@ __device__ __forceinline__ void store_logit(const LogitArgs& a, int row, int v, 
     ((__half*)a.y)[at] = __float2half_rn(y);
 }
 
-// Eight columns of x from `at` for lane t of a quad, as the pairs (i, i + 4) that a word of weights unpacks to: one
-// fragment for a 16-bit x, three for f32, which is cut into three bf16 whose sum it is, exactly.
+// 16-bit x enters the products as it is.  f32 x enters them as a sum of two f16, times a power of two of its row that
+// brings the row's largest finite value to 2^14 or more: off by at most 2^-24 of itself or 2^-39 of that value, which is
+// below what an f32 sum of the products loses.  (Three bf16, exact without a power of two, cost a product more, 97 us
+// instead of 77 for a row of 128256 x 4096.)
 template <typename T>
-__device__ __forceinline__ void fragments_of(const T* row, int at, int D, bool vec, uint4 (&f)[sizeof(T) == 4 ? 3 : 1]) {
-  constexpr int P = sizeof(T) == 4 ? 3 : 1;
+constexpr int pieces = sizeof(T) == 4 ? 2 : 1;
+template <typename T>
+constexpr bool in_bf16 = std::is_same<T, __nv_bfloat16>::value;
+
+// Eight columns of a row of x.
+template <typename T>
+struct EightX {
   uint32_t raw[2 * sizeof(T)];
-  if (vec && at + 8 <= D) {
+
+  __device__ __forceinline__ void load(const T* row, int at, int D, bool vec) {
+    if (vec && at + 8 <= D) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
-      const uint4 w = *((const uint4*)(row + at) + i);
-      raw[4 * i] = w.x;
-      raw[4 * i + 1] = w.y;
-      raw[4 * i + 2] = w.z;
-      raw[4 * i + 3] = w.w;
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) *((uint4*)raw + i) = *((const uint4*)(row + at) + i);
+    } else {
+      T* v = (T*)raw;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = at + i < D ? row[at + i] : from_f32<T>(0.0f);
     }
-  } else {
-    T* v = (T*)raw;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = at + i < D ? row[at + i] : from_f32<T>(0.0f);
   }
+
+  __device__ __forceinline__ float at(int i) const { return to_f32(((const T*)raw)[i]); }
+
+  // The largest finite magnitude.
+  __device__ __forceinline__ float most() const {
+    float m = 0.0f;
 #pragma unroll
-  for (int p = 0; p < P; ++p) {
-    uint32_t bits[8];  // in the upper half
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, isfinite(at(i)) ? fabsf(at(i)) : 0.0f);
+    return m;
+  }
+
+  // The pairs (i, i + 4) that a word of weights unpacks to (f32: times up.x * up.y).
+  __device__ __forceinline__ void fragments(float2 up, uint4 (&f)[pieces<T>]) const {
+    if constexpr (sizeof(T) == 2) {
+      f[0] = make_uint4(__byte_perm(raw[0], raw[2], 0x5410), __byte_perm(raw[0], raw[2], 0x7632),
+                        __byte_perm(raw[1], raw[3], 0x5410), __byte_perm(raw[1], raw[3], 0x7632));
+    } else {
+      float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if constexpr (P == 1) {
-        bits[i] = i & 1 ? raw[i / 2] : raw[i / 2] << 16;
-      } else {
-        bits[i] = raw[i];
-        // an infinity or a NaN is in the first piece (with a bit in its upper half)
-        const bool whole = (raw[i] & 0x7f800000u) == 0x7f800000u;
-        if (whole && (raw[i] & 0x7fffffu)) bits[i] |= 0x400000u;
-        raw[i] = whole ? 0u : fbits(bitsf(raw[i]) - bitsf(raw[i] & 0xffff0000u));
+      for (int i = 0; i < 8; ++i) v[i] = at(i) * up.x * up.y;
+#pragma unroll
+      for (int p = 0; p < pieces<T>; ++p) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const __half lo = __float2half_rn(v[i]), hi = __float2half_rn(v[i + 4]);
+          w[i] = (uint32_t)__half_as_ushort(lo) | (uint32_t)__half_as_ushort(hi) << 16;
+          // an infinity or a NaN is in the first of two
+          v[i] = isfinite(v[i]) ? v[i] - __half2float(lo) : 0.0f;
+          v[i + 4] = isfinite(v[i + 4]) ? v[i + 4] - __half2float(hi) : 0.0f;
+        }
+        f[p] = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
-    f[p] = make_uint4(__byte_perm(bits[0], bits[4], 0x7632), __byte_perm(bits[1], bits[5], 0x7632),
-                      __byte_perm(bits[2], bits[6], 0x7632), __byte_perm(bits[3], bits[7], 0x7632));
   }
+};
+
+// The row's power of two as a product of two f32, and its inverse.
+template <typename T>
+__device__ __forceinline__ float2 row_scale(float most, bool inverse) {
+  if (sizeof(T) == 2 || most == 0.0f) return make_float2(1.0f, 1.0f);
+  const int e = inverse ? ilogbf(most) - 14 : 14 - ilogbf(most), a = e / 2;
+  return make_float2(bitsf((uint32_t)(a + 127) << 23), bitsf((uint32_t)(e - a + 127) << 23));
 }
 
-// Nibbles i and i + 4 of a word as two 16-bit floats q: the nibble becomes the mantissa's low end of 128 (bf16) or
-// 1024 (f16), and 8 more than that is taken off, exactly.
-template <bool F16>
-__device__ __forceinline__ uint32_t unpack(uint32_t word, int i) {
+// Nibbles i and i + 4 of a word as two 16-bit floats q: a nibble becomes the mantissa's low end of 128 (bf16) or 1024
+// (f16), and 8 more than that is taken off, exactly.  In f16 16 times a nibble does as well, which takes no shift.
+__device__ __forceinline__ uint32_t masked(uint32_t word, uint32_t mask, uint32_t upper) {
   uint32_t v;
-  asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xea;" : "=r"(v) : "r"(word >> (4 * i)), "r"(F16 ? 0x64006400u : 0x43004300u));
-  if constexpr (F16) {
-    const __half2 r = __hsub2(*(__half2*)&v, __half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408)));
-    return *(const uint32_t*)&r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(word), "r"(mask), "r"(upper));
+  return v;
+}
+template <bool BF16>
+__device__ __forceinline__ void unpack(uint32_t word, uint32_t (&q)[4]) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 low = __nv_bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308));  // 136
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t v = masked(word >> (4 * i), 0x000f000fu, 0x43004300u);
+      const __nv_bfloat162 r = __hsub2(*(const __nv_bfloat162*)&v, low);
+      q[i] = *(const uint32_t*)&r;
+    }
   } else {
-    const __nv_bfloat162 r =
-        __hsub2(*(__nv_bfloat162*)&v, __nv_bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308)));
-    return *(const uint32_t*)&r;
+    const __half2 low = __half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408));   // 1032
+    const __half2 part = __half2(__ushort_as_half(0x2c00), __ushort_as_half(0x2c00));  // 1 / 16
+    const __half2 high = __half2(__ushort_as_half(0xd480), __ushort_as_half(0xd480));  // -72
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t v = masked(i < 2 ? word : word >> 8, i & 1 ? 0x00f000f0u : 0x000f000fu, 0x64006400u);
+      const __half2 x = *(const __half2*)&v, r = i & 1 ? __hfma2(x, part, high) : __hsub2(x, low);
+      q[i] = *(const uint32_t*)&r;
+    }
   }
 }
 
 // c (+)= A B over 16 of K.
-template <bool F16, bool ADD>
+template <bool BF16, bool ADD>
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   const float z0 = ADD ? c[0] : 0.0f, z1 = ADD ? c[1] : 0.0f, z2 = ADD ? c[2] : 0.0f, z3 = ADD ? c[3] : 0.0f;
-  if constexpr (F16)
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+  if constexpr (BF16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
         "{%10, %11, %12, %13};"
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(z0), "f"(z1), "f"(z2), "f"(z3));
   else
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
         "{%10, %11, %12, %13};"
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(z0), "f"(z1), "f"(z2), "f"(z3));
@@ -426,7 +469,7 @@ struct Weights {
 constexpr int STACK = 4;  // tiles of a warp, one above the other: x's fragments of a block serve them all
 
 // Warps that multiply: their registers hold a stack's sums and next weights and the fragments of a block of x.
-__host__ __device__ constexpr int few_warps(int pieces) { return pieces == 1 ? 16 : 12; }
+constexpr int FEW_WARPS = 16;
 
 // Barriers 1 to 7 and 8 to 14 of a block, one for each slot.
 constexpr int MOST_SLOTS = 7;
@@ -442,10 +485,11 @@ __device__ __forceinline__ void named_arrive(int id, int threads) {
 // their order.  x is laid out in shared memory once, while the first weights are on their way; a tile's weights are
 // loaded a block ahead.
 template <typename T, int GROUP>
-__global__ void __launch_bounds__(few_warps(sizeof(T) == 4 ? 3 : 1) * 32, 1) q4_logits_kernel(const LogitArgs a) {
-  constexpr bool F16 = std::is_same<T, __half>::value;
-  constexpr int P = sizeof(T) == 4 ? 3 : 1, WARPS = few_warps(P);
+__global__ void __launch_bounds__(FEW_WARPS * 32, 1) q4_logits_kernel(const LogitArgs a) {
+  constexpr bool BF16 = in_bf16<T>;
+  constexpr int P = pieces<T>, WARPS = FEW_WARPS;
   extern __shared__ uint4 xs[];
+  __shared__ float most[8];  // of each row of x
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int kw = a.k_warps, slots = WARPS / kw, part = warp % kw, slot = warp / kw;
   const int columns = a.rows, per_block = 16 * P * columns;  // 16-byte fragments of a block of x
@@ -490,10 +534,28 @@ __global__ void __launch_bounds__(few_warps(sizeof(T) == 4 ? 3 : 1) * 32, 1) q4_
   for (int i = 0; i < STACK; ++i) load(i);
   advance();
 
+  if (sizeof(T) == 4) {
+    if (threadIdx.x < 8) most[threadIdx.x] = 0.0f;
+    __syncthreads();
+    for (int c = 0; c < columns; ++c) {
+      float m = 0.0f;
+      for (int e = threadIdx.x; e < a.blocks * 16; e += WARPS * 32) {
+        EightX<T> v;
+        v.load((const T*)a.x + c * a.x_ld, 8 * e, a.D, a.x_vec);
+        m = fmaxf(m, v.most());
+      }
+      m = warp_reduce_fmax(m);
+      if (lane == 0) atomicMax((int*)&most[c], __float_as_int(m));  // (not negative)
+    }
+    __syncthreads();
+  }
   for (int c = 0; c < columns; ++c) {
+    const float2 up = row_scale<T>(sizeof(T) == 4 ? most[c] : 0.0f, false);
     for (int e = threadIdx.x; e < a.blocks * 16; e += WARPS * 32) {
+      EightX<T> v;
       uint4 f[P];
-      fragments_of((const T*)a.x + c * a.x_ld, 8 * e, a.D, a.x_vec, f);  // block, j, t
+      v.load((const T*)a.x + c * a.x_ld, 8 * e, a.D, a.x_vec);  // block, j, t
+      v.fragments(up, f);
 #pragma unroll
       for (int p = 0; p < P; ++p) xs[((e >> 2) * P + p) * columns * 4 + c * 4 + (e & 3)] = f[p];
     }
@@ -522,22 +584,17 @@ __global__ void __launch_bounds__(few_warps(sizeof(T) == 4 ? 3 : 1) * 32, 1) q4_
 #pragma unroll
           for (int jj = 0; jj < GROUP / 32; ++jj) {
             const int j = gr * (GROUP / 32) + jj;
-            uint32_t fa[2][4];
-            const uint32_t w0 = ((const uint32_t*)&w.w[0])[j], w1 = ((const uint32_t*)&w.w[1])[j];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              fa[h][0] = unpack<F16>(w0, 2 * h);
-              fa[h][1] = unpack<F16>(w1, 2 * h);
-              fa[h][2] = unpack<F16>(w0, 2 * h + 1);
-              fa[h][3] = unpack<F16>(w1, 2 * h + 1);
-            }
+            uint32_t q0[4], q1[4];
+            unpack<BF16>(((const uint32_t*)&w.w[0])[j], q0);
+            unpack<BF16>(((const uint32_t*)&w.w[1])[j], q1);
+            const uint32_t fa[2][4] = {{q0[0], q1[0], q0[1], q1[1]}, {q0[2], q1[2], q0[3], q1[3]}};
 #pragma unroll
             for (int p = 0; p < P; ++p) {
               if (jj == 0 && p == 0)
-                mma<F16, false>(sum, fa[0], f[j][p].x, f[j][p].y);
+                mma<BF16, false>(sum, fa[0], f[j][p].x, f[j][p].y);
               else
-                mma<F16, true>(sum, fa[0], f[j][p].x, f[j][p].y);
-              mma<F16, true>(sum, fa[1], f[j][p].z, f[j][p].w);
+                mma<BF16, true>(sum, fa[0], f[j][p].x, f[j][p].y);
+              mma<BF16, true>(sum, fa[1], f[j][p].z, f[j][p].w);
             }
           }
           const float s0 = w.scale(0, gr), s1 = w.scale(1, gr);
@@ -569,10 +626,13 @@ __global__ void __launch_bounds__(few_warps(sizeof(T) == 4 ? 3 : 1) * 32, 1) q4_
       }
     }
     if (part || stack >= a.stacks) continue;
+    float2 down[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) down[e] = row_scale<T>(sizeof(T) == 4 && 2 * t + e < a.rows ? most[2 * t + e] : 0.0f, true);
 #pragma unroll
     for (int e = 0; e < STACK * 4; ++e) {
       const int c = 2 * t + (e & 1), v = (stack * STACK + (e >> 2)) * ROWS + 8 * (e >> 1 & 1) + g;
-      if (c < a.rows && v < a.V) store_logit(a, c, v, acc[e >> 2][e & 3]);
+      if (c < a.rows && v < a.V) store_logit(a, c, v, acc[e >> 2][e & 3] * down[e & 1].x * down[e & 1].y);
     }
   }
 }
@@ -584,20 +644,41 @@ __global__ void __launch_bounds__(few_warps(sizeof(T) == 4 ? 3 : 1) * 32, 1) q4_
 // for all rows of x.  So the weights pass through shared memory once, in 4 bits.
 
 // x as the products' second operand, [blocks][2][pieces][columns][128 bytes]: half a block's 64 columns in the order
-// that words of weights unpack in, 16-byte chunks exchanged as 128-byte swizzled atoms hold them.
+// that words of weights unpack in, 16-byte chunks exchanged as 128-byte swizzled atoms hold them; behind it (f32) the
+// rows' inverse powers of two.  A block a row.
 template <typename T>
 __global__ void __launch_bounds__(256) q4_operand_kernel(const LogitArgs a, int columns) {
   pesti_umma::depend_wait();
   pesti_umma::depend_launch();
-  constexpr int P = sizeof(T) == 4 ? 3 : 1;
-  const int b = blockIdx.x;
-  for (int e = threadIdx.x; e < 16 * columns; e += 256) {
-    const int c = e & 7, h = e >> 3 & 1, n = e >> 4;
+  constexpr int P = pieces<T>;
+  __shared__ float scratch[33];
+  const int n = blockIdx.x, chunks = a.blocks * 16;
+  const T* row = (const T*)a.x + n * a.x_ld;
+  const bool there = n < a.rows;
+  float most = 0.0f;
+  if (sizeof(T) == 4 && there) {
+    for (int e = threadIdx.x; e < chunks; e += 256) {
+      EightX<T> v;
+      v.load(row, 8 * e, a.D, a.x_vec);
+      most = fmaxf(most, v.most());
+    }
+  }
+  if (sizeof(T) == 4) most = block_reduce_max(most, scratch);
+  const float2 up = row_scale<T>(most, false);
+  for (int e = threadIdx.x; e < chunks; e += 256) {
+    EightX<T> v;
     uint4 f[P] = {};
-    if (n < a.rows) fragments_of((const T*)a.x + n * a.x_ld, b * BLOCK + 8 * (8 * h + c), a.D, a.x_vec, f);
+    if (there) {
+      v.load(row, 8 * e, a.D, a.x_vec);
+      v.fragments(up, f);
+    }
 #pragma unroll
     for (int p = 0; p < P; ++p)
-      a.operand[((long long)((b * 2 + h) * P + p) * columns + n) * 8 + (c ^ (n & 7))] = f[p];
+      a.operand[((long long)((e >> 3) * P + p) * columns + n) * 8 + ((e & 7) ^ (n & 7))] = f[p];
+  }
+  if (sizeof(T) == 4 && threadIdx.x == 0) {
+    const float2 down = row_scale<T>(most, true);
+    ((float2*)(a.operand + (long long)chunks * P * columns))[n] = down;
   }
 }
 
@@ -613,12 +694,10 @@ __device__ __forceinline__ uint32_t d_column(int slot, int buf) { return slot * 
 // Warps 0 to 7 unpack (four a slot, a quarter of the rows each), 8 to 15 add up, 16 copies, 17 and 18 issue a slot's
 // products.  Issuing is what the rest waits for (a commit takes as long as ten products of 64 rows), so that a block's
 // buffers are handed back by the warps that see its last sums, and only sums are committed.
-template <typename T, int GROUP, int COLUMNS>
+template <bool BF16, int P, int GROUP, int COLUMNS>
 __global__ void __launch_bounds__(WIDE_THREADS, 1)
     q4_wide_kernel(const __grid_constant__ CUtensorMap weights, const LogitArgs a) {
   using namespace pesti_umma;
-  constexpr bool F16 = std::is_same<T, __half>::value;
-  constexpr int P = sizeof(T) == 4 ? 3 : 1;
   constexpr uint32_t x_half = COLUMNS * 128, x_bytes = 2 * P * x_half, stage = SLOTS * WIDE_BYTES + x_bytes;
   extern __shared__ char raw[];
   const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
@@ -681,9 +760,10 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
           uint32_t v[32];
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
-            const uint32_t word = ((const uint32_t*)&w[c & 3])[2 * h + (c >> 2)];
+            uint32_t q[4];
+            unpack<BF16>(((const uint32_t*)&w[c & 3])[2 * h + (c >> 2)], q);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[4 * c + i] = unpack<F16>(word, i);
+            for (int i = 0; i < 4; ++i) v[4 * c + i] = q[i];
           }
           if (h == 0) {
             if (!(ok = bar_wait(a_empty + 8 * (2 * slot + buf), buf_ph ^ 1))) break;
@@ -782,9 +862,13 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
         }
       }
       if (v < a.V) {
+        const float2* down = (const float2*)((const char*)a.operand + (long long)a.blocks * x_bytes);
 #pragma unroll
-        for (int c = 0; c < COLUMNS; ++c)
-          if (c < a.rows) store_logit(a, c, v, ok ? acc[c] : NAN);  // NaN: a wait gave up
+        for (int c = 0; c < COLUMNS; ++c) {
+          if (c >= a.rows) continue;
+          const float y = P == 1 ? acc[c] : acc[c] * down[c].x * down[c].y;
+          store_logit(a, c, v, ok ? y : NAN);  // NaN: a wait gave up
+        }
       }
     }
   } else if (warp == 8 * SLOTS) {  // copies
@@ -820,7 +904,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
         for (int i = 0; i < a.stages; ++i) bar_wait(full + 8 * i, ph);  // copies in flight
     }
   } else {  // issues a slot's products; the warp runs through as one, so that addresses are uniform
-    constexpr uint32_t desc = mma_desc(!F16, false, false, WIDE, COLUMNS);
+    constexpr uint32_t desc = mma_desc(BF16, false, false, WIDE, COLUMNS);
     const int slot = __shfl_sync(PESTI_FULL_MASK, warp, 0) - (8 * SLOTS + 1);
     int s = 0, ph = 0, abuf = 0, a_ph = 0, dbuf = 0, d_ph = 0;
     bool ok = true;

@@ -232,8 +232,9 @@ def _logits_workspace(dtype: int, B: int, D: int) -> int:
 def head_logits(x, held: QuantizedHead, dtype=None, out=None, stream=None):
     """pesti_q4_logits: x [B, D] times the held weight, [B, V] logits.
 
-    x: float32, bfloat16 or float16 (rows may be strided); products are exact and
-    summed in float32, times the scales in float32.  dtype: the logits' type
+    x: float32, bfloat16 or float16 (rows may be strided); products are
+    summed in float32, times the scales in float32 (pesti_sampler.h says how x
+    enters them).  dtype: the logits' type
     (None: x's), or out: the [B, V] tensor to fill (rows may be strided).  Made
     for the few rows of a decode step: the weight is read once for every 64 rows
     of x."""
