@@ -177,9 +177,9 @@ int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o
                 cudaStream_t st) {
   auto kernel = head_gemm_kernel<CG, BF16, A_MN, B_MN, E>;
   static PestiShared shared;
-  const int rc = pesti_allow_shared(shared, kernel, dev.index, smem_bytes(CG), "head_gemm_kernel shared memory");
+  const int rc = pesti_allow_shared(shared, kernel, dev.index, smem_bytes(CG, E), "head_gemm_kernel shared memory");
   if (rc) return rc;
-  return launch("head_gemm_kernel launch", kernel, CG, dev.sms / CG * CG, THREADS, smem_bytes(CG), st, a, b, out, g);
+  return launch("head_gemm_kernel launch", kernel, CG, dev.sms / CG * CG, THREADS, smem_bytes(CG, E), st, a, b, out, g);
 }
 
 RowArgs row_args(const Call& c, const Layout& l, int cg, int sms) {
@@ -289,18 +289,7 @@ int backward(const Call& c, const Layout& l, RowArgs r, void* dh, int64_t dh_ld,
     g.out_y = (int)l.rows_pad;
     rc = launch_gemm<CG, BF16, false, false, GRAD>(rows_k, head_k, grad_out, g, dev, st);
     if (rc) return rc;
-    if (dw) {  // dW = G^T h
-      g = gemm_args(l);
-      g.m_tiles = (int)((width + 128 * CG - 1) / (128 * CG));
-      g.n_tiles = d_tiles;
-      g.k_iters = -1;
-      g.v0 = (int)v0;
-      g.out_x = (int)c.D;
-      g.out_y = (int)c.V;
-      rc = launch_gemm<CG, BF16, true, true, OUT16>(grad_mn, rows_mn, out_w, g, dev, st);
-      if (rc) return rc;
-    }
-    if (dh) {  // dh += G W
+    if (dh) {  // dh += G W, first: this piece of the head is in L2 yet
       g = gemm_args(l);
       g.m_tiles = -1;
       g.a_box = a_box(c.N);
@@ -311,6 +300,17 @@ int backward(const Call& c, const Layout& l, RowArgs r, void* dh, int64_t dh_ld,
       g.out_x = (int)c.D;
       g.out_y = INT_MAX;
       rc = launch_gemm<CG, BF16, false, true, PART32>(grad_k, head_mn, out_h, g, dev, st);
+      if (rc) return rc;
+    }
+    if (dw) {  // dW = G^T h
+      g = gemm_args(l);
+      g.m_tiles = (int)((width + 128 * CG - 1) / (128 * CG));
+      g.n_tiles = d_tiles;
+      g.k_iters = -1;
+      g.v0 = (int)v0;
+      g.out_x = (int)c.D;
+      g.out_y = (int)c.V;
+      rc = launch_gemm<CG, BF16, true, true, OUT16>(grad_mn, rows_mn, out_w, g, dev, st);
       if (rc) return rc;
     }
   }

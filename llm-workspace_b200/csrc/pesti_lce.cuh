@@ -32,10 +32,6 @@ constexpr int PART_K = 16;
 constexpr float LOG2E = 1.44269504f;
 
 __host__ __device__ constexpr int b_bytes(int cg) { return BN / cg * BK * 2; }
-__host__ __device__ constexpr int stages(int cg) { return cg == 1 ? 4 : 6; }
-__host__ __device__ constexpr int smem_bytes(int cg) {
-  return 1024 + stages(cg) * (A_BYTES + b_bytes(cg)) + EPI_WARPS * OUT_BYTES + 256;
-}
 
 // What the host does not know: written by the plan kernel, on the device.
 struct Plan {
@@ -51,6 +47,15 @@ struct RowCoef {
 };
 
 enum Epilogue { STATS, GRAD, OUT16, PART32 };
+
+// Stages in shared memory, beside what is on its way out.
+__host__ __device__ constexpr int out_bytes(Epilogue e) { return e == STATS ? 4096 : EPI_WARPS * 2 * OUT_BYTES; }
+__host__ __device__ constexpr int stages(int cg, Epilogue e) {
+  return (230000 - out_bytes(e)) / (A_BYTES + b_bytes(cg));
+}
+__host__ __device__ constexpr int smem_bytes(int cg, Epilogue e) {
+  return 1024 + stages(cg, e) * (A_BYTES + b_bytes(cg)) + out_bytes(e) + 256;
+}
 
 struct GemmArgs {
   Plan* plan;
@@ -107,11 +112,11 @@ template <int CG, bool BF16, bool A_MN, bool B_MN, Epilogue E>
 __global__ void __launch_bounds__(THREADS, 1)
     head_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                      const __grid_constant__ CUtensorMap map_out, const GemmArgs g) {
-  constexpr int ST = stages(CG), B_BYTES = b_bytes(CG), STAGE = A_BYTES + B_BYTES, TM = 128 * CG;
+  constexpr int ST = stages(CG, E), B_BYTES = b_bytes(CG), STAGE = A_BYTES + B_BYTES, TM = 128 * CG;
   extern __shared__ char raw[];
   const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
   const uint32_t out0 = base + ST * STAGE;
-  const uint32_t bars = out0 + EPI_WARPS * OUT_BYTES;
+  const uint32_t bars = out0 + out_bytes(E);
   const uint32_t full = bars, empty = bars + 8 * ST, acc_full = empty + 8 * ST, acc_empty = acc_full + 16,
                  given = acc_empty + 16, taken = given + 32;
   __shared__ uint32_t tmem_base;
@@ -261,7 +266,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int shift = (E == GRAD || E == OUT16) ? grad_shift<BF16>(g.plan) : 0;
     const float scale = pow2(E == OUT16 ? -shift : shift);
     const int quarter = warp & 3, half0 = (warp >> 2) * HALF;
-    const uint32_t out = out0 + warp * OUT_BYTES;
+    const uint32_t out = out0 + warp * 2 * OUT_BYTES;  // two boxes
     const uint32_t row_out = out + lane * 128, swz = (lane & 7) << 4;
     const uint32_t acc_empty_to = CG == 1 ? acc_empty : peer_addr(acc_empty, 0);
     int acc = 0, acc_ph = 0, pair_ph = 0;
@@ -285,27 +290,51 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (acc == 0) acc_ph ^= 1;
       };
 
-      // 128 bytes of each of the warp's rows: written swizzled, so that eight lanes write to eight banks' groups
+      // the warp's accumulators, which are free for the next tile but one then
+      uint32_t v[HALF];
+      auto take_acc = [&]() {
+        const uint32_t from = wait_acc();
+#pragma unroll
+        for (int c = 0; c < HALF; c += 32) tmem_load32(from + c, *(uint32_t(*)[32])(v + c));
+        tmem_load_wait();
+        leave_acc();
+      };
+      // 128 bytes of each of the warp's rows in one of two boxes: written swizzled, so that eight lanes write to eight
+      // banks' groups
       auto begin_out = [&]() {
         if (lane == 0) store_wait_read<0>();
         __syncwarp();
       };
-      auto put16 = [&](int chunk, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_out + ((uint32_t)(chunk << 4) ^ swz)), "r"(x),
-                     "r"(y), "r"(z), "r"(w)
+      auto put16 = [&](int box, int chunk, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_out + box * OUT_BYTES +
+                                                                      ((uint32_t)(chunk << 4) ^ swz)),
+                     "r"(x), "r"(y), "r"(z), "r"(w)
                      : "memory");
       };
-      auto end_out = [&](int x, int y, bool add) {
+      auto end_out = [&](int x0, int x1, int y, bool add) {
         fence_smem_async();
         __syncwarp();
         if (lane == 0) {
-          if (y < g.out_y) {
+#pragma unroll
+          for (int box = 0; box < 2; ++box) {
+            const int x = box ? x1 : x0;
+            if (y >= g.out_y || x >= g.out_x) continue;
             if (add)
-              tma_add(&map_out, out, x, y);
+              tma_add(&map_out, out + box * OUT_BYTES, x, y);
             else
-              tma_store(&map_out, out, x, y);
+              tma_store(&map_out, out + box * OUT_BYTES, x, y);
           }
           store_commit();
+        }
+      };
+      auto put_pairs = [&](int c) {  // 32 columns from c, in 16 bits
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            w[i] = pack2<BF16>(__uint_as_float(v[c + 8 * j + 2 * i]), __uint_as_float(v[c + 8 * j + 2 * i + 1]));
+          put16(c / 64, c % 64 / 8 + j, w[0], w[1], w[2], w[3]);
         }
       };
 
@@ -319,11 +348,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           const uint32_t from = wait_acc();
 #pragma unroll
           for (int c = 0; c < HALF; c += 32) {
-            uint32_t v[32];
-            tmem_load32(from + c, v);
+            uint32_t w[32];
+            tmem_load32(from + c, w);
             tmem_load_wait();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) z[c + j] = __uint_as_float(v[j]) + (part ? z[c + j] : 0.0f);
+            for (int j = 0; j < 32; ++j) z[c + j] = __uint_as_float(w[j]) + (part ? z[c + j] : 0.0f);
           }
           leave_acc();
         }
@@ -384,7 +413,6 @@ __global__ void __launch_bounds__(THREADS, 1)
         pair_ph ^= 1;
         if (!ok) atomicExch(&g.plan->failed, 1);
       } else if constexpr (E == GRAD) {
-        const uint32_t from = wait_acc();
         const bool live = row < active;
         RowCoef k = {0.0f, 0.0f, 0.0f, 0.0f};
         int t = -1;
@@ -393,84 +421,51 @@ __global__ void __launch_bounds__(THREADS, 1)
           t = g.target[row] - (g.v0 + col0);
         }
         const float c1 = k.c1 * scale, c2 = k.c2 * scale, c3 = k.c3 * scale;
-#pragma unroll 1
-        for (int c = 0; c < HALF && col0 + c < g.out_x; c += 64) {
-          begin_out();
+        take_acc();
+        begin_out();
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t v[32];
-            tmem_load32(from + c + 32 * h, v);
-            tmem_load_wait();
-            const int at = c + 32 * h;
+        for (int c = 0; c < HALF; c += 32) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float p = ex2(fmaf(__uint_as_float(v[j]), LOG2E, -k.c));
-              v[j] = __float_as_uint(fmaf(c1, p, -c3));
-            }
-            if (__any_sync(PESTI_FULL_MASK, t >= at && t < at + 32)) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (t == at + j) v[j] = __float_as_uint(__uint_as_float(v[j]) - c2);
-            }
-            if (!live) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = 0;
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint32_t w[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                w[i] = pack2<BF16>(__uint_as_float(v[8 * j + 2 * i]), __uint_as_float(v[8 * j + 2 * i + 1]));
-              put16(4 * h + j, w[0], w[1], w[2], w[3]);
-            }
+          for (int j = c; j < c + 32; ++j) {
+            const float p = ex2(fmaf(__uint_as_float(v[j]), LOG2E, -k.c));
+            v[j] = __float_as_uint(fmaf(c1, p, -c3));
           }
-          end_out(col0 + c, warp_row, false);
+          if (__any_sync(PESTI_FULL_MASK, t >= c && t < c + 32)) {
+#pragma unroll
+            for (int j = c; j < c + 32; ++j)
+              if (t == j) v[j] = __float_as_uint(__uint_as_float(v[j]) - c2);
+          }
+          if (!live) {
+#pragma unroll
+            for (int j = c; j < c + 32; ++j) v[j] = 0;
+          }
+          put_pairs(c);
         }
-        leave_acc();
+        end_out(col0, col0 + 64, warp_row, false);
       } else if constexpr (E == OUT16) {
-        const uint32_t from = wait_acc();
-#pragma unroll 1
-        for (int c = 0; c < HALF && col0 + c < g.out_x; c += 64) {
-          begin_out();
+        take_acc();
+        begin_out();
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t v[32];
-            tmem_load32(from + c + 32 * h, v);
-            tmem_load_wait();
+        for (int c = 0; c < HALF; c += 32) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = kn ? __float_as_uint(__uint_as_float(v[j]) * scale) : 0u;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint32_t w[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                w[i] = pack2<BF16>(__uint_as_float(v[8 * j + 2 * i]), __uint_as_float(v[8 * j + 2 * i + 1]));
-              put16(4 * h + j, w[0], w[1], w[2], w[3]);
-            }
-          }
-          end_out(col0 + c, g.v0 + warp_row, false);
+          for (int j = c; j < c + 32; ++j) v[j] = kn ? __float_as_uint(__uint_as_float(v[j]) * scale) : 0u;
+          put_pairs(c);
         }
-        leave_acc();
+        end_out(col0, col0 + 64, g.v0 + warp_row, false);
       } else {
-        const uint32_t from = wait_acc();
+        take_acc();
         if (warp_row < active) {
-#pragma unroll 1
-          for (int c = 0; c < HALF && col0 + c < g.out_x; c += 32) {
+#pragma unroll
+          for (int c = 0; c < HALF; c += 64) {
             begin_out();
-            uint32_t v[32];
-            tmem_load32(from + c, v);
-            tmem_load_wait();
-            if (kn == 0) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = 0;
+            for (int j = 0; j < 16; ++j) {
+              const int i = c + 4 * j;
+              put16(j / 8, j % 8, kn ? v[i] : 0u, kn ? v[i + 1] : 0u, kn ? v[i + 2] : 0u, kn ? v[i + 3] : 0u);
             }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) put16(j, v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-            end_out(col0 + c, split * g.plan->part_rows + warp_row, g.add != 0);
+            end_out(col0 + c, col0 + c + 32, split * g.plan->part_rows + warp_row, g.add != 0);
           }
         }
-        leave_acc();
       }
     }
     if (lane == 0) store_wait_all();
