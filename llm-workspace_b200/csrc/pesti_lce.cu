@@ -99,6 +99,32 @@ Cut cut_of(int64_t N, int64_t V, int64_t D) {
   return c;
 }
 
+constexpr int SMS = 148;  // by which sizes of scratch are chosen
+
+// Pairs of blocks read each operand's tile half as often, which is what large products need (4096 x 128256 x 4096: 12.7
+// ms against 14.7 with single blocks); up to 128 rows the products are bound by reading the head, and a pair's second
+// block would only add empty rows (16 x 152064 x 2048: 142 us against 122).
+int blocks_per_tile(int64_t N) { return N > 128 ? 2 : 1; }
+
+// Columns of the logits' tiles: 256, or fewer where that makes a twentieth fewer columns in whole rounds of tiles over
+// the SMs, with 24 for a tile's own beginning and end.  (594 tiles of 256 columns are five rounds of 148, and so are 732
+// of 208: 16 x 152064 x 2048 125 -> 121 us; 240 instead of 256 for 1024 x 256000 x 2048 saves a fiftieth of the columns
+// and takes that much longer.)
+int tile_width(int64_t N, int64_t V) {
+  const int cg = blocks_per_tile(N), units = SMS / cg;
+  const long long rows = (N + 128 * cg - 1) / (128 * cg);
+  long long best = 0;
+  int at = BN;
+  for (int w = BN; w >= 128; w -= 16) {
+    const long long rounds = (rows * ((V + w - 1) / w) + units - 1) / units, t = rounds * (w + 24) * (w < BN ? 20 : 19);
+    if (!best || t < best) {
+      best = t;
+      at = w;
+    }
+  }
+  return at;
+}
+
 struct Layout {
   Plan* plan;
   int *idx, *packed, *place;
@@ -110,6 +136,7 @@ struct Layout {
   uint16_t* grad;
   float* part32;
   long long rows_pad, ldc, ld32;
+  int width;
   Cut cut;
   long long bytes;
 };
@@ -124,7 +151,7 @@ Layout layout(char* base, int64_t N, int64_t V, int64_t D, bool forward, bool gr
     return p;
   };
   l.rows_pad = up_to(N, 256);
-  l.ldc = up_to(D, 8);
+  l.ldc = up_to(D, 64);  // whole lines of L2
   l.ld32 = up_to(D, 4);
   l.plan = (Plan*)take(sizeof(Plan));
   l.idx = (int*)take(l.rows_pad * 4);
@@ -133,7 +160,8 @@ Layout layout(char* base, int64_t N, int64_t V, int64_t D, bool forward, bool gr
   l.coef = (RowCoef*)take(l.rows_pad * sizeof(RowCoef));
   l.zt = (float*)take(l.rows_pad * 4);
   l.rows = (uint16_t*)take(l.rows_pad * l.ldc * 2);
-  const long long tiles = up_to(V, BN) / BN;
+  l.width = tile_width(N, V);
+  const long long tiles = (V + l.width - 1) / l.width;
   if (forward) {
     l.parts = (float2*)take(tiles * l.rows_pad * 8);
     l.zsum = (float*)take(tiles * l.rows_pad * 4);
@@ -203,7 +231,7 @@ RowArgs row_args(const Call& c, const Layout& l, int cg, int sms) {
   r.rows = l.rows;
   r.ldc = l.ldc;
   r.rows_pad = l.rows_pad;
-  r.tiles = (int)(up_to(c.V, BN) / BN);
+  r.tiles = (int)((c.V + l.width - 1) / l.width);
   r.part32 = l.part32;
   r.ld32 = l.ld32;
   r.k_piece = (int)(l.cut.piece / BK);
@@ -224,11 +252,6 @@ GemmArgs gemm_args(const Layout& l) {
   return g;
 }
 
-// Pairs of blocks read each operand's tile half as often, which is what large products need (4096 x 128256 x 4096: 12.7
-// ms against 14.7 with single blocks); up to 128 rows the products are bound by reading the head, and a pair's second
-// block would only add empty rows (16 x 152064 x 2048: 142 us against 122).
-int blocks_per_tile(int64_t N) { return N > 128 ? 2 : 1; }
-
 // Few rows: only the 32-row boxes that hold some are copied.
 int a_box(int64_t N) { return N > 96 ? 128 : 32; }
 
@@ -237,9 +260,10 @@ template <int CG, bool BF16>
 int forward(const Call& c, const Layout& l, RowArgs r, bool grads, Device dev, cudaStream_t st) {
   CUtensorMap rows, head;
   int rc = pesti_tensor_map(&rows, pesti_map_type(c.dtype), l.rows, c.D, l.rows_pad, l.ldc * 2, 64, a_box(c.N));
-  if (!rc) rc = pesti_tensor_map(&head, pesti_map_type(c.dtype), c.head, c.D, c.V, c.w_ld * 2, 64, 128);
+  if (!rc) rc = pesti_tensor_map(&head, pesti_map_type(c.dtype), c.head, c.D, c.V, c.w_ld * 2, 64, l.width / CG);
   if (rc) return rc;
   GemmArgs g = gemm_args(l);
+  g.width = l.width;
   g.m_tiles = -1;
   g.a_box = a_box(c.N);
   g.n_tiles = r.tiles;
@@ -252,8 +276,10 @@ int forward(const Call& c, const Layout& l, RowArgs r, bool grads, Device dev, c
   if (rc) return rc;
   r.parts = l.parts;
   r.zsum = g.zsum;
-  return launch("lce_join_kernel launch", grads ? lce_join_kernel<true> : lce_join_kernel<false>, 1, (c.N + 7) / 8, 256,
-                0, st, r);
+  const char* what = "lce_join_kernel launch";
+  if (c.N <= 512)
+    return launch(what, grads ? lce_join_kernel<1, true> : lce_join_kernel<1, false>, 1, c.N, 256, 0, st, r);
+  return launch(what, grads ? lce_join_kernel<8, true> : lce_join_kernel<8, false>, 1, (c.N + 7) / 8, 256, 0, st, r);
 }
 
 // Packed rows, plan and coefficients are there.
@@ -263,7 +289,7 @@ int backward(const Call& c, const Layout& l, RowArgs r, void* dh, int64_t dh_ld,
   CUtensorMap rows_k, rows_mn, head_k, head_mn, out_w, out_h;
   int rc = pesti_tensor_map(&rows_k, pesti_map_type(c.dtype), l.rows, c.D, l.rows_pad, l.ldc * 2, 64, a_box(c.N));
   if (!rc) rc = pesti_tensor_map(&rows_mn, pesti_map_type(c.dtype), l.rows, c.D, l.rows_pad, l.ldc * 2, 64, 64);
-  if (!rc) rc = pesti_tensor_map(&head_k, pesti_map_type(c.dtype), c.head, c.D, c.V, c.w_ld * 2, 64, 128);
+  if (!rc) rc = pesti_tensor_map(&head_k, pesti_map_type(c.dtype), c.head, c.D, c.V, c.w_ld * 2, 64, BN / CG);
   if (!rc) rc = pesti_tensor_map(&head_mn, pesti_map_type(c.dtype), c.head, c.D, c.V, c.w_ld * 2, 64, 64);
   if (!rc && dw) rc = pesti_tensor_map(&out_w, pesti_map_type(c.dtype), dw, c.D, c.V, dw_ld * 2, 64, 32);
   if (!rc && dh) rc = pesti_tensor_map(&out_h, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, l.part32, c.D, l.cut.part_room, l.ld32 * 4, 32, 32);
@@ -329,7 +355,9 @@ int backward(const Call& c, const Layout& l, const RowArgs& r, int cg, void* dh,
 
 template <bool BACKWARD>
 int pack(const RowArgs& r, cudaStream_t st) {
-  const int rc = launch("lce_plan_kernel launch", lce_plan_kernel<BACKWARD>, 1, 1, 1024, 0, st, r);
+  const char* what = "lce_pack_kernel launch";
+  if (r.N <= PACK_ROWS) return launch(what, lce_pack_kernel<BACKWARD, true>, 1, r.rows_pad, PACK_ROWS, 0, st, r);
+  const int rc = launch(what, lce_pack_kernel<BACKWARD, false>, 1, 1, PACK_ROWS, 0, st, r);
   return rc ? rc : launch("lce_gather_kernel launch", lce_gather_kernel, 1, r.rows_pad, 256, 0, st, r);
 }
 

@@ -67,7 +67,7 @@ struct GemmArgs {
   int a_box;             // rows of a copy of a K-major A: 128, or 32 where few rows count
   // STATS and GRAD
   const int* target;  // [rows], of the packed rows
-  int v0, V;          // the tiles' first token, and the vocabulary
+  int v0, V;          // GRAD: the tiles' first token; the vocabulary
   float2* parts;      // [tiles, rows_pad] (maximum, sum) of a tile's logits, in powers of two
   float* zsum;        // [tiles, rows_pad] their plain sum, or null
   float* zt;          // [rows] the target's logit
@@ -75,6 +75,7 @@ struct GemmArgs {
   const RowCoef* coef;
   int add;            // PART32: add to what is there
   int out_x, out_y;   // where the output ends
+  int width;          // columns of a tile (STATS: a multiple of 16)
 };
 
 template <bool BF16>
@@ -177,10 +178,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         int m, n, split, k0, kn;
         locate(tile, m, n, split, k0, kn);
         const int row_a = g.a_row0 + m * TM + (int)rank * 128;
+        const int width = E == STATS ? g.width : BN;
         // rows of A that nothing comes of stay what they were in shared memory: they reach no row but their own
         const int boxes = A_MN || g.a_box == 128 ? 1 : max(1, min(4, (active - row_a + 31) / 32));
-        const uint32_t bytes = CG * STAGE - (A_MN || g.a_box == 128 ? 0 : A_BYTES - boxes * (A_BYTES / 4));
-        const int row_b = g.b_row0 + n * BN + (int)rank * (BN / CG);
+        const uint32_t bytes = CG * (A_MN || g.a_box == 128 ? A_BYTES : boxes * (A_BYTES / 4)) + width * BK * 2;
+        const int row_b = g.b_row0 + n * width + (int)rank * (width / CG);
         for (int k = 0; k < kn; ++k) {
           if (!bar_wait(empty + 8 * s, ph ^ 1)) {
             ok = false;
@@ -198,7 +200,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           if constexpr (B_MN) {
             for (int i = 0; i < 4 / CG; ++i) tma_load<CG>(b + i * 8192, &map_b, bar, row_b + 64 * i, kb);
           } else {
-            for (int i = 0; i < 2 / CG; ++i) tma_load<CG>(b + i * A_BYTES, &map_b, bar, kb, row_b + 128 * i);
+            tma_load<CG>(b, &map_b, bar, kb, row_b);  // a block's whole share of the tile
           }
           if (++s == ST) {
             s = 0;
@@ -221,7 +223,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else if (warp == EPI_WARPS + 1) {
     if (rank == 0 && elect_one()) {
-      constexpr uint32_t desc = mma_desc(BF16, A_MN, B_MN, TM, BN);
+      const uint32_t desc = mma_desc(BF16, A_MN, B_MN, TM, E == STATS ? g.width : BN);
       int s = 0, ph = 0, acc = 0, acc_ph = 0;
       bool ok = true;
       for (int tile = first; tile < tiles && ok; tile += step) {
@@ -275,7 +277,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       int m, n, split, k0, kn;
       locate(tile, m, n, split, k0, kn);
       const int warp_row = m * TM + (int)rank * 128 + quarter * 32, row = warp_row + lane;
-      const int col0 = n * BN + half0;
+      const int col0 = n * (E == STATS ? g.width : BN) + half0;
       auto wait_acc = [&]() {
         ok = bar_wait(acc_full + 8 * acc, acc_ph);
         if (!ok) atomicExch(&g.plan->failed, 1);
@@ -340,7 +342,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 
       if constexpr (E == STATS) {
         const bool live = row < active;
-        const int t = live ? g.target[row] - (g.v0 + col0) : -1;
+        const int t = live ? g.target[row] - col0 : -1;
         float z[HALF];
         const int parts = parts_of(kn);
 #pragma unroll 1
@@ -357,7 +359,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           leave_acc();
         }
         float mx = -INFINITY, sum = 0.0f, zs = 0.0f, zt = 0.0f;
-        const int left = g.V - (g.v0 + col0);
+        const int left = min(g.V - col0, g.width - half0);  // columns of this half
 #pragma unroll
         for (int c = 0; c < HALF; c += 32) {
           if (c >= left) continue;
@@ -388,7 +390,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           sum = sum * ex2(mx - ref) + ((a[0] + a[1]) + (a[2] + a[3]));
           mx = now;
         }
-        if (t >= 0 && t < HALF) g.zt[row] = zt;
+        if (t >= 0 && t < min(HALF, left)) g.zt[row] = zt;
         // the tile's other half: its warp hands its sums over in shared memory
         float* other = (float*)(raw + (out0 - smem_addr(raw))) + quarter * 128 + lane;
         if (half0) {
@@ -405,7 +407,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (lane == 0) bar_arrive(taken + 8 * quarter);
           const float now = fmaxf(mx, m2), ref = now == -INFINITY ? 0.0f : now;
           if (live) {
-            const long long at = (long long)((g.v0 + col0) / BN) * g.rows_pad + row;
+            const long long at = (long long)n * g.rows_pad + row;
             g.parts[at] = make_float2(now, sum * ex2(mx - ref) + s2 * ex2(m2 - ref));
             if (g.zsum) g.zsum[at] = zs + z2;
           }
@@ -538,16 +540,40 @@ __device__ __forceinline__ unsigned split_time(const RowArgs& a, int active, int
   return (unsigned)fminf(4e9f, (float)rounds * (float)((a.k_piece + splits - 1) / splits + 16) + (float)splits * part);
 }
 
-// One block: packs the rows that count, in their order.  BACKWARD: their coefficients as well.
-template <bool BACKWARD>
-__global__ void __launch_bounds__(1024) lce_plan_kernel(const RowArgs a) {
+// Packed row i: a row that counts, or zeros behind them to a whole tile.
+__device__ __forceinline__ void put_row(const RowArgs& a, long long i, int active, long long n) {
+  uint16_t* to = (uint16_t*)a.rows + i * a.ldc;
+  if (i >= active) {
+    if (i < (active + 255) / 256 * 256)
+      for (long long d = threadIdx.x * 8; d < a.ldc; d += blockDim.x * 8) *(uint4*)(to + d) = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const uint16_t* from = (const uint16_t*)a.hidden + n * a.h_ld;
+  if (((uintptr_t)from & 15) == 0) {
+    long long d = threadIdx.x * 8;
+    for (; d + 8 <= a.D; d += blockDim.x * 8) *(uint4*)(to + d) = *(const uint4*)(from + d);
+    if (d < a.D)
+      for (long long e = d; e < a.D; ++e) to[e] = from[e];
+  } else {
+    for (long long d = threadIdx.x; d < a.D; d += blockDim.x) to[d] = from[d];
+  }
+}
+
+constexpr int PACK_ROWS = 1024;  // that a block counts through for each row it copies
+
+// Packs the rows that count, in their order (BACKWARD: with their coefficients).  COPY: a block for each packed row,
+// which counts for itself and then copies it; the first one writes the rest.  Otherwise one block, and
+// lce_gather_kernel copies.
+template <bool BACKWARD, bool COPY>
+__global__ void __launch_bounds__(PACK_ROWS) lce_pack_kernel(const RowArgs a) {
   depend_wait();
   depend_launch();
-  __shared__ int scratch[33];
+  __shared__ int scratch[33], mine;
   __shared__ unsigned most[33];
+  const bool writes = !COPY || blockIdx.x == 0;
   int before = 0;
   unsigned bound = 0;
-  for (long long n0 = 0; n0 < a.N; n0 += 1024) {
+  for (long long n0 = 0; n0 < a.N; n0 += PACK_ROWS) {
     const long long n = n0 + threadIdx.x;
     long long t = -1;
     float w = 1.0f;
@@ -558,7 +584,7 @@ __global__ void __launch_bounds__(1024) lce_plan_kernel(const RowArgs a) {
     const bool live = t >= 0 && t < a.V && w != 0.0f;
     int total;
     const int at = before + block_excl_scan_add<int>(live ? 1 : 0, scratch, total);
-    if (n < a.N) {
+    if (writes && n < a.N) {
       a.place[n] = live ? at : -1;
       if (!BACKWARD && !live) {
         a.loss[n] = 0.0f;
@@ -566,16 +592,24 @@ __global__ void __launch_bounds__(1024) lce_plan_kernel(const RowArgs a) {
       }
     }
     if (live) {
-      a.idx[at] = (int)n;
-      a.packed[at] = (int)t;
-      if (BACKWARD) {
-        const RowCoef k = coef_of(a, w * a.up[n * a.up_stride], a.lse_in[n]);
-        a.coef[at] = k;
-        bound = max(bound, bound_of(k));
+      if (COPY && at == blockIdx.x) mine = (int)n;
+      if (writes) {
+        a.idx[at] = (int)n;
+        a.packed[at] = (int)t;
+        if (BACKWARD) {
+          const RowCoef k = coef_of(a, w * a.up[n * a.up_stride], a.lse_in[n]);
+          a.coef[at] = k;
+          bound = max(bound, bound_of(k));
+        }
       }
     }
     before += total;
   }
+  if (COPY) {
+    __syncthreads();
+    put_row(a, blockIdx.x, before, mine);
+  }
+  if (!writes) return;
   if (BACKWARD) bound = block_reduce_max<unsigned>(bound, most);
   if (threadIdx.x < 32 && a.part_room) {
     unsigned best = split_time(a, before, threadIdx.x + 1, a.tile_rows, a.units), at = threadIdx.x + 1;
@@ -598,40 +632,25 @@ __global__ void __launch_bounds__(1024) lce_plan_kernel(const RowArgs a) {
   }
 }
 
-// The packed rows, behind them zeros to a whole tile.
 __global__ void __launch_bounds__(256) lce_gather_kernel(const RowArgs a) {
   depend_wait();
   depend_launch();
-  const int active = a.plan->active, tile_end = (active + 255) / 256 * 256;
-  const long long i = blockIdx.x;
-  if (i >= tile_end) return;
-  uint16_t* to = (uint16_t*)a.rows + i * a.ldc;
-  if (i >= active) {
-    for (long long d = threadIdx.x * 8; d < a.ldc; d += 2048) *(uint4*)(to + d) = make_uint4(0, 0, 0, 0);
-    return;
-  }
-  const uint16_t* from = (const uint16_t*)a.hidden + (long long)a.idx[i] * a.h_ld;
-  if (((uintptr_t)from & 15) == 0) {
-    long long d = threadIdx.x * 8;
-    for (; d + 8 <= a.D; d += 2048) *(uint4*)(to + d) = *(const uint4*)(from + d);
-    for (; d < a.D && d + 8 > a.D; d += 2048)
-      for (long long e = d; e < a.D; ++e) to[e] = from[e];
-  } else {
-    for (long long d = threadIdx.x; d < a.D; d += 256) to[d] = from[d];
-  }
+  const int active = a.plan->active;
+  put_row(a, blockIdx.x, active, blockIdx.x < active ? a.idx[blockIdx.x] : 0);
 }
 
-// A row's tiles joined: 8 rows a block, 32 threads a row.  GRADS: the coefficients of its gradient too (up = 1).
-template <bool GRADS>
+// A row's tiles joined: ROWS rows a block (8 share what is read; 1 where there are few).  GRADS: the coefficients of its
+// gradient too (up = 1).
+template <int ROWS, bool GRADS>
 __global__ void __launch_bounds__(256) lce_join_kernel(const RowArgs a) {
-  __shared__ float sm[8][8];
-  __shared__ double ss[8][8], sz[8][8];
+  __shared__ float sm[8][ROWS];
+  __shared__ double ss[8][ROWS], sz[8][ROWS];
   depend_wait();
   depend_launch();
-  const int r = threadIdx.x & 7, part = threadIdx.x >> 3, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = threadIdx.x % ROWS, part = threadIdx.x / ROWS, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int active = a.plan->active;
-  const long long i = (long long)blockIdx.x * 8 + r;
-  if ((long long)blockIdx.x * 8 >= active) return;
+  const long long i = (long long)blockIdx.x * ROWS + r;
+  if ((long long)blockIdx.x * ROWS >= active) return;
   float m = -INFINITY;
   double s = 0.0, z = 0.0;
   auto join = [&](float m2, double s2) {
@@ -640,26 +659,26 @@ __global__ void __launch_bounds__(256) lce_join_kernel(const RowArgs a) {
     m = most;
   };
   if (i < active) {
-    for (int t = part; t < a.tiles; t += 32) {
+    for (int t = part; t < a.tiles; t += 256 / ROWS) {
       const float2 p = a.parts[(long long)t * a.rows_pad + i];
       join(p.x, p.y);
       if (a.zsum) z += a.zsum[(long long)t * a.rows_pad + i];
     }
   }
 #pragma unroll
-  for (int o = 8; o < 32; o <<= 1) {
+  for (int o = ROWS; o < 32; o <<= 1) {
     const float m2 = __shfl_xor_sync(PESTI_FULL_MASK, m, o);
     const double s2 = __shfl_xor_sync(PESTI_FULL_MASK, s, o);
     z += __shfl_xor_sync(PESTI_FULL_MASK, z, o);
     join(m2, s2);
   }
-  if (lane < 8) {
+  if (lane < ROWS) {
     sm[warp][r] = m;
     ss[warp][r] = s;
     sz[warp][r] = z;
   }
   __syncthreads();
-  if (threadIdx.x >= 8 || i >= active) return;
+  if (threadIdx.x >= ROWS || i >= active) return;
   for (int w = 1; w < 8; ++w) {
     join(sm[w][r], ss[w][r]);
     z += sz[w][r];
@@ -680,7 +699,7 @@ __global__ void __launch_bounds__(256) lce_join_kernel(const RowArgs a) {
 }
 
 // The hidden states' gradient: the parts summed in their order, to the rows' own places; padded rows get zeros.
-// Four columns a thread, four parts at a time in flight.
+// Four columns a thread, eight parts at a time in flight.
 template <bool BF16>
 __global__ void __launch_bounds__(256) lce_finish_kernel(const RowArgs a) {
   depend_wait();
@@ -695,7 +714,7 @@ __global__ void __launch_bounds__(256) lce_finish_kernel(const RowArgs a) {
   for (long long d = threadIdx.x * 4; d < a.D; d += 1024) {
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (i >= 0) {  // (columns of a part are padded to four)
-#pragma unroll 4
+#pragma unroll 8
       for (int s = 0; s < splits; ++s) {
         const float4 x = __ldcs((const float4*)(from + s * part + d));
         v.x += x.x;
