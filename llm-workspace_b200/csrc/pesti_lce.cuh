@@ -266,7 +266,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else {
     const int shift = (E == GRAD || E == OUT16) ? grad_shift<BF16>(g.plan) : 0;
-    const float scale = pow2(E == OUT16 ? -shift : shift);
+    // (a wait that gave up in an earlier kernel makes NaN of what comes out)
+    const float scale = g.plan->failed ? NAN : pow2(E == OUT16 ? -shift : shift);
     const int quarter = warp & 3, half0 = (warp >> 2) * HALF;
     const uint32_t out = out0 + warp * 2 * OUT_BYTES;  // two boxes
     const uint32_t row_out = out + lane * 128, swz = (lane & 7) << 4;

@@ -111,7 +111,8 @@ int convert(bool there, pesti_dtype dtype, int64_t group, const void* w, int64_t
 }
 
 constexpr int MOST_ROWS = 64;            // of x, a pass over the weight
-constexpr int SHARED_BYTES = 200 << 10;  // for x, or for the stages
+constexpr int SHARED_BYTES = 200 << 10;  // for the stages
+constexpr int FEW_BYTES = 196 << 10;     // for few rows of x, beside 30 KB of sums
 
 int pieces_of(pesti_dtype d) { return d == PESTI_F32 ? pieces<float> : 1; }
 
@@ -120,7 +121,7 @@ int columns_of(int64_t rows) { return (int)(rows + 15) / 16 * 16; }
 // Few rows of x that fit shared memory whole.  A column tile of the products by warps holds 8; f32 rows cost them two
 // products (us for 4 / 8 / on tensor memory, 128256 x 4096: 82 / 88 / 89; 32001 x 1000: 12 / 14 / 11).
 bool few(int64_t D, int pieces, int64_t rows) {
-  return rows <= (pieces == 1 ? 8 : 4) && blocks_of(D) * rows * pieces * (BLOCK * 2) <= SHARED_BYTES;
+  return rows <= (pieces == 1 ? 8 : 4) && blocks_of(D) * rows * pieces * (BLOCK * 2) <= FEW_BYTES;
 }
 
 // How a pass with few rows shares its stacks and K out: the least time of the busiest SM, by the weight's bytes that it

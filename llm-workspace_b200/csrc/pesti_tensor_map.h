@@ -3,6 +3,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "../../include/pesti_sampler.h"
 #include "pesti_error.h"
 
@@ -20,7 +22,8 @@ static inline int pesti_tensor_map(CUtensorMap* map, CUtensorMapDataType type, c
   typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-  static Encode encode = nullptr;  // the same value whoever writes it
+  static std::atomic<Encode> found_encode{nullptr};  // the same value whoever writes it
+  Encode encode = found_encode.load(std::memory_order_relaxed);
   if (!encode) {
     void* f = nullptr;
     cudaDriverEntryPointQueryResult found;
@@ -29,6 +32,7 @@ static inline int pesti_tensor_map(CUtensorMap* map, CUtensorMapDataType type, c
     if (found != cudaDriverEntryPointSuccess || !f)
       return pesti_set_error(PESTI_E_UNSUPPORTED, "the driver has no cuTensorMapEncodeTiled");
     encode = (Encode)f;
+    found_encode.store(encode, std::memory_order_relaxed);
   }
   const cuuint64_t dims[2] = {(cuuint64_t)columns, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)row_bytes};
   const cuuint32_t box[2] = {(cuuint32_t)box_columns, (cuuint32_t)box_rows}, ones[2] = {1, 1};

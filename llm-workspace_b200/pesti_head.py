@@ -162,6 +162,14 @@ class QuantizedHead:
     layout (pesti_q4_quantize); scale is tile_scale by rows, [V, ceil(D / group)]."""
 
     def __init__(self, packed, tile_scale, V: int, D: int, group: int):
+        _need(V >= 1 and D >= 1 and group in (32, 64, 128), "V and D must be at least 1, group 32, 64 or 128")
+        tiles = -(-V // _ROWS), -(-D // _BLOCK), _ROWS
+        _need(packed.dtype == torch.uint8 and packed.shape == (*tiles, _BLOCK // 2) and packed.is_contiguous(),
+              "packed must be a contiguous [ceil(V / 16), ceil(D / 128), 16, 64] uint8 tensor")
+        _need(tile_scale.dtype == torch.bfloat16 and tile_scale.shape == (*tiles, _BLOCK // group)
+              and tile_scale.is_contiguous() and tile_scale.device == packed.device,
+              "tile_scale must be a contiguous [ceil(V / 16), ceil(D / 128), 16, 128 / group] bfloat16 tensor on "
+              "packed's device")
         self.packed, self.tile_scale, self.V, self.D, self.group = packed, tile_scale, int(V), int(D), int(group)
 
     @property
@@ -237,7 +245,7 @@ def head_logits(x, held: QuantizedHead, dtype=None, out=None, stream=None):
     enters them).  dtype: the logits' type
     (None: x's), or out: the [B, V] tensor to fill (rows may be strided).  Made
     for the few rows of a decode step: the weight is read once for every 64 rows
-    of x."""
+    of x, and no gradient reaches it."""
     _need(x.dim() == 2 and x.dtype in _DTYPES, "x must be a [B, D] float32, bfloat16 or float16 tensor")
     (B, D), dev = x.shape, x.device
     _need(D == held.D, "x and the held weight have different D")

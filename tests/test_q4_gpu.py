@@ -144,6 +144,15 @@ def test_rounds(B, V):
     _check_logits(x, held, want, torch.float32)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("B,D", [(8, 12544), (8, 12545), (4, 12544), (4, 12673), (1, 100_352), (1, 100_353), (3, 70_000)])
+def test_long_rows(dtype, B, D):
+    """x at, and just above, what is held in shared memory."""
+    held, want = _check_held(_weight(40, D, "bf16"), 128)
+    x = torch.randn(B, D, generator=torch.Generator().manual_seed(D)).to(DT[dtype]).cuda()
+    _check_logits(x, held, want, torch.float32)
+
+
 @pytest.mark.parametrize("B", [1, 5, 64])
 def test_wide_values_of_x(B):
     """f32 rows of all magnitudes, f16 subnormals, bf16 extremes, infinities and NaN."""
