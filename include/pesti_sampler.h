@@ -559,9 +559,12 @@ int pesti_linear_ce_backward(const void* d_hidden, pesti_dtype dtype, int64_t N,
  * (exact in F32, else rounded once).  Buffers do not overlap (refused).
  * pesti_q4_logits: d_logits [B, ld] (first V columns; F32, BF16 or F16) = x
  * [B, x_ld] (first D columns; F32, BF16 or F16) times the held weight.
- * Products with q are exact, summed in f32 over a group and then over the groups
- * with their scales, and rounded once; 16-bit x enters them as it is, F32
- * x within 2^-24 of itself or 2^-39 of its row's largest finite value.  The weight is read once for
+ * Sums are f32.  Up to 8 rows of x (4 of F32): over a group of exact products with
+ * q, then over the groups with their scales.  More rows: of products with q s,
+ * which is exact, over 512 columns (256 for F32 x), then over those; scales below
+ * 2^-25 of the largest of these columns of their row lose bits.  16-bit x enters
+ * as it is (more rows of BF16: down to 2^-39 of their largest finite value), F32 x
+ * within 2^-24 of itself or 2^-39 of its row's largest finite value. The weight is read once for
  * every 64 rows of x.  The logits overlap no input
  * (refused).  d_ws: device scratch of pesti_q4_logits_workspace(...) bytes
  * (0 for few rows: NULL will do), 256-byte aligned, any contents; calls whose GPU work may overlap need scratch

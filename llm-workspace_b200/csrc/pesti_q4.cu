@@ -159,9 +159,9 @@ int launch(const char* what, void (*kernel)(K...), long long blocks, int threads
   return e == cudaSuccess ? PESTI_OK : pesti_set_cuda_error(e, what);
 }
 
-template <bool BF16, int P, int GROUP, int COLUMNS>
+template <int P, int GROUP, int COLUMNS>
 int wide_pass(const LogitArgs& a, Device dev, const CUtensorMap& weights, cudaStream_t st) {
-  const auto kernel = q4_wide_kernel<BF16, P, GROUP, COLUMNS>;
+  const auto kernel = q4_wide_kernel<P, GROUP, COLUMNS>;
   const int smem = 1024 + a.stages * (SLOTS * WIDE_BYTES + COLUMNS * P * (BLOCK * 2));
   static PestiShared shared;
   const int rc = pesti_allow_shared(shared, kernel, dev.index, smem, "q4_wide_kernel shared memory");
@@ -193,10 +193,10 @@ int pass(LogitArgs a, Device dev, cudaStream_t st) {
   if (!rc) rc = launch("q4_operand_kernel launch", q4_operand_kernel<T>, columns, 256, 0, st, a, columns);
   if (rc) return rc;
   a.stages = std::min(8, SHARED_BYTES / (SLOTS * WIDE_BYTES + columns * P * (BLOCK * 2)));
-  if (columns == 16) return wide_pass<in_bf16<T>, P, GROUP, 16>(a, dev, weights, st);
-  if (columns == 32) return wide_pass<in_bf16<T>, P, GROUP, 32>(a, dev, weights, st);
-  if (columns == 48) return wide_pass<in_bf16<T>, P, GROUP, 48>(a, dev, weights, st);
-  return wide_pass<in_bf16<T>, P, GROUP, 64>(a, dev, weights, st);
+  if (columns == 16) return wide_pass<P, GROUP, 16>(a, dev, weights, st);
+  if (columns == 32) return wide_pass<P, GROUP, 32>(a, dev, weights, st);
+  if (columns == 48) return wide_pass<P, GROUP, 48>(a, dev, weights, st);
+  return wide_pass<P, GROUP, 64>(a, dev, weights, st);
 }
 
 template <typename T>

@@ -325,14 +325,17 @@ __device__ __forceinline__ void store_logit(const LogitArgs& a, int row, int v, 
     ((__half*)a.y)[at] = __float2half_rn(y);
 }
 
-// 16-bit x enters the products as it is.  f32 x enters them as a sum of two f16, times a power of two of its row that
-// brings the row's largest finite value to 2^14 or more: off by at most 2^-24 of itself or 2^-39 of that value, which is
-// below what an f32 sum of the products loses.  (Three bf16, exact without a power of two, cost a product more, 97 us
-// instead of 77 for a row of 128256 x 4096.)
+// f32 x enters the products as a sum of two f16, times a power of two of its row that brings the row's largest finite
+// value to 2^14 or more: off by at most 2^-24 of itself or 2^-39 of that value, which is below what an f32 sum of the
+// products loses.  (Three bf16, exact without a power of two, cost a product more, 97 us instead of 77 for a row of
+// 128256 x 4096.)  16-bit x enters them as it is, or (IN_F16) bf16 as f16 times such a power: exactly, down to 2^-39 of
+// the row's largest value.
 template <typename T>
 constexpr int pieces = sizeof(T) == 4 ? 2 : 1;
 template <typename T>
 constexpr bool in_bf16 = std::is_same<T, __nv_bfloat16>::value;
+template <typename T, bool IN_F16>
+constexpr bool scaled = sizeof(T) == 4 || (IN_F16 && in_bf16<T>);
 
 // Eight columns of a row of x.
 template <typename T>
@@ -360,9 +363,10 @@ struct EightX {
     return m;
   }
 
-  // The pairs (i, i + 4) that a word of weights unpacks to (f32: times up.x * up.y).
+  // The pairs (i, i + 4) that a word of weights unpacks to (scaled: times up.x * up.y).
+  template <bool IN_F16>
   __device__ __forceinline__ void fragments(float2 up, uint4 (&f)[pieces<T>]) const {
-    if constexpr (sizeof(T) == 2) {
+    if constexpr (!scaled<T, IN_F16>) {
       f[0] = make_uint4(__byte_perm(raw[0], raw[2], 0x5410), __byte_perm(raw[0], raw[2], 0x7632),
                         __byte_perm(raw[1], raw[3], 0x5410), __byte_perm(raw[1], raw[3], 0x7632));
     } else {
@@ -387,9 +391,8 @@ struct EightX {
 };
 
 // The row's power of two as a product of two f32, and its inverse.
-template <typename T>
 __device__ __forceinline__ float2 row_scale(float most, bool inverse) {
-  if (sizeof(T) == 2 || most == 0.0f) return make_float2(1.0f, 1.0f);
+  if (most == 0.0f) return make_float2(1.0f, 1.0f);
   const int e = inverse ? ilogbf(most) - 14 : 14 - ilogbf(most), a = e / 2;
   return make_float2(bitsf((uint32_t)(a + 127) << 23), bitsf((uint32_t)(e - a + 127) << 23));
 }
@@ -550,12 +553,12 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) q4_logits_kernel(const Logi
     __syncthreads();
   }
   for (int c = 0; c < columns; ++c) {
-    const float2 up = row_scale<T>(sizeof(T) == 4 ? most[c] : 0.0f, false);
+    const float2 up = row_scale(sizeof(T) == 4 ? most[c] : 0.0f, false);
     for (int e = threadIdx.x; e < a.blocks * 16; e += WARPS * 32) {
       EightX<T> v;
       uint4 f[P];
       v.load((const T*)a.x + c * a.x_ld, 8 * e, a.D, a.x_vec);  // block, j, t
-      v.fragments(up, f);
+      v.template fragments<false>(up, f);
 #pragma unroll
       for (int p = 0; p < P; ++p) xs[((e >> 2) * P + p) * columns * 4 + c * 4 + (e & 3)] = f[p];
     }
@@ -628,7 +631,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) q4_logits_kernel(const Logi
     if (part || stack >= a.stacks) continue;
     float2 down[2];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) down[e] = row_scale<T>(sizeof(T) == 4 && 2 * t + e < a.rows ? most[2 * t + e] : 0.0f, true);
+    for (int e = 0; e < 2; ++e) down[e] = row_scale(sizeof(T) == 4 && 2 * t + e < a.rows ? most[2 * t + e] : 0.0f, true);
 #pragma unroll
     for (int e = 0; e < STACK * 4; ++e) {
       const int c = 2 * t + (e & 1), v = (stack * STACK + (e >> 2)) * ROWS + 8 * (e >> 1 & 1) + g;
@@ -639,65 +642,109 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) q4_logits_kernel(const Logi
 
 // --- more rows: products on the tensor cores' own memory
 //
-// A product's 128 x 64 operand of weights is unpacked into tensor memory, exactly, as whole numbers; x comes from shared
-// memory; the sums of a group come back, times its scale, into registers, where a thread adds up one row of the weight
-// for all rows of x.  So the weights pass through shared memory once, in 4 bits.
+// A product's 128 x 128 operand of weights is unpacked into tensor memory as q s, which f16 holds exactly: q has three
+// bits beside its sign (or is a power of two) and s eight, once the scales of a part (a few blocks) of a row are brought
+// to the right magnitude by a power of two.  Scales below 2^-25 of a part's largest lose bits, which is 2^-35 of what
+// that one's weights amount to.  x comes from shared memory.  The sums of a part come back times the inverse power, into
+// registers, where a thread adds up one row of the weight for all rows of x.  Tensor memory is read at some 60 bytes a
+// clock and SM: taking each group's sums out, to scale them there, bound 48 rows to 107 us (128256 x 4096).  And parts
+// keep the tensor cores' sums short, which are cut off and not rounded every 16 of K.
+
+// Blocks of a part: 64 products of 16 of K into one sum, off by up to 6e-7 of it then.
+__host__ __device__ constexpr int part_of(int pieces) { return 4 / pieces; }
 
 // x as the products' second operand, [blocks][2][pieces][columns][128 bytes]: half a block's 64 columns in the order
-// that words of weights unpack in, 16-byte chunks exchanged as 128-byte swizzled atoms hold them; behind it (f32) the
-// rows' inverse powers of two.  A block a row.
+// that words of weights unpack in, 16-byte chunks exchanged as 128-byte swizzled atoms hold them; behind it the rows'
+// inverse powers of two.  A block a row.
 template <typename T>
 __global__ void __launch_bounds__(256) q4_operand_kernel(const LogitArgs a, int columns) {
   pesti_umma::depend_wait();
   pesti_umma::depend_launch();
   constexpr int P = pieces<T>;
+  constexpr bool SCALED = scaled<T, true>;
   __shared__ float scratch[33];
   const int n = blockIdx.x, chunks = a.blocks * 16;
   const T* row = (const T*)a.x + n * a.x_ld;
   const bool there = n < a.rows;
   float most = 0.0f;
-  if (sizeof(T) == 4 && there) {
-    for (int e = threadIdx.x; e < chunks; e += 256) {
+  if (SCALED) {
+    for (int e = threadIdx.x; there && e < chunks; e += 256) {
       EightX<T> v;
       v.load(row, 8 * e, a.D, a.x_vec);
       most = fmaxf(most, v.most());
     }
+    most = block_reduce_max(most, scratch);
   }
-  if (sizeof(T) == 4) most = block_reduce_max(most, scratch);
-  const float2 up = row_scale<T>(most, false);
+  const float2 up = row_scale(most, false);
   for (int e = threadIdx.x; e < chunks; e += 256) {
     EightX<T> v;
     uint4 f[P] = {};
     if (there) {
       v.load(row, 8 * e, a.D, a.x_vec);
-      v.fragments(up, f);
+      v.template fragments<true>(up, f);
     }
 #pragma unroll
     for (int p = 0; p < P; ++p)
       a.operand[((long long)((e >> 3) * P + p) * columns + n) * 8 + ((e & 7) ^ (n & 7))] = f[p];
   }
-  if (sizeof(T) == 4 && threadIdx.x == 0) {
-    const float2 down = row_scale<T>(most, true);
-    ((float2*)(a.operand + (long long)chunks * P * columns))[n] = down;
-  }
+  if (threadIdx.x == 0) ((float2*)(a.operand + (long long)chunks * P * columns))[n] = row_scale(most, true);
 }
+
+// A row's scales of a part, as they are held, and the power of two that brings the largest below 2^11 (q s below 2^15).
+template <int GROUP, int PART>
+struct PartScales {
+  uint2 s[PART];  // up to four bf16 a block
+
+  __device__ __forceinline__ void load(const __nv_bfloat16* scales, int b, int blocks) {
+#pragma unroll
+    for (int i = 0; i < PART; ++i) {
+      s[i] = make_uint2(0, 0);
+      if (b + i >= blocks) continue;
+      const __nv_bfloat16* p = scales + (long long)(b + i) * (ROWS * BLOCK / GROUP);
+      if constexpr (GROUP == 32)
+        s[i] = __ldg((const uint2*)p);
+      else if constexpr (GROUP == 64)
+        s[i].x = __ldg((const uint32_t*)p);
+      else
+        s[i].x = __ldg((const uint16_t*)p);
+    }
+  }
+
+  __device__ __forceinline__ float at(int block, int g) const {
+    const uint32_t v = g < 2 ? s[block].x : s[block].y;
+    return bitsf(g & 1 ? v & 0xffff0000u : v << 16);
+  }
+
+  // The exponent of that power.
+  __device__ __forceinline__ int shift() const {
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < PART; ++i)
+#pragma unroll
+      for (int g = 0; g < BLOCK / GROUP; ++g) most = max(most, fbits(at(i, g)) & 0x7fffffffu);
+    const int e = (int)(most >> 23);  // (255: a scale that is NaN, which makes all of the row's sums NaN)
+    return min(126, 127 + 10 - e);
+  }
+};
+
+__device__ __forceinline__ float power(int e) { return bitsf((uint32_t)(e + 127) << 23); }
 
 constexpr int WIDE = 128;                       // rows of the weight, eight tiles
 constexpr int SLOTS = 2;                        // of them at once
 constexpr int WIDE_THREADS = (9 * SLOTS + 1) * 32;
 constexpr int WIDE_BYTES = WIDE * BLOCK_BYTES;  // of a block
 
-// Where a slot's buffers are in tensor memory: two blocks of unpacked weights, and two groups' sums.
+// Where a slot's buffers are in tensor memory: two blocks of unpacked weights, and two parts' sums.
 __device__ __forceinline__ uint32_t a_column(int slot, int buf) { return slot * 256 + buf * 64; }
 __device__ __forceinline__ uint32_t d_column(int slot, int buf) { return slot * 256 + 128 + buf * 64; }
 
 // Warps 0 to 7 unpack (four a slot, a quarter of the rows each), 8 to 15 add up, 16 copies, 17 and 18 issue a slot's
-// products.  Issuing is what the rest waits for (a commit takes as long as ten products of 64 rows), so that a block's
-// buffers are handed back by the warps that see its last sums, and only sums are committed.
-template <bool BF16, int P, int GROUP, int COLUMNS>
+// products.
+template <int P, int GROUP, int COLUMNS>
 __global__ void __launch_bounds__(WIDE_THREADS, 1)
     q4_wide_kernel(const __grid_constant__ CUtensorMap weights, const LogitArgs a) {
   using namespace pesti_umma;
+  constexpr int PART = part_of(P);
   constexpr uint32_t x_half = COLUMNS * 128, x_bytes = 2 * P * x_half, stage = SLOTS * WIDE_BYTES + x_bytes;
   extern __shared__ char raw[];
   const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
@@ -709,11 +756,11 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < a.stages; ++s) {
       bar_init(full + 8 * s, 1);
-      bar_init(empty + 8 * s, 8 * SLOTS);  // read by the warps that unpack, and its products done
+      bar_init(empty + 8 * s, 5 * SLOTS);  // read by the warps that unpack, and its products done
     }
     for (int s = 0; s < 2 * SLOTS; ++s) {
       bar_init(a_full + 8 * s, 4);
-      bar_init(a_empty + 8 * s, 4);
+      bar_init(a_empty + 8 * s, 1);
       bar_init(d_full + 8 * s, 1);
       bar_init(d_empty + 8 * s, 4);
     }
@@ -729,146 +776,115 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
 
   const int per_round = gridDim.x * SLOTS, rounds = (a.stacks + per_round - 1) / per_round;
   auto stack_of = [&](int round, int slot) { return round * per_round + slot * (int)gridDim.x + (int)blockIdx.x; };
+  // the scales of the thread's row in a stack
+  auto scales_of = [&](int stack) {
+    const int v = stack * WIDE + (warp & 3) * 32 + lane;
+    return a.scale + (tile_of(min(v, a.V - 1), a.blocks, 0) * ROWS + (v & 15)) * (BLOCK / GROUP);
+  };
 
-  // 96 registers a thread at the start; eight warps' 24 go to eight others
   if (warp < 4 * SLOTS) {  // unpacks
-    give_registers<72>();
     const int slot = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t quarter = (uint32_t)(warp & 3) << 21;
     int s = 0, ph = 0, buf = 0, buf_ph = 0;
     bool ok = true;
     for (int r = 0; r < rounds && ok; ++r) {
       const bool there = stack_of(r, slot) < a.stacks;
-      for (int b = 0; b < a.blocks && ok; ++b) {
-        if (!(ok = bar_wait(full + 8 * s, ph))) break;
-        uint4 w[4];
-        const uint32_t at = base + s * stage + slot * WIDE_BYTES + row * BLOCK_BYTES;
+      const __nv_bfloat16* scales = scales_of(min(stack_of(r, slot), a.stacks - 1));
+      PartScales<GROUP, PART> next;
+      next.load(scales, 0, a.blocks);
+      for (int b0 = 0; b0 < a.blocks && ok; b0 += PART) {
+        const PartScales<GROUP, PART> now = next;
+        next.load(scales, b0 + PART, a.blocks);
+        const float up = power(now.shift());
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(w[t].x), "=r"(w[t].y), "=r"(w[t].z), "=r"(w[t].w)
-                       : "r"(at + (chunk_at(row, t) << 4)));
-        __syncwarp();
-        if (lane == 0) bar_arrive(empty + 8 * s);
-        if (++s == a.stages) {
-          s = 0;
-          ph ^= 1;
-        }
-        if (!there) continue;
+        for (int i = 0; i < PART; ++i) {
+          if (b0 + i >= a.blocks || !ok) break;
+          if (!(ok = bar_wait(full + 8 * s, ph))) break;
+          uint4 w[4];
+          const uint32_t at = base + s * stage + slot * WIDE_BYTES + row * BLOCK_BYTES;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t v[32];
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            uint32_t q[4];
-            unpack<BF16>(((const uint32_t*)&w[c & 3])[2 * h + (c >> 2)], q);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[4 * c + i] = q[i];
-          }
-          if (h == 0) {
-            if (!(ok = bar_wait(a_empty + 8 * (2 * slot + buf), buf_ph ^ 1))) break;
-            fence_after();
-          }
-          tmem_store32(tmem + a_column(slot, buf) + 32 * h + quarter, v);
-        }
-        tmem_store_wait();
-        fence_before();
-        __syncwarp();
-        if (lane == 0 && ok) bar_arrive(a_full + 8 * (2 * slot + buf));
-        buf ^= 1;
-        if (buf == 0) buf_ph ^= 1;
-      }
-    }
-  } else if (warp < 8 * SLOTS) {  // adds up
-    take_registers<120>();
-    constexpr int PER = BLOCK / GROUP;             // groups of a block
-    constexpr int CHUNK = COLUMNS == 64 ? 32 : COLUMNS;  // columns in registers at once, beside their sums
-    const int slot = (warp - 4 * SLOTS) >> 2;
-    const uint32_t quarter = (uint32_t)(warp & 3) << 21;
-    int buf = 0, buf_ph = 0, s = 0, ph = 0, a_buf = 0;
-    bool ok = true;
-    for (int r = 0; r < rounds && ok; ++r) {
-      const int stack = stack_of(r, slot);
-      if (stack >= a.stacks) {  // nothing of these stages is this slot's
-        for (int b = 0; b < a.blocks && ok; ++b) {
-          ok = bar_wait(full + 8 * s, ph);
+          for (int t = 0; t < 4; ++t)
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[t].x), "=r"(w[t].y), "=r"(w[t].z), "=r"(w[t].w)
+                         : "r"(at + (chunk_at(row, t) << 4)));
           __syncwarp();
           if (lane == 0) bar_arrive(empty + 8 * s);
           if (++s == a.stages) {
             s = 0;
             ph ^= 1;
           }
-        }
-        continue;
-      }
-      const int v = stack * WIDE + (warp & 3) * 32 + lane;
-      const long long tile = tile_of(min(v, a.V - 1), a.blocks, 0);
-      const __nv_bfloat16* scales = a.scale + (tile * ROWS + (v & 15)) * PER;
-      auto scale_of = [&](int b) {
-        uint2 s = make_uint2(0, 0);
-        if (b < a.blocks) {
-          const __nv_bfloat16* p = scales + b * (ROWS * PER);
-          if constexpr (GROUP == 32)
-            s = __ldcs((const uint2*)p);
-          else if constexpr (GROUP == 64)
-            s.x = __ldcs((const uint32_t*)p);
-          else
-            s.x = __ldcs((const uint16_t*)p);
-        }
-        return s;
-      };
-      float acc[COLUMNS];
+          if (!there) continue;
 #pragma unroll
-      for (int c = 0; c < COLUMNS; ++c) acc[c] = 0.0f;
-      uint2 next = scale_of(0), after = scale_of(1);
-      for (int b = 0; b < a.blocks && ok; ++b) {
-        const uint2 now = next;
-        next = after;
-        after = scale_of(b + 2);
+          for (int h = 0; h < 2; ++h) {
+            uint32_t v[32];
 #pragma unroll
-        for (int g = 0; g < PER; ++g) {
-          const uint32_t two = g < 2 ? now.x : now.y;
-          const float scale = bitsf(g & 1 ? two & 0xffff0000u : two << 16);
-          if (!(ok = bar_wait(d_full + 8 * (2 * slot + buf), buf_ph))) break;
-          fence_after();
-          if (g == PER - 1) {  // the block's products are done
-            if (lane == 0) {
-              bar_arrive(a_empty + 8 * (2 * slot + a_buf));
-              bar_arrive(empty + 8 * s);
+            for (int j = 2 * h; j < 2 * h + 2; ++j) {
+              const __half2 scale = __float2half2_rn(now.at(i, j * 32 / GROUP) * up);
+#pragma unroll
+              for (int t = 0; t < 4; ++t) {
+                uint32_t q[4];
+                unpack<false>(((const uint32_t*)&w[t])[j], q);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const __half2 x = __hmul2(*(const __half2*)&q[e], scale);
+                  v[16 * (j & 1) + 4 * t + e] = *(const uint32_t*)&x;
+                }
+              }
             }
-            a_buf ^= 1;
-            if (++s == a.stages) {
-              s = 0;
-              ph ^= 1;
+            if (h == 0) {
+              if (!(ok = bar_wait(a_empty + 8 * (2 * slot + buf), buf_ph ^ 1))) break;
+              fence_after();
             }
+            tmem_store32(tmem + a_column(slot, buf) + 32 * h + quarter, v);
           }
-          const uint32_t from = tmem + d_column(slot, buf) + quarter;
-#pragma unroll
-          for (int c = 0; c < COLUMNS; c += CHUNK) {
-            uint32_t sum[CHUNK / 16][16];
-#pragma unroll
-            for (int i = 0; i < CHUNK / 16; ++i) tmem_load16(from + c + 16 * i, sum[i]);
-            tmem_load_wait();
-            if (c + CHUNK == COLUMNS) {
-              fence_before();
-              __syncwarp();
-              if (lane == 0) bar_arrive(d_empty + 8 * (2 * slot + buf));
-            }
-#pragma unroll
-            for (int i = 0; i < CHUNK; ++i) acc[c + i] = fmaf(scale, bitsf(sum[i / 16][i % 16]), acc[c + i]);
-          }
+          tmem_store_wait();
+          fence_before();
+          __syncwarp();
+          if (lane == 0 && ok) bar_arrive(a_full + 8 * (2 * slot + buf));
           buf ^= 1;
           if (buf == 0) buf_ph ^= 1;
         }
       }
-      if (v < a.V) {
-        const float2* down = (const float2*)((const char*)a.operand + (long long)a.blocks * x_bytes);
+    }
+  } else if (warp < 8 * SLOTS) {  // adds up
+    const int slot = (warp - 4 * SLOTS) >> 2;
+    const uint32_t quarter = (uint32_t)(warp & 3) << 21;
+    int buf = 0, buf_ph = 0;
+    bool ok = true;
+    for (int r = 0; r < rounds && ok; ++r) {
+      const int stack = stack_of(r, slot);
+      if (stack >= a.stacks) break;
+      const __nv_bfloat16* scales = scales_of(stack);
+      float acc[COLUMNS];
 #pragma unroll
-        for (int c = 0; c < COLUMNS; ++c) {
-          if (c >= a.rows) continue;
-          const float y = P == 1 ? acc[c] : acc[c] * down[c].x * down[c].y;
-          store_logit(a, c, v, ok ? y : NAN);  // NaN: a wait gave up
+      for (int c = 0; c < COLUMNS; ++c) acc[c] = 0.0f;
+      for (int b0 = 0; b0 < a.blocks && ok; b0 += PART) {
+        PartScales<GROUP, PART> now;
+        now.load(scales, b0, a.blocks);
+        const float down = power(-now.shift());
+        if (!(ok = bar_wait(d_full + 8 * (2 * slot + buf), buf_ph))) break;
+        fence_after();
+        const uint32_t from = tmem + d_column(slot, buf) + quarter;
+#pragma unroll
+        for (int c = 0; c < COLUMNS; c += 16) {
+          uint32_t sum[16];
+          tmem_load16(from + c, sum);
+          tmem_load_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[c + i] = fmaf(down, bitsf(sum[i]), acc[c + i]);
         }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(d_empty + 8 * (2 * slot + buf));
+        buf ^= 1;
+        if (buf == 0) buf_ph ^= 1;
+      }
+      const int v = stack * WIDE + (warp & 3) * 32 + lane;
+      if (v < a.V) {
+        const float2* back = (const float2*)((const char*)a.operand + (long long)a.blocks * x_bytes);
+#pragma unroll
+        for (int c = 0; c < COLUMNS; ++c)
+          if (c < a.rows) store_logit(a, c, v, ok ? acc[c] * back[c].x * back[c].y : NAN);  // NaN: a wait gave up
       }
     }
   } else if (warp == 8 * SLOTS) {  // copies
@@ -904,38 +920,44 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
         for (int i = 0; i < a.stages; ++i) bar_wait(full + 8 * i, ph);  // copies in flight
     }
   } else {  // issues a slot's products; the warp runs through as one, so that addresses are uniform
-    constexpr uint32_t desc = mma_desc(BF16, false, false, WIDE, COLUMNS);
+    constexpr uint32_t desc = mma_desc(false, false, false, WIDE, COLUMNS);
     const int slot = __shfl_sync(PESTI_FULL_MASK, warp, 0) - (8 * SLOTS + 1);
     int s = 0, ph = 0, abuf = 0, a_ph = 0, dbuf = 0, d_ph = 0;
     bool ok = true;
     for (int r = 0; r < rounds && ok; ++r) {
-      if (stack_of(r, slot) >= a.stacks) break;
+      const bool there = stack_of(r, slot) < a.stacks;
       for (int b = 0; b < a.blocks && ok; ++b) {
         ok = __all_sync(PESTI_FULL_MASK, bar_wait(full + 8 * s, ph));
-        if (ok) ok = __all_sync(PESTI_FULL_MASK, bar_wait(a_full + 8 * (2 * slot + abuf), a_ph));
-        if (!ok) break;
-        const uint32_t x = base + s * stage + SLOTS * WIDE_BYTES;
-#pragma unroll
-        for (int at = 0; at < BLOCK; at += GROUP) {
+        if (ok && there) ok = __all_sync(PESTI_FULL_MASK, bar_wait(a_full + 8 * (2 * slot + abuf), a_ph));
+        if (ok && there && b % PART == 0)
           ok = __all_sync(PESTI_FULL_MASK, bar_wait(d_empty + 8 * (2 * slot + dbuf), d_ph ^ 1));
-          if (!ok) break;
+        if (!ok) break;
+        if (!there) {  // nothing of this stage is this slot's
+          if (lane == 0) bar_arrive(empty + 8 * s);
+        } else {
           fence_after();
+          const bool last = b % PART == PART - 1 || b == a.blocks - 1;
           if (elect_one()) {
             const uint32_t d = tmem + d_column(slot, dbuf), from = tmem + a_column(slot, abuf);
-            const uint64_t xd = operand_desc(x, 0);
+            const uint64_t xd = operand_desc(base + s * stage + SLOTS * WIDE_BYTES, 0);
 #pragma unroll
-            for (int k = at; k < at + GROUP; k += 16)
+            for (int k = 0; k < BLOCK; k += 16)
 #pragma unroll
               for (int p = 0; p < P; ++p)
-                mma_f16_tmem(d, from + k / 2, xd + ((k / 64 * P + p) * x_half >> 4) + k % 64 / 8, desc, k > at || p > 0);
-            mma_commit<1>(d_full + 8 * (2 * slot + dbuf));
+                mma_f16_tmem(d, from + k / 2, xd + ((k / 64 * P + p) * x_half >> 4) + k % 64 / 8, desc,
+                             b % PART || k || p);
+            mma_commit<1>(a_empty + 8 * (2 * slot + abuf));
+            mma_commit<1>(empty + 8 * s);
+            if (last) mma_commit<1>(d_full + 8 * (2 * slot + dbuf));
           }
           __syncwarp();
-          dbuf ^= 1;
-          if (dbuf == 0) d_ph ^= 1;
+          if (last) {
+            dbuf ^= 1;
+            if (dbuf == 0) d_ph ^= 1;
+          }
+          abuf ^= 1;
+          if (abuf == 0) a_ph ^= 1;
         }
-        abuf ^= 1;
-        if (abuf == 0) a_ph ^= 1;
         if (++s == a.stages) {
           s = 0;
           ph ^= 1;

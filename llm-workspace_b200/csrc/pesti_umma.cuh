@@ -137,16 +137,6 @@ __device__ __forceinline__ void store_wait_all() { asm volatile("cp.async.bulk.w
 // Shared memory written by threads is visible to bulk copies issued behind this.
 __device__ __forceinline__ void fence_smem_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// Registers of a warpgroup's threads from here on; what is taken has to have been given by others.
-template <int N>
-__device__ __forceinline__ void give_registers() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void take_registers() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-
 // --- tensor memory
 
 template <int CG>

@@ -87,8 +87,29 @@ def test_groups_that_are_not_finite():
     bad = torch.zeros(4, 256, dtype=torch.bool, device="cuda")
     bad[1, 64:128], bad[2, :64], bad[3, 192:] = True, True, True
     assert torch.equal(torch.isnan(got), bad) and torch.equal(got[~bad], want[~bad])
-    logits = ph.head_logits(torch.ones(2, 256, device="cuda"), ph.quantize_head(w, 64))
-    assert torch.isnan(logits[:, 1:]).all() and torch.isfinite(logits[:, 0]).all()
+    for rows in (2, 20):
+        logits = ph.head_logits(torch.ones(rows, 256, device="cuda"), ph.quantize_head(w, 64))
+        assert torch.isnan(logits[:, 1:]).all() and torch.isfinite(logits[:, 0]).all()
+
+
+@pytest.mark.parametrize("B", [3, 20])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_scales_of_all_magnitudes(B, dtype):
+    """Groups of a row that are 2^-60 to 2^60 of one another.  With more rows, scales below 2^-25 of the largest of their
+    columns lose bits: an element q s is off by at most 2^-25 steps of what f16 holds, 2^-36 of the largest s, and no
+    more than half of itself."""
+    V, D, group = 200, 1500, 32
+    w = _weight(V, D, "f32")
+    n = -(-D // group)
+    sizes = torch.exp2(torch.randint(-30, 31, (V, n), generator=torch.Generator().manual_seed(B)).float()).cuda()
+    w = w * sizes.repeat_interleave(group, 1)[:, :D]
+    held, want = _check_held(w, group)
+    x = torch.randn(B, D, generator=torch.Generator().manual_seed(9)).to(DT[dtype]).cuda()
+    got = ph.head_logits(x, held, dtype=torch.float32).double()
+    exact, S = x.double() @ want.T, x.double().abs() @ want.abs().T
+    tol = (D / 16 + D / group + 8) * 2.0 ** -22 * S
+    tol = tol + 2.0 ** -36 * x.double().abs().sum(1, keepdim=True) * held.scale.double().abs().amax(1)[None]
+    assert ((got - exact).abs() <= tol + 2.0 ** -24 * exact.abs()).all()
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
@@ -277,6 +298,10 @@ def test_a_whole_step(sampler):
     said = ph.linear_cross_entropy(hidden[rows], back, token.reshape(-1))
     o = OH.cross_entropy(hidden[rows], back, token.reshape(-1))
     want = OH.cross_entropy(hidden[rows], held.dequantize(torch.float32), token.reshape(-1))
-    assert torch.allclose(-score.reshape(-1).double(), want["loss"], rtol=0, atol=2e-5)
+    # a score is a logit less the logarithm of a sum of them, each off by the bound at the top of this file; the sum is
+    # off by 2e-6 of itself, and scores of up to 70 are rounded to f32 twice
+    S = (hidden.double().abs() @ held.dequantize(torch.float32).double().abs().T).amax()
+    room = float(2 * (D / 16 + D / 32 + 8) * 2.0 ** -22 * S + 2e-6 + 70 * 2.0 ** -23)
+    assert want["loss"].max() < 70 and torch.allclose(-score.reshape(-1).double(), want["loss"], rtol=0, atol=room)
     assert torch.allclose(said.double(), o["loss"], rtol=0, atol=float(2 * (D / 16 + 4) * 2.0 ** -22 * o["size"].max()) + 2e-5)
     assert exact.shape == logits.shape
