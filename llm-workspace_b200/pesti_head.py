@@ -246,29 +246,33 @@ def head_logits(x, held: QuantizedHead, dtype=None, out=None, stream=None):
     (None: x's), or out: the [B, V] tensor to fill (rows may be strided).  Made
     for the few rows of a decode step: the weight is read once for every 64 rows
     of x, and no gradient reaches it."""
-    _need(x.dim() == 2 and x.dtype in _DTYPES, "x must be a [B, D] float32, bfloat16 or float16 tensor")
-    (B, D), dev = x.shape, x.device
-    _need(D == held.D, "x and the held weight have different D")
-    _need(held.device == dev, "x and the held weight must be on the same device")
-    _need(D == 1 or x.stride(1) == 1, "x rows must be contiguous")
+    code, shape, to_x, dev = _DTYPES.get(x.dtype), x.shape, x.stride(), x.device
+    if code is None or len(shape) != 2:
+        raise ValueError("x must be a [B, D] float32, bfloat16 or float16 tensor")
+    (B, D), V, packed = shape, held.V, held.packed
+    if D != held.D:
+        raise ValueError("x and the held weight have different D")
+    if packed.device != dev:
+        raise ValueError("x and the held weight must be on the same device")
+    if D > 1 and to_x[1] != 1:
+        raise ValueError("x rows must be contiguous")
     if out is not None:
-        _need(out.device == dev and out.shape == (B, held.V) and out.dtype in _DTYPES
-              and (held.V == 1 or out.stride(1) == 1),
+        _need(out.device == dev and out.shape == (B, V) and out.dtype in _DTYPES and (V == 1 or out.stride(1) == 1),
               "out must be a [B, V] float32, bfloat16 or float16 tensor with contiguous rows on x's device")
+        kind = out.dtype
     else:
-        dtype = dtype or x.dtype
-        _need(dtype in _DTYPES, "dtype must be float32, bfloat16 or float16")
-    x = x.detach()
-    code = _DTYPES[x.dtype]
+        kind = dtype or x.dtype
+        if kind not in _DTYPES:
+            raise ValueError("dtype must be float32, bfloat16 or float16")
 
     def call(st):
-        to = out if out is not None else x.new_empty((B, held.V), dtype=dtype)
+        to = out if out is not None else x.new_empty((B, V), dtype=kind)
         if B:
             need = _logits_workspace(code, B, D)
             ws = x.new_empty(need, dtype=torch.uint8) if need else None
             rc = load_library().pesti_q4_logits(
-                x.data_ptr(), code, B, D, _row_stride(x), held.packed.data_ptr(), held.tile_scale.data_ptr(),
-                held.V, held.group, to.data_ptr(), _DTYPES[to.dtype], _row_stride(to), _ptr(ws), need, st)
+                x.data_ptr(), code, B, D, to_x[0] if B > 1 else D, packed.data_ptr(), held.tile_scale.data_ptr(), V,
+                held.group, to.data_ptr(), _DTYPES[kind], _row_stride(to) if out is not None else V, _ptr(ws), need, st)
             if rc:
                 _check(rc)
             if out is not None:
