@@ -507,8 +507,9 @@ int pesti_distill_topk_backward(const void* d_logits, pesti_dtype dtype, int64_t
  *              - label_smoothing / V ]
  *   grad_hidden = G head,  grad_head = G^T hidden      (in the inputs' type)
  * Products are summed in f32, the rows' sums of exponentials joined in 64 bits;
- * G is rounded once to the inputs' type (F16: times a power of two that brings
- * its largest value to about 2^14; what is 2^38 below that is lost).  Logits
+ * G is rounded once to the inputs' type, or (up to 64 rows) held as the sum of two
+ * such values (F16: times a power of two that brings its largest value to about
+ * 2^14; what is 2^38 below that is lost).  Logits
  * that are NaN or +inf make their row's loss NaN, and the gradients that the row
  * has part in.
  *

@@ -237,14 +237,16 @@ RowArgs row_args(const Call& c, const Layout& l, int cg, int sms) {
   r.k_piece = (int)(l.cut.piece / BK);
   r.part_room = l.cut.part_room;
   r.tile_rows = 128 * cg;
+  r.twice = c.N <= TWICE;
   r.units = sms / cg;
   return r;
 }
 
-GemmArgs gemm_args(const Layout& l) {
+GemmArgs gemm_args(const Layout& l, bool twice) {
   GemmArgs g = {};
   g.plan = l.plan;
   g.a_box = 128;
+  g.twice = twice;
   g.target = l.packed;
   g.rows_pad = l.rows_pad;
   g.coef = l.coef;
@@ -262,7 +264,7 @@ int forward(const Call& c, const Layout& l, RowArgs r, bool grads, Device dev, c
   int rc = pesti_tensor_map(&rows, pesti_map_type(c.dtype), l.rows, c.D, l.rows_pad, l.ldc * 2, 64, a_box(c.N));
   if (!rc) rc = pesti_tensor_map(&head, pesti_map_type(c.dtype), c.head, c.D, c.V, c.w_ld * 2, 64, l.width / CG);
   if (rc) return rc;
-  GemmArgs g = gemm_args(l);
+  GemmArgs g = gemm_args(l, r.twice);
   g.width = l.width;
   g.m_tiles = -1;
   g.a_box = a_box(c.N);
@@ -302,7 +304,7 @@ int backward(const Call& c, const Layout& l, RowArgs r, void* dh, int64_t dh_ld,
     if (!rc) rc = pesti_tensor_map(&grad_k, pesti_map_type(c.dtype), l.grad, width, l.rows_pad, l.cut.piece * 2, 64, a_box(c.N));
     if (!rc) rc = pesti_tensor_map(&grad_mn, pesti_map_type(c.dtype), l.grad, width, l.rows_pad, l.cut.piece * 2, 64, 64);
     if (rc) return rc;
-    GemmArgs g = gemm_args(l);  // G of this piece
+    GemmArgs g = gemm_args(l, r.twice);  // G of this piece
     g.m_tiles = -1;
     g.a_box = a_box(c.N);
     g.n_tiles = (int)((width + BN - 1) / BN);
@@ -316,7 +318,7 @@ int backward(const Call& c, const Layout& l, RowArgs r, void* dh, int64_t dh_ld,
     rc = launch_gemm<CG, BF16, false, false, GRAD>(rows_k, head_k, grad_out, g, dev, st);
     if (rc) return rc;
     if (dh) {  // dh += G W, first: this piece of the head is in L2 yet
-      g = gemm_args(l);
+      g = gemm_args(l, r.twice);
       g.m_tiles = -1;
       g.a_box = a_box(c.N);
       g.n_tiles = d_tiles;
@@ -329,7 +331,7 @@ int backward(const Call& c, const Layout& l, RowArgs r, void* dh, int64_t dh_ld,
       if (rc) return rc;
     }
     if (dw) {  // dW = G^T h
-      g = gemm_args(l);
+      g = gemm_args(l, r.twice);
       g.m_tiles = (int)((width + 128 * CG - 1) / (128 * CG));
       g.n_tiles = d_tiles;
       g.k_iters = -1;

@@ -11,6 +11,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <climits>
+
 #include "pesti_common.cuh"
 #include "pesti_umma.cuh"
 
@@ -48,6 +50,11 @@ struct RowCoef {
 
 enum Epilogue { STATS, GRAD, OUT16, PART32 };
 
+// Up to this many rows G is held as a sum of two 16-bit values, the second in rows TWICE behind the first, and the packed
+// rows are there twice.  A tile has 128 rows in any case, so that this costs a little writing, and few rows' gradients,
+// which hang on few values of G, are as exact as their own type: a single row's were off by 2^-8 instead of 2^-9.
+constexpr int TWICE = 64;
+
 // Stages in shared memory, beside what is on its way out.
 __host__ __device__ constexpr int out_bytes(Epilogue e) { return e == STATS ? 4096 : EPI_WARPS * 2 * OUT_BYTES; }
 __host__ __device__ constexpr int stages(int cg, Epilogue e) {
@@ -76,6 +83,7 @@ struct GemmArgs {
   int add;            // PART32: add to what is there
   int out_x, out_y;   // where the output ends
   int width;          // columns of a tile (STATS: a multiple of 16)
+  int twice;          // G and the packed rows are held twice
 };
 
 template <bool BF16>
@@ -86,6 +94,11 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   else
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+template <bool BF16>
+__device__ __forceinline__ float rounded(float x) {
+  return BF16 ? __bfloat162float(__float2bfloat16_rn(x)) : __half2float(__float2half_rn(x));
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -148,7 +161,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int active = g.plan->active;
   const int m_tiles = g.m_tiles < 0 ? (active + TM - 1) / TM : g.m_tiles;
   const int n_tiles = g.n_tiles;
-  const int k_iters = g.k_iters < 0 ? (active + BK - 1) / BK : g.k_iters;
+  const int k_rows = active && g.twice ? 2 * TWICE : active;
+  const int k_iters = g.k_iters < 0 ? (k_rows + BK - 1) / BK : g.k_iters;
   const int splits = E == PART32 ? g.plan->splits : 1, k_split = (k_iters + splits - 1) / splits;
   const int per_split = m_tiles * n_tiles, tiles = per_split * splits;
   const int first = blockIdx.x / CG, step = gridDim.x / CG;
@@ -180,7 +194,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int row_a = g.a_row0 + m * TM + (int)rank * 128;
         const int width = E == STATS ? g.width : BN;
         // rows of A that nothing comes of stay what they were in shared memory: they reach no row but their own
-        const int boxes = A_MN || g.a_box == 128 ? 1 : max(1, min(4, (active - row_a + 31) / 32));
+        const int rows_a = E == PART32 && g.twice ? 2 * TWICE : active;
+        const int boxes = A_MN || g.a_box == 128 ? 1 : max(1, min(4, (rows_a - row_a + 31) / 32));
         const uint32_t bytes = CG * (A_MN || g.a_box == 128 ? A_BYTES : boxes * (A_BYTES / 4)) + width * BK * 2;
         const int row_b = g.b_row0 + n * width + (int)rank * (width / CG);
         for (int k = 0; k < kn; ++k) {
@@ -444,7 +459,19 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           put_pairs(c);
         }
-        end_out(col0, col0 + 64, warp_row, false);
+        if (!g.twice) {
+          end_out(col0, col0 + 64, warp_row, false);
+        } else if (warp_row < TWICE) {
+          end_out(col0, col0 + 64, warp_row, false);
+          begin_out();
+#pragma unroll
+          for (int c = 0; c < HALF; c += 32) {
+#pragma unroll
+            for (int j = c; j < c + 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) - rounded<BF16>(__uint_as_float(v[j])));
+            put_pairs(c);
+          }
+          end_out(col0, col0 + 64, TWICE + warp_row, false);
+        }
       } else if constexpr (E == OUT16) {
         take_acc();
         begin_out();
@@ -457,7 +484,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         end_out(col0, col0 + 64, g.v0 + warp_row, false);
       } else {
         take_acc();
-        if (warp_row < active) {
+        if ((g.twice ? warp_row % TWICE : warp_row) < active) {
 #pragma unroll
           for (int c = 0; c < HALF; c += 64) {
             begin_out();
@@ -497,6 +524,7 @@ struct RowArgs {
   float* zt;
   void* rows;  // [rows_pad, ldc]
   long long ldc, rows_pad;
+  int twice;
   // forward
   const float2* parts;
   const float* zsum;
@@ -541,10 +569,10 @@ __device__ __forceinline__ unsigned split_time(const RowArgs& a, int active, int
   return (unsigned)fminf(4e9f, (float)rounds * (float)((a.k_piece + splits - 1) / splits + 16) + (float)splits * part);
 }
 
-// Packed row i: a row that counts, or zeros behind them to a whole tile.
+// Packed row i: row n, or (n < 0) zeros, behind the rows that count to a whole tile.
 __device__ __forceinline__ void put_row(const RowArgs& a, long long i, int active, long long n) {
   uint16_t* to = (uint16_t*)a.rows + i * a.ldc;
-  if (i >= active) {
+  if (n < 0) {
     if (i < (active + 255) / 256 * 256)
       for (long long d = threadIdx.x * 8; d < a.ldc; d += blockDim.x * 8) *(uint4*)(to + d) = make_uint4(0, 0, 0, 0);
     return;
@@ -572,6 +600,9 @@ __global__ void __launch_bounds__(PACK_ROWS) lce_pack_kernel(const RowArgs a) {
   __shared__ int scratch[33], mine;
   __shared__ unsigned most[33];
   const bool writes = !COPY || blockIdx.x == 0;
+  // of the rows that count, the one to copy
+  const int wanted = !a.twice ? blockIdx.x : blockIdx.x < 2 * TWICE ? blockIdx.x % TWICE : INT_MAX;
+  if (threadIdx.x == 0) mine = -1;
   int before = 0;
   unsigned bound = 0;
   for (long long n0 = 0; n0 < a.N; n0 += PACK_ROWS) {
@@ -593,7 +624,7 @@ __global__ void __launch_bounds__(PACK_ROWS) lce_pack_kernel(const RowArgs a) {
       }
     }
     if (live) {
-      if (COPY && at == blockIdx.x) mine = (int)n;
+      if (COPY && at == wanted) mine = (int)n;
       if (writes) {
         a.idx[at] = (int)n;
         a.packed[at] = (int)t;
@@ -637,7 +668,7 @@ __global__ void __launch_bounds__(256) lce_gather_kernel(const RowArgs a) {
   depend_wait();
   depend_launch();
   const int active = a.plan->active;
-  put_row(a, blockIdx.x, active, blockIdx.x < active ? a.idx[blockIdx.x] : 0);
+  put_row(a, blockIdx.x, active, blockIdx.x < active ? a.idx[blockIdx.x] : -1);
 }
 
 // A row's tiles joined: ROWS rows a block (8 share what is read; 1 where there are few).  GRADS: the coefficients of its
@@ -722,6 +753,13 @@ __global__ void __launch_bounds__(256) lce_finish_kernel(const RowArgs a) {
         v.y += x.y;
         v.z += x.z;
         v.w += x.w;
+        if (a.twice) {
+          const float4 y = __ldcs((const float4*)(from + TWICE * a.ld32 + s * part + d));
+          v.x += y.x;
+          v.y += y.y;
+          v.z += y.z;
+          v.w += y.w;
+        }
       }
     }
     // a NaN scale marks a wait that gave up, in padded rows too
