@@ -181,10 +181,10 @@ struct Device {
 
 // Every kernel waits on the device for the one before it, so it may be launched while that one still runs.
 template <typename... K, typename... A>
-int launch(const char* what, void (*kernel)(K...), int cg, long long blocks, int threads, int smem, cudaStream_t st,
+int launch(const char* what, void (*kernel)(K...), int cg, dim3 blocks, int threads, int smem, cudaStream_t st,
            const A&... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.gridDim = blocks;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -207,7 +207,7 @@ int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o
   static PestiShared shared;
   const int rc = pesti_allow_shared(shared, kernel, dev.index, smem_bytes(CG, E), "head_gemm_kernel shared memory");
   if (rc) return rc;
-  return launch("head_gemm_kernel launch", kernel, CG, dev.sms / CG * CG, THREADS, smem_bytes(CG, E), st, a, b, out, g);
+  return launch("head_gemm_kernel launch", kernel, CG, dim3(dev.sms / CG * CG), THREADS, smem_bytes(CG, E), st, a, b, out, g);
 }
 
 RowArgs row_args(const Call& c, const Layout& l, int cg, int sms) {
@@ -280,8 +280,10 @@ int forward(const Call& c, const Layout& l, RowArgs r, bool grads, Device dev, c
   r.zsum = g.zsum;
   const char* what = "lce_join_kernel launch";
   if (c.N <= 512)
-    return launch(what, grads ? lce_join_kernel<1, true> : lce_join_kernel<1, false>, 1, c.N, 256, 0, st, r);
-  return launch(what, grads ? lce_join_kernel<8, true> : lce_join_kernel<8, false>, 1, (c.N + 7) / 8, 256, 0, st, r);
+    return launch(what, grads ? lce_join_kernel<1, true> : lce_join_kernel<1, false>, 1, dim3((unsigned)c.N), 256, 0,
+                  st, r);
+  return launch(what, grads ? lce_join_kernel<8, true> : lce_join_kernel<8, false>, 1, dim3((unsigned)((c.N + 7) / 8)),
+                256, 0, st, r);
 }
 
 // Packed rows, plan and coefficients are there.
@@ -345,7 +347,19 @@ int backward(const Call& c, const Layout& l, RowArgs r, void* dh, int64_t dh_ld,
   if (!dh) return PESTI_OK;
   r.d_hidden = dh;
   r.dh_ld = dh_ld;
-  return launch("lce_finish_kernel launch", lce_finish_kernel<BF16>, 1, c.N, 256, 0, st, r);
+  const char* what = "lce_finish_kernel launch";
+  if (c.N <= 256)
+    return launch(what, lce_finish_kernel<BF16, 8>, 1, dim3((unsigned)((c.D + 127) / 128), (unsigned)c.N), 256, 0, st, r);
+  // (rows beyond a grid's second dimension in further launches)
+  for (long long n = 0; n < c.N; n += 65535) {
+    RowArgs some = r;
+    some.place += n;
+    some.d_hidden = (char*)dh + n * dh_ld * 2;
+    const dim3 grid((unsigned)((c.D + 1023) / 1024), (unsigned)std::min<long long>(65535, c.N - n));
+    rc = launch(what, lce_finish_kernel<BF16, 1>, 1, grid, 256, 0, st, some);
+    if (rc) return rc;
+  }
+  return PESTI_OK;
 }
 
 int backward(const Call& c, const Layout& l, const RowArgs& r, int cg, void* dh, int64_t dh_ld, void* dw, int64_t dw_ld,
@@ -358,9 +372,11 @@ int backward(const Call& c, const Layout& l, const RowArgs& r, int cg, void* dh,
 template <bool BACKWARD>
 int pack(const RowArgs& r, cudaStream_t st) {
   const char* what = "lce_pack_kernel launch";
-  if (r.N <= PACK_ROWS) return launch(what, lce_pack_kernel<BACKWARD, true>, 1, r.rows_pad, PACK_ROWS, 0, st, r);
-  const int rc = launch(what, lce_pack_kernel<BACKWARD, false>, 1, 1, PACK_ROWS, 0, st, r);
-  return rc ? rc : launch("lce_gather_kernel launch", lce_gather_kernel, 1, r.rows_pad, 256, 0, st, r);
+  const dim3 rows((unsigned)r.rows_pad);
+  if (r.N <= PACK_ROWS)
+    return launch(what, lce_pack_kernel<BACKWARD, true>, 1, rows, (int)std::max<long long>(256, up_to(r.N, 32)), 0, st, r);
+  const int rc = launch(what, lce_pack_kernel<BACKWARD, false>, 1, dim3(1), PACK_ROWS, 0, st, r);
+  return rc ? rc : launch("lce_gather_kernel launch", lce_gather_kernel, 1, rows, 256, 0, st, r);
 }
 
 int check_scratch(const void* ws, int64_t have, long long need) {

@@ -605,7 +605,7 @@ __global__ void __launch_bounds__(PACK_ROWS) lce_pack_kernel(const RowArgs a) {
   if (threadIdx.x == 0) mine = -1;
   int before = 0;
   unsigned bound = 0;
-  for (long long n0 = 0; n0 < a.N; n0 += PACK_ROWS) {
+  for (long long n0 = 0; n0 < a.N; n0 += blockDim.x) {
     const long long n = n0 + threadIdx.x;
     long long t = -1;
     float w = 1.0f;
@@ -730,48 +730,53 @@ __global__ void __launch_bounds__(256) lce_join_kernel(const RowArgs a) {
   }
 }
 
-// The hidden states' gradient: the parts summed in their order, to the rows' own places; padded rows get zeros.
-// Four columns a thread, eight parts at a time in flight.
-template <bool BF16>
+// The hidden states' gradient: the parts summed in their order, to the rows' own places; padded rows get zeros.  Four
+// columns a thread, eight parts at a time in flight.  TEAMS 8: a block has 128 columns of a row, and eight teams an
+// eighth of the parts each (few rows: 37 rows of 64 parts took 28 us in one team, 11 in eight); TEAMS 1: 1024 columns.
+template <bool BF16, int TEAMS>
 __global__ void __launch_bounds__(256) lce_finish_kernel(const RowArgs a) {
   depend_wait();
   depend_launch();
-  const long long n = blockIdx.x;
-  const int i = a.place[n], splits = a.plan->splits;
-  uint16_t* to = (uint16_t*)a.d_hidden + n * a.dh_ld;
-  const float scale = a.plan->failed ? NAN : pow2(-grad_shift<BF16>(a.plan));
-  const long long part = (long long)a.plan->part_rows * a.ld32;
-  const float* from = a.part32 + (long long)max(i, 0) * a.ld32;
-  const bool whole = ((uintptr_t)to & 7) == 0;
-  for (long long d = threadIdx.x * 4; d < a.D; d += 1024) {
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (i >= 0) {  // (columns of a part are padded to four)
+  constexpr int THREADS = 256 / TEAMS;
+  __shared__ float4 sums[TEAMS > 1 ? TEAMS : 1][THREADS];
+  const long long n = blockIdx.y;
+  const int i = a.place[n], splits = a.plan->splits, at = threadIdx.x % THREADS, team = threadIdx.x / THREADS;
+  const long long part = (long long)a.plan->part_rows * a.ld32, d = ((long long)blockIdx.x * THREADS + at) * 4;
+  const float* from = a.part32 + (long long)max(i, 0) * a.ld32 + d;
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  auto add = [&](float4 x) {
+    v.x += x.x;
+    v.y += x.y;
+    v.z += x.z;
+    v.w += x.w;
+  };
+  if (i >= 0 && d < a.D) {  // (columns of a part are padded to four)
+    const int s1 = splits * (team + 1) / TEAMS;
 #pragma unroll 8
-      for (int s = 0; s < splits; ++s) {
-        const float4 x = __ldcs((const float4*)(from + s * part + d));
-        v.x += x.x;
-        v.y += x.y;
-        v.z += x.z;
-        v.w += x.w;
-        if (a.twice) {
-          const float4 y = __ldcs((const float4*)(from + TWICE * a.ld32 + s * part + d));
-          v.x += y.x;
-          v.y += y.y;
-          v.z += y.z;
-          v.w += y.w;
-        }
-      }
+    for (int s = splits * team / TEAMS; s < s1; ++s) add(__ldcs((const float4*)(from + s * part)));
+    if (a.twice) {
+#pragma unroll 8
+      for (int s = splits * team / TEAMS; s < s1; ++s) add(__ldcs((const float4*)(from + s * part + TWICE * a.ld32)));
     }
-    // a NaN scale marks a wait that gave up, in padded rows too
-    const uint2 w = make_uint2(pack2<BF16>(v.x * scale, v.y * scale), pack2<BF16>(v.z * scale, v.w * scale));
-    if (whole && d + 4 <= a.D) {
-      *(uint2*)(to + d) = w;
-    } else {
-      const uint16_t h[4] = {(uint16_t)w.x, (uint16_t)(w.x >> 16), (uint16_t)w.y, (uint16_t)(w.y >> 16)};
+  }
+  if (TEAMS > 1) {
+    sums[team][at] = v;
+    __syncthreads();
+    if (team) return;
+    for (int k = 1; k < TEAMS; ++k) add(sums[k][at]);
+  }
+  if (d >= a.D) return;
+  // (a wait that gave up makes NaN, in padded rows too)
+  const float scale = a.plan->failed ? NAN : pow2(-grad_shift<BF16>(a.plan));
+  const uint2 w = make_uint2(pack2<BF16>(v.x * scale, v.y * scale), pack2<BF16>(v.z * scale, v.w * scale));
+  uint16_t* to = (uint16_t*)a.d_hidden + n * a.dh_ld + d;
+  if (((uintptr_t)to & 7) == 0 && d + 4 <= a.D) {
+    *(uint2*)to = w;
+  } else {
+    const uint16_t h[4] = {(uint16_t)w.x, (uint16_t)(w.x >> 16), (uint16_t)w.y, (uint16_t)(w.y >> 16)};
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (d + j < a.D) to[d + j] = h[j];
-    }
+    for (int j = 0; j < 4; ++j)
+      if (d + j < a.D) to[j] = h[j];
   }
 }
 

@@ -158,6 +158,12 @@ def test_pieces_of_the_vocabulary():
     _all_ways(hidden, head, target, up=up)
 
 
+def test_many_rows():
+    """More rows than a grid's second dimension."""
+    hidden, head, target = _make(70_001, 300, 24, "bf16", pad=0.3)
+    _all_ways(hidden, head, target)
+
+
 def test_long_vocabulary_with_few_rows():
     """K of the hidden states' gradient in many ranges."""
     for N in (2, 200):
