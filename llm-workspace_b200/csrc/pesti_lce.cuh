@@ -120,6 +120,8 @@ __device__ __forceinline__ int grad_shift(const Plan* plan) {
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
 
+// With 4096 rows x 128256 x 4096 each product runs at 521 clocks for a pair's 256 x 256 x 64, of the tensor cores' 512
+// (1.37 PFLOP/s at the clock that the power limit leaves); with 16 rows the head passes at 6.1 TB/s.
 // One block (CG 1) or a pair of them (CG 2) takes tiles of 128 CG x 256, one after another.  Warp 8 copies the stages
 // in, one thread of warp 9 issues the products, warps 0 to 7 empty one set of accumulators while the other is filled.
 template <int CG, bool BF16, bool A_MN, bool B_MN, Epilogue E>
