@@ -411,3 +411,23 @@ def test_trains():
         with torch.no_grad():
             for p, g_ in zip(params, grads):
                 p -= 0.5 * g_
+
+
+def test_modes():
+    """Inference mode, no grad, a head that is a view of a larger table, and no second derivative."""
+    hidden, head, target = _make(70, 900, 64, "bf16")
+    want = ph.linear_cross_entropy_grad(hidden, head, target)
+    with torch.inference_mode():
+        assert torch.equal(ph.linear_cross_entropy(hidden, head, target), want[0])
+        got = ph.linear_cross_entropy_grad(hidden, head, target)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    table = torch.zeros(1000, 64, dtype=head.dtype, device="cuda")
+    table[50:950] = head
+    table.requires_grad_()
+    loss = ph.linear_cross_entropy(hidden, table[50:950], target)
+    g, = torch.autograd.grad(loss.sum(), table)
+    assert torch.equal(g[50:950], want[2]) and (g[:50] == 0).all() and (g[950:] == 0).all()
+    x = hidden.requires_grad_()
+    g, = torch.autograd.grad(ph.linear_cross_entropy(x, head, target).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.float().sum().backward()

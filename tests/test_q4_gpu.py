@@ -305,3 +305,27 @@ def test_a_whole_step(sampler):
     assert want["loss"].max() < 70 and torch.allclose(-score.reshape(-1).double(), want["loss"], rtol=0, atol=room)
     assert torch.allclose(said.double(), o["loss"], rtol=0, atol=float(2 * (D / 16 + 4) * 2.0 ** -22 * o["size"].max()) + 2e-5)
     assert exact.shape == logits.shape
+
+
+def test_modes(sampler):
+    """Inference mode, tensors that require gradients, and outputs whose old values a backward pass needs."""
+    head = _weight(300, 256, "bf16")
+    x = torch.randn(5, 256, device="cuda").bfloat16()
+    held = ph.quantize_head(head.clone().requires_grad_(), 64)
+    want = ph.head_logits(x, held)
+    with torch.inference_mode():
+        assert torch.equal(ph.head_logits(x, ph.quantize_head(head, 64)), want)
+        out = torch.empty(5, 300, device="cuda", dtype=torch.bfloat16)
+        assert torch.equal(ph.head_logits(x, held, out=out), want)
+        back = torch.empty(300, 256, device="cuda")
+        assert torch.equal(held.dequantize(out=back), held.dequantize(torch.float32))
+        u = torch.rand(5, device="cuda")
+        a = sampler.sample_hidden(x, held, ps.SamplingConfig(top_k=5, top_p=1.0), u)
+    assert torch.equal(a, sampler.sample_hidden(x, held, ps.SamplingConfig(top_k=5, top_p=1.0), u))
+    got = ph.head_logits(x.requires_grad_(), held)
+    assert not got.requires_grad and torch.equal(got, want)
+    out = torch.randn(5, 300, device="cuda", requires_grad=True)
+    loss = (out * out).sum()
+    ph.head_logits(x, held, out=out.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
