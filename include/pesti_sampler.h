@@ -550,10 +550,10 @@ int pesti_linear_ce_backward(const void* d_hidden, pesti_dtype dtype, int64_t N,
  *   s = bf16(-m / 8), m the group's largest value by magnitude, the first of
  *       equal ones;  q = clamp(round-half-even(w / s), -8, 7)  (0 where s is 0)
  * A group with an infinity or a NaN is held as NaN.
- * Layout: tiles of 16 rows and 128 columns.  d_q: 1024 bytes a tile, [ceil(V /
- * 16)][ceil(D / 128)][16 rows][4 chunks][4 words]; d_scale: bf16 [ceil(V / 16)]
- * [ceil(D / 128)][16 rows][128 / group]; both 16-byte aligned.  Chunk c of row r
- * (0 to 15) of a tile has t = c ^ (r / 2 % 4); its 32-bit word j holds the tile's
+ * Layout: tiles of 64 rows and 128 columns.  d_q: 4096 bytes a tile, [ceil(V /
+ * 64)][ceil(D / 128)][64 rows][4 chunks][4 words]; d_scale: bf16 [ceil(V / 64)]
+ * [ceil(D / 128)][64 rows][128 / group]; both 16-byte aligned.  Chunk c of row r
+ * (0 to 63) of a tile has t = c ^ (r / 2 % 4); its 32-bit word j holds the tile's
  * columns 32j + 8t to 32j + 8t + 7 as q + 8, the first in its lowest 4 bits.
  * Columns from D on and rows from V on hold 8 (q = 0), rows from V on scales of 0.
  * pesti_q4_quantize fills d_q and d_scale.  pesti_q4_dequantize writes q s

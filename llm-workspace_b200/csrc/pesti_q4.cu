@@ -9,7 +9,6 @@
 #include "pesti_device.h"
 #include "pesti_error.h"
 #include "pesti_q4.cuh"
-#include "pesti_tensor_map.h"
 
 namespace {
 
@@ -83,7 +82,7 @@ int convert(bool there, const void* w, int64_t V, int64_t D, int64_t ld, void* q
   a.blocks = (int)blocks_of(D);
   a.V = (int)V;
   a.runs = (a.blocks + per<T>(there) - 1) / per<T>(there);
-  a.total = (V + ROWS - 1) / ROWS * (there ? ROWS : 1) * a.runs;
+  a.total = (V + ROWS - 1) / ROWS * (there ? ROWS : ROWS / 16) * a.runs;
   const int align = there || sizeof(T) == 4 ? 32 : 16, runs = there ? 32 : 1;  // of a thread block
   a.vec = (uintptr_t)w % align == 0 && (V == 1 || ld * sizeof(T) % align == 0);
   const long long grid = (a.total + runs - 1) / runs;
@@ -119,13 +118,15 @@ int pieces_of(pesti_dtype d) { return d == PESTI_F32 ? pieces<float> : 1; }
 int columns_of(int64_t rows) { return (int)(rows + 15) / 16 * 16; }
 
 // Few rows of x that fit shared memory whole.  A column tile of the products by warps holds 8; f32 rows cost them two
-// products (us for 4 / 8 / on tensor memory, 128256 x 4096: 82 / 88 / 89; 32001 x 1000: 12 / 14 / 11).
+// products, and each row some us before the first, so that more than 4 pay from 2048 columns on (us for 5 / 8, and on
+// tensor memory: 128256 x 4096: 78 / 82, 92 / 93; 8000 x 4096: 14 / 17, 22; 32000 x 2048: 18 / 20, 18 / 19; 32001 x 1000:
+// 12 / 14, 11 / 12).
 bool few(int64_t D, int pieces, int64_t rows) {
-  return rows <= (pieces == 1 ? 8 : 4) && blocks_of(D) * rows * pieces * (BLOCK * 2) <= FEW_BYTES;
+  return rows <= (pieces == 1 || D >= 2048 ? 8 : 4) && blocks_of(D) * rows * pieces * (BLOCK * 2) <= FEW_BYTES;
 }
 
-// How a pass with few rows shares its stacks and K out: the least time of the busiest SM, by the weight's bytes that it
-// reads (44 bytes a nanosecond), half a microsecond per round of stacks, and 50 ns for each part of a sum that is joined.
+// How a pass with few rows shares its tiles and their K out: the least time of the busiest SM, by the weight's bytes that it
+// reads (44 bytes a nanosecond), half a microsecond per round of tiles, and 50 ns for each part of a sum that is joined.
 int k_warps_of(long long stacks, int blocks, int warps, int sms) {
   double best = 1e30;
   int at = 1;
@@ -133,7 +134,7 @@ int k_warps_of(long long stacks, int blocks, int warps, int sms) {
     if (warps % kw || (kw > 1 && warps / kw > MOST_SLOTS)) continue;
     const int slots = warps / kw, turns = (blocks + kw - 1) / kw;
     const long long rounds = (stacks + (long long)sms * slots - 1) / ((long long)sms * slots);
-    const double t = (double)rounds * (warps * turns * (STACK * TILE_BYTES) / 44.0 + 500.0 + 50.0 * kw);
+    const double t = (double)rounds * (warps * turns * TILE_BYTES / 44.0 + 500.0 + 50.0 * kw);
     if (t < best) {
       best = t;
       at = kw;
@@ -160,23 +161,23 @@ int launch(const char* what, void (*kernel)(K...), long long blocks, int threads
 }
 
 template <int P, int GROUP, int COLUMNS>
-int wide_pass(const LogitArgs& a, Device dev, const CUtensorMap& weights, cudaStream_t st) {
+int wide_pass(const LogitArgs& a, Device dev, cudaStream_t st) {
   const auto kernel = q4_wide_kernel<P, GROUP, COLUMNS>;
   const int smem = 1024 + a.stages * (SLOTS * WIDE_BYTES + COLUMNS * P * (BLOCK * 2));
   static PestiShared shared;
   const int rc = pesti_allow_shared(shared, kernel, dev.index, smem, "q4_wide_kernel shared memory");
   if (rc) return rc;
-  return launch("q4_wide_kernel launch", kernel, std::min(dev.sms, a.stacks), WIDE_THREADS, smem, st, weights, a);
+  return launch("q4_wide_kernel launch", kernel, std::min(dev.sms, a.stacks), WIDE_THREADS, smem, st, a);
 }
 
 template <typename T, int GROUP>
 int pass(LogitArgs a, Device dev, cudaStream_t st) {
   constexpr int P = pieces<T>;
   if (few(a.D, P, a.rows)) {
-    a.stacks = (a.V + STACK * ROWS - 1) / (STACK * ROWS);
+    a.stacks = (a.V + ROWS - 1) / ROWS;
     a.k_warps = k_warps_of(a.stacks, a.blocks, FEW_WARPS, dev.sms);
     const int slots = FEW_WARPS / a.k_warps;
-    const int smem = a.blocks * a.rows * P * (BLOCK * 2) + 16 + (FEW_WARPS - slots) * STACK * 4 * 32 * 4;
+    const int smem = a.blocks * a.rows * P * (BLOCK * 2) + 16 + (FEW_WARPS - slots) * 16 * 32 * 4;
     const auto kernel = q4_logits_kernel<T, GROUP>;
     static PestiShared shared;
     const int rc = pesti_allow_shared(shared, kernel, dev.index, smem, "q4_logits_kernel shared memory");
@@ -186,17 +187,13 @@ int pass(LogitArgs a, Device dev, cudaStream_t st) {
   }
   a.stacks = (a.V + WIDE - 1) / WIDE;
   const int columns = columns_of(a.rows);
-  CUtensorMap weights;
-  const long long row = (long long)a.blocks * TILE_BYTES;
-  int rc = pesti_tensor_map(&weights, CU_TENSOR_MAP_DATA_TYPE_UINT32, a.q, row / 4, (a.V + ROWS - 1) / ROWS, row,
-                            TILE_WORDS, WIDE / ROWS, CU_TENSOR_MAP_SWIZZLE_NONE);
-  if (!rc) rc = launch("q4_operand_kernel launch", q4_operand_kernel<T>, columns, 256, 0, st, a, columns);
+  const int rc = launch("q4_operand_kernel launch", q4_operand_kernel<T>, columns, 256, 0, st, a, columns);
   if (rc) return rc;
   a.stages = std::min(8, SHARED_BYTES / (SLOTS * WIDE_BYTES + columns * P * (BLOCK * 2)));
-  if (columns == 16) return wide_pass<P, GROUP, 16>(a, dev, weights, st);
-  if (columns == 32) return wide_pass<P, GROUP, 32>(a, dev, weights, st);
-  if (columns == 48) return wide_pass<P, GROUP, 48>(a, dev, weights, st);
-  return wide_pass<P, GROUP, 64>(a, dev, weights, st);
+  if (columns == 16) return wide_pass<P, GROUP, 16>(a, dev, st);
+  if (columns == 32) return wide_pass<P, GROUP, 32>(a, dev, st);
+  if (columns == 48) return wide_pass<P, GROUP, 48>(a, dev, st);
+  return wide_pass<P, GROUP, 64>(a, dev, st);
 }
 
 template <typename T>

@@ -3,11 +3,11 @@
 //   s = bf16(-m / 8), m the group's largest value by magnitude (the first of equal ones)
 //   q = clamp(rint(w / s), -8, 7),  y = x (q s)^T
 //
-// Layout.  Tiles of 16 rows and 128 columns of 1024 bytes, [ceil(V / 16)][ceil(D / 128)][16 rows][64 bytes].  A row's
-// 16-byte chunk t is at place t ^ (row / 2 % 4), and its word j holds columns 32 j + 8 t to + 7: eight nibbles q + 8
-// from its low end.  So a chunk is what lane t of a quad of an m16n8k16 product needs for four steps of 32 columns, none
-// of which crosses a group; a warp reads a tile in two whole loads; and threads that take a row of a tile each read
-// their chunks from shared memory without bank conflicts.  Scales: [ceil(V / 16)][ceil(D / 128)][16 rows][128 / group].
+// Layout.  Tiles of 64 rows and 128 columns of 4 KB, [ceil(V / 64)][ceil(D / 128)][64 rows][64 bytes].  A row's 16-byte
+// chunk t is at place t ^ (row / 2 % 4), and its word j holds columns 32 j + 8 t to + 7: eight nibbles q + 8 from its low
+// end.  So a chunk is what lane t of a quad of an m16n8k16 product needs for four steps of 32 columns, none of which
+// crosses a group; a tile is one copy; and its rows' chunks are read from shared memory without bank conflicts, by quads
+// or by threads that take a row each.  Scales: [ceil(V / 64)][ceil(D / 128)][64 rows][128 / group].
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -42,16 +42,16 @@ __device__ __forceinline__ T from_f32(float v) {
     return __float2bfloat16_rn(v);
 }
 
-constexpr int ROWS = 16;                          // of a tile
+constexpr int ROWS = 64;                          // of a tile
 constexpr int TILE_WORDS = ROWS * BLOCK_BYTES / 4;
 
 // Where chunk t of a row is among the row's four.
 __host__ __device__ __forceinline__ int chunk_at(int row, int t) { return t ^ (row >> 1 & 3); }
 
 // The tile of a row's block, and in it the word of its columns 8 i to 8 i + 7, i = 4 j + t.
-__device__ __forceinline__ long long tile_of(long long row, int blocks, int block) { return (row >> 4) * blocks + block; }
+__device__ __forceinline__ long long tile_of(long long row, int blocks, int block) { return (row >> 6) * blocks + block; }
 __device__ __forceinline__ int word_of(int row, int i) {
-  return (row & 15) * (BLOCK_BYTES / 4) + chunk_at(row, i & 3) * 4 + (i >> 2);
+  return (row & 63) * (BLOCK_BYTES / 4) + chunk_at(row, i & 3) * 4 + (i >> 2);
 }
 
 template <typename T>
@@ -62,7 +62,7 @@ struct Held {
   __nv_bfloat16* scale;
   int D, blocks, runs;  // blocks of a row, and runs of PER blocks that its team takes
   int V;
-  long long total;      // runs of all rows, or of all tiles
+  long long total;      // runs of all rows, or of all sixteens of rows
   int vec;              // whole vectors of 8 columns can be read or written
 };
 
@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(256) q4_quantize_kernel(const Held<T> a) {
   const bool real = row < a.V;  // (rows to a whole tile are held as zeros)
   uint32_t* to = a.q + b * TILE_WORDS;
   const int word0 = word_of(row, 2 * i), word1 = word_of(row, 2 * i + 1);
-  __nv_bfloat16* scale = a.scale + (b * ROWS + (row & 15)) * (BLOCK / GROUP) + i / (GROUP / 16);
+  __nv_bfloat16* scale = a.scale + (b * ROWS + (row & 63)) * (BLOCK / GROUP) + i / (GROUP / 16);
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
     float hi, neg;
@@ -254,17 +254,17 @@ __global__ void __launch_bounds__(256) q4_quantize_kernel(const Held<T> a) {
 template <typename T, int GROUP, int PER>
 __global__ void __launch_bounds__(256) q4_dequantize_kernel(const Held<T> a) {
   const int i = threadIdx.x & 15;
-  // sixteen teams for a tile's sixteen rows, which are read whole
+  // sixteen teams for sixteen rows of a tile, whose bytes are next to one another
   long long row;
   int b0;
   if (!place_of(blockIdx.x, a.total, a.runs, row, b0)) return;
-  row = row * ROWS + (threadIdx.x >> 4);
+  row = row * 16 + (threadIdx.x >> 4);
   b0 *= PER;
   if (row >= a.V) return;
   const int n = min(PER, a.blocks - b0);
   const long long b = tile_of(row, a.blocks, b0);
   const uint32_t* from = a.q + b * TILE_WORDS + word_of(row, i);
-  const __nv_bfloat16* scale = a.scale + (b * ROWS + (row & 15)) * (BLOCK / GROUP) + i / (GROUP / 8);
+  const __nv_bfloat16* scale = a.scale + (b * ROWS + (row & 63)) * (BLOCK / GROUP) + i / (GROUP / 8);
   uint32_t w[PER];
   float s[PER];
 #pragma unroll
@@ -306,13 +306,13 @@ struct LogitArgs {
   int x_vec;    // whole vectors of 8 columns can be read
   const uint4* q;
   const __nv_bfloat16* scale;
-  int V, blocks, stacks;  // stacks of 64 rows, or of 128
+  int V, blocks, stacks;  // tiles of 64 rows, or pairs of them
   uint4* operand;        // x for the tensor cores (q4_operand_kernel)
   int stages;            // blocks in shared memory at once
   void* y;
   long long y_ld;
   int out;               // 0 f32, 1 bf16, 2 f16
-  int k_warps;           // warps that share a stack's K
+  int k_warps;           // warps that share a tile's K
 };
 
 __device__ __forceinline__ void store_logit(const LogitArgs& a, int row, int v, float y) {
@@ -443,7 +443,7 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(z0), "f"(z1), "f"(z2), "f"(z3));
 }
 
-// A lane's weights of a tile: 16 bytes of two rows (8 apart), and their groups' scales.
+// A lane's weights of 16 rows of a tile: 16 bytes of two rows (8 apart), and their groups' scales.
 template <int GROUP>
 struct Weights {
   uint4 w[2];
@@ -452,7 +452,7 @@ struct Weights {
   __device__ __forceinline__ void load(const uint4* q, const __nv_bfloat16* sc) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      w[i] = __ldcs(q + i * (TILE_WORDS / 8));
+      w[i] = __ldcs(q + i * 8 * (BLOCK_BYTES / 16));
       const __nv_bfloat16* p = sc + i * 8 * (BLOCK / GROUP);
       if constexpr (GROUP == 32)
         s[i] = __ldcs((const uint2*)p);
@@ -469,9 +469,7 @@ struct Weights {
   }
 };
 
-constexpr int STACK = 4;  // tiles of a warp, one above the other: x's fragments of a block serve them all
-
-// Warps that multiply: their registers hold a stack's sums and next weights and the fragments of a block of x.
+// Warps that multiply: their registers hold a tile's sums, the next weights and the fragments of a block of x.
 constexpr int FEW_WARPS = 16;
 
 // Barriers 1 to 7 and 8 to 14 of a block, one for each slot.
@@ -483,11 +481,13 @@ __device__ __forceinline__ void named_arrive(int id, int threads) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
-// Up to 8 rows of x: a warp multiplies a stack of 64 rows of the weight by all of them over its share of K (every
-// k_warps-th block), and goes on to its next stack; the k_warps warps of a stack join their sums in shared memory, in
+// Up to 8 rows of x: a warp multiplies a tile of 64 rows of the weight by all of them over its share of K (every
+// k_warps-th block), and goes on to its next tile; the k_warps warps of a tile join their sums in shared memory, in
 // their order.  x is laid out in shared memory once, while the first weights are on their way; a tile's weights are
-// loaded a block ahead.  A row of 128256 x 4096, g 64: 64 us in bf16, 61 in f16, 76 in f32 (4.4 to 3.7 TB/s), bound by the
-// integer pipe that unpacks; with a fragment of x read for each tile, and rows apart from one another, 80.
+// loaded a block ahead, and on their way to L2 another block ahead.  A row of 128256 x 4096, g 64: 60 us in bf16, 56 in
+// f16, 74 in f32 (4.7 to 3.8 TB/s), bound by the integer pipe that unpacks; with tiles of 16 rows, 1 KB at a time, 64.
+// Of 32000 x 2048, g 32: 11.5 us, without the prefetch 13.9.  Copies into four stages of shared memory: 59 and 11.5, but
+// 8 rows of 64000 x 8192, which leave them no room, 80 instead of 68.
 template <typename T, int GROUP>
 __global__ void __launch_bounds__(FEW_WARPS * 32, 1) q4_logits_kernel(const LogitArgs a) {
   constexpr bool BF16 = in_bf16<T>;
@@ -502,26 +502,18 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) q4_logits_kernel(const Logi
   pesti_umma::depend_wait();
   pesti_umma::depend_launch();
 
-  // the block to load next, of the stack of `load_round`
+  // the block to load next, of the tile of `load_round`
   const uint4* q;
   const __nv_bfloat16* sc;
   int load_round = 0, load_b = part;
-  Weights<GROUP> held[STACK];
+  Weights<GROUP> held[4];
   auto stack_of = [&](int round) { return (round * (int)gridDim.x + (int)blockIdx.x) * slots + slot; };
-  int q_up[STACK], s_up[STACK];
   auto begin = [&]() {
-    const int stack = min(stack_of(load_round), a.stacks - 1);
-    const long long tile = (long long)stack * STACK * a.blocks + part;
+    const long long tile = (long long)min(stack_of(load_round), a.stacks - 1) * a.blocks + part;
     q = a.q + tile * (TILE_WORDS / 4) + g * 4 + chunk_at(g, t);
     sc = a.scale + (tile * ROWS + g) * (BLOCK / GROUP);
-#pragma unroll
-    for (int i = 0; i < STACK; ++i) {  // a tile past the last row's is the last one again
-      const int up = min(i, (a.V - 1) / ROWS - stack * STACK) * a.blocks;
-      q_up[i] = up * (TILE_WORDS / 4);
-      s_up[i] = up * (ROWS * BLOCK / GROUP);
-    }
   };
-  auto load = [&](int i) { held[i].load(q + q_up[i], sc + s_up[i]); };
+  auto load = [&](int i) { held[i].load(q + i * 16 * (BLOCK_BYTES / 16), sc + i * 16 * (BLOCK / GROUP)); };
   auto advance = [&]() {
     load_b += kw;
     if (load_b < a.blocks) {
@@ -532,10 +524,14 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) q4_logits_kernel(const Logi
       ++load_round;
       begin();
     }  // behind the last block of all it stays where it is, and loads that once more
+    if (lane == 0) {  // whose q and sc are where the tile begins
+      pesti_umma::l2_prefetch(q, TILE_WORDS * 4);
+      pesti_umma::l2_prefetch(sc, ROWS * (BLOCK / GROUP) * 2);
+    }
   };
   begin();
 #pragma unroll
-  for (int i = 0; i < STACK; ++i) load(i);
+  for (int i = 0; i < 4; ++i) load(i);
   advance();
 
   if (sizeof(T) == 4) {
@@ -572,7 +568,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) q4_logits_kernel(const Logi
   const int x_block = there ? per_block : 0, x_step = there ? 4 * columns : 0;
 
   for (int r = 0; r < rounds; ++r) {
-    float acc[STACK][4] = {};
+    float acc[4][4] = {};
     for (int b = part; b < a.blocks; b += kw) {
       uint4 f[4][P];
 #pragma unroll
@@ -580,7 +576,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) q4_logits_kernel(const Logi
 #pragma unroll
         for (int p = 0; p < P; ++p) f[j][p] = mine[b * x_block + (j * P + p) * x_step];
 #pragma unroll
-      for (int i = 0; i < STACK; ++i) {
+      for (int i = 0; i < 4; ++i) {  // 16 rows
         const Weights<GROUP>& w = held[i];
 #pragma unroll
         for (int gr = 0; gr < BLOCK / GROUP; ++gr) {
@@ -616,16 +612,16 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) q4_logits_kernel(const Logi
       const int threads = kw * 32;
       if (part) {
         if (r) named_sync(8 + slot, threads);  // the last round's sums are read
-        float* to = sums + (slot * (kw - 1) + (part - 1)) * STACK * 4 * 32 + lane;
+        float* to = sums + (slot * (kw - 1) + (part - 1)) * 16 * 32 + lane;
 #pragma unroll
-        for (int e = 0; e < STACK * 4; ++e) to[e * 32] = acc[e >> 2][e & 3];
+        for (int e = 0; e < 16; ++e) to[e * 32] = acc[e >> 2][e & 3];
         named_arrive(1 + slot, threads);
       } else {
         named_sync(1 + slot, threads);
         for (int k = 0; k < kw - 1; ++k)
 #pragma unroll
-          for (int e = 0; e < STACK * 4; ++e)
-            acc[e >> 2][e & 3] += sums[((slot * (kw - 1) + k) * STACK * 4 + e) * 32 + lane];
+          for (int e = 0; e < 16; ++e)
+            acc[e >> 2][e & 3] += sums[((slot * (kw - 1) + k) * 16 + e) * 32 + lane];
         if (r + 1 < rounds) named_arrive(8 + slot, threads);
       }
     }
@@ -634,8 +630,8 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) q4_logits_kernel(const Logi
 #pragma unroll
     for (int e = 0; e < 2; ++e) down[e] = row_scale(sizeof(T) == 4 && 2 * t + e < a.rows ? most[2 * t + e] : 0.0f, true);
 #pragma unroll
-    for (int e = 0; e < STACK * 4; ++e) {
-      const int c = 2 * t + (e & 1), v = (stack * STACK + (e >> 2)) * ROWS + 8 * (e >> 1 & 1) + g;
+    for (int e = 0; e < 16; ++e) {
+      const int c = 2 * t + (e & 1), v = stack * ROWS + (e >> 2) * 16 + 8 * (e >> 1 & 1) + g;
       if (c < a.rows && v < a.V) store_logit(a, c, v, acc[e >> 2][e & 3] * down[e & 1].x * down[e & 1].y);
     }
   }
@@ -730,7 +726,7 @@ struct PartScales {
 
 __device__ __forceinline__ float power(int e) { return bitsf((uint32_t)(e + 127) << 23); }
 
-constexpr int WIDE = 128;                       // rows of the weight, eight tiles
+constexpr int WIDE = 128;                       // rows of the weight, two tiles
 constexpr int SLOTS = 2;                        // of them at once
 constexpr int WIDE_THREADS = (9 * SLOTS + 1) * 32;
 constexpr int WIDE_BYTES = WIDE * BLOCK_BYTES;  // of a block
@@ -740,11 +736,10 @@ __device__ __forceinline__ uint32_t a_column(int slot, int buf) { return slot * 
 __device__ __forceinline__ uint32_t d_column(int slot, int buf) { return slot * 256 + 128 + buf * 64; }
 
 // Warps 0 to 7 unpack (four a slot, a quarter of the rows each), 8 to 15 add up, 16 copies, 17 and 18 issue a slot's
-// products.  128256 x 4096, g 64, f16: 82 us for 16 rows, 97 for 48, 100 for 64, bound by the products' number: 16 for a
+// products.  128256 x 4096, g 64, f16: 85 us for 16 rows, 98 for 48, 102 for 64, bound by the products' number: 16 for a
 // stage of two blocks, some 64 clocks each from tensor memory whatever the columns.
 template <int P, int GROUP, int COLUMNS>
-__global__ void __launch_bounds__(WIDE_THREADS, 1)
-    q4_wide_kernel(const __grid_constant__ CUtensorMap weights, const LogitArgs a) {
+__global__ void __launch_bounds__(WIDE_THREADS, 1) q4_wide_kernel(const LogitArgs a) {
   using namespace pesti_umma;
   constexpr int PART = part_of(P);
   constexpr uint32_t x_half = COLUMNS * 128, x_bytes = 2 * P * x_half, stage = SLOTS * WIDE_BYTES + x_bytes;
@@ -781,7 +776,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
   // the scales of the thread's row in a stack
   auto scales_of = [&](int stack) {
     const int v = stack * WIDE + (warp & 3) * 32 + lane;
-    return a.scale + (tile_of(min(v, a.V - 1), a.blocks, 0) * ROWS + (v & 15)) * (BLOCK / GROUP);
+    return a.scale + (tile_of(min(v, a.V - 1), a.blocks, 0) * ROWS + (v & 63)) * (BLOCK / GROUP);
   };
 
   if (warp < 4 * SLOTS) {  // unpacks
@@ -891,19 +886,20 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
     }
   } else if (warp == 8 * SLOTS) {  // copies
     if (elect_one()) {
-      tma_prefetch(&weights);
+      const int tiles = (a.V + ROWS - 1) / ROWS;
       int s = 0, ph = 0;
       bool ok = true;
       for (int r = 0; r < rounds && ok; ++r) {
-        int there = 0;
-        for (int slot = 0; slot < SLOTS; ++slot) there += stack_of(r, slot) < a.stacks;
+        int there = 0;  // tiles of this round's stacks
+        for (int slot = 0; slot < SLOTS; ++slot) there += max(0, min(2, tiles - 2 * stack_of(r, slot)));
         for (int b = 0; b < a.blocks; ++b) {
           if (!(ok = bar_wait(empty + 8 * s, ph ^ 1))) break;
           const uint32_t to = base + s * stage;
-          bar_expect(full + 8 * s, there * WIDE_BYTES + x_bytes);
-          for (int slot = 0; slot < there; ++slot)
-            tma_load<1>(to + slot * WIDE_BYTES, &weights, full + 8 * s, b * TILE_WORDS,
-                        stack_of(r, slot) * (WIDE / ROWS));
+          bar_expect(full + 8 * s, there * (WIDE_BYTES / 2) + x_bytes);
+          for (int i = 0; i < there; ++i) {
+            const long long tile = (long long)(2 * stack_of(r, i >> 1) + (i & 1)) * a.blocks + b;
+            bulk_load(to + i * (WIDE_BYTES / 2), (const char*)a.q + tile * (WIDE_BYTES / 2), full + 8 * s, WIDE_BYTES / 2);
+          }
           bulk_load(to + SLOTS * WIDE_BYTES, (const char*)a.operand + (long long)b * x_bytes, full + 8 * s, x_bytes);
           if (++s == a.stages) {
             s = 0;

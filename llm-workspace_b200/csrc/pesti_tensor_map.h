@@ -15,10 +15,9 @@ static inline CUtensorMapDataType pesti_map_type(pesti_dtype dtype) {
 }
 
 // `rows` rows of `columns` elements, row_bytes apart (a multiple of 16); boxes of box_columns x box_rows, whose rows are
-// 128 bytes where they are swizzled.  Elements outside the matrix are read as 0 and not written.
+// 128 bytes.  Elements outside the matrix are read as 0 and not written.
 static inline int pesti_tensor_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, long long columns,
-                                   long long rows, long long row_bytes, int box_columns, int box_rows,
-                                   CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
+                                   long long rows, long long row_bytes, int box_columns, int box_rows) {
   typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -37,6 +36,7 @@ static inline int pesti_tensor_map(CUtensorMap* map, CUtensorMapDataType type, c
   const cuuint64_t dims[2] = {(cuuint64_t)columns, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)row_bytes};
   const cuuint32_t box[2] = {(cuuint32_t)box_columns, (cuuint32_t)box_rows}, ones[2] = {1, 1};
   const CUresult rc = encode(map, type, 2, (void*)base, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                             swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return rc == CUDA_SUCCESS ? PESTI_OK : pesti_set_error(PESTI_E_CUDA, "cuTensorMapEncodeTiled failed");
 }

@@ -150,25 +150,25 @@ def linear_cross_entropy_grad(hidden, head, target, weight=None, label_smoothing
     return loss, gh, gw
 
 
-_BLOCK, _ROWS = 128, 16  # of a tile of the held layout
+_BLOCK, _ROWS = 128, 64  # of a tile of the held layout
 
 
 class QuantizedHead:
     """A [V, D] weight in 4 bits with a scale for every `group` columns of a row
     (quantize_head), about (4.5, 4.25 or 4.125) / 16 of its bfloat16 size.
 
-    packed [ceil(V / 16), ceil(D / 128), 16, 64] uint8 and tile_scale
-    [ceil(V / 16), ceil(D / 128), 16, 128 / group] bfloat16 are the library's
+    packed [ceil(V / 64), ceil(D / 128), 64, 64] uint8 and tile_scale
+    [ceil(V / 64), ceil(D / 128), 64, 128 / group] bfloat16 are the library's
     layout (pesti_q4_quantize); scale is tile_scale by rows, [V, ceil(D / group)]."""
 
     def __init__(self, packed, tile_scale, V: int, D: int, group: int):
         _need(V >= 1 and D >= 1 and group in (32, 64, 128), "V and D must be at least 1, group 32, 64 or 128")
         tiles = -(-V // _ROWS), -(-D // _BLOCK), _ROWS
         _need(packed.dtype == torch.uint8 and packed.shape == (*tiles, _BLOCK // 2) and packed.is_contiguous(),
-              "packed must be a contiguous [ceil(V / 16), ceil(D / 128), 16, 64] uint8 tensor")
+              "packed must be a contiguous [ceil(V / 64), ceil(D / 128), 64, 64] uint8 tensor")
         _need(tile_scale.dtype == torch.bfloat16 and tile_scale.shape == (*tiles, _BLOCK // group)
               and tile_scale.is_contiguous() and tile_scale.device == packed.device,
-              "tile_scale must be a contiguous [ceil(V / 16), ceil(D / 128), 16, 128 / group] bfloat16 tensor on "
+              "tile_scale must be a contiguous [ceil(V / 64), ceil(D / 128), 64, 128 / group] bfloat16 tensor on "
               "packed's device")
         self.packed, self.tile_scale, self.V, self.D, self.group = packed, tile_scale, int(V), int(D), int(group)
 

@@ -59,13 +59,13 @@ def held_values(q, scale, group):
 
 
 def unpack(packed, V, D):
-    """q [V, D] from the library's layout, tiles of 16 rows and 128 columns: word j
+    """q [V, D] from the library's layout, tiles of 64 rows and 128 columns: word j
     of chunk t ^ (row // 2 % 4) of a row holds the tile's columns 32j + 8t to
     32j + 8t + 7, the first lowest."""
     T, B = packed.shape[:2]
-    b = packed.cpu().view(T, B, 16, 4, 4, 4).long()          # tile, block, row, chunk, j, byte
-    nib = torch.stack([b & 15, b >> 4], -1).reshape(T, B, 16, 4, 4, 8)
-    row, t = torch.arange(16)[:, None], torch.arange(4)[None, :]
+    b = packed.cpu().view(T, B, 64, 4, 4, 4).long()          # tile, block, row, chunk, j, byte
+    nib = torch.stack([b & 15, b >> 4], -1).reshape(T, B, 64, 4, 4, 8)
+    row, t = torch.arange(64)[:, None], torch.arange(4)[None, :]
     nib = nib[:, :, row, t ^ (row // 2 % 4)]                  # tile, block, row, t, j, column
-    q = nib.permute(0, 2, 1, 4, 3, 5).reshape(T * 16, B * 128)
+    q = nib.permute(0, 2, 1, 4, 3, 5).reshape(T * 64, B * 128)
     return (q[:V, :D] - 8).to(packed.device)

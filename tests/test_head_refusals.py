@@ -125,12 +125,12 @@ def test_python_refusals():
                       ((w, 48), "group"), ((w,), "CUDA device")]:
         with pytest.raises(ValueError, match=msg):
             ph.quantize_head(*args)
-    held = ph.QuantizedHead(torch.zeros(1, 1, 16, 64, dtype=torch.uint8), torch.zeros(1, 1, 16, 2).bfloat16(), 10, 64, 64)
+    held = ph.QuantizedHead(torch.zeros(1, 1, 64, 64, dtype=torch.uint8), torch.zeros(1, 1, 64, 2).bfloat16(), 10, 64, 64)
     assert held.V == 10 and held.scale.shape == (10, 1)
-    for change, msg in [(dict(V=0), "at least 1"), (dict(group=16), "group"), (dict(V=17), "packed must"),
+    for change, msg in [(dict(V=0), "at least 1"), (dict(group=16), "group"), (dict(V=65), "packed must"),
                         (dict(D=129), "packed must"), (dict(packed=held.packed.int()), "packed must"),
                         (dict(group=32), "tile_scale must"), (dict(tile_scale=held.tile_scale.float()), "tile_scale must"),
-                        (dict(packed=torch.zeros(1, 1, 64, 16, dtype=torch.uint8).transpose(2, 3)), "packed must")]:
+                        (dict(packed=torch.zeros(1, 1, 64, 64, dtype=torch.uint8).transpose(2, 3)), "packed must")]:
         with pytest.raises(ValueError, match=msg):
             ph.QuantizedHead(**{**dict(packed=held.packed, tile_scale=held.tile_scale, V=10, D=64, group=64), **change})
     for args, msg in [((h[0], held), "x must"), ((h.int(), held), "x must"), ((h[:, :32], held), "different D"),

@@ -165,8 +165,23 @@ def test_rounds(B, V):
     _check_logits(x, held, want, torch.float32)
 
 
+@pytest.mark.parametrize("B,dtype", [(1, "bf16"), (6, "f32"), (8, "f16"), (20, "bf16"), (33, "f32")])
+@pytest.mark.parametrize("V", [63, 64, 65, 127, 128, 129, 191, 193])
+@pytest.mark.parametrize("D", [2047, 2048])
+def test_tile_edges(B, dtype, V, D):
+    """Rows that end inside, at and just behind a tile and a pair of them."""
+    held, want = _check_held(_weight(V, D, "bf16"), 64)
+    assert held.packed.shape == ((V + 63) // 64, 16, 64, 64)
+    x = torch.randn(B, D, generator=torch.Generator().manual_seed(V)).to(DT[dtype]).cuda()
+    room = torch.full((B, V + 130), 7.0, device="cuda")
+    _check_logits(x, held, want, torch.float32, out=room[:, 1:1 + V])
+    assert (room[:, 0] == 7).all() and (room[:, 1 + V:] == 7).all()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("B,D", [(8, 12544), (8, 12545), (4, 12544), (4, 12673), (1, 100_352), (1, 100_353), (3, 70_000)])
+@pytest.mark.parametrize("B,D", [
+    (8, 6272), (8, 6273), (8, 12544), (8, 12545), (4, 12544), (4, 12673), (1, 100_352), (1, 100_353), (3, 70_000),
+])
 def test_long_rows(dtype, B, D):
     """x at, and just above, what is held in shared memory."""
     held, want = _check_held(_weight(40, D, "bf16"), 128)
