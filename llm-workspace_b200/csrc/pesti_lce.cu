@@ -406,6 +406,7 @@ int pesti_linear_ce(const void* d_hidden, pesti_dtype dtype, int64_t N, int64_t 
   if (rc) return rc;
   if (N == 0 && !d_grad_head) return PESTI_OK;
   if (N && !d_loss) return refuse("null loss");
+  if ((uintptr_t)d_loss % 4 || (uintptr_t)d_lse % 4) return refuse("loss or lse is not aligned to its type");
   const bool grads = d_grad_hidden || d_grad_head;
   if (grads) {
     rc = check_grads(c, d_grad_hidden, gh_ld, d_grad_head, gw_ld);
@@ -450,6 +451,7 @@ int pesti_linear_ce_backward(const void* d_hidden, pesti_dtype dtype, int64_t N,
   if (!d_grad_hidden && !d_grad_head) return refuse("no gradient is asked for");
   if (N == 0 && !d_grad_head) return PESTI_OK;
   if (N && (!d_lse || !d_up)) return refuse("null lse or upstream gradient");
+  if ((uintptr_t)d_lse % 4 || (uintptr_t)d_up % 4) return refuse("lse or upstream gradient is not aligned to its type");
   rc = check_grads(c, d_grad_hidden, gh_ld, d_grad_head, gw_ld);
   if (rc) return rc;
   Device dev = {};

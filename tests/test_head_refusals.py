@@ -41,7 +41,9 @@ COMMON = [
 ]
 
 
-@pytest.mark.parametrize("change,msg", COMMON + [(dict(loss=None), "null loss")])
+@pytest.mark.parametrize("change,msg", COMMON + [
+    (dict(loss=None), "null loss"), (dict(loss=P + 2), "loss or lse is not"), (dict(lse=P + 1), "loss or lse is not"),
+])
 def test_forward_refusals(lib, change, msg):
     assert lib.pesti_linear_ce(*{**CE, **FORWARD, **change}.values()) == BAD
     assert msg in lib.pesti_last_error().decode()
@@ -49,7 +51,8 @@ def test_forward_refusals(lib, change, msg):
 
 @pytest.mark.parametrize("change,msg", COMMON + [
     (dict(lse=None), "null lse"), (dict(up=None), "null lse"), (dict(up_stride=-1), "negative stride"),
-    (dict(gh=None, gw=None), "no gradient"),
+    (dict(gh=None, gw=None), "no gradient"), (dict(lse=P + 2), "gradient is not aligned"),
+    (dict(up=P + 1), "gradient is not aligned"),
 ])
 def test_backward_refusals(lib, change, msg):
     assert lib.pesti_linear_ce_backward(*{**CE, **BACKWARD, **change}.values()) == BAD
