@@ -726,6 +726,18 @@ struct PartScales {
 
 __device__ __forceinline__ float power(int e) { return bitsf((uint32_t)(e + 127) << 23); }
 
+// Nibbles i and i + 4 of a word as two f16 values q s, in one product: a nibble becomes the four highest bits of 16's
+// mantissa, 16 + q + 8, and minus = -24 s, which has 8 + 2 bits and is exact as s is; so is q s.  (q first, then times s,
+// by products and sums of two: 86, 99 and 102 us of the kernel below.)
+__device__ __forceinline__ void unpack_scaled(uint32_t word, __half2 s, __half2 minus, uint32_t (&q)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t v = masked(i == 0 ? word << 6 : i == 1 ? word << 2 : i == 2 ? word >> 2 : word >> 6, 0x03c003c0u, 0x4c004c00u);
+    const __half2 r = __hfma2(*(const __half2*)&v, s, minus);
+    q[i] = *(const uint32_t*)&r;
+  }
+}
+
 constexpr int WIDE = 128;                       // rows of the weight, two tiles
 constexpr int SLOTS = 2;                        // of them at once
 constexpr int WIDE_THREADS = (9 * SLOTS + 1) * 32;
@@ -736,8 +748,8 @@ __device__ __forceinline__ uint32_t a_column(int slot, int buf) { return slot * 
 __device__ __forceinline__ uint32_t d_column(int slot, int buf) { return slot * 256 + 128 + buf * 64; }
 
 // Warps 0 to 7 unpack (four a slot, a quarter of the rows each), 8 to 15 add up, 16 copies, 17 and 18 issue a slot's
-// products.  128256 x 4096, g 64, f16: 85 us for 16 rows, 98 for 48, 102 for 64, bound by the products' number: 16 for a
-// stage of two blocks, some 64 clocks each from tensor memory whatever the columns.
+// products.  128256 x 4096, g 64, f16: 80 us for 16 rows, 95 for 48, 98 for 64, bound by the packed f16 arithmetic that
+// unpacks (64, 81 and 87 without it; half of the products would save 1; twice as many warps that unpack take 5 more).
 template <int P, int GROUP, int COLUMNS>
 __global__ void __launch_bounds__(WIDE_THREADS, 1) q4_wide_kernel(const LogitArgs a) {
   using namespace pesti_umma;
@@ -816,16 +828,13 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) q4_wide_kernel(const LogitArg
             uint32_t v[32];
 #pragma unroll
             for (int j = 2 * h; j < 2 * h + 2; ++j) {
-              const __half2 scale = __float2half2_rn(now.at(i, j * 32 / GROUP) * up);
+              const __half2 scale = __float2half2_rn(now.at(i, j * 32 / GROUP) * up), minus = __hmul2(scale, __float2half2_rn(-24.0f));
 #pragma unroll
               for (int t = 0; t < 4; ++t) {
                 uint32_t q[4];
-                unpack<false>(((const uint32_t*)&w[t])[j], q);
+                unpack_scaled(((const uint32_t*)&w[t])[j], scale, minus, q);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const __half2 x = __hmul2(*(const __half2*)&q[e], scale);
-                  v[16 * (j & 1) + 4 * t + e] = *(const uint32_t*)&x;
-                }
+                for (int e = 0; e < 4; ++e) v[16 * (j & 1) + 4 * t + e] = q[e];
               }
             }
             if (h == 0) {
