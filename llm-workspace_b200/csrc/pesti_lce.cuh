@@ -29,7 +29,9 @@ constexpr int A_BYTES = 128 * BK * 2;
 constexpr int OUT_BYTES = 32 * 128;  // a warp's 32 rows of 128 bytes on their way out
 // Stages that logits are summed over in the tensor cores at once; the sums of several are added in registers.  The
 // cores' own sums are cut off and not rounded, every 16 of K, and always towards 0: over 4096 of K that shrank the
-// largest logits by 5e-6 of themselves, four times as much as in parts of 1024.
+// largest logits by 5e-6 of themselves, four times as much as in parts of 1024.  The gradients' logits are summed in the
+// same parts: p = exp(z - lse) takes its logits to be the very ones that lse was made from.  (Cut otherwise, they left a
+// target's p too small by 1e-4 of itself, which is all of 1 - p of a row with p = 0.9999.)
 constexpr int PART_K = 16;
 constexpr float LOG2E = 1.44269504f;
 
@@ -182,7 +184,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     kn = max(0, min(k_split, k_iters - k0));
   };
 
-  auto parts_of = [&](int kn) { return E == STATS ? (kn + PART_K - 1) / PART_K : 1; };
+  auto parts_of = [&](int kn) { return E == STATS || E == GRAD ? (kn + PART_K - 1) / PART_K : 1; };
 
   if (warp == EPI_WARPS) {
     if (elect_one()) {
@@ -311,13 +313,33 @@ __global__ void __launch_bounds__(THREADS, 1)
       };
 
       // the warp's accumulators, which are free for the next tile but one then
-      uint32_t v[HALF];
+      float v[HALF];
       auto take_acc = [&]() {
         const uint32_t from = wait_acc();
+        uint32_t w[HALF];
 #pragma unroll
-        for (int c = 0; c < HALF; c += 32) tmem_load32(from + c, *(uint32_t(*)[32])(v + c));
+        for (int c = 0; c < HALF; c += 32) tmem_load32(from + c, *(uint32_t(*)[32])(w + c));
         tmem_load_wait();
         leave_acc();
+#pragma unroll
+        for (int j = 0; j < HALF; ++j) v[j] = __uint_as_float(w[j]);
+      };
+      // the same of logits: the sums of their parts
+      auto sum_acc = [&]() {
+        const int parts = parts_of(kn);
+#pragma unroll 1
+        for (int part = 0; part < parts && ok; ++part) {
+          const uint32_t from = wait_acc();
+#pragma unroll
+          for (int c = 0; c < HALF; c += 32) {
+            uint32_t w[32];
+            tmem_load32(from + c, w);
+            tmem_load_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[c + j] = __uint_as_float(w[j]) + (part ? v[c + j] : 0.0f);
+          }
+          leave_acc();
+        }
       };
       // 128 bytes of each of the warp's rows in one of two boxes: written swizzled, so that eight lanes write to eight
       // banks' groups
@@ -352,8 +374,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int j = 0; j < 4; ++j) {
           uint32_t w[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            w[i] = pack2<BF16>(__uint_as_float(v[c + 8 * j + 2 * i]), __uint_as_float(v[c + 8 * j + 2 * i + 1]));
+          for (int i = 0; i < 4; ++i) w[i] = pack2<BF16>(v[c + 8 * j + 2 * i], v[c + 8 * j + 2 * i + 1]);
           put16(c / 64, c % 64 / 8 + j, w[0], w[1], w[2], w[3]);
         }
       };
@@ -361,21 +382,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if constexpr (E == STATS) {
         const bool live = row < active;
         const int t = live ? g.target[row] - col0 : -1;
-        float z[HALF];
-        const int parts = parts_of(kn);
-#pragma unroll 1
-        for (int part = 0; part < parts && ok; ++part) {
-          const uint32_t from = wait_acc();
-#pragma unroll
-          for (int c = 0; c < HALF; c += 32) {
-            uint32_t w[32];
-            tmem_load32(from + c, w);
-            tmem_load_wait();
-#pragma unroll
-            for (int j = 0; j < 32; ++j) z[c + j] = __uint_as_float(w[j]) + (part ? z[c + j] : 0.0f);
-          }
-          leave_acc();
-        }
+        sum_acc();
         float mx = -INFINITY, sum = 0.0f, zs = 0.0f, zt = 0.0f;
         const int left = min(g.V - col0, g.width - half0);  // columns of this half
 #pragma unroll
@@ -384,27 +391,27 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (__any_sync(PESTI_FULL_MASK, t >= c && t < c + 32)) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (t == c + j) zt = z[c + j];
+              if (t == c + j) zt = v[c + j];
           }
           if (c + 32 > left) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (c + j >= left) z[c + j] = -INFINITY;
+              if (c + j >= left) v[c + j] = -INFINITY;
           }
           if (g.zsum) {
             float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int j = 0; j < 32; ++j) a[j & 3] += c + j < left ? z[c + j] : 0.0f;
+            for (int j = 0; j < 32; ++j) a[j & 3] += c + j < left ? v[c + j] : 0.0f;
             zs += (a[0] + a[1]) + (a[2] + a[3]);
           }
           float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int j = 0; j < 32; ++j) most[j & 3] = fmaxf(most[j & 3], z[c + j]);
+          for (int j = 0; j < 32; ++j) most[j & 3] = fmaxf(most[j & 3], v[c + j]);
           const float now = fmaxf(mx, fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * LOG2E);
           const float ref = now == -INFINITY ? 0.0f : now;
           float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int j = 0; j < 32; ++j) a[j & 3] += ex2(fmaf(z[c + j], LOG2E, -ref));
+          for (int j = 0; j < 32; ++j) a[j & 3] += ex2(fmaf(v[c + j], LOG2E, -ref));
           sum = sum * ex2(mx - ref) + ((a[0] + a[1]) + (a[2] + a[3]));
           mx = now;
         }
@@ -433,6 +440,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         pair_ph ^= 1;
         if (!ok) atomicExch(&g.plan->failed, 1);
       } else if constexpr (E == GRAD) {
+        sum_acc();
         const bool live = row < active;
         RowCoef k = {0.0f, 0.0f, 0.0f, 0.0f};
         int t = -1;
@@ -441,23 +449,22 @@ __global__ void __launch_bounds__(THREADS, 1)
           t = g.target[row] - (g.v0 + col0);
         }
         const float c1 = k.c1 * scale, c2 = k.c2 * scale, c3 = k.c3 * scale;
-        take_acc();
         begin_out();
 #pragma unroll
         for (int c = 0; c < HALF; c += 32) {
 #pragma unroll
           for (int j = c; j < c + 32; ++j) {
-            const float p = ex2(fmaf(__uint_as_float(v[j]), LOG2E, -k.c));
-            v[j] = __float_as_uint(fmaf(c1, p, -c3));
+            const float p = ex2(fmaf(v[j], LOG2E, -k.c));
+            v[j] = fmaf(c1, p, -c3);
           }
           if (__any_sync(PESTI_FULL_MASK, t >= c && t < c + 32)) {
 #pragma unroll
             for (int j = c; j < c + 32; ++j)
-              if (t == j) v[j] = __float_as_uint(__uint_as_float(v[j]) - c2);
+              if (t == j) v[j] -= c2;
           }
           if (!live) {
 #pragma unroll
-            for (int j = c; j < c + 32; ++j) v[j] = 0;
+            for (int j = c; j < c + 32; ++j) v[j] = 0.0f;
           }
           put_pairs(c);
         }
@@ -469,7 +476,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int c = 0; c < HALF; c += 32) {
 #pragma unroll
-            for (int j = c; j < c + 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) - rounded<BF16>(__uint_as_float(v[j])));
+            for (int j = c; j < c + 32; ++j) v[j] -= rounded<BF16>(v[j]);
             put_pairs(c);
           }
           end_out(col0, col0 + 64, TWICE + warp_row, false);
@@ -480,7 +487,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int c = 0; c < HALF; c += 32) {
 #pragma unroll
-          for (int j = c; j < c + 32; ++j) v[j] = kn ? __float_as_uint(__uint_as_float(v[j]) * scale) : 0u;
+          for (int j = c; j < c + 32; ++j) v[j] = kn ? v[j] * scale : 0.0f;
           put_pairs(c);
         }
         end_out(col0, col0 + 64, g.v0 + warp_row, false);
@@ -493,7 +500,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               const int i = c + 4 * j;
-              put16(j / 8, j % 8, kn ? v[i] : 0u, kn ? v[i + 1] : 0u, kn ? v[i + 2] : 0u, kn ? v[i + 3] : 0u);
+              put16(j / 8, j % 8, kn ? __float_as_uint(v[i]) : 0u, kn ? __float_as_uint(v[i + 1]) : 0u,
+                    kn ? __float_as_uint(v[i + 2]) : 0u, kn ? __float_as_uint(v[i + 3]) : 0u);
             }
             end_out(col0 + c, col0 + c + 32, split * g.plan->part_rows + warp_row, g.add != 0);
           }
