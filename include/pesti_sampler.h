@@ -506,7 +506,9 @@ int pesti_distill_topk_backward(const void* d_logits, pesti_dtype dtype, int64_t
  *   G_v  = up w [ (1 + 2 z_loss lse) exp(z_v - lse) - (1 - label_smoothing) [v = t]
  *              - label_smoothing / V ]
  *   grad_hidden = G head,  grad_head = G^T hidden      (in the inputs' type)
- * Products are summed in f32, the rows' sums of exponentials joined in 64 bits;
+ * Products are summed in f32 (logits of loss and gradients in the same order), a
+ * row's exponentials without its target's, joined in 64 bits, so that losses of
+ * targets of probability near 1 are exact relative to themselves;
  * G is rounded once to the inputs' type, or (up to 64 rows) held as the sum of two
  * such values (F16: times a power of two that brings its largest value to about
  * 2^14; what is 2^38 below that is lost).  Logits
@@ -518,6 +520,10 @@ int pesti_distill_topk_backward(const void* d_logits, pesti_dtype dtype, int64_t
  * gh_ld], d_grad_head [V, gw_ld] (16-byte aligned, gw_ld a multiple of 8).
  * pesti_linear_ce_backward: the gradients of sum_n d_up[n*up_stride] * loss_n
  * (up_stride 0: one value for all rows) from the forward call's inputs and lse.
+ * G_t of that lse, an f32, is off by up to 2^-22 (1 + |lse|) w up.  The two _nll
+ * calls pass on d_nll [N] f32 besides (lse - z_t, 0 for padding; NULL: as without),
+ * from which G_t is exact relative to itself, as it is in the gradients of
+ * pesti_linear_ce.
  * Outputs overlap neither inputs nor one another.  d_ws: device scratch of
  * pesti_linear_ce_workspace(...) bytes for what the call computes (passes:
  * PESTI_LINEAR_CE_FORWARD, _GRADS, or both), 256-byte aligned, any contents;
@@ -539,6 +545,17 @@ int pesti_linear_ce_backward(const void* d_hidden, pesti_dtype dtype, int64_t N,
                              const float* d_weight, double label_smoothing, double z_loss, const float* d_lse,
                              const float* d_up, int64_t up_stride, void* d_grad_hidden, int64_t gh_ld,
                              void* d_grad_head, int64_t gw_ld, void* d_ws, int64_t ws_bytes, void* stream);
+int pesti_linear_ce_nll(const void* d_hidden, pesti_dtype dtype, int64_t N, int64_t D, int64_t h_ld,
+                        const void* d_head, int64_t V, int64_t w_ld, const void* d_target, int target_bytes,
+                        const float* d_weight, double label_smoothing, double z_loss, float* d_loss, float* d_lse,
+                        float* d_nll, void* d_grad_hidden, int64_t gh_ld, void* d_grad_head, int64_t gw_ld, void* d_ws,
+                        int64_t ws_bytes, void* stream);
+int pesti_linear_ce_nll_backward(const void* d_hidden, pesti_dtype dtype, int64_t N, int64_t D, int64_t h_ld,
+                                 const void* d_head, int64_t V, int64_t w_ld, const void* d_target, int target_bytes,
+                                 const float* d_weight, double label_smoothing, double z_loss, const float* d_lse,
+                                 const float* d_nll, const float* d_up, int64_t up_stride, void* d_grad_hidden,
+                                 int64_t gh_ld, void* d_grad_head, int64_t gw_ld, void* d_ws, int64_t ws_bytes,
+                                 void* stream);
 
 /*
  * The vocabulary projection's weight in 4 bits with group scales, and logits

@@ -242,11 +242,12 @@ RowArgs row_args(const Call& c, const Layout& l, int cg, int sms) {
   return r;
 }
 
-GemmArgs gemm_args(const Layout& l, bool twice) {
+GemmArgs gemm_args(const Layout& l, bool twice, bool whole = false) {
   GemmArgs g = {};
   g.plan = l.plan;
   g.a_box = 128;
   g.twice = twice;
+  g.whole = whole;
   g.target = l.packed;
   g.rows_pad = l.rows_pad;
   g.coef = l.coef;
@@ -306,7 +307,7 @@ int backward(const Call& c, const Layout& l, RowArgs r, void* dh, int64_t dh_ld,
     if (!rc) rc = pesti_tensor_map(&grad_k, pesti_map_type(c.dtype), l.grad, width, l.rows_pad, l.cut.piece * 2, 64, a_box(c.N));
     if (!rc) rc = pesti_tensor_map(&grad_mn, pesti_map_type(c.dtype), l.grad, width, l.rows_pad, l.cut.piece * 2, 64, 64);
     if (rc) return rc;
-    GemmArgs g = gemm_args(l, r.twice);  // G of this piece
+    GemmArgs g = gemm_args(l, r.twice, !r.lse_in || r.nll_in);  // G of this piece
     g.m_tiles = -1;
     g.a_box = a_box(c.N);
     g.n_tiles = (int)((width + BN - 1) / BN);
@@ -400,13 +401,34 @@ int pesti_linear_ce(const void* d_hidden, pesti_dtype dtype, int64_t N, int64_t 
                     int64_t V, int64_t w_ld, const void* d_target, int target_bytes, const float* d_weight,
                     double label_smoothing, double z_loss, float* d_loss, float* d_lse, void* d_grad_hidden,
                     int64_t gh_ld, void* d_grad_head, int64_t gw_ld, void* d_ws, int64_t ws_bytes, void* stream) {
+  return pesti_linear_ce_nll(d_hidden, dtype, N, D, h_ld, d_head, V, w_ld, d_target, target_bytes, d_weight,
+                             label_smoothing, z_loss, d_loss, d_lse, nullptr, d_grad_hidden, gh_ld, d_grad_head, gw_ld,
+                             d_ws, ws_bytes, stream);
+}
+
+int pesti_linear_ce_backward(const void* d_hidden, pesti_dtype dtype, int64_t N, int64_t D, int64_t h_ld,
+                             const void* d_head, int64_t V, int64_t w_ld, const void* d_target, int target_bytes,
+                             const float* d_weight, double label_smoothing, double z_loss, const float* d_lse,
+                             const float* d_up, int64_t up_stride, void* d_grad_hidden, int64_t gh_ld,
+                             void* d_grad_head, int64_t gw_ld, void* d_ws, int64_t ws_bytes, void* stream) {
+  return pesti_linear_ce_nll_backward(d_hidden, dtype, N, D, h_ld, d_head, V, w_ld, d_target, target_bytes, d_weight,
+                                      label_smoothing, z_loss, d_lse, nullptr, d_up, up_stride, d_grad_hidden, gh_ld,
+                                      d_grad_head, gw_ld, d_ws, ws_bytes, stream);
+}
+
+int pesti_linear_ce_nll(const void* d_hidden, pesti_dtype dtype, int64_t N, int64_t D, int64_t h_ld,
+                        const void* d_head, int64_t V, int64_t w_ld, const void* d_target, int target_bytes,
+                        const float* d_weight, double label_smoothing, double z_loss, float* d_loss, float* d_lse,
+                        float* d_nll, void* d_grad_hidden, int64_t gh_ld, void* d_grad_head, int64_t gw_ld, void* d_ws,
+                        int64_t ws_bytes, void* stream) {
   const Call c = {d_hidden, dtype, N, D, h_ld, d_head, V, w_ld, d_target, target_bytes, d_weight, label_smoothing,
                   z_loss};
   int rc = check(c);
   if (rc) return rc;
   if (N == 0 && !d_grad_head) return PESTI_OK;
   if (N && !d_loss) return refuse("null loss");
-  if ((uintptr_t)d_loss % 4 || (uintptr_t)d_lse % 4) return refuse("loss or lse is not aligned to its type");
+  if ((uintptr_t)d_loss % 4 || (uintptr_t)d_lse % 4 || (uintptr_t)d_nll % 4)
+    return refuse("loss or lse is not aligned to its type");
   const bool grads = d_grad_hidden || d_grad_head;
   if (grads) {
     rc = check_grads(c, d_grad_hidden, gh_ld, d_grad_head, gw_ld);
@@ -429,6 +451,7 @@ int pesti_linear_ce(const void* d_hidden, pesti_dtype dtype, int64_t N, int64_t 
   RowArgs r = row_args(c, l, cg, dev.sms);
   r.loss = d_loss;
   r.lse = d_lse;
+  r.nll = d_nll;
   rc = pack<false>(r, st);
   if (rc) return rc;
   const bool bf16 = dtype == PESTI_BF16;
@@ -438,11 +461,12 @@ int pesti_linear_ce(const void* d_hidden, pesti_dtype dtype, int64_t N, int64_t 
   return backward(c, l, r, cg, d_grad_hidden, gh_ld, d_grad_head, gw_ld, dev, st);
 }
 
-int pesti_linear_ce_backward(const void* d_hidden, pesti_dtype dtype, int64_t N, int64_t D, int64_t h_ld,
-                             const void* d_head, int64_t V, int64_t w_ld, const void* d_target, int target_bytes,
-                             const float* d_weight, double label_smoothing, double z_loss, const float* d_lse,
-                             const float* d_up, int64_t up_stride, void* d_grad_hidden, int64_t gh_ld,
-                             void* d_grad_head, int64_t gw_ld, void* d_ws, int64_t ws_bytes, void* stream) {
+int pesti_linear_ce_nll_backward(const void* d_hidden, pesti_dtype dtype, int64_t N, int64_t D, int64_t h_ld,
+                                 const void* d_head, int64_t V, int64_t w_ld, const void* d_target, int target_bytes,
+                                 const float* d_weight, double label_smoothing, double z_loss, const float* d_lse,
+                                 const float* d_nll, const float* d_up, int64_t up_stride, void* d_grad_hidden,
+                                 int64_t gh_ld, void* d_grad_head, int64_t gw_ld, void* d_ws, int64_t ws_bytes,
+                                 void* stream) {
   const Call c = {d_hidden, dtype, N, D, h_ld, d_head, V, w_ld, d_target, target_bytes, d_weight, label_smoothing,
                   z_loss};
   int rc = check(c);
@@ -451,7 +475,8 @@ int pesti_linear_ce_backward(const void* d_hidden, pesti_dtype dtype, int64_t N,
   if (!d_grad_hidden && !d_grad_head) return refuse("no gradient is asked for");
   if (N == 0 && !d_grad_head) return PESTI_OK;
   if (N && (!d_lse || !d_up)) return refuse("null lse or upstream gradient");
-  if ((uintptr_t)d_lse % 4 || (uintptr_t)d_up % 4) return refuse("lse or upstream gradient is not aligned to its type");
+  if ((uintptr_t)d_lse % 4 || (uintptr_t)d_nll % 4 || (uintptr_t)d_up % 4)
+    return refuse("lse or upstream gradient is not aligned to its type");
   rc = check_grads(c, d_grad_hidden, gh_ld, d_grad_head, gw_ld);
   if (rc) return rc;
   Device dev = {};
@@ -470,6 +495,7 @@ int pesti_linear_ce_backward(const void* d_hidden, pesti_dtype dtype, int64_t N,
   const int cg = blocks_per_tile(N);
   RowArgs r = row_args(c, l, cg, dev.sms);
   r.lse_in = d_lse;
+  r.nll_in = d_nll;
   r.up = d_up;
   r.up_stride = up_stride;
   rc = pack<true>(r, st);

@@ -4,6 +4,11 @@
 //   G = dloss/dz = c1 p - c2 [v = t] - c3,  c1 = a up (1 + 2 zeta lse), c2 = a up (1 - eps), c3 = a up eps / V
 //   dh = G W,  dW = G^T h
 //
+// Where p_t is near 1, neither lse - z_t nor c1 p_t - c2 is left much of in f32.  So a row's other logits are summed
+// without the target's, and from r = (their sum) / exp z_t come
+//   -log p_t = log(1 + r),  G_t = a up [(1 + 2 zeta lse) (p_t - 1) + 2 zeta lse + eps - eps / V],  p_t - 1 = -r / (1 + r)
+// as exact, relative to themselves, as r is.
+//
 // Three products of one size each way, and the logits' product again, since they are not kept: 8 N V D operations
 // with gradients.  All four run in head_gemm_kernel, which differs in its operands' majors and in what becomes of the
 // accumulators.
@@ -47,7 +52,8 @@ struct Plan {
 };
 
 struct RowCoef {
-  float c, c1, c2, c3;  // p = 2^(z log2e - c)
+  float c, c1, c3;  // p = 2^(z log2e - c)
+  float target;     // G_t, or what p_t's part of it lacks, -c2
 };
 
 enum Epilogue { STATS, GRAD, OUT16, PART32 };
@@ -77,11 +83,12 @@ struct GemmArgs {
   // STATS and GRAD
   const int* target;  // [rows], of the packed rows
   int v0, V;          // GRAD: the tiles' first token; the vocabulary
-  float2* parts;      // [tiles, rows_pad] (maximum, sum) of a tile's logits, in powers of two
+  float2* parts;      // [tiles, rows_pad] (maximum, sum) of a tile's logits but the target's, in powers of two
   float* zsum;        // [tiles, rows_pad] their plain sum, or null
   float* zt;          // [rows] the target's logit
   long long rows_pad;
   const RowCoef* coef;
+  int whole;          // GRAD: the coefficients have G_t
   int add;            // PART32: add to what is there
   int out_x, out_y;   // where the output ends
   int width;          // columns of a tile (STATS: a multiple of 16)
@@ -388,7 +395,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int c = 0; c < HALF; c += 32) {
           if (c >= left) continue;
-          if (__any_sync(PESTI_FULL_MASK, t >= c && t < c + 32)) {
+          const bool here = __any_sync(PESTI_FULL_MASK, t >= c && t < c + 32);
+          if (here) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
               if (t == c + j) zt = v[c + j];
@@ -403,6 +411,11 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int j = 0; j < 32; ++j) a[j & 3] += c + j < left ? v[c + j] : 0.0f;
             zs += (a[0] + a[1]) + (a[2] + a[3]);
+          }
+          if (here) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (t == c + j) v[c + j] = -INFINITY;
           }
           float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -442,13 +455,13 @@ __global__ void __launch_bounds__(THREADS, 1)
       } else if constexpr (E == GRAD) {
         sum_acc();
         const bool live = row < active;
-        RowCoef k = {0.0f, 0.0f, 0.0f, 0.0f};
+        RowCoef k = {};
         int t = -1;
         if (live) {
           k = g.coef[row];
           t = g.target[row] - (g.v0 + col0);
         }
-        const float c1 = k.c1 * scale, c2 = k.c2 * scale, c3 = k.c3 * scale;
+        const float c1 = k.c1 * scale, c3 = k.c3 * scale, target = k.target * scale;
         begin_out();
 #pragma unroll
         for (int c = 0; c < HALF; c += 32) {
@@ -460,7 +473,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (__any_sync(PESTI_FULL_MASK, t >= c && t < c + 32)) {
 #pragma unroll
             for (int j = c; j < c + 32; ++j)
-              if (t == j) v[j] -= c2;
+              if (t == j) v[j] = (g.whole ? 0.0f : v[j]) + target;
           }
           if (!live) {
 #pragma unroll
@@ -541,8 +554,10 @@ struct RowArgs {
   int tiles;
   float* loss;
   float* lse;
+  float* nll;
   // backward
   const float* lse_in;
+  const float* nll_in;  // or null
   const float* up;
   long long up_stride;
   // finish
@@ -555,17 +570,21 @@ struct RowArgs {
   long long dh_ld;
 };
 
-__device__ __forceinline__ RowCoef coef_of(const RowArgs& a, float factor, float lse) {
+// The coefficients of a row's gradient (nll: -log p_t, or less than 0: unknown), and an f32 that no |G| exceeds.
+__device__ __forceinline__ RowCoef coef_of(const RowArgs& a, float factor, float lse, double nll, unsigned& bound) {
   RowCoef k;
   k.c = lse * LOG2E;
   k.c1 = factor * fmaf(2.0f * a.zeta, lse, 1.0f);
-  k.c2 = factor * (1.0f - a.eps);
   k.c3 = factor * a.eps / (float)a.V;
+  const float c2 = factor * (1.0f - a.eps);
+  if (nll < 0.0) {
+    k.target = -c2;
+  } else {
+    const double z2 = 2.0 * a.zeta * lse, eps = a.eps;
+    k.target = (float)(factor * ((1.0 + z2) * expm1(-nll) + z2 + eps - eps / (double)a.V));
+  }
+  bound = __float_as_uint(fabsf(k.c1) + fabsf(c2) + fabsf(k.c3));
   return k;
-}
-
-__device__ __forceinline__ unsigned bound_of(const RowCoef& k) {
-  return __float_as_uint(fabsf(k.c1) + fabsf(k.c2) + fabsf(k.c3));
 }
 
 // Into how many ranges the hidden states' gradient cuts a piece's K.  Its time in stages of a tile (64 of K, 0.28 us):
@@ -631,6 +650,7 @@ __global__ void __launch_bounds__(PACK_ROWS) lce_pack_kernel(const RowArgs a) {
       if (!BACKWARD && !live) {
         a.loss[n] = 0.0f;
         if (a.lse) a.lse[n] = 0.0f;
+        if (a.nll) a.nll[n] = 0.0f;
       }
     }
     if (live) {
@@ -639,9 +659,9 @@ __global__ void __launch_bounds__(PACK_ROWS) lce_pack_kernel(const RowArgs a) {
         a.idx[at] = (int)n;
         a.packed[at] = (int)t;
         if (BACKWARD) {
-          const RowCoef k = coef_of(a, w * a.up[n * a.up_stride], a.lse_in[n]);
-          a.coef[at] = k;
-          bound = max(bound, bound_of(k));
+          unsigned most_of;
+          a.coef[at] = coef_of(a, w * a.up[n * a.up_stride], a.lse_in[n], a.nll_in ? (double)a.nll_in[n] : -1.0, most_of);
+          bound = max(bound, most_of);
         }
       }
     }
@@ -726,17 +746,22 @@ __global__ void __launch_bounds__(256) lce_join_kernel(const RowArgs a) {
     z += sz[w][r];
   }
   const int n = a.idx[i];
-  const double lse = ((double)m + log2(s)) / (double)LOG2E;
+  // log2 of the others' sum, and how far it is above the target's logit
+  const double zt = a.zt[i], rest = (double)m + log2(s), over = rest - zt * (double)LOG2E;
+  const double log1p_r = log1p(exp2(-fabs(over)));
+  double nll = over > 0.0 ? over / (double)LOG2E + log1p_r : log1p_r;
+  if (zt == (double)INFINITY || a.plan->failed) nll = NAN;
+  const double lse = over > 0.0 ? rest / (double)LOG2E + log1p_r : zt + nll, eps = a.eps;
   const float w = a.weight ? a.weight[n] : 1.0f;
-  double loss = lse - (double)(1.0f - a.eps) * a.zt[i] + (double)a.zeta * lse * lse;
-  if (a.eps != 0.0f) loss -= (double)a.eps * z / (double)a.V;
-  if (a.plan->failed) loss = NAN;
+  double loss = (1.0 - eps) * nll + (double)a.zeta * lse * lse;
+  if (a.eps != 0.0f) loss += eps * (lse - z / (double)a.V);
   a.loss[n] = (float)(w * loss);
   if (a.lse) a.lse[n] = (float)lse;
+  if (a.nll) a.nll[n] = (float)nll;
   if (GRADS) {
-    const RowCoef k = coef_of(a, w, (float)lse);
-    a.coef[i] = k;
-    atomicMax(&a.plan->gmax, bound_of(k));
+    unsigned bound;
+    a.coef[i] = coef_of(a, w, (float)lse, nll, bound);
+    atomicMax(&a.plan->gmax, bound);
   }
 }
 

@@ -71,19 +71,19 @@ def _rows_like(t, rows: int, D: int):
     return t.new_empty((rows, D)) if D % 8 == 0 else t.new_empty((rows, -(-D // 8) * 8))[:, :D]
 
 
-def _ce_forward(args, like, lse: bool, grads: bool, st):
+def _ce_forward(args, like, keep: bool, grads: bool, st):
     dtype, N, D, V = args[1], args[2], args[3], args[6]
     loss = like.new_empty(N, dtype=torch.float32)
-    lse = like.new_empty(N, dtype=torch.float32) if lse else None
+    lse, nll = (like.new_empty(N, dtype=torch.float32) for _ in range(2)) if keep else (None, None)
     gh = like.new_empty((N, D)) if grads else None
     gw = _rows_like(like, V, D) if grads else None
     need = _ce_workspace(dtype, N, V, D, _FORWARD | _GRADS if grads else _FORWARD)
     ws = like.new_empty(need, dtype=torch.uint8)
-    rc = load_library().pesti_linear_ce(*args, loss.data_ptr(), _ptr(lse), _ptr(gh), D, _ptr(gw), -(-D // 8) * 8,
-                                        ws.data_ptr(), need, st)
+    rc = load_library().pesti_linear_ce_nll(*args, loss.data_ptr(), _ptr(lse), _ptr(nll), _ptr(gh), D, _ptr(gw),
+                                            -(-D // 8) * 8, ws.data_ptr(), need, st)
     if rc:
         _check(rc)
-    return loss, lse, gh, gw
+    return loss, lse, nll, gh, gw
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
@@ -91,19 +91,19 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def forward(ctx, hidden, head, target, weight, label_smoothing, z_loss):
         args = _ce_args(hidden, head, target, weight, label_smoothing, z_loss)
         keep = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
-        loss, lse, _, _ = _launch(hidden.device, None, lambda st: _ce_forward(args, hidden, keep, False, st))
+        loss, lse, nll, _, _ = _launch(hidden.device, None, lambda st: _ce_forward(args, hidden, keep, False, st))
         if keep:
             ctx.more = label_smoothing, z_loss
-            ctx.save_for_backward(hidden, head, target, weight, lse)
+            ctx.save_for_backward(hidden, head, target, weight, lse, nll)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, up):
         # hooks (activation checkpointing, offloading) may hand back tensors at other addresses and of other strides
-        hidden, head, target, weight, lse = ctx.saved_tensors
+        hidden, head, target, weight, lse, nll = ctx.saved_tensors
         args = _ce_args(hidden, head, target, weight, *ctx.more)
-        lse = lse.contiguous()
+        lse, nll = lse.contiguous(), nll.contiguous()
         if up.dtype != torch.float32:
             up = up.to(torch.float32)
         dtype, N, D, V = args[1], args[2], args[3], args[6]
@@ -113,8 +113,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
             gw = _rows_like(head, V, D) if ctx.needs_input_grad[1] else None
             need = _ce_workspace(dtype, N, V, D, _GRADS)
             ws = hidden.new_empty(need, dtype=torch.uint8)
-            rc = load_library().pesti_linear_ce_backward(
-                *args, lse.data_ptr(), up.data_ptr(), up.stride(0), _ptr(gh), D, _ptr(gw), -(-D // 8) * 8,
+            rc = load_library().pesti_linear_ce_nll_backward(
+                *args, lse.data_ptr(), nll.data_ptr(), up.data_ptr(), up.stride(0), _ptr(gh), D, _ptr(gw), -(-D // 8) * 8,
                 ws.data_ptr(), need, st)
             if rc:
                 _check(rc)
@@ -146,7 +146,7 @@ def linear_cross_entropy_grad(hidden, head, target, weight=None, label_smoothing
     mask)."""
     hidden, head = hidden.detach(), head.detach()
     args = _ce_args(hidden, head, target, weight, label_smoothing, z_loss)
-    loss, _, gh, gw = _launch(hidden.device, stream, lambda st: _ce_forward(args, hidden, False, True, st))
+    loss, _, _, gh, gw = _launch(hidden.device, stream, lambda st: _ce_forward(args, hidden, False, True, st))
     return loss, gh, gw
 
 

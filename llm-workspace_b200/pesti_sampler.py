@@ -159,6 +159,10 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.pesti_linear_ce.restype = c_int
     lib.pesti_linear_ce_backward.argtypes = head + [vp, vp, i64, vp, i64, vp, i64, vp, i64, vp]
     lib.pesti_linear_ce_backward.restype = c_int
+    lib.pesti_linear_ce_nll.argtypes = head + [vp, vp, vp, vp, i64, vp, i64, vp, i64, vp]
+    lib.pesti_linear_ce_nll.restype = c_int
+    lib.pesti_linear_ce_nll_backward.argtypes = head + [vp, vp, vp, i64, vp, i64, vp, i64, vp, i64, vp]
+    lib.pesti_linear_ce_nll_backward.restype = c_int
     lib.pesti_q4_quantize.argtypes = [vp, c_int, i64, i64, i64, i64, vp, vp, vp]
     lib.pesti_q4_quantize.restype = c_int
     lib.pesti_q4_dequantize.argtypes = [vp, vp, i64, i64, i64, vp, c_int, i64, vp]

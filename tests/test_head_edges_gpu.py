@@ -80,3 +80,90 @@ def test_confident_rows(way, dtype, N, V, D):
     and 2^x to f32 (some units of 2^-24 each): 2^-22 (2 + |lse|), at |lse| < 22."""
     doubt = torch.logspace(-2, -4, N, device="cuda")
     _compare(way, *_confident(N, V, D, dtype, doubt), 2.0 ** -22 * 24)
+
+
+def _loss_room(hidden, o):
+    """Bound of -log p_t off its definition, relative to itself: the others' sum over the target's exponential, whose
+    logits are off by d each, whose 2^x by 2^-22, and which some tens of f32 additions make, 2^-19."""
+    D = hidden.shape[1]
+    d = (_step(min(D, PART)) + (D // PART) * 2.0 ** -24) * o["size"]
+    return torch.expm1(2 * d) + 2.0 ** -19
+
+
+@pytest.mark.parametrize("way", ["one call", "autograd"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("N,V,D", [(1, 2001, 4096), (40, 2000, 1000), (48, 30_001, 4096), (200, 3000, 4096), (1100, 2000, 520)])
+def test_very_confident_rows(way, dtype, N, V, D):
+    """1 - p of 1e-2 to 1e-7: losses and gradients are exact relative to themselves, ABS is 0."""
+    doubt = torch.logspace(-7, -2, N, device="cuda")
+    hidden, head, target = _confident(N, V, D, dtype, doubt)
+    o = OH.cross_entropy(hidden, head, target)
+    loss = ph.linear_cross_entropy(hidden, head, target)
+    _check(loss, o["loss"], (_loss_room(hidden, o) + 2.0 ** -24) * o["loss"], "loss")
+    _compare(way, hidden, head, target, 0.0)
+
+
+def test_a_target_of_any_probability():
+    """z_t far above, near and far below the other logits, alone in the vocabulary, and infinite."""
+    V, D = 1500, 64
+    g = torch.Generator(device="cuda").manual_seed(4)
+    head = torch.randn(V, D, generator=g, device="cuda").mul_(0.2).bfloat16()
+    for N in (60, 300):
+        target = torch.randint(0, V, (N,), generator=g, device="cuda")
+        w = head[target].float()
+        hidden = (w * torch.linspace(-60, 60, N, device="cuda")[:, None]).bfloat16()
+        o = OH.cross_entropy(hidden, head, target)
+        got = ph.linear_cross_entropy(hidden, head, target)
+        # (the oracle's own loss is a difference of 64-bit numbers)
+        _check(got, o["loss"], (_loss_room(hidden, o) + 2.0 ** -24) * o["loss"] + 2.0 ** -50 * (1 + o["lse"].abs()), "loss")
+        alone = ph.linear_cross_entropy(hidden, head[:1], torch.zeros_like(target))
+        assert (alone == 0).all()
+        z = hidden.double() @ head[0].double()
+        square = ph.linear_cross_entropy(hidden, head[:1], torch.zeros_like(target), z_loss=0.5, label_smoothing=0.25)
+        # z_t is off by d, and its square by 2 z d; loss rounded once
+        size = (hidden.double().abs() @ head[0].double().abs())
+        assert ((square.double() - 0.5 * z * z).abs() <= z.abs() * _step(D) * size + (_step(D) * size) ** 2 + 2.0 ** -23 * z * z).all()
+    hidden = torch.ones(3, D, device="cuda").bfloat16()
+    head[7] = float("inf")
+    head[8] = -float("inf")
+    loss, gh, _ = ph.linear_cross_entropy_grad(hidden, head, torch.tensor([7, 8, 9], device="cuda"))
+    assert torch.isnan(loss).all()
+    head[7] = 0
+    loss = ph.linear_cross_entropy(hidden, head, torch.tensor([7, 8, 9], device="cuda"))
+    want = -torch.log_softmax(hidden.double() @ head.double().T, 1)[torch.arange(3), torch.tensor([7, 8, 9])]
+    assert loss[1] == float("inf") and torch.allclose(loss[[0, 2]].double(), want[[0, 2]].to(loss.device), rtol=1e-4)
+    smooth = ph.linear_cross_entropy(hidden, head, torch.tensor([7, 8, 9], device="cuda"), label_smoothing=0.1)
+    assert (smooth == float("inf")).all()
+
+
+@pytest.mark.parametrize("eps,zeta", [(0.0, 0.0), (0.1, 1e-3)])
+def test_gradients_of_an_f32_lse(eps, zeta):
+    """pesti_linear_ce and pesti_linear_ce_backward, which pass on no -log p: G_t is off by 2^-22 (1 + |lse|) w up more."""
+    import ctypes
+
+    import pesti_sampler as ps
+    lib = ps.load_library()
+    for N, V, D in ((50, 900, 264), (200, 2000, 520)):
+        hidden, head, target = _confident(N, V, D, "bf16", torch.logspace(-1, -4, N, device="cuda"))
+        weight, up = torch.rand(N, device="cuda") + 0.5, torch.rand(N, device="cuda") + 0.5
+        need = lib.pesti_linear_ce_workspace(ps.PESTI_BF16, N, V, D, 3)
+        ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+        loss, lse = torch.empty(2, N, device="cuda")
+        gh, gw = torch.empty_like(hidden), torch.empty_like(head)
+        args = (hidden.data_ptr(), ps.PESTI_BF16, N, D, D, head.data_ptr(), V, D, target.data_ptr(), 8,
+                weight.data_ptr(), eps, zeta)
+        st = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+        assert lib.pesti_linear_ce(*args, loss.data_ptr(), lse.data_ptr(), None, D, None, D, ws.data_ptr(), need, st) == 0
+        assert lib.pesti_linear_ce_backward(*args, lse.data_ptr(), up.data_ptr(), 1, gh.data_ptr(), D, gw.data_ptr(), D,
+                                            ws.data_ptr(), need, st) == 0
+        o = OH.cross_entropy(hidden, head, target, weight, eps, zeta, up)
+        assert ((lse.double() - o["lse"]).abs() <= _step(D) * o["size"] + 2.0 ** -20 * (1 + o["lse"].abs())).all()
+        o["hot"] = torch.zeros_like(o["G"]).scatter_(1, target[:, None], 1.0)
+        # smoothing and z-loss: sums of parts, each off by some units of 2^-24, beside the target's own
+        dG = _room(hidden, o, 0.0) + 2.0 ** -22 * o["parts"] + o["hot"] * (2.0 ** -22 * (2 + o["lse"].abs()) * weight.double() * up.double())[:, None]
+        dG = dG + torch.expm1(2 * _step(D) * o["size"])[:, None] * o["p"] * (1.0 if eps or zeta else 0.0)
+        half = 2.0 ** -8  # a step of bfloat16's 8 bits of mantissa is 2^-7 of the power of two below a value
+        tol = (dG + _step(V) * (o["G"].abs() + dG)) @ o["abs_head"]
+        _check(gh, o["grad_hidden"], tol + half * (o["grad_hidden"].abs() + tol) + TINY["bf16"], "grad_hidden")
+        tol = (dG + _step(N) * (o["G"].abs() + dG)).T @ o["abs_hidden"]
+        _check(gw, o["grad_head"], tol + half * (o["grad_head"].abs() + tol) + TINY["bf16"], "grad_head")
