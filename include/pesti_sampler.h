@@ -511,7 +511,8 @@ int pesti_distill_topk_backward(const void* d_logits, pesti_dtype dtype, int64_t
  * targets of probability near 1 are exact relative to themselves;
  * G is rounded once to the inputs' type, or (up to 64 rows) held as the sum of two
  * such values (F16: times a power of two that brings its largest value to about
- * 2^14; what is 2^38 below that is lost).  Logits
+ * 2^14, of the rows whose loss and upstream gradient are finite; what is 2^38 below
+ * that is lost).  Logits
  * that are NaN or +inf make their row's loss NaN, and the gradients that the row
  * has part in.
  *

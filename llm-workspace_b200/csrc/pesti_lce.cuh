@@ -45,7 +45,7 @@ __host__ __device__ constexpr int b_bytes(int cg) { return BN / cg * BK * 2; }
 // What the host does not know: written by the plan kernel, on the device.
 struct Plan {
   int active;     // rows with a target and a weight
-  unsigned gmax;  // bits of an f32 that no |G| exceeds (f16 only)
+  unsigned gmax;  // bits of an f32 that no |G| of a row with finite coefficients exceeds (f16 only)
   int splits;     // ranges of K in the hidden states' gradient
   int part_rows;  // rows of a range's part: the active ones, to a whole tile
   int failed;     // a wait gave up
@@ -122,7 +122,7 @@ template <bool BF16>
 __device__ __forceinline__ int grad_shift(const Plan* plan) {
   if (BF16) return 0;
   const float m = __uint_as_float(plan->gmax);
-  if (!(m > 0.0f) || isinf(m)) return 0;
+  if (!(m > 0.0f)) return 0;
   const int s = 14 - ilogbf(m);
   return max(-100, min(100, s));
 }
@@ -570,7 +570,8 @@ struct RowArgs {
   long long dh_ld;
 };
 
-// The coefficients of a row's gradient (nll: -log p_t, or less than 0: unknown), and an f32 that no |G| exceeds.
+// The coefficients of a row's gradient (nll: -log p_t, or less than 0: unknown), and an f32 that no |G| exceeds: 0 where
+// that is not finite, so that such a row takes no part in the power of two that it shares with others.
 __device__ __forceinline__ RowCoef coef_of(const RowArgs& a, float factor, float lse, double nll, unsigned& bound) {
   RowCoef k;
   k.c = lse * LOG2E;
@@ -583,7 +584,8 @@ __device__ __forceinline__ RowCoef coef_of(const RowArgs& a, float factor, float
     const double z2 = 2.0 * a.zeta * lse, eps = a.eps;
     k.target = (float)(factor * ((1.0 + z2) * expm1(-nll) + z2 + eps - eps / (double)a.V));
   }
-  bound = __float_as_uint(fabsf(k.c1) + fabsf(c2) + fabsf(k.c3));
+  const float most = fabsf(k.c1) + fabsf(c2) + fabsf(k.c3);
+  bound = isfinite(most) ? __float_as_uint(most) : 0u;
   return k;
 }
 

@@ -167,3 +167,44 @@ def test_gradients_of_an_f32_lse(eps, zeta):
         _check(gh, o["grad_hidden"], tol + half * (o["grad_hidden"].abs() + tol) + TINY["bf16"], "grad_hidden")
         tol = (dG + _step(N) * (o["G"].abs() + dG)).T @ o["abs_hidden"]
         _check(gw, o["grad_head"], tol + half * (o["grad_head"].abs() + tol) + TINY["bf16"], "grad_head")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("scale", [1e-4, 1.0, 1e5])
+@pytest.mark.parametrize("N", [40, 200, 1100])
+def test_rows_beside_ones_that_are_not_finite(dtype, scale, N):
+    """Rows with NaN or infinite logits, weights or upstream gradients leave the other rows' outputs as they are without
+    them: in f16 too, where G is held times a power of two that all rows share."""
+    g = torch.Generator(device="cuda").manual_seed(N)
+    V, D = 3001, 72
+    head = torch.randn(V, D, generator=g, device="cuda").mul_(1.5 / D ** 0.5).to(DT[dtype])
+    hidden = torch.randn(N, D, generator=g, device="cuda").to(DT[dtype])
+    target = torch.randint(0, V, (N,), generator=g, device="cuda")
+    weight = scale * (0.5 + torch.rand(N, generator=g, device="cuda"))
+    up = 0.5 + torch.rand(N, generator=g, device="cuda")
+    bad = torch.zeros(N, dtype=torch.bool, device="cuda")
+    bad[[7, 20, 33]] = True
+    clean = torch.where(bad, -1, target)
+    ill = weight.clone()
+    ill[33] = float("inf")
+    dirty = hidden.clone()
+    dirty[7, 3], dirty[20, 0] = float("nan"), float("inf")
+    want = ph.linear_cross_entropy_grad(hidden, head, clean, weight)
+    loss, gh, _ = ph.linear_cross_entropy_grad(dirty, head, target, ill)
+    assert torch.isnan(loss[[7, 20]]).all() and not torch.isfinite(loss[33])
+    assert torch.equal(loss[~bad], want[0][~bad]) and torch.equal(gh[~bad], want[1][~bad])
+    o = OH.cross_entropy(hidden, head, clean, weight)
+    if dtype == "bf16" or scale < 1e4:
+        assert torch.isfinite(gh[~bad].float()).all()
+        assert ((gh.double() - o["grad_hidden"]).norm(dim=1) <= 2.0 ** -7 * o["grad_hidden"].norm(dim=1))[~bad].all()
+
+    def backward(h, t, w, u):
+        x, y = h.detach().requires_grad_(), head.detach().requires_grad_()
+        return torch.autograd.grad(ph.linear_cross_entropy(x, y, t, w), (x, y), u)
+
+    u2 = up.clone()
+    u2[20] = float("nan")
+    u2[33] = float("inf")
+    want = backward(hidden, clean, weight, up)
+    got = backward(dirty, target, weight, u2)
+    assert torch.equal(got[0][~bad], want[0][~bad])
