@@ -100,10 +100,17 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, up):
-        # hooks (activation checkpointing, offloading) may hand back tensors at other addresses and of other strides
         hidden, head, target, weight, lse, nll = ctx.saved_tensors
+        # hooks (activation checkpointing, offloading) may hand back tensors at other addresses and of other strides: without
+        # the room behind the rows of a head whose D is no multiple of 8, for one
+        if hidden.stride(1) != 1:
+            hidden = hidden.contiguous()
+        if head.stride(1) != 1 or head.stride(0) % 8 or head.data_ptr() % 16:
+            head = _rows_like(head, *head.shape).copy_(head)
+        target, lse, nll = target.contiguous(), lse.contiguous(), nll.contiguous()
+        if weight is not None:
+            weight = weight.contiguous()
         args = _ce_args(hidden, head, target, weight, *ctx.more)
-        lse, nll = lse.contiguous(), nll.contiguous()
         if up.dtype != torch.float32:
             up = up.to(torch.float32)
         dtype, N, D, V = args[1], args[2], args[3], args[6]

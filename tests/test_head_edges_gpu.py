@@ -6,6 +6,8 @@ are summed at once, and an addition for each part) change each G but the target'
 of at most expm1(2 d), beside 2^-22 for the hardware's 2^x and 2^-22 (1 + |lse|)
 for lse and its product with log2(e) in f32, and so does G_t = p_t - 1, minus the sum of the others, if the logits are
 the very ones that are in lse.  All further errors of p_t are absolute: ABS."""
+import contextlib
+
 import pytest
 import torch
 
@@ -208,3 +210,53 @@ def test_rows_beside_ones_that_are_not_finite(dtype, scale, N):
     want = backward(hidden, clean, weight, up)
     got = backward(dirty, target, weight, u2)
     assert torch.equal(got[0][~bad], want[0][~bad])
+
+
+@pytest.mark.parametrize("pin", [False, True])
+@pytest.mark.parametrize("V,D", [(300, 1001), (1, 1001), (300, 1000), (37, 1)])
+def test_saved_on_the_host(V, D, pin):
+    """Saved tensors come back without the room behind their rows."""
+    g = torch.Generator(device="cuda").manual_seed(D)
+    N = 50
+    room = torch.full((V, -(-D // 8) * 8), float("nan"), device="cuda").bfloat16()
+    head = room[:, :D].copy_(torch.randn(V, D, generator=g, device="cuda") / D ** 0.5)
+    hidden = torch.randn(N, D, generator=g, device="cuda").bfloat16()
+    target = torch.randint(0, V, (N,), generator=g, device="cuda")
+    weight, up = torch.rand(2, N, generator=g, device="cuda")
+
+    def gradient(saved):
+        x, y = hidden.detach().requires_grad_(), head.detach().requires_grad_()
+        with saved:
+            loss = ph.linear_cross_entropy(x, y, target, weight)
+        return torch.autograd.grad(loss, (x, y), up)
+
+    want = gradient(contextlib.nullcontext())
+    got = gradient(torch.autograd.graph.save_on_cpu(pin_memory=pin))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_saved_elsewhere():
+    """A head that comes back at another alignment, or by columns."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    N, V, D = 30, 200, 64
+    head = (torch.randn(V, D, generator=g, device="cuda") / 8).bfloat16()
+    hidden = torch.randn(N, D, generator=g, device="cuda").bfloat16()
+    target = torch.randint(0, V, (N,), generator=g, device="cuda")
+
+    def moved(t):
+        t = t.detach()
+        return t.new_empty(t.numel() + 4)[4:].copy_(t.reshape(-1)).view(t.shape)
+
+    def turned(t):
+        t = t.detach()
+        return t.t().contiguous().t() if t.dim() == 2 else t.clone()
+
+    def gradient(pack):
+        x, y = hidden.detach().requires_grad_(), head.detach().requires_grad_()
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+            loss = ph.linear_cross_entropy(x, y, target)
+        return torch.autograd.grad(loss.sum(), (x, y))
+
+    want = gradient(lambda t: t)
+    for pack in (moved, turned):
+        assert all(torch.equal(a, b) for a, b in zip(gradient(pack), want))
