@@ -58,6 +58,16 @@ typedef struct {
 } pesti_testing_plan;
 int pesti_testing_beam_plan(pesti_dtype dtype, int64_t G, int64_t W, int64_t V, int64_t K, int sms,
                             pesti_testing_plan* plan);
+
+/* What the vocabulary projection's tensor core kernels do when a wait on the
+ * device gives up (which no sound run's does): from the next launch on, each
+ * block takes the sums of its `round`-th tile (from 0) as if its wait for them had,
+ * in the cross entropy's product `product` (0 logits, 1 G, 2 the head's gradient,
+ * 3 the hidden states') or the 4-bit logits of more than 8 rows (4).  round -1:
+ * in none, the default.  The block's other waits then run out for real, within a
+ * second or two; what it has not finished comes out as NaN.  Process-wide; for
+ * tests. */
+int pesti_testing_give_up(int product, int round);
 #ifdef __cplusplus
 }
 #endif

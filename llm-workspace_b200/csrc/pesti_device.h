@@ -24,6 +24,14 @@ static inline int pesti_current_device(int& device, int& sms) {
   return PESTI_OK;
 }
 
+// For tests (pesti_testing_give_up): the product whose sums are taken as if a wait for them had given up, and the round.
+constexpr int PESTI_Q4_SUMS = 4;  // 0 to 3: the epilogues of the cross entropy's products
+inline std::atomic<int64_t> pesti_give_up_at{0xffffffffLL};
+static inline int pesti_give_up(int product) {
+  const int64_t at = pesti_give_up_at.load(std::memory_order_relaxed);
+  return at >> 32 == product ? (int)(uint32_t)at : -1;
+}
+
 // Lets `kernel` have `bytes` of dynamic shared memory on `device`; `had` is the kernel's own record of what it may have.
 struct PestiShared {
   std::atomic<int> bytes[PESTI_MOST_DEVICES];

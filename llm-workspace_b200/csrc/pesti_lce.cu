@@ -6,6 +6,7 @@
 #include <cmath>
 
 #include "../../include/pesti_sampler.h"
+#include "../../include/pesti_testing.h"
 #include "pesti_device.h"
 #include "pesti_error.h"
 #include "pesti_lce.cuh"
@@ -207,7 +208,10 @@ int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o
   static PestiShared shared;
   const int rc = pesti_allow_shared(shared, kernel, dev.index, smem_bytes(CG, E), "head_gemm_kernel shared memory");
   if (rc) return rc;
-  return launch("head_gemm_kernel launch", kernel, CG, dim3(dev.sms / CG * CG), THREADS, smem_bytes(CG, E), st, a, b, out, g);
+  GemmArgs args = g;
+  args.give_up = pesti_give_up(E);
+  return launch("head_gemm_kernel launch", kernel, CG, dim3(dev.sms / CG * CG), THREADS, smem_bytes(CG, E), st, a, b, out,
+                args);
 }
 
 RowArgs row_args(const Call& c, const Layout& l, int cg, int sms) {
@@ -501,6 +505,12 @@ int pesti_linear_ce_nll_backward(const void* d_hidden, pesti_dtype dtype, int64_
   rc = pack<true>(r, st);
   if (rc) return rc;
   return backward(c, l, r, cg, d_grad_hidden, gh_ld, d_grad_head, gw_ld, dev, st);
+}
+
+int pesti_testing_give_up(int product, int round) {
+  if (product < 0 || product > PESTI_Q4_SUMS || round < -1) return refuse("product must be 0 to 4, round -1 or more");
+  pesti_give_up_at.store((int64_t)product << 32 | (uint32_t)round, std::memory_order_relaxed);
+  return PESTI_OK;
 }
 
 }  // extern "C"

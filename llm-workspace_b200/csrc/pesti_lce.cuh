@@ -48,7 +48,7 @@ struct Plan {
   unsigned gmax;  // bits of an f32 that no |G| of a row with finite coefficients exceeds (f16 only)
   int splits;     // ranges of K in the hidden states' gradient
   int part_rows;  // rows of a range's part: the active ones, to a whole tile
-  int failed;     // a wait gave up
+  int failed;     // a wait gave up: what is made behind it is NaN
 };
 
 struct RowCoef {
@@ -93,6 +93,7 @@ struct GemmArgs {
   int out_x, out_y;   // where the output ends
   int width;          // columns of a tile (STATS: a multiple of 16)
   int twice;          // G and the packed rows are held twice
+  int give_up;        // for tests: which of a block's tiles is taken for one whose wait gave up (-1: none)
 };
 
 template <bool BF16>
@@ -235,16 +236,16 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
       // every stage is read, and the products' arrivals have reached this block
-      for (int i = 0; i < ST && ok; ++i) {
-        ok = bar_wait(empty + 8 * s, ph ^ 1);
-        if (++s == ST) {
-          s = 0;
-          ph ^= 1;
+      for (int i = 0, at = s, at_ph = ph; i < ST && ok; ++i) {
+        ok = bar_wait(empty + 8 * at, at_ph ^ 1);
+        if (++at == ST) {
+          at = 0;
+          at_ph ^= 1;
         }
       }
       if (!ok) {
         atomicExch(&g.plan->failed, 1);
-        for (int i = 0; i < ST && rank == 0; ++i) bar_wait(full + 8 * i, ph);  // copies in flight
+        for (int i = 0; i < ST && rank == 0; ++i) bar_wait(full + 8 * i, i < s ? ph : ph ^ 1);  // copies in flight
       }
     }
   } else if (warp == EPI_WARPS + 1) {
@@ -299,14 +300,17 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t row_out = out + lane * 128, swz = (lane & 7) << 4;
     const uint32_t acc_empty_to = CG == 1 ? acc_empty : peer_addr(acc_empty, 0);
     int acc = 0, acc_ph = 0, pair_ph = 0;
+    // Once a wait has given up, kernels behind this one see it in the plan.  The head's gradient may be the last one: its
+    // tiles from there on are written as NaN, without more waiting.  (`ok` is the same in all lanes.)
     bool ok = true;
-    for (int tile = first; tile < tiles && ok; tile += step) {
+    int round = 0;
+    for (int tile = first; tile < tiles && (ok || E == OUT16); tile += step, ++round) {
       int m, n, split, k0, kn;
       locate(tile, m, n, split, k0, kn);
       const int warp_row = m * TM + (int)rank * 128 + quarter * 32, row = warp_row + lane;
       const int col0 = n * (E == STATS ? g.width : BN) + half0;
       auto wait_acc = [&]() {
-        ok = bar_wait(acc_full + 8 * acc, acc_ph);
+        ok = __all_sync(PESTI_FULL_MASK, bar_wait(acc_full + 8 * acc, acc_ph)) && round != g.give_up;
         if (!ok) atomicExch(&g.plan->failed, 1);
         fence_after();
         return tmem + acc * BN + half0 + ((uint32_t)quarter << 21);
@@ -322,7 +326,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       // the warp's accumulators, which are free for the next tile but one then
       float v[HALF];
       auto take_acc = [&]() {
-        const uint32_t from = wait_acc();
+        const uint32_t from = ok ? wait_acc() : 0;
+        if (!ok) {
+#pragma unroll
+          for (int j = 0; j < HALF; ++j) v[j] = NAN;
+          return;
+        }
         uint32_t w[HALF];
 #pragma unroll
         for (int c = 0; c < HALF; c += 32) tmem_load32(from + c, *(uint32_t(*)[32])(w + c));
@@ -335,8 +344,9 @@ __global__ void __launch_bounds__(THREADS, 1)
       auto sum_acc = [&]() {
         const int parts = parts_of(kn);
 #pragma unroll 1
-        for (int part = 0; part < parts && ok; ++part) {
+        for (int part = 0; part < parts; ++part) {
           const uint32_t from = wait_acc();
+          if (!ok) break;
 #pragma unroll
           for (int c = 0; c < HALF; c += 32) {
             uint32_t w[32];
@@ -432,14 +442,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         // the tile's other half: its warp hands its sums over in shared memory
         float* other = (float*)(raw + (out0 - smem_addr(raw))) + quarter * 128 + lane;
         if (half0) {
-          ok = ok && bar_wait(taken + 8 * quarter, pair_ph ^ 1);
+          ok = ok && __all_sync(PESTI_FULL_MASK, bar_wait(taken + 8 * quarter, pair_ph ^ 1));
           other[0] = mx;
           other[32] = sum;
           other[64] = zs;
           __syncwarp();
           if (lane == 0) bar_arrive(given + 8 * quarter);
         } else {
-          ok = ok && bar_wait(given + 8 * quarter, pair_ph);
+          ok = ok && __all_sync(PESTI_FULL_MASK, bar_wait(given + 8 * quarter, pair_ph));
           const float m2 = other[0], s2 = other[32], z2 = other[64];
           __syncwarp();
           if (lane == 0) bar_arrive(taken + 8 * quarter);
@@ -749,10 +759,11 @@ __global__ void __launch_bounds__(256) lce_join_kernel(const RowArgs a) {
   }
   const int n = a.idx[i];
   // log2 of the others' sum, and how far it is above the target's logit
-  const double zt = a.zt[i], rest = (double)m + log2(s), over = rest - zt * (double)LOG2E;
+  double zt = a.zt[i];
+  if (zt == (double)INFINITY || a.plan->failed) zt = NAN;
+  const double rest = (double)m + log2(s), over = rest - zt * (double)LOG2E;
   const double log1p_r = log1p(exp2(-fabs(over)));
-  double nll = over > 0.0 ? over / (double)LOG2E + log1p_r : log1p_r;
-  if (zt == (double)INFINITY || a.plan->failed) nll = NAN;
+  const double nll = over > 0.0 ? over / (double)LOG2E + log1p_r : log1p_r;
   const double lse = over > 0.0 ? rest / (double)LOG2E + log1p_r : zt + nll, eps = a.eps;
   const float w = a.weight ? a.weight[n] : 1.0f;
   double loss = (1.0 - eps) * nll + (double)a.zeta * lse * lse;

@@ -189,6 +189,7 @@ int pass(LogitArgs a, Device dev, cudaStream_t st) {
   const int columns = columns_of(a.rows);
   const int rc = launch("q4_operand_kernel launch", q4_operand_kernel<T>, columns, 256, 0, st, a, columns);
   if (rc) return rc;
+  a.give_up = pesti_give_up(PESTI_Q4_SUMS);
   a.stages = std::min(8, SHARED_BYTES / (SLOTS * WIDE_BYTES + columns * P * (BLOCK * 2)));
   if (columns == 16) return wide_pass<P, GROUP, 16>(a, dev, st);
   if (columns == 32) return wide_pass<P, GROUP, 32>(a, dev, st);

@@ -313,6 +313,7 @@ struct LogitArgs {
   long long y_ld;
   int out;               // 0 f32, 1 bf16, 2 f16
   int k_warps;           // warps that share a tile's K
+  int give_up;           // for tests: which of a slot's rounds is taken for one whose wait gave up (-1: none)
 };
 
 __device__ __forceinline__ void store_logit(const LogitArgs& a, int row, int v, float y) {
@@ -808,7 +809,9 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) q4_wide_kernel(const LogitArg
 #pragma unroll
         for (int i = 0; i < PART; ++i) {
           if (b0 + i >= a.blocks || !ok) break;
-          if (!(ok = bar_wait(full + 8 * s, ph))) break;
+          // (one vote for both, before the loads: lanes never part at a tensor memory instruction)
+          ok = bar_wait(full + 8 * s, ph) && (!there || bar_wait(a_empty + 8 * (2 * slot + buf), buf_ph ^ 1));
+          if (!(ok = __all_sync(PESTI_FULL_MASK, ok))) break;
           uint4 w[4];
           const uint32_t at = base + s * stage + slot * WIDE_BYTES + row * BLOCK_BYTES;
 #pragma unroll
@@ -837,10 +840,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) q4_wide_kernel(const LogitArg
                 for (int e = 0; e < 4; ++e) v[16 * (j & 1) + 4 * t + e] = q[e];
               }
             }
-            if (h == 0) {
-              if (!(ok = bar_wait(a_empty + 8 * (2 * slot + buf), buf_ph ^ 1))) break;
-              fence_after();
-            }
+            if (h == 0) fence_after();
             tmem_store32(tmem + a_column(slot, buf) + 32 * h + quarter, v);
           }
           tmem_store_wait();
@@ -856,8 +856,8 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) q4_wide_kernel(const LogitArg
     const int slot = (warp - 4 * SLOTS) >> 2;
     const uint32_t quarter = (uint32_t)(warp & 3) << 21;
     int buf = 0, buf_ph = 0;
-    bool ok = true;
-    for (int r = 0; r < rounds && ok; ++r) {
+    bool ok = true;  // (the same in all lanes; once a wait has given up, the rounds from there on are NaN, without more waiting)
+    for (int r = 0; r < rounds; ++r) {
       const int stack = stack_of(r, slot);
       if (stack >= a.stacks) break;
       const __nv_bfloat16* scales = scales_of(stack);
@@ -868,7 +868,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) q4_wide_kernel(const LogitArg
         PartScales<GROUP, PART> now;
         now.load(scales, b0, a.blocks);
         const float down = power(-now.shift());
-        if (!(ok = bar_wait(d_full + 8 * (2 * slot + buf), buf_ph))) break;
+        if (!(ok = __all_sync(PESTI_FULL_MASK, bar_wait(d_full + 8 * (2 * slot + buf), buf_ph)) && r != a.give_up)) break;
         fence_after();
         const uint32_t from = tmem + d_column(slot, buf) + quarter;
 #pragma unroll
@@ -890,7 +890,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) q4_wide_kernel(const LogitArg
         const float2* back = (const float2*)((const char*)a.operand + (long long)a.blocks * x_bytes);
 #pragma unroll
         for (int c = 0; c < COLUMNS; ++c)
-          if (c < a.rows) store_logit(a, c, v, ok ? acc[c] * back[c].x * back[c].y : NAN);  // NaN: a wait gave up
+          if (c < a.rows) store_logit(a, c, v, ok ? acc[c] * back[c].x * back[c].y : NAN);
       }
     }
   } else if (warp == 8 * SLOTS) {  // copies
@@ -916,15 +916,15 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) q4_wide_kernel(const LogitArg
           }
         }
       }
-      for (int i = 0; i < a.stages && ok; ++i) {  // every stage is read
-        ok = bar_wait(empty + 8 * s, ph ^ 1);
-        if (++s == a.stages) {
-          s = 0;
-          ph ^= 1;
+      for (int i = 0, at = s, at_ph = ph; i < a.stages && ok; ++i) {  // every stage is read
+        ok = bar_wait(empty + 8 * at, at_ph ^ 1);
+        if (++at == a.stages) {
+          at = 0;
+          at_ph ^= 1;
         }
       }
       if (!ok)
-        for (int i = 0; i < a.stages; ++i) bar_wait(full + 8 * i, ph);  // copies in flight
+        for (int i = 0; i < a.stages; ++i) bar_wait(full + 8 * i, i < s ? ph : ph ^ 1);  // copies in flight
     }
   } else {  // issues a slot's products; the warp runs through as one, so that addresses are uniform
     constexpr uint32_t desc = mma_desc(false, false, false, WIDE, COLUMNS);

@@ -177,6 +177,8 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.pesti_last_gathered_reasons.restype = c_int
     lib.pesti_testing_set_cluster.argtypes = [c_int]
     lib.pesti_testing_set_cluster.restype = c_int
+    lib.pesti_testing_give_up.argtypes = [c_int, c_int]
+    lib.pesti_testing_give_up.restype = c_int
     _lib = lib
     return lib
 

@@ -32,3 +32,9 @@ def test_backward(lib, change, msg):
     assert lib.pesti_linear_ce_nll_backward(*{**args, **change}.values()) == R.BAD
     assert msg in lib.pesti_last_error().decode()
     assert lib.pesti_linear_ce_nll_backward(*{**args, "N": 0, "gw": None}.values()) == ps.PESTI_OK
+
+
+def test_giving_up(lib):
+    for product, round in ((-1, 0), (5, 0), (0, -2)):
+        assert lib.pesti_testing_give_up(product, round) == R.BAD
+    assert lib.pesti_testing_give_up(4, -1) == ps.PESTI_OK
