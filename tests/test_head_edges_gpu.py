@@ -1,11 +1,14 @@
-"""Cross entropy from hidden states where it can go wrong: confident rows.
+"""Cross entropy from hidden states where it can go wrong: confident rows,
+rows beside ones that are not finite, saved tensors that come back otherwise,
+pairs of blocks on narrow tiles.
 
 Confident rows (p of the target t near 1) against the 64-bit oracle.  Logits
-off by d (tests/test_head_gpu.py, here of the parts of at most 1024 of K that
-are summed at once, and an addition for each part) change each G but the target's by a factor
-of at most expm1(2 d), beside 2^-22 for the hardware's 2^x and 2^-22 (1 + |lse|)
-for lse and its product with log2(e) in f32, and so does G_t = p_t - 1, minus the sum of the others, if the logits are
-the very ones that are in lse.  All further errors of p_t are absolute: ABS."""
+off by d (tests/test_head_gpu.py; here of the at most 1024 of K that are summed
+at once, and an addition for each such part) change each G but the target's by
+a factor of at most expm1(2 d), beside 2^-22 for the hardware's 2^x and
+2^-22 (1 + |lse|) for lse and its product with log2(e) in f32; and so they do
+G_t = p_t - 1, minus the sum of the others, if the logits are the very ones that
+are in lse.  All further errors of p_t are absolute: ABS."""
 import contextlib
 
 import pytest
@@ -13,6 +16,7 @@ import torch
 
 import head as OH
 import pesti_head as ph
+import test_head_gpu as OE
 
 pytestmark = pytest.mark.gpu
 
@@ -260,3 +264,12 @@ def test_saved_elsewhere():
     want = gradient(lambda t: t)
     for pack in (moved, turned):
         assert all(torch.equal(a, b) for a, b in zip(gradient(pack), want))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("N,V", [(200, 20000), (1024, 3001), (700, 20000), (500, 50000), (200, 50257), (1000, 5000)])
+def test_pairs_on_narrow_tiles(dtype, N, V):
+    """More than 128 rows on tiles of 144, 176, 208 and 240 columns, an odd multiple of 16: each block of a pair copies
+    half a tile, whose rows are no multiple of 16."""
+    hidden, head, target = OE._make(N, V, 64, dtype, pad=0.1)
+    OE._all_ways(hidden, head, target, eps=0.1, zeta=1e-3, up=torch.rand(N, device="cuda") + 0.5)
