@@ -760,10 +760,12 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) q4_wide_kernel(const LogitArg
   const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
   __shared__ uint64_t bars[16 + 8 * SLOTS];
   __shared__ uint32_t tmem_base;
+  __shared__ volatile int lost;  // a warp that unpacks gave up
   const uint32_t full = smem_addr(bars), empty = full + 64, a_full = empty + 64, a_empty = a_full + 16 * SLOTS,
                  d_full = a_empty + 16 * SLOTS, d_empty = d_full + 16 * SLOTS;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
+    lost = 0;
     for (int s = 0; s < a.stages; ++s) {
       bar_init(full + 8 * s, 1);
       bar_init(empty + 8 * s, 5 * SLOTS);  // read by the warps that unpack, and its products done
@@ -796,22 +798,22 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) q4_wide_kernel(const LogitArg
     const int slot = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t quarter = (uint32_t)(warp & 3) << 21;
     int s = 0, ph = 0, buf = 0, buf_ph = 0;
+    // A lane whose wait gives up goes on with the others, so that none part at a tensor memory instruction (a vote on each
+    // wait took 5 us more than the 80 for 16 rows), but waits no more and marks what its slots have left as lost.
     bool ok = true;
-    for (int r = 0; r < rounds && ok; ++r) {
+    for (int r = 0; r < rounds; ++r) {
       const bool there = stack_of(r, slot) < a.stacks;
       const __nv_bfloat16* scales = scales_of(min(stack_of(r, slot), a.stacks - 1));
       PartScales<GROUP, PART> next;
       next.load(scales, 0, a.blocks);
-      for (int b0 = 0; b0 < a.blocks && ok; b0 += PART) {
+      for (int b0 = 0; b0 < a.blocks; b0 += PART) {
         const PartScales<GROUP, PART> now = next;
         next.load(scales, b0 + PART, a.blocks);
         const float up = power(now.shift());
 #pragma unroll
         for (int i = 0; i < PART; ++i) {
-          if (b0 + i >= a.blocks || !ok) break;
-          // (one vote for both, before the loads: lanes never part at a tensor memory instruction)
-          ok = bar_wait(full + 8 * s, ph) && (!there || bar_wait(a_empty + 8 * (2 * slot + buf), buf_ph ^ 1));
-          if (!(ok = __all_sync(PESTI_FULL_MASK, ok))) break;
+          if (b0 + i >= a.blocks) break;
+          ok = ok && bar_wait(full + 8 * s, ph);
           uint4 w[4];
           const uint32_t at = base + s * stage + slot * WIDE_BYTES + row * BLOCK_BYTES;
 #pragma unroll
@@ -820,7 +822,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) q4_wide_kernel(const LogitArg
                          : "=r"(w[t].x), "=r"(w[t].y), "=r"(w[t].z), "=r"(w[t].w)
                          : "r"(at + (chunk_at(row, t) << 4)));
           __syncwarp();
-          if (lane == 0) bar_arrive(empty + 8 * s);
+          if (lane == 0 && ok) bar_arrive(empty + 8 * s);
           if (++s == a.stages) {
             s = 0;
             ph ^= 1;
@@ -840,9 +842,13 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) q4_wide_kernel(const LogitArg
                 for (int e = 0; e < 4; ++e) v[16 * (j & 1) + 4 * t + e] = q[e];
               }
             }
-            if (h == 0) fence_after();
+            if (h == 0) {
+              ok = ok && bar_wait(a_empty + 8 * (2 * slot + buf), buf_ph ^ 1);
+              fence_after();
+            }
             tmem_store32(tmem + a_column(slot, buf) + 32 * h + quarter, v);
           }
+          if (!ok) lost = 1;
           tmem_store_wait();
           fence_before();
           __syncwarp();
@@ -856,7 +862,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) q4_wide_kernel(const LogitArg
     const int slot = (warp - 4 * SLOTS) >> 2;
     const uint32_t quarter = (uint32_t)(warp & 3) << 21;
     int buf = 0, buf_ph = 0;
-    bool ok = true;  // (the same in all lanes; once a wait has given up, the rounds from there on are NaN, without more waiting)
+    bool ok = true;  // once a lane's wait has given up, its rows from there on are NaN, without more waiting
     for (int r = 0; r < rounds; ++r) {
       const int stack = stack_of(r, slot);
       if (stack >= a.stacks) break;
@@ -864,11 +870,11 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) q4_wide_kernel(const LogitArg
       float acc[COLUMNS];
 #pragma unroll
       for (int c = 0; c < COLUMNS; ++c) acc[c] = 0.0f;
-      for (int b0 = 0; b0 < a.blocks && ok; b0 += PART) {
+      for (int b0 = 0; b0 < a.blocks; b0 += PART) {
         PartScales<GROUP, PART> now;
         now.load(scales, b0, a.blocks);
         const float down = power(-now.shift());
-        if (!(ok = __all_sync(PESTI_FULL_MASK, bar_wait(d_full + 8 * (2 * slot + buf), buf_ph)) && r != a.give_up)) break;
+        ok = ok && bar_wait(d_full + 8 * (2 * slot + buf), buf_ph) && r != a.give_up;
         fence_after();
         const uint32_t from = tmem + d_column(slot, buf) + quarter;
 #pragma unroll
@@ -881,10 +887,11 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) q4_wide_kernel(const LogitArg
         }
         fence_before();
         __syncwarp();
-        if (lane == 0) bar_arrive(d_empty + 8 * (2 * slot + buf));
+        if (lane == 0 && ok) bar_arrive(d_empty + 8 * (2 * slot + buf));
         buf ^= 1;
         if (buf == 0) buf_ph ^= 1;
       }
+      ok = ok && !lost;
       const int v = stack * WIDE + (warp & 3) * 32 + lane;
       if (v < a.V) {
         const float2* back = (const float2*)((const char*)a.operand + (long long)a.blocks * x_bytes);
