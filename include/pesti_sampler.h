@@ -506,15 +506,17 @@ int pesti_distill_topk_backward(const void* d_logits, pesti_dtype dtype, int64_t
  *   G_v  = up w [ (1 + 2 z_loss lse) exp(z_v - lse) - (1 - label_smoothing) [v = t]
  *              - label_smoothing / V ]
  *   grad_hidden = G head,  grad_head = G^T hidden      (in the inputs' type)
- * Products are summed in f32 (logits of loss and gradients in the same order), a
- * row's exponentials without its target's, joined in 64 bits, so that losses of
- * targets of probability near 1 are exact relative to themselves;
+ * Products are summed in f32, which cuts off after every 16 of K; logits, those
+ * of the loss and the same again for G, in runs of 1024 of K whose sums are
+ * rounded.  A row's exponentials are summed without its target's, in f32 over a
+ * tile and in 64 bits over the tiles, and -log p_t and G_t are made of that sum:
+ * their errors are relative to themselves, where p_t is near 1 too.  The other G
+ * are off by up to 2^-22 (2 + |lse|) of themselves besides their logits' errors.
  * G is rounded once to the inputs' type, or (up to 64 rows) held as the sum of two
  * such values (F16: times a power of two that brings its largest value to about
  * 2^14, of the rows whose loss and upstream gradient are finite; what is 2^38 below
- * that is lost).  Logits
- * that are NaN or +inf make their row's loss NaN, and the gradients that the row
- * has part in.
+ * that is lost).  Logits that are NaN or +inf make their row's loss NaN, and the
+ * gradients that the row has part in.
  *
  * pesti_linear_ce: d_loss [N] f32, optionally d_lse [N] f32 (0 for padding) and
  * the gradients of the losses' sum (either may be NULL): d_grad_hidden [N,
@@ -523,15 +525,15 @@ int pesti_distill_topk_backward(const void* d_logits, pesti_dtype dtype, int64_t
  * (up_stride 0: one value for all rows) from the forward call's inputs and lse.
  * G_t of that lse, an f32, is off by up to 2^-22 (1 + |lse|) w up.  The two _nll
  * calls pass on d_nll [N] f32 besides (lse - z_t, 0 for padding; NULL: as without),
- * from which G_t is exact relative to itself, as it is in the gradients of
- * pesti_linear_ce.
+ * from which G_t is made as in the gradients of pesti_linear_ce.
  * Outputs overlap neither inputs nor one another.  d_ws: device scratch of
  * pesti_linear_ce_workspace(...) bytes for what the call computes (passes:
  * PESTI_LINEAR_CE_FORWARD, _GRADS, or both), 256-byte aligned, any contents;
  * calls whose GPU work may overlap need scratch of their own.
  * Both run on the calling thread's current device, stream-ordered (NULL: the
  * legacy default stream), allocate nothing, add in a fixed order (the same
- * inputs give the same bits) and may be captured into a graph.
+ * inputs give the same bits) and may be captured into a graph.  If a wait inside
+ * a kernel ever gives up, after about a second, what it leaves unfinished is NaN.
  */
 #define PESTI_LINEAR_CE_FORWARD 1
 #define PESTI_LINEAR_CE_GRADS 2
@@ -583,11 +585,13 @@ int pesti_linear_ce_nll_backward(const void* d_hidden, pesti_dtype dtype, int64_
  * which is exact, over 512 columns (256 for F32 x), then over those; scales below
  * 2^-25 of the largest of these columns of their row lose bits.  16-bit x enters
  * as it is (more rows of BF16: down to 2^-39 of their largest finite value), F32 x
- * within 2^-24 of itself or 2^-39 of its row's largest finite value. The weight is read once for
- * every 64 rows of x.  The logits overlap no input
- * (refused).  d_ws: device scratch of pesti_q4_logits_workspace(...) bytes
- * (0 for few rows: NULL will do), 256-byte aligned, any contents; calls whose GPU work may overlap need scratch
- * of their own.
+ * within 2^-24 of itself or 2^-39 of its row's largest finite value.  Products of
+ * BF16 x with q (up to 8 rows) overflow from some 2^117 of x on.  The weight is
+ * read once for every 64 rows of x.  The logits overlap no input (refused).  If a
+ * wait inside a kernel ever gives up, after about a second, the logits that it
+ * leaves unfinished are NaN.  d_ws: device scratch of
+ * pesti_q4_logits_workspace(...) bytes (0 for few rows: NULL will do), 256-byte
+ * aligned, any contents; calls whose GPU work may overlap need scratch of their own.
  * All run on the calling thread's current device, stream-ordered (NULL: the
  * legacy default stream), allocate nothing, add in a fixed order (the same
  * inputs give the same bits) and may be captured into a graph.
