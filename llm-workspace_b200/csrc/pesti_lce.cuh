@@ -124,8 +124,7 @@ __device__ __forceinline__ int grad_shift(const Plan* plan) {
   if (BF16) return 0;
   const float m = __uint_as_float(plan->gmax);
   if (!(m > 0.0f)) return 0;
-  const int s = 14 - ilogbf(m);
-  return max(-100, min(100, s));
+  return min(126, 14 - ilogbf(m));  // (-113 at least: the power and its inverse are both normal)
 }
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }

@@ -273,3 +273,21 @@ def test_pairs_on_narrow_tiles(dtype, N, V):
     half a tile, whose rows are no multiple of 16."""
     hidden, head, target = OE._make(N, V, 64, dtype, pad=0.1)
     OE._all_ways(hidden, head, target, eps=0.1, zeta=1e-3, up=torch.rand(N, device="cuda") + 0.5)
+
+
+@pytest.mark.parametrize("N", [20, 200])
+@pytest.mark.parametrize("scale", [1e33, 1e36, 3e38])
+def test_weights_near_the_end_of_f32(N, scale):
+    """f16 gradients of rows of any finite weight: where the other factor is 0, 0, and beyond f16 infinite, but not NaN."""
+    g = torch.Generator(device="cuda").manual_seed(N)
+    V, D = 500, 64
+    head = torch.randn(V, D, generator=g, device="cuda").div_(8).half()
+    hidden = torch.randn(N, D, generator=g, device="cuda").half()
+    target = torch.randint(0, V, (N,), generator=g, device="cuda")
+    head[:, 5] = 0
+    hidden[:, 7] = 0
+    weight = torch.full((N,), scale, device="cuda")
+    # (G's own bound, twice the weight, has to be finite)
+    _, gh, gw = ph.linear_cross_entropy_grad(hidden, head, target, weight / 2)
+    assert (gh[:, 5] == 0).all() and (gw[:, 7] == 0).all()
+    assert not torch.isnan(gh).any() and not torch.isnan(gw).any()
