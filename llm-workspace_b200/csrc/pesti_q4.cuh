@@ -749,8 +749,9 @@ __device__ __forceinline__ uint32_t a_column(int slot, int buf) { return slot * 
 __device__ __forceinline__ uint32_t d_column(int slot, int buf) { return slot * 256 + 128 + buf * 64; }
 
 // Warps 0 to 7 unpack (four a slot, a quarter of the rows each), 8 to 15 add up, 16 copies, 17 and 18 issue a slot's
-// products.  128256 x 4096, g 64, f16: 80 us for 16 rows, 95 for 48, 98 for 64, bound by the packed f16 arithmetic that
-// unpacks (64, 81 and 87 without it; half of the products would save 1; twice as many warps that unpack take 5 more).
+// products.  128256 x 4096, g 64, f16: 81 us for 16 rows, 95 to 97 for 48, 102 to 112 for 64.  15 or so of them are the packed
+// f16 arithmetic that unpacks (64, 81 and 87 without it, of 80, 95 and 98; half of the products would save 1; twice as many
+// warps that unpack take 5 more); the weight's bytes would take 43, and what holds the rest is not known.
 template <int P, int GROUP, int COLUMNS>
 __global__ void __launch_bounds__(WIDE_THREADS, 1) q4_wide_kernel(const LogitArgs a) {
   using namespace pesti_umma;
